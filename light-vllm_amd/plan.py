@@ -113,6 +113,13 @@ class Staging:
         self._next = 0
         self._slot = -1
 
+    def __del__(self) -> None:
+        # The copies are the library's: torch's pinned allocator does not know of
+        # them and would hand a freed buffer out again while one still reads it.
+        for event in getattr(self, "_events", ()):
+            if event is not None:
+                event.synchronize()
+
     def take(self, n: int = 0) -> np.ndarray:
         """The next buffer of the ring, whole (at least ``n`` int32 entries),
         once the copy that last read it has finished."""
