@@ -487,6 +487,167 @@ int lvamd_stage_upload(void* device_dst, const void* pinned_src, int64_t bytes, 
 int lvamd_hbm_read_probe(const void* buf, int64_t bytes, uint32_t* sink, int32_t workgroups,
                          lvamd_stream_t stream);
 
+/*
+ * ---- 8-bit paged cache ------------------------------------------------------
+ *
+ * Keys and values as e4m3 codes, each pool [num_blocks, block_size,
+ * num_kv_heads, head_size] bytes, with fp32 scales [num_blocks, num_kv_heads]
+ * of its own: a row stands for code * scale of its block and kv head.  Scales
+ * are powers of two, 2^e with e the smallest exponent (at least -100) that
+ * brings the largest finite magnitude of the rows they were set for within
+ * 448.  The step's tensors (dtype) are bf16 or fp16; head_size as above.
+ */
+
+/*
+ * Quantising append: token i's row (or token sources[i]'s, where sources is
+ * given) goes to slot slots[i], for every i with slots[i] >= 0.  The slots that
+ * lie in one block must be consecutive in the list; slots are unique and less
+ * than num_blocks * block_size <= 2^31 - 1 (the caller proves this).  Per block
+ * and kv head, for K and V each:
+ *   - a block whose offset 0 is written starts anew: its scale is that of the
+ *     rows written now; bytes that are not written stay;
+ *   - any other block takes the larger of its scale and that of the rows
+ *     written now; if it grew, the block's other rows are re-scaled (exactly,
+ *     unless a code becomes subnormal), then the new ones written.
+ * A value is stored as the nearest code (ties to even) of value / scale.
+ * Non-finite values are stored as NaN and do not count for the scale;
+ * magnitudes above the largest value of dtype with four significant bits
+ * (1.875 * 2^127, 61440) are stored as that value.
+ *
+ * No counterpart in the reference, whose cache holds the model's dtype; the
+ * write it quantises is PagedKVCache.write_prepared
+ * (src/light_vllm/runtime/execution/paged_cache.py:209-254).
+ */
+int lvamd_kv_append_q8(const void* key, int64_t key_token_stride, int64_t key_head_stride,
+                       const void* value, int64_t value_token_stride, int64_t value_head_stride,
+                       void* key_pool, float* key_scales, void* value_pool, float* value_scales,
+                       const int64_t* slots, const int64_t* sources, int64_t num_slots,
+                       int32_t num_kv_heads, int32_t head_size, int32_t block_size, int32_t dtype,
+                       lvamd_stream_t stream);
+
+/*
+ * Decode attention over an 8-bit cache that holds the step's tokens already:
+ * lvamd_paged_decode's stream-K work lists (col_tiles 1, pieces of requests
+ * with q_len * group <= 16) and partials; no append.  K and V are the cache's
+ * values, so results are those of attention over the dequantised cache.
+ */
+int lvamd_paged_decode_q8(const void* q, int64_t q_token_stride, int64_t q_head_stride,
+                          const void* key_pool, const float* key_scales,
+                          const void* value_pool, const float* value_scales,
+                          void* out, int64_t out_token_stride, int64_t out_head_stride,
+                          const int32_t* pieces, const int32_t* wave_first, int32_t waves_per_head,
+                          const int32_t* tables, const uint32_t* vis,
+                          void* part_acc, float* part_ml, int64_t num_partial_slots,
+                          int32_t num_kv_heads, int32_t group, int32_t head_size, int32_t block_size,
+                          float scale, int32_t dtype, lvamd_stream_t stream);
+
+/* Its tile (the planner's unit) and how many of its waves the current device
+ * holds at once (needs a GPU). */
+int lvamd_paged_decode_q8_tile_tokens(int32_t dtype, int32_t head_size);
+int lvamd_paged_decode_q8_resident_waves(int32_t dtype, int32_t head_size);
+
+/*
+ * Prefill and tree attention over an 8-bit cache that holds the step's tokens
+ * already: lvamd_paged_prefill's unit records (128 columns) and partials.
+ */
+int lvamd_paged_prefill_q8(const void* q, int64_t q_token_stride, int64_t q_head_stride,
+                           const void* key_pool, const float* key_scales,
+                           const void* value_pool, const float* value_scales,
+                           void* out, int64_t out_token_stride, int64_t out_head_stride,
+                           const int32_t* tables, const uint32_t* vis,
+                           const int32_t* units, int32_t num_units,
+                           void* part_acc, float* part_ml, int64_t num_partial_slots,
+                           int32_t num_kv_heads, int32_t group, int32_t head_size, int32_t block_size,
+                           float scale, int32_t dtype, lvamd_stream_t stream);
+
+/* Keys per tile of it (key ranges start on multiples), and its workgroups that
+ * the current device holds at once (needs a GPU). */
+int lvamd_paged_prefill_q8_key_tokens(int32_t dtype, int32_t head_size);
+int lvamd_paged_prefill_q8_resident_units(int32_t dtype, int32_t head_size);
+
+/* One layer's launch facts over an 8-bit cache: lvamd_attention_plan (col_tiles
+ * 1, group_waves 1, prefill_col_tiles 8) with the step's slots, and where the
+ * scales lie: scale_offset bytes (a multiple of 16) after each pool's base. */
+typedef struct lvamd_attention_plan_q8 {
+  lvamd_attention_plan base;
+  const int64_t* slots; /* [num_tokens], a block's slots consecutive */
+  int64_t num_tokens;
+  int64_t scale_offset;
+} lvamd_attention_plan_q8;
+
+/*
+ * A layer's whole step over an 8-bit cache, on one stream: the quantising
+ * append (unless new_key / new_value are NULL), then the decode, merge, prefill
+ * and merge launches.  A query attends what the cache holds, its own token's
+ * stored K and V included.  Arguments as lvamd_paged_attention.
+ */
+int lvamd_paged_attention_q8(const lvamd_attention_plan_q8* plan,
+                             const void* q, int64_t q_token_stride, int64_t q_head_stride,
+                             const void* new_key, int64_t new_key_token_stride, int64_t new_key_head_stride,
+                             const void* new_value, int64_t new_value_token_stride, int64_t new_value_head_stride,
+                             void* key_pool, void* value_pool,
+                             void* out, int64_t out_token_stride, int64_t out_head_stride,
+                             float scale, lvamd_stream_t stream);
+
+/*
+ * Compact over an 8-bit cache, all layers: row dst_slots[i] of keys[l] and
+ * values[l] takes the value that row src_slots[i] had before the call.  The
+ * pairs come grouped by destination block (group g: pairs [block_starts[g],
+ * block_starts[g + 1]), device int64, each block in one group); destinations are
+ * unique.  Per layer, K or V and kv head, a destination block's scale becomes
+ * the largest of its own and those of its rows' source blocks; if it grew, its
+ * other rows are re-scaled (exactly, unless a code becomes subnormal).
+ * layer_*_ptrs: device arrays of pool base addresses, whose scales lie
+ * scale_offset bytes on.  workspace: lvamd_kv_compact_q8_workspace_size bytes
+ * of device memory, 16-byte aligned.
+ *
+ * The 8-bit form of lvamd_kv_compact (PagedKVCache.compact,
+ * src/light_vllm/runtime/execution/paged_cache.py:315-326).
+ */
+int lvamd_kv_compact_q8(const uint64_t* layer_key_ptrs, const uint64_t* layer_value_ptrs,
+                        int32_t num_layers, int32_t num_kv_heads, int32_t head_size, int32_t block_size,
+                        int64_t scale_offset, const int64_t* src_slots, const int64_t* dst_slots, int64_t num_pairs,
+                        const int64_t* block_starts, int64_t num_dst_blocks,
+                        void* workspace, int64_t workspace_bytes, lvamd_stream_t stream);
+int64_t lvamd_kv_compact_q8_workspace_size(int64_t num_pairs, int32_t num_layers, int32_t num_kv_heads,
+                                           int32_t head_size);
+
+/*
+ * Verification of drafted tokens.  Request r's drafts are [draft_starts[r],
+ * draft_starts[r + 1]) (at most LVAMD_VERIFY_MAX_DRAFTS), parents first:
+ * parents[i] is the index within the request of draft i's parent (-1: the
+ * root), siblings[i] that of the sibling before it (-1: none).  target holds
+ * one row of probabilities per node, packed: row draft_starts[r] + r is request
+ * r's root, the rows after it its drafts; node_uniforms has one number per row
+ * and sample_uniforms one per request (fp32, or fp64 with uniforms_f64), in
+ * [0, 1).  draft_probs (NULL, or one row per draft: the distribution it was
+ * drawn from; then every request's drafts are a chain) has target's dtype.
+ *
+ * From the root on, with u the node's number and p its row: without
+ * draft_probs, the child whose interval of p(c1), p(c1) + p(c2), .. holds u is
+ * accepted; with them, the child c when u * q(c) < p(c).  Where no child is,
+ * the token is the first x with r(0) + .. + r(x) > u' * sum(r), r being p
+ * without the children's tokens, or max(p - q, 0) (p itself where that is all
+ * zero; the last x with r(x) > 0 where no x passes; -1 where p is all zero).
+ * Entries that are not finite and positive count as 0; sums are in fp64.
+ *
+ * counts[r]: drafts accepted; paths[r][0..path_width): their indices within the
+ * request, then -1 (path_width at least the longest request's drafts, and 1);
+ * out_tokens[r]: the drawn token.  workspace: device memory, 8-byte aligned.
+ *
+ * Replaces: GreedyTreeAcceptanceSampler.accept
+ *   (src/light_vllm/runtime/execution/speculative.py:220-257), which takes the
+ *   target's greedy tokens only.
+ */
+#define LVAMD_VERIFY_MAX_DRAFTS 1024
+int lvamd_verify_drafts(const void* target, int64_t target_row_stride, const void* draft_probs,
+                        int64_t draft_row_stride, int32_t vocab, int32_t dtype, const int32_t* draft_starts,
+                        const int64_t* draft_tokens, const int32_t* parents, const int32_t* siblings,
+                        int64_t num_requests, const void* node_uniforms, const void* sample_uniforms,
+                        int32_t uniforms_f64, int32_t* counts, int32_t* paths, int32_t path_width,
+                        int64_t* out_tokens, void* workspace, int64_t workspace_bytes, lvamd_stream_t stream);
+int64_t lvamd_verify_drafts_workspace_size(int64_t num_requests, int32_t vocab, int32_t dtype);
+
 #ifdef __cplusplus
 }
 #endif

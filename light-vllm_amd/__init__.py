@@ -10,7 +10,11 @@ import sys as _sys
 
 _sys.modules.setdefault("light_vllm_amd", _sys.modules[__name__])
 
-from light_vllm_amd.backend import HipPagedAttention, HipPagedAttentionBackend  # noqa: E402
+from light_vllm_amd.backend import (  # noqa: E402
+    HipPagedAttention,
+    HipPagedAttentionBackend,
+    HipQuantizedPagedAttention,
+)
 from light_vllm_amd import errors  # noqa: E402
 from light_vllm_amd.interfaces import (  # noqa: E402
     AttentionLayerSpec,
@@ -35,6 +39,13 @@ from light_vllm_amd.paged_cache import (  # noqa: E402
     hip_compact,
     kv_cache_bytes_per_block,
 )
+from light_vllm_amd.quantized_cache import (  # noqa: E402
+    QuantizedKVWriteMapping,
+    QuantizedPagedKVCache,
+    QuantizedPagedLayerCache,
+    quantized_kv_cache_bytes_per_block,
+)
+from light_vllm_amd.verify import DraftBatch, DraftVerdict, verify_drafts  # noqa: E402
 
 # ``from light_vllm_amd import errors`` registers the submodule under the
 # directory's name and ``import light_vllm_amd.errors`` under the alias; a
@@ -49,11 +60,14 @@ del _name, _module, _have, _add
 
 __all__ = [
     "AttentionLayerSpec",
+    "DraftBatch",
     "DraftTree",
+    "DraftVerdict",
     "ExecutionError",
     "ExecutionNotReadyError",
     "HipPagedAttention",
     "HipPagedAttentionBackend",
+    "HipQuantizedPagedAttention",
     "KVCacheCapacityError",
     "KVCacheError",
     "ModelKVCacheSpec",
@@ -62,6 +76,9 @@ __all__ = [
     "PagedKVCacheConfig",
     "PagedKVWriteMapping",
     "PagedLayerCache",
+    "QuantizedKVWriteMapping",
+    "QuantizedPagedKVCache",
+    "QuantizedPagedLayerCache",
     "QueryLayout",
     "SharedPrefix",
     "append_draft_layout",
@@ -70,9 +87,11 @@ __all__ = [
     "hip_compact",
     "kv_cache_bytes_per_block",
     "linear_query_layout",
+    "quantized_kv_cache_bytes_per_block",
     "query_visibility",
     "semantic_positions",
     "share_prefix",
+    "verify_drafts",
 ]
 
 

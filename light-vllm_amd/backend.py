@@ -33,7 +33,7 @@ from torch import Tensor
 
 from light_vllm_amd import errors, native
 from light_vllm_amd.metadata import PagedAttentionMetadata
-from light_vllm_amd.paged_cache import current_stream, dtype_code, hip_append_rotary
+from light_vllm_amd.paged_cache import current_stream, dtype_code, hip_append_rotary, is_quantized
 from light_vllm_amd.plan import (
     DECODE_MAX_COLUMNS, DECODE_MERGE_PIECES, DECODE_MIN_UNITS_PER_WAVE, PREFILL_MIN_TILES, UNIT_TOKENS, LayerShapes,
     Staging, StepPlan,
@@ -100,6 +100,15 @@ def _rows_aligned(t: Tensor) -> bool:
     return t.stride(2) == 1 and t.data_ptr() % 16 == 0 and (t.stride(0) * es) % 16 == 0 and (
         t.stride(1) * es
     ) % 16 == 0
+
+
+def _aligned(t: Tensor) -> Tensor:
+    """``t``, or a copy of 16-byte aligned rows."""
+
+    if _rows_aligned(t):
+        return t
+    copy = t.contiguous()
+    return copy if _rows_aligned(copy) else copy.clone()
 
 
 def _partial_layout(work, spec, prefill_columns: int, element_size: int) -> tuple[int, int, int, int]:
@@ -228,6 +237,7 @@ class HipPagedAttention:
         self._rotary_bound: dict[tuple, tuple] = {}
         self._attend_tensors = backend._attend_tensors
         self._attend_fn = backend._attend_fn
+        self._attend_layer = backend._lib.lvamd_paged_attention  # the same entry point, through ctypes
 
     @property
     def layer_ids(self) -> frozenset[str]:
@@ -353,13 +363,11 @@ class HipPagedAttention:
                 f"HIP paged attention supports head sizes {SUPPORTED_HEAD_SIZES}, not {spec.head_size}"
             )
 
-        if not _rows_aligned(query):
-            query = query.contiguous()
+        query = _aligned(query)
         out = torch.empty(query.shape, dtype=query.dtype, device=query.device)
         launch = self._launch(spec)
         layer = self._cache.layer(layer_id)
         stream = current_stream(query.device)
-        lib = self._lib
         plan = self._plan
         if rotary is not None:
             # The rotated queries go to a fresh buffer and the pool receives
@@ -371,12 +379,9 @@ class HipPagedAttention:
             # The decode and prefill kernels append their own requests'
             # tokens (fused append): they read this step's keys and values
             # from the inputs and write each token's row to its slot.
-            if not _rows_aligned(key):
-                key = key.contiguous()
-            if not _rows_aligned(value):
-                value = value.contiguous()
+            key, value = _aligned(key), _aligned(value)
             new_kv = (key.data_ptr(), key.stride(0), key.stride(1), value.data_ptr(), value.stride(0), value.stride(1))
-        native.check(lib.lvamd_paged_attention(
+        native.check(self._attend_layer(
             launch.plan_ptr, query.data_ptr(), query.stride(0), query.stride(1), *new_kv,
             layer.keys.data_ptr(), layer.values.data_ptr(), out.data_ptr(), out.stride(0), out.stride(1),
             float(scale), stream,
@@ -440,6 +445,68 @@ class HipPagedAttention:
             if sum(sizes):
                 ptr = backend.workspace.get(sum(sizes), self._config.device).data_ptr()
             found = _LayerLaunch(plan, work, spec, code, self._config.block_size, ptr, columns, sizes)
+            plan.launches[key] = found
+        return found
+
+
+class _QuantizedLaunch(_LayerLaunch):
+    """``_LayerLaunch`` over an 8-bit cache: its plan also holds the step's slots
+    and where the scales lie behind each pool's codes."""
+
+    __slots__ = ("quantized_plan",)
+
+    def __init__(self, plan: StepPlan, work, spec, dtype: int, block_size: int, workspace_ptr: int | None,
+                 sizes: tuple[int, int, int, int], scale_offset: int) -> None:
+        super().__init__(plan, work, spec, dtype, block_size, workspace_ptr, native.PREFILL_Q8_COLUMNS, sizes)
+        q = self.quantized_plan = native.AttentionPlanQ8(
+            base=self.plan, slots=plan.slots_ptr, num_tokens=plan.num_tokens, scale_offset=scale_offset)
+        self.plan_ptr = ctypes.addressof(q)
+
+
+class HipQuantizedPagedAttention(HipPagedAttention):
+    """The per-step context over a ``QuantizedPagedKVCache``.
+
+    ``forward`` quantises the layer's K/V into the cache, then attends what the
+    cache holds (a query's own token included) in the step's dtype: one native
+    call per layer (``lvamd_paged_attention_q8``).  Queries and keys come
+    rotated (``supports_rotary`` is False)."""
+
+    supports_rotary = False
+
+    def __init__(self, backend: "HipPagedAttentionBackend", cache, plan: StepPlan) -> None:
+        super().__init__(backend, cache, plan)
+        self._attend_fn = backend._attend_q8_fn
+        self._attend_layer = backend._lib.lvamd_paged_attention_q8
+
+    def forward(self, layer_id: str, query: Tensor, key: Tensor, value: Tensor, *, scale: float,
+                rotary: tuple[Tensor, Tensor] | None = None) -> Tensor:
+        if rotary is not None:
+            raise errors.KVCacheError("the 8-bit KV cache takes rotated queries and keys (supports_rotary is False)")
+        return super().forward(layer_id, query, key, value, scale=scale)
+
+    def decode_launch(self, layer_id: str, query: Tensor, out: Tensor, *, scale: float, key: Tensor | None = None,
+                      value: Tensor | None = None):
+        raise errors.ExecutionError("single-kernel launches are not offered over an 8-bit KV cache")
+
+    def prefill(self, layer_id: str, query: Tensor, out: Tensor, *, scale: float) -> None:
+        raise errors.ExecutionError("single-kernel launches are not offered over an 8-bit KV cache")
+
+    def _launch(self, spec) -> _LayerLaunch:
+        backend = self._backend
+        code = dtype_code(self._config.dtype)
+        key = (spec.num_query_heads, spec.num_kv_heads, spec.head_size, code, "8-bit")
+        plan = self._plan
+        found = plan.launches.get(key)
+        if found is not None and found.workspace_ptr is not None and found.workspace_ptr != backend.workspace.ptr():
+            found = None  # the workspace (shared by all plans) was regrown since
+        if found is None:
+            work = plan.layer_work(backend.quantized_facts(spec, code, self._config.block_size))
+            sizes = _partial_layout(work, spec, native.PREFILL_Q8_COLUMNS, self._config.dtype.itemsize)
+            ptr = None
+            if sum(sizes):
+                ptr = backend.workspace.get(sum(sizes), self._config.device).data_ptr()
+            found = _QuantizedLaunch(plan, work, spec, code, self._config.block_size, ptr, sizes,
+                                     self._cache.scale_offset(spec))
             plan.launches[key] = found
         return found
 
@@ -546,6 +613,7 @@ class HipPagedAttentionBackend:
         self._attend_rotary = native.host().attend_rotary
         self._rotary_fn = native.rotary_entry()
         self._attend_fn = native.attention_entry()
+        self._attend_q8_fn = native.attention_q8_entry()
 
     def prefill_columns(self, code: int, head_size: int) -> int:
         return native.prefill_unit_columns(code, head_size) if self._use_prefill else 0
@@ -577,6 +645,27 @@ class HipPagedAttentionBackend:
                 native.xcd_count() if columns else 0, self._prefill_order,
                 native.decode_split_groups(code, d) if self._decode_workgroups else 0,
                 native.decode_split_waves(code, d), DECODE_MERGE_PIECES,
+            )
+            self._facts[key] = found
+        return found
+
+    def quantized_facts(self, spec, code: int, block_size: int) -> tuple[int, ...]:
+        """``kernel_facts`` of the kernels over an 8-bit cache: one decode shape
+        (one column tile, stream-K) and one prefill shape (four waves); the
+        options that choose among the 16-bit kernels' shapes do not apply."""
+
+        key = (spec.num_query_heads, spec.num_kv_heads, spec.head_size, code, block_size, torch.cuda.current_device(),
+               "8-bit")
+        found = self._facts.get(key)
+        if found is None:
+            d = spec.head_size
+            found = (
+                spec.num_query_heads // spec.num_kv_heads, spec.num_kv_heads, block_size, native.PREFILL_Q8_COLUMNS,
+                native.prefill_q8_key_tokens(code, d), int(self._split_prefill), 1, 4, 1, 0,
+                native.resident_decode_q8_waves(code, d), native.decode_q8_tile_tokens(code, d), 0, 0,
+                native.prefill_q8_resident_units(code, d), 0, self._partition_tokens or 0, DECODE_MAX_COLUMNS,
+                DECODE_MIN_UNITS_PER_WAVE, PREFILL_MIN_TILES, int(self._shared_prefix), native.xcd_count(),
+                self._prefill_order, 0, 0, DECODE_MERGE_PIECES,
             )
             self._facts[key] = found
         return found
@@ -634,8 +723,9 @@ class HipPagedAttentionBackend:
             config = cache.config
             code = dtype_code(config.dtype)
             shapes = {(s.num_query_heads, s.num_kv_heads, s.head_size): s for s in cache.model_spec.layers}
+            facts = self.quantized_facts if is_quantized(cache) else self.kernel_facts
             found = self._shapes[cache] = LayerShapes(
-                self.kernel_facts(spec, code, config.block_size) for spec in shapes.values()
+                facts(spec, code, config.block_size) for spec in shapes.values()
                 if spec.head_size in SUPPORTED_HEAD_SIZES)
         return found
 
@@ -647,8 +737,9 @@ class HipPagedAttentionBackend:
         # rule to re-check (the cache's configuration does not change).
         key = metadata.facts if isinstance(metadata, PagedAttentionMetadata) else metadata
         last = self._last
+        context = HipQuantizedPagedAttention if is_quantized(cache) else HipPagedAttention
         if last is not None and last[1] is key and last[3]() is cache:
-            return HipPagedAttention(self, cache, last[2])
+            return context(self, cache, last[2])
         config = cache.config
         if config.device.type != "cuda":
             raise errors.KVCacheError("HIP paged attention requires a GPU KV cache")
@@ -657,10 +748,10 @@ class HipPagedAttentionBackend:
         # A plan is reusable by a cache of the same pool geometry, dtype and
         # layer shapes: its work lists were built from the kernel facts of
         # those shapes in that dtype.
-        geometry = (config.num_blocks, config.block_size, config.device, config.dtype, shapes.keys)
+        geometry = (config.num_blocks, config.block_size, config.device, config.dtype, shapes.keys, context)
         if last is not None and last[1] is key and last[0] == geometry:
             self._last = (geometry, key, last[2], weakref.ref(cache))
-            return HipPagedAttention(self, cache, last[2])
+            return context(self, cache, last[2])
         staging = self._staging.get(config.device)
         if staging is None:
             staging = self._staging[config.device] = Staging(config.device)
@@ -669,4 +760,4 @@ class HipPagedAttentionBackend:
         plan = StepPlan(metadata, block_size=config.block_size, device=config.device, num_blocks=config.num_blocks,
                         partition_tokens=self._partition_tokens, staging=staging, shapes=shapes)
         self._last = (geometry, key, plan, weakref.ref(cache))
-        return HipPagedAttention(self, cache, plan)
+        return context(self, cache, plan)

@@ -1,0 +1,348 @@
+// Writing the 8-bit paged cache on gfx950: the quantising append and the
+// compact of accepted rows.
+//
+// Codes are e4m3, [block][offset][kv head][D] as in the 16-bit cache; a block
+// holds one scale per kv head, 2^e with e the smallest exponent that brings
+// the largest magnitude of its rows within 448 (lvamd_q8.h).
+
+#include <cmath>
+
+#include "lvamd_q8.h"
+
+namespace lvamd {
+
+// Largest of a wave's 64 values (not negative).
+__device__ __forceinline__ float wave_max(float v) {
+  v = row_max4(v);  // across the four 16-lane rows
+#pragma unroll
+  for (int d = 8; d >= 1; d >>= 1) v = fmaxf(v, __shfl_xor(v, d));
+  return v;
+}
+
+// Every store that this wave has issued is done (same-wave stores to one
+// address then land in program order).
+__device__ __forceinline__ void stores_done() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+
+// ---------------------------------------------------------------------------
+// Append.  A run is the tokens of one call that go to one block; they are
+// consecutive in the slot list.  One wave per (run, K or V, kv head):
+//   amax over the run's rows, then scale = 2^e(amax) for a block that starts
+//   anew (its offset 0 is in the run), else max(old, 2^e(amax)); if that is
+//   above the old scale, the block's rows are re-scaled by old / new; then the
+//   run's codes and the scale.
+// A token whose predecessor in the list is in the same block leaves the work
+// to the run's first token: n x (units / 4) workgroups, of which a prompt's
+// exit at once but for one per block.
+//
+// HBM-bound for prompts (each row read once and held in registers, up to
+// kHeld passes of 64 lanes; longer runs read their later rows again), a chain
+// of three round trips (slots, rows and old scale, stores) for single tokens.
+// ---------------------------------------------------------------------------
+struct Q8AppendArgs {
+  const char* key;
+  const char* value;
+  int64_t key_tok_bytes, key_head_bytes;
+  int64_t value_tok_bytes, value_head_bytes;
+  uint8_t* key_pool;
+  uint8_t* value_pool;
+  float* key_scales;
+  float* value_scales;
+  const int64_t* sources;  // token of each slot, or null: token i
+  int64_t num_slots;
+  int32_t num_kv_heads;
+  int32_t head_size;
+  int32_t block_size;
+  FastDiv by_block, by_lanes;  // / block_size, / lanes per row
+};
+
+constexpr int kHeld = 4;  // passes of rows that stay in registers
+constexpr int kAppendWaves = 4;
+
+template <typename T>
+__global__ __launch_bounds__(64 * kAppendWaves) void q8_append_kernel(const int64_t* __restrict__ slots,
+                                                                      const Q8AppendArgs a) {
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+  const int64_t i0 = blockIdx.x;
+  const int unit = blockIdx.y * kAppendWaves + wave;
+  const int64_t slot0 = slots[i0];
+  if (slot0 < 0 || unit >= 2 * a.num_kv_heads) return;
+  const int bs = a.block_size;
+  const int block = fast_div((int)slot0, a.by_block);
+  if (i0 > 0) {
+    const int64_t before = slots[i0 - 1];
+    if (before >= 0 && fast_div((int)before, a.by_block) == block) return;  // not the run's first token
+  }
+  // The run: how many slots from here on lie in the block, and whether one is
+  // its offset 0.
+  int n = 0;
+  bool fresh = false;
+  for (;; n += 64) {
+    const int64_t i = i0 + n + lane;
+    const int64_t s = i < a.num_slots && n + lane < bs ? slots[i] : -1;
+    const bool in = s >= 0 && fast_div((int)s, a.by_block) == block;
+    const uint64_t out = ~__ballot(in);
+    const int len = out == 0 ? 64 : __builtin_ctzll(out);
+    fresh |= __any(in && lane < len && (int)s - block * bs == 0);
+    if (len < 64) {
+      n += len;
+      break;
+    }
+  }
+  const bool is_v = unit >= a.num_kv_heads;
+  const int h = is_v ? unit - a.num_kv_heads : unit;
+  const char* src = (is_v ? a.value + h * a.value_head_bytes : a.key + h * a.key_head_bytes);
+  const int64_t tok_bytes = is_v ? a.value_tok_bytes : a.key_tok_bytes;
+  float* const scale_at = (is_v ? a.value_scales : a.key_scales) + (int64_t)block * a.num_kv_heads + h;
+  const int64_t row_bytes = (int64_t)a.num_kv_heads * a.head_size;
+  uint8_t* const pool = (is_v ? a.value_pool : a.key_pool) + (int64_t)h * a.head_size;
+  const float old = fresh ? 0.f : *scale_at;
+
+  // Eight elements per lane, lanes-per-row lanes to a row, R rows a pass.
+  const int lpr = a.head_size / 8;
+  const int R = fast_div(64, a.by_lanes);
+  const int r0 = fast_div(lane, a.by_lanes);
+  const int c = lane - r0 * lpr;
+  auto load = [&](int r) -> uint4 {
+    const int64_t i = i0 + r;
+    const int64_t t = a.sources ? a.sources[i] : i;
+    return load16(reinterpret_cast<const T*>(src + t * tok_bytes) + 8 * c);
+  };
+  auto row_of = [&](int pass) -> int { return r0 < R ? pass * R + r0 : n; };  // n: none
+  uint4 held[kHeld];
+  float amax = 0.f;
+  auto largest = [&](uint4 v) {
+    T x[8];
+    __builtin_memcpy(x, &v, 16);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float m = __builtin_fabsf(to_f32(x[e]));
+      amax = fmaxf(amax, m < INFINITY ? m : 0.f);  // (NaN compares false)
+    }
+  };
+#pragma unroll
+  for (int p = 0; p < kHeld; ++p) held[p] = row_of(p) < n ? load(row_of(p)) : zero_u4();
+#pragma unroll
+  for (int p = 0; p < kHeld; ++p) largest(held[p]);
+  for (int p = kHeld; p * R < n; ++p)
+    if (row_of(p) < n) largest(load(row_of(p)));
+  amax = wave_max(amax);
+  const float scale = fmaxf(old, q8_scale(amax));
+  const float inverse = q8_inverse(scale);
+
+  if (!fresh && scale > old) {
+    // The rows that the block holds, at the new scale.
+    const float ratio = old * inverse;
+    for (int r = r0; r < bs; r += R) {
+      if (r0 >= R) break;
+      uint2* const at = reinterpret_cast<uint2*>(pool + ((int64_t)block * bs + r) * row_bytes + 8 * c);
+      const uint2 w = *at;
+      *at = make_uint2(q8_rescale4(w.x, ratio), q8_rescale4(w.y, ratio));
+    }
+    stores_done();
+  }
+  auto store = [&](int r, uint4 v) {
+    T x[8];
+    __builtin_memcpy(x, &v, 16);
+    float f[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) f[e] = q8_scaled<T>(to_f32(x[e]), inverse);
+    const int64_t s = slots[i0 + r];
+    *reinterpret_cast<uint2*>(pool + s * row_bytes + 8 * c) =
+        make_uint2(q8_pack4(f[0], f[1], f[2], f[3]), q8_pack4(f[4], f[5], f[6], f[7]));
+  };
+#pragma unroll
+  for (int p = 0; p < kHeld; ++p)
+    if (row_of(p) < n) store(row_of(p), held[p]);
+  for (int p = kHeld; p * R < n; ++p)
+    if (row_of(p) < n) store(row_of(p), load(row_of(p)));
+  if (lane == 0) *scale_at = scale;
+}
+
+// ---------------------------------------------------------------------------
+// Compact of accepted rows, two launches: the first copies every pair's row
+// (codes and its block's scale, for every layer, K and V) to the workspace,
+// the second writes them.  Pairs come grouped by destination block; one wave
+// per (destination block, layer, K or V, kv head) takes the larger of the
+// block's scale and those its rows come with, re-scales the block's rows if
+// that is above its own, then writes the moved rows at it.  (Every source is
+// read before any block changes: a source's block may be another's
+// destination.)
+// ---------------------------------------------------------------------------
+struct Q8CompactArgs {
+  const uint64_t* layer_keys;
+  const uint64_t* layer_values;
+  int64_t scale_offset;  // bytes from a pool's base to its scales
+  const int64_t* src;
+  const int64_t* dst;
+  uint8_t* rows;         // workspace: [pairs][layers * 2][kv heads][D]
+  float* row_scales;     // workspace: [pairs][layers * 2][kv heads]
+  int32_t num_layers, num_kv_heads, head_size, block_size;
+  FastDiv by_block, by_heads, by_chunks, by_sides;
+};
+
+constexpr int kCompactThreads = 256;
+
+// One thread per (pair, layer side, kv head, 16-byte chunk).
+__global__ __launch_bounds__(kCompactThreads) void q8_gather_kernel(const int64_t total, const Q8CompactArgs a) {
+  const int64_t id = (int64_t)blockIdx.x * kCompactThreads + threadIdx.x;
+  if (id >= total) return;
+  const int chunks = a.head_size / 16;
+  const int row = fast_div((int)id, a.by_chunks);  // (pair, layer side, kv head)
+  const int c = (int)id - row * chunks;
+  const int ps = fast_div(row, a.by_heads);
+  const int h = row - ps * a.num_kv_heads;
+  const int sides = 2 * a.num_layers;
+  const int pair = fast_div(ps, a.by_sides);
+  const int side = ps - pair * sides;
+  const char* base = reinterpret_cast<const char*>(side & 1 ? a.layer_values[side >> 1] : a.layer_keys[side >> 1]);
+  const int64_t s = a.src[pair];
+  const uint4 v = load16(reinterpret_cast<const uint8_t*>(base) + (s * a.num_kv_heads + h) * a.head_size + 16 * c);
+  *reinterpret_cast<uint4*>(a.rows + (int64_t)row * a.head_size + 16 * c) = v;
+  if (c == 0) {
+    const float* scales = reinterpret_cast<const float*>(base + a.scale_offset);
+    a.row_scales[row] = scales[(int64_t)fast_div((int)s, a.by_block) * a.num_kv_heads + h];
+  }
+}
+
+// Grid: (destination groups, kv heads x layer sides / waves).
+__global__ __launch_bounds__(64 * kAppendWaves) void q8_scatter_kernel(const int64_t* __restrict__ starts,
+                                                                       const Q8CompactArgs a) {
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+  const int unit = blockIdx.y * kAppendWaves + wave;  // (layer side, kv head)
+  const int sides = 2 * a.num_layers;
+  if (unit >= sides * a.num_kv_heads) return;
+  const int side = fast_div(unit, a.by_heads);
+  const int h = unit - side * a.num_kv_heads;
+  const int64_t first = starts[blockIdx.x], last = starts[blockIdx.x + 1];
+  char* base = reinterpret_cast<char*>(side & 1 ? a.layer_values[side >> 1] : a.layer_keys[side >> 1]);
+  const int block = fast_div((int)a.dst[first], a.by_block);
+  float* const scale_at = reinterpret_cast<float*>(base + a.scale_offset) + (int64_t)block * a.num_kv_heads + h;
+  auto row = [&](int64_t pair) { return (pair * sides + side) * a.num_kv_heads + h; };
+  const float old = *scale_at;
+  float most = 0.f;
+  for (int64_t p = first + lane; p < last; p += 64) most = fmaxf(most, a.row_scales[row(p)]);
+  const float scale = fmaxf(old, wave_max(most));
+  const int chunks = a.head_size / 16;
+  const int R = fast_div(64, a.by_chunks);
+  const int r0 = fast_div(lane, a.by_chunks);
+  const int c = lane - r0 * chunks;
+  if (r0 >= R) return;
+  const int64_t row_bytes = (int64_t)a.num_kv_heads * a.head_size;
+  uint8_t* const pool = reinterpret_cast<uint8_t*>(base) + (int64_t)h * a.head_size + 16 * c;
+  const float inverse = q8_inverse(scale);
+  auto rescaled = [&](uint4 w, float ratio) {
+    return make_uint4(q8_rescale4(w.x, ratio), q8_rescale4(w.y, ratio), q8_rescale4(w.z, ratio), q8_rescale4(w.w, ratio));
+  };
+  if (scale > old) {
+    const float ratio = old * inverse;
+    for (int r = r0; r < a.block_size; r += R) {
+      uint4* const at = reinterpret_cast<uint4*>(pool + ((int64_t)block * a.block_size + r) * row_bytes);
+      *at = rescaled(*at, ratio);
+    }
+    stores_done();
+    if (lane == 0) *scale_at = scale;
+  }
+  for (int64_t p = first + r0; p < last; p += R) {
+    const float from = a.row_scales[row(p)];
+    uint4 w = load16(a.rows + row(p) * a.head_size + 16 * c);
+    if (from < scale) w = rescaled(w, from * inverse);
+    *reinterpret_cast<uint4*>(pool + a.dst[p] * row_bytes) = w;
+  }
+}
+
+static bool q8_head_size(int d) { return d >= 32 && d <= 256 && d % 16 == 0; }
+static bool aligned_to(const void* p, unsigned n) { return ((uintptr_t)p & (n - 1)) == 0; }
+
+}  // namespace lvamd
+
+using namespace lvamd;
+
+extern "C" int lvamd_kv_append_q8(const void* key, int64_t key_token_stride, int64_t key_head_stride, const void* value,
+                                  int64_t value_token_stride, int64_t value_head_stride, void* key_pool,
+                                  float* key_scales, void* value_pool, float* value_scales, const int64_t* slots,
+                                  const int64_t* sources, int64_t num_slots, int32_t num_kv_heads, int32_t head_size,
+                                  int32_t block_size, int32_t dtype, lvamd_stream_t stream) {
+  if ((dtype != LVAMD_BF16 && dtype != LVAMD_F16) || !q8_head_size(head_size)) return LVAMD_ERR_UNSUPPORTED;
+  if (num_slots < 0 || num_kv_heads <= 0 || num_kv_heads > 32768 || block_size <= 0) return LVAMD_ERR_INVALID_ARGUMENT;
+  if (num_slots == 0) return LVAMD_OK;
+  if (!key || !value || !key_pool || !key_scales || !value_pool || !value_scales || !slots || num_slots > 0x7fffffffLL)
+    return LVAMD_ERR_INVALID_ARGUMENT;
+  if (!aligned_to(key, 16) || !aligned_to(value, 16) || !aligned_to(key_pool, 16) || !aligned_to(value_pool, 16) ||
+      !aligned_to(key_scales, 4) || !aligned_to(value_scales, 4) || key_token_stride % 8 != 0 ||
+      key_head_stride % 8 != 0 || value_token_stride % 8 != 0 || value_head_stride % 8 != 0)
+    return LVAMD_ERR_INVALID_ARGUMENT;
+  Q8AppendArgs a{.by_block = FastDiv(block_size), .by_lanes = FastDiv(head_size / 8)};
+  a.key = static_cast<const char*>(key);
+  a.value = static_cast<const char*>(value);
+  a.key_tok_bytes = key_token_stride * 2;
+  a.key_head_bytes = key_head_stride * 2;
+  a.value_tok_bytes = value_token_stride * 2;
+  a.value_head_bytes = value_head_stride * 2;
+  a.key_pool = static_cast<uint8_t*>(key_pool);
+  a.value_pool = static_cast<uint8_t*>(value_pool);
+  a.key_scales = key_scales;
+  a.value_scales = value_scales;
+  a.sources = sources;
+  a.num_slots = num_slots;
+  a.num_kv_heads = num_kv_heads;
+  a.head_size = head_size;
+  a.block_size = block_size;
+  const dim3 grid((unsigned)num_slots, (unsigned)((2 * num_kv_heads + kAppendWaves - 1) / kAppendWaves));
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  if (dtype == LVAMD_BF16)
+    hipLaunchKernelGGL((q8_append_kernel<__bf16>), grid, dim3(64 * kAppendWaves), 0, s, slots, a);
+  else
+    hipLaunchKernelGGL((q8_append_kernel<_Float16>), grid, dim3(64 * kAppendWaves), 0, s, slots, a);
+  return launch_status();
+}
+
+extern "C" int64_t lvamd_kv_compact_q8_workspace_size(int64_t num_pairs, int32_t num_layers, int32_t num_kv_heads,
+                                                      int32_t head_size) {
+  if (num_pairs <= 0 || num_layers <= 0 || num_kv_heads <= 0 || head_size <= 0) return 0;
+  return num_pairs * num_layers * 2 * num_kv_heads * ((int64_t)head_size + 4);
+}
+
+extern "C" int lvamd_kv_compact_q8(const uint64_t* layer_key_ptrs, const uint64_t* layer_value_ptrs, int32_t num_layers,
+                                   int32_t num_kv_heads, int32_t head_size, int32_t block_size, int64_t scale_offset,
+                                   const int64_t* src_slots, const int64_t* dst_slots, int64_t num_pairs,
+                                   const int64_t* block_starts, int64_t num_dst_blocks, void* workspace,
+                                   int64_t workspace_bytes, lvamd_stream_t stream) {
+  if (!q8_head_size(head_size)) return LVAMD_ERR_UNSUPPORTED;
+  if (num_pairs < 0 || num_layers <= 0 || num_kv_heads <= 0 || block_size <= 0 || num_dst_blocks < 0 ||
+      num_dst_blocks > num_pairs || (num_pairs > 0) != (num_dst_blocks > 0) || scale_offset < 0 || scale_offset % 4 != 0)
+    return LVAMD_ERR_INVALID_ARGUMENT;
+  if (num_pairs == 0) return LVAMD_OK;
+  if (!layer_key_ptrs || !layer_value_ptrs || !src_slots || !dst_slots || !block_starts) return LVAMD_ERR_INVALID_ARGUMENT;
+  const int64_t units = (int64_t)num_layers * 2 * num_kv_heads;
+  const int64_t chunks = num_pairs * units * (head_size / 16);
+  const int64_t groups_y = (units + kAppendWaves - 1) / kAppendWaves;
+  // 32-bit indexes in the kernels, and the grid's limits.
+  if (units > 0x7fffffffLL / 64 || num_pairs > 0x7fffffffLL || chunks > 0x7fffffffLL || groups_y > 65535)
+    return LVAMD_ERR_INVALID_ARGUMENT;
+  if (!workspace || !aligned_to(workspace, 16) ||
+      workspace_bytes < lvamd_kv_compact_q8_workspace_size(num_pairs, num_layers, num_kv_heads, head_size))
+    return LVAMD_ERR_WORKSPACE;
+  Q8CompactArgs a{.by_block = FastDiv(block_size), .by_heads = FastDiv(num_kv_heads), .by_chunks = FastDiv(head_size / 16),
+                  .by_sides = FastDiv(2 * num_layers)};
+  a.layer_keys = layer_key_ptrs;
+  a.layer_values = layer_value_ptrs;
+  a.scale_offset = scale_offset;
+  a.src = src_slots;
+  a.dst = dst_slots;
+  a.rows = static_cast<uint8_t*>(workspace);
+  a.row_scales = reinterpret_cast<float*>(a.rows + num_pairs * units * head_size);
+  a.num_layers = num_layers;
+  a.num_kv_heads = num_kv_heads;
+  a.head_size = head_size;
+  a.block_size = block_size;
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  hipLaunchKernelGGL(q8_gather_kernel, dim3((unsigned)((chunks + kCompactThreads - 1) / kCompactThreads)),
+                     dim3(kCompactThreads), 0, s, chunks, a);
+  const int status = launch_status();
+  if (status != LVAMD_OK) return status;
+  hipLaunchKernelGGL(q8_scatter_kernel, dim3((unsigned)num_dst_blocks, (unsigned)groups_y), dim3(64 * kAppendWaves), 0, s,
+                     block_starts, a);
+  return launch_status();
+}

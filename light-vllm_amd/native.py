@@ -19,7 +19,7 @@ from pathlib import Path
 from light_vllm_amd import errors
 
 LIB_NAME = "liblvamd_hip.so"
-ABI_VERSION = 20
+ABI_VERSION = 21
 PACKAGE_DIR = Path(__file__).resolve().parent
 REPO_ROOT = PACKAGE_DIR.parent
 HEADER = REPO_ROOT / "include" / "lvamd_paged_kv.h"
@@ -104,6 +104,38 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
         ctypes.c_int,
         [_p, _p, _i32, _i64, _p, _p, _i64, _p],
     ),
+    "lvamd_kv_append_q8": (
+        ctypes.c_int,
+        [_p, _i64, _i64, _p, _i64, _i64, _p, _p, _p, _p, _p, _p, _i64, _i32, _i32, _i32, _i32, _p],
+    ),
+    "lvamd_paged_decode_q8": (
+        ctypes.c_int,
+        [_p, _i64, _i64, _p, _p, _p, _p, _p, _i64, _i64, _p, _p, _i32, _p, _p, _p, _p, _i64,
+         _i32, _i32, _i32, _i32, _f32, _i32, _p],
+    ),
+    "lvamd_paged_decode_q8_tile_tokens": (ctypes.c_int, [_i32, _i32]),
+    "lvamd_paged_decode_q8_resident_waves": (ctypes.c_int, [_i32, _i32]),
+    "lvamd_paged_prefill_q8": (
+        ctypes.c_int,
+        [_p, _i64, _i64, _p, _p, _p, _p, _p, _i64, _i64, _p, _p, _p, _i32, _p, _p, _i64,
+         _i32, _i32, _i32, _i32, _f32, _i32, _p],
+    ),
+    "lvamd_paged_prefill_q8_key_tokens": (ctypes.c_int, [_i32, _i32]),
+    "lvamd_paged_prefill_q8_resident_units": (ctypes.c_int, [_i32, _i32]),
+    "lvamd_paged_attention_q8": (
+        ctypes.c_int,
+        [_p, _p, _i64, _i64, _p, _i64, _i64, _p, _i64, _i64, _p, _p, _p, _i64, _i64, _f32, _p],
+    ),
+    "lvamd_kv_compact_q8": (
+        ctypes.c_int,
+        [_p, _p, _i32, _i32, _i32, _i32, _i64, _p, _p, _i64, _p, _i64, _p, _i64, _p],
+    ),
+    "lvamd_kv_compact_q8_workspace_size": (_i64, [_i64, _i32, _i32, _i32]),
+    "lvamd_verify_drafts": (
+        ctypes.c_int,
+        [_p, _i64, _p, _i64, _i32, _i32, _p, _p, _p, _p, _i64, _p, _p, _i32, _p, _p, _i32, _p, _p, _i64, _p],
+    ),
+    "lvamd_verify_drafts_workspace_size": (_i64, [_i64, _i32, _i32]),
     "lvamd_stage_upload": (ctypes.c_int, [_p, _p, _i64, _p, _p]),
     "lvamd_hbm_read_probe": (ctypes.c_int, [_p, _i64, _p, _i32, _p]),
 }
@@ -123,6 +155,18 @@ class AttentionPlan(ctypes.Structure):
         ("prefill_col_tiles", _i32), ("num_kv_heads", _i32),
         ("tables", _p), ("vis", _p), ("group", _i32), ("head_size", _i32), ("block_size", _i32), ("dtype", _i32),
     ]
+
+
+class AttentionPlanQ8(ctypes.Structure):
+    """``lvamd_attention_plan_q8``: an ``AttentionPlan`` over an 8-bit cache."""
+
+    _fields_ = [("base", AttentionPlan), ("slots", _p), ("num_tokens", _i64), ("scale_offset", _i64)]
+
+
+# Most drafts of a request that lvamd_verify_drafts takes.
+VERIFY_MAX_DRAFTS = 1024
+# Columns per prefill unit of the 8-bit kernel.
+PREFILL_Q8_COLUMNS = 128
 
 
 def library_path() -> Path:
@@ -276,12 +320,52 @@ def prefill_waves_built(dtype_code: int, head_size: int, waves: int) -> bool:
     return bool(load().lvamd_paged_prefill_waves_built(dtype_code, head_size, waves))
 
 
+def resident_decode_q8_waves(dtype_code: int, head_size: int) -> int:
+    """Waves of the 8-bit decode kernel the current GPU holds at once."""
+
+    found = int(load().lvamd_paged_decode_q8_resident_waves(dtype_code, head_size))
+    check(min(found, 0), "lvamd_paged_decode_q8_resident_waves")
+    return found
+
+
+@functools.lru_cache(maxsize=None)
+def decode_q8_tile_tokens(dtype_code: int, head_size: int) -> int:
+    """Tokens per tile of the 8-bit decode kernel (the planner's unit)."""
+
+    found = int(load().lvamd_paged_decode_q8_tile_tokens(dtype_code, head_size))
+    check(min(found, 0), "lvamd_paged_decode_q8_tile_tokens")
+    return found
+
+
+@functools.lru_cache(maxsize=None)
+def prefill_q8_key_tokens(dtype_code: int, head_size: int) -> int:
+    """Keys per tile of the 8-bit prefill kernel."""
+
+    found = int(load().lvamd_paged_prefill_q8_key_tokens(dtype_code, head_size))
+    check(min(found, 0), "lvamd_paged_prefill_q8_key_tokens")
+    return found
+
+
+def prefill_q8_resident_units(dtype_code: int, head_size: int) -> int:
+    """Workgroups of the 8-bit prefill kernel the current GPU holds at once."""
+
+    found = int(load().lvamd_paged_prefill_q8_resident_units(dtype_code, head_size))
+    check(min(found, 0), "lvamd_paged_prefill_q8_resident_units")
+    return found
+
+
 @functools.lru_cache(maxsize=1)
 def attention_entry() -> int:
     """Address of ``lvamd_paged_attention``, for the host module's ``attend``
     (which calls it with plain integers)."""
 
     return ctypes.cast(load().lvamd_paged_attention, ctypes.c_void_p).value
+
+
+def attention_q8_entry() -> int:
+    """Address of ``lvamd_paged_attention_q8``, for the host module's ``attend_tensors``."""
+
+    return ctypes.cast(load().lvamd_paged_attention_q8, ctypes.c_void_p).value
 
 
 def rotary_entry() -> int:

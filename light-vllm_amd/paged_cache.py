@@ -141,6 +141,13 @@ def _layer_pointers(cache) -> _CacheState:
     return found
 
 
+def is_quantized(cache) -> bool:
+    """Whether ``cache`` holds 8-bit codes with scales (``QuantizedPagedKVCache``),
+    whose rows cannot be moved without their blocks' scales."""
+
+    return getattr(cache, "quantized", False) is True
+
+
 def _require_gpu(cache) -> None:
     if cache.config.device.type != "cuda":
         raise errors.KVCacheError("the HIP paged KV path requires a GPU KV cache")
@@ -288,6 +295,8 @@ def hip_compact_many(cache, requests) -> tuple[int, ...]:
     _require_gpu(cache)
     if not isinstance(requests, (list, tuple)):
         requests = tuple(requests)
+    if is_quantized(cache):
+        return cache.compact_many(requests)
     moved, src, dst = _compact_plan(cache.config, requests)
     if src.size:
         _launch_compact(cache, src, dst, moved)
@@ -386,6 +395,21 @@ def hip_block_copy(cache, src_blocks, dst_blocks) -> None:
     """
 
     _require_gpu(cache)
+    src, dst = _block_copy_pairs(cache, src_blocks, dst_blocks)
+    if not src:
+        return
+    if is_quantized(cache):
+        cache.copy_blocks(src, dst)
+        return
+    pointers = _layer_pointers(cache)
+    bs = cache.config.block_size
+    _launch_block_copy(cache.config.device, src, dst, pointers.staging, pointers.small_copies,
+                       [(row_bytes * bs, *rest) for row_bytes, *rest in pointers.groups])
+
+
+def _block_copy_pairs(cache, src_blocks, dst_blocks) -> tuple[tuple[int, ...], tuple[int, ...]]:
+    """The blocks of a copy, checked."""
+
     src = tuple(src_blocks)
     dst = tuple(dst_blocks)
     if len(src) != len(dst):
@@ -398,26 +422,28 @@ def hip_block_copy(cache, src_blocks, dst_blocks) -> None:
         raise errors.KVCacheError("block copy writes the same physical block twice")
     if set(src) & set(dst):
         raise errors.KVCacheError("block copy sources and destinations must be disjoint")
-    if not src:
-        return
-    pointers = _layer_pointers(cache)
+    return src, dst
+
+
+def _launch_block_copy(device, src, dst, staging: Staging, small: int, groups) -> None:
+    """Copy blocks of every group (block bytes, pools, table, K and V base addresses)."""
+
     lib = native.load()
-    stream = current_stream(cache.config.device)
-    bs = cache.config.block_size
-    if len(src) <= pointers.small_copies:
+    stream = current_stream(device)
+    if len(src) <= small:
         # A step's few copies ride in the kernel arguments.
         src_a = np.asarray(src, dtype=np.int64)
         dst_a = np.asarray(dst, dtype=np.int64)
-        for row_bytes, num_layers, _, kptrs, vptrs in pointers.groups:
-            native.check(lib.lvamd_kv_block_copy_small(kptrs, vptrs, num_layers, row_bytes * bs, src_a.ctypes.data,
+        for block_bytes, num_layers, _, kptrs, vptrs in groups:
+            native.check(lib.lvamd_kv_block_copy_small(kptrs, vptrs, num_layers, block_bytes, src_a.ctypes.data,
                                                        dst_a.ctypes.data, len(src), stream),
                          "lvamd_kv_block_copy_small")
         return
-    blob, (src_off, dst_off) = pointers.staging.stage([np.asarray(src, dtype=np.int64).view(np.int32),
-                                                       np.asarray(dst, dtype=np.int64).view(np.int32)])
-    for row_bytes, num_layers, _, kptrs, vptrs in pointers.groups:
+    blob, (src_off, dst_off) = staging.stage([np.asarray(src, dtype=np.int64).view(np.int32),
+                                              np.asarray(dst, dtype=np.int64).view(np.int32)])
+    for block_bytes, num_layers, _, kptrs, vptrs in groups:
         status = lib.lvamd_kv_block_copy(
-            kptrs, vptrs, num_layers, row_bytes * bs,
+            kptrs, vptrs, num_layers, block_bytes,
             blob.data_ptr() + 4 * src_off, blob.data_ptr() + 4 * dst_off, len(src), stream,
         )
         native.check(status, "lvamd_kv_block_copy")

@@ -1,0 +1,172 @@
+"""Verification of drafted tokens against the target model's probabilities.
+
+light-vllm verifies draft trees greedily: a draft is accepted when it is the
+target's most likely token (``GreedyTreeAcceptanceSampler``,
+src/light_vllm/runtime/execution/speculative.py:220-257).  ``verify_drafts``
+verifies them for sampled decoding: the tokens that come out follow the target's
+distribution, whatever was drafted.  It runs in the gfx950 kernels of
+``liblvamd_hip.so`` on the device's probabilities; the random numbers are the
+caller's.
+"""
+
+from __future__ import annotations
+
+from dataclasses import dataclass
+from typing import Sequence
+
+import numpy as np
+import torch
+from torch import Tensor
+
+from light_vllm_amd import errors, native
+from light_vllm_amd.interfaces import DraftTree
+from light_vllm_amd.paged_cache import dtype_code
+from light_vllm_amd.plan import current_stream
+from light_vllm_amd.quantized_cache import on_device
+
+
+class DraftBatch:
+    """The draft trees of one step's requests, on the device.
+
+    Made when the step is built (one upload), used by ``verify_drafts`` once the
+    target's probabilities are there.  A request without drafts has an empty
+    tree.  Rows of probabilities are packed request by request: the root's (the
+    distribution after the request's last formal token), then one per draft."""
+
+    __slots__ = ("num_requests", "num_drafts", "num_rows", "path_width", "chains", "max_token", "counts", "device",
+                 "_blob", "_ptrs")
+
+    def __init__(self, drafts: Sequence[DraftTree], *, device: str | torch.device) -> None:
+        self.device = torch.device(device)
+        if self.device.type != "cuda":
+            raise errors.ExecutionError("draft verification requires a GPU (cuda) device")
+        if self.device.index is None:
+            self.device = torch.device("cuda", torch.cuda.current_device())
+        self.counts = tuple(len(d) for d in drafts)
+        arrays, self.chains, self.max_token = pack_drafts(drafts)
+        self.num_requests = len(self.counts)
+        self.num_drafts = sum(self.counts)
+        self.num_rows = self.num_drafts + self.num_requests
+        self.path_width = max((1, *self.counts))
+        sizes = [a.size for a in arrays]
+        blob = self._blob = torch.from_numpy(np.concatenate(arrays)).to(self.device)
+        at = blob.data_ptr()
+        # Addresses of tokens (int64, first: aligned), starts, parents and siblings.
+        self._ptrs = tuple(at + 4 * sum(sizes[:i]) for i in range(4))
+
+    def __len__(self) -> int:
+        return self.num_requests
+
+
+def pack_drafts(drafts: Sequence[DraftTree]) -> tuple[list[np.ndarray], bool, int]:
+    """int32 arrays [tokens as int64 pairs, first drafts per request, parents,
+    earlier siblings], whether every tree is a chain, and the largest token."""
+
+    starts, tokens, parents, siblings = [0], [], [], []
+    chains, top = True, -1
+    if not len(drafts):
+        raise ValueError("draft verification needs at least one request")
+    for tree in drafts:
+        n = len(tree.token_ids)
+        if n > native.VERIFY_MAX_DRAFTS:
+            raise ValueError(f"draft verification takes at most {native.VERIFY_MAX_DRAFTS} drafts per request")
+        last: dict[int, int] = {}
+        for i, parent in enumerate(tree.parent_indices):
+            siblings.append(last.get(parent, -1))
+            last[parent] = i
+            chains = chains and parent == i - 1
+        parents.extend(tree.parent_indices)
+        tokens.extend(tree.token_ids)
+        starts.append(len(tokens))
+        top = max((top, *tree.token_ids))
+    if top >= 2**31:
+        raise ValueError("draft tokens must be below 2**31")
+    return [np.asarray(tokens, dtype=np.int64).view(np.int32), np.asarray(starts, dtype=np.int32),
+            np.asarray(parents, dtype=np.int32), np.asarray(siblings, dtype=np.int32)], chains, top
+
+
+@dataclass(frozen=True, slots=True)
+class DraftVerdict:
+    """What ``verify_drafts`` decided, on the device: per request how many drafts
+    were accepted (int32), their indices in the tree, then -1 (int32
+    ``[requests, longest tree]``), and the token that follows them (int64)."""
+
+    counts: Tensor
+    paths: Tensor
+    tokens: Tensor
+
+    def retained_query_indices(self, num_input_queries: Sequence[int]) -> tuple[tuple[int, ...], ...]:
+        """Per request the query indices that ``compact`` keeps: the formal
+        inputs, then the accepted path (light-vllm: speculative.py:399-401).
+        Copies the verdict to the host."""
+
+        counts, paths = self.counts.tolist(), self.paths.tolist()
+        if len(num_input_queries) != len(counts):
+            raise ValueError("num_input_queries needs one count per request")
+        return tuple(tuple(range(n)) + tuple(n + i for i in path[:count])
+                     for n, count, path in zip(num_input_queries, counts, paths))
+
+
+@torch.inference_mode()
+def verify_drafts(batch: DraftBatch, target_probs: Tensor, node_uniforms: Tensor, sample_uniforms: Tensor, *,
+                  draft_probs: Tensor | None = None) -> DraftVerdict:
+    """Accept drafts and draw the token after them, on the current stream.
+
+    ``target_probs`` ``[rows, vocab]`` (fp32, fp16 or bf16; any row stride): the
+    target's probabilities at every node, packed as ``DraftBatch`` says.
+    ``node_uniforms`` ``[rows]`` and ``sample_uniforms`` ``[requests]`` (fp32 or
+    fp64): uniform numbers in [0, 1).  Without ``draft_probs`` the drafts are
+    fixed tokens (an n-gram proposer's tree): at each node the children's
+    probabilities are laid end to end, and the child whose interval holds the
+    node's number is accepted.  With ``draft_probs`` ``[drafts, vocab]`` (the
+    distribution that each draft was drawn from; chains only) draft x is accepted
+    when u q(x) < p(x).  At the first node that accepts no child the request's
+    token is drawn from what is left there: p without the children's tokens, or
+    max(p - q, 0); p itself where nothing is left.  A row with no positive
+    probability gives token -1.  Sums are in fp64.
+    """
+
+    def shape(t, *want) -> bool:
+        return isinstance(t, Tensor) and tuple(t.shape) == want
+
+    vocab = target_probs.shape[1] if isinstance(target_probs, Tensor) and target_probs.ndim == 2 else 0
+    both = [target_probs] if draft_probs is None else [target_probs, draft_probs]
+    rules = (
+        (lambda: vocab > 0 and vocab <= 1 << 30 and shape(target_probs, batch.num_rows, vocab),
+         f"target probabilities must have shape [{batch.num_rows}, vocab]"),
+        (lambda: draft_probs is None or shape(draft_probs, batch.num_drafts, vocab),
+         f"draft probabilities must have shape [{batch.num_drafts}, vocab]"),
+        (lambda: draft_probs is None or batch.chains, "draft probabilities need chains of drafts, not trees"),
+        (lambda: all(t.dtype in (torch.float32, torch.float16, torch.bfloat16) and t.dtype == target_probs.dtype
+                     for t in both), "probabilities must be float32, float16 or bfloat16, all of one dtype"),
+        (lambda: shape(node_uniforms, batch.num_rows), f"node uniforms must have shape [{batch.num_rows}]"),
+        (lambda: shape(sample_uniforms, batch.num_requests), f"sample uniforms must have shape [{batch.num_requests}]"),
+        (lambda: node_uniforms.dtype == sample_uniforms.dtype and node_uniforms.dtype in (torch.float32, torch.float64),
+         "uniforms must be float32 or float64, both of one dtype"),
+        (lambda: all(t.device == batch.device for t in (*both, node_uniforms, sample_uniforms)),
+         "probabilities and uniforms must be on the draft batch's device"),
+        (lambda: batch.max_token < vocab, "a draft token lies outside the vocabulary"),
+        (lambda: batch.num_requests <= 65535, "draft verification takes at most 65535 requests"),
+    )
+    for holds, message in rules:
+        if not holds():
+            raise ValueError(message)
+    rows = [t if t.stride(1) == 1 or vocab == 1 else t.contiguous() for t in both]
+    node_uniforms, sample_uniforms = node_uniforms.contiguous(), sample_uniforms.contiguous()
+    lib = native.load()
+    code, n = dtype_code(target_probs.dtype), batch.num_requests
+    device = batch.device
+    with on_device(device):
+        counts = torch.empty(n, dtype=torch.int32, device=device)
+        paths = torch.empty((n, batch.path_width), dtype=torch.int32, device=device)
+        tokens = torch.empty(n, dtype=torch.int64, device=device)
+        nbytes = lib.lvamd_verify_drafts_workspace_size(n, vocab, code)
+        workspace = torch.empty(nbytes, dtype=torch.uint8, device=device)
+        token_ptr, start_ptr, parent_ptr, sibling_ptr = batch._ptrs
+        native.check(lib.lvamd_verify_drafts(
+            rows[0].data_ptr(), rows[0].stride(0), rows[1].data_ptr() if len(rows) > 1 and batch.num_drafts else None,
+            rows[1].stride(0) if len(rows) > 1 else 0, vocab, code, start_ptr, token_ptr, parent_ptr, sibling_ptr, n,
+            node_uniforms.data_ptr(), sample_uniforms.data_ptr(), int(node_uniforms.dtype == torch.float64),
+            counts.data_ptr(), paths.data_ptr(), batch.path_width, tokens.data_ptr(), workspace.data_ptr(), nbytes,
+            current_stream(device)), "lvamd_verify_drafts")
+    return DraftVerdict(counts, paths, tokens)

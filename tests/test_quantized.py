@@ -1,0 +1,184 @@
+"""CPU tests of the 8-bit cache and draft verification: the oracle against
+torch's e4m3 and against the distribution it must keep, the drafts' packing,
+refusals, and the C entry points' argument checks (before any HIP call)."""
+
+from __future__ import annotations
+
+import ctypes
+
+import numpy as np
+import pytest
+import torch
+
+import light_vllm_amd as lv
+from light_vllm_amd import native
+from light_vllm_amd.verify import pack_drafts
+from oracle import quantized_oracle as Q
+
+X = ctypes.c_void_p(16)  # an address that no check dereferences
+
+
+def test_oracle_rounding_is_torchs_e4m3() -> None:
+    every = torch.arange(256, dtype=torch.uint8).view(torch.float8_e4m3fn).float()
+    every = every[every.isfinite()].unique()
+    middle = (every[1:] + every[:-1]) / 2  # ties
+    rng = np.random.default_rng(0)
+    x = torch.cat([every, middle, torch.from_numpy(rng.uniform(-448, 448, 4000).astype(np.float32)),
+                   torch.from_numpy((rng.standard_normal(4000) * 0.01).astype(np.float32))])
+    np.testing.assert_array_equal(Q.round_e4m3(x.double().numpy()), x.to(torch.float8_e4m3fn).double().numpy())
+
+
+@pytest.mark.parametrize("amax,e", [(0.0, -100), (448.0, 0), (448.1, 1), (449.0, 1), (224.0, -1), (1.0, -8), (1e-38, -100), (3.3e38, 120)])
+def test_scale_of_a_largest_magnitude(amax, e) -> None:
+    assert Q.scale_of(np.float32(amax)) == 2.0**e
+
+
+def test_token_at_a_time_gives_what_a_whole_prompt_gives() -> None:
+    # Exponent-only re-scaling: the same codes unless one became subnormal
+    # (magnitudes below 2^-6 of the block's final scale).
+    rng = np.random.default_rng(1)
+    rows = np.exp2(rng.integers(-3, 4, (16, 1, 1))) * rng.choice([-1, 1], (16, 2, 32)) * rng.uniform(1, 2, (16, 2, 32))
+    whole, ws = np.zeros((1, 16, 2, 32)), np.full((1, 2), 2.0**-100)
+    one, os_ = whole.copy(), ws.copy()
+    Q.append(whole, ws, rows, range(16), 61440.0)
+    for i in range(16):
+        Q.append(one, os_, rows[i : i + 1], [i], 61440.0)
+    np.testing.assert_array_equal(one, whole)
+    np.testing.assert_array_equal(os_, ws)
+
+
+@pytest.mark.parametrize("mode", ("chain", "tree"))
+def test_verified_tokens_follow_the_target(mode) -> None:
+    # The first emitted token over a grid of uniforms (and, for the chain, every
+    # drafted token with its draft probability) against p: each cell's share is
+    # exact to the grid's step per interval border.
+    rng = np.random.default_rng(2)
+    p, q = rng.dirichlet(np.ones(6)), rng.dirichlet(np.ones(6))
+    grid = (np.arange(200) + 0.5) / 200
+    found = np.zeros(6)
+    drafts = [((-1,), (t,), q[t]) for t in range(6)] if mode == "chain" else [((-1, -1, 0), (4, 1, 2), 1.0)]
+    target = np.stack([p] * 4)
+    for parents, tokens, weight in drafts:
+        probs = np.stack([q]) if mode == "chain" else None
+        for u in grid:
+            for s in grid:
+                path, token = Q.verify(parents, tokens, target, [u] * 4, s, probs)
+                found[tokens[path[0]] if path else token] += weight / grid.size**2
+    # Borders: one of u per drafted token, up to six of u'.
+    np.testing.assert_allclose(found, p, atol=7 / 200)
+
+
+def test_drafts_are_packed_with_their_earlier_siblings() -> None:
+    trees = [lv.DraftTree((7, 9, 8, 5), (-1, -1, 0, -1)), lv.DraftTree((), ()), lv.DraftTree((3, 4), (-1, 0))]
+    (tokens, starts, parents, siblings), chains, top = pack_drafts(trees)
+    assert tokens.view(np.int64).tolist() == [7, 9, 8, 5, 3, 4]
+    assert starts.tolist() == [0, 4, 4, 6]
+    assert parents.tolist() == [-1, -1, 0, -1, -1, 0]
+    assert siblings.tolist() == [-1, 0, -1, 1, -1, -1]
+    assert not chains and top == 9
+    assert pack_drafts(trees[1:])[1]
+    with pytest.raises(ValueError, match="at least one request"):
+        pack_drafts([])
+    n = native.VERIFY_MAX_DRAFTS
+    pack_drafts([lv.DraftTree(tuple(range(n)), tuple(range(-1, n - 1)))])
+    with pytest.raises(ValueError, match="at most 1024 drafts"):
+        pack_drafts([lv.DraftTree(tuple(range(n + 1)), tuple(range(-1, n)))])
+    with pytest.raises(ValueError, match="below 2"):
+        pack_drafts([lv.DraftTree((2**31,), (-1,))])
+
+
+def test_refusals_without_a_gpu() -> None:
+    spec = lv.ModelKVCacheSpec((lv.AttentionLayerSpec("a", 4, 2, 64),))
+    config = lambda **kw: lv.PagedKVCacheConfig(**{**dict(num_blocks=4, block_size=16, dtype=torch.bfloat16, device="cuda:0"), **kw})  # noqa: E731
+    with pytest.raises(lv.KVCacheError, match="requires a GPU"):
+        lv.QuantizedPagedKVCache(spec, config(device="cpu"))
+    with pytest.raises(lv.KVCacheError, match="bfloat16 or float16"):
+        lv.QuantizedPagedKVCache(spec, config(dtype=torch.float32))
+    with pytest.raises(lv.KVCacheError, match="at most 2"):
+        lv.QuantizedPagedKVCache(spec, config(num_blocks=2**27))
+    odd = lv.ModelKVCacheSpec((lv.AttentionLayerSpec("a", 4, 2, 40),))
+    with pytest.raises(lv.KVCacheError, match="head sizes"):
+        lv.QuantizedPagedKVCache(odd, config())
+    with pytest.raises(lv.ExecutionError, match="requires a GPU"):
+        lv.DraftBatch([lv.DraftTree((), ())], device="cpu")
+    mixed = lv.ModelKVCacheSpec((lv.AttentionLayerSpec("a", 4, 2, 64), lv.AttentionLayerSpec("b", 4, 1, 128)))
+    assert lv.quantized_kv_cache_bytes_per_block(mixed, block_size=16) == 2 * (2 * (16 * 64 + 4) + 16 * 128 + 4)
+
+
+def test_append_entry_point_checks() -> None:
+    lib = native.load()
+
+    def call(key=X, strides=(256, 128), pool=X, n=4, heads=2, d=128, bs=16, dtype=2):
+        return lib.lvamd_kv_append_q8(key, *strides, X, 256, 128, pool, X, X, X, X, None, n, heads, d, bs, dtype, None)
+
+    assert call(n=0) == 0
+    assert call(dtype=0) == -2 and call(dtype=7) == -2 and call(d=40) == -2 and call(d=272) == -2
+    for bad in (dict(key=None), dict(pool=None), dict(n=-1), dict(heads=0), dict(bs=0), dict(strides=(4, 128)),
+                dict(strides=(256, 12)), dict(key=ctypes.c_void_p(8)), dict(pool=ctypes.c_void_p(24))):
+        assert call(**bad) == -1, bad
+
+
+def test_attention_entry_point_checks() -> None:
+    lib = native.load()
+    f = ctypes.c_float(0.1)
+
+    def decode(q=X, waves=1, slots=0, heads=4, group=7, d=128, bs=16, dtype=2, qs=(3584, 128), part=None):
+        return lib.lvamd_paged_decode_q8(q, *qs, X, X, X, X, X, 3584, 128, X, X, waves, X, X, part, part, slots, heads, group, d,
+                                         bs, f, dtype, None)
+
+    def prefill(q=X, units=1, slots=0, heads=4, group=7, d=128, bs=16, dtype=2, qs=(3584, 128), part=None):
+        return lib.lvamd_paged_prefill_q8(q, *qs, X, X, X, X, X, 3584, 128, X, X, X, units, part, part, slots, heads, group, d,
+                                          bs, f, dtype, None)
+
+    for call, none in ((decode, "waves"), (prefill, "units")):
+        assert call(**{none: 0}) == 0
+        assert call(dtype=0) == -2 and call(d=24) == -2 and call(d=264) == -2
+        for bad in (dict(q=None), dict(heads=0), dict(group=0), dict(bs=0), dict(qs=(3580, 128)), {none: -1}):
+            assert call(**bad) == -1, bad
+        assert call(slots=3) == -3
+    assert decode(group=17) == -1
+    for d in (32, 64, 80, 128, 256):
+        assert lib.lvamd_paged_decode_q8_tile_tokens(2, d) * d <= 8192
+        assert lib.lvamd_paged_prefill_q8_key_tokens(1, d) == (64 if d <= 128 else 32)
+    assert lib.lvamd_paged_decode_q8_tile_tokens(0, 128) == -2 and lib.lvamd_paged_prefill_q8_key_tokens(2, 40) == -2
+    plan = native.AttentionPlanQ8(base=native.AttentionPlan(num_kv_heads=4, group=7, head_size=128, block_size=16, dtype=2))
+    empty = (None, 0, 0, None, 0, 0)
+    call = lambda p, kv=empty, pool=X: lib.lvamd_paged_attention_q8(p, X, 0, 0, *kv, pool, X, X, 0, 0, f, None)  # noqa: E731
+    assert call(None) == -1
+    assert call(ctypes.addressof(plan)) == 0  # nothing to append, no rows
+    assert call(ctypes.addressof(plan), pool=None) == -1
+    assert call(ctypes.addressof(plan), kv=(X, 0, 0, None, 0, 0)) == -1
+    plan.scale_offset = 24
+    assert call(ctypes.addressof(plan)) == -1
+
+
+def test_compact_entry_point_checks() -> None:
+    lib = native.load()
+
+    def call(keys=X, layers=2, heads=2, d=128, bs=16, offset=1024, n=3, groups=1, ws=X, nbytes=1 << 20):
+        return lib.lvamd_kv_compact_q8(keys, X, layers, heads, d, bs, offset, X, X, n, X, groups, ws, nbytes, None)
+
+    assert call(n=0, groups=0) == 0
+    assert call(d=40) == -2
+    for bad in (dict(keys=None), dict(layers=0), dict(heads=0), dict(bs=0), dict(offset=-4), dict(offset=2), dict(n=-1),
+                dict(groups=0), dict(groups=4), dict(n=0, groups=1)):
+        assert call(**bad) == -1, bad
+    need = lib.lvamd_kv_compact_q8_workspace_size(3, 2, 2, 128)
+    assert need == 3 * 2 * 2 * 2 * (128 + 4) and lib.lvamd_kv_compact_q8_workspace_size(0, 2, 2, 128) == 0
+    assert call(ws=None) == -3 and call(nbytes=need - 1) == -3 and call(ws=ctypes.c_void_p(8)) == -3
+
+
+def test_verify_entry_point_checks() -> None:
+    lib = native.load()
+
+    def call(target=X, stride=100, vocab=100, dtype=0, starts=X, n=2, width=1, ws=X, nbytes=1 << 20):
+        return lib.lvamd_verify_drafts(target, stride, None, 0, vocab, dtype, starts, X, X, X, n, X, X, 0, X, X, width, X, ws,
+                                       nbytes, None)
+
+    assert call(n=0) == 0
+    assert call(dtype=3) == -2
+    for bad in (dict(target=None), dict(starts=None), dict(vocab=0), dict(vocab=(1 << 30) + 1), dict(n=-1), dict(n=65536),
+                dict(width=0), dict(stride=-1)):
+        assert call(**bad) == -1, bad
+    need = lib.lvamd_verify_drafts_workspace_size(2, 100, 0)
+    assert need > 0 and call(nbytes=need - 1) == -3 and call(ws=None) == -3 and call(ws=ctypes.c_void_p(4)) == -3
