@@ -83,7 +83,7 @@ __device__ __forceinline__ Q8Piece read_q8_piece(const int32_t* __restrict__ pie
 }  // namespace
 
 template <typename T, int D>
-__global__ __launch_bounds__(64) void q8_decode_kernel(const int32_t* __restrict__ wave_first,
+__global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(1, 1))) void q8_decode_kernel(const int32_t* __restrict__ wave_first,
                                                        const int32_t* __restrict__ pieces, const int32_t waves_per_head,
                                                        const uint32_t wg_magic, const int32_t wg_shift,
                                                        const Q8DecodeArgs a) {
@@ -110,10 +110,12 @@ __global__ __launch_bounds__(64) void q8_decode_kernel(const int32_t* __restrict
   gptr<const float> const kscales = (gptr<const float>)(a.k_scales) + kvh;
   gptr<const float> const vscales = (gptr<const float>)(a.v_scales) + kvh;
 
-  // This lane's rows of a tile: their physical slots and the index of their
-  // blocks' scales.  Rows past the piece repeat its last one (masked).
+  // This lane's rows of a tile: their blocks and offsets in them.  (The slot is
+  // made of them where the codes are requested: here it would wait for the
+  // table's load, and with it for the tile's loads before it.)  Rows past the
+  // piece repeat its last one (masked).
   struct Rows {
-    int slot[SPL], block[SPL];
+    int block[SPL], off[SPL];
   };
   auto lookup = [&](int table_off, int t0, int tok_end) -> Rows {
     Rows r;
@@ -122,7 +124,7 @@ __global__ __launch_bounds__(64) void q8_decode_kernel(const int32_t* __restrict
       const int pos = min(t0 + 64 * i + lane, tok_end - 1);
       const int lb = fast_div(pos, a.by_block);
       r.block[i] = a.tables[table_off + lb];
-      r.slot[i] = r.block[i] * a.block_size + (pos - lb * a.block_size);
+      r.off[i] = pos - lb * a.block_size;
     }
     return r;
   };
@@ -141,49 +143,59 @@ __global__ __launch_bounds__(64) void q8_decode_kernel(const int32_t* __restrict
     float ks[SPL], vs[SPL];
   };
   auto issue = [&](const Rows& r, Tile& t) {
+    // (The scales first: loads return in order, and every row's conversion
+    // needs one.)
+    int slot[SPL];
+#pragma unroll
+    for (int i = 0; i < SPL; ++i) {
+      slot[i] = r.block[i] * a.block_size + r.off[i];
+      const int64_t at = (int64_t)r.block[i] * Hkv;
+      t.ks[i] = kscales[at];
+      t.vs[i] = vscales[at];
+    }
 #pragma unroll
     for (int j = 0; j < LPT; ++j) {
       const int id = lane + 64 * j;
       const int row = id / C8, c = id - row * C8;
-      const int64_t off = (int64_t)shuffled(r.slot, row & (TT - 1)) * row_bytes + 16 * c;
+      const int64_t off = (int64_t)shuffled(slot, row & (TT - 1)) * row_bytes + 16 * c;
       t.k[j] = t.v[j] = zero_u4();
       if (64 * LPT == TT * C8 || row < TT) {
         t.k[j] = load16_stream(kbase + off);
         t.v[j] = load16_stream(vbase + off);
       }
     }
-#pragma unroll
-    for (int i = 0; i < SPL; ++i) {
-      const int64_t at = (int64_t)r.block[i] * Hkv;
-      t.ks[i] = kscales[at];
-      t.vs[i] = vscales[at];
-    }
   };
   // Tile into LDS as T.  Rows from first_new on hold this step's tokens: their
   // NaN values are left out (returns whether there were any).
-  auto stage = [&](const Tile& t, int first_new) -> bool {
+  auto stage_rows = [&]<bool NEW>(const Tile& t, int first_new) __attribute__((always_inline)) -> bool {
     bool any = false;
 #pragma unroll
     for (int j = 0; j < LPT; ++j) {
       const int id = lane + 64 * j;
       const int row = id / C8, c = id - row * C8;
       const float ks = shuffled(t.ks, row & (TT - 1)), vs = shuffled(t.vs, row & (TT - 1));
+      uint4 v = t.v[j];
+      if constexpr (NEW) {
+        const bool nan = row >= first_new && q8_has_nan(v);
+        any |= nan;
+        v = make_uint4(nan ? q8_without_nan4(v.x) : v.x, nan ? q8_without_nan4(v.y) : v.y,
+                       nan ? q8_without_nan4(v.z) : v.z, nan ? q8_without_nan4(v.w) : v.w);
+      }
+      uint4 klo, khi, vlo, vhi;
+      q8_values16<T>(t.k[j], ks, klo, khi);
+      q8_values16<T>(v, vs, vlo, vhi);
       if (64 * LPT == TT * C8 || row < TT) {
-        uint4 v = t.v[j];
-        if (first_new < TT && row >= first_new && q8_has_nan(v)) {
-          any = true;
-          v = make_uint4(q8_without_nan4(v.x), q8_without_nan4(v.y), q8_without_nan4(v.z), q8_without_nan4(v.w));
-        }
-        uint4 lo, hi;
-        q8_values16<T>(t.k[j], ks, lo, hi);
-        klds[row * RS + 2 * c] = lo;
-        klds[row * RS + 2 * c + 1] = hi;
-        q8_values16<T>(v, vs, lo, hi);
-        vlds[row * RS + 2 * c] = lo;
-        vlds[row * RS + 2 * c + 1] = hi;
+        klds[row * RS + 2 * c] = klo;
+        klds[row * RS + 2 * c + 1] = khi;
+        vlds[row * RS + 2 * c] = vlo;
+        vlds[row * RS + 2 * c + 1] = vhi;
       }
     }
-    return first_new < TT && __any(any);
+    return NEW && __any(any);
+  };
+  auto stage = [&](const Tile& t, int first_new) -> bool {
+    if (first_new >= TT) return stage_rows.template operator()<false>(t, first_new);
+    return stage_rows.template operator()<true>(t, first_new);
   };
 
   // This lane's column: query qi, head qhead, and which of the step's tokens
@@ -239,7 +251,6 @@ __global__ __launch_bounds__(64) void q8_decode_kernel(const int32_t* __restrict
   advance(at);
   if (at.p < p_end) rows = lookup(at.table_off, at.t0, at.tok_end);
   int t0 = cur.tok_begin;
-  bool poisoned = stage(tile, cur.computed - t0);
 
   float m_run = -INFINITY, l_run = 0.f;
   f32x4 acc[NT];
@@ -250,6 +261,7 @@ __global__ __launch_bounds__(64) void q8_decode_kernel(const int32_t* __restrict
   Column ncol = col;
   uint4 qn[NCH];
   while (true) {
+    const bool poisoned = stage(tile, cur.computed - t0);
     // The next tile's codes, the rows of the one after it and, where the next
     // tile starts a piece, that piece's record and queries.
     const bool has_next = at.p < p_end;
@@ -288,7 +300,8 @@ __global__ __launch_bounds__(64) void q8_decode_kernel(const int32_t* __restrict
         for (int r = 0; r < 4; ++r) {
           const int pos = t0 + 16 * s + 4 * g + r;
           const int j = pos - cur.computed;
-          const bool vis = pos < cur.tok_end && (j < 0 || ((col.sees >> (j & 31)) & 1u));
+          const bool seen = (int)(j < 0) | (int)((col.sees >> (j & 31)) & 1u);
+          const bool vis = (int)seen & (int)(pos < cur.tok_end);
           st[s][r] = vis ? st[s][r] * a.scale_log2 : -INFINITY;
         }
     } else {
@@ -385,7 +398,6 @@ __global__ __launch_bounds__(64) void q8_decode_kernel(const int32_t* __restrict
       for (int n = 0; n < NT; ++n) acc[n] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
     t0 = nt0;
-    poisoned = stage(tile, cur.computed - t0);
   }
 }
 
