@@ -609,6 +609,13 @@ int lvamd_kv_compact_q8(const uint64_t* layer_key_ptrs, const uint64_t* layer_va
                         int64_t scale_offset, const int64_t* src_slots, const int64_t* dst_slots, int64_t num_pairs,
                         const int64_t* block_starts, int64_t num_dst_blocks,
                         void* workspace, int64_t workspace_bytes, lvamd_stream_t stream);
+/* The same for at most lvamd_kv_compact_q8_few_pairs() pairs given in HOST
+ * memory (grouped by destination block too): one launch, no workspace. */
+int lvamd_kv_compact_q8_few(const uint64_t* layer_key_ptrs, const uint64_t* layer_value_ptrs,
+                            int32_t num_layers, int32_t num_kv_heads, int32_t head_size, int32_t block_size,
+                            int64_t scale_offset, const int64_t* src_slots, const int64_t* dst_slots,
+                            int64_t num_pairs, lvamd_stream_t stream);
+int64_t lvamd_kv_compact_q8_few_pairs(void);
 int64_t lvamd_kv_compact_q8_workspace_size(int64_t num_pairs, int32_t num_layers, int32_t num_kv_heads,
                                            int32_t head_size);
 
@@ -633,7 +640,9 @@ int64_t lvamd_kv_compact_q8_workspace_size(int64_t num_pairs, int32_t num_layers
  *
  * counts[r]: drafts accepted; paths[r][0..path_width): their indices within the
  * request, then -1 (path_width at least the longest request's drafts, and 1);
- * out_tokens[r]: the drawn token.  workspace: device memory, 8-byte aligned.
+ * out_tokens[r]: the drawn token.  num_drafts: all requests' together.  workspace: device
+ * memory, 16-byte aligned, of
+ * lvamd_verify_drafts_workspace_size(...) bytes.
  *
  * Replaces: GreedyTreeAcceptanceSampler.accept
  *   (src/light_vllm/runtime/execution/speculative.py:220-257), which takes the
@@ -643,10 +652,10 @@ int64_t lvamd_kv_compact_q8_workspace_size(int64_t num_pairs, int32_t num_layers
 int lvamd_verify_drafts(const void* target, int64_t target_row_stride, const void* draft_probs,
                         int64_t draft_row_stride, int32_t vocab, int32_t dtype, const int32_t* draft_starts,
                         const int64_t* draft_tokens, const int32_t* parents, const int32_t* siblings,
-                        int64_t num_requests, const void* node_uniforms, const void* sample_uniforms,
+                        int64_t num_requests, int64_t num_drafts, const void* node_uniforms, const void* sample_uniforms,
                         int32_t uniforms_f64, int32_t* counts, int32_t* paths, int32_t path_width,
                         int64_t* out_tokens, void* workspace, int64_t workspace_bytes, lvamd_stream_t stream);
-int64_t lvamd_verify_drafts_workspace_size(int64_t num_requests, int32_t vocab, int32_t dtype);
+int64_t lvamd_verify_drafts_workspace_size(int64_t num_requests, int64_t num_drafts, int32_t vocab, int32_t dtype);
 
 #ifdef __cplusplus
 }

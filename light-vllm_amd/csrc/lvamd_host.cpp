@@ -2362,6 +2362,205 @@ PyObject* attend_rotary(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   return PyLong_FromLong(status);
 }
 
+// ---------------------------------------------------------------------------
+// append_tensors(facts, key, value, slots, sources, num_slots, tokens) -> status,
+// or kNotFast
+//
+// The 8-bit cache's write in one call, as attend_tensors: facts = (fn, dtype
+// object, device index, element size, kv heads, head size, block size, dtype
+// code, key pool, key scales, value pool, value scales, raw-stream getter), made
+// once per layer; slots and sources are device addresses (0: no sources).
+// ---------------------------------------------------------------------------
+typedef int (*AppendQ8Fn)(const void*, int64_t, int64_t, const void*, int64_t, int64_t, void*, float*, void*, float*,
+                          const int64_t*, const int64_t*, int64_t, int32_t, int32_t, int32_t, int32_t, void*);
+
+// The raw handle of a device's current stream, or -1 with a Python error.
+int64_t raw_stream(PyObject* getter, long device) {
+  PyObject* dev = PyLong_FromLong(device);
+  if (dev == nullptr) return -1;
+  PyObject* stream = PyObject_CallOneArg(getter, dev);
+  Py_DECREF(dev);
+  if (stream == nullptr) return -1;
+  const int64_t s = PyLong_AsLongLong(stream);
+  Py_DECREF(stream);
+  return s;
+}
+
+PyObject* append_tensors(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  if (!want_args(nargs, 7, "append_tensors")) return nullptr;
+  PyObject* b = args[0];
+  if (!PyTuple_Check(b) || PyTuple_GET_SIZE(b) != 13) {
+    PyErr_SetString(PyExc_ValueError, "append_tensors: facts must be a 13-tuple");
+    return nullptr;
+  }
+  int64_t f[13];
+  for (int i = 0; i < 12; ++i) {
+    if (i == 1) continue;
+    f[i] = (int64_t)PyLong_AsLongLong(PyTuple_GET_ITEM(b, i));
+  }
+  int64_t v[4];
+  for (int i = 0; i < 4; ++i) v[i] = (int64_t)PyLong_AsLongLong(args[3 + i]);
+  if (PyErr_Occurred()) return nullptr;
+  if (f[0] == 0) {
+    PyErr_SetString(PyExc_ValueError, "append_tensors: null function");
+    return nullptr;
+  }
+  PyObject* dtype = PyTuple_GET_ITEM(b, 1);
+  int64_t kp, ks0, ks1, vp, vs0, vs1;
+  int r = tensor_facts(args[1], dtype, (long)f[2], v[3], f[4], f[5], f[3], &kp, &ks0, &ks1);
+  if (r == 1) r = tensor_facts(args[2], dtype, (long)f[2], v[3], f[4], f[5], f[3], &vp, &vs0, &vs1);
+  if (r < 0) return nullptr;
+  if (r == 0) return PyLong_FromLong(kNotFast);
+  const int64_t stream = raw_stream(PyTuple_GET_ITEM(b, 12), (long)f[2]);
+  if (PyErr_Occurred()) return nullptr;
+  const AppendQ8Fn fn = reinterpret_cast<AppendQ8Fn>((intptr_t)f[0]);
+  const int status = fn(as_ptr(kp), ks0, ks1, as_ptr(vp), vs0, vs1, as_ptr(f[8]), static_cast<float*>(as_ptr(f[9])),
+                        as_ptr(f[10]), static_cast<float*>(as_ptr(f[11])), static_cast<const int64_t*>(as_ptr(v[0])),
+                        static_cast<const int64_t*>(as_ptr(v[1])), v[2], (int32_t)f[4], (int32_t)f[5], (int32_t)f[6],
+                        (int32_t)f[7], as_ptr(stream));
+  return PyLong_FromLong(status);
+}
+
+// ---------------------------------------------------------------------------
+// block_runs(moved, dst, block_size) -> (rule, starts)
+//
+// The runs of equal destination block in a compact's pairs (moved: int64 pairs
+// per request, dst: int64 slots; bytes objects): starts as int64 bytes, one per
+// run and the end.  Rule 1: a block in two runs (two requests').
+// ---------------------------------------------------------------------------
+PyObject* block_runs(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  if (!want_args(nargs, 3, "block_runs")) return nullptr;
+  const int64_t bs = PyLong_AsLongLong(args[2]);
+  if (PyErr_Occurred()) return nullptr;
+  if (!PyBytes_Check(args[0]) || !PyBytes_Check(args[1]) || bs <= 0) {
+    PyErr_SetString(PyExc_ValueError, "block_runs: moved and dst must be bytes, block_size positive");
+    return nullptr;
+  }
+  const int64_t* moved = reinterpret_cast<const int64_t*>(PyBytes_AS_STRING(args[0]));
+  const int64_t* dst = reinterpret_cast<const int64_t*>(PyBytes_AS_STRING(args[1]));
+  const int64_t requests = PyBytes_GET_SIZE(args[0]) / 8, n = PyBytes_GET_SIZE(args[1]) / 8;
+  std::vector<int64_t> starts, blocks;
+  int64_t i = 0;
+  for (int64_t r = 0; r < requests; ++r) {
+    if (moved[r] < 0 || moved[r] > n - i) break;
+    for (const int64_t first = i, end = i + moved[r]; i < end; ++i) {
+      const int64_t block = dst[i] / bs;
+      if (i > first && block == blocks.back()) continue;
+      blocks.push_back(block);
+      starts.push_back(i);
+    }
+  }
+  if (i != n) {
+    PyErr_SetString(PyExc_ValueError, "block_runs: the counts do not match the pairs");
+    return nullptr;
+  }
+  starts.push_back(n);
+  std::sort(blocks.begin(), blocks.end());
+  const bool twice = std::adjacent_find(blocks.begin(), blocks.end()) != blocks.end();
+  return Py_BuildValue("(iy#)", twice ? 1 : 0, reinterpret_cast<const char*>(starts.data()),
+                       (Py_ssize_t)(starts.size() * sizeof(int64_t)));
+}
+
+// ---------------------------------------------------------------------------
+// verify_tensors(facts, outputs, target, node_uniforms, sample_uniforms,
+//                draft_probs, vocab, dtype object, dtype code) -> status, or kNotFast
+//
+// verify_drafts' launch in one call: reads the tensors' dtypes, devices, shapes,
+// strides and pointers and, when every rule holds, calls lvamd_verify_drafts.
+// facts = (fn, device index, rows, drafts, requests, path width, starts, tokens,
+// parents, siblings, fp32 dtype, fp64 dtype, raw-stream getter), made once per
+// batch; outputs = (counts, paths, tokens, workspace, workspace bytes)
+// addresses.  draft_probs: a tensor, or None.
+// ---------------------------------------------------------------------------
+typedef int (*VerifyFn)(const void*, int64_t, const void*, int64_t, int32_t, int32_t, const int32_t*, const int64_t*,
+                        const int32_t*, const int32_t*, int64_t, int64_t, const void*, const void*, int32_t, int32_t*,
+                        int32_t*, int32_t, int64_t*, void*, int64_t, void*);
+
+// 1: t is a contiguous vector of n of the dtype and device, 0: it is not, -1: a
+// Python error.
+int vector_facts(PyObject* t, PyObject* dtype, long device, int64_t n, int64_t* ptr) {
+  PyObject* dt = PyObject_GetAttr(t, g_str_dtype);
+  if (dt == nullptr) return -1;
+  Py_DECREF(dt);
+  if (dt != dtype) return 0;
+  PyObject* dev = PyObject_CallMethodNoArgs(t, g_str_get_device);
+  if (dev == nullptr) return -1;
+  const long at = PyLong_AsLong(dev);
+  Py_DECREF(dev);
+  PyObject* shape = PyObject_GetAttr(t, g_str_shape);
+  if (shape == nullptr) return -1;
+  const bool fits = PyTuple_Check(shape) && PyTuple_GET_SIZE(shape) == 1 &&
+                    PyLong_AsLongLong(PyTuple_GET_ITEM(shape, 0)) == n;
+  Py_DECREF(shape);
+  PyObject* stride = PyObject_CallMethodNoArgs(t, g_str_stride);
+  if (stride == nullptr) return -1;
+  const bool packed = PyTuple_Check(stride) && PyTuple_GET_SIZE(stride) == 1 &&
+                      PyLong_AsLongLong(PyTuple_GET_ITEM(stride, 0)) == 1;
+  Py_DECREF(stride);
+  if (PyErr_Occurred()) return -1;
+  if (!fits || !packed || at != device) return 0;
+  PyObject* dp = PyObject_CallMethodNoArgs(t, g_str_data_ptr);
+  if (dp == nullptr) return -1;
+  *ptr = PyLong_AsLongLong(dp);
+  Py_DECREF(dp);
+  return PyErr_Occurred() ? -1 : 1;
+}
+
+// A failed read of an argument that is no tensor is no error: the general path
+// has the message.
+int unless_no_tensor(int r) {
+  if (r < 0 && (PyErr_ExceptionMatches(PyExc_AttributeError) || PyErr_ExceptionMatches(PyExc_TypeError))) {
+    PyErr_Clear();
+    return 0;
+  }
+  return r;
+}
+
+PyObject* verify_tensors(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  if (!want_args(nargs, 9, "verify_tensors")) return nullptr;
+  PyObject *b = args[0], *o = args[1];
+  if (!PyTuple_Check(b) || PyTuple_GET_SIZE(b) != 13 || !PyTuple_Check(o) || PyTuple_GET_SIZE(o) != 5) {
+    PyErr_SetString(PyExc_ValueError, "verify_tensors: facts must be a 13-tuple, outputs a 5-tuple");
+    return nullptr;
+  }
+  int64_t f[10], out[5];
+  for (int i = 0; i < 10; ++i) f[i] = (int64_t)PyLong_AsLongLong(PyTuple_GET_ITEM(b, i));
+  for (int i = 0; i < 5; ++i) out[i] = (int64_t)PyLong_AsLongLong(PyTuple_GET_ITEM(o, i));
+  const int64_t vocab = PyLong_AsLongLong(args[6]), code = PyLong_AsLongLong(args[8]);
+  if (PyErr_Occurred()) return nullptr;
+  if (f[0] == 0) {
+    PyErr_SetString(PyExc_ValueError, "verify_tensors: null function");
+    return nullptr;
+  }
+  const long device = (long)f[1];
+  int64_t tp, ts, qp = 0, qs = 0, np, sp;
+  int r = row_facts(args[2], args[7], device, f[2], vocab, &tp, &ts);
+  if (r == 1 && args[5] != Py_None) r = row_facts(args[5], args[7], device, f[3], vocab, &qp, &qs);
+  r = unless_no_tensor(r);
+  if (r < 0) return nullptr;
+  if (r == 0) return PyLong_FromLong(kNotFast);
+  int64_t f64 = 0;
+  r = vector_facts(args[3], PyTuple_GET_ITEM(b, 10), device, f[2], &np);
+  if (r == 0) {
+    f64 = 1;
+    r = vector_facts(args[3], PyTuple_GET_ITEM(b, 11), device, f[2], &np);
+  }
+  if (r == 1) r = vector_facts(args[4], PyTuple_GET_ITEM(b, f64 ? 11 : 10), device, f[4], &sp);
+  r = unless_no_tensor(r);
+  if (r < 0) return nullptr;
+  if (r == 0) return PyLong_FromLong(kNotFast);
+  const int64_t stream = raw_stream(PyTuple_GET_ITEM(b, 12), device);
+  if (PyErr_Occurred()) return nullptr;
+  const VerifyFn fn = reinterpret_cast<VerifyFn>((intptr_t)f[0]);
+  const int status = fn(as_ptr(tp), ts, f[3] > 0 ? as_ptr(qp) : nullptr, qs, (int32_t)vocab, (int32_t)code,
+                        static_cast<const int32_t*>(as_ptr(f[6])), static_cast<const int64_t*>(as_ptr(f[7])),
+                        static_cast<const int32_t*>(as_ptr(f[8])), static_cast<const int32_t*>(as_ptr(f[9])), f[4], f[3],
+                        as_ptr(np), as_ptr(sp), (int32_t)f64, static_cast<int32_t*>(as_ptr(out[0])),
+                        static_cast<int32_t*>(as_ptr(out[1])), (int32_t)f[5], static_cast<int64_t*>(as_ptr(out[2])),
+                        as_ptr(out[3]), out[4], as_ptr(stream));
+  return PyLong_FromLong(status);
+}
+
 PyMethodDef kMethods[] = {
     {"flatten", (PyCFunction)(void (*)(void))flatten, METH_FASTCALL, "int sequences -> (flat, counts int64, status)"},
     {"validate", (PyCFunction)(void (*)(void))validate, METH_FASTCALL, "block-table rules -> (rule, request)"},
@@ -2379,6 +2578,11 @@ PyMethodDef kMethods[] = {
      "forward's fast path: tensor rules and the lvamd_paged_attention call"},
     {"attend_rotary", (PyCFunction)(void (*)(void))attend_rotary, METH_FASTCALL,
      "forward's fast path with rotary: the rotary append, then lvamd_paged_attention"},
+    {"append_tensors", (PyCFunction)(void (*)(void))append_tensors, METH_FASTCALL,
+     "the 8-bit cache's write: tensor rules and the lvamd_kv_append_q8 call"},
+    {"block_runs", (PyCFunction)(void (*)(void))block_runs, METH_FASTCALL, "destination-block runs of a compact's pairs"},
+    {"verify_tensors", (PyCFunction)(void (*)(void))verify_tensors, METH_FASTCALL,
+     "verify_drafts' rules and the lvamd_verify_drafts call"},
     {nullptr, nullptr, 0, nullptr},
 };
 

@@ -5,6 +5,7 @@
 // holds one scale per kv head, 2^e with e the smallest exponent that brings
 // the largest magnitude of its rows within 448 (lvamd_q8.h).
 
+#include <algorithm>
 #include <cmath>
 
 #include "lvamd_q8.h"
@@ -30,9 +31,15 @@ __device__ __forceinline__ void stores_done() { asm volatile("s_waitcnt vmcnt(0)
 //   anew (its offset 0 is in the run), else max(old, 2^e(amax)); if that is
 //   above the old scale, the block's rows are re-scaled by old / new; then the
 //   run's codes and the scale.
-// A token whose predecessor in the list is in the same block leaves the work
-// to the run's first token: n x (units / 4) workgroups, of which a prompt's
-// exit at once but for one per block.
+//
+// The waves find the runs themselves: a workgroup looks at a window of 64
+// entries of the list, one per lane, and a ballot marks those whose
+// predecessor is in another block.  The window's (run, unit) tasks go round
+// robin over the waves of gridDim.y workgroups, enough of them that a window
+// of single tokens (64 runs) has few tasks per wave; a prompt's window has few
+// runs and most of its workgroups exit at once.  (With a workgroup per entry,
+// the runs of a prompt's blocks of 16 all began on workgroups of one XCD: 2,048
+// tokens 17 us against 7 for the same tokens in 128 requests.)
 //
 // HBM-bound for prompts (each row read once and held in registers, up to
 // kHeld passes of 64 lanes; longer runs read their later rows again), a chain
@@ -52,41 +59,41 @@ struct Q8AppendArgs {
   int32_t num_kv_heads;
   int32_t head_size;
   int32_t block_size;
-  FastDiv by_block, by_lanes;  // / block_size, / lanes per row
+  FastDiv by_block, by_lanes, by_units;  // / block_size, / lanes per row, / (K and V, kv heads)
 };
 
 constexpr int kHeld = 4;  // passes of rows that stay in registers
 constexpr int kAppendWaves = 4;
 
 template <typename T>
-__global__ __launch_bounds__(64 * kAppendWaves) void q8_append_kernel(const int64_t* __restrict__ slots,
-                                                                      const Q8AppendArgs a) {
-  const int lane = threadIdx.x & 63;
-  const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-  const int64_t i0 = blockIdx.x;
-  const int unit = blockIdx.y * kAppendWaves + wave;
-  const int64_t slot0 = slots[i0];
-  if (slot0 < 0 || unit >= 2 * a.num_kv_heads) return;
+__device__ __forceinline__ void append_run(const Q8AppendArgs& a, const int64_t* __restrict__ slots, int lane,
+                                           int64_t base, uint64_t leads, uint64_t ends, uint64_t zeros, int my_block,
+                                           int task) {
   const int bs = a.block_size;
-  const int block = fast_div((int)slot0, a.by_block);
-  if (i0 > 0) {
-    const int64_t before = slots[i0 - 1];
-    if (before >= 0 && fast_div((int)before, a.by_block) == block) return;  // not the run's first token
-  }
-  // The run: how many slots from here on lie in the block, and whether one is
-  // its offset 0.
-  int n = 0;
-  bool fresh = false;
-  for (;; n += 64) {
-    const int64_t i = i0 + n + lane;
-    const int64_t s = i < a.num_slots && n + lane < bs ? slots[i] : -1;
-    const bool in = s >= 0 && fast_div((int)s, a.by_block) == block;
-    const uint64_t out = ~__ballot(in);
-    const int len = out == 0 ? 64 : __builtin_ctzll(out);
-    fresh |= __any(in && lane < len && (int)s - block * bs == 0);
-    if (len < 64) {
-      n += len;
-      break;
+  const int run = fast_div(task, a.by_units);
+  const int unit = task - run * 2 * a.num_kv_heads;
+  // The run's first entry, the run-th of the window's.
+  for (int i = 0; i < run; ++i) leads &= leads - 1;
+  const int l = __builtin_ctzll(leads);
+  const int64_t i0 = base + l;
+  const int block = __builtin_amdgcn_readlane(my_block, l);
+  // Its length, and whether it holds the block's offset 0.
+  const uint64_t after = l < 63 ? ends >> (l + 1) : 0;
+  int n = after ? __builtin_ctzll(after) + 1 : 64 - l;
+  bool fresh = ((zeros >> l) & (n < 64 ? ((uint64_t)1 << n) - 1 : ~(uint64_t)0)) != 0;
+  if (l + n == 64) {
+    // On into the next windows.
+    for (;; n += 64) {
+      const int64_t i = i0 + n + lane;
+      const int64_t s = i < a.num_slots ? slots[i] : -1;
+      const bool in = s >= 0 && fast_div((int)s, a.by_block) == block;
+      const uint64_t out = ~__ballot(in);
+      const int len = out == 0 ? 64 : __builtin_ctzll(out);
+      fresh |= __any(in && lane < len && (int)s == block * bs);
+      if (len < 64) {
+        n += len;
+        break;
+      }
     }
   }
   const bool is_v = unit >= a.num_kv_heads;
@@ -110,6 +117,7 @@ __global__ __launch_bounds__(64 * kAppendWaves) void q8_append_kernel(const int6
   };
   auto row_of = [&](int pass) -> int { return r0 < R ? pass * R + r0 : n; };  // n: none
   uint4 held[kHeld];
+  int64_t to[kHeld];
   float amax = 0.f;
   auto largest = [&](uint4 v) {
     T x[8];
@@ -121,7 +129,10 @@ __global__ __launch_bounds__(64 * kAppendWaves) void q8_append_kernel(const int6
     }
   };
 #pragma unroll
-  for (int p = 0; p < kHeld; ++p) held[p] = row_of(p) < n ? load(row_of(p)) : zero_u4();
+  for (int p = 0; p < kHeld; ++p) {
+    held[p] = row_of(p) < n ? load(row_of(p)) : zero_u4();
+    to[p] = row_of(p) < n ? slots[i0 + row_of(p)] : 0;
+  }
 #pragma unroll
   for (int p = 0; p < kHeld; ++p) largest(held[p]);
   for (int p = kHeld; p * R < n; ++p)
@@ -141,22 +152,42 @@ __global__ __launch_bounds__(64 * kAppendWaves) void q8_append_kernel(const int6
     }
     stores_done();
   }
-  auto store = [&](int r, uint4 v) {
+  auto store = [&](int64_t s, uint4 v) {
     T x[8];
     __builtin_memcpy(x, &v, 16);
     float f[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) f[e] = q8_scaled<T>(to_f32(x[e]), inverse);
-    const int64_t s = slots[i0 + r];
     *reinterpret_cast<uint2*>(pool + s * row_bytes + 8 * c) =
         make_uint2(q8_pack4(f[0], f[1], f[2], f[3]), q8_pack4(f[4], f[5], f[6], f[7]));
   };
 #pragma unroll
   for (int p = 0; p < kHeld; ++p)
-    if (row_of(p) < n) store(row_of(p), held[p]);
+    if (row_of(p) < n) store(to[p], held[p]);
   for (int p = kHeld; p * R < n; ++p)
-    if (row_of(p) < n) store(row_of(p), load(row_of(p)));
+    if (row_of(p) < n) store(slots[i0 + row_of(p)], load(row_of(p)));
   if (lane == 0) *scale_at = scale;
+}
+
+template <typename T>
+__global__ __launch_bounds__(64 * kAppendWaves) void q8_append_kernel(const int64_t* __restrict__ slots,
+                                                                      const Q8AppendArgs a) {
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+  const int bs = a.block_size;
+  const int units = 2 * a.num_kv_heads;
+  const int64_t base = (int64_t)blockIdx.x * 64;
+  auto block_of = [&](int64_t s) -> int { return s < 0 ? -1 : fast_div((int)s, a.by_block); };
+  // The window: this lane's entry, which entries begin a run, which end one.
+  const int64_t mine = base + lane < a.num_slots ? slots[base + lane] : -1;
+  const int64_t before = base + lane > 0 && base + lane <= a.num_slots ? slots[base + lane - 1] : -1;
+  const int my_block = block_of(mine);
+  const uint64_t leads = __ballot(mine >= 0 && block_of(before) != my_block);
+  const uint64_t ends = leads | __ballot(mine < 0);
+  const uint64_t zeros = __ballot(mine >= 0 && (int)mine == my_block * bs);  // offset 0 of a block
+  const int tasks = __popcll(leads) * units;
+  for (int task = blockIdx.y * kAppendWaves + wave; task < tasks; task += gridDim.y * kAppendWaves)
+    append_run<T>(a, slots, lane, base, leads, ends, zeros, my_block, task);
 }
 
 // ---------------------------------------------------------------------------
@@ -252,6 +283,94 @@ __global__ __launch_bounds__(64 * kAppendWaves) void q8_scatter_kernel(const int
   }
 }
 
+// ---------------------------------------------------------------------------
+// Compact of a few rows (one chat's accepted drafts): one launch, no workspace,
+// the pairs in the kernel's arguments.  A wave owns one kv head of one layer's
+// K or V, so it can hold all the call's rows of it in registers (kFewPairs
+// rows of D bytes, 16 per lane and pass) before it writes any.  Lane i has
+// pair i's slots and scales; a segmented scan gives each destination block's
+// new scale.  A chain of three round trips (scales and rows, re-scaled rows,
+// stores).
+// ---------------------------------------------------------------------------
+constexpr int kFewPairs = 32;
+struct Q8FewArgs {
+  const uint64_t* layer_keys;
+  const uint64_t* layer_values;
+  int64_t scale_offset;
+  int32_t num_pairs, num_kv_heads, head_size, block_size;
+  FastDiv by_block, by_heads, by_chunks;
+  int32_t src[kFewPairs], dst[kFewPairs];
+};
+
+__global__ __launch_bounds__(64) void q8_compact_few_kernel(const Q8FewArgs a) {
+  constexpr int kPasses = kFewPairs * 16 / 64;  // head size 256
+  const int lane = threadIdx.x & 63;
+  const int side = fast_div((int)blockIdx.x, a.by_heads);
+  const int h = (int)blockIdx.x - side * a.num_kv_heads;
+  const int n = a.num_pairs;
+  char* base = reinterpret_cast<char*>(side & 1 ? a.layer_values[side >> 1] : a.layer_keys[side >> 1]);
+  float* const scales = reinterpret_cast<float*>(base + a.scale_offset) + h;
+  const int64_t row_bytes = (int64_t)a.num_kv_heads * a.head_size;
+  uint8_t* const pool = reinterpret_cast<uint8_t*>(base) + (int64_t)h * a.head_size;
+  const int pair = lane < n ? lane : n - 1;  // (lanes past the pairs repeat the last)
+  const int from = a.src[pair], to = a.dst[pair];
+  const int to_block = fast_div(to, a.by_block);
+  const float from_scale = scales[(int64_t)fast_div(from, a.by_block) * a.num_kv_heads];
+  const float old = scales[(int64_t)to_block * a.num_kv_heads];
+  const int chunks = a.head_size / 16;
+  uint4 rows[kPasses];
+#pragma unroll
+  for (int p = 0; p < kPasses; ++p) {
+    const int row = fast_div(lane + 64 * p, a.by_chunks);
+    const int c = lane + 64 * p - row * chunks;
+    const int slot = __shfl(from, row & 31);
+    rows[p] = row < n ? load16(pool + slot * row_bytes + 16 * c) : zero_u4();
+  }
+  // Groups of one destination block; the largest scale of a group is at its
+  // last lane.
+  const int before = __shfl_up(to_block, 1);
+  const uint64_t leads = __ballot(lane < n && (lane == 0 || before != to_block));
+  const int group = __popcll(leads & ((2ull << lane) - 1));
+  float most = fmaxf(from_scale, old);
+#pragma unroll
+  for (int d = 1; d < kFewPairs; d <<= 1) {
+    const float other = __shfl_up(most, d);
+    const int other_group = __shfl_up(group, d);
+    if (lane >= d && other_group == group) most = fmaxf(most, other);
+  }
+  const uint64_t after = lane < 63 ? leads >> (lane + 1) : 0;
+  const int last = after ? lane + __builtin_ctzll(after) : n - 1;
+  const float scale = __shfl(most, last);
+  const bool grew = ((leads >> lane) & 1) && scale > old;
+  stores_done();  // (every row is loaded before any is written)
+  for (uint64_t todo = __ballot(grew); todo; todo &= todo - 1) {
+    const int l = __builtin_ctzll(todo);
+    const int64_t block = __builtin_amdgcn_readlane(to_block, l);
+    const float ratio = __shfl(old, l) * q8_inverse(__shfl(scale, l));
+    for (int i = lane; i < a.block_size * chunks; i += 64) {
+      const int r = fast_div(i, a.by_chunks);
+      uint4* const at = reinterpret_cast<uint4*>(pool + (block * a.block_size + r) * row_bytes + 16 * (i - r * chunks));
+      const uint4 w = *at;
+      *at = make_uint4(q8_rescale4(w.x, ratio), q8_rescale4(w.y, ratio), q8_rescale4(w.z, ratio), q8_rescale4(w.w, ratio));
+    }
+  }
+  stores_done();
+  if (grew) scales[(int64_t)to_block * a.num_kv_heads] = scale;
+#pragma unroll
+  for (int p = 0; p < kPasses; ++p) {
+    const int row = fast_div(lane + 64 * p, a.by_chunks);
+    const int c = lane + 64 * p - row * chunks;
+    const int slot = __shfl(to, row & 31);
+    const float ratio = __shfl(from_scale, row & 31) * q8_inverse(__shfl(scale, row & 31));
+    if (row < n) {
+      uint4 w = rows[p];
+      if (ratio < 1.f)
+        w = make_uint4(q8_rescale4(w.x, ratio), q8_rescale4(w.y, ratio), q8_rescale4(w.z, ratio), q8_rescale4(w.w, ratio));
+      *reinterpret_cast<uint4*>(pool + slot * row_bytes + 16 * c) = w;
+    }
+  }
+}
+
 static bool q8_head_size(int d) { return d >= 32 && d <= 256 && d % 16 == 0; }
 static bool aligned_to(const void* p, unsigned n) { return ((uintptr_t)p & (n - 1)) == 0; }
 
@@ -273,7 +392,8 @@ extern "C" int lvamd_kv_append_q8(const void* key, int64_t key_token_stride, int
       !aligned_to(key_scales, 4) || !aligned_to(value_scales, 4) || key_token_stride % 8 != 0 ||
       key_head_stride % 8 != 0 || value_token_stride % 8 != 0 || value_head_stride % 8 != 0)
     return LVAMD_ERR_INVALID_ARGUMENT;
-  Q8AppendArgs a{.by_block = FastDiv(block_size), .by_lanes = FastDiv(head_size / 8)};
+  Q8AppendArgs a{.by_block = FastDiv(block_size), .by_lanes = FastDiv(head_size / 8),
+                 .by_units = FastDiv(2 * num_kv_heads)};
   a.key = static_cast<const char*>(key);
   a.value = static_cast<const char*>(value);
   a.key_tok_bytes = key_token_stride * 2;
@@ -289,7 +409,12 @@ extern "C" int lvamd_kv_append_q8(const void* key, int64_t key_token_stride, int
   a.num_kv_heads = num_kv_heads;
   a.head_size = head_size;
   a.block_size = block_size;
-  const dim3 grid((unsigned)num_slots, (unsigned)((2 * num_kv_heads + kAppendWaves - 1) / kAppendWaves));
+  // Workgroups per window: about 4,096 in all, at most one wave per task of a
+  // window of 64 runs.
+  const int64_t windows = (num_slots + 63) / 64;
+  const int64_t most = (64 * 2 * (int64_t)num_kv_heads + kAppendWaves - 1) / kAppendWaves;
+  const int64_t share = std::max<int64_t>(1, std::min<int64_t>(4096 / windows, most));
+  const dim3 grid((unsigned)windows, (unsigned)share);
   hipStream_t s = static_cast<hipStream_t>(stream);
   if (dtype == LVAMD_BF16)
     hipLaunchKernelGGL((q8_append_kernel<__bf16>), grid, dim3(64 * kAppendWaves), 0, s, slots, a);
@@ -344,5 +469,37 @@ extern "C" int lvamd_kv_compact_q8(const uint64_t* layer_key_ptrs, const uint64_
   if (status != LVAMD_OK) return status;
   hipLaunchKernelGGL(q8_scatter_kernel, dim3((unsigned)num_dst_blocks, (unsigned)groups_y), dim3(64 * kAppendWaves), 0, s,
                      block_starts, a);
+  return launch_status();
+}
+
+extern "C" int64_t lvamd_kv_compact_q8_few_pairs(void) { return kFewPairs; }
+
+extern "C" int lvamd_kv_compact_q8_few(const uint64_t* layer_key_ptrs, const uint64_t* layer_value_ptrs,
+                                       int32_t num_layers, int32_t num_kv_heads, int32_t head_size, int32_t block_size,
+                                       int64_t scale_offset, const int64_t* src_slots, const int64_t* dst_slots,
+                                       int64_t num_pairs, lvamd_stream_t stream) {
+  if (!q8_head_size(head_size)) return LVAMD_ERR_UNSUPPORTED;
+  if (num_pairs < 0 || num_pairs > kFewPairs || num_layers <= 0 || num_kv_heads <= 0 || block_size <= 0 ||
+      scale_offset < 0 || scale_offset % 4 != 0 || (int64_t)block_size * (head_size / 16) > 0x7fffffffLL ||
+      (int64_t)num_layers * 2 * num_kv_heads > 0x7fffffffLL)
+    return LVAMD_ERR_INVALID_ARGUMENT;
+  if (num_pairs == 0) return LVAMD_OK;
+  if (!layer_key_ptrs || !layer_value_ptrs || !src_slots || !dst_slots) return LVAMD_ERR_INVALID_ARGUMENT;
+  Q8FewArgs a{.by_block = FastDiv(block_size), .by_heads = FastDiv(num_kv_heads), .by_chunks = FastDiv(head_size / 16)};
+  for (int64_t i = 0; i < num_pairs; ++i) {
+    if (src_slots[i] < 0 || src_slots[i] > 0x7fffffffLL || dst_slots[i] < 0 || dst_slots[i] > 0x7fffffffLL)
+      return LVAMD_ERR_INVALID_ARGUMENT;
+    a.src[i] = (int32_t)src_slots[i];
+    a.dst[i] = (int32_t)dst_slots[i];
+  }
+  a.layer_keys = layer_key_ptrs;
+  a.layer_values = layer_value_ptrs;
+  a.scale_offset = scale_offset;
+  a.num_pairs = (int32_t)num_pairs;
+  a.num_kv_heads = num_kv_heads;
+  a.head_size = head_size;
+  a.block_size = block_size;
+  hipLaunchKernelGGL(q8_compact_few_kernel, dim3((unsigned)(num_layers * 2 * num_kv_heads)), dim3(64), 0,
+                     static_cast<hipStream_t>(stream), a);
   return launch_status();
 }

@@ -123,36 +123,50 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(D <
   auto issue = [&](int t, const int (&block)[LPT], Tile& x) {
 #pragma unroll
     for (int j = 0; j < LPT; ++j) {
+      const int64_t at = (int64_t)block[j] * Hkv;
+      x.ks[j] = kscales[at];
+      x.vs[j] = vscales[at];
+    }
+#pragma unroll
+    for (int j = 0; j < LPT; ++j) {
       const int c = (tid + P::THREADS * j) % C8;
       const int pos = key_pos(t, j);
       const int64_t s = (int64_t)block[j] * bs + (pos - fast_div(pos, a.by_block) * bs);
       const int64_t off = s * row_bytes + 16 * c;
       x.k[j] = load16(kbase + off);
       x.v[j] = load16(vbase + off);
-      const int64_t at = (int64_t)block[j] * Hkv;
-      x.ks[j] = kscales[at];
-      x.vs[j] = vscales[at];
     }
   };
-  auto stage = [&](int t, const Tile& x, uint4* kd, uint4* vd, int* flag) {
-    const int first_new = computed - (tile0 + t) * KT;  // rows from it on hold this step's tokens
+  auto stage_rows = [&]<bool NEW>(int first_new, const Tile& x, uint4* kd, uint4* vd, int* flag)
+      __attribute__((always_inline)) {
 #pragma unroll
     for (int j = 0; j < LPT; ++j) {
       const int id = tid + P::THREADS * j;
       const int row = id / C8, c = id - row * C8;
-      if (P::THREADS * LPT != KT * C8 && row >= KT) break;
       uint4 v = x.v[j];
-      if (first_new < KT && row >= first_new && q8_has_nan(v)) {
-        *flag = 1;
-        v = make_uint4(q8_without_nan4(v.x), q8_without_nan4(v.y), q8_without_nan4(v.z), q8_without_nan4(v.w));
+      if constexpr (NEW) {
+        if (row >= first_new && q8_has_nan(v)) {
+          *flag = 1;
+          v = make_uint4(q8_without_nan4(v.x), q8_without_nan4(v.y), q8_without_nan4(v.z), q8_without_nan4(v.w));
+        }
       }
-      uint4 lo, hi;
-      q8_values16<T>(x.k[j], x.ks[j], lo, hi);
-      kd[row * RS + 2 * c] = lo;
-      kd[row * RS + 2 * c + 1] = hi;
-      q8_values16<T>(v, x.vs[j], lo, hi);
-      vd[row * RS + 2 * c] = lo;
-      vd[row * RS + 2 * c + 1] = hi;
+      uint4 klo, khi, vlo, vhi;
+      q8_values16<T>(x.k[j], x.ks[j], klo, khi);
+      q8_values16<T>(v, x.vs[j], vlo, vhi);
+      if (P::THREADS * LPT == KT * C8 || row < KT) {
+        kd[row * RS + 2 * c] = klo;
+        kd[row * RS + 2 * c + 1] = khi;
+        vd[row * RS + 2 * c] = vlo;
+        vd[row * RS + 2 * c + 1] = vhi;
+      }
+    }
+  };
+  auto stage = [&](int t, const Tile& x, uint4* kd, uint4* vd, int* flag) __attribute__((always_inline)) {
+    const int first_new = computed - (tile0 + t) * KT;  // rows from it on hold this step's tokens
+    if (first_new >= KT) {
+      stage_rows.template operator()<false>(first_new, x, kd, vd, flag);
+    } else {
+      stage_rows.template operator()<true>(first_new, x, kd, vd, flag);
     }
   };
 
@@ -209,25 +223,36 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(D <
     }
   };
 
-  auto compute = [&](int tr, const uint4* kt, const uint4* vt, const int* flag) {
+  // MASKED: the tile may reach past what every column of the unit sees.  LDS
+  // reads run LEAD operands ahead of the matrix instructions, held there by
+  // scheduling barriers.
+  auto compute = [&]<bool MASKED>(int tr, const uint4* kt, const uint4* vt, const int* flag)
+      __attribute__((always_inline)) {
     const int t = tile0 + tr;
-    if (!wave_active || t * KT >= wave_kmax) return;
+    if (!wave_active || (MASKED && t * KT >= wave_kmax)) return;
     f32x4 st[CT][KS];
     __builtin_amdgcn_s_setprio(1);
+    {
+      constexpr int TOT = KS * NCH, LEAD = TOT < 3 ? TOT : 3;
+      auto rd = [&](int i) -> uint4 {
+        const int s = i / NCH, ch = (i % NCH) * 4 + g;
+        return (CPR % 4 == 0 || ch < CPR) ? kt[(16 * s + l16) * RS + ch] : zero_u4();
+      };
+      uint4 kf[LEAD];
 #pragma unroll
-    for (int s = 0; s < KS; ++s) {
+      for (int i = 0; i < LEAD; ++i) kf[i] = rd(i);
+      const f32x4 z = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int ct = 0; ct < CT; ++ct) st[ct][s] = f32x4{0.f, 0.f, 0.f, 0.f};
+      for (int i = 0; i < TOT; ++i) {
+        const int s = i / NCH, kk = i % NCH;
 #pragma unroll
-      for (int kk = 0; kk < NCH; ++kk) {
-        const int ch = kk * 4 + g;
-        const uint4 k = (CPR % 4 == 0 || ch < CPR) ? kt[(16 * s + l16) * RS + ch] : zero_u4();
-#pragma unroll
-        for (int ct = 0; ct < CT; ++ct) st[ct][s] = Mma<T>::qk(k, qf[ct][kk], st[ct][s]);
+        for (int ct = 0; ct < CT; ++ct) st[ct][s] = Mma<T>::qk(kf[i % LEAD], qf[ct][kk], kk == 0 ? z : st[ct][s]);
+        if (i + LEAD < TOT) kf[i % LEAD] = rd(i + LEAD);
+        __builtin_amdgcn_sched_barrier(0);
       }
     }
     __builtin_amdgcn_s_setprio(0);
-    if (t >= full_tiles) {
+    if (MASKED && t >= full_tiles) {
       const int j0 = t * KT - computed;  // the tile's first key as a token of the step
       if (!tree) {
 #pragma unroll
@@ -291,22 +316,35 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(D <
     __builtin_amdgcn_s_setprio(1);
     const char* vbytes = reinterpret_cast<const char*>(vt);
     const int q4 = l16 & 3;
-#pragma unroll
-    for (int h = 0; h < KS / 2; ++h) {
-#pragma unroll
-      for (int ct = 0; ct < CT; ++ct) l_run[ct] = mm(ones, pb[ct][h], l_run[ct]);
-#pragma unroll
-      for (int n = 0; n < NT; ++n) {
+    {
+      constexpr int TOT = KS / 2 * NT, LEAD = TOT < 2 ? TOT : 2;
+      auto rd = [&](int i) -> V8 {
+        const int h = i / NT, n = i % NT;
         const int lo = ((32 * h + 4 * g + (l16 >> 2)) * RS + 2 * n + (q4 >> 1)) * 16 + (q4 & 1) * 8;
         const s16x4 v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_t*)(vbytes + lo));
         const s16x4 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_t*)(vbytes + lo + 16 * RS * 16));
         const s16x4 both[2] = {v0, v1};
+        return bitcast<V8>(both);
+      };
+      V8 vf[LEAD];
 #pragma unroll
-        for (int ct = 0; ct < CT; ++ct) acc[ct][n] = mm(bitcast<V8>(both), pb[ct][h], acc[ct][n]);
+      for (int i = 0; i < LEAD; ++i) vf[i] = rd(i);
+#pragma unroll
+      for (int h = 0; h < KS / 2; ++h)
+#pragma unroll
+        for (int ct = 0; ct < CT; ++ct) l_run[ct] = mm(ones, pb[ct][h], l_run[ct]);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int i = 0; i < TOT; ++i) {
+        const int h = i / NT, n = i % NT;
+#pragma unroll
+        for (int ct = 0; ct < CT; ++ct) acc[ct][n] = mm(vf[i % LEAD], pb[ct][h], acc[ct][n]);
+        if (i + LEAD < TOT) vf[i % LEAD] = rd(i + LEAD);
+        __builtin_amdgcn_sched_barrier(0);
       }
     }
     __builtin_amdgcn_s_setprio(0);
-    if ((t + 1) * KT > computed && *flag) {
+    if (MASKED && *flag) {
       for (int pos = max(t * KT, computed); pos < min((t + 1) * KT, kmax); ++pos) {
         const int lb = fast_div(pos, a.by_block);
         const int64_t s = (int64_t)table[lb] * bs + (pos - lb * bs);
@@ -337,19 +375,24 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(D <
   __syncthreads();
   stage(0, x, klds[0], vlds[0], &poison[0]);
   __syncthreads();
-  for (int t = 0; t < ntiles; ++t) {
-    const int b = t & 1;
-    const bool more = t + 1 < ntiles;
+  auto step = [&]<bool MASKED>(int t, int b) __attribute__((always_inline)) {
+    const bool more = !MASKED || t + 1 < ntiles;
     if (more) {
       issue(t + 1, block, x);
-      if (t + 2 < ntiles) lookup(t + 2, block);
+      if (!MASKED || t + 2 < ntiles) lookup(t + 2, block);
     }
-    compute(t, klds[b], vlds[b], &poison[b]);
+    compute.template operator()<MASKED>(t, klds[b], vlds[b], &poison[b]);
     if (more) {
       stage(t + 1, x, klds[b ^ 1], vlds[b ^ 1], &poison[b ^ 1]);
       __syncthreads();
     }
-  }
+  };
+  // Tiles that every column sees, before the step's own tokens, with one to
+  // follow; then the rest.  (lookup past the last tile repeats its last key.)
+  const int nfull = min(min(full_tiles, computed / KT) - tile0, ntiles - 1);
+  int t = 0;
+  for (; t < nfull; ++t) step.template operator()<false>(t, t & 1);
+  for (; t < ntiles; ++t) step.template operator()<true>(t, t & 1);
 
   // ---- normalised output rows, or this piece's partials
   if (!wave_active) return;

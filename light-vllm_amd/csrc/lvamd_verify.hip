@@ -20,12 +20,15 @@
 // split (a sum's error, 1e-13, against the 1e-6 of a 150,000-token border).
 //
 // HBM-bound in large batches: one row of p per request (and one of q), 16-byte
-// loads; two dependent launches otherwise.  The accept tests need only p and q
-// at the drafts themselves, so every workgroup of the first launch finds its
-// request's last node itself (a gather of n values and a walk in LDS, in place
-// of a launch before it), then sums its chunk of the residual; the second
-// finds the chunk that holds the draw and scans it.
+// loads, several per lane in flight; a chain of round trips in small ones, over
+// two dependent launches.  The accept tests need only p and q at the drafts
+// themselves, so every workgroup of the first launch finds its request's last
+// node itself (a gather of n values and a walk in LDS, in place of a launch
+// before it); then its waves sum chunks of the residual, 4 KiB of a row each.
+// The second launch is one wave per request, without a barrier: it scans the
+// chunks' sums, then the one chunk that holds the draw.
 
+#include <algorithm>
 #include <cmath>
 
 #include "lvamd_common.h"
@@ -35,8 +38,15 @@ namespace lvamd {
 namespace {
 
 constexpr int kMaxDrafts = LVAMD_VERIFY_MAX_DRAFTS;
-constexpr int kThreads = 256;
-constexpr int kMaxChunks = kThreads;  // one partial sum per thread of the second launch
+constexpr int kWaves = 4;
+constexpr int kThreads = 64 * kWaves;
+constexpr int kLoads = 4;  // 16-byte loads per lane and chunk
+
+// What the first launch leaves the second: the last node (0: the root), its
+// children, and the draft whose q is subtracted there (-1: none).
+struct Stop {
+  int32_t node, num_children, draft, unused;
+};
 
 struct VerifyArgs {
   const void* target;
@@ -49,12 +59,13 @@ struct VerifyArgs {
   const int32_t* siblings;  // [drafts]: the sibling before it, or -1
   const void* node_uniforms;
   const void* sample_uniforms;
-  double* sums;             // [requests][chunks][2]: the residual's sum, p's sum
-  int32_t* stops;           // [requests]: the last node, 0 the root
+  double2* sums;            // [requests][chunks]: the residual's sum, p's sum
+  Stop* stops;              // [requests]
+  int64_t* children;        // [drafts]: the last node's children's tokens, from the request's first draft on
   int32_t* counts;
   int32_t* paths;
   int64_t* out_tokens;
-  int32_t vocab, chunks, chunk, path_width;
+  int32_t vocab, chunks, path_width;
   int32_t uniforms_f64;
 };
 
@@ -67,65 +78,88 @@ __device__ __forceinline__ double uniform_at(const void* u, int64_t i, int f64) 
 
 template <typename T>
 struct Wide {
-  static constexpr int N = 16 / (int)sizeof(T);
+  static constexpr int N = 16 / (int)sizeof(T);   // elements per load
+  static constexpr int CHUNK = 64 * kLoads * N;   // elements per chunk
 };
 
-// N = 16 bytes of a row from element i on (the row's alignment is that of its
-// elements: rows of odd length start anywhere); elements from `end` on are 0.
+// 16 bytes of a row (its alignment is that of its elements: rows of odd length
+// start anywhere): elements [at, at + N), at = i but for the row's end, where
+// the load begins earlier and its elements before i do not count.
 template <typename T>
-__device__ __forceinline__ void load_wide(const T* row, int i, int end, float (&x)[Wide<T>::N]) {
+struct Pack {
+  typedef T Vec __attribute__((ext_vector_type(Wide<T>::N)));
+  Vec e;
+};
+template <typename T>
+__device__ __forceinline__ int pack_at(int i, int end) {
+  return min(i, max(end - Wide<T>::N, 0));
+}
+template <typename T>
+__device__ __forceinline__ Pack<T> load_pack(const T* row, int i, int end) {
   constexpr int N = Wide<T>::N;
-  if (i + N <= end) {
-    struct __attribute__((packed, aligned(sizeof(T)))) V {
-      T e[N];
-    };
-    const V v = *reinterpret_cast<const V*>(row + i);
+  Pack<T> v;
+  if (end >= N) {
+    typedef T Loose __attribute__((ext_vector_type(N), aligned(sizeof(T))));
+    v.e = *reinterpret_cast<const Loose*>(row + pack_at<T>(i, end));
+  } else {  // a row shorter than the load
 #pragma unroll
-    for (int k = 0; k < N; ++k) x[k] = mass(to_f32(v.e[k]));
-  } else {
-#pragma unroll
-    for (int k = 0; k < N; ++k) x[k] = i + k < end ? mass(to_f32(row[i + k])) : 0.f;
+    for (int k = 0; k < N; ++k) v.e[k] = row[min(k, end - 1)];
   }
+  return v;
 }
-
-// The node's children: their tokens (any order), and the draft whose q is
-// subtracted (the first found; a chain has one).
-struct Children {
-  int count, draft;
-};
-__device__ __forceinline__ void list_children(const VerifyArgs& a, int first, int n, int node, int64_t* tokens,
-                                              Children* found) {
-  if (threadIdx.x == 0) *found = {0, -1};
-  __syncthreads();
-  for (int c = threadIdx.x; c < n; c += kThreads)
-    if (a.parents[first + c] + 1 == node) {
-      tokens[atomicAdd(&found->count, 1)] = a.tokens[first + c];
-      found->draft = first + c;
-    }
-  __syncthreads();
-}
-
-// Residual and p of N elements from i on.  p is exact, and so is p - q in
-// fp64 (the residual of two 24-bit values).
 template <typename T>
-__device__ __forceinline__ void residual(const T* prow, const T* qrow, const int64_t* kids, int nkids, int i, int end,
-                                         float (&p)[Wide<T>::N], double (&r)[Wide<T>::N]) {
-  constexpr int N = Wide<T>::N;
-  load_wide<T>(prow, i, end, p);
-  if (qrow != nullptr) {
-    float q[N];
-    load_wide<T>(qrow, i, end, q);
+__device__ __forceinline__ void masses(const Pack<T>& v, int i, int end, float (&x)[Wide<T>::N]) {
+  const int at = pack_at<T>(i, end);
 #pragma unroll
-    for (int k = 0; k < N; ++k) r[k] = p[k] > q[k] ? (double)p[k] - (double)q[k] : 0.0;
+  for (int k = 0; k < Wide<T>::N; ++k) x[k] = at + k >= i && at + k < end ? mass(to_f32((T)v.e[k])) : 0.f;
+}
+
+// A lane's packs of a chunk, pack j from element first + j * step on.
+template <typename T>
+struct Packs {
+  Pack<T> v[kLoads];
+  int first, step;
+  __device__ __forceinline__ int from(int j) const { return first + j * step; }
+};
+template <typename T>
+__device__ __forceinline__ void load_packs(Packs<T>& x, const T* row, int first, int step, int end) {
+  x.first = first;
+  x.step = step;
+#pragma unroll
+  for (int j = 0; j < kLoads; ++j) x.v[j] = load_pack<T>(row, x.from(j), end);
+}
+// The children's tokens that lie in the chunk from `begin` on taken out; whether
+// there are any.
+template <typename T>
+__device__ __forceinline__ bool take_out(Packs<T>& x, const int64_t* kids, int nkids, int begin, int end) {
+  bool any = false;
+  for (int c = 0; c < nkids; ++c) {
+    const int64_t kid = kids[c];
+    if (kid < begin || kid >= begin + Wide<T>::CHUNK) continue;  // (uniform)
+    any = true;
+#pragma unroll
+    for (int j = 0; j < kLoads; ++j)
+#pragma unroll
+      for (int k = 0; k < Wide<T>::N; ++k)
+        if (pack_at<T>(x.from(j), end) + k == kid) x.v[j].e[k] = (T)0.f;
+  }
+  return any;
+}
+// Residual of pack j's elements: p, or p - q (exact in fp64: two 24-bit values)
+// where that is positive.
+template <typename T, bool DRAWN>
+__device__ __forceinline__ void residual(const Packs<T>& p, const Packs<T>& q, int j, int end, double (&r)[Wide<T>::N]) {
+  constexpr int N = Wide<T>::N;
+  float x[N];
+  masses<T>(p.v[j], p.from(j), end, x);
+  if constexpr (DRAWN) {
+    float y[N];
+    masses<T>(q.v[j], q.from(j), end, y);
+#pragma unroll
+    for (int k = 0; k < N; ++k) r[k] = x[k] > y[k] ? (double)x[k] - (double)y[k] : 0.0;
   } else {
 #pragma unroll
-    for (int k = 0; k < N; ++k) r[k] = (double)p[k];
-    for (int c = 0; c < nkids; ++c) {
-      const int64_t at = kids[c] - i;
-#pragma unroll
-      for (int k = 0; k < N; ++k)
-        if (at == k) r[k] = 0.0;
-    }
+    for (int k = 0; k < N; ++k) r[k] = (double)x[k];
   }
 }
 
@@ -137,235 +171,260 @@ __device__ __forceinline__ double wave_sum(double v) {
 
 }  // namespace
 
-// Grid: (chunks, requests).
-template <typename T>
-__global__ __launch_bounds__(kThreads) void verify_sums_kernel(const VerifyArgs a) {
+// Grid: (workgroups per request, requests); a request's waves take its chunks
+// in turn.
+template <typename T, bool DRAWN>
+__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(4))) void verify_sums_kernel(
+    const VerifyArgs a) {
   __shared__ float mp[kMaxDrafts], mq[kMaxDrafts];
   __shared__ int next[kMaxDrafts + 1];
   __shared__ int64_t kids[kMaxDrafts];
-  __shared__ Children found;
-  __shared__ int stop;
-  __shared__ double part[kThreads / 64][2];
+  __shared__ int stop, num_kids, kid_draft;
   const int req = blockIdx.y;
   const int first = a.starts[req];
   const int n = min(a.starts[req + 1] - first, kMaxDrafts);
   const int64_t row0 = (int64_t)first + req;  // the root's row
+  const bool leader = blockIdx.x == 0;         // writes what is found
   const T* target = static_cast<const T*>(a.target);
   const T* drafts = static_cast<const T*>(a.draft_probs);
-  for (int c = threadIdx.x; c < n; c += kThreads) {
-    const int64_t tok = a.tokens[first + c];
-    const bool in = tok >= 0 && tok < a.vocab;
-    mp[c] = in ? mass(to_f32(target[(row0 + a.parents[first + c] + 1) * a.target_stride + tok])) : 0.f;
-    mq[c] = in && drafts ? mass(to_f32(drafts[(int64_t)(first + c) * a.draft_stride + tok])) : 0.f;
-  }
-  for (int c = threadIdx.x; c <= n; c += kThreads) next[c] = -1;
-  __syncthreads();
-  for (int c = threadIdx.x; c < n; c += kThreads) {
-    const int parent = a.parents[first + c] + 1;
-    const double u = uniform_at(a.node_uniforms, row0 + parent, a.uniforms_f64);
-    bool taken;
-    if (drafts) {
-      taken = u * (double)mq[c] < (double)mp[c];
-    } else {
-      double before = 0.0;
-      for (int s = a.siblings[first + c]; s >= 0; s = a.siblings[first + s]) before += (double)mp[s];
-      taken = u >= before && u < before + (double)mp[c];
-    }
-    if (taken) next[parent] = c + 1;
-  }
-  __syncthreads();
   if (threadIdx.x == 0) {
-    const bool write = blockIdx.x == 0;
-    int node = 0, count = 0;
-    for (int to = next[0]; to >= 0 && count < n; to = next[to]) {
-      node = to;
-      if (write && count < a.path_width) a.paths[(int64_t)req * a.path_width + count] = node - 1;
-      ++count;
+    stop = num_kids = 0;
+    kid_draft = -1;
+  }
+  if (n > 0) {
+    for (int c = threadIdx.x; c < n; c += kThreads) {
+      const int64_t tok = a.tokens[first + c];
+      const bool in = tok >= 0 && tok < a.vocab;
+      mp[c] = in ? mass(to_f32(target[(row0 + a.parents[first + c] + 1) * a.target_stride + tok])) : 0.f;
+      if constexpr (DRAWN) mq[c] = in ? mass(to_f32(drafts[(int64_t)(first + c) * a.draft_stride + tok])) : 0.f;
     }
+    for (int c = threadIdx.x; c <= n; c += kThreads) next[c] = -1;
+    __syncthreads();
+    for (int c = threadIdx.x; c < n; c += kThreads) {
+      const int parent = a.parents[first + c] + 1;
+      const double u = uniform_at(a.node_uniforms, row0 + parent, a.uniforms_f64);
+      bool taken;
+      if constexpr (DRAWN) {
+        taken = u * (double)mq[c] < (double)mp[c];
+      } else {
+        double before = 0.0;
+        for (int s = a.siblings[first + c]; s >= 0; s = a.siblings[first + s]) before += (double)mp[s];
+        taken = u >= before && u < before + (double)mp[c];
+      }
+      if (taken) next[parent] = c + 1;
+    }
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) {
+    int node = 0, count = 0;
+    if (n > 0)
+      for (int to = next[0]; to >= 0 && count < n; to = next[to]) {
+        node = to;
+        if (leader && count < a.path_width) a.paths[(int64_t)req * a.path_width + count] = node - 1;
+        ++count;
+      }
     stop = node;
-    if (write) {
+    if (leader) {
       a.counts[req] = count;
-      a.stops[req] = node;
       for (int i = count; i < a.path_width; ++i) a.paths[(int64_t)req * a.path_width + i] = -1;
     }
   }
   __syncthreads();
   const int node = stop;
-  list_children(a, first, n, node, kids, &found);
+  if (n > 0) {
+    for (int c = threadIdx.x; c < n; c += kThreads)
+      if (a.parents[first + c] + 1 == node) {
+        kids[atomicAdd(&num_kids, 1)] = a.tokens[first + c];
+        kid_draft = first + c;  // (a chain has one)
+      }
+    __syncthreads();
+  }
+  const int nkids = num_kids;
+  const int draft = DRAWN ? kid_draft : -1;
+  if (leader) {
+    if (threadIdx.x == 0) a.stops[req] = {node, nkids, draft, 0};
+    for (int c = threadIdx.x; c < nkids; c += kThreads) a.children[first + c] = kids[c];
+  }
   const T* prow = target + (row0 + node) * a.target_stride;
-  const T* qrow = drafts && found.draft >= 0 ? drafts + (int64_t)found.draft * a.draft_stride : nullptr;
-  const int nkids = drafts ? 0 : found.count;
-  const int begin = blockIdx.x * a.chunk;
-  const int end = min(begin + a.chunk, a.vocab);
+  const T* qrow = DRAWN && draft >= 0 ? drafts + (int64_t)draft * a.draft_stride : nullptr;
   constexpr int N = Wide<T>::N;
-  double rest = 0.0, full = 0.0;
-  for (int i = begin + threadIdx.x * N; i < end; i += kThreads * N) {
-    float p[N];
-    double r[N];
-    residual<T>(prow, qrow, kids, nkids, i, end, p, r);
-#pragma unroll
-    for (int k = 0; k < N; ++k) {
-      rest += r[k];
-      full += (double)p[k];
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+  for (int chunk = blockIdx.x * kWaves + wave; chunk < a.chunks; chunk += gridDim.x * kWaves) {
+    const int begin = chunk * Wide<T>::CHUNK;
+    Packs<T> p, q = {};
+    load_packs<T>(p, prow, begin + lane * N, 64 * N, a.vocab);
+    if constexpr (DRAWN) {
+      if (qrow) load_packs<T>(q, qrow, begin + lane * N, 64 * N, a.vocab);  // (else zeros: nothing to subtract)
     }
-  }
-  rest = wave_sum(rest);
-  full = wave_sum(full);
-  const int wave = threadIdx.x >> 6;
-  if ((threadIdx.x & 63) == 0) {
-    part[wave][0] = rest;
-    part[wave][1] = full;
-  }
-  __syncthreads();
-  if (threadIdx.x < 2) {
-    double s = 0.0;
+    double full = 0.0, rest = 0.0;
+    auto sum = [&]<bool LESS>() -> double {
+      double s = 0.0;
 #pragma unroll
-    for (int i = 0; i < kThreads / 64; ++i) s += part[i][threadIdx.x];
-    a.sums[((int64_t)req * a.chunks + blockIdx.x) * 2 + threadIdx.x] = s;
+      for (int j = 0; j < kLoads; ++j) {
+        double r[N];
+        residual<T, LESS>(p, q, j, a.vocab, r);
+#pragma unroll
+        for (int k = 0; k < N; ++k) s += r[k];
+      }
+      return s;
+    };
+    full = rest = sum.template operator()<false>();
+    if constexpr (DRAWN) {
+      if (qrow) rest = sum.template operator()<true>();
+    } else {
+      if (take_out<T>(p, kids, nkids, begin, a.vocab)) rest = sum.template operator()<false>();
+    }
+    rest = wave_sum(rest);
+    full = wave_sum(full);
+    if (lane == 0) a.sums[(int64_t)req * a.chunks + chunk] = make_double2(rest, full);
   }
 }
 
 namespace {
 
-// Inclusive sum over the workgroup's threads, in thread order.
-__device__ __forceinline__ double scan(double v, double* waves) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+// Inclusive sum over the wave's lanes.
+__device__ __forceinline__ double wave_scan(double v, int lane) {
 #pragma unroll
   for (int d = 1; d < 64; d <<= 1) {
     const double o = __shfl_up(v, d);
     if (lane >= d) v += o;
   }
-  __syncthreads();
-  if (lane == 63) waves[wave] = v;
-  __syncthreads();
-  double before = 0.0;
-  for (int i = 0; i < wave; ++i) before += waves[i];
-  return before + v;
+  return v;
 }
 
 }  // namespace
 
-// Grid: requests.
-template <typename T>
-__global__ __launch_bounds__(kThreads) void verify_draw_kernel(const VerifyArgs a) {
-  __shared__ int64_t kids[kMaxDrafts];
-  __shared__ Children found;
-  __shared__ double waves[kThreads / 64];
-  __shared__ double ends[kThreads];  // inclusive sums per chunk
-  __shared__ int hit, tail;
+// Grid: requests, one wave each.
+template <typename T, bool DRAWN>
+__global__ __launch_bounds__(64) void verify_draw_kernel(const VerifyArgs a) {
+  constexpr int N = Wide<T>::N;
+  constexpr int kHeld = 4;  // rounds of 64 chunks whose sums stay in registers
   const int req = blockIdx.x;
-  const int tid = threadIdx.x;
+  const int lane = threadIdx.x & 63;
+  const double2* sums = a.sums + (int64_t)req * a.chunks;
+  const Stop stop = a.stops[req];
   const int first = a.starts[req];
-  const int n = min(a.starts[req + 1] - first, kMaxDrafts);
-  const int node = a.stops[req];
   const double u = uniform_at(a.sample_uniforms, req, a.uniforms_f64);
-  const double* sums = a.sums + (int64_t)req * a.chunks * 2;
-  const double rest = tid < a.chunks ? sums[2 * tid] : 0.0;
-  const double full = tid < a.chunks ? sums[2 * tid + 1] : 0.0;
-  if (tid == 0) {
-    hit = kThreads;
-    tail = -1;
+  double2 held[kHeld];
+#pragma unroll
+  for (int i = 0; i < kHeld; ++i) held[i] = 64 * i + lane < a.chunks ? sums[64 * i + lane] : make_double2(0.0, 0.0);
+  double rest = 0.0, full = 0.0;
+#pragma unroll
+  for (int i = 0; i < kHeld; ++i) {
+    rest += held[i].x;
+    full += held[i].y;
   }
-  list_children(a, first, n, node, kids, &found);
-  const bool residual_left = __syncthreads_or(rest > 0.0);
-  const double mine = residual_left ? rest : full;
-  const double upto = scan(mine, waves);
-  ends[tid] = upto;
-  __syncthreads();
-  const double goal = u * ends[kThreads - 1];
-  if (upto > goal) atomicMin(&hit, tid);
-  if (mine > 0.0) atomicMax(&tail, tid);
-  __syncthreads();
-  const int at = hit < kThreads ? hit : tail;  // (u >= 1: the last chunk that holds anything)
+  for (int c = 64 * kHeld + lane; c < a.chunks; c += 64) {
+    rest += sums[c].x;
+    full += sums[c].y;
+  }
+  rest = wave_sum(rest);
+  full = wave_sum(full);
+  const bool residual_left = rest > 0.0;
+  const double goal = u * (residual_left ? rest : full);
+  // The first chunk whose sums pass the goal; the last that holds anything
+  // where none does (u >= 1, or by rounding).
+  int at = -1, tail = -1;
+  double done = 0.0, base = 0.0, tail_base = 0.0;
+  auto round = [&](int r, double2 s) {
+    const double mine = residual_left ? s.x : s.y;
+    const double upto = done + wave_scan(mine, lane);
+    const uint64_t pass = __ballot(upto > goal), some = __ballot(mine > 0.0);
+    if (pass && at < 0) {
+      const int l = __builtin_ctzll(pass);
+      at = 64 * r + l;
+      base = __shfl(upto - mine, l);
+    }
+    if (some) {
+      const int l = 63 - __builtin_clzll(some);
+      tail = 64 * r + l;
+      tail_base = __shfl(upto - mine, l);
+    }
+    done = __shfl(upto, 63);
+  };
+#pragma unroll
+  for (int i = 0; i < kHeld; ++i)
+    if (at < 0 && 64 * i < a.chunks) round(i, held[i]);
+  for (int i = kHeld; at < 0 && 64 * i < a.chunks; ++i)
+    round(i, 64 * i + lane < a.chunks ? sums[64 * i + lane] : make_double2(0.0, 0.0));
   if (at < 0) {
-    if (tid == 0) a.out_tokens[req] = -1;
+    at = tail;
+    base = tail_base;
+  }
+  if (at < 0) {
+    if (lane == 0) a.out_tokens[req] = -1;
     return;
   }
-  const double base = at > 0 ? ends[at - 1] : 0.0;
-  __syncthreads();
-  if (tid == 0) {
-    hit = 0x7fffffff;
-    tail = -1;
-  }
-  __syncthreads();
-  // The chunk, N elements per thread and round, until the draw is reached.
+  // The chunk, kLoads * N elements in a row per lane.
   const T* drafts = static_cast<const T*>(a.draft_probs);
-  const T* prow = static_cast<const T*>(a.target) + ((int64_t)first + req + node) * a.target_stride;
-  const T* qrow =
-      residual_left && drafts && found.draft >= 0 ? drafts + (int64_t)found.draft * a.draft_stride : nullptr;
-  const int nkids = residual_left && !drafts ? found.count : 0;
-  constexpr int N = Wide<T>::N;
-  const int begin = at * a.chunk;
-  const int end = min(begin + a.chunk, a.vocab);
-  double done = base;
-  for (int i0 = begin; i0 < end; i0 += kThreads * N) {
-    const int i = i0 + tid * N;
-    float p[N];
-    double r[N];
-    residual<T>(prow, qrow, kids, nkids, min(i, end), end, p, r);
-    double s = 0.0;
+  const T* prow = static_cast<const T*>(a.target) + ((int64_t)first + req + stop.node) * a.target_stride;
+  const T* qrow = residual_left && stop.draft >= 0 ? drafts + (int64_t)stop.draft * a.draft_stride : nullptr;
+  const int begin = at * Wide<T>::CHUNK + lane * kLoads * N;
+  Packs<T> p, q = {};
+  load_packs<T>(p, prow, begin, N, a.vocab);
+  if constexpr (DRAWN) {
+    if (qrow) load_packs<T>(q, qrow, begin, N, a.vocab);
+  } else {
+    if (residual_left) take_out<T>(p, a.children + first, stop.num_children, at * Wide<T>::CHUNK, a.vocab);
+  }
+  double r[kLoads][N], s = 0.0;
 #pragma unroll
-    for (int k = 0; k < N; ++k) s += r[k];
-    const double last = done + scan(s, waves);
-    double c = last - s;
-    // Sums over the elements again, from the thread's own start: the first
-    // that passes the goal (the thread's end passes it too, to rounding).
-    int mine_hit = 0x7fffffff, mine_tail = -1;
+  for (int j = 0; j < kLoads; ++j) {
+    residual<T, DRAWN>(p, q, j, a.vocab, r[j]);
+#pragma unroll
+    for (int k = 0; k < N; ++k) s += r[j][k];
+  }
+  double c = base + (wave_scan(s, lane) - s);
+  int hit = -1, last = -1;
+#pragma unroll
+  for (int j = 0; j < kLoads; ++j)
 #pragma unroll
     for (int k = 0; k < N; ++k) {
-      c += r[k];
-      if (r[k] > 0.0) {
-        if (c > goal && mine_hit == 0x7fffffff) mine_hit = i + k;
-        mine_tail = i + k;
+      c += r[j][k];
+      if (r[j][k] > 0.0) {
+        last = pack_at<T>(begin + j * N, a.vocab) + k;
+        if (c > goal && hit < 0) hit = last;
       }
     }
-    if (mine_hit != 0x7fffffff) atomicMin(&hit, mine_hit);
-    if (mine_tail >= 0) atomicMax(&tail, mine_tail);
-    __syncthreads();
-    if (hit != 0x7fffffff) break;
-    if (tid == kThreads - 1) ends[0] = last;
-    __syncthreads();
-    done = ends[0];
-  }
-  if (tid == 0) a.out_tokens[req] = hit != 0x7fffffff ? hit : tail;
+  const uint64_t hits = __ballot(hit >= 0), lasts = __ballot(last >= 0);
+  const int token = hits ? __shfl(hit, __builtin_ctzll(hits)) : lasts ? __shfl(last, 63 - __builtin_clzll(lasts)) : -1;
+  if (lane == 0) a.out_tokens[req] = token;
 }
 
 }  // namespace lvamd
 
 using namespace lvamd;
 
-// Chunks of a row: about 2,048 workgroups over the batch, each with at least
-// one 16-byte load per thread, at most kMaxChunks.
-static int verify_chunks(int64_t requests, int32_t vocab, int32_t dtype) {
-  const int64_t least = kThreads * (dtype == LVAMD_F32 ? 4 : 8);
-  const int64_t most = (vocab + least - 1) / least;
-  const int64_t want = requests > 0 ? (2048 + requests - 1) / requests : 1;
-  const int64_t n = most < want ? most : want;
-  return (int)(n < 1 ? 1 : n > kMaxChunks ? kMaxChunks : n);
+static int verify_chunks(int32_t vocab, int32_t dtype) {
+  const int chunk = 64 * kLoads * (dtype == LVAMD_F32 ? 4 : 8);
+  return (vocab + chunk - 1) / chunk;
 }
 
-extern "C" int64_t lvamd_verify_drafts_workspace_size(int64_t num_requests, int32_t vocab, int32_t dtype) {
-  if (num_requests <= 0 || vocab <= 0) return 0;
-  return num_requests * ((int64_t)verify_chunks(num_requests, vocab, dtype) * 16 + 4);
+extern "C" int64_t lvamd_verify_drafts_workspace_size(int64_t num_requests, int64_t num_drafts, int32_t vocab,
+                                                      int32_t dtype) {
+  if (num_requests <= 0 || num_drafts < 0 || vocab <= 0) return 0;
+  return num_requests * ((int64_t)verify_chunks(vocab, dtype) * (int64_t)sizeof(double2) + (int64_t)sizeof(Stop)) +
+         num_drafts * 8;
 }
 
 extern "C" int lvamd_verify_drafts(const void* target, int64_t target_row_stride, const void* draft_probs,
                                    int64_t draft_row_stride, int32_t vocab, int32_t dtype, const int32_t* draft_starts,
                                    const int64_t* draft_tokens, const int32_t* parents, const int32_t* siblings,
-                                   int64_t num_requests, const void* node_uniforms, const void* sample_uniforms,
+                                   int64_t num_requests, int64_t num_drafts, const void* node_uniforms, const void* sample_uniforms,
                                    int32_t uniforms_f64, int32_t* counts, int32_t* paths, int32_t path_width,
                                    int64_t* out_tokens, void* workspace, int64_t workspace_bytes,
                                    lvamd_stream_t stream) {
   if (dtype_size(dtype) == 0) return LVAMD_ERR_UNSUPPORTED;
-  if (num_requests < 0 || num_requests > 65535 || vocab <= 0 || vocab > (1 << 30) || path_width < 1 ||
+  if (num_requests < 0 || num_requests > 65535 || num_drafts < 0 || vocab <= 0 || vocab > (1 << 30) || path_width < 1 ||
       target_row_stride < 0 || draft_row_stride < 0)
     return LVAMD_ERR_INVALID_ARGUMENT;
   if (num_requests == 0) return LVAMD_OK;
   if (!target || !draft_starts || !draft_tokens || !parents || !siblings || !node_uniforms || !sample_uniforms ||
       !counts || !paths || !out_tokens)
     return LVAMD_ERR_INVALID_ARGUMENT;
-  if (!workspace || ((uintptr_t)workspace & 7u) != 0 ||
-      workspace_bytes < lvamd_verify_drafts_workspace_size(num_requests, vocab, dtype))
+  if (!workspace || ((uintptr_t)workspace & 15u) != 0 ||
+      workspace_bytes < lvamd_verify_drafts_workspace_size(num_requests, num_drafts, vocab, dtype))
     return LVAMD_ERR_WORKSPACE;
   VerifyArgs a{};
   a.target = target;
@@ -378,11 +437,10 @@ extern "C" int lvamd_verify_drafts(const void* target, int64_t target_row_stride
   a.siblings = siblings;
   a.node_uniforms = node_uniforms;
   a.sample_uniforms = sample_uniforms;
-  a.chunks = verify_chunks(num_requests, vocab, dtype);
-  // (Whole 16-byte groups.)
-  a.chunk = (((vocab + a.chunks - 1) / a.chunks) + 7) / 8 * 8;
-  a.sums = static_cast<double*>(workspace);
-  a.stops = reinterpret_cast<int32_t*>(a.sums + num_requests * a.chunks * 2);
+  a.chunks = verify_chunks(vocab, dtype);
+  a.sums = static_cast<double2*>(workspace);
+  a.stops = reinterpret_cast<Stop*>(a.sums + num_requests * a.chunks);
+  a.children = reinterpret_cast<int64_t*>(a.stops + num_requests);
   a.counts = counts;
   a.paths = paths;
   a.path_width = path_width;
@@ -390,18 +448,25 @@ extern "C" int lvamd_verify_drafts(const void* target, int64_t target_row_stride
   a.vocab = vocab;
   a.uniforms_f64 = uniforms_f64 != 0;
   hipStream_t s = static_cast<hipStream_t>(stream);
-  const dim3 grid((unsigned)a.chunks, (unsigned)num_requests), draw((unsigned)num_requests), threads(kThreads);
+  // A chunk per wave while about kWorkgroups of them suffice; several in larger
+  // batches, which spreads the walk over more of the row.
+  constexpr int64_t kWorkgroups = 2048;
+  const int64_t most = (a.chunks + kWaves - 1) / kWaves;
+  const int64_t share = std::max<int64_t>(1, std::min<int64_t>(most, kWorkgroups / num_requests));
+  const dim3 grid((unsigned)share, (unsigned)num_requests), draw((unsigned)num_requests), threads(kThreads);
+  auto launch = [&]<typename T, bool DRAWN>() -> int {
+    hipLaunchKernelGGL((verify_sums_kernel<T, DRAWN>), grid, threads, 0, s, a);
+    const int status = launch_status();
+    if (status != LVAMD_OK) return status;
+    hipLaunchKernelGGL((verify_draw_kernel<T, DRAWN>), draw, dim3(64), 0, s, a);
+    return launch_status();
+  };
+  auto launch_t = [&]<typename T>() -> int {
+    return draft_probs ? launch.template operator()<T, true>() : launch.template operator()<T, false>();
+  };
   switch (dtype) {
-    case LVAMD_BF16: hipLaunchKernelGGL((verify_sums_kernel<__bf16>), grid, threads, 0, s, a); break;
-    case LVAMD_F16: hipLaunchKernelGGL((verify_sums_kernel<_Float16>), grid, threads, 0, s, a); break;
-    default: hipLaunchKernelGGL((verify_sums_kernel<float>), grid, threads, 0, s, a); break;
+    case LVAMD_BF16: return launch_t.template operator()<__bf16>();
+    case LVAMD_F16: return launch_t.template operator()<_Float16>();
+    default: return launch_t.template operator()<float>();
   }
-  const int status = launch_status();
-  if (status != LVAMD_OK) return status;
-  switch (dtype) {
-    case LVAMD_BF16: hipLaunchKernelGGL((verify_draw_kernel<__bf16>), draw, threads, 0, s, a); break;
-    case LVAMD_F16: hipLaunchKernelGGL((verify_draw_kernel<_Float16>), draw, threads, 0, s, a); break;
-    default: hipLaunchKernelGGL((verify_draw_kernel<float>), draw, threads, 0, s, a); break;
-  }
-  return launch_status();
 }

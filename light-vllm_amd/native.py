@@ -130,12 +130,14 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
         ctypes.c_int,
         [_p, _p, _i32, _i32, _i32, _i32, _i64, _p, _p, _i64, _p, _i64, _p, _i64, _p],
     ),
+    "lvamd_kv_compact_q8_few": (ctypes.c_int, [_p, _p, _i32, _i32, _i32, _i32, _i64, _p, _p, _i64, _p]),
+    "lvamd_kv_compact_q8_few_pairs": (_i64, []),
     "lvamd_kv_compact_q8_workspace_size": (_i64, [_i64, _i32, _i32, _i32]),
     "lvamd_verify_drafts": (
         ctypes.c_int,
-        [_p, _i64, _p, _i64, _i32, _i32, _p, _p, _p, _p, _i64, _p, _p, _i32, _p, _p, _i32, _p, _p, _i64, _p],
+        [_p, _i64, _p, _i64, _i32, _i32, _p, _p, _p, _p, _i64, _i64, _p, _p, _i32, _p, _p, _i32, _p, _p, _i64, _p],
     ),
-    "lvamd_verify_drafts_workspace_size": (_i64, [_i64, _i32, _i32]),
+    "lvamd_verify_drafts_workspace_size": (_i64, [_i64, _i64, _i32, _i32]),
     "lvamd_stage_upload": (ctypes.c_int, [_p, _p, _i64, _p, _p]),
     "lvamd_hbm_read_probe": (ctypes.c_int, [_p, _i64, _p, _i32, _p]),
 }
@@ -366,6 +368,18 @@ def attention_q8_entry() -> int:
     """Address of ``lvamd_paged_attention_q8``, for the host module's ``attend_tensors``."""
 
     return ctypes.cast(load().lvamd_paged_attention_q8, ctypes.c_void_p).value
+
+
+def append_q8_entry() -> int:
+    """Address of ``lvamd_kv_append_q8``, for the host module's ``append_tensors``."""
+
+    return ctypes.cast(load().lvamd_kv_append_q8, ctypes.c_void_p).value
+
+
+def verify_entry() -> int:
+    """Address of ``lvamd_verify_drafts``, for the host module's ``verify_tensors``."""
+
+    return ctypes.cast(load().lvamd_verify_drafts, ctypes.c_void_p).value
 
 
 def rotary_entry() -> int:

@@ -241,9 +241,9 @@ _COMPACT_RULES = {
 }
 
 
-def _compact_plan(config, requests, *, keep_equal: bool = False):
+def _compact_bytes(config, requests, *, keep_equal: bool = False) -> tuple[bytearray, bytearray, bytearray]:
     """(moved per request, source slots, target slots) of compact requests,
-    as int64 arrays; the first broken rule raises its error."""
+    as int64 bytes; the first broken rule raises its error."""
 
     rule, _, moved, src, dst = native.host().compact_pairs(requests, config.num_blocks, config.block_size,
                                                            keep_equal)
@@ -252,6 +252,13 @@ def _compact_plan(config, requests, *, keep_equal: bool = False):
         if kind == "kv":
             raise errors.KVCacheError(message)
         raise (ValueError if kind == "value" else TypeError)(message)
+    return moved, src, dst
+
+
+def _compact_plan(config, requests, *, keep_equal: bool = False):
+    """``_compact_bytes`` as int64 arrays."""
+
+    moved, src, dst = _compact_bytes(config, requests, keep_equal=keep_equal)
     return np.frombuffer(moved, dtype=np.int64), np.frombuffer(src, dtype=np.int64), np.frombuffer(dst, dtype=np.int64)
 
 

@@ -19,6 +19,7 @@ are stored as NaN and do not count for the scale.
 
 from __future__ import annotations
 
+import functools
 import weakref
 from dataclasses import dataclass
 
@@ -29,7 +30,7 @@ from torch import Tensor
 from light_vllm_amd import errors, native
 from light_vllm_amd.interfaces import AttentionLayerSpec, ModelKVCacheSpec
 from light_vllm_amd.paged_cache import (
-    PagedKVCacheConfig, PagedKVWriteMapping, _block_copy_pairs, _compact_plan, _compact_request, _launch_block_copy,
+    PagedKVCacheConfig, PagedKVWriteMapping, _block_copy_pairs, _compact_bytes, _compact_request, _launch_block_copy,
     dtype_code,
 )
 from light_vllm_amd.plan import Staging, current_stream
@@ -38,6 +39,14 @@ CODE_DTYPE = torch.float8_e4m3fn
 # Scale of a block that was never written.
 LOWEST_SCALE = 2.0 ** -100
 _HEAD_SIZES = range(32, 257, 16)
+_NOT_FAST = 1 << 30  # append_tensors: a tensor rule of the fast path does not hold
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
+@functools.lru_cache(maxsize=1)
+def _append_tensors():
+    return native.host().append_tensors
 
 
 def quantized_kv_cache_bytes_per_block(model_spec: ModelKVCacheSpec, *, block_size: int) -> int:
@@ -59,8 +68,11 @@ class QuantizedPagedLayerCache:
 
 @dataclass(frozen=True, slots=True)
 class QuantizedKVWriteMapping(PagedKVWriteMapping):
-    """Write slots of one step in which each block's slots are consecutive
+    """Write slots of one step in which each block's slots are consecutive, for
+    caches of this many blocks and block size
     (``QuantizedPagedKVCache.prepare_write``)."""
+
+    geometry: tuple[int, int] = (0, 0)
 
 
 class _State:
@@ -87,7 +99,9 @@ class _State:
         # (block bytes, layers, table, K and V addresses) of codes and scales.
         self.blocks = [(bs * heads * size, *rest) for heads, size, *rest in self.shapes]
         self.blocks += [(4 * heads, *table(ptrs)) for heads, ptrs in scales.items()]
-        self.small_copies = int(native.load().lvamd_kv_block_copy_small_pairs())
+        lib = native.load()
+        self.small_copies = int(lib.lvamd_kv_block_copy_small_pairs())
+        self.few_pairs = int(lib.lvamd_kv_compact_q8_few_pairs())
         self.staging = Staging(device)
 
 
@@ -117,6 +131,9 @@ class QuantizedPagedKVCache:
         self._config = config
         self._layer_specs = {layer.layer_id: layer for layer in model_spec.layers}
         self._layers = {layer.layer_id: self._allocate_layer(layer) for layer in model_spec.layers}
+        self._geometry = (config.num_blocks, config.block_size)
+        # What append_tensors takes of a layer, made at its first write.
+        self._append_facts: dict[str, tuple] = {}
 
     @property
     def config(self) -> PagedKVCacheConfig:
@@ -159,7 +176,8 @@ class QuantizedPagedKVCache:
             raise errors.KVCacheError("slot mapping device must match the cache")
         num_tokens = slot_mapping.numel()
         if not validate:
-            return QuantizedKVWriteMapping(slots=slot_mapping.to(torch.long).contiguous(), num_query_tokens=num_tokens)
+            return QuantizedKVWriteMapping(slots=slot_mapping.to(torch.long).contiguous(), num_query_tokens=num_tokens,
+                                           geometry=self._geometry)
         host = slot_mapping.to("cpu", torch.long).numpy()
         written = np.flatnonzero(host >= 0)
         written = written[np.argsort(host[written], kind="stable")]
@@ -175,12 +193,25 @@ class QuantizedPagedKVCache:
             slots=torch.from_numpy(chosen).to(device),
             num_query_tokens=num_tokens,
             source_indices=None if in_place else torch.from_numpy(written).to(device),
+            geometry=self._geometry,
         )
 
-    @torch.inference_mode()
     def write_prepared(self, layer_id: str, key: Tensor, value: Tensor, mapping: PagedKVWriteMapping) -> None:
         """Quantise one layer's K/V into the slots of a prepared mapping."""
 
+        # The common case in one native call, as the backend's forward: it reads
+        # the tensors itself and launches when every rule holds; anything else
+        # takes the rules below.
+        facts = self._append_facts.get(layer_id) or self._bind_append(layer_id)
+        if (type(mapping) is QuantizedKVWriteMapping and mapping.geometry == self._geometry
+                and mapping.slots.device == self._config.device and torch.cuda.current_device() == facts[2]):
+            slots, sources = mapping.slots, mapping.source_indices
+            status = _append_tensors()(facts, key, value, slots.data_ptr(), 0 if sources is None else sources.data_ptr(),
+                                       slots.numel(), mapping.num_query_tokens)
+            if status == 0:
+                return
+            if status != _NOT_FAST:
+                native.check(status, "lvamd_kv_append_q8")
         layer = self.layer(layer_id)
         spec = self.layer_spec(layer_id)
         cfg = self._config
@@ -189,7 +220,7 @@ class QuantizedPagedKVCache:
             (lambda: key.ndim == 3 and tuple(key.shape[1:]) == tail,
              "paged KV update must have shape [tokens, kv_heads, head_size]"),
             (lambda: value.shape == key.shape, "paged K/V updates must have the same shape"),
-            (lambda: isinstance(mapping, QuantizedKVWriteMapping),
+            (lambda: isinstance(mapping, QuantizedKVWriteMapping) and mapping.geometry == self._geometry,
              "an 8-bit KV cache takes a mapping of its own prepare_write"),
             (lambda: mapping.num_query_tokens == key.shape[0], "slot mapping must have one entry per query token"),
             (lambda: key.dtype == cfg.dtype and key.device == cfg.device,
@@ -215,13 +246,21 @@ class QuantizedPagedKVCache:
                 slots.numel(), spec.num_kv_heads, spec.head_size, cfg.block_size, dtype_code(cfg.dtype),
                 current_stream(cfg.device)), "lvamd_kv_append_q8")
 
-    @torch.inference_mode()
+    def _bind_append(self, layer_id: str) -> tuple:
+        layer, spec, cfg = self.layer(layer_id), self.layer_spec(layer_id), self._config
+        index = cfg.device.index if cfg.device.index is not None else torch.cuda.current_device()
+        found = self._append_facts[layer_id] = (
+            native.append_q8_entry(), cfg.dtype, index, cfg.dtype.itemsize, spec.num_kv_heads, spec.head_size,
+            cfg.block_size, dtype_code(cfg.dtype), layer.keys.data_ptr(), layer.key_scales.data_ptr(),
+            layer.values.data_ptr(), layer.value_scales.data_ptr(), _raw_stream,
+        )
+        return found
+
     def write(self, layer_id: str, key: Tensor, value: Tensor, slot_mapping: Tensor) -> None:
         """Quantise the active tokens' K/V into their physical slots."""
 
         self.write_prepared(layer_id, key, value, self.prepare_write(slot_mapping))
 
-    @torch.inference_mode()
     def compact(
         self,
         block_ids: tuple[int, ...],
@@ -240,7 +279,6 @@ class QuantizedPagedKVCache:
             num_reserved_query_tokens=num_reserved_query_tokens, retained_query_indices=retained_query_indices,
             num_readonly_prefix_blocks=num_readonly_prefix_blocks),))[0]
 
-    @torch.inference_mode()
     def compact_many(self, requests) -> tuple[int, ...]:
         """``compact`` for every request of a step together.  Moved rows keep
         their values; a block that takes one from a block of a larger scale takes
@@ -250,39 +288,42 @@ class QuantizedPagedKVCache:
         if not isinstance(requests, (list, tuple)):
             requests = tuple(requests)
         cfg = self._config
-        moved, src, dst = _compact_plan(cfg, requests)
-        n = int(src.size)
-        if n:
-            blocks = dst // cfg.block_size
-            order = np.argsort(blocks, kind="stable")
-            blocks = blocks[order]
-            first = np.flatnonzero(np.concatenate(([True], blocks[1:] != blocks[:-1])))
-            owner = np.repeat(np.arange(moved.size), moved)[order]
-            if np.any((owner[1:] != owner[:-1]) & (blocks[1:] == blocks[:-1])):
+        moved, src, dst = _compact_bytes(cfg, requests)
+        if src:
+            src, dst = bytes(src), bytes(dst)
+            twice, starts = native.host().block_runs(bytes(moved), dst, cfg.block_size)
+            if twice:
                 raise errors.KVCacheError("compact requests of one step must not write the same block of an 8-bit cache")
-            self._launch_compact(src[order], dst[order], np.append(first, n))
-        return tuple(moved.tolist())
+            with on_device(cfg.device):
+                self._launch_compact(src, dst, starts)
+        return tuple(np.frombuffer(moved, dtype=np.int64).tolist())
 
-    def _launch_compact(self, src: np.ndarray, dst: np.ndarray, starts: np.ndarray) -> None:
+    def _launch_compact(self, src: bytes, dst: bytes, starts: bytes) -> None:
         state = self._state()
         cfg = self._config
-        n, groups = src.size, starts.size - 1
+        n, groups = len(src) // 8, len(starts) // 8 - 1
         lib = native.load()
-        with on_device(cfg.device):
-            packed = np.concatenate((src, dst, starts)).astype(np.int64, copy=False)
-            buf = state.staging.buffer(2 * packed.size)
-            buf[:] = packed.view(np.int32)
-            blob = state.staging.upload(buf)
-            at = blob.data_ptr()
+        slots = cfg.num_blocks * cfg.block_size
+        stream = current_stream(cfg.device)
+        if n <= state.few_pairs:
+            # A few pairs ride in the kernel arguments.
             for heads, size, layers, _, kptrs, vptrs in state.shapes:
-                nbytes = lib.lvamd_kv_compact_q8_workspace_size(n, layers, heads, size)
-                workspace = torch.empty(nbytes, dtype=torch.uint8, device=cfg.device)
-                native.check(lib.lvamd_kv_compact_q8(
-                    kptrs, vptrs, layers, heads, size, cfg.block_size,
-                    cfg.num_blocks * cfg.block_size * heads * size, at, at + 8 * n, n, at + 16 * n, groups,
-                    workspace.data_ptr(), nbytes, current_stream(cfg.device)), "lvamd_kv_compact_q8")
+                native.check(lib.lvamd_kv_compact_q8_few(kptrs, vptrs, layers, heads, size, cfg.block_size,
+                                                         slots * heads * size, src, dst, n, stream),
+                             "lvamd_kv_compact_q8_few")
+            return
+        buf = state.staging.buffer((len(src) + len(dst) + len(starts)) // 4)
+        buf[:] = np.frombuffer(src + dst + starts, dtype=np.int32)
+        blob = state.staging.upload(buf)
+        at = blob.data_ptr()
+        for heads, size, layers, _, kptrs, vptrs in state.shapes:
+            # (Of the call's own stream: two streams' compacts do not share one.)
+            nbytes = lib.lvamd_kv_compact_q8_workspace_size(n, layers, heads, size)
+            workspace = torch.empty(nbytes, dtype=torch.uint8, device=cfg.device)
+            native.check(lib.lvamd_kv_compact_q8(
+                kptrs, vptrs, layers, heads, size, cfg.block_size, slots * heads * size, at, at + 8 * n, n,
+                at + 16 * n, groups, workspace.data_ptr(), nbytes, stream), "lvamd_kv_compact_q8")
 
-    @torch.inference_mode()
     def copy_blocks(self, src_blocks, dst_blocks) -> None:
         """Copy-on-write of whole blocks, codes and scales, across every layer."""
 

@@ -20,9 +20,9 @@ from torch import Tensor
 
 from light_vllm_amd import errors, native
 from light_vllm_amd.interfaces import DraftTree
-from light_vllm_amd.paged_cache import dtype_code
-from light_vllm_amd.plan import current_stream
-from light_vllm_amd.quantized_cache import on_device
+from light_vllm_amd.quantized_cache import _NOT_FAST, _raw_stream, on_device
+
+_CODES = {torch.float32: native.DTYPE_F32, torch.float16: native.DTYPE_F16, torch.bfloat16: native.DTYPE_BF16}
 
 
 class DraftBatch:
@@ -34,7 +34,7 @@ class DraftBatch:
     distribution after the request's last formal token), then one per draft."""
 
     __slots__ = ("num_requests", "num_drafts", "num_rows", "path_width", "chains", "max_token", "counts", "device",
-                 "_blob", "_ptrs")
+                 "_blob", "_facts", "_verify")
 
     def __init__(self, drafts: Sequence[DraftTree], *, device: str | torch.device) -> None:
         self.device = torch.device(device)
@@ -51,8 +51,11 @@ class DraftBatch:
         sizes = [a.size for a in arrays]
         blob = self._blob = torch.from_numpy(np.concatenate(arrays)).to(self.device)
         at = blob.data_ptr()
-        # Addresses of tokens (int64, first: aligned), starts, parents and siblings.
-        self._ptrs = tuple(at + 4 * sum(sizes[:i]) for i in range(4))
+        # (Tokens first: int64, aligned.)
+        tokens, starts, parents, siblings = (at + 4 * sum(sizes[:i]) for i in range(4))
+        self._facts = (native.verify_entry(), self.device.index, self.num_rows, self.num_drafts, self.num_requests,
+                       self.path_width, starts, tokens, parents, siblings, torch.float32, torch.float64, _raw_stream)
+        self._verify = native.host().verify_tensors
 
     def __len__(self) -> int:
         return self.num_requests
@@ -107,7 +110,6 @@ class DraftVerdict:
                      for n, count, path in zip(num_input_queries, counts, paths))
 
 
-@torch.inference_mode()
 def verify_drafts(batch: DraftBatch, target_probs: Tensor, node_uniforms: Tensor, sample_uniforms: Tensor, *,
                   draft_probs: Tensor | None = None) -> DraftVerdict:
     """Accept drafts and draw the token after them, on the current stream.
@@ -126,19 +128,49 @@ def verify_drafts(batch: DraftBatch, target_probs: Tensor, node_uniforms: Tensor
     probability gives token -1.  Sums are in fp64.
     """
 
+    vocab = target_probs.shape[1] if isinstance(target_probs, Tensor) and target_probs.ndim == 2 else 0
+    code = _CODES.get(target_probs.dtype) if vocab else None
+    if (code is None or vocab > 1 << 30 or batch.max_token >= vocab or batch.num_requests > 65535
+            or (draft_probs is not None and not batch.chains)):
+        _refuse(batch, target_probs, node_uniforms, sample_uniforms, draft_probs, vocab)
+    n, device = batch.num_requests, batch.device
+    with on_device(device):
+        counts = torch.empty(n, dtype=torch.int32, device=device)
+        paths = torch.empty((n, batch.path_width), dtype=torch.int32, device=device)
+        tokens = torch.empty(n, dtype=torch.int64, device=device)
+        nbytes = native.load().lvamd_verify_drafts_workspace_size(n, batch.num_drafts, vocab, code)
+        # (Of the call's own stream or graph: no two share one.)
+        workspace = torch.empty(nbytes, dtype=torch.uint8, device=device)
+        outputs = (counts.data_ptr(), paths.data_ptr(), tokens.data_ptr(), workspace.data_ptr(), nbytes)
+        # One native call reads the tensors and launches when every rule holds.
+        status = batch._verify(batch._facts, outputs, target_probs, node_uniforms, sample_uniforms, draft_probs, vocab,
+                               target_probs.dtype, code)
+        if status == _NOT_FAST:
+            _refuse(batch, target_probs, node_uniforms, sample_uniforms, draft_probs, vocab)
+            # Only the layout does not fit.
+            rows = [t if t is None or t.stride(1) == 1 else t.contiguous() for t in (target_probs, draft_probs)]
+            rows = [t if t is None or t.stride(1) == 1 else t.clone(memory_format=torch.contiguous_format) for t in rows]
+            status = batch._verify(batch._facts, outputs, rows[0], node_uniforms.contiguous(),
+                                   sample_uniforms.contiguous(), rows[1], vocab, target_probs.dtype, code)
+        native.check(status, "lvamd_verify_drafts")
+    return DraftVerdict(counts, paths, tokens)
+
+
+def _refuse(batch: DraftBatch, target_probs, node_uniforms, sample_uniforms, draft_probs, vocab: int) -> None:
+    """Raise the first broken rule's message."""
+
     def shape(t, *want) -> bool:
         return isinstance(t, Tensor) and tuple(t.shape) == want
 
-    vocab = target_probs.shape[1] if isinstance(target_probs, Tensor) and target_probs.ndim == 2 else 0
     both = [target_probs] if draft_probs is None else [target_probs, draft_probs]
     rules = (
-        (lambda: vocab > 0 and vocab <= 1 << 30 and shape(target_probs, batch.num_rows, vocab),
+        (lambda: 0 < vocab <= 1 << 30 and shape(target_probs, batch.num_rows, vocab),
          f"target probabilities must have shape [{batch.num_rows}, vocab]"),
         (lambda: draft_probs is None or shape(draft_probs, batch.num_drafts, vocab),
          f"draft probabilities must have shape [{batch.num_drafts}, vocab]"),
         (lambda: draft_probs is None or batch.chains, "draft probabilities need chains of drafts, not trees"),
-        (lambda: all(t.dtype in (torch.float32, torch.float16, torch.bfloat16) and t.dtype == target_probs.dtype
-                     for t in both), "probabilities must be float32, float16 or bfloat16, all of one dtype"),
+        (lambda: all(t.dtype in _CODES and t.dtype == target_probs.dtype for t in both),
+         "probabilities must be float32, float16 or bfloat16, all of one dtype"),
         (lambda: shape(node_uniforms, batch.num_rows), f"node uniforms must have shape [{batch.num_rows}]"),
         (lambda: shape(sample_uniforms, batch.num_requests), f"sample uniforms must have shape [{batch.num_requests}]"),
         (lambda: node_uniforms.dtype == sample_uniforms.dtype and node_uniforms.dtype in (torch.float32, torch.float64),
@@ -151,22 +183,3 @@ def verify_drafts(batch: DraftBatch, target_probs: Tensor, node_uniforms: Tensor
     for holds, message in rules:
         if not holds():
             raise ValueError(message)
-    rows = [t if t.stride(1) == 1 or vocab == 1 else t.contiguous() for t in both]
-    node_uniforms, sample_uniforms = node_uniforms.contiguous(), sample_uniforms.contiguous()
-    lib = native.load()
-    code, n = dtype_code(target_probs.dtype), batch.num_requests
-    device = batch.device
-    with on_device(device):
-        counts = torch.empty(n, dtype=torch.int32, device=device)
-        paths = torch.empty((n, batch.path_width), dtype=torch.int32, device=device)
-        tokens = torch.empty(n, dtype=torch.int64, device=device)
-        nbytes = lib.lvamd_verify_drafts_workspace_size(n, vocab, code)
-        workspace = torch.empty(nbytes, dtype=torch.uint8, device=device)
-        token_ptr, start_ptr, parent_ptr, sibling_ptr = batch._ptrs
-        native.check(lib.lvamd_verify_drafts(
-            rows[0].data_ptr(), rows[0].stride(0), rows[1].data_ptr() if len(rows) > 1 and batch.num_drafts else None,
-            rows[1].stride(0) if len(rows) > 1 else 0, vocab, code, start_ptr, token_ptr, parent_ptr, sibling_ptr, n,
-            node_uniforms.data_ptr(), sample_uniforms.data_ptr(), int(node_uniforms.dtype == torch.float64),
-            counts.data_ptr(), paths.data_ptr(), batch.path_width, tokens.data_ptr(), workspace.data_ptr(), nbytes,
-            current_stream(device)), "lvamd_verify_drafts")
-    return DraftVerdict(counts, paths, tokens)

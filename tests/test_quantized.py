@@ -168,17 +168,46 @@ def test_compact_entry_point_checks() -> None:
     assert call(ws=None) == -3 and call(nbytes=need - 1) == -3 and call(ws=ctypes.c_void_p(8)) == -3
 
 
+def test_compact_few_entry_point_checks() -> None:
+    lib = native.load()
+    n = int(lib.lvamd_kv_compact_q8_few_pairs())
+    assert n == 32
+    pairs = np.arange(n + 1, dtype=np.int64)
+
+    def call(keys=X, layers=2, heads=2, d=128, bs=16, offset=1024, src=pairs, dst=pairs, n=n):
+        return lib.lvamd_kv_compact_q8_few(keys, X, layers, heads, d, bs, offset, src.ctypes.data, dst.ctypes.data, n, None)
+
+    assert call(n=0) == 0
+    assert call(d=40) == -2
+    for bad in (dict(keys=None), dict(layers=0), dict(heads=0), dict(bs=0), dict(offset=-4), dict(offset=2), dict(n=-1),
+                dict(n=n + 1), dict(src=pairs - 1), dict(dst=pairs + 2**31)):
+        assert call(**bad) == -1, bad
+
+
+def test_block_runs() -> None:
+    runs = native.host().block_runs
+    packed = lambda *slots: np.asarray(slots, dtype=np.int64).tobytes()  # noqa: E731
+    twice, starts = runs(packed(3, 0, 4), packed(33, 34, 48, 5, 6, 15, 16), 16)
+    assert not twice and np.frombuffer(starts, dtype=np.int64).tolist() == [0, 2, 3, 6, 7]
+    assert runs(packed(1, 1), packed(33, 34), 16)[0] == 1
+    assert runs(packed(3), packed(33, 48, 34), 16)[0] == 1
+    assert np.frombuffer(runs(b"", b"", 16)[1], dtype=np.int64).tolist() == [0]
+    for bad in ((packed(1), packed(1), 0), (packed(1), packed(1, 2), 4), (packed(2), packed(1), 4), (packed(-1, 2), packed(1), 4)):
+        with pytest.raises(ValueError):
+            runs(*bad)
+
+
 def test_verify_entry_point_checks() -> None:
     lib = native.load()
 
-    def call(target=X, stride=100, vocab=100, dtype=0, starts=X, n=2, width=1, ws=X, nbytes=1 << 20):
-        return lib.lvamd_verify_drafts(target, stride, None, 0, vocab, dtype, starts, X, X, X, n, X, X, 0, X, X, width, X, ws,
-                                       nbytes, None)
+    def call(target=X, stride=100, vocab=100, dtype=0, starts=X, n=2, drafts=3, width=1, ws=X, nbytes=1 << 20):
+        return lib.lvamd_verify_drafts(target, stride, None, 0, vocab, dtype, starts, X, X, X, n, drafts, X, X, 0, X, X, width, X,
+                                       ws, nbytes, None)
 
     assert call(n=0) == 0
     assert call(dtype=3) == -2
     for bad in (dict(target=None), dict(starts=None), dict(vocab=0), dict(vocab=(1 << 30) + 1), dict(n=-1), dict(n=65536),
-                dict(width=0), dict(stride=-1)):
+                dict(width=0), dict(stride=-1), dict(drafts=-1)):
         assert call(**bad) == -1, bad
-    need = lib.lvamd_verify_drafts_workspace_size(2, 100, 0)
+    need = lib.lvamd_verify_drafts_workspace_size(2, 3, 100, 0)
     assert need > 0 and call(nbytes=need - 1) == -3 and call(ws=None) == -3 and call(ws=ctypes.c_void_p(4)) == -3
