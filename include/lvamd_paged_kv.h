@@ -528,8 +528,9 @@ int lvamd_kv_append_q8(const void* key, int64_t key_token_stride, int64_t key_he
 /*
  * Decode attention over an 8-bit cache that holds the step's tokens already:
  * lvamd_paged_decode's stream-K work lists (col_tiles 1, pieces of requests
- * with q_len * group <= 16) and partials; no append.  K and V are the cache's
- * values, so results are those of attention over the dequantised cache.
+ * with q_len * group <= 16) and partials, the rows in fp32 (part_acc
+ * [slots][num_kv_heads][16][head_size] floats); no append.  K and V are the
+ * cache's values, so results are those of attention over the dequantised cache.
  */
 int lvamd_paged_decode_q8(const void* q, int64_t q_token_stride, int64_t q_head_stride,
                           const void* key_pool, const float* key_scales,
@@ -548,7 +549,9 @@ int lvamd_paged_decode_q8_resident_waves(int32_t dtype, int32_t head_size);
 
 /*
  * Prefill and tree attention over an 8-bit cache that holds the step's tokens
- * already: lvamd_paged_prefill's unit records (128 columns) and partials.
+ * already: lvamd_paged_prefill's unit records, of up to `columns` columns (128, or
+ * 64 where every request has at most 64), and partials, [slots][num_kv_heads]
+ * [columns], the rows in fp32.
  */
 int lvamd_paged_prefill_q8(const void* q, int64_t q_token_stride, int64_t q_head_stride,
                            const void* key_pool, const float* key_scales,
@@ -557,16 +560,25 @@ int lvamd_paged_prefill_q8(const void* q, int64_t q_token_stride, int64_t q_head
                            const int32_t* tables, const uint32_t* vis,
                            const int32_t* units, int32_t num_units,
                            void* part_acc, float* part_ml, int64_t num_partial_slots,
-                           int32_t num_kv_heads, int32_t group, int32_t head_size, int32_t block_size,
-                           float scale, int32_t dtype, lvamd_stream_t stream);
+                           int32_t num_kv_heads, int32_t group, int32_t head_size, int32_t columns,
+                           int32_t block_size, float scale, int32_t dtype, lvamd_stream_t stream);
 
-/* Keys per tile of it (key ranges start on multiples), and its workgroups that
- * the current device holds at once (needs a GPU). */
+/* Keys per tile of it (key ranges start on multiples), and its workgroups (of
+ * units of 64 or 128 columns) that the current device holds at once (needs a
+ * GPU). */
 int lvamd_paged_prefill_q8_key_tokens(int32_t dtype, int32_t head_size);
-int lvamd_paged_prefill_q8_resident_units(int32_t dtype, int32_t head_size);
+int lvamd_paged_prefill_q8_resident_units(int32_t dtype, int32_t head_size, int32_t columns);
+
+/* lvamd_paged_attention_merge of fp32 partial rows (dtype, 16 bits, is the
+ * output's): combines those of the two entry points above. */
+int lvamd_paged_attention_merge_q8(const void* part_acc, const float* part_ml,
+                                   void* out, int64_t out_token_stride, int64_t out_head_stride,
+                                   const int32_t* jobs, int32_t num_jobs,
+                                   int32_t num_kv_heads, int32_t group, int32_t head_size, int32_t col_tiles,
+                                   int32_t max_columns, int32_t dtype, lvamd_stream_t stream);
 
 /* One layer's launch facts over an 8-bit cache: lvamd_attention_plan (col_tiles
- * 1, group_waves 1, prefill_col_tiles 8) with the step's slots, and where the
+ * 1, group_waves 1, prefill_col_tiles 8 or 4: units of 128 or 64 columns) with the step's slots, and where the
  * scales lie: scale_offset bytes (a multiple of 16) after each pool's base. */
 typedef struct lvamd_attention_plan_q8 {
   lvamd_attention_plan base;

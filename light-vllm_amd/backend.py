@@ -32,6 +32,7 @@ import torch
 from torch import Tensor
 
 from light_vllm_amd import errors, native
+from light_vllm_amd.facts import facts_of
 from light_vllm_amd.metadata import PagedAttentionMetadata
 from light_vllm_amd.paged_cache import current_stream, dtype_code, hip_append_rotary, is_quantized
 from light_vllm_amd.plan import (
@@ -449,6 +450,15 @@ class HipPagedAttention:
         return found
 
 
+def _quantized_columns(facts, spec) -> int:
+    """Unit width of the 8-bit prefill kernel for a step: 64 columns (one column
+    tile per wave, several tiles in flight) where no request has more, else 128."""
+
+    group = spec.num_query_heads // spec.num_kv_heads
+    return (native.PREFILL_Q8_NARROW if facts.longest * group <= native.PREFILL_Q8_NARROW
+            else native.PREFILL_Q8_COLUMNS)
+
+
 class _QuantizedLaunch(_LayerLaunch):
     """``_LayerLaunch`` over an 8-bit cache: its plan also holds the step's slots
     and where the scales lie behind each pool's codes."""
@@ -456,8 +466,8 @@ class _QuantizedLaunch(_LayerLaunch):
     __slots__ = ("quantized_plan",)
 
     def __init__(self, plan: StepPlan, work, spec, dtype: int, block_size: int, workspace_ptr: int | None,
-                 sizes: tuple[int, int, int, int], scale_offset: int) -> None:
-        super().__init__(plan, work, spec, dtype, block_size, workspace_ptr, native.PREFILL_Q8_COLUMNS, sizes)
+                 prefill_columns: int, sizes: tuple[int, int, int, int], scale_offset: int) -> None:
+        super().__init__(plan, work, spec, dtype, block_size, workspace_ptr, prefill_columns, sizes)
         q = self.quantized_plan = native.AttentionPlanQ8(
             base=self.plan, slots=plan.slots_ptr, num_tokens=plan.num_tokens, scale_offset=scale_offset)
         self.plan_ptr = ctypes.addressof(q)
@@ -500,12 +510,13 @@ class HipQuantizedPagedAttention(HipPagedAttention):
         if found is not None and found.workspace_ptr is not None and found.workspace_ptr != backend.workspace.ptr():
             found = None  # the workspace (shared by all plans) was regrown since
         if found is None:
-            work = plan.layer_work(backend.quantized_facts(spec, code, self._config.block_size))
-            sizes = _partial_layout(work, spec, native.PREFILL_Q8_COLUMNS, self._config.dtype.itemsize)
+            columns = _quantized_columns(plan.facts, spec)
+            work = plan.layer_work(backend.quantized_facts(spec, code, self._config.block_size, columns))
+            sizes = _partial_layout(work, spec, columns, 4)  # fp32 rows
             ptr = None
             if sum(sizes):
                 ptr = backend.workspace.get(sum(sizes), self._config.device).data_ptr()
-            found = _QuantizedLaunch(plan, work, spec, code, self._config.block_size, ptr, sizes,
+            found = _QuantizedLaunch(plan, work, spec, code, self._config.block_size, ptr, columns, sizes,
                                      self._cache.scale_offset(spec))
             plan.launches[key] = found
         return found
@@ -649,21 +660,22 @@ class HipPagedAttentionBackend:
             self._facts[key] = found
         return found
 
-    def quantized_facts(self, spec, code: int, block_size: int) -> tuple[int, ...]:
+    def quantized_facts(self, spec, code: int, block_size: int, columns: int) -> tuple[int, ...]:
         """``kernel_facts`` of the kernels over an 8-bit cache: one decode shape
-        (one column tile, stream-K) and one prefill shape (four waves); the
-        options that choose among the 16-bit kernels' shapes do not apply."""
+        (one column tile, stream-K) and the prefill shape of ``columns`` columns
+        (four waves); the options that choose among the 16-bit kernels' shapes do
+        not apply."""
 
         key = (spec.num_query_heads, spec.num_kv_heads, spec.head_size, code, block_size, torch.cuda.current_device(),
-               "8-bit")
+               columns, "8-bit")
         found = self._facts.get(key)
         if found is None:
             d = spec.head_size
             found = (
-                spec.num_query_heads // spec.num_kv_heads, spec.num_kv_heads, block_size, native.PREFILL_Q8_COLUMNS,
+                spec.num_query_heads // spec.num_kv_heads, spec.num_kv_heads, block_size, columns,
                 native.prefill_q8_key_tokens(code, d), int(self._split_prefill), 1, 4, 1, 0,
                 native.resident_decode_q8_waves(code, d), native.decode_q8_tile_tokens(code, d), 0, 0,
-                native.prefill_q8_resident_units(code, d), 0, self._partition_tokens or 0, DECODE_MAX_COLUMNS,
+                native.prefill_q8_resident_units(code, d, columns), 0, self._partition_tokens or 0, DECODE_MAX_COLUMNS,
                 DECODE_MIN_UNITS_PER_WAVE, PREFILL_MIN_TILES, int(self._shared_prefix), native.xcd_count(),
                 self._prefill_order, 0, 0, DECODE_MERGE_PIECES,
             )
@@ -714,6 +726,21 @@ class HipPagedAttentionBackend:
                 )
         self._head_sizes_ok.add(cache)
 
+    def _quantized_shapes(self, cache, facts) -> LayerShapes:
+        """``_cache_shapes`` of an 8-bit cache, whose prefill shape goes by the
+        step's widest request."""
+
+        config = cache.config
+        code = dtype_code(config.dtype)
+        shapes = {(s.num_query_heads, s.num_kv_heads, s.head_size): s for s in cache.model_spec.layers}
+        columns = tuple(_quantized_columns(facts, spec) for spec in shapes.values())
+        by_columns = self._shapes.setdefault(cache, {})
+        found = by_columns.get(columns)
+        if found is None:
+            found = by_columns[columns] = LayerShapes(
+                self.quantized_facts(spec, code, config.block_size, c) for spec, c in zip(shapes.values(), columns))
+        return found
+
     def _cache_shapes(self, cache) -> LayerShapes:
         """Kernel facts of each distinct supported layer shape of ``cache``
         (looked up once per cache object)."""
@@ -723,9 +750,8 @@ class HipPagedAttentionBackend:
             config = cache.config
             code = dtype_code(config.dtype)
             shapes = {(s.num_query_heads, s.num_kv_heads, s.head_size): s for s in cache.model_spec.layers}
-            facts = self.quantized_facts if is_quantized(cache) else self.kernel_facts
             found = self._shapes[cache] = LayerShapes(
-                facts(spec, code, config.block_size) for spec in shapes.values()
+                self.kernel_facts(spec, code, config.block_size) for spec in shapes.values()
                 if spec.head_size in SUPPORTED_HEAD_SIZES)
         return found
 
@@ -744,7 +770,7 @@ class HipPagedAttentionBackend:
         if config.device.type != "cuda":
             raise errors.KVCacheError("HIP paged attention requires a GPU KV cache")
         self._check_head_sizes(cache)
-        shapes = self._cache_shapes(cache)
+        shapes = self._quantized_shapes(cache, facts_of(metadata)) if is_quantized(cache) else self._cache_shapes(cache)
         # A plan is reusable by a cache of the same pool geometry, dtype and
         # layer shapes: its work lists were built from the kernel facts of
         # those shapes in that dtype.

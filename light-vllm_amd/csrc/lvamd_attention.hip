@@ -82,7 +82,7 @@ extern "C" int lvamd_paged_attention_q8(const lvamd_attention_plan_q8* plan,
     if (p.num_jobs > 0) {
       status = launch_merge(p.part_acc, p.part_ml, out, out_token_stride, out_head_stride, p.jobs, p.num_jobs,
                             p.num_partial_slots, p.merge_depth, p.num_kv_heads, p.group, p.head_size, 1,
-                            p.merge_columns, p.dtype, static_cast<hipStream_t>(stream));
+                            p.merge_columns, p.dtype, static_cast<hipStream_t>(stream), true);
       if (status != LVAMD_OK) return status;
     }
   }
@@ -90,13 +90,14 @@ extern "C" int lvamd_paged_attention_q8(const lvamd_attention_plan_q8* plan,
     status = lvamd_paged_prefill_q8(q, q_token_stride, q_head_stride, key_pool, key_scales, value_pool, value_scales,
                                     out, out_token_stride, out_head_stride, p.tables, p.vis, p.units, p.num_units,
                                     p.prefill_part_acc, p.prefill_part_ml, p.num_prefill_partial_slots, p.num_kv_heads,
-                                    p.group, p.head_size, p.block_size, scale, p.dtype, stream);
+                                    p.group, p.head_size, 16 * p.prefill_col_tiles, p.block_size, scale, p.dtype,
+                                    stream);
     if (status != LVAMD_OK) return status;
     if (p.num_prefill_jobs > 0) {
       status = launch_merge(p.prefill_part_acc, p.prefill_part_ml, out, out_token_stride, out_head_stride,
                             p.prefill_jobs, p.num_prefill_jobs, p.num_prefill_partial_slots, 0, p.num_kv_heads, p.group,
                             p.head_size, p.prefill_col_tiles, p.prefill_merge_columns, p.dtype,
-                            static_cast<hipStream_t>(stream));
+                            static_cast<hipStream_t>(stream), true);
     }
   }
   return status;

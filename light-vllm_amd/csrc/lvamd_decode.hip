@@ -1004,7 +1004,9 @@ struct MergeShape {
 template <typename T, int D, int P>
 constexpr int merge_columns = MergeShape<T, D>::CW * (merge_waves(P) / P);  // per workgroup
 
-template <typename T, int D, int P>
+// T: the partials' type, TO: the output's (they differ over an 8-bit cache only,
+// whose partials are fp32).
+template <typename T, int D, int P, typename TO = T>
 __global__ __launch_bounds__(64 * merge_waves(P)) void paged_merge_kernel(
     const int32_t* __restrict__ jobs,  // [num_jobs][LVAMD_MERGE_FIELDS]
     const int32_t groups,              // workgroups (of merge_columns columns) per (job, kv head)
@@ -1126,9 +1128,9 @@ __global__ __launch_bounds__(64 * merge_waves(P)) void paged_merge_kernel(
   }
   if (!act) return;
   const float inv = lsum > 0.f ? 1.f / lsum : 0.f;
-  T* orow = static_cast<T*>(a.out) + (int64_t)(q_start + qi) * a.out_tok_stride + (int64_t)qhead * a.out_head_stride;
+  TO* orow = static_cast<TO*>(a.out) + (int64_t)(q_start + qi) * a.out_tok_stride + (int64_t)qhead * a.out_head_stride;
 #pragma unroll
-  for (int k = 0; k < EPC; ++k) orow[ch * EPC + k] = from_f32<T>(o[k] * inv);
+  for (int k = 0; k < EPC; ++k) orow[ch * EPC + k] = from_f32<TO>(o[k] * inv);
 }
 
 // ---------------------------------------------------------------------------
@@ -1197,13 +1199,13 @@ static int dispatch_decode(int dtype, int head_size, int col_tiles, F f) {
 
 // One workgroup per (job, kv head, merge_columns columns), over the columns
 // the jobs use; columns past a job's own count exit at once.
-template <typename T, int D, int P>
+template <typename T, int D, int P, typename TO = T>
 static int launch_merge_p(int64_t job_heads, int64_t max_columns, hipStream_t s, const int32_t* jobs,
                           int32_t num_kv_heads, int32_t group, int32_t col_tiles, const MergeArgs& a) {
   const int64_t groups = (max_columns + merge_columns<T, D, P> - 1) / merge_columns<T, D, P>;
   if (job_heads * groups > 0x7fffffffLL) return LVAMD_ERR_INVALID_ARGUMENT;
   const FastDiv by_groups((int32_t)groups), by_heads(num_kv_heads);
-  hipLaunchKernelGGL((paged_merge_kernel<T, D, P>), dim3((unsigned)(job_heads * groups)), dim3(64 * merge_waves(P)), 0,
+  hipLaunchKernelGGL((paged_merge_kernel<T, D, P, TO>), dim3((unsigned)(job_heads * groups)), dim3(64 * merge_waves(P)), 0,
                      s, jobs, (int32_t)groups, num_kv_heads, group, col_tiles, by_groups.magic, by_groups.shift,
                      by_heads.magic, by_heads.shift, a);
   return launch_status();
@@ -1238,7 +1240,7 @@ static int merge_sharing(int64_t num_jobs, int64_t num_partials, int64_t merge_d
 int launch_merge(const void* part_acc, const float* part_ml, void* out, int64_t out_token_stride,
                  int64_t out_head_stride, const int32_t* jobs, int32_t num_jobs, int64_t num_partials,
                  int64_t merge_depth, int32_t num_kv_heads, int32_t group, int32_t head_size, int32_t col_tiles, int32_t max_columns,
-                 int32_t dtype, hipStream_t s) {
+                 int32_t dtype, hipStream_t s, bool fp32_partials) {
   if (dtype_size(dtype) == 0 || !head_size_supported(head_size) || col_tiles < 1 || col_tiles > 16)
     return LVAMD_ERR_UNSUPPORTED;
   if (max_columns < 1 || max_columns > 16 * col_tiles) return LVAMD_ERR_INVALID_ARGUMENT;
@@ -1252,6 +1254,20 @@ int launch_merge(const void* part_acc, const float* part_ml, void* out, int64_t 
   a.out_tok_stride = out_token_stride;
   a.out_head_stride = out_head_stride;
   const int64_t job_heads = (int64_t)num_jobs * num_kv_heads;
+  if (fp32_partials && dtype_size(dtype) == 2) {
+    return dispatch_decode(dtype, head_size, 1, [&]<typename T, int D, int CTW>() -> int {
+      if constexpr (sizeof(T) == 2) {
+        switch (merge_sharing(num_jobs, num_partials, merge_depth,
+                              job_heads * ((max_columns + merge_columns<float, D, 16> - 1) / merge_columns<float, D, 16>))) {
+          case 16: return launch_merge_p<float, D, 16, T>(job_heads, max_columns, s, jobs, num_kv_heads, group, col_tiles, a);
+          case 4: return launch_merge_p<float, D, 4, T>(job_heads, max_columns, s, jobs, num_kv_heads, group, col_tiles, a);
+          default: return launch_merge_p<float, D, 1, T>(job_heads, max_columns, s, jobs, num_kv_heads, group, col_tiles, a);
+        }
+      } else {
+        return LVAMD_ERR_UNSUPPORTED;  // (not reached)
+      }
+    });
+  }
   return dispatch_decode(dtype, head_size, 1, [&]<typename T, int D, int CTW>() -> int {
     switch (merge_sharing(num_jobs, num_partials, merge_depth,
                           job_heads * ((max_columns + merge_columns<T, D, 16> - 1) / merge_columns<T, D, 16>))) {
@@ -1401,4 +1417,14 @@ extern "C" int lvamd_paged_attention_merge(const void* part_acc, const float* pa
                                            int32_t max_columns, int32_t dtype, lvamd_stream_t stream) {
   return launch_merge(part_acc, part_ml, out, out_token_stride, out_head_stride, jobs, num_jobs, 0, 0, num_kv_heads,
                       group, head_size, col_tiles, max_columns, dtype, static_cast<hipStream_t>(stream));
+}
+
+extern "C" int lvamd_paged_attention_merge_q8(const void* part_acc, const float* part_ml,
+                                              void* out, int64_t out_token_stride, int64_t out_head_stride,
+                                              const int32_t* jobs, int32_t num_jobs, int32_t num_kv_heads,
+                                              int32_t group, int32_t head_size, int32_t col_tiles,
+                                              int32_t max_columns, int32_t dtype, lvamd_stream_t stream) {
+  if (dtype != LVAMD_BF16 && dtype != LVAMD_F16) return LVAMD_ERR_UNSUPPORTED;
+  return launch_merge(part_acc, part_ml, out, out_token_stride, out_head_stride, jobs, num_jobs, 0, 0, num_kv_heads,
+                      group, head_size, col_tiles, max_columns, dtype, static_cast<hipStream_t>(stream), true);
 }

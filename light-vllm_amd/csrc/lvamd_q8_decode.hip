@@ -378,9 +378,10 @@ __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(1, 1))) void
           for (int n = 0; n < NT; ++n) store_partial4<false, T>(row + 16 * n + 4 * g, acc[n], l_tot == l_tot ? inv : l_tot);
         } else {
           const int64_t cs = ((int64_t)cur.slot * Hkv + kvh) * 16 + l16;
-          T* row = static_cast<T*>(a.part_acc) + cs * D;
+          float* row = static_cast<float*>(a.part_acc) + cs * D;
 #pragma unroll
-          for (int n = 0; n < NT; ++n) store_partial4<false, T>(row + 16 * n + 4 * g, acc[n], l_tot == l_tot ? inv : l_tot);
+          for (int n = 0; n < NT; ++n)
+            store_partial4<false, float>(row + 16 * n + 4 * g, acc[n], l_tot == l_tot ? inv : l_tot);
           // (A NaN sum keeps a finite maximum: the merge passes over a
           // partial whose maximum is -inf.)
           const float m = l_tot == l_tot || m_run != -INFINITY ? m_run : 0.f;

@@ -9,7 +9,10 @@
 // Mapping onto CDNA4:
 //   * A unit is up to 128 columns, (query, head-in-group) pairs of one kv head;
 //     four waves of two 16-column tiles share every key tile (64 keys, 32
-//     above D = 128).
+//     above D = 128).  Steps whose requests all have at most 64 columns (tree
+//     verification, short chunks) take units of 64, one column tile per wave:
+//     no wave is left without columns, and the registers hold several tiles in
+//     flight, as such units are bound by the latency of their few tiles.
 //   * A tile's codes go to registers (16 per load and thread) while the last
 //     tile computes, become T with their block's scale (exactly, lvamd_q8.h)
 //     and are written to the other of two LDS buffers; one barrier per tile.
@@ -29,9 +32,8 @@ namespace lvamd {
 namespace {
 
 constexpr float kSlack = 8.0f;  // lazy-rescale threshold, log2 units
-constexpr int kUnitColumns = 128;
 constexpr int kWaves = 4;
-constexpr int kColTiles = 2;  // per wave
+constexpr int unit_columns(int col_tiles) { return 16 * kWaves * col_tiles; }
 
 struct Q8PrefillArgs {
   const void* q;
@@ -52,7 +54,7 @@ struct Q8PrefillArgs {
   float scale_log2;
 };
 
-template <int D>
+template <int D, int CT>
 struct Q8PrefillShape {
   static constexpr int KT = D <= 128 ? 64 : 32;
   static constexpr int KS = KT / 16;
@@ -63,17 +65,19 @@ struct Q8PrefillShape {
   static constexpr int LPT = (KT * C8 + THREADS - 1) / THREADS;  // loads per thread and tensor
   static constexpr int NCH = (D + 31) / 32;
   static constexpr int NT = D / 16;
+  static constexpr int PD = CT == 2 ? 1 : D <= 128 ? 4 : 2;  // tiles in flight
 };
 
 }  // namespace
 
-template <typename T, int D>
+// CT: column tiles per wave, 2 or 1.
+template <typename T, int D, int CT>
 __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(D <= 128 ? 2 : 1))) void q8_prefill_kernel(
     const int32_t* __restrict__ units, const int32_t num_kv_heads, const uint32_t heads_magic, const int32_t heads_shift,
     const Q8PrefillArgs a) {
-  using P = Q8PrefillShape<D>;
+  using P = Q8PrefillShape<D, CT>;
   constexpr int KT = P::KT, KS = P::KS, C8 = P::C8, CPR = P::CPR, RS = P::RS, LPT = P::LPT, NCH = P::NCH, NT = P::NT;
-  constexpr int CT = kColTiles;
+  constexpr int PD = P::PD;
   using V8 = typename std::conditional<std::is_same<T, __bf16>::value, bf16x8, f16x8>::type;
   __shared__ __attribute__((aligned(16))) uint4 klds[2][KT * RS];
   __shared__ __attribute__((aligned(16))) uint4 vlds[2][KT * RS];
@@ -91,6 +95,7 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(D <
   const int32_t* u = units + (int64_t)unit * LVAMD_PREFILL_FIELDS;
   const int col0 = u[1], ncols = u[2], key_begin = u[3], key_end = u[4], slot = u[5];
   const int table_off = u[6], q_start = u[7], computed = u[8], q_len = u[9], vis_off = u[10], vis_words = u[11];
+  const int b0 = u[12], b1 = u[13], b2 = u[14], b3 = u[15];  // of the unit's first tile; -1: take them from the table
   if (ncols <= 0) return;  // a padding record (the host's per-XCD unit order)
   const int col_end = col0 + ncols;
   const int kneed = computed + fast_div(col_end - 1, a.by_group) + 1;
@@ -115,6 +120,18 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(D <
   auto lookup = [&](int t, int (&block)[LPT]) {
 #pragma unroll
     for (int j = 0; j < LPT; ++j) block[j] = table[fast_div(key_pos(t, j), a.by_block)];
+  };
+  // Tile 0's from the unit's record where it has them: no wait for the table.
+  auto lookup_first = [&](int (&block)[LPT]) {
+    if (b0 < 0) {
+      lookup(0, block);
+      return;
+    }
+#pragma unroll
+    for (int j = 0; j < LPT; ++j) {
+      const int k = fast_div(key_pos(0, j), a.by_block) - fast_div(key_begin, a.by_block);
+      block[j] = k == 0 ? b0 : k == 1 ? b1 : k == 2 ? b2 : b3;
+    }
   };
   struct Tile {
     uint4 k[LPT], v[LPT];
@@ -196,6 +213,16 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(D <
   // Tiles below this bound are visible to every column of the unit.
   const int full_tiles = (tree ? computed : computed + fast_div(col0, a.by_group) + 1) / KT;
   const float c_log2 = a.scale_log2;
+  // A tree's ancestor words: the first two of each column's row are loaded here
+  // (a load among the tiles' would wait for those before it); longer rows are
+  // read where a tile needs them.
+  const bool few_words = vis_words <= 2;
+  uint32_t row_word0[CT], row_word1[CT];
+#pragma unroll
+  for (int ct = 0; ct < CT; ++ct) {
+    row_word0[ct] = tree && few_words ? a.vis[vis_off + qi[ct] * vis_words] : 0u;
+    row_word1[ct] = tree && vis_words == 2 ? a.vis[vis_off + qi[ct] * vis_words + 1] : 0u;
+  }
   // Whether a column sees the step's token j.
   auto sees = [&](int ct, int j) -> bool {
     if (!tree) return j <= qi[ct];
@@ -274,7 +301,10 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(D <
             const int wi = (j0 >> 5) + i;
             const int left = q_len - 32 * wi;
             const uint32_t valid = left >= 32 ? ~0u : left <= 0 ? 0u : (1u << left) - 1;
-            const uint32_t row = a.vis[vis_off + qi[ct] * vis_words + min(max(wi, 0), vis_words - 1)];
+            const int wc = min(max(wi, 0), vis_words - 1);
+            const uint32_t w0 = row_word0[ct], w1 = row_word1[ct];
+            uint32_t row = wc == 0 ? w0 + 0u : w1 + 0u;  // (values: a choice of lvalues would put the arrays in memory)
+            if (!few_words) row = a.vis[vis_off + qi[ct] * vis_words + wc];
             const uint32_t word = wi < 0 ? ~0u : row & valid;
             if (i > 0) {
               const uint32_t bits = __builtin_amdgcn_alignbit(word, low, j0 & 31) >> (4 * g);
@@ -363,36 +393,52 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(D <
     }
   };
 
-  // ---- tile t computes while tile t + 1's codes and tile t + 2's table
-  // entries are in flight.  (A buffer's flag stays set: compute looks at the
-  // rows themselves.)
-  Tile x;
-  int block[LPT];
+  // ---- PD tiles' codes are in flight while a tile computes; the table entries
+  // of a tile are loaded PD tiles before its codes.  Tile t is staged into buffer
+  // t % 2; the barrier after it tells that every wave is done with tile t - 1's
+  // predecessor in that buffer.  (A buffer's flag stays set: compute looks at
+  // the rows themselves.)  No load is conditional in the steady loop, so that
+  // each wait counts only the loads before its own: past the last tile they
+  // repeat it.
+  const int last_tile = ntiles - 1;
+  Tile x[PD];
+  int block[PD][LPT];
   if (tid < 2) poison[tid] = 0;
-  lookup(0, block);
-  issue(0, block, x);
-  if (ntiles > 1) lookup(1, block);
-  __syncthreads();
-  stage(0, x, klds[0], vlds[0], &poison[0]);
-  __syncthreads();
-  auto step = [&]<bool MASKED>(int t, int b) __attribute__((always_inline)) {
-    const bool more = !MASKED || t + 1 < ntiles;
-    if (more) {
-      issue(t + 1, block, x);
-      if (!MASKED || t + 2 < ntiles) lookup(t + 2, block);
-    }
-    compute.template operator()<MASKED>(t, klds[b], vlds[b], &poison[b]);
-    if (more) {
-      stage(t + 1, x, klds[b ^ 1], vlds[b ^ 1], &poison[b ^ 1]);
+  lookup_first(block[0]);
+#pragma unroll
+  for (int i = 1; i < PD; ++i) lookup(min(i, last_tile), block[i]);
+  int ahead[PD][LPT];
+#pragma unroll
+  for (int i = 0; i < PD; ++i) lookup(min(PD + i, last_tile), ahead[i]);
+#pragma unroll
+  for (int i = 0; i < PD; ++i) issue(min(i, last_tile), block[i], x[i]);
+  __syncthreads();  // (the flags are clear)
+  // PD tiles from t on.  MORE: tiles follow them; MASKED: as compute's.
+  auto run = [&]<bool MORE, bool MASKED>(int t0) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < PD; ++i) {
+      const int t = t0 + i;
+      if (!MORE && t > last_tile) return;
+      const int b = t & 1;
+      stage(t, x[i], klds[b], vlds[b], &poison[b]);
+      if constexpr (MORE) {
+#pragma unroll
+        for (int j = 0; j < LPT; ++j) block[i][j] = ahead[i][j];
+        lookup(min(t + 2 * PD, last_tile), ahead[i]);
+        issue(min(t + PD, last_tile), block[i], x[i]);
+      }
       __syncthreads();
+      compute.template operator()<MASKED>(t, klds[b], vlds[b], &poison[b]);
     }
   };
-  // Tiles that every column sees, before the step's own tokens, with one to
-  // follow; then the rest.  (lookup past the last tile repeats its last key.)
-  const int nfull = min(min(full_tiles, computed / KT) - tile0, ntiles - 1);
   int t = 0;
-  for (; t < nfull; ++t) step.template operator()<false>(t, t & 1);
-  for (; t < ntiles; ++t) step.template operator()<true>(t, t & 1);
+  if constexpr (PD == 1) {
+    // Tiles that every column sees, before the step's own tokens; then the rest.
+    const int nfull = min(min(full_tiles, computed / KT) - tile0, last_tile);
+    for (; t < nfull; ++t) run.template operator()<true, false>(t);
+  }
+  for (; t + PD <= last_tile; t += PD) run.template operator()<true, true>(t);
+  run.template operator()<false, true>(t);
 
   // ---- normalised output rows, or this piece's partials
   if (!wave_active) return;
@@ -402,10 +448,10 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(D <
     const float l_tot = l_run[ct][0];
     const float inv = l_tot > 0.f ? 1.f / l_tot : l_tot == 0.f ? 0.f : l_tot;  // (NaN stays)
     if (slot >= 0) {
-      const int64_t cs = ((int64_t)slot * Hkv + kvh) * kUnitColumns + 16 * (CT * wave + ct) + l16;
-      T* row = static_cast<T*>(a.part_acc) + cs * D;
+      const int64_t cs = ((int64_t)slot * Hkv + kvh) * unit_columns(CT) + 16 * (CT * wave + ct) + l16;
+      float* row = static_cast<float*>(a.part_acc) + cs * D;
 #pragma unroll
-      for (int n = 0; n < NT; ++n) store_partial4<true, T>(row + 16 * n + 4 * g, acc[ct][n], inv);
+      for (int n = 0; n < NT; ++n) store_partial4<true, float>(row + 16 * n + 4 * g, acc[ct][n], inv);
       // (A NaN sum keeps a finite maximum: the merge passes over a partial
       // whose maximum is -inf.)
       const float m = l_tot == l_tot || m_run[ct] != -INFINITY ? m_run[ct] : 0.f;
@@ -426,30 +472,34 @@ bool prefill_q8_supported(int dtype, int head_size) {
   return (dtype == LVAMD_BF16 || dtype == LVAMD_F16) && head_size >= 32 && head_size <= 256 && head_size % 16 == 0;
 }
 
-template <typename T, typename F>
+template <typename T, int CT, typename F>
 int with_prefill_head_size(int head_size, F& f) {
   switch (head_size) {
-    case 32: return f.template operator()<T, 32>();
-    case 48: return f.template operator()<T, 48>();
-    case 64: return f.template operator()<T, 64>();
-    case 80: return f.template operator()<T, 80>();
-    case 96: return f.template operator()<T, 96>();
-    case 112: return f.template operator()<T, 112>();
-    case 128: return f.template operator()<T, 128>();
-    case 144: return f.template operator()<T, 144>();
-    case 160: return f.template operator()<T, 160>();
-    case 176: return f.template operator()<T, 176>();
-    case 192: return f.template operator()<T, 192>();
-    case 208: return f.template operator()<T, 208>();
-    case 224: return f.template operator()<T, 224>();
-    case 240: return f.template operator()<T, 240>();
-    case 256: return f.template operator()<T, 256>();
+    case 32: return f.template operator()<T, 32, CT>();
+    case 48: return f.template operator()<T, 48, CT>();
+    case 64: return f.template operator()<T, 64, CT>();
+    case 80: return f.template operator()<T, 80, CT>();
+    case 96: return f.template operator()<T, 96, CT>();
+    case 112: return f.template operator()<T, 112, CT>();
+    case 128: return f.template operator()<T, 128, CT>();
+    case 144: return f.template operator()<T, 144, CT>();
+    case 160: return f.template operator()<T, 160, CT>();
+    case 176: return f.template operator()<T, 176, CT>();
+    case 192: return f.template operator()<T, 192, CT>();
+    case 208: return f.template operator()<T, 208, CT>();
+    case 224: return f.template operator()<T, 224, CT>();
+    case 240: return f.template operator()<T, 240, CT>();
+    case 256: return f.template operator()<T, 256, CT>();
     default: return LVAMD_ERR_UNSUPPORTED;
   }
 }
 template <typename F>
-int dispatch_prefill(int dtype, int head_size, F f) {
-  return dtype == LVAMD_BF16 ? with_prefill_head_size<__bf16>(head_size, f) : with_prefill_head_size<_Float16>(head_size, f);
+int dispatch_prefill(int dtype, int head_size, int columns, F f) {
+  if (columns == 64)
+    return dtype == LVAMD_BF16 ? with_prefill_head_size<__bf16, 1>(head_size, f)
+                               : with_prefill_head_size<_Float16, 1>(head_size, f);
+  return dtype == LVAMD_BF16 ? with_prefill_head_size<__bf16, 2>(head_size, f)
+                             : with_prefill_head_size<_Float16, 2>(head_size, f);
 }
 
 }  // namespace
@@ -463,14 +513,14 @@ extern "C" int lvamd_paged_prefill_q8_key_tokens(int32_t dtype, int32_t head_siz
   return head_size <= 128 ? 64 : 32;
 }
 
-extern "C" int lvamd_paged_prefill_q8_resident_units(int32_t dtype, int32_t head_size) {
-  if (!prefill_q8_supported(dtype, head_size)) return LVAMD_ERR_UNSUPPORTED;
-  return dispatch_prefill(dtype, head_size, []<typename T, int D>() -> int {
+extern "C" int lvamd_paged_prefill_q8_resident_units(int32_t dtype, int32_t head_size, int32_t columns) {
+  if (!prefill_q8_supported(dtype, head_size) || (columns != 64 && columns != 128)) return LVAMD_ERR_UNSUPPORTED;
+  return dispatch_prefill(dtype, head_size, columns, []<typename T, int D, int CT>() -> int {
     int device = 0, cus = 0, per_cu = 0;
     if (hipGetDevice(&device) != hipSuccess) return LVAMD_ERR_LAUNCH;
     if (hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, device) != hipSuccess)
       return LVAMD_ERR_LAUNCH;
-    if (hipOccupancyMaxActiveBlocksPerMultiprocessor(&per_cu, reinterpret_cast<const void*>(&q8_prefill_kernel<T, D>),
+    if (hipOccupancyMaxActiveBlocksPerMultiprocessor(&per_cu, reinterpret_cast<const void*>(&q8_prefill_kernel<T, D, CT>),
                                                      64 * kWaves, 0) != hipSuccess)
       return LVAMD_ERR_LAUNCH;
     return per_cu * cus;
@@ -482,9 +532,9 @@ extern "C" int lvamd_paged_prefill_q8(const void* q, int64_t q_token_stride, int
                                       void* out, int64_t out_token_stride, int64_t out_head_stride,
                                       const int32_t* tables, const uint32_t* vis, const int32_t* units,
                                       int32_t num_units, void* part_acc, float* part_ml, int64_t num_partial_slots,
-                                      int32_t num_kv_heads, int32_t group, int32_t head_size, int32_t block_size,
-                                      float scale, int32_t dtype, lvamd_stream_t stream) {
-  if (!prefill_q8_supported(dtype, head_size)) return LVAMD_ERR_UNSUPPORTED;
+                                      int32_t num_kv_heads, int32_t group, int32_t head_size, int32_t columns,
+                                      int32_t block_size, float scale, int32_t dtype, lvamd_stream_t stream) {
+  if (!prefill_q8_supported(dtype, head_size) || (columns != 64 && columns != 128)) return LVAMD_ERR_UNSUPPORTED;
   if (num_units < 0 || num_kv_heads <= 0 || group <= 0 || block_size <= 0 || num_partial_slots < 0)
     return LVAMD_ERR_INVALID_ARGUMENT;
   if (num_units == 0) return LVAMD_OK;
@@ -515,8 +565,8 @@ extern "C" int lvamd_paged_prefill_q8(const void* q, int64_t q_token_stride, int
   a.scale_log2 = scale * 1.4426950408889634f;
   const FastDiv by_heads(num_kv_heads);
   hipStream_t s = static_cast<hipStream_t>(stream);
-  return dispatch_prefill(dtype, head_size, [&]<typename T, int D>() -> int {
-    hipLaunchKernelGGL((q8_prefill_kernel<T, D>), dim3((unsigned)(num_units * num_kv_heads)), dim3(64 * kWaves), 0, s,
+  return dispatch_prefill(dtype, head_size, columns, [&]<typename T, int D, int CT>() -> int {
+    hipLaunchKernelGGL((q8_prefill_kernel<T, D, CT>), dim3((unsigned)(num_units * num_kv_heads)), dim3(64 * kWaves), 0, s,
                        units, num_kv_heads, by_heads.magic, by_heads.shift, a);
     return launch_status();
   });

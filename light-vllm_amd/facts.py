@@ -100,6 +100,12 @@ class StepFacts:
     vis = _array_property(8, "vis")
 
     @property
+    def longest(self) -> int:
+        """Most queries of a request."""
+
+        return int(self.q_lens.max())
+
+    @property
     def num_blocks_listed(self) -> int:
         return len(self.raw[0]) // 4
 

@@ -118,10 +118,14 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "lvamd_paged_prefill_q8": (
         ctypes.c_int,
         [_p, _i64, _i64, _p, _p, _p, _p, _p, _i64, _i64, _p, _p, _p, _i32, _p, _p, _i64,
-         _i32, _i32, _i32, _i32, _f32, _i32, _p],
+         _i32, _i32, _i32, _i32, _i32, _f32, _i32, _p],
     ),
     "lvamd_paged_prefill_q8_key_tokens": (ctypes.c_int, [_i32, _i32]),
-    "lvamd_paged_prefill_q8_resident_units": (ctypes.c_int, [_i32, _i32]),
+    "lvamd_paged_prefill_q8_resident_units": (ctypes.c_int, [_i32, _i32, _i32]),
+    "lvamd_paged_attention_merge_q8": (
+        ctypes.c_int,
+        [_p, _p, _p, _i64, _i64, _p, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _p],
+    ),
     "lvamd_paged_attention_q8": (
         ctypes.c_int,
         [_p, _p, _i64, _i64, _p, _i64, _i64, _p, _i64, _i64, _p, _p, _p, _i64, _i64, _f32, _p],
@@ -167,8 +171,8 @@ class AttentionPlanQ8(ctypes.Structure):
 
 # Most drafts of a request that lvamd_verify_drafts takes.
 VERIFY_MAX_DRAFTS = 1024
-# Columns per prefill unit of the 8-bit kernel.
-PREFILL_Q8_COLUMNS = 128
+# Columns per prefill unit of the 8-bit kernel: steps of narrow requests, others.
+PREFILL_Q8_NARROW, PREFILL_Q8_COLUMNS = 64, 128
 
 
 def library_path() -> Path:
@@ -348,10 +352,10 @@ def prefill_q8_key_tokens(dtype_code: int, head_size: int) -> int:
     return found
 
 
-def prefill_q8_resident_units(dtype_code: int, head_size: int) -> int:
-    """Workgroups of the 8-bit prefill kernel the current GPU holds at once."""
+def prefill_q8_resident_units(dtype_code: int, head_size: int, columns: int) -> int:
+    """Workgroups of the 8-bit prefill kernel of this unit width the current GPU holds at once."""
 
-    found = int(load().lvamd_paged_prefill_q8_resident_units(dtype_code, head_size))
+    found = int(load().lvamd_paged_prefill_q8_resident_units(dtype_code, head_size, columns))
     check(min(found, 0), "lvamd_paged_prefill_q8_resident_units")
     return found
 

@@ -126,9 +126,9 @@ def test_attention_entry_point_checks() -> None:
         return lib.lvamd_paged_decode_q8(q, *qs, X, X, X, X, X, 3584, 128, X, X, waves, X, X, part, part, slots, heads, group, d,
                                          bs, f, dtype, None)
 
-    def prefill(q=X, units=1, slots=0, heads=4, group=7, d=128, bs=16, dtype=2, qs=(3584, 128), part=None):
+    def prefill(q=X, units=1, slots=0, heads=4, group=7, d=128, bs=16, dtype=2, qs=(3584, 128), part=None, columns=128):
         return lib.lvamd_paged_prefill_q8(q, *qs, X, X, X, X, X, 3584, 128, X, X, X, units, part, part, slots, heads, group, d,
-                                          bs, f, dtype, None)
+                                          columns, bs, f, dtype, None)
 
     for call, none in ((decode, "waves"), (prefill, "units")):
         assert call(**{none: 0}) == 0
@@ -137,6 +137,9 @@ def test_attention_entry_point_checks() -> None:
             assert call(**bad) == -1, bad
         assert call(slots=3) == -3
     assert decode(group=17) == -1
+    assert prefill(columns=32) == -2 and prefill(columns=256) == -2 and prefill(columns=64, q=None) == -1
+    merge = lambda dtype, jobs, cols=1: lib.lvamd_paged_attention_merge_q8(X, X, X, 0, 0, X, jobs, 4, 7, 128, cols, 16, dtype, None)  # noqa: E731
+    assert merge(2, 0) == 0 and merge(0, 1) == -2 and merge(2, -1) == -1 and merge(1, 1, 17) == -2
     for d in (32, 64, 80, 128, 256):
         assert lib.lvamd_paged_decode_q8_tile_tokens(2, d) * d <= 8192
         assert lib.lvamd_paged_prefill_q8_key_tokens(1, d) == (64 if d <= 128 else 32)
