@@ -526,15 +526,20 @@ int lvamd_kv_append_q8(const void* key, int64_t key_token_stride, int64_t key_he
                        lvamd_stream_t stream);
 
 /*
- * Decode attention over an 8-bit cache that holds the step's tokens already:
- * lvamd_paged_decode's stream-K work lists (col_tiles 1, pieces of requests
- * with q_len * group <= 16) and partials, the rows in fp32 (part_acc
- * [slots][num_kv_heads][16][head_size] floats); no append.  K and V are the
- * cache's values, so results are those of attention over the dequantised cache.
+ * Decode attention over an 8-bit cache: lvamd_paged_decode's stream-K work lists
+ * (col_tiles 1, pieces of requests with q_len * group <= 16, cut on multiples
+ * of the tile) and partials, the rows in fp32 (part_acc [slots][num_kv_heads]
+ * [16][head_size] floats).  K and V are the cache's values, so results are those
+ * of attention over the dequantised cache.
+ * Append: when new_key / new_value are given, the kernel appends this step's
+ * tokens of its requests as lvamd_kv_append_q8 does, and attends them as stored;
+ * block_size must then divide the tile.  When they are NULL the cache must hold
+ * them already.
  */
 int lvamd_paged_decode_q8(const void* q, int64_t q_token_stride, int64_t q_head_stride,
-                          const void* key_pool, const float* key_scales,
-                          const void* value_pool, const float* value_scales,
+                          const void* new_key, int64_t new_key_token_stride, int64_t new_key_head_stride,
+                          const void* new_value, int64_t new_value_token_stride, int64_t new_value_head_stride,
+                          void* key_pool, float* key_scales, void* value_pool, float* value_scales,
                           void* out, int64_t out_token_stride, int64_t out_head_stride,
                           const int32_t* pieces, const int32_t* wave_first, int32_t waves_per_head,
                           const int32_t* tables, const uint32_t* vis,
@@ -582,7 +587,7 @@ int lvamd_paged_attention_merge_q8(const void* part_acc, const float* part_ml,
  * scales lie: scale_offset bytes (a multiple of 16) after each pool's base. */
 typedef struct lvamd_attention_plan_q8 {
   lvamd_attention_plan base;
-  const int64_t* slots; /* [num_tokens], a block's slots consecutive */
+  const int64_t* slots; /* [num_tokens], a block's slots consecutive; or NULL */
   int64_t num_tokens;
   int64_t scale_offset;
 } lvamd_attention_plan_q8;
@@ -591,7 +596,8 @@ typedef struct lvamd_attention_plan_q8 {
  * A layer's whole step over an 8-bit cache, on one stream: the quantising
  * append (unless new_key / new_value are NULL), then the decode, merge, prefill
  * and merge launches.  A query attends what the cache holds, its own token's
- * stored K and V included.  Arguments as lvamd_paged_attention.
+ * stored K and V included.  With slots NULL the decode launch appends; there
+ * must be no prefill units then.  Arguments as lvamd_paged_attention.
  */
 int lvamd_paged_attention_q8(const lvamd_attention_plan_q8* plan,
                              const void* q, int64_t q_token_stride, int64_t q_head_stride,

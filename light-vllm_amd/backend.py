@@ -459,6 +459,25 @@ def _quantized_columns(facts, spec) -> int:
             else native.PREFILL_Q8_COLUMNS)
 
 
+_APPEND_UNITS = 3
+
+
+def _decode_appends(work, dtype: int, head_size: int, block_size: int) -> bool:
+    """Whether a step's decode launch appends its tokens itself: steps without
+    prefill units, of at most three tiles per wave, with whole blocks per tile.
+
+    It saves a launch, but the waves that append wait for the tokens' rows, and
+    the registers it takes slow the loop over the other tiles.  Microseconds a
+    step, a launch of its own against none, at D = 128 bf16: 12.4 / 9.1 (64
+    sequences of 16 tokens, 1 tile per wave), 18.5 / 16.2 (of 300, 2), 23.1 /
+    21.6 (of 600, 3), 24.9 / 26.1 (of 1000, 4), 39.8 / 48.4 (of 2500, 10); 16
+    sequences of 2500, 3 tiles: 21.2 / 21.5; D = 64: 26.9 / 25.0 (3), 32.6 / 32.1
+    (5)."""
+
+    return (not work.num_prefill_units and 0 < work.units_per_wave <= _APPEND_UNITS
+            and native.load().lvamd_paged_decode_q8_tile_tokens(dtype, head_size) % block_size == 0)
+
+
 class _QuantizedLaunch(_LayerLaunch):
     """``_LayerLaunch`` over an 8-bit cache: its plan also holds the step's slots
     and where the scales lie behind each pool's codes."""
@@ -468,8 +487,9 @@ class _QuantizedLaunch(_LayerLaunch):
     def __init__(self, plan: StepPlan, work, spec, dtype: int, block_size: int, workspace_ptr: int | None,
                  prefill_columns: int, sizes: tuple[int, int, int, int], scale_offset: int) -> None:
         super().__init__(plan, work, spec, dtype, block_size, workspace_ptr, prefill_columns, sizes)
+        appends = _decode_appends(work, dtype, spec.head_size, block_size)
         q = self.quantized_plan = native.AttentionPlanQ8(
-            base=self.plan, slots=plan.slots_ptr, num_tokens=plan.num_tokens, scale_offset=scale_offset)
+            base=self.plan, slots=None if appends else plan.slots_ptr, num_tokens=plan.num_tokens, scale_offset=scale_offset)
         self.plan_ptr = ctypes.addressof(q)
 
 

@@ -67,14 +67,18 @@ extern "C" int lvamd_paged_attention_q8(const lvamd_attention_plan_q8* plan,
   float* const key_scales = reinterpret_cast<float*>(static_cast<char*>(key_pool) + plan->scale_offset);
   float* const value_scales = reinterpret_cast<float*>(static_cast<char*>(value_pool) + plan->scale_offset);
   int status = LVAMD_OK;
-  if (new_key) {
+  const bool fused = new_key && !plan->slots;
+  if (fused && p.num_units > 0) return LVAMD_ERR_INVALID_ARGUMENT;
+  if (new_key && !fused) {
     status = lvamd_kv_append_q8(new_key, new_key_token_stride, new_key_head_stride, new_value, new_value_token_stride,
                                 new_value_head_stride, key_pool, key_scales, value_pool, value_scales, plan->slots,
                                 nullptr, plan->num_tokens, p.num_kv_heads, p.head_size, p.block_size, p.dtype, stream);
     if (status != LVAMD_OK) return status;
   }
   if (p.waves_per_head > 0) {
-    status = lvamd_paged_decode_q8(q, q_token_stride, q_head_stride, key_pool, key_scales, value_pool, value_scales, out,
+    status = lvamd_paged_decode_q8(q, q_token_stride, q_head_stride, fused ? new_key : nullptr, new_key_token_stride,
+                                   new_key_head_stride, fused ? new_value : nullptr, new_value_token_stride,
+                                   new_value_head_stride, key_pool, key_scales, value_pool, value_scales, out,
                                    out_token_stride, out_head_stride, p.pieces, p.wave_first, p.waves_per_head,
                                    p.tables, p.vis, p.part_acc, p.part_ml, p.num_partial_slots, p.num_kv_heads, p.group,
                                    p.head_size, p.block_size, scale, p.dtype, stream);

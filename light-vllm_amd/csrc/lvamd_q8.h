@@ -67,6 +67,37 @@ __device__ __forceinline__ uint2 q8_values4(uint32_t w, float scale) {
                       bitcast<uint32_t>((f16x2)__builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, scale, true)));
   }
 }
+// Sixteen elements (two 16-byte chunks of T): the largest finite magnitude, as
+// its fp32 bits (which order as the magnitudes do), and their codes.
+template <typename T>
+__device__ __forceinline__ uint32_t q8_largest16(uint4 lo, uint4 hi) {
+  T e[16];
+  __builtin_memcpy(e, &lo, 16);
+  __builtin_memcpy(e + 8, &hi, 16);
+  float m = 0.f;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const float f = __builtin_fabsf(to_f32(e[i]));
+    m = fmaxf(m, f < INFINITY ? f : 0.f);  // (NaN compares false)
+  }
+  return __float_as_uint(m);
+}
+template <typename T>
+__device__ __forceinline__ uint4 q8_codes16(uint4 lo, uint4 hi, float scale) {
+  T e[16];
+  __builtin_memcpy(e, &lo, 16);
+  __builtin_memcpy(e + 8, &hi, 16);
+  const float inverse = q8_inverse(scale);
+  float f[16];
+#pragma unroll
+  for (int i = 0; i < 16; ++i) f[i] = q8_scaled<T>(to_f32(e[i]), inverse);
+  return make_uint4(q8_pack4(f[0], f[1], f[2], f[3]), q8_pack4(f[4], f[5], f[6], f[7]),
+                    q8_pack4(f[8], f[9], f[10], f[11]), q8_pack4(f[12], f[13], f[14], f[15]));
+}
+// Sixteen codes times ratio, as q8_rescale4.
+__device__ __forceinline__ uint4 q8_rescale16(uint4 c, float ratio) {
+  return make_uint4(q8_rescale4(c.x, ratio), q8_rescale4(c.y, ratio), q8_rescale4(c.z, ratio), q8_rescale4(c.w, ratio));
+}
 // Sixteen codes times scale as two 16-byte chunks of T.
 template <typename T>
 __device__ __forceinline__ void q8_values16(uint4 codes, float scale, uint4& lo, uint4& hi) {
@@ -82,10 +113,21 @@ __device__ __forceinline__ uint32_t q8_nan4(uint32_t w) { return ((w & 0x7f7f7f7
 __device__ __forceinline__ bool q8_has_nan(uint4 c) {
   return (q8_nan4(c.x) | q8_nan4(c.y) | q8_nan4(c.z) | q8_nan4(c.w)) != 0;
 }
+// The same mask for four elements of T that are about to be stored: NaN codes
+// are what its values that are not finite become.
+template <typename T>
+__device__ __forceinline__ uint32_t q8_nan4_of(uint2 x) {
+  constexpr uint32_t e = std::is_same<T, __bf16>::value ? 0x7f80u : 0x7c00u;
+  auto bit = [&](uint32_t w, int from, int to) { return ((w >> from) & e) == e ? 0x80u << to : 0u; };
+  return bit(x.x, 0, 0) | bit(x.x, 16, 8) | bit(x.y, 0, 16) | bit(x.y, 16, 24);
+}
 // The codes with every NaN replaced by zero.
 __device__ __forceinline__ uint32_t q8_without_nan4(uint32_t w) {
   const uint32_t n = q8_nan4(w) >> 7;  // 1 per NaN byte
   return w & ~(n * 255u);
+}
+__device__ __forceinline__ uint4 q8_without_nan16(uint4 c) {
+  return make_uint4(q8_without_nan4(c.x), q8_without_nan4(c.y), q8_without_nan4(c.z), q8_without_nan4(c.w));
 }
 
 // Row stride, in 16-byte chunks, of a tile of dequantised rows of `chunks`

@@ -2,10 +2,10 @@
 // queries x group fit one 16-column MFMA tile (single tokens, short trees).
 //
 // Semantics are the 16-bit decode kernel's (lvamd_decode.hip) with K and V the
-// cache's values, code * scale; the step's tokens are in the cache already
-// (lvamd_kv_append_q8 runs first).  The work lists are the same too: stream-K
-// pieces over the (request) segments, one wave64 per share, split segments
-// merged by lvamd_paged_attention_merge.
+// cache's values, code * scale.  The step's tokens are in the cache already
+// (lvamd_kv_append_q8 ran), or the kernel appends them.  The work lists are the
+// same too: stream-K pieces over the (request) segments, one wave64 per share,
+// split segments merged by lvamd_paged_attention_merge_q8.
 //
 // Mapping onto CDNA4:
 //   * A tile is TT tokens of one kv head, 16 KiB of K and V codes (TT = 64 at
@@ -23,6 +23,13 @@
 //     of the codes); the lanes that load or convert a row fetch them by shuffles.
 //   * S^T = K Q^T and O^T = V^T P^T on MFMA 16x16x32, the online softmax in the
 //     log2 domain with lazy rescaling: as in the 16-bit kernel.
+//   * Append: with block sizes that divide the tile, each block that the step
+//     writes lies in one tile, and a kv head's tile belongs to one wave: that
+//     wave quantises the new rows, re-scales the block's others if its scale
+//     grows and stores what changed, after it staged the tile (append_rows; one
+//     tile per request and kv head).  It saves the append's launch, 3 us of
+//     the 12 that a step of short sequences takes per layer, and costs more
+//     than that in long ones: an instance of its own (APPEND).
 //   * A row that some column does not see may hold NaN (a sibling's draft),
 //     which a zero probability would not hide: rows of this step go to LDS
 //     with NaN as zero, and the columns that do see such a row get it back
@@ -41,10 +48,13 @@ constexpr float kSlack = 8.0f;  // lazy-rescale threshold, log2 units
 struct Q8DecodeArgs {
   const void* q;
   int64_t q_tok_stride, q_head_stride;
-  const uint8_t* k_pool;
-  const uint8_t* v_pool;
-  const float* k_scales;
-  const float* v_scales;
+  const void* k_new;  // this step's K/V [tokens][kv heads][D], or null: nothing to append
+  const void* v_new;
+  int64_t kn_tok_stride, kn_head_stride, vn_tok_stride, vn_head_stride;
+  uint8_t* k_pool;
+  uint8_t* v_pool;
+  float* k_scales;
+  float* v_scales;
   void* out;
   int64_t out_tok_stride, out_head_stride;
   const int32_t* __restrict__ tables;
@@ -82,7 +92,7 @@ __device__ __forceinline__ Q8Piece read_q8_piece(const int32_t* __restrict__ pie
 
 }  // namespace
 
-template <typename T, int D>
+template <typename T, int D, bool APPEND>
 __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(1, 1))) void q8_decode_kernel(const int32_t* __restrict__ wave_first,
                                                        const int32_t* __restrict__ pieces, const int32_t waves_per_head,
                                                        const uint32_t wg_magic, const int32_t wg_shift,
@@ -105,15 +115,15 @@ __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(1, 1))) void
   const int p_end = wave_first[w + 1];
   if (p >= p_end) return;
   const int64_t row_bytes = (int64_t)Hkv * D;
-  gptr<const uint8_t> const kbase = (gptr<const uint8_t>)(a.k_pool) + (int64_t)kvh * D;
-  gptr<const uint8_t> const vbase = (gptr<const uint8_t>)(a.v_pool) + (int64_t)kvh * D;
-  gptr<const float> const kscales = (gptr<const float>)(a.k_scales) + kvh;
-  gptr<const float> const vscales = (gptr<const float>)(a.v_scales) + kvh;
+  gptr<uint8_t> const kbase = (gptr<uint8_t>)(a.k_pool) + (int64_t)kvh * D;
+  gptr<uint8_t> const vbase = (gptr<uint8_t>)(a.v_pool) + (int64_t)kvh * D;
+  gptr<float> const kscales = (gptr<float>)(a.k_scales) + kvh;
+  gptr<float> const vscales = (gptr<float>)(a.v_scales) + kvh;
 
   // This lane's rows of a tile: their blocks and offsets in them.  (The slot is
   // made of them where the codes are requested: here it would wait for the
   // table's load, and with it for the tile's loads before it.)  Rows past the
-  // piece repeat its last one (masked).
+  // piece repeat its last one.
   struct Rows {
     int block[SPL], off[SPL];
   };
@@ -160,26 +170,31 @@ __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(1, 1))) void
       const int64_t off = (int64_t)shuffled(slot, row & (TT - 1)) * row_bytes + 16 * c;
       t.k[j] = t.v[j] = zero_u4();
       if (64 * LPT == TT * C8 || row < TT) {
-        t.k[j] = load16_stream(kbase + off);
-        t.v[j] = load16_stream(vbase + off);
+        t.k[j] = load16_stream((gptr<const uint8_t>)(kbase + off));
+        t.v[j] = load16_stream((gptr<const uint8_t>)(vbase + off));
       }
     }
   };
-  // Tile into LDS as T.  Rows from first_new on hold this step's tokens: their
-  // NaN values are left out (returns whether there were any).
+  // Tile into LDS as T.  NEW: rows from first_new on hold this step's tokens, or
+  // are past the end.  Their V rows' NaN values are left out (returns whether
+  // there were any); zeros, where this launch has yet to write them.
   auto stage_rows = [&]<bool NEW>(const Tile& t, int first_new) __attribute__((always_inline)) -> bool {
     bool any = false;
 #pragma unroll
     for (int j = 0; j < LPT; ++j) {
       const int id = lane + 64 * j;
       const int row = id / C8, c = id - row * C8;
-      const float ks = shuffled(t.ks, row & (TT - 1)), vs = shuffled(t.vs, row & (TT - 1));
+      const float ks = shuffled(t.ks, row & (TT - 1));
+      float vs = shuffled(t.vs, row & (TT - 1));
       uint4 v = t.v[j];
       if constexpr (NEW) {
+        if (APPEND && row >= first_new) {
+          v = zero_u4();
+          vs = 0.f;
+        }
         const bool nan = row >= first_new && q8_has_nan(v);
         any |= nan;
-        v = make_uint4(nan ? q8_without_nan4(v.x) : v.x, nan ? q8_without_nan4(v.y) : v.y,
-                       nan ? q8_without_nan4(v.z) : v.z, nan ? q8_without_nan4(v.w) : v.w);
+        if (nan) v = q8_without_nan16(v);
       }
       uint4 klo, khi, vlo, vhi;
       q8_values16<T>(t.k[j], ks, klo, khi);
@@ -193,9 +208,108 @@ __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(1, 1))) void
     }
     return NEW && __any(any);
   };
-  auto stage = [&](const Tile& t, int first_new) -> bool {
-    if (first_new >= TT) return stage_rows.template operator()<false>(t, first_new);
-    return stage_rows.template operator()<true>(t, first_new);
+  // 16 elements of a new token's K and V row.
+  struct Raw {
+    uint4 k0, k1, v0, v1;
+  };
+  auto load_new = [&](int tok, int c) -> Raw {
+    gptr<const T> const k = (gptr<const T>)(a.k_new) + (int64_t)tok * a.kn_tok_stride + kvh * a.kn_head_stride + 16 * c;
+    gptr<const T> const v = (gptr<const T>)(a.v_new) + (int64_t)tok * a.vn_tok_stride + kvh * a.vn_head_stride + 16 * c;
+    return {load16(k), load16(k + 8), load16(v), load16(v + 8)};
+  };
+  // The piece's new rows of the tile at t0 (at most 16: a piece has no more
+  // queries), after the tile was staged without them: into the cache, and into
+  // LDS as they are stored.  Loops, not unrolled: a launch pays for code that it
+  // fetches, and waves that append do it once or twice.
+  auto append_rows = [&](const Tile& t, const Rows& rows, const Q8Piece& x, int t0)
+      __attribute__((always_inline)) -> bool {
+    const int row0 = max(x.computed - t0, 0), end = min(x.tok_end - t0, TT);
+    const int n = end - row0;
+    const int tok0 = x.q_start + t0 - x.computed;  // row r is token tok0 + r
+    const int block0 = fast_div(row0, a.by_block), begin0 = block0 * a.block_size;
+    const int blocks = fast_div(end - 1, a.by_block) - block0 + 1;
+    const Raw raw = load_new(tok0 + row0 + min(lane, n * C8 - 1) / C8, min(lane, n * C8 - 1) % C8);
+    // Lane b < blocks is at block block0 + b.  Only the first may hold earlier rows.
+    const bool first = lane == 0 && begin0 < x.computed - t0;
+    const int from = min((block0 + lane) * a.block_size, end - 1);
+    const int block = shuffled(rows.block, from);
+    const int64_t at = (int64_t)block * Hkv;
+    const float kheld = shuffled(t.ks, from), vheld = shuffled(t.vs, from);
+    const float kold = first ? kheld : 0.f, vold = first ? vheld : 0.f;
+    // Each block's largest magnitudes, in the first new rows' place.
+    static_assert(D >= 32, "16 words in a row");
+    uint32_t* const kmax = reinterpret_cast<uint32_t*>(klds + row0 * RS);
+    uint32_t* const vmax = reinterpret_cast<uint32_t*>(vlds + row0 * RS);
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    if (lane < 16) kmax[lane] = vmax[lane] = 0u;
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    // (All lanes take part in each pass, the last chunk's again past the end: the
+    // shuffles read any of them.)
+    Raw e = raw;
+#pragma unroll 1
+    for (int i = 0;;) {
+      const int row = row0 + min(i + lane, n * C8 - 1) / C8;
+      const int b = fast_div(row, a.by_block) - block0;
+      atomicMax(kmax + b, q8_largest16<T>(e.k0, e.k1));
+      atomicMax(vmax + b, q8_largest16<T>(e.v0, e.v1));
+      if ((i += 64) >= n * C8) break;
+      const int id = min(i + lane, n * C8 - 1);
+      e = load_new(tok0 + row0 + id / C8, id % C8);
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    const float kscale = fmaxf(kold, q8_scale(__uint_as_float(kmax[lane & 15])));
+    const float vscale = fmaxf(vold, q8_scale(__uint_as_float(vmax[lane & 15])));
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    if (lane < blocks) {
+      kscales[at] = kscale;
+      vscales[at] = vscale;
+    }
+    bool nan = false;
+    e = raw;
+#pragma unroll 1
+    for (int i = 0;;) {
+      const int id = min(i + lane, n * C8 - 1);
+      const int row = row0 + id / C8, c = id % C8;
+      const int lb = fast_div(row, a.by_block), b = lb - block0;
+      const float ks = __shfl(kscale, b), vs = __shfl(vscale, b);
+      const int64_t off = ((int64_t)__shfl(block, b) * a.block_size + (row - lb * a.block_size)) * row_bytes + 16 * c;
+      const uint4 kc = q8_codes16<T>(e.k0, e.k1, ks);
+      uint4 vc = q8_codes16<T>(e.v0, e.v1, vs);
+      store16(kbase + off, kc);
+      store16(vbase + off, vc);
+      nan |= q8_has_nan(vc);
+      vc = q8_without_nan16(vc);
+      uint4* const kto = klds + row * RS + 2 * c;
+      uint4* const vto = vlds + row * RS + 2 * c;
+      q8_values16<T>(kc, ks, kto[0], kto[1]);
+      q8_values16<T>(vc, vs, vto[0], vto[1]);
+      if ((i += 64) >= n * C8) break;
+      const int next = min(i + lane, n * C8 - 1);
+      e = load_new(tok0 + row0 + next / C8, next % C8);
+    }
+    // The first block's other rows, where its scale grew.
+    if (__any(first && (kscale > kold || vscale > vold))) {
+      const float ks = __shfl(kscale, 0), vs = __shfl(vscale, 0);
+      const float kratio = __shfl(kold, 0) * q8_inverse(ks), vratio = __shfl(vold, 0) * q8_inverse(vs);
+      const int64_t slot0 = (int64_t)__shfl(block, 0) * a.block_size;
+#pragma unroll 1
+      for (int id = lane; id < a.block_size * C8; id += 64) {
+        const int r = id / C8, c = id % C8;
+        const int row = begin0 + r;
+        if (row >= row0 && row < end) continue;
+        const int64_t off = (slot0 + r) * row_bytes + 16 * c;
+        const uint4 kc = q8_rescale16(load16((gptr<const uint8_t>)(kbase + off)), kratio);
+        const uint4 vc = q8_rescale16(load16((gptr<const uint8_t>)(vbase + off)), vratio);
+        if (kratio < 1.f) store16(kbase + off, kc);
+        if (vratio < 1.f) store16(vbase + off, vc);
+        if (row >= row0) continue;  // (past the tokens: stale)
+        uint4* const kto = klds + row * RS + 2 * c;
+        uint4* const vto = vlds + row * RS + 2 * c;
+        q8_values16<T>(kc, ks, kto[0], kto[1]);
+        q8_values16<T>(vc, vs, vto[0], vto[1]);
+      }
+    }
+    return __any(nan);
   };
 
   // This lane's column: query qi, head qhead, and which of the step's tokens
@@ -245,6 +359,7 @@ __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(1, 1))) void
   Rows rows = lookup(at.table_off, at.t0, at.tok_end);
   Tile tile;
   issue(rows, tile);
+  Rows staged = rows;
   Column col = column(cur);
   uint4 qf[NCH];
   load_q(cur, col, qf);
@@ -261,7 +376,13 @@ __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(1, 1))) void
   Column ncol = col;
   uint4 qn[NCH];
   while (true) {
-    const bool poisoned = stage(tile, cur.computed - t0);
+    bool poisoned = false;
+    if (const int first_new = cur.computed - t0; first_new >= TT) {
+      stage_rows.template operator()<false>(tile, first_new);
+    } else {
+      poisoned = stage_rows.template operator()<true>(tile, first_new);
+      if constexpr (APPEND) poisoned = append_rows(tile, staged, cur, t0);
+    }
     // The next tile's codes, the rows of the one after it and, where the next
     // tile starts a piece, that piece's record and queries.
     const bool has_next = at.p < p_end;
@@ -269,6 +390,7 @@ __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(1, 1))) void
     const int nt0 = at.t0;
     if (has_next) {
       issue(rows, tile);
+      staged = rows;
       if (ends) {
         p = at.p;
         nxt = read_q8_piece(pieces, p);
@@ -358,7 +480,10 @@ __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(1, 1))) void
         const bool sees = (col.sees >> ((pos - cur.computed) & 31)) & 1u;
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-          const uint32_t nan = q8_nan4(*(gptr<const uint32_t>)(vbase + slot * row_bytes + 16 * n + 4 * g));
+          const uint32_t nan =
+              APPEND ? q8_nan4_of<T>(*(const uint2*)((const T*)a.v_new + (int64_t)(cur.q_start + pos - cur.computed) * a.vn_tok_stride +
+                                                      kvh * a.vn_head_stride + 16 * n + 4 * g))
+                     : q8_nan4(*(gptr<const uint32_t>)(vbase + slot * row_bytes + 16 * n + 4 * g));
 #pragma unroll
           for (int r = 0; r < 4; ++r)
             if (sees && ((nan >> (8 * r + 7)) & 1u)) acc[n][r] = __uint_as_float(0x7fc00000u);
@@ -440,11 +565,12 @@ static int q8_dispatch(int dtype, int head_size, F f) {
 
 using namespace lvamd;
 
-extern "C" int lvamd_paged_decode_q8(const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* key_pool,
-                                     const float* key_scales, const void* value_pool, const float* value_scales,
-                                     void* out, int64_t out_token_stride, int64_t out_head_stride,
-                                     const int32_t* pieces, const int32_t* wave_first, int32_t waves_per_head,
-                                     const int32_t* tables, const uint32_t* vis, void* part_acc, float* part_ml,
+extern "C" int lvamd_paged_decode_q8(const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* new_key,
+                                     int64_t new_key_token_stride, int64_t new_key_head_stride, const void* new_value,
+                                     int64_t new_value_token_stride, int64_t new_value_head_stride, void* key_pool,
+                                     float* key_scales, void* value_pool, float* value_scales, void* out,
+                                     int64_t out_token_stride, int64_t out_head_stride, const int32_t* pieces, const int32_t* wave_first,
+                                     int32_t waves_per_head, const int32_t* tables, const uint32_t* vis, void* part_acc, float* part_ml,
                                      int64_t num_partial_slots, int32_t num_kv_heads, int32_t group, int32_t head_size,
                                      int32_t block_size, float scale, int32_t dtype, lvamd_stream_t stream) {
   if ((dtype != LVAMD_BF16 && dtype != LVAMD_F16) || !q8_head_size(head_size)) return LVAMD_ERR_UNSUPPORTED;
@@ -457,13 +583,25 @@ extern "C" int lvamd_paged_decode_q8(const void* q, int64_t q_token_stride, int6
   if (!aligned16(q) || !aligned16(key_pool) || !aligned16(value_pool) || q_token_stride % 8 != 0 ||
       q_head_stride % 8 != 0 || ((uintptr_t)out & 7u) != 0 || out_token_stride % 4 != 0 || out_head_stride % 4 != 0)
     return LVAMD_ERR_INVALID_ARGUMENT;
+  if ((new_key == nullptr) != (new_value == nullptr)) return LVAMD_ERR_INVALID_ARGUMENT;
+  // Appending needs whole blocks per tile.
+  if (new_key && (!aligned16(new_key) || !aligned16(new_value) || new_key_token_stride % 8 != 0 ||
+                  new_key_head_stride % 8 != 0 || new_value_token_stride % 8 != 0 || new_value_head_stride % 8 != 0 ||
+                  lvamd_paged_decode_q8_tile_tokens(dtype, head_size) % block_size != 0))
+    return LVAMD_ERR_INVALID_ARGUMENT;
   if ((int64_t)waves_per_head * num_kv_heads > 0x7fffffffLL) return LVAMD_ERR_INVALID_ARGUMENT;
   Q8DecodeArgs a{.by_block = FastDiv(block_size), .by_group = FastDiv(group)};
   a.q = q;
   a.q_tok_stride = q_token_stride;
   a.q_head_stride = q_head_stride;
-  a.k_pool = static_cast<const uint8_t*>(key_pool);
-  a.v_pool = static_cast<const uint8_t*>(value_pool);
+  a.k_new = new_key;
+  a.v_new = new_value;
+  a.kn_tok_stride = new_key_token_stride;
+  a.kn_head_stride = new_key_head_stride;
+  a.vn_tok_stride = new_value_token_stride;
+  a.vn_head_stride = new_value_head_stride;
+  a.k_pool = static_cast<uint8_t*>(key_pool);
+  a.v_pool = static_cast<uint8_t*>(value_pool);
   a.k_scales = key_scales;
   a.v_scales = value_scales;
   a.out = out;
@@ -481,8 +619,8 @@ extern "C" int lvamd_paged_decode_q8(const void* q, int64_t q_token_stride, int6
   const FastDiv by_waves(waves_per_head);
   hipStream_t s = static_cast<hipStream_t>(stream);
   return q8_dispatch(dtype, head_size, [&]<typename T, int D>() -> int {
-    hipLaunchKernelGGL((q8_decode_kernel<T, D>), grid, dim3(64), 0, s, wave_first, pieces, waves_per_head,
-                       by_waves.magic, by_waves.shift, a);
+    hipLaunchKernelGGL((new_key ? q8_decode_kernel<T, D, true> : q8_decode_kernel<T, D, false>), grid, dim3(64), 0, s,
+                       wave_first, pieces, waves_per_head, by_waves.magic, by_waves.shift, a);
     return launch_status();
   });
 }
@@ -498,7 +636,7 @@ extern "C" int lvamd_paged_decode_q8_resident_waves(int32_t dtype, int32_t head_
     if (hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, device) != hipSuccess)
       return LVAMD_ERR_LAUNCH;
     if (hipOccupancyMaxActiveBlocksPerMultiprocessor(
-            &per_cu, reinterpret_cast<const void*>(&q8_decode_kernel<T, D>), 64, 0) != hipSuccess)
+            &per_cu, reinterpret_cast<const void*>(&q8_decode_kernel<T, D, false>), 64, 0) != hipSuccess)
       return LVAMD_ERR_LAUNCH;
     return per_cu * cus;
   });

@@ -110,8 +110,8 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     ),
     "lvamd_paged_decode_q8": (
         ctypes.c_int,
-        [_p, _i64, _i64, _p, _p, _p, _p, _p, _i64, _i64, _p, _p, _i32, _p, _p, _p, _p, _i64,
-         _i32, _i32, _i32, _i32, _f32, _i32, _p],
+        [_p, _i64, _i64, _p, _i64, _i64, _p, _i64, _i64, _p, _p, _p, _p, _p, _i64, _i64,
+         _p, _p, _i32, _p, _p, _p, _p, _i64, _i32, _i32, _i32, _i32, _f32, _i32, _p],
     ),
     "lvamd_paged_decode_q8_tile_tokens": (ctypes.c_int, [_i32, _i32]),
     "lvamd_paged_decode_q8_resident_waves": (ctypes.c_int, [_i32, _i32]),

@@ -272,6 +272,50 @@ def test_attention_matches_the_oracle(hq, hkv, d, bs, computed, layouts, dtype) 
     _attend_and_check(*_step(hq, hkv, d, bs, DTYPES[dtype], computed, layouts, seed=d + bs + len(computed)), DTYPES[dtype])
 
 
+@pytest.mark.parametrize("dtype", ("bf16", "fp16"))
+@pytest.mark.parametrize("hq,hkv,d,bs,computed,layouts", [
+    (8, 2, 128, 16, [0, 1, 15, 16, 47, 63, 64, 700], [1, 2, 3, 4, 1, 4, 4, 1]),
+    (4, 4, 64, 32, [0, 5, 31, 120, 127, 128, 1000], [16, 16, 9, 16, 16, 1, 1]),     # runs over a block's and a tile's end
+    (4, 4, 32, 1, [3, 127, 200], [16, 7, 1]),                                         # sixteen blocks of one token
+    (6, 2, 80, 64, [10, 60, 130], [(-1, 0, 0), 5, 1]),
+    (4, 2, 256, 4, [30, 29, 700], [8, 1, 3]),
+    (3, 3, 112, 8, [50, 100], [(-1, 0, 0, 1, 1, 2, 3, 0, 7), 12]),
+    (2, 2, 64, 128, [100, 200], [16, 1]),
+])
+def test_append_inside_the_decode_launch(monkeypatch, hq, hkv, d, bs, computed, layouts, dtype) -> None:
+    """The same codes, scales and rows, bit for bit, as with a launch for the
+    append, for tokens that raise their block's scale by 2^-1 .. 2^12 or not at all."""
+    print(f"[gpu] q8 decode appends {hq}/{hkv}x{d} bs {bs} {dtype}", file=sys.stderr, flush=True)
+    t = DTYPES[dtype]
+    cache, metadata, q, k, v = _step(hq, hkv, d, bs, t, computed, layouts, seed=d + bs)
+    gen = torch.Generator(device=DEV).manual_seed(d)
+    k, v = (x * torch.exp2(torch.randint(-8, 5, (x.shape[0], hkv, 1), generator=gen, device=DEV).float()).to(t) for x in (k, v))
+    q = q / 16  # (keys of up to 2^4 times the usual: the scores' bound holds)
+    layer = cache.layer("layer0")
+    parts = (layer.keys.view(torch.uint8), layer.key_scales, layer.values.view(torch.uint8), layer.value_scales)
+    before = [p.clone() for p in parts]
+    found = []
+    for units in (1 << 20, 0):
+        for p, b in zip(parts, before):
+            p.copy_(b)
+        monkeypatch.setattr(sys.modules["light_vllm_amd.backend"], "_APPEND_UNITS", units)
+        found.append([_attend_and_check(cache, metadata, q, k, v, t).view(torch.int16).clone()] + [p.clone() for p in parts])
+    for a, b in zip(*found):
+        assert torch.equal(a, b)
+    # NaN and infinities among the tokens: the same once more.
+    k[0, 0, 1], v[-1, 0, 2], v[0, -1, 3], v[0, -1, 4] = math.nan, math.nan, math.inf, -math.inf
+    found = []
+    for units in (1 << 20, 0):
+        for p, b in zip(parts, before):
+            p.copy_(b)
+        monkeypatch.setattr(sys.modules["light_vllm_amd.backend"], "_APPEND_UNITS", units)
+        out = lv.HipPagedAttentionBackend().create(cache, metadata).forward("layer0", q, k, v, scale=1 / math.sqrt(d))
+        found.append([torch.nan_to_num(out, nan=-7.0)] + [p.clone() for p in parts])
+    assert bool((found[0][0] == -7.0).any())
+    for a, b in zip(*found):
+        assert torch.equal(a, b)
+
+
 @pytest.mark.parametrize("d", range(32, 257, 16))
 def test_every_head_size(d) -> None:
     print(f"[gpu] q8 attention head size {d}", file=sys.stderr, flush=True)

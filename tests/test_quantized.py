@@ -122,21 +122,28 @@ def test_attention_entry_point_checks() -> None:
     lib = native.load()
     f = ctypes.c_float(0.1)
 
-    def decode(q=X, waves=1, slots=0, heads=4, group=7, d=128, bs=16, dtype=2, qs=(3584, 128), part=None):
-        return lib.lvamd_paged_decode_q8(q, *qs, X, X, X, X, X, 3584, 128, X, X, waves, X, X, part, part, slots, heads, group, d,
-                                         bs, f, dtype, None)
+    none = (None, 0, 0, None, 0, 0)
+    new = (X, 512, 128, X, 512, 128)
+
+    def decode(q=X, waves=1, slots=0, heads=4, group=7, d=128, bs=16, dtype=2, qs=(3584, 128), part=None, kv=none):
+        return lib.lvamd_paged_decode_q8(q, *qs, *kv, X, X, X, X, X, 3584, 128, X, X, waves, X, X, part, part, slots, heads,
+                                         group, d, bs, f, dtype, None)
 
     def prefill(q=X, units=1, slots=0, heads=4, group=7, d=128, bs=16, dtype=2, qs=(3584, 128), part=None, columns=128):
         return lib.lvamd_paged_prefill_q8(q, *qs, X, X, X, X, X, 3584, 128, X, X, X, units, part, part, slots, heads, group, d,
                                           columns, bs, f, dtype, None)
 
-    for call, none in ((decode, "waves"), (prefill, "units")):
-        assert call(**{none: 0}) == 0
+    for call, count in ((decode, "waves"), (prefill, "units")):
+        assert call(**{count: 0}) == 0
         assert call(dtype=0) == -2 and call(d=24) == -2 and call(d=264) == -2
-        for bad in (dict(q=None), dict(heads=0), dict(group=0), dict(bs=0), dict(qs=(3580, 128)), {none: -1}):
+        for bad in (dict(q=None), dict(heads=0), dict(group=0), dict(bs=0), dict(qs=(3580, 128)), {count: -1}):
             assert call(**bad) == -1, bad
         assert call(slots=3) == -3
     assert decode(group=17) == -1
+    # The decode launch's append: both tensors, aligned rows, whole blocks per tile.
+    for kv in ((X, 512, 128, None, 512, 128), (X, 508, 128, X, 512, 128), (ctypes.c_void_p(8), 512, 128, X, 512, 128)):
+        assert decode(kv=kv) == -1, kv
+    assert decode(kv=new, bs=12) == -1 and decode(kv=new, bs=128) == -1
     assert prefill(columns=32) == -2 and prefill(columns=256) == -2 and prefill(columns=64, q=None) == -1
     merge = lambda dtype, jobs, cols=1: lib.lvamd_paged_attention_merge_q8(X, X, X, 0, 0, X, jobs, 4, 7, 128, cols, 16, dtype, None)  # noqa: E731
     assert merge(2, 0) == 0 and merge(0, 1) == -2 and merge(2, -1) == -1 and merge(1, 1, 17) == -2
