@@ -61,7 +61,7 @@ struct VerifyArgs {
   const void* sample_uniforms;
   double2* sums;            // [requests][chunks]: the residual's sum, p's sum
   Stop* stops;              // [requests]
-  int64_t* children;        // [drafts]: the last node's children's tokens, from the request's first draft on
+  int32_t* children;        // [drafts]: the last node's children's tokens, from the request's first draft on
   int32_t* counts;
   int32_t* paths;
   int64_t* out_tokens;
@@ -69,8 +69,8 @@ struct VerifyArgs {
   int32_t uniforms_f64;
 };
 
-// (Finite and positive: else zero.)
-__device__ __forceinline__ float mass(float p) { return p > 0.f && p < INFINITY ? p : 0.f; }
+// (Finite and positive: else zero.  Class bits: positive subnormal or normal.)
+__device__ __forceinline__ float mass(float p) { return __builtin_amdgcn_classf(p, 0x180) ? p : 0.f; }
 
 __device__ __forceinline__ double uniform_at(const void* u, int64_t i, int f64) {
   return f64 ? static_cast<const double*>(u)[i] : (double)static_cast<const float*>(u)[i];
@@ -111,7 +111,8 @@ template <typename T>
 __device__ __forceinline__ void masses(const Pack<T>& v, int i, int end, float (&x)[Wide<T>::N]) {
   const int at = pack_at<T>(i, end);
 #pragma unroll
-  for (int k = 0; k < Wide<T>::N; ++k) x[k] = at + k >= i && at + k < end ? mass(to_f32((T)v.e[k])) : 0.f;
+  for (int k = 0; k < Wide<T>::N; ++k)
+    x[k] = at + k >= i && at + k < end ? mass(to_f32((T)v.e[k])) : 0.f;
 }
 
 // A lane's packs of a chunk, pack j from element first + j * step on.
@@ -131,10 +132,10 @@ __device__ __forceinline__ void load_packs(Packs<T>& x, const T* row, int first,
 // The children's tokens that lie in the chunk from `begin` on taken out; whether
 // there are any.
 template <typename T>
-__device__ __forceinline__ bool take_out(Packs<T>& x, const int64_t* kids, int nkids, int begin, int end) {
+__device__ __forceinline__ bool take_out(Packs<T>& x, const int32_t* kids, int nkids, int begin, int end) {
   bool any = false;
   for (int c = 0; c < nkids; ++c) {
-    const int64_t kid = kids[c];
+    const int kid = kids[c];
     if (kid < begin || kid >= begin + Wide<T>::CHUNK) continue;  // (uniform)
     any = true;
 #pragma unroll
@@ -169,121 +170,7 @@ __device__ __forceinline__ double wave_sum(double v) {
   return v;
 }
 
-}  // namespace
-
-// Grid: (workgroups per request, requests); a request's waves take its chunks
-// in turn.
-template <typename T, bool DRAWN>
-__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(4))) void verify_sums_kernel(
-    const VerifyArgs a) {
-  __shared__ float mp[kMaxDrafts], mq[kMaxDrafts];
-  __shared__ int next[kMaxDrafts + 1];
-  __shared__ int64_t kids[kMaxDrafts];
-  __shared__ int stop, num_kids, kid_draft;
-  const int req = blockIdx.y;
-  const int first = a.starts[req];
-  const int n = min(a.starts[req + 1] - first, kMaxDrafts);
-  const int64_t row0 = (int64_t)first + req;  // the root's row
-  const bool leader = blockIdx.x == 0;         // writes what is found
-  const T* target = static_cast<const T*>(a.target);
-  const T* drafts = static_cast<const T*>(a.draft_probs);
-  if (threadIdx.x == 0) {
-    stop = num_kids = 0;
-    kid_draft = -1;
-  }
-  if (n > 0) {
-    for (int c = threadIdx.x; c < n; c += kThreads) {
-      const int64_t tok = a.tokens[first + c];
-      const bool in = tok >= 0 && tok < a.vocab;
-      mp[c] = in ? mass(to_f32(target[(row0 + a.parents[first + c] + 1) * a.target_stride + tok])) : 0.f;
-      if constexpr (DRAWN) mq[c] = in ? mass(to_f32(drafts[(int64_t)(first + c) * a.draft_stride + tok])) : 0.f;
-    }
-    for (int c = threadIdx.x; c <= n; c += kThreads) next[c] = -1;
-    __syncthreads();
-    for (int c = threadIdx.x; c < n; c += kThreads) {
-      const int parent = a.parents[first + c] + 1;
-      const double u = uniform_at(a.node_uniforms, row0 + parent, a.uniforms_f64);
-      bool taken;
-      if constexpr (DRAWN) {
-        taken = u * (double)mq[c] < (double)mp[c];
-      } else {
-        double before = 0.0;
-        for (int s = a.siblings[first + c]; s >= 0; s = a.siblings[first + s]) before += (double)mp[s];
-        taken = u >= before && u < before + (double)mp[c];
-      }
-      if (taken) next[parent] = c + 1;
-    }
-    __syncthreads();
-  }
-  if (threadIdx.x == 0) {
-    int node = 0, count = 0;
-    if (n > 0)
-      for (int to = next[0]; to >= 0 && count < n; to = next[to]) {
-        node = to;
-        if (leader && count < a.path_width) a.paths[(int64_t)req * a.path_width + count] = node - 1;
-        ++count;
-      }
-    stop = node;
-    if (leader) {
-      a.counts[req] = count;
-      for (int i = count; i < a.path_width; ++i) a.paths[(int64_t)req * a.path_width + i] = -1;
-    }
-  }
-  __syncthreads();
-  const int node = stop;
-  if (n > 0) {
-    for (int c = threadIdx.x; c < n; c += kThreads)
-      if (a.parents[first + c] + 1 == node) {
-        kids[atomicAdd(&num_kids, 1)] = a.tokens[first + c];
-        kid_draft = first + c;  // (a chain has one)
-      }
-    __syncthreads();
-  }
-  const int nkids = num_kids;
-  const int draft = DRAWN ? kid_draft : -1;
-  if (leader) {
-    if (threadIdx.x == 0) a.stops[req] = {node, nkids, draft, 0};
-    for (int c = threadIdx.x; c < nkids; c += kThreads) a.children[first + c] = kids[c];
-  }
-  const T* prow = target + (row0 + node) * a.target_stride;
-  const T* qrow = DRAWN && draft >= 0 ? drafts + (int64_t)draft * a.draft_stride : nullptr;
-  constexpr int N = Wide<T>::N;
-  const int lane = threadIdx.x & 63;
-  const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-  for (int chunk = blockIdx.x * kWaves + wave; chunk < a.chunks; chunk += gridDim.x * kWaves) {
-    const int begin = chunk * Wide<T>::CHUNK;
-    Packs<T> p, q = {};
-    load_packs<T>(p, prow, begin + lane * N, 64 * N, a.vocab);
-    if constexpr (DRAWN) {
-      if (qrow) load_packs<T>(q, qrow, begin + lane * N, 64 * N, a.vocab);  // (else zeros: nothing to subtract)
-    }
-    double full = 0.0, rest = 0.0;
-    auto sum = [&]<bool LESS>() -> double {
-      double s = 0.0;
-#pragma unroll
-      for (int j = 0; j < kLoads; ++j) {
-        double r[N];
-        residual<T, LESS>(p, q, j, a.vocab, r);
-#pragma unroll
-        for (int k = 0; k < N; ++k) s += r[k];
-      }
-      return s;
-    };
-    full = rest = sum.template operator()<false>();
-    if constexpr (DRAWN) {
-      if (qrow) rest = sum.template operator()<true>();
-    } else {
-      if (take_out<T>(p, kids, nkids, begin, a.vocab)) rest = sum.template operator()<false>();
-    }
-    rest = wave_sum(rest);
-    full = wave_sum(full);
-    if (lane == 0) a.sums[(int64_t)req * a.chunks + chunk] = make_double2(rest, full);
-  }
-}
-
-namespace {
-
-// Inclusive sum over the wave's lanes.
+// Sum over the wave's lanes up to each.
 __device__ __forceinline__ double wave_scan(double v, int lane) {
 #pragma unroll
   for (int d = 1; d < 64; d <<= 1) {
@@ -293,18 +180,159 @@ __device__ __forceinline__ double wave_scan(double v, int lane) {
   return v;
 }
 
-}  // namespace
+template <bool DRAWN>
+struct WalkShared {
+  float p[kMaxDrafts], q[DRAWN ? kMaxDrafts : 1];  // the drafts' own probabilities
+  int16_t sibling[kMaxDrafts], next[kMaxDrafts + 1];
+  int32_t kids[kMaxDrafts];
+  int node, num_kids, kid_draft;
+};
 
-// Grid: requests, one wave each.
+// The request's last node, its children's tokens (s.kids) and its one draft
+// (chains drawn from q), found by a workgroup: two rounds of loads and a walk in
+// LDS.  `leader` writes the accepted path.
+template <typename T, bool DRAWN, int THREADS>
+__device__ __forceinline__ Stop walk(const VerifyArgs& a, int req, bool leader, WalkShared<DRAWN>& s) {
+  constexpr int PER = kMaxDrafts / THREADS;
+  const int first = a.starts[req];
+  const int n = min(a.starts[req + 1] - first, kMaxDrafts);
+  const int64_t row0 = (int64_t)first + req;  // the root's row
+  const T* target = static_cast<const T*>(a.target);
+  const T* drafts = static_cast<const T*>(a.draft_probs);
+  if (threadIdx.x == 0) {
+    s.node = s.num_kids = 0;
+    s.kid_draft = -1;
+  }
+  int parent[PER], token[PER];
+  double u[PER];
+  if (n > 0) {
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int c = threadIdx.x + THREADS * i;
+      if (c >= n) break;
+      const int64_t tok = a.tokens[first + c];
+      token[i] = tok >= 0 && tok < a.vocab ? (int)tok : -1;
+      parent[i] = a.parents[first + c] + 1;
+      s.sibling[c] = (int16_t)a.siblings[first + c];
+      s.next[c] = -1;
+    }
+    if (threadIdx.x == 0) s.next[n] = -1;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int c = threadIdx.x + THREADS * i;
+      if (c >= n) break;
+      const int64_t tok = max(token[i], 0);
+      const float p = to_f32(target[(row0 + parent[i]) * a.target_stride + tok]);
+      u[i] = uniform_at(a.node_uniforms, row0 + parent[i], a.uniforms_f64);
+      if constexpr (DRAWN) {
+        const float q = to_f32(drafts[(int64_t)(first + c) * a.draft_stride + tok]);
+        s.q[c] = token[i] >= 0 ? mass(q) : 0.f;
+      }
+      s.p[c] = token[i] >= 0 ? mass(p) : 0.f;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int c = threadIdx.x + THREADS * i;
+      if (c >= n) break;
+      bool taken;
+      if constexpr (DRAWN) {
+        taken = u[i] * (double)s.q[c] < (double)s.p[c];
+      } else {
+        double before = 0.0;
+        for (int k = s.sibling[c]; k >= 0; k = s.sibling[k]) before += (double)s.p[k];
+        taken = u[i] >= before && u[i] < before + (double)s.p[c];
+      }
+      if (taken) s.next[parent[i]] = (int16_t)(c + 1);
+    }
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) {
+    int node = 0, count = 0;
+    if (n > 0)
+      for (int to = s.next[0]; to >= 0 && count < n; to = s.next[to]) {
+        node = to;
+        if (leader && count < a.path_width) a.paths[(int64_t)req * a.path_width + count] = node - 1;
+        ++count;
+      }
+    s.node = node;
+    if (leader) {
+      a.counts[req] = count;
+      for (int i = count; i < a.path_width; ++i) a.paths[(int64_t)req * a.path_width + i] = -1;
+    }
+  }
+  __syncthreads();
+  const int node = s.node;
+  if (n > 0) {
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int c = threadIdx.x + THREADS * i;
+      if (c >= n) break;
+      if (parent[i] == node) {
+        s.kids[atomicAdd(&s.num_kids, 1)] = token[i];
+        s.kid_draft = first + c;  // (a chain has one)
+      }
+    }
+    __syncthreads();
+  }
+  return {node, s.num_kids, DRAWN ? s.kid_draft : -1, 0};
+}
+
+// The rows at the request's last node: p, and what is subtracted from it (null:
+// nothing).
+template <typename T>
+struct Rows {
+  const T *p, *q;
+};
 template <typename T, bool DRAWN>
-__global__ __launch_bounds__(64) void verify_draw_kernel(const VerifyArgs a) {
+__device__ __forceinline__ Rows<T> rows_at(const VerifyArgs& a, int req, const Stop& stop) {
+  const int64_t row = (int64_t)a.starts[req] + req + stop.node;
+  return {static_cast<const T*>(a.target) + row * a.target_stride,
+          DRAWN && stop.draft >= 0 ? static_cast<const T*>(a.draft_probs) + (int64_t)stop.draft * a.draft_stride : nullptr};
+}
+
+// A lane's part of a chunk's sums: the residual's, and p's.
+template <typename T, bool DRAWN>
+struct Chunk {
+  static constexpr int N = Wide<T>::N;
+  Packs<T> p, q = {};
+  __device__ __forceinline__ void load(const Rows<T>& rows, int chunk, int lane, int vocab) {
+    load_packs<T>(p, rows.p, chunk * Wide<T>::CHUNK + lane * N, 64 * N, vocab);
+    if constexpr (DRAWN) {
+      if (rows.q) load_packs<T>(q, rows.q, chunk * Wide<T>::CHUNK + lane * N, 64 * N, vocab);  // (else zeros)
+    }
+  }
+  template <bool LESS>
+  __device__ __forceinline__ double sum(int vocab) const {
+    double s = 0.0;
+#pragma unroll
+    for (int j = 0; j < kLoads; ++j) {
+      double r[N];
+      residual<T, LESS>(p, q, j, vocab, r);
+#pragma unroll
+      for (int k = 0; k < N; ++k) s += r[k];
+    }
+    return s;
+  }
+  __device__ __forceinline__ double2 sums(const Rows<T>& rows, const int32_t* kids, int nkids, int chunk, int vocab) {
+    const double full = sum<false>(vocab);
+    double rest = full;
+    if constexpr (DRAWN) {
+      if (rows.q) rest = sum<true>(vocab);
+    } else {
+      if (take_out<T>(p, kids, nkids, chunk * Wide<T>::CHUNK, vocab)) rest = sum<false>(vocab);
+    }
+    return make_double2(wave_sum(rest), wave_sum(full));
+  }
+};
+
+// The draw, by one wave: the chunk that holds it from the chunks' sums, then the
+// element.
+template <typename T, bool DRAWN>
+__device__ __forceinline__ void draw(const VerifyArgs& a, int req, int lane, const double2* sums, const Rows<T>& rows,
+                                     const int32_t* kids, int nkids) {
   constexpr int N = Wide<T>::N;
   constexpr int kHeld = 4;  // rounds of 64 chunks whose sums stay in registers
-  const int req = blockIdx.x;
-  const int lane = threadIdx.x & 63;
-  const double2* sums = a.sums + (int64_t)req * a.chunks;
-  const Stop stop = a.stops[req];
-  const int first = a.starts[req];
   const double u = uniform_at(a.sample_uniforms, req, a.uniforms_f64);
   double2 held[kHeld];
 #pragma unroll
@@ -357,16 +385,14 @@ __global__ __launch_bounds__(64) void verify_draw_kernel(const VerifyArgs a) {
     return;
   }
   // The chunk, kLoads * N elements in a row per lane.
-  const T* drafts = static_cast<const T*>(a.draft_probs);
-  const T* prow = static_cast<const T*>(a.target) + ((int64_t)first + req + stop.node) * a.target_stride;
-  const T* qrow = residual_left && stop.draft >= 0 ? drafts + (int64_t)stop.draft * a.draft_stride : nullptr;
+  const T* qrow = residual_left ? rows.q : nullptr;
   const int begin = at * Wide<T>::CHUNK + lane * kLoads * N;
   Packs<T> p, q = {};
-  load_packs<T>(p, prow, begin, N, a.vocab);
+  load_packs<T>(p, rows.p, begin, N, a.vocab);
   if constexpr (DRAWN) {
     if (qrow) load_packs<T>(q, qrow, begin, N, a.vocab);
   } else {
-    if (residual_left) take_out<T>(p, a.children + first, stop.num_children, at * Wide<T>::CHUNK, a.vocab);
+    if (residual_left) take_out<T>(p, kids, nkids, at * Wide<T>::CHUNK, a.vocab);
   }
   double r[kLoads][N], s = 0.0;
 #pragma unroll
@@ -392,6 +418,41 @@ __global__ __launch_bounds__(64) void verify_draw_kernel(const VerifyArgs a) {
   if (lane == 0) a.out_tokens[req] = token;
 }
 
+}  // namespace
+
+// Grid of the first launch: (workgroups per request, requests); every
+// workgroup walks, then a request's waves take its chunks in turn.
+template <typename T, bool DRAWN>
+__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(4))) void verify_sums_kernel(
+    const VerifyArgs a) {
+  __shared__ WalkShared<DRAWN> s;
+  const int req = blockIdx.y;
+  const bool leader = blockIdx.x == 0;  // writes what is found
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+  const Stop stop = walk<T, DRAWN, kThreads>(a, req, leader, s);
+  if (leader) {
+    if (threadIdx.x == 0) a.stops[req] = stop;
+    for (int c = threadIdx.x; c < stop.num_children; c += kThreads) a.children[a.starts[req] + c] = s.kids[c];
+  }
+  const Rows<T> rows = rows_at<T, DRAWN>(a, req, stop);
+  for (int chunk = blockIdx.x * kWaves + wave; chunk < a.chunks; chunk += gridDim.x * kWaves) {
+    Chunk<T, DRAWN> x;
+    x.load(rows, chunk, lane, a.vocab);
+    const double2 sum = x.sums(rows, s.kids, stop.num_children, chunk, a.vocab);
+    if (lane == 0) a.sums[(int64_t)req * a.chunks + chunk] = sum;
+  }
+}
+
+// Grid of the second: requests, one wave each.
+template <typename T, bool DRAWN>
+__global__ __launch_bounds__(64) void verify_draw_kernel(const VerifyArgs a) {
+  const int req = blockIdx.x;
+  const Stop stop = a.stops[req];
+  draw<T, DRAWN>(a, req, threadIdx.x & 63, a.sums + (int64_t)req * a.chunks, rows_at<T, DRAWN>(a, req, stop),
+                 a.children + a.starts[req], stop.num_children);
+}
+
 }  // namespace lvamd
 
 using namespace lvamd;
@@ -405,7 +466,7 @@ extern "C" int64_t lvamd_verify_drafts_workspace_size(int64_t num_requests, int6
                                                       int32_t dtype) {
   if (num_requests <= 0 || num_drafts < 0 || vocab <= 0) return 0;
   return num_requests * ((int64_t)verify_chunks(vocab, dtype) * (int64_t)sizeof(double2) + (int64_t)sizeof(Stop)) +
-         num_drafts * 8;
+         num_drafts * 4;
 }
 
 extern "C" int lvamd_verify_drafts(const void* target, int64_t target_row_stride, const void* draft_probs,
@@ -440,7 +501,7 @@ extern "C" int lvamd_verify_drafts(const void* target, int64_t target_row_stride
   a.chunks = verify_chunks(vocab, dtype);
   a.sums = static_cast<double2*>(workspace);
   a.stops = reinterpret_cast<Stop*>(a.sums + num_requests * a.chunks);
-  a.children = reinterpret_cast<int64_t*>(a.stops + num_requests);
+  a.children = reinterpret_cast<int32_t*>(a.stops + num_requests);
   a.counts = counts;
   a.paths = paths;
   a.path_width = path_width;
@@ -448,9 +509,9 @@ extern "C" int lvamd_verify_drafts(const void* target, int64_t target_row_stride
   a.vocab = vocab;
   a.uniforms_f64 = uniforms_f64 != 0;
   hipStream_t s = static_cast<hipStream_t>(stream);
-  // A chunk per wave while about kWorkgroups of them suffice; several in larger
-  // batches, which spreads the walk over more of the row.
-  constexpr int64_t kWorkgroups = 2048;
+  // A chunk per wave while kWorkgroups (six per CU, all resident) suffice; several
+  // in larger batches, which spreads the walk over more of the row.
+  constexpr int64_t kWorkgroups = 1536;
   const int64_t most = (a.chunks + kWaves - 1) / kWaves;
   const int64_t share = std::max<int64_t>(1, std::min<int64_t>(most, kWorkgroups / num_requests));
   const dim3 grid((unsigned)share, (unsigned)num_requests), draw((unsigned)num_requests), threads(kThreads);
