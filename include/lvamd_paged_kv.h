@@ -554,9 +554,9 @@ int lvamd_paged_decode_q8_resident_waves(int32_t dtype, int32_t head_size);
 
 /*
  * Prefill and tree attention over an 8-bit cache that holds the step's tokens
- * already: lvamd_paged_prefill's unit records, of up to `columns` columns (128, or
- * 64 where every request has at most 64), and partials, [slots][num_kv_heads]
- * [columns], the rows in fp32.
+ * already: lvamd_paged_prefill's unit records, of up to `columns` columns (128;
+ * 64 where every request has at most 64; 256 for head sizes 80 ... 128), and
+ * partials, [slots][num_kv_heads][columns], the rows in fp32.
  */
 int lvamd_paged_prefill_q8(const void* q, int64_t q_token_stride, int64_t q_head_stride,
                            const void* key_pool, const float* key_scales,
@@ -569,7 +569,7 @@ int lvamd_paged_prefill_q8(const void* q, int64_t q_token_stride, int64_t q_head
                            int32_t block_size, float scale, int32_t dtype, lvamd_stream_t stream);
 
 /* Keys per tile of it (key ranges start on multiples), and its workgroups (of
- * units of 64 or 128 columns) that the current device holds at once (needs a
+ * units of that many columns) that the current device holds at once (needs a
  * GPU). */
 int lvamd_paged_prefill_q8_key_tokens(int32_t dtype, int32_t head_size);
 int lvamd_paged_prefill_q8_resident_units(int32_t dtype, int32_t head_size, int32_t columns);
@@ -583,8 +583,9 @@ int lvamd_paged_attention_merge_q8(const void* part_acc, const float* part_ml,
                                    int32_t max_columns, int32_t dtype, lvamd_stream_t stream);
 
 /* One layer's launch facts over an 8-bit cache: lvamd_attention_plan (col_tiles
- * 1, group_waves 1, prefill_col_tiles 8 or 4: units of 128 or 64 columns) with the step's slots, and where the
- * scales lie: scale_offset bytes (a multiple of 16) after each pool's base. */
+ * 1, group_waves 1, prefill_col_tiles 4, 8 or 16: a sixteenth of the units'
+ * columns) with the step's slots, and where the scales lie: scale_offset bytes
+ * (a multiple of 16) after each pool's base. */
 typedef struct lvamd_attention_plan_q8 {
   lvamd_attention_plan base;
   const int64_t* slots; /* [num_tokens], a block's slots consecutive; or NULL */

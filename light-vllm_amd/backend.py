@@ -26,6 +26,7 @@ decode / prefill work lists go to the GPU in one non-blocking copy.
 from __future__ import annotations
 
 import ctypes
+import math
 import weakref
 
 import torch
@@ -450,13 +451,32 @@ class HipPagedAttention:
         return found
 
 
-def _quantized_columns(facts, spec) -> int:
-    """Unit width of the 8-bit prefill kernel for a step: 64 columns (one column
-    tile per wave, several tiles in flight) where no request has more, else 128."""
+def _quantized_columns(facts, spec, code: int) -> int:
+    """Unit width of the 8-bit prefill kernel for a step: 64 columns (several
+    tiles in flight) where no request has more; 256 (half the conversions) where
+    units of long key ranges fill the GPU's last round of them to four fifths;
+    else 128.
 
-    group = spec.num_query_heads // spec.num_kv_heads
-    return (native.PREFILL_Q8_NARROW if facts.longest * group <= native.PREFILL_Q8_NARROW
-            else native.PREFILL_Q8_COLUMNS)
+    Microseconds for chunks of n tokens after c, 28 heads over 4, D = 128, 128
+    columns against 256: n 2048, c 14336 (0.88 rounds) 545 / 489; n 4096, c 0 (1.75
+    rounds, 2048 keys on average) 172 / 147; n 8192, c 0 (3.5) 555 / 521; but n
+    2048, c 0 (1024 keys) 65 / 71; n 1536, c 14336 (0.66 rounds) 416 / 465; n 3000,
+    c 14336 (1.3) 819 / 905.  At D = 80 and 96 n 2048, c 8192: 273 / 263, 288 / 271;
+    at D = 64 the same either way."""
+
+    group, d = spec.num_query_heads // spec.num_kv_heads, spec.head_size
+    if facts.longest * group <= native.PREFILL_Q8_NARROW:
+        return native.PREFILL_Q8_NARROW
+    if 64 < d <= 128 and facts.longest * group > native.PREFILL_Q8_COLUMNS:
+        q = facts.q_lens
+        rows = q * group > DECODE_MAX_COLUMNS  # (the others are the decode kernel's)
+        q, computed = q[rows], facts.computed[rows]
+        units = int((-(-q * group // native.PREFILL_Q8_WIDE)).sum()) * spec.num_kv_heads
+        rounds = units / native.prefill_q8_resident_units(code, d, native.PREFILL_Q8_WIDE)
+        keys = float((q * (2 * computed + q)).sum()) / (2 * float(q.sum()))
+        if keys >= 2048 and rounds >= 0.8 * math.ceil(rounds):
+            return native.PREFILL_Q8_WIDE
+    return native.PREFILL_Q8_COLUMNS
 
 
 _APPEND_UNITS = 3
@@ -530,7 +550,7 @@ class HipQuantizedPagedAttention(HipPagedAttention):
         if found is not None and found.workspace_ptr is not None and found.workspace_ptr != backend.workspace.ptr():
             found = None  # the workspace (shared by all plans) was regrown since
         if found is None:
-            columns = _quantized_columns(plan.facts, spec)
+            columns = _quantized_columns(plan.facts, spec, code)
             work = plan.layer_work(backend.quantized_facts(spec, code, self._config.block_size, columns))
             sizes = _partial_layout(work, spec, columns, 4)  # fp32 rows
             ptr = None
@@ -682,8 +702,8 @@ class HipPagedAttentionBackend:
 
     def quantized_facts(self, spec, code: int, block_size: int, columns: int) -> tuple[int, ...]:
         """``kernel_facts`` of the kernels over an 8-bit cache: one decode shape
-        (one column tile, stream-K) and the prefill shape of ``columns`` columns
-        (four waves); the options that choose among the 16-bit kernels' shapes do
+        (one column tile, stream-K) and the prefill shape of ``columns`` columns;
+        the options that choose among the 16-bit kernels' shapes do
         not apply."""
 
         key = (spec.num_query_heads, spec.num_kv_heads, spec.head_size, code, block_size, torch.cuda.current_device(),
@@ -753,7 +773,7 @@ class HipPagedAttentionBackend:
         config = cache.config
         code = dtype_code(config.dtype)
         shapes = {(s.num_query_heads, s.num_kv_heads, s.head_size): s for s in cache.model_spec.layers}
-        columns = tuple(_quantized_columns(facts, spec) for spec in shapes.values())
+        columns = tuple(_quantized_columns(facts, spec, code) for spec in shapes.values())
         by_columns = self._shapes.setdefault(cache, {})
         found = by_columns.get(columns)
         if found is None:

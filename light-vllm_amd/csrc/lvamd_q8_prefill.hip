@@ -7,17 +7,26 @@
 // merge are the same too.
 //
 // Mapping onto CDNA4:
-//   * A unit is up to 128 columns, (query, head-in-group) pairs of one kv head;
-//     four waves of two 16-column tiles share every key tile (64 keys, 32
-//     above D = 128).  Steps whose requests all have at most 64 columns (tree
-//     verification, short chunks) take units of 64, one column tile per wave:
-//     no wave is left without columns, and the registers hold several tiles in
-//     flight, as such units are bound by the latency of their few tiles.
+//   * A unit is up to 128 columns, (query, head-in-group) pairs of one kv head:
+//     eight waves of one 16-column tile share every key tile (64 keys, 32 above
+//     D = 128).  Four waves of two tiles each read half as much of LDS, but fill
+//     the registers: half as many waves per SIMD, none beside it above D = 128.
+//     A chunk of 1024 tokens after 4096 (16 heads, 4 kv heads) took 182 us so at
+//     D = 160 against 125, 219 against 154 at D = 256; at D = 128 2048 tokens (28
+//     heads, 4 kv heads) 73 against 65, and 536 against 555 for 8192.
+//   * Units of 256 columns, eight waves of two tiles, for chunks that fill the
+//     GPU with them (64 < D <= 128, backend.py's rule): each code is converted
+//     for twice the products.  2048 tokens after 14336, 28 heads, 4 kv heads, D
+//     = 128: 485 us (930 TFLOP/s) against 545.
+//   * Units of 64 columns, four waves, for steps whose requests all have at most
+//     64 (tree verification, short chunks): no wave is left without columns, and
+//     the registers hold several tiles in flight, as such units are bound by the
+//     latency of their few tiles.
 //   * A tile's codes go to registers (16 per load and thread) while the last
 //     tile computes, become T with their block's scale (exactly, lvamd_q8.h)
 //     and are written to the other of two LDS buffers; one barrier per tile.
 //     Converting before LDS, each code is converted once per workgroup;
-//     direct loads to LDS would leave it to each of the four waves.
+//     direct loads to LDS would leave it to each of the waves.
 //   * S^T = K Q^T, O^T = V^T P^T and the softmax sums on MFMA 16x16x32, online
 //     softmax in the log2 domain with lazy rescaling, as in the 16-bit kernel.
 //   * NaN values of this step's tokens: as in the 8-bit decode kernel, they go
@@ -32,8 +41,6 @@ namespace lvamd {
 namespace {
 
 constexpr float kSlack = 8.0f;  // lazy-rescale threshold, log2 units
-constexpr int kWaves = 4;
-constexpr int unit_columns(int col_tiles) { return 16 * kWaves * col_tiles; }
 
 struct Q8PrefillArgs {
   const void* q;
@@ -54,28 +61,29 @@ struct Q8PrefillArgs {
   float scale_log2;
 };
 
-template <int D, int CT>
+// CT: column tiles per wave, 2 or 1; W: waves.
+template <int D, int CT, int W>
 struct Q8PrefillShape {
+  static constexpr int COLUMNS = 16 * W * CT;
   static constexpr int KT = D <= 128 ? 64 : 32;
   static constexpr int KS = KT / 16;
   static constexpr int C8 = D / 16;              // 16-code chunks per row
   static constexpr int CPR = D / 8;              // 16-byte chunks of T per row
   static constexpr int RS = q8_row_stride(CPR);  // LDS row stride in chunks
-  static constexpr int THREADS = 64 * kWaves;
+  static constexpr int THREADS = 64 * W;
   static constexpr int LPT = (KT * C8 + THREADS - 1) / THREADS;  // loads per thread and tensor
   static constexpr int NCH = (D + 31) / 32;
   static constexpr int NT = D / 16;
-  static constexpr int PD = CT == 2 ? 1 : D <= 128 ? 4 : 2;  // tiles in flight
+  static constexpr int PD = CT == 2 || W == 8 ? 1 : D <= 128 ? 4 : 2;  // tiles in flight
 };
 
 }  // namespace
 
-// CT: column tiles per wave, 2 or 1.
-template <typename T, int D, int CT>
-__global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(D <= 128 ? 2 : 1))) void q8_prefill_kernel(
+template <typename T, int D, int CT, int W>
+__global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(W == 4 ? (D <= 128 ? 2 : 1) : CT == 1 && D <= 128 ? 4 : 2))) void q8_prefill_kernel(
     const int32_t* __restrict__ units, const int32_t num_kv_heads, const uint32_t heads_magic, const int32_t heads_shift,
     const Q8PrefillArgs a) {
-  using P = Q8PrefillShape<D, CT>;
+  using P = Q8PrefillShape<D, CT, W>;
   constexpr int KT = P::KT, KS = P::KS, C8 = P::C8, CPR = P::CPR, RS = P::RS, LPT = P::LPT, NCH = P::NCH, NT = P::NT;
   constexpr int PD = P::PD;
   using V8 = typename std::conditional<std::is_same<T, __bf16>::value, bf16x8, f16x8>::type;
@@ -448,7 +456,7 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(D <
     const float l_tot = l_run[ct][0];
     const float inv = l_tot > 0.f ? 1.f / l_tot : l_tot == 0.f ? 0.f : l_tot;  // (NaN stays)
     if (slot >= 0) {
-      const int64_t cs = ((int64_t)slot * Hkv + kvh) * unit_columns(CT) + 16 * (CT * wave + ct) + l16;
+      const int64_t cs = ((int64_t)slot * Hkv + kvh) * P::COLUMNS + 16 * (CT * wave + ct) + l16;
       float* row = static_cast<float*>(a.part_acc) + cs * D;
 #pragma unroll
       for (int n = 0; n < NT; ++n) store_partial4<true, float>(row + 16 * n + 4 * g, acc[ct][n], inv);
@@ -472,34 +480,48 @@ bool prefill_q8_supported(int dtype, int head_size) {
   return (dtype == LVAMD_BF16 || dtype == LVAMD_F16) && head_size >= 32 && head_size <= 256 && head_size % 16 == 0;
 }
 
-template <typename T, int CT, typename F>
+template <typename T, int CT, int W, typename F>
 int with_prefill_head_size(int head_size, F& f) {
   switch (head_size) {
-    case 32: return f.template operator()<T, 32, CT>();
-    case 48: return f.template operator()<T, 48, CT>();
-    case 64: return f.template operator()<T, 64, CT>();
-    case 80: return f.template operator()<T, 80, CT>();
-    case 96: return f.template operator()<T, 96, CT>();
-    case 112: return f.template operator()<T, 112, CT>();
-    case 128: return f.template operator()<T, 128, CT>();
-    case 144: return f.template operator()<T, 144, CT>();
-    case 160: return f.template operator()<T, 160, CT>();
-    case 176: return f.template operator()<T, 176, CT>();
-    case 192: return f.template operator()<T, 192, CT>();
-    case 208: return f.template operator()<T, 208, CT>();
-    case 224: return f.template operator()<T, 224, CT>();
-    case 240: return f.template operator()<T, 240, CT>();
-    case 256: return f.template operator()<T, 256, CT>();
+    case 32: return f.template operator()<T, 32, CT, W>();
+    case 48: return f.template operator()<T, 48, CT, W>();
+    case 64: return f.template operator()<T, 64, CT, W>();
+    case 80: return f.template operator()<T, 80, CT, W>();
+    case 96: return f.template operator()<T, 96, CT, W>();
+    case 112: return f.template operator()<T, 112, CT, W>();
+    case 128: return f.template operator()<T, 128, CT, W>();
+    case 144: return f.template operator()<T, 144, CT, W>();
+    case 160: return f.template operator()<T, 160, CT, W>();
+    case 176: return f.template operator()<T, 176, CT, W>();
+    case 192: return f.template operator()<T, 192, CT, W>();
+    case 208: return f.template operator()<T, 208, CT, W>();
+    case 224: return f.template operator()<T, 224, CT, W>();
+    case 240: return f.template operator()<T, 240, CT, W>();
+    case 256: return f.template operator()<T, 256, CT, W>();
     default: return LVAMD_ERR_UNSUPPORTED;
   }
 }
+// (Units of 256 columns: the head sizes whose two tiles per wave fit the
+// registers, and whose products are long enough to gain by them.)
+template <typename T, typename F>
+int with_wide_head_size(int head_size, F& f) {
+  switch (head_size) {
+    case 80: return f.template operator()<T, 80, 2, 8>();
+    case 96: return f.template operator()<T, 96, 2, 8>();
+    case 112: return f.template operator()<T, 112, 2, 8>();
+    case 128: return f.template operator()<T, 128, 2, 8>();
+    default: return LVAMD_ERR_UNSUPPORTED;
+  }
+}
+bool prefill_q8_columns(int columns) { return columns == 64 || columns == 128 || columns == 256; }
 template <typename F>
 int dispatch_prefill(int dtype, int head_size, int columns, F f) {
-  if (columns == 64)
-    return dtype == LVAMD_BF16 ? with_prefill_head_size<__bf16, 1>(head_size, f)
-                               : with_prefill_head_size<_Float16, 1>(head_size, f);
-  return dtype == LVAMD_BF16 ? with_prefill_head_size<__bf16, 2>(head_size, f)
-                             : with_prefill_head_size<_Float16, 2>(head_size, f);
+  const bool bf16 = dtype == LVAMD_BF16;
+  switch (columns) {
+    case 64: return bf16 ? with_prefill_head_size<__bf16, 1, 4>(head_size, f) : with_prefill_head_size<_Float16, 1, 4>(head_size, f);
+    case 128: return bf16 ? with_prefill_head_size<__bf16, 1, 8>(head_size, f) : with_prefill_head_size<_Float16, 1, 8>(head_size, f);
+    default: return bf16 ? with_wide_head_size<__bf16>(head_size, f) : with_wide_head_size<_Float16>(head_size, f);
+  }
 }
 
 }  // namespace
@@ -514,14 +536,14 @@ extern "C" int lvamd_paged_prefill_q8_key_tokens(int32_t dtype, int32_t head_siz
 }
 
 extern "C" int lvamd_paged_prefill_q8_resident_units(int32_t dtype, int32_t head_size, int32_t columns) {
-  if (!prefill_q8_supported(dtype, head_size) || (columns != 64 && columns != 128)) return LVAMD_ERR_UNSUPPORTED;
-  return dispatch_prefill(dtype, head_size, columns, []<typename T, int D, int CT>() -> int {
+  if (!prefill_q8_supported(dtype, head_size) || !prefill_q8_columns(columns)) return LVAMD_ERR_UNSUPPORTED;
+  return dispatch_prefill(dtype, head_size, columns, []<typename T, int D, int CT, int W>() -> int {
     int device = 0, cus = 0, per_cu = 0;
     if (hipGetDevice(&device) != hipSuccess) return LVAMD_ERR_LAUNCH;
     if (hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, device) != hipSuccess)
       return LVAMD_ERR_LAUNCH;
-    if (hipOccupancyMaxActiveBlocksPerMultiprocessor(&per_cu, reinterpret_cast<const void*>(&q8_prefill_kernel<T, D, CT>),
-                                                     64 * kWaves, 0) != hipSuccess)
+    if (hipOccupancyMaxActiveBlocksPerMultiprocessor(&per_cu, reinterpret_cast<const void*>(&q8_prefill_kernel<T, D, CT, W>),
+                                                     64 * W, 0) != hipSuccess)
       return LVAMD_ERR_LAUNCH;
     return per_cu * cus;
   });
@@ -534,7 +556,7 @@ extern "C" int lvamd_paged_prefill_q8(const void* q, int64_t q_token_stride, int
                                       int32_t num_units, void* part_acc, float* part_ml, int64_t num_partial_slots,
                                       int32_t num_kv_heads, int32_t group, int32_t head_size, int32_t columns,
                                       int32_t block_size, float scale, int32_t dtype, lvamd_stream_t stream) {
-  if (!prefill_q8_supported(dtype, head_size) || (columns != 64 && columns != 128)) return LVAMD_ERR_UNSUPPORTED;
+  if (!prefill_q8_supported(dtype, head_size) || !prefill_q8_columns(columns)) return LVAMD_ERR_UNSUPPORTED;
   if (num_units < 0 || num_kv_heads <= 0 || group <= 0 || block_size <= 0 || num_partial_slots < 0)
     return LVAMD_ERR_INVALID_ARGUMENT;
   if (num_units == 0) return LVAMD_OK;
@@ -565,8 +587,8 @@ extern "C" int lvamd_paged_prefill_q8(const void* q, int64_t q_token_stride, int
   a.scale_log2 = scale * 1.4426950408889634f;
   const FastDiv by_heads(num_kv_heads);
   hipStream_t s = static_cast<hipStream_t>(stream);
-  return dispatch_prefill(dtype, head_size, columns, [&]<typename T, int D, int CT>() -> int {
-    hipLaunchKernelGGL((q8_prefill_kernel<T, D, CT>), dim3((unsigned)(num_units * num_kv_heads)), dim3(64 * kWaves), 0, s,
+  return dispatch_prefill(dtype, head_size, columns, [&]<typename T, int D, int CT, int W>() -> int {
+    hipLaunchKernelGGL((q8_prefill_kernel<T, D, CT, W>), dim3((unsigned)(num_units * num_kv_heads)), dim3(64 * W), 0, s,
                        units, num_kv_heads, by_heads.magic, by_heads.shift, a);
     return launch_status();
   });

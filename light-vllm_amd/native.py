@@ -172,7 +172,7 @@ class AttentionPlanQ8(ctypes.Structure):
 # Most drafts of a request that lvamd_verify_drafts takes.
 VERIFY_MAX_DRAFTS = 1024
 # Columns per prefill unit of the 8-bit kernel: steps of narrow requests, others.
-PREFILL_Q8_NARROW, PREFILL_Q8_COLUMNS = 64, 128
+PREFILL_Q8_NARROW, PREFILL_Q8_COLUMNS, PREFILL_Q8_WIDE = 64, 128, 256
 
 
 def library_path() -> Path:

@@ -323,6 +323,43 @@ def test_every_head_size(d) -> None:
         _attend_and_check(*_step(6, 2, d, 16, dtype, [333, 70, 90], [1, (-1, 0, 0), 50], seed=d), dtype)
 
 
+@pytest.mark.parametrize("dtype", ("bf16", "fp16"))
+@pytest.mark.parametrize("d", (80, 96, 112, 128))
+def test_units_of_256_columns(monkeypatch, d, dtype) -> None:
+    """Chunks and trees in units of 256 columns (large chunks only, by the backend's
+    rule): more and fewer columns than a unit, split key ranges, NaN."""
+    print(f"[gpu] q8 attention, 256 columns, head size {d} {dtype}", file=sys.stderr, flush=True)
+    t = DTYPES[dtype]
+    monkeypatch.setattr(sys.modules["light_vllm_amd.backend"], "_quantized_columns", lambda *a: 256)
+    rng = np.random.default_rng(d)
+    tree = tuple([-1] + [int(rng.integers(0, i)) for i in range(1, 70)])
+    _attend_and_check(*_step(12, 2, d, 16, t, [0, 100, 1500, 7], [130, 41, tree, 1], seed=d), t)
+    _attend_and_check(*_step(4, 1, d, 12, t, [5000], [90], seed=d + 1), t)
+    _attend_and_check(*_step(12, 2, d, 16, t, [256 + 5 * i for i in range(6)], [50] * 6, seed=d + 2, prefix=16), t)
+    cache, metadata, q, k, v = _step(6, 2, d, 16, t, [40], [60], seed=d + 3)
+    v[50, 1, 5] = math.nan
+    out = lv.HipPagedAttentionBackend().create(cache, metadata).forward("layer0", q, k, v, scale=1 / math.sqrt(d))
+    nan = torch.isnan(out)
+    assert bool(nan[50:, 3:, 5].all()) and int(nan.sum()) == 10 * 3
+
+
+def test_unit_width_rule() -> None:
+    import light_vllm_amd.backend as B
+
+    def width(c, n, hq=28, hkv=4, d=128, requests=1):
+        spec = lv.AttentionLayerSpec("l", hq, hkv, d)
+        blocks = -(-(c + n) // 64)
+        md = lv.PagedAttentionMetadata(
+            block_tables=tuple(tuple(range(i * blocks, (i + 1) * blocks)) for i in range(requests)),
+            num_computed_tokens=(c,) * requests, query_layouts=(lv.QueryLayout(tuple(range(-1, n - 1))),) * requests)
+        return B._quantized_columns(B.facts_of(md), spec, 2)
+
+    assert width(5000, 1) == width(100, 9) == 64 and width(100, 10) == 128
+    if torch.cuda.get_device_properties(0).multi_processor_count == 256:
+        assert width(14336, 2048) == width(0, 4096) == width(2048, 512, requests=4) == 256
+        assert width(0, 2048) == width(14336, 1536) == width(14336, 2048, d=64) == width(14336, 2048, d=144) == 128
+
+
 def test_long_tree_and_deep_split() -> None:
     print("[gpu] q8 attention trees of 40 and 70 queries, one long sequence", file=sys.stderr, flush=True)
     rng = np.random.default_rng(8)

@@ -144,7 +144,7 @@ def test_attention_entry_point_checks() -> None:
     for kv in ((X, 512, 128, None, 512, 128), (X, 508, 128, X, 512, 128), (ctypes.c_void_p(8), 512, 128, X, 512, 128)):
         assert decode(kv=kv) == -1, kv
     assert decode(kv=new, bs=12) == -1 and decode(kv=new, bs=128) == -1
-    assert prefill(columns=32) == -2 and prefill(columns=256) == -2 and prefill(columns=64, q=None) == -1
+    assert prefill(columns=32) == -2 and prefill(columns=512) == -2 and prefill(columns=256, d=64) == -2 and prefill(columns=64, q=None) == -1
     merge = lambda dtype, jobs, cols=1: lib.lvamd_paged_attention_merge_q8(X, X, X, 0, 0, X, jobs, 4, 7, 128, cols, 16, dtype, None)  # noqa: E731
     assert merge(2, 0) == 0 and merge(0, 1) == -2 and merge(2, -1) == -1 and merge(1, 1, 17) == -2
     for d in (32, 64, 80, 128, 256):
