@@ -34,6 +34,11 @@
 //     which a zero probability would not hide: rows of this step go to LDS
 //     with NaN as zero, and the columns that do see such a row get it back
 //     (poison, below; code that no ordinary step enters).
+//
+// HBM-bound in long steps, a chain of dependent round trips in short ones.  28
+// heads over 4, D = 128: 64 sequences of 512-4095 tokens (bf16) 33 us for 159 MB,
+// 4.8 TB/s; 16 of 32767 (fp16) 88 us for 537 MB, 6.1 TB/s.  4 sequences of
+// 37-511 tokens, 14 heads over 2, D = 64: 8 us with the append.
 
 #include <cmath>
 

@@ -31,6 +31,11 @@
 //     softmax in the log2 domain with lazy rescaling, as in the 16-bit kernel.
 //   * NaN values of this step's tokens: as in the 8-bit decode kernel, they go
 //     to LDS as zero and the columns that see the row get them back.
+//
+// Bound by the matrix units' schedule in chunks (they are busy 48% of the time;
+// LDS reads, the softmax and the conversions share the issue), by the chain of a
+// unit's few tiles in tree steps: 32 trees of 9 queries after 500-2560 tokens, 12
+// heads over 2, D = 128: 14 us, and 5 for the merge.
 
 #include <cmath>
 

@@ -27,6 +27,12 @@
 // before it); then its waves sum chunks of the residual, 4 KiB of a row each.
 // The second launch is one wave per request, without a barrier: it scans the
 // chunks' sums, then the one chunk that holds the draw.
+//
+// One request of 4 drafts, 151,936 tokens, fp32 with q: 4.8 + 4.0 us.  128 trees
+// over 100,003 tokens, bf16: 12.5 + 4.8 us for 26 MB, of which the walk's two
+// rounds of loads take about 4.  One launch of a workgroup per request won 1-2 us
+// below 1000 tokens and lost up to four times at 151,936 (one CU then converts
+// and adds every element).
 
 #include <algorithm>
 #include <cmath>
@@ -510,7 +516,9 @@ extern "C" int lvamd_verify_drafts(const void* target, int64_t target_row_stride
   a.uniforms_f64 = uniforms_f64 != 0;
   hipStream_t s = static_cast<hipStream_t>(stream);
   // A chunk per wave while kWorkgroups (six per CU, all resident) suffice; several
-  // in larger batches, which spreads the walk over more of the row.
+  // in larger batches, which spreads the walk over more of the row.  (512 requests
+  // of 151,936 fp32 tokens: 1024 91 us, 1536 78, 2048 93, 4096 83; 128 of 100,003:
+  // 20.9, 19.2, 22.4, 21.8; up to 8 requests no difference.)
   constexpr int64_t kWorkgroups = 1536;
   const int64_t most = (a.chunks + kWaves - 1) / kWaves;
   const int64_t share = std::max<int64_t>(1, std::min<int64_t>(most, kWorkgroups / num_requests));
