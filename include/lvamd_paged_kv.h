@@ -628,13 +628,19 @@ int lvamd_kv_compact_q8(const uint64_t* layer_key_ptrs, const uint64_t* layer_va
                         int64_t scale_offset, const int64_t* src_slots, const int64_t* dst_slots, int64_t num_pairs,
                         const int64_t* block_starts, int64_t num_dst_blocks,
                         void* workspace, int64_t workspace_bytes, lvamd_stream_t stream);
-/* The same for at most lvamd_kv_compact_q8_few_pairs() pairs given in HOST
- * memory (grouped by destination block too): one launch, no workspace. */
+/* The same for at most lvamd_kv_compact_q8_few_call_pairs() pairs given in HOST
+ * memory (grouped by destination block too): one launch, no workspace.  The pairs
+ * come in at most 32 chunks (chunk c: pairs chunk_starts[c] ... chunk_starts[c + 1],
+ * HOST memory) of at most lvamd_kv_compact_q8_few_pairs() each; no block that one
+ * chunk writes is another's, as destination or as source (the caller proves
+ * this: a step's requests touch their own blocks). */
 int lvamd_kv_compact_q8_few(const uint64_t* layer_key_ptrs, const uint64_t* layer_value_ptrs,
                             int32_t num_layers, int32_t num_kv_heads, int32_t head_size, int32_t block_size,
                             int64_t scale_offset, const int64_t* src_slots, const int64_t* dst_slots,
-                            int64_t num_pairs, lvamd_stream_t stream);
+                            int64_t num_pairs, const int32_t* chunk_starts, int32_t num_chunks,
+                            lvamd_stream_t stream);
 int64_t lvamd_kv_compact_q8_few_pairs(void);
+int64_t lvamd_kv_compact_q8_few_call_pairs(void);
 int64_t lvamd_kv_compact_q8_workspace_size(int64_t num_pairs, int32_t num_layers, int32_t num_kv_heads,
                                            int32_t head_size);
 

@@ -2462,6 +2462,63 @@ PyObject* block_runs(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
 }
 
 // ---------------------------------------------------------------------------
+// compact_chunks(moved, src, dst, block_size, most) -> int32 bytes, or None
+//
+// A compact's pairs (as block_runs') in chunks of whole requests, at most `most`
+// pairs each, of which none reads a block that another writes: the chunks' first
+// pairs and the end.  None where there is no such cut (a longer request, tables
+// that share a written block).
+// ---------------------------------------------------------------------------
+PyObject* compact_chunks(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  if (!want_args(nargs, 5, "compact_chunks")) return nullptr;
+  const int64_t bs = PyLong_AsLongLong(args[3]), most = PyLong_AsLongLong(args[4]);
+  if (PyErr_Occurred()) return nullptr;
+  if (!PyBytes_Check(args[0]) || !PyBytes_Check(args[1]) || !PyBytes_Check(args[2]) || bs <= 0 || most <= 0 ||
+      PyBytes_GET_SIZE(args[1]) != PyBytes_GET_SIZE(args[2])) {
+    PyErr_SetString(PyExc_ValueError, "compact_chunks: moved, src and dst must be bytes, block_size and most positive");
+    return nullptr;
+  }
+  const int64_t* moved = reinterpret_cast<const int64_t*>(PyBytes_AS_STRING(args[0]));
+  const int64_t* src = reinterpret_cast<const int64_t*>(PyBytes_AS_STRING(args[1]));
+  const int64_t* dst = reinterpret_cast<const int64_t*>(PyBytes_AS_STRING(args[2]));
+  const int64_t requests = PyBytes_GET_SIZE(args[0]) / 8, n = PyBytes_GET_SIZE(args[1]) / 8;
+  if (n > INT32_MAX) Py_RETURN_NONE;
+  std::vector<int32_t> starts{0};
+  std::vector<std::pair<int64_t, int32_t>> written;  // (block, chunk)
+  int64_t i = 0;
+  for (int64_t r = 0; r < requests; ++r) {
+    const int64_t m = moved[r];
+    if (m < 0 || m > n - i) break;
+    if (m > most) Py_RETURN_NONE;
+    if (m > 0 && i + m - starts.back() > most) starts.push_back((int32_t)i);
+    const int32_t chunk = (int32_t)starts.size() - 1;
+    for (const int64_t end = i + m; i < end; ++i) {
+      const std::pair<int64_t, int32_t> w{dst[i] / bs, chunk};
+      if (written.empty() || written.back() != w) written.push_back(w);
+    }
+  }
+  if (i != n) {
+    PyErr_SetString(PyExc_ValueError, "compact_chunks: the counts do not match the pairs");
+    return nullptr;
+  }
+  if (starts.size() > 1) {
+    std::sort(written.begin(), written.end());
+    for (size_t k = 1; k < written.size(); ++k)
+      if (written[k].first == written[k - 1].first && written[k].second != written[k - 1].second) Py_RETURN_NONE;
+    int32_t chunk = 0;
+    for (int64_t p = 0; p < n; ++p) {
+      while ((size_t)chunk + 1 < starts.size() && p >= starts[chunk + 1]) ++chunk;
+      const int64_t block = src[p] / bs;
+      const auto at = std::lower_bound(written.begin(), written.end(), std::pair<int64_t, int32_t>{block, INT32_MIN});
+      if (at != written.end() && at->first == block && at->second != chunk) Py_RETURN_NONE;
+    }
+  }
+  starts.push_back((int32_t)n);
+  return PyBytes_FromStringAndSize(reinterpret_cast<const char*>(starts.data()),
+                                   (Py_ssize_t)(starts.size() * sizeof(int32_t)));
+}
+
+// ---------------------------------------------------------------------------
 // verify_tensors(facts, outputs, target, node_uniforms, sample_uniforms,
 //                draft_probs, vocab, dtype object, dtype code) -> status, or kNotFast
 //
@@ -2581,6 +2638,7 @@ PyMethodDef kMethods[] = {
     {"append_tensors", (PyCFunction)(void (*)(void))append_tensors, METH_FASTCALL,
      "the 8-bit cache's write: tensor rules and the lvamd_kv_append_q8 call"},
     {"block_runs", (PyCFunction)(void (*)(void))block_runs, METH_FASTCALL, "destination-block runs of a compact's pairs"},
+    {"compact_chunks", (PyCFunction)(void (*)(void))compact_chunks, METH_FASTCALL, "compact pairs in independent chunks"},
     {"verify_tensors", (PyCFunction)(void (*)(void))verify_tensors, METH_FASTCALL,
      "verify_drafts' rules and the lvamd_verify_drafts call"},
     {nullptr, nullptr, 0, nullptr},

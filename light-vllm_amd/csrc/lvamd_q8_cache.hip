@@ -193,7 +193,8 @@ __global__ __launch_bounds__(64 * kAppendWaves) void q8_append_kernel(const int6
 }
 
 // ---------------------------------------------------------------------------
-// Compact of accepted rows, two launches: the first copies every pair's row
+// Compact of accepted rows that the kernel after this one does not take (more
+// pairs, a request of more than 32, tables that share blocks), two launches: the first copies every pair's row
 // (codes and its block's scale, for every layer, K and V) to the workspace,
 // the second writes them.  Pairs come grouped by destination block; one wave
 // per (destination block, layer, K or V, kv head) takes the larger of the
@@ -266,14 +267,11 @@ __global__ __launch_bounds__(64 * kAppendWaves) void q8_scatter_kernel(const int
   const int64_t row_bytes = (int64_t)a.num_kv_heads * a.head_size;
   uint8_t* const pool = reinterpret_cast<uint8_t*>(base) + (int64_t)h * a.head_size + 16 * c;
   const float inverse = q8_inverse(scale);
-  auto rescaled = [&](uint4 w, float ratio) {
-    return make_uint4(q8_rescale4(w.x, ratio), q8_rescale4(w.y, ratio), q8_rescale4(w.z, ratio), q8_rescale4(w.w, ratio));
-  };
   if (scale > old) {
     const float ratio = old * inverse;
     for (int r = r0; r < a.block_size; r += R) {
       uint4* const at = reinterpret_cast<uint4*>(pool + ((int64_t)block * a.block_size + r) * row_bytes);
-      *at = rescaled(*at, ratio);
+      *at = q8_rescale16(*at, ratio);
     }
     stores_done();
     if (lane == 0) *scale_at = scale;
@@ -281,43 +279,53 @@ __global__ __launch_bounds__(64 * kAppendWaves) void q8_scatter_kernel(const int
   for (int64_t p = first + r0; p < last; p += R) {
     const float from = a.row_scales[row(p)];
     uint4 w = load16(a.rows + row(p) * a.head_size + 16 * c);
-    if (from < scale) w = rescaled(w, from * inverse);
+    if (from < scale) w = q8_rescale16(w, from * inverse);
     *reinterpret_cast<uint4*>(pool + a.dst[p] * row_bytes) = w;
   }
 }
 
 // ---------------------------------------------------------------------------
-// Compact of a few rows (one chat's accepted drafts): one launch, no workspace,
-// the pairs in the kernel's arguments.  A wave owns one kv head of one layer's
-// K or V, so it can hold all the call's rows of it in registers (kFewPairs
-// rows of D bytes, 16 per lane and pass) before it writes any.  Lane i has
-// pair i's slots and scales; a segmented scan gives each destination block's
-// new scale.  A chain of three round trips (scales and rows, re-scaled rows,
-// stores): 3.4 us for one request's rows of 12 layers, against 7.5 in two
-// launches behind an upload.
+// Compact of a step's accepted drafts: one launch, no workspace, the pairs in the
+// kernel's arguments, cut into chunks of at most kFewPairs that do not touch each
+// other's blocks.  A wave owns one kv head of one layer's K or V and one chunk, so
+// it can hold all the chunk's rows of it in registers (kFewPairs rows of D bytes,
+// 16 per lane and pass) before it writes any.  Lane i has pair i's slots and
+// scales; a segmented scan gives each destination block's new scale.  A chain of
+// three round trips (scales and rows, re-scaled rows, stores): 3.4 us for one
+// request's rows of 12 layers, 4.2 for those of 128, against 7.5 in two launches
+// behind an upload (a call of 128 requests 28.5 us against 41).
 // ---------------------------------------------------------------------------
-constexpr int kFewPairs = 32;
+constexpr int kFewPairs = 32;     // of a chunk
+constexpr int kCallPairs = 384;   // of a call (3 KB of arguments)
+constexpr int kCallChunks = 32;
+// (A single chunk travels in arguments of its own size: the larger ones cost the
+// launch 1.2 us of host time, 7.7 us against 6.9 a call of one request.)
+template <int PAIRS, int CHUNKS>
 struct Q8FewArgs {
   const uint64_t* layer_keys;
   const uint64_t* layer_values;
   int64_t scale_offset;
-  int32_t num_pairs, num_kv_heads, head_size, block_size;
+  int32_t num_kv_heads, head_size, block_size;
   FastDiv by_block, by_heads, by_chunks;
-  int32_t src[kFewPairs], dst[kFewPairs];
+  int32_t starts[CHUNKS + 1];  // each chunk's first pair
+  int32_t src[PAIRS], dst[PAIRS];
 };
 
-__global__ __launch_bounds__(64) void q8_compact_few_kernel(const Q8FewArgs a) {
+// Grid: (layer sides x kv heads, chunks).
+
+template <int PAIRS, int CHUNKS>
+__global__ __launch_bounds__(64) void q8_compact_few_kernel(const Q8FewArgs<PAIRS, CHUNKS> a) {
   constexpr int kPasses = kFewPairs * 16 / 64;  // head size 256
   const int lane = threadIdx.x & 63;
   const int side = fast_div((int)blockIdx.x, a.by_heads);
   const int h = (int)blockIdx.x - side * a.num_kv_heads;
-  const int n = a.num_pairs;
+  const int first = a.starts[blockIdx.y], n = a.starts[blockIdx.y + 1] - first;
   char* base = reinterpret_cast<char*>(side & 1 ? a.layer_values[side >> 1] : a.layer_keys[side >> 1]);
   float* const scales = reinterpret_cast<float*>(base + a.scale_offset) + h;
   const int64_t row_bytes = (int64_t)a.num_kv_heads * a.head_size;
   uint8_t* const pool = reinterpret_cast<uint8_t*>(base) + (int64_t)h * a.head_size;
   const int pair = lane < n ? lane : n - 1;  // (lanes past the pairs repeat the last)
-  const int from = a.src[pair], to = a.dst[pair];
+  const int from = a.src[first + pair], to = a.dst[first + pair];
   const int to_block = fast_div(to, a.by_block);
   const float from_scale = scales[(int64_t)fast_div(from, a.by_block) * a.num_kv_heads];
   const float old = scales[(int64_t)to_block * a.num_kv_heads];
@@ -354,8 +362,7 @@ __global__ __launch_bounds__(64) void q8_compact_few_kernel(const Q8FewArgs a) {
     for (int i = lane; i < a.block_size * chunks; i += 64) {
       const int r = fast_div(i, a.by_chunks);
       uint4* const at = reinterpret_cast<uint4*>(pool + (block * a.block_size + r) * row_bytes + 16 * (i - r * chunks));
-      const uint4 w = *at;
-      *at = make_uint4(q8_rescale4(w.x, ratio), q8_rescale4(w.y, ratio), q8_rescale4(w.z, ratio), q8_rescale4(w.w, ratio));
+      *at = q8_rescale16(*at, ratio);
     }
   }
   stores_done();
@@ -368,8 +375,7 @@ __global__ __launch_bounds__(64) void q8_compact_few_kernel(const Q8FewArgs a) {
     const float ratio = __shfl(from_scale, row & 31) * q8_inverse(__shfl(scale, row & 31));
     if (row < n) {
       uint4 w = rows[p];
-      if (ratio < 1.f)
-        w = make_uint4(q8_rescale4(w.x, ratio), q8_rescale4(w.y, ratio), q8_rescale4(w.z, ratio), q8_rescale4(w.w, ratio));
+      if (ratio < 1.f) w = q8_rescale16(w, ratio);
       *reinterpret_cast<uint4*>(pool + slot * row_bytes + 16 * c) = w;
     }
   }
@@ -477,33 +483,47 @@ extern "C" int lvamd_kv_compact_q8(const uint64_t* layer_key_ptrs, const uint64_
 }
 
 extern "C" int64_t lvamd_kv_compact_q8_few_pairs(void) { return kFewPairs; }
+extern "C" int64_t lvamd_kv_compact_q8_few_call_pairs(void) { return kCallPairs; }
 
 extern "C" int lvamd_kv_compact_q8_few(const uint64_t* layer_key_ptrs, const uint64_t* layer_value_ptrs,
                                        int32_t num_layers, int32_t num_kv_heads, int32_t head_size, int32_t block_size,
                                        int64_t scale_offset, const int64_t* src_slots, const int64_t* dst_slots,
-                                       int64_t num_pairs, lvamd_stream_t stream) {
+                                       int64_t num_pairs, const int32_t* chunk_starts, int32_t num_chunks,
+                                       lvamd_stream_t stream) {
   if (!q8_head_size(head_size)) return LVAMD_ERR_UNSUPPORTED;
-  if (num_pairs < 0 || num_pairs > kFewPairs || num_layers <= 0 || num_kv_heads <= 0 || block_size <= 0 ||
-      scale_offset < 0 || scale_offset % 4 != 0 || (int64_t)block_size * (head_size / 16) > 0x7fffffffLL ||
-      (int64_t)num_layers * 2 * num_kv_heads > 0x7fffffffLL)
+  if (num_pairs < 0 || num_pairs > kCallPairs || num_chunks < 0 || num_chunks > kCallChunks || num_layers <= 0 ||
+      num_kv_heads <= 0 || block_size <= 0 || scale_offset < 0 || scale_offset % 4 != 0 ||
+      (int64_t)block_size * (head_size / 16) > 0x7fffffffLL || (int64_t)num_layers * 2 * num_kv_heads > 0x7fffffffLL)
     return LVAMD_ERR_INVALID_ARGUMENT;
   if (num_pairs == 0) return LVAMD_OK;
-  if (!layer_key_ptrs || !layer_value_ptrs || !src_slots || !dst_slots) return LVAMD_ERR_INVALID_ARGUMENT;
-  Q8FewArgs a{.by_block = FastDiv(block_size), .by_heads = FastDiv(num_kv_heads), .by_chunks = FastDiv(head_size / 16)};
-  for (int64_t i = 0; i < num_pairs; ++i) {
+  if (!layer_key_ptrs || !layer_value_ptrs || !src_slots || !dst_slots || !chunk_starts || num_chunks == 0)
+    return LVAMD_ERR_INVALID_ARGUMENT;
+  for (int c = 0; c < num_chunks; ++c) {
+    const int64_t pairs = (int64_t)chunk_starts[c + 1] - chunk_starts[c];
+    if (pairs < 1 || pairs > kFewPairs) return LVAMD_ERR_INVALID_ARGUMENT;
+  }
+  if (chunk_starts[0] != 0 || chunk_starts[num_chunks] != num_pairs) return LVAMD_ERR_INVALID_ARGUMENT;
+  for (int64_t i = 0; i < num_pairs; ++i)
     if (src_slots[i] < 0 || src_slots[i] > 0x7fffffffLL || dst_slots[i] < 0 || dst_slots[i] > 0x7fffffffLL)
       return LVAMD_ERR_INVALID_ARGUMENT;
-    a.src[i] = (int32_t)src_slots[i];
-    a.dst[i] = (int32_t)dst_slots[i];
-  }
-  a.layer_keys = layer_key_ptrs;
-  a.layer_values = layer_value_ptrs;
-  a.scale_offset = scale_offset;
-  a.num_pairs = (int32_t)num_pairs;
-  a.num_kv_heads = num_kv_heads;
-  a.head_size = head_size;
-  a.block_size = block_size;
-  hipLaunchKernelGGL(q8_compact_few_kernel, dim3((unsigned)(num_layers * 2 * num_kv_heads)), dim3(64), 0,
-                     static_cast<hipStream_t>(stream), a);
-  return launch_status();
+  auto launch = [&]<int PAIRS, int CHUNKS>() -> int {
+    Q8FewArgs<PAIRS, CHUNKS> a{
+        .by_block = FastDiv(block_size), .by_heads = FastDiv(num_kv_heads), .by_chunks = FastDiv(head_size / 16)};
+    for (int c = 0; c <= num_chunks; ++c) a.starts[c] = chunk_starts[c];
+    for (int64_t i = 0; i < num_pairs; ++i) {
+      a.src[i] = (int32_t)src_slots[i];
+      a.dst[i] = (int32_t)dst_slots[i];
+    }
+    a.layer_keys = layer_key_ptrs;
+    a.layer_values = layer_value_ptrs;
+    a.scale_offset = scale_offset;
+    a.num_kv_heads = num_kv_heads;
+    a.head_size = head_size;
+    a.block_size = block_size;
+    hipLaunchKernelGGL((q8_compact_few_kernel<PAIRS, CHUNKS>),
+                       dim3((unsigned)(num_layers * 2 * num_kv_heads), (unsigned)num_chunks), dim3(64), 0,
+                       static_cast<hipStream_t>(stream), a);
+    return launch_status();
+  };
+  return num_chunks == 1 ? launch.template operator()<kFewPairs, 1>() : launch.template operator()<kCallPairs, kCallChunks>();
 }

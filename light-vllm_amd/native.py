@@ -134,7 +134,8 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
         ctypes.c_int,
         [_p, _p, _i32, _i32, _i32, _i32, _i64, _p, _p, _i64, _p, _i64, _p, _i64, _p],
     ),
-    "lvamd_kv_compact_q8_few": (ctypes.c_int, [_p, _p, _i32, _i32, _i32, _i32, _i64, _p, _p, _i64, _p]),
+    "lvamd_kv_compact_q8_few": (ctypes.c_int, [_p, _p, _i32, _i32, _i32, _i32, _i64, _p, _p, _i64, _p, _i32, _p]),
+    "lvamd_kv_compact_q8_few_call_pairs": (_i64, []),
     "lvamd_kv_compact_q8_few_pairs": (_i64, []),
     "lvamd_kv_compact_q8_workspace_size": (_i64, [_i64, _i32, _i32, _i32]),
     "lvamd_verify_drafts": (

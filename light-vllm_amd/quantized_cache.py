@@ -102,6 +102,7 @@ class _State:
         lib = native.load()
         self.small_copies = int(lib.lvamd_kv_block_copy_small_pairs())
         self.few_pairs = int(lib.lvamd_kv_compact_q8_few_pairs())
+        self.call_pairs = int(lib.lvamd_kv_compact_q8_few_call_pairs())
         self.staging = Staging(device)
 
 
@@ -290,27 +291,29 @@ class QuantizedPagedKVCache:
         cfg = self._config
         moved, src, dst = _compact_bytes(cfg, requests)
         if src:
-            src, dst = bytes(src), bytes(dst)
-            twice, starts = native.host().block_runs(bytes(moved), dst, cfg.block_size)
+            src, dst, counts = bytes(src), bytes(dst), bytes(moved)
+            twice, starts = native.host().block_runs(counts, dst, cfg.block_size)
             if twice:
                 raise errors.KVCacheError("compact requests of one step must not write the same block of an 8-bit cache")
             with on_device(cfg.device):
-                self._launch_compact(src, dst, starts)
+                self._launch_compact(counts, src, dst, starts)
         return tuple(np.frombuffer(moved, dtype=np.int64).tolist())
 
-    def _launch_compact(self, src: bytes, dst: bytes, starts: bytes) -> None:
+    def _launch_compact(self, counts: bytes, src: bytes, dst: bytes, starts: bytes) -> None:
         state = self._state()
         cfg = self._config
         n, groups = len(src) // 8, len(starts) // 8 - 1
         lib = native.load()
         slots = cfg.num_blocks * cfg.block_size
         stream = current_stream(cfg.device)
-        if n <= state.few_pairs:
-            # A few pairs ride in the kernel arguments.
+        # A step's accepted drafts ride in the kernel arguments.
+        chunks = (native.host().compact_chunks(counts, src, dst, cfg.block_size, state.few_pairs)
+                  if n <= state.call_pairs else None)
+        if chunks is not None:
             for heads, size, layers, _, kptrs, vptrs in state.shapes:
                 native.check(lib.lvamd_kv_compact_q8_few(kptrs, vptrs, layers, heads, size, cfg.block_size,
-                                                         slots * heads * size, src, dst, n, stream),
-                             "lvamd_kv_compact_q8_few")
+                                                         slots * heads * size, src, dst, n, chunks, len(chunks) // 4 - 1,
+                                                         stream), "lvamd_kv_compact_q8_few")
             return
         buf = state.staging.buffer((len(src) + len(dst) + len(starts)) // 4)
         buf[:] = np.frombuffer(src + dst + starts, dtype=np.int32)

@@ -29,7 +29,8 @@ class DraftBatch:
     """The draft trees of one step's requests, on the device.
 
     Made when the step is built (one upload), used by ``verify_drafts`` once the
-    target's probabilities are there.  A request without drafts has an empty
+    target's probabilities are there (a graph that captured such a call reads
+    the batch's arrays: keep it as long).  A request without drafts has an empty
     tree.  Rows of probabilities are packed request by request: the root's (the
     distribution after the request's last formal token), then one per draft."""
 

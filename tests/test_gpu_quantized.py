@@ -602,6 +602,41 @@ def test_compact_matches_the_oracle(dtype, bs, shapes) -> None:
         _same(cache, state, layer_id)
 
 
+@pytest.mark.parametrize("requests,nodes", [(40, 5), (128, 5), (300, 5), (3, 45), (2, 20)])
+def test_compact_of_many_requests(requests, nodes) -> None:
+    """Chunks in one launch (33 to 384 pairs), the workspace's two launches (more,
+    or a request of more than 32 moved rows)."""
+    print(f"[gpu] q8 compact of {requests} requests, paths of {nodes}", file=sys.stderr, flush=True)
+    rng = np.random.default_rng(requests)
+    bs, n = 16, 2 * nodes
+    computed = [int(c) for c in rng.integers(0, 40, requests)]
+    need = [-(-(c + n) // bs) for c in computed]
+    free = [int(b) for b in rng.permutation(sum(need) + 3)]
+    tables = []
+    for m in need:
+        tables.append(tuple(free[:m]))
+        free = free[m:]
+    cache = _cache(4, 2, 64, bs, sum(need) + 3, torch.bfloat16, layers=2)
+    _fill(cache, requests)
+    src, dst, calls = [], [], []
+    for t, c in zip(tables, computed):
+        kept = (0, *sorted(rng.choice(np.arange(1, n), nodes - 1, replace=False).tolist()))
+        for i, j in enumerate(kept):
+            if i != j:
+                src.append(t[(c + j) // bs] * bs + (c + j) % bs)
+                dst.append(t[(c + i) // bs] * bs + (c + i) % bs)
+        calls.append(dict(block_ids=t, num_computed_tokens=c, num_query_tokens=n, num_reserved_query_tokens=n,
+                          retained_query_indices=kept, num_readonly_prefix_blocks=0))
+    want = {f"layer{i}": _state(cache, f"layer{i}") for i in range(2)}
+    for state in want.values():
+        for codes, scales in state:
+            Q.compact(codes, scales, src, dst)
+    assert sum(cache.compact_many(calls)) == len(src)
+    torch.cuda.synchronize()
+    for layer_id, state in want.items():
+        _same(cache, state, layer_id)
+
+
 def test_compact_refuses_a_block_of_two_requests() -> None:
     cache = _cache(4, 2, 64, 16, 4, torch.bfloat16)
     one = dict(block_ids=(0,), num_computed_tokens=2, num_query_tokens=3, num_reserved_query_tokens=3, retained_query_indices=(2,))

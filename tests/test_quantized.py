@@ -180,18 +180,47 @@ def test_compact_entry_point_checks() -> None:
 
 def test_compact_few_entry_point_checks() -> None:
     lib = native.load()
-    n = int(lib.lvamd_kv_compact_q8_few_pairs())
-    assert n == 32
-    pairs = np.arange(n + 1, dtype=np.int64)
+    assert int(lib.lvamd_kv_compact_q8_few_pairs()) == 32
+    most = int(lib.lvamd_kv_compact_q8_few_call_pairs())
+    assert most == 384
+    pairs = np.arange(most + 1, dtype=np.int64)
 
-    def call(keys=X, layers=2, heads=2, d=128, bs=16, offset=1024, src=pairs, dst=pairs, n=n):
-        return lib.lvamd_kv_compact_q8_few(keys, X, layers, heads, d, bs, offset, src.ctypes.data, dst.ctypes.data, n, None)
+    def call(keys=X, layers=2, heads=2, d=128, bs=16, offset=1024, src=pairs, dst=pairs, n=32, chunks=(0, 32), count=None):
+        starts = np.asarray(chunks, dtype=np.int32)
+        return lib.lvamd_kv_compact_q8_few(keys, X, layers, heads, d, bs, offset, src.ctypes.data, dst.ctypes.data, n,
+                                           starts.ctypes.data, len(starts) - 1 if count is None else count, None)
 
     assert call(n=0) == 0
     assert call(d=40) == -2
     for bad in (dict(keys=None), dict(layers=0), dict(heads=0), dict(bs=0), dict(offset=-4), dict(offset=2), dict(n=-1),
-                dict(n=n + 1), dict(src=pairs - 1), dict(dst=pairs + 2**31)):
+                dict(n=33), dict(n=33, chunks=(0, 33)), dict(n=33, chunks=(0, 32, 32, 33)), dict(n=33, chunks=(1, 33)),
+                dict(n=34, chunks=(0, 32, 33)), dict(n=32, count=0), dict(n=32, chunks=range(34), count=33),
+                dict(n=most + 1, chunks=(*range(0, most, 32), most, most + 1)), dict(src=pairs - 1), dict(dst=pairs + 2**31)):
         assert call(**bad) == -1, bad
+
+
+def test_compact_chunks() -> None:
+    chunks = native.host().compact_chunks
+    packed = lambda *slots: np.asarray(slots, dtype=np.int64).tobytes()  # noqa: E731
+
+    def cut(moved, src, dst, most=4, bs=16):
+        found = chunks(packed(*moved), packed(*src), packed(*dst), bs, most)
+        return None if found is None else np.frombuffer(found, dtype=np.int32).tolist()
+
+    assert cut((3, 0, 1), (5, 6, 7, 40), (2, 3, 4, 33)) == [0, 4]
+    assert cut((3, 2), (5, 6, 7, 40, 41), (2, 3, 4, 33, 34)) == [0, 3, 5]
+    assert cut((4, 4, 1), (5, 6, 7, 8, 37, 38, 39, 40, 70), (1, 2, 3, 4, 33, 34, 35, 36, 66)) == [0, 4, 8, 9]
+    assert cut((5,), (5, 6, 7, 8, 9), (1, 2, 3, 4, 5)) is None                                   # a longer request
+    assert cut((3, 2), (5, 6, 7, 40, 9), (2, 3, 4, 33, 34)) is None                              # reads a block the first writes
+    assert cut((3, 2), (5, 40, 7, 41, 42), (2, 3, 4, 33, 34)) is None                            # and the other way round
+    assert cut((3, 2), (5, 6, 7, 8, 9), (2, 3, 4, 0, 1)) is None                                 # both write one block
+    assert cut((2, 2), (5, 6, 8, 9), (2, 3, 0, 1)) == [0, 4]                                     # in one chunk that is no matter
+    assert cut((), (), ()) == [0, 0]
+    for bad in (((3,), (1, 2), (3, 4)), ((-1,), (1,), (2,))):
+        with pytest.raises(ValueError):
+            cut(*bad)
+    with pytest.raises(ValueError):
+        chunks(packed(1), packed(1, 2), packed(1), 16, 4)
 
 
 def test_block_runs() -> None:
@@ -221,3 +250,15 @@ def test_verify_entry_point_checks() -> None:
         assert call(**bad) == -1, bad
     need = lib.lvamd_verify_drafts_workspace_size(2, 3, 100, 0)
     assert need > 0 and call(nbytes=need - 1) == -3 and call(ws=None) == -3 and call(ws=ctypes.c_void_p(4)) == -3
+
+
+@pytest.mark.parametrize("kernel,count", [("q8_append_kernel", 2), ("q8_compact_few_kernel", 2), ("q8_gather_kernel", 1),
+                                          ("q8_scatter_kernel", 1), ("q8_decode_kernel", 60), ("q8_prefill_kernel", 68),
+                                          ("verify_sums_kernel", 6), ("verify_draw_kernel", 6)])
+def test_kernels_hold_their_registers(kernel, count) -> None:
+    pytest.importorskip("msgpack")
+    from test_kernel_resources import _kernels
+
+    found = {n: k for n, k in _kernels().items() if kernel in n}
+    assert len(found) == count
+    assert not {n for n, k in found.items() if k[".vgpr_spill_count"] or k[".private_segment_fixed_size"]}
