@@ -306,9 +306,14 @@ class QuantizedPagedKVCache:
         lib = native.load()
         slots = cfg.num_blocks * cfg.block_size
         stream = current_stream(cfg.device)
-        # A step's accepted drafts ride in the kernel arguments.
-        chunks = (native.host().compact_chunks(counts, src, dst, cfg.block_size, state.few_pairs)
-                  if n <= state.call_pairs else None)
+        # A step's accepted drafts ride in the kernel arguments: a few as one chunk
+        # (int32 starts 0 and n), more in chunks that do not touch each other.
+        if n <= state.few_pairs:
+            chunks = (n << 32).to_bytes(8, "little")
+        elif n <= state.call_pairs:
+            chunks = native.host().compact_chunks(counts, src, dst, cfg.block_size, state.few_pairs)
+        else:
+            chunks = None
         if chunks is not None:
             for heads, size, layers, _, kptrs, vptrs in state.shapes:
                 native.check(lib.lvamd_kv_compact_q8_few(kptrs, vptrs, layers, heads, size, cfg.block_size,
