@@ -525,5 +525,6 @@ extern "C" int lvamd_kv_compact_q8_few(const uint64_t* layer_key_ptrs, const uin
                        static_cast<hipStream_t>(stream), a);
     return launch_status();
   };
-  return num_chunks == 1 ? launch.template operator()<kFewPairs, 1>() : launch.template operator()<kCallPairs, kCallChunks>();
+  return num_chunks == 1 ? launch.template operator()<kFewPairs, 1>()
+                         : launch.template operator()<kCallPairs, kCallChunks>();
 }

@@ -98,10 +98,9 @@ __device__ __forceinline__ Q8Piece read_q8_piece(const int32_t* __restrict__ pie
 }  // namespace
 
 template <typename T, int D, bool APPEND>
-__global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(1, 1))) void q8_decode_kernel(const int32_t* __restrict__ wave_first,
-                                                       const int32_t* __restrict__ pieces, const int32_t waves_per_head,
-                                                       const uint32_t wg_magic, const int32_t wg_shift,
-                                                       const Q8DecodeArgs a) {
+__global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(1, 1))) void q8_decode_kernel(
+    const int32_t* __restrict__ wave_first, const int32_t* __restrict__ pieces, const int32_t waves_per_head,
+    const uint32_t wg_magic, const int32_t wg_shift, const Q8DecodeArgs a) {
   using S = Q8Tile<D>;
   constexpr int TT = S::TT, SUB = S::SUB, C8 = S::C8, CPR = S::CPR, RS = S::RS, LPT = S::LPT, SPL = S::SPL;
   constexpr int NCH = S::NCH, NT = S::NT;
@@ -485,10 +484,14 @@ __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(1, 1))) void
         const bool sees = (col.sees >> ((pos - cur.computed) & 31)) & 1u;
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-          const uint32_t nan =
-              APPEND ? q8_nan4_of<T>(*(const uint2*)((const T*)a.v_new + (int64_t)(cur.q_start + pos - cur.computed) * a.vn_tok_stride +
-                                                      kvh * a.vn_head_stride + 16 * n + 4 * g))
-                     : q8_nan4(*(gptr<const uint32_t>)(vbase + slot * row_bytes + 16 * n + 4 * g));
+          uint32_t nan;
+          if constexpr (APPEND) {  // (the token's own values: the codes' stores may be on their way)
+            const int64_t tok = cur.q_start + pos - cur.computed;
+            const T* const v = static_cast<const T*>(a.v_new) + tok * a.vn_tok_stride + kvh * a.vn_head_stride;
+            nan = q8_nan4_of<T>(*reinterpret_cast<const uint2*>(v + 16 * n + 4 * g));
+          } else {
+            nan = q8_nan4(*(gptr<const uint32_t>)(vbase + slot * row_bytes + 16 * n + 4 * g));
+          }
 #pragma unroll
           for (int r = 0; r < 4; ++r)
             if (sees && ((nan >> (8 * r + 7)) & 1u)) acc[n][r] = __uint_as_float(0x7fc00000u);
@@ -574,8 +577,9 @@ extern "C" int lvamd_paged_decode_q8(const void* q, int64_t q_token_stride, int6
                                      int64_t new_key_token_stride, int64_t new_key_head_stride, const void* new_value,
                                      int64_t new_value_token_stride, int64_t new_value_head_stride, void* key_pool,
                                      float* key_scales, void* value_pool, float* value_scales, void* out,
-                                     int64_t out_token_stride, int64_t out_head_stride, const int32_t* pieces, const int32_t* wave_first,
-                                     int32_t waves_per_head, const int32_t* tables, const uint32_t* vis, void* part_acc, float* part_ml,
+                                     int64_t out_token_stride, int64_t out_head_stride, const int32_t* pieces,
+                                     const int32_t* wave_first, int32_t waves_per_head, const int32_t* tables,
+                                     const uint32_t* vis, void* part_acc, float* part_ml,
                                      int64_t num_partial_slots, int32_t num_kv_heads, int32_t group, int32_t head_size,
                                      int32_t block_size, float scale, int32_t dtype, lvamd_stream_t stream) {
   if ((dtype != LVAMD_BF16 && dtype != LVAMD_F16) || !q8_head_size(head_size)) return LVAMD_ERR_UNSUPPORTED;

@@ -84,8 +84,12 @@ struct Q8PrefillShape {
 
 }  // namespace
 
+// (Waves per SIMD: what the registers and the resident workgroups allow.)
+constexpr int prefill_waves_per_eu(int d, int col_tiles, int waves) {
+  return waves == 4 ? (d <= 128 ? 2 : 1) : col_tiles == 1 && d <= 128 ? 4 : 2;
+}
 template <typename T, int D, int CT, int W>
-__global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(W == 4 ? (D <= 128 ? 2 : 1) : CT == 1 && D <= 128 ? 4 : 2))) void q8_prefill_kernel(
+__global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(prefill_waves_per_eu(D, CT, W)))) void q8_prefill_kernel(
     const int32_t* __restrict__ units, const int32_t num_kv_heads, const uint32_t heads_magic, const int32_t heads_shift,
     const Q8PrefillArgs a) {
   using P = Q8PrefillShape<D, CT, W>;
@@ -523,8 +527,12 @@ template <typename F>
 int dispatch_prefill(int dtype, int head_size, int columns, F f) {
   const bool bf16 = dtype == LVAMD_BF16;
   switch (columns) {
-    case 64: return bf16 ? with_prefill_head_size<__bf16, 1, 4>(head_size, f) : with_prefill_head_size<_Float16, 1, 4>(head_size, f);
-    case 128: return bf16 ? with_prefill_head_size<__bf16, 1, 8>(head_size, f) : with_prefill_head_size<_Float16, 1, 8>(head_size, f);
+    case 64:
+      return bf16 ? with_prefill_head_size<__bf16, 1, 4>(head_size, f)
+                  : with_prefill_head_size<_Float16, 1, 4>(head_size, f);
+    case 128:
+      return bf16 ? with_prefill_head_size<__bf16, 1, 8>(head_size, f)
+                  : with_prefill_head_size<_Float16, 1, 8>(head_size, f);
     default: return bf16 ? with_wide_head_size<__bf16>(head_size, f) : with_wide_head_size<_Float16>(head_size, f);
   }
 }

@@ -478,8 +478,8 @@ extern "C" int64_t lvamd_verify_drafts_workspace_size(int64_t num_requests, int6
 extern "C" int lvamd_verify_drafts(const void* target, int64_t target_row_stride, const void* draft_probs,
                                    int64_t draft_row_stride, int32_t vocab, int32_t dtype, const int32_t* draft_starts,
                                    const int64_t* draft_tokens, const int32_t* parents, const int32_t* siblings,
-                                   int64_t num_requests, int64_t num_drafts, const void* node_uniforms, const void* sample_uniforms,
-                                   int32_t uniforms_f64, int32_t* counts, int32_t* paths, int32_t path_width,
+                                   int64_t num_requests, int64_t num_drafts, const void* node_uniforms,
+                                   const void* sample_uniforms, int32_t uniforms_f64, int32_t* counts, int32_t* paths, int32_t path_width,
                                    int64_t* out_tokens, void* workspace, int64_t workspace_bytes,
                                    lvamd_stream_t stream) {
   if (dtype_size(dtype) == 0) return LVAMD_ERR_UNSUPPORTED;
