@@ -91,6 +91,34 @@ def test_vocabularies_of_a_few_tokens() -> None:
                 _compare(trees, target, node, sample, lv.verify_drafts(batch, target, node, sample, draft_probs=q), q)
 
 
+@pytest.mark.parametrize("vocab,dtype", [(600001, torch.float32), (1200007, torch.bfloat16)])
+def test_rows_of_many_chunks(vocab, dtype) -> None:
+    """More chunks than the draw holds in registers; draws all along the row."""
+    print(f"[gpu] verify vocab {vocab} {dtype}", file=sys.stderr, flush=True)
+    rng = np.random.default_rng(vocab)
+    gen = torch.Generator(device=DEV).manual_seed(vocab)
+    trees = _trees(rng, [2, 0, 1, 0], vocab, True)
+    batch = lv.DraftBatch(trees, device=DEV)
+    target, drafts = (_probs(gen, n, vocab, dtype) for n in (batch.num_rows, batch.num_drafts))
+    node = torch.rand(batch.num_rows, generator=gen, device=DEV, dtype=torch.float64)
+    for values in ((0.05, 0.3, 0.55, 0.8), (0.45, 0.9, 0.99, 0.9999)):
+        sample = torch.tensor(values, device=DEV, dtype=torch.float64)
+        for q in (None, drafts):
+            _compare(trees, target, node, sample, lv.verify_drafts(batch, target, node, sample, draft_probs=q), q)
+
+
+def test_many_requests() -> None:
+    print("[gpu] verify 5000 requests", file=sys.stderr, flush=True)
+    rng = np.random.default_rng(9)
+    gen = torch.Generator(device=DEV).manual_seed(9)
+    trees = _trees(rng, [int(n) for n in rng.integers(0, 4, 5000)], 2100, False)
+    batch = lv.DraftBatch(trees, device=DEV)
+    target = _probs(gen, batch.num_rows, 2100, torch.bfloat16, trees, 0.3)
+    node, sample = (torch.rand(n, generator=gen, device=DEV) for n in (batch.num_rows, 5000))
+    verdict = lv.verify_drafts(batch, target, node, sample)
+    _compare(trees, target, node, sample, verdict)
+
+
 def test_strided_rows() -> None:
     print("[gpu] verify strided rows", file=sys.stderr, flush=True)
     rng = np.random.default_rng(2)
