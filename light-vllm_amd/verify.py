@@ -29,13 +29,14 @@ class DraftBatch:
     """The draft trees of one step's requests, on the device.
 
     Made when the step is built (one upload), used by ``verify_drafts`` once the
-    target's probabilities are there (a graph that captured such a call reads
-    the batch's arrays: keep it as long).  A request without drafts has an empty
+    target's probabilities are there, on any stream that runs after the one it
+    was made on.  It may be dropped after the call (a graph that captured such a
+    call reads the batch's arrays: keep it as long).  A request without drafts has an empty
     tree.  Rows of probabilities are packed request by request: the root's (the
     distribution after the request's last formal token), then one per draft."""
 
     __slots__ = ("num_requests", "num_drafts", "num_rows", "path_width", "chains", "max_token", "counts", "device",
-                 "_blob", "_facts", "_verify")
+                 "_blob", "_stream", "_facts", "_verify")
 
     def __init__(self, drafts: Sequence[DraftTree], *, device: str | torch.device) -> None:
         self.device = torch.device(device)
@@ -51,6 +52,7 @@ class DraftBatch:
         self.path_width = max((1, *self.counts))
         sizes = [a.size for a in arrays]
         blob = self._blob = torch.from_numpy(np.concatenate(arrays)).to(self.device)
+        self._stream = _raw_stream(self.device.index)  # the allocator's, for the blob
         at = blob.data_ptr()
         # (Tokens first: int64, aligned.)
         tokens, starts, parents, siblings = (at + 4 * sum(sizes[:i]) for i in range(4))
@@ -136,6 +138,10 @@ def verify_drafts(batch: DraftBatch, target_probs: Tensor, node_uniforms: Tensor
         _refuse(batch, target_probs, node_uniforms, sample_uniforms, draft_probs, vocab)
     n, device = batch.num_requests, batch.device
     with on_device(device):
+        if _raw_stream(device.index) != batch._stream:
+            # The caller may drop the batch while the kernels are pending: its
+            # arrays are theirs until then.
+            batch._blob.record_stream(torch.cuda.current_stream(device))
         counts = torch.empty(n, dtype=torch.int32, device=device)
         paths = torch.empty((n, batch.path_width), dtype=torch.int32, device=device)
         tokens = torch.empty(n, dtype=torch.int64, device=device)

@@ -211,6 +211,30 @@ def test_captured_and_on_another_stream() -> None:
             _compare(trees, target, node, sample, lv.verify_drafts(batch, target, node, sample, draft_probs=drafts), drafts)
 
 
+def test_a_batch_dropped_behind_another_stream() -> None:
+    """The batch's arrays stay its own until a pending call on another stream has
+    read them: a tensor that asks for their memory meanwhile gets other memory."""
+    print("[gpu] verify, the batch dropped at once", file=sys.stderr, flush=True)
+    rng = np.random.default_rng(14)
+    gen = torch.Generator(device=DEV).manual_seed(14)
+    trees = _trees(rng, [5, 0, 7, 3], 1000, True)
+    batch = lv.DraftBatch(trees, device=DEV)
+    target = _probs(gen, batch.num_rows, 1000, torch.float32, trees, 0.6)
+    node, sample = torch.rand(batch.num_rows, generator=gen, device=DEV), torch.rand(4, generator=gen, device=DEV)
+    stream, blob = torch.cuda.Stream(), batch._blob
+    at, nbytes = blob.data_ptr(), 4 * blob.numel()
+    del blob
+    torch.cuda.synchronize()
+    with torch.cuda.stream(stream):
+        torch.cuda._sleep(50_000_000)
+        verdict = lv.verify_drafts(batch, target, node, sample)
+    del batch
+    others = [torch.zeros(nbytes, dtype=torch.uint8, device=DEV) for _ in range(4)]
+    assert at not in [t.data_ptr() for t in others]
+    torch.cuda.synchronize()
+    _compare(trees, target, node, sample, verdict)
+
+
 def test_refusals() -> None:
     batch = lv.DraftBatch([lv.DraftTree((5, 6), (-1, -1)), lv.DraftTree((), ())], device=DEV)
     assert len(batch) == 2 and batch.num_rows == 4 and not batch.chains
