@@ -153,6 +153,11 @@ def _require_gpu(cache) -> None:
         raise errors.KVCacheError("the HIP paged KV path requires a GPU KV cache")
 
 
+def _require_rows(cache) -> None:
+    if is_quantized(cache):
+        raise errors.KVCacheError("an 8-bit KV cache takes tokens by its own write_prepared")
+
+
 def hip_append(cache, layer_id: str, key: Tensor, value: Tensor, slots_ptr: int, num_tokens: int) -> None:
     """``flatK[slots[t]] = key[t]``, ``flatV[slots[t]] = value[t]`` on the current stream.
 
@@ -160,6 +165,7 @@ def hip_append(cache, layer_id: str, key: Tensor, value: Tensor, slots_ptr: int,
     (negative = skip), ``num_tokens`` of them.
     """
 
+    _require_rows(cache)
     layer = cache.layer(layer_id)
     spec = cache.layer_spec(layer_id)
     if key.stride(2) != 1 or value.stride(2) != 1:
@@ -188,6 +194,7 @@ def hip_append_rotary(cache, layer_id: str, query: Tensor, key: Tensor, value: T
     append: src/light_vllm/runtime/execution/paged_cache.py:209-248.
     """
 
+    _require_rows(cache)
     spec = cache.layer_spec(layer_id)
     cosines, sines = rotary
     tokens = query.shape[0]

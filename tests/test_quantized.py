@@ -105,6 +105,31 @@ def test_refusals_without_a_gpu() -> None:
     assert lv.quantized_kv_cache_bytes_per_block(mixed, block_size=16) == 2 * (2 * (16 * 64 + 4) + 16 * 128 + 4)
 
 
+def test_16_bit_appends_refuse_an_8_bit_cache() -> None:
+    # Their rows are twice as long as the pool's.  (Nothing to append: the calls
+    # reach no kernel either way.)
+    from light_vllm_amd import paged_cache
+
+    spec = lv.AttentionLayerSpec("a", 4, 2, 64)
+    rows = torch.zeros((0, 1, 2, 64), dtype=torch.bfloat16)
+
+    class Cache:
+        quantized = True
+
+        def layer(self, layer_id):
+            return lv.QuantizedPagedLayerCache(rows, rows, rows, rows)
+
+        def layer_spec(self, layer_id):
+            return spec
+
+    q, k = torch.zeros((0, 4, 64), dtype=torch.bfloat16), rows[:, 0]
+    angles = torch.zeros((0, 64), dtype=torch.bfloat16)
+    with pytest.raises(lv.KVCacheError, match="8-bit KV cache"):
+        paged_cache.hip_append(Cache(), "a", k, k, 0, 0)
+    with pytest.raises(lv.KVCacheError, match="8-bit KV cache"):
+        paged_cache.hip_append_rotary(Cache(), "a", q, k, k, (angles, angles), 0, 0)
+
+
 def test_append_entry_point_checks() -> None:
     lib = native.load()
 
