@@ -74,6 +74,16 @@ class QuantizedKVWriteMapping(PagedKVWriteMapping):
 
     geometry: tuple[int, int] = (0, 0)
 
+    def __post_init__(self) -> None:
+        # The launch reads them by address.
+        slots, sources = self.slots, self.source_indices
+        count = self.num_query_tokens if sources is None else sources.numel()
+        if not (all(t.ndim == 1 and t.dtype == torch.long and t.is_contiguous() and t.device == slots.device
+                    for t in (slots, sources) if t is not None)
+                and slots.numel() == count <= self.num_query_tokens):
+            raise errors.KVCacheError("slots and source indices of an 8-bit cache's mapping must be contiguous int64 "
+                                      "vectors on one device, one entry per token written")
+
 
 class _State:
     """Per-cache launch state: device tables of the layers' pool addresses by

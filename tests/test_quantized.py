@@ -5,6 +5,7 @@ refusals, and the C entry points' argument checks (before any HIP call)."""
 from __future__ import annotations
 
 import ctypes
+import dataclasses
 
 import numpy as np
 import pytest
@@ -128,6 +129,21 @@ def test_16_bit_appends_refuse_an_8_bit_cache() -> None:
         paged_cache.hip_append(Cache(), "a", k, k, 0, 0)
     with pytest.raises(lv.KVCacheError, match="8-bit KV cache"):
         paged_cache.hip_append_rotary(Cache(), "a", q, k, k, (angles, angles), 0, 0)
+
+
+def test_a_mappings_tensors_are_checked_where_it_is_made() -> None:
+    # The launch reads int64 slots, and as many sources, on the cache's device.
+    slots = torch.tensor([3, 4], dtype=torch.long)
+    good = lv.QuantizedKVWriteMapping(slots, 4, slots, (4, 16))
+    assert good.geometry == (4, 16)
+    lv.QuantizedKVWriteMapping(slots, 2, None, (4, 16))
+    for bad in ((slots.int(), 2, None), (slots.view(1, 2), 2, None), (slots, 3, None), (slots.repeat(2)[::2], 2, None),
+                (slots, 4, slots[:1]), (slots, 4, slots.int()), (slots, 4, slots.repeat(2)[::2]), (slots, 1, slots),
+                (slots, 4, slots.to("meta"))):
+        with pytest.raises(lv.KVCacheError, match="slots and source indices"):
+            lv.QuantizedKVWriteMapping(*bad, (4, 16))
+    with pytest.raises(lv.KVCacheError, match="slots and source indices"):
+        dataclasses.replace(good, source_indices=slots.to("meta"))
 
 
 def test_append_entry_point_checks() -> None:
