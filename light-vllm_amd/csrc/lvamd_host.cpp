@@ -2533,8 +2533,8 @@ typedef int (*VerifyFn)(const void*, int64_t, const void*, int64_t, int32_t, int
                         const int32_t*, const int32_t*, int64_t, int64_t, const void*, const void*, int32_t, int32_t*,
                         int32_t*, int32_t, int64_t*, void*, int64_t, void*);
 
-// 1: t is a contiguous vector of n of the dtype and device, 0: it is not, -1: a
-// Python error.
+// 1: t is a contiguous vector of n of the dtype and device (one element is
+// whatever its stride: contiguous() leaves that), 0: it is not, -1: a Python error.
 int vector_facts(PyObject* t, PyObject* dtype, long device, int64_t n, int64_t* ptr) {
   PyObject* dt = PyObject_GetAttr(t, g_str_dtype);
   if (dt == nullptr) return -1;
@@ -2552,7 +2552,7 @@ int vector_facts(PyObject* t, PyObject* dtype, long device, int64_t n, int64_t* 
   PyObject* stride = PyObject_CallMethodNoArgs(t, g_str_stride);
   if (stride == nullptr) return -1;
   const bool packed = PyTuple_Check(stride) && PyTuple_GET_SIZE(stride) == 1 &&
-                      PyLong_AsLongLong(PyTuple_GET_ITEM(stride, 0)) == 1;
+                      (n <= 1 || PyLong_AsLongLong(PyTuple_GET_ITEM(stride, 0)) == 1);
   Py_DECREF(stride);
   if (PyErr_Occurred()) return -1;
   if (!fits || !packed || at != device) return 0;

@@ -132,6 +132,20 @@ def test_strided_rows() -> None:
         _compare(trees, target, node, sample, lv.verify_drafts(batch, target, node, sample, draft_probs=q), q)
 
 
+def test_one_request_with_strided_uniforms() -> None:
+    """Vectors of one element keep their stride through ``contiguous()``."""
+    print("[gpu] verify one request, strided uniforms", file=sys.stderr, flush=True)
+    gen = torch.Generator(device=DEV).manual_seed(12)
+    for uniforms in (torch.float32, torch.float64):
+        for tree in (lv.DraftTree((5, 9), (-1, -1)), lv.DraftTree((), ())):
+            batch = lv.DraftBatch([tree], device=DEV)
+            target = _probs(gen, batch.num_rows, 33, torch.float32, [tree], 0.3)
+            node = torch.rand((batch.num_rows, 4), generator=gen, device=DEV, dtype=uniforms)[:, 1]
+            sample = torch.rand((1, 4), generator=gen, device=DEV, dtype=uniforms)[:, 2]
+            assert sample.stride() == (4,)
+            _compare([tree], target, node, sample, lv.verify_drafts(batch, target, node, sample))
+
+
 def test_rows_that_leave_nothing() -> None:
     print("[gpu] verify empty residuals", file=sys.stderr, flush=True)
     vocab = 300
