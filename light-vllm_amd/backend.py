@@ -107,10 +107,8 @@ def _rows_aligned(t: Tensor) -> bool:
 def _aligned(t: Tensor) -> Tensor:
     """``t``, or a copy of 16-byte aligned rows."""
 
-    if _rows_aligned(t):
-        return t
-    copy = t.contiguous()
-    return copy if _rows_aligned(copy) else copy.clone()
+    # (contiguous() leaves the strides of single tokens and heads as they are.)
+    return t if _rows_aligned(t) else t.clone(memory_format=torch.contiguous_format)
 
 
 def _partial_layout(work, spec, prefill_columns: int, element_size: int) -> tuple[int, int, int, int]:

@@ -378,10 +378,8 @@ def _aligned_rows(t: Tensor) -> Tensor:
     def fits(x: Tensor) -> bool:
         return x.stride(2) == 1 and x.data_ptr() % 16 == 0 and x.stride(0) % 8 == 0 and x.stride(1) % 8 == 0
 
-    if fits(t):
-        return t
-    copy = t.contiguous()
-    return copy if fits(copy) else copy.clone()
+    # (contiguous() leaves the strides of single tokens and heads as they are.)
+    return t if fits(t) else t.clone(memory_format=torch.contiguous_format)
 
 
 class on_device:

@@ -110,6 +110,23 @@ def test_append_skips_negative_slots_and_takes_strided_rows(validate) -> None:
     _write_and_compare(cache, packed[:0, 8:10], packed[:0, 10:], slots[:0], validate=validate)
 
 
+def test_one_token_of_an_odd_row() -> None:
+    """One token and one kv head: strides of single elements, which no copy of
+    theirs changes by itself, are no multiple of 16 bytes."""
+    print("[gpu] q8 one token, one kv head, odd strides", file=sys.stderr, flush=True)
+    gen = torch.Generator(device=DEV).manual_seed(31)
+    cache = _cache(1, 1, 32, 16, 3, torch.bfloat16)
+    x = _rows(gen, 1, 1, 133, torch.bfloat16).view(1, 133)
+    odd = x[:, None, :32]
+    assert odd.stride(1) % 8
+    _write_and_compare(cache, odd, odd, torch.tensor([17], device=DEV))
+    _write_and_compare(cache, x[:, None, 1:33], odd, torch.tensor([18], device=DEV))
+    cache, md, q, k, v = _step(1, 1, 32, 16, torch.bfloat16, [40], [1], seed=31)
+    want = lv.HipPagedAttentionBackend().create(cache, md).forward("layer0", odd.clone(), odd.clone(), odd.clone(), scale=0.2)
+    for views in ((odd, odd, odd), (odd, odd.contiguous().view(-1)[None, None], odd)):
+        assert torch.equal(lv.HipPagedAttentionBackend().create(cache, md).forward("layer0", *views, scale=0.2), want)
+
+
 def test_append_in_any_order_of_slots() -> None:
     print("[gpu] q8 append shuffled slots", file=sys.stderr, flush=True)
     gen = torch.Generator(device=DEV).manual_seed(6)
