@@ -16,8 +16,8 @@
 // zeros (p <= q everywhere by rounding) falls back to p.  Entries that are not
 // finite and positive count as zero; with nothing to draw from the token is -1.
 //
-// All sums are in fp64, so the drawn index does not depend on how they are
-// split (a sum's error, 1e-13, against the 1e-6 of a 150,000-token border).
+// All sums are in fp64: how they are split can change the drawn index only where
+// the number lies within their rounding error (1e-13 of the sum) of a border.
 //
 // HBM-bound in large batches: one row of p per request (and one of q), 16-byte
 // loads, several per lane in flight; a chain of round trips in small ones, over
@@ -189,7 +189,8 @@ __device__ __forceinline__ double wave_scan(double v, int lane) {
 template <bool DRAWN>
 struct WalkShared {
   float p[kMaxDrafts], q[DRAWN ? kMaxDrafts : 1];  // the drafts' own probabilities
-  int16_t sibling[kMaxDrafts], next[kMaxDrafts + 1];
+  int16_t next[kMaxDrafts + 1];                       // per node, the draft accepted there (plus one), or -1
+  int16_t after[DRAWN ? 1 : kMaxDrafts];              // per draft, the next sibling, or -1
   int32_t kids[kMaxDrafts];
   int node, num_kids, kid_draft;
 };
@@ -209,7 +210,7 @@ __device__ __forceinline__ Stop walk(const VerifyArgs& a, int req, bool leader, 
     s.node = s.num_kids = 0;
     s.kid_draft = -1;
   }
-  int parent[PER], token[PER];
+  int parent[PER], token[PER], sibling[PER];
   double u[PER];
   if (n > 0) {
 #pragma unroll
@@ -219,14 +220,18 @@ __device__ __forceinline__ Stop walk(const VerifyArgs& a, int req, bool leader, 
       const int64_t tok = a.tokens[first + c];
       token[i] = tok >= 0 && tok < a.vocab ? (int)tok : -1;
       parent[i] = a.parents[first + c] + 1;
-      s.sibling[c] = (int16_t)a.siblings[first + c];
+      sibling[i] = a.siblings[first + c];
       s.next[c] = -1;
+      if constexpr (!DRAWN) s.after[c] = -1;
     }
     if (threadIdx.x == 0) s.next[n] = -1;
+    if constexpr (!DRAWN) __syncthreads();
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
       const int c = threadIdx.x + THREADS * i;
       if (c >= n) break;
+      if constexpr (!DRAWN)
+        if (sibling[i] >= 0 && sibling[i] < c) s.after[sibling[i]] = (int16_t)c;
       const int64_t tok = max(token[i], 0);
       const float p = to_f32(target[(row0 + parent[i]) * a.target_stride + tok]);
       u[i] = uniform_at(a.node_uniforms, row0 + parent[i], a.uniforms_f64);
@@ -241,15 +246,20 @@ __device__ __forceinline__ Stop walk(const VerifyArgs& a, int req, bool leader, 
     for (int i = 0; i < PER; ++i) {
       const int c = threadIdx.x + THREADS * i;
       if (c >= n) break;
-      bool taken;
       if constexpr (DRAWN) {
-        taken = u[i] * (double)s.q[c] < (double)s.p[c];
-      } else {
-        double before = 0.0;
-        for (int k = s.sibling[c]; k >= 0; k = s.sibling[k]) before += (double)s.p[k];
-        taken = u[i] >= before && u[i] < before + (double)s.p[c];
+        if (u[i] * (double)s.q[c] < (double)s.p[c]) s.next[parent[i]] = (int16_t)(c + 1);
+      } else if (sibling[i] < 0 && u[i] >= 0.0) {
+        // A node's first child takes them all in order, so an interval's upper
+        // border is the next one's lower border bit for bit.
+        double upto = 0.0;
+        for (int k = c; k >= 0; k = s.after[k]) {
+          upto += (double)s.p[k];
+          if (u[i] < upto) {
+            s.next[parent[i]] = (int16_t)(k + 1);
+            break;
+          }
+        }
       }
-      if (taken) s.next[parent[i]] = (int16_t)(c + 1);
     }
     __syncthreads();
   }

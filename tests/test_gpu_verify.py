@@ -146,6 +146,29 @@ def test_one_request_with_strided_uniforms() -> None:
             _compare([tree], target, node, sample, lv.verify_drafts(batch, target, node, sample))
 
 
+def test_siblings_intervals_meet() -> None:
+    """Numbers on the borders between siblings and one step beside them, where the
+    sums of their probabilities round: each lies in one interval."""
+    print("[gpu] verify borders of siblings", file=sys.stderr, flush=True)
+    rng = np.random.default_rng(13)
+    k, requests = 6, 2000
+    trees = [lv.DraftTree(tuple(range(k)), (-1,) * k)] * requests
+    batch = lv.DraftBatch(trees, device=DEV)
+    probs = (rng.uniform(1, 2, (requests, k)) * np.exp2(-rng.integers(3, 45, (requests, k)))).astype(np.float32)
+    target = torch.zeros((requests, k + 1, k + 2), device=DEV)
+    target[:, 0, :k] = torch.from_numpy(probs).to(DEV)
+    target[..., k] = 0.25
+    target = target.view(-1, k + 2)
+    borders = np.cumsum(probs.astype(np.float64), axis=1)
+    sample = torch.full((requests,), 0.5, dtype=torch.float64, device=DEV)
+    for j in range(k):
+        for u in (borders[:, j], np.nextafter(borders[:, j], 0.0), np.nextafter(borders[:, j], 1.0)):
+            node = torch.zeros((requests, k + 1), dtype=torch.float64)
+            node[:, 0] = torch.from_numpy(u)
+            node = node.view(-1).to(DEV)
+            _compare(trees, target, node, sample, lv.verify_drafts(batch, target, node, sample))
+
+
 def test_rows_that_leave_nothing() -> None:
     print("[gpu] verify empty residuals", file=sys.stderr, flush=True)
     vocab = 300
