@@ -454,9 +454,12 @@ __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(1, 1))) void
     for (int s = 0; s < SUB; ++s)
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        const float pr = fast_exp2(st[s][r] + base);
-        l_run += pr;
-        pb[s >> 1][(s & 1) * 4 + r] = from_f32<T>(pr);
+        // The weights are rounded to T for the products with V; the sum that
+        // divides them counts them as rounded, so a weight's rounding moves the
+        // result by its share of v - out, not of v.
+        const T pr = from_f32<T>(fast_exp2(st[s][r] + base));
+        l_run += to_f32(pr);
+        pb[s >> 1][(s & 1) * 4 + r] = pr;
       }
     // ---- O^T += V^T P^T, V^T by transpose reads
     const char* vbytes = reinterpret_cast<const char*>(vlds);

@@ -377,6 +377,40 @@ def test_unit_width_rule() -> None:
         assert width(0, 2048) == width(14336, 1536) == width(14336, 2048, d=64) == width(14336, 2048, d=144) == 128
 
 
+@pytest.mark.parametrize("dtype", ("bf16", "fp16"))
+def test_weights_are_summed_as_they_are_multiplied(dtype) -> None:
+    """Values of 0.5 and 0.5625: the sum that divides is that of the rounded weights,
+    so a weight's rounding moves the result o by its share of v - o, not of v.
+
+    Bound: the output's rounding, half a step in [0.5, 1), which is u / 2; the
+    weights', u A with A = sum p |v - o| / sum p, and as in the module's bound 2^-12 A
+    for the scores; a few sums in fp32, 2^-20; and (1 + 2 u) for the divisor."""
+    print(f"[gpu] q8 attention, nearly equal values {dtype}", file=sys.stderr, flush=True)
+    t = DTYPES[dtype]
+    u = torch.finfo(t).eps / 2
+    for computed, layouts in (([0, 1, 2, 3, 4, 5, 6, 9] * 4, [1] * 32), ([1, 2, 70], [2, 1, 4]), ([0, 3, 500], [20, 30, 17])):
+        cache, md, q, k, v = _step(8, 4, 64, 16, t, computed, layouts, seed=32)
+        layer = cache.layer("layer0")
+        gen = torch.Generator(device=DEV).manual_seed(33)
+        pick = lambda shape: 0.5 + 0.0625 * torch.randint(0, 2, shape, generator=gen, device=DEV).float()  # noqa: E731
+        layer.values.copy_((pick(layer.values.shape) / layer.value_scales[:, None, :, None]).to(torch.float8_e4m3fn))
+        v = pick(v.shape).to(t)
+        want = _state(cache)
+        for (codes, scales), rows in zip(want, (k, v)):
+            Q.append(codes, scales, rows.double().cpu().numpy(), _slots(md, 16).tolist(), LARGEST[t])
+        out = lv.HipPagedAttentionBackend().create(cache, md).forward("layer0", q, k, v, scale=0.125).double().cpu().numpy()
+        keys, values = (codes * scales[:, None, :, None] for codes, scales in want)
+        args = (md.block_tables, md.num_computed_tokens, [l.parent_indices for l in md.query_layouts])
+        expect = O.dense_attention(q.double().cpu().numpy(), keys, values, *args, scale=0.125)
+        # sum p |v - o| / sum p: the share of 0.5625 is x = (o - 0.5) / 0.0625, so 2 x (1 - x) 0.0625.
+        assert expect.min() > 0.5 - 1e-12 and expect.max() < 0.5625 + 1e-12
+        x = (expect - 0.5) / 0.0625
+        bound = u / 2 + (1 + 2 * u) * (u + 2.0**-12) * 0.125 * x * (1 - x) + 2.0**-20
+        worst = float((np.abs(out - expect) / bound).max())
+        print(f"[margin] q8 nearly equal values: {100 * worst:.1f}% of the bound", file=sys.stderr, flush=True)
+        assert worst <= 1.0
+
+
 def test_long_tree_and_deep_split() -> None:
     print("[gpu] q8 attention trees of 40 and 70 queries, one long sequence", file=sys.stderr, flush=True)
     rng = np.random.default_rng(8)
