@@ -556,7 +556,8 @@ int lvamd_paged_decode_q8_resident_waves(int32_t dtype, int32_t head_size);
  * Prefill and tree attention over an 8-bit cache that holds the step's tokens
  * already: lvamd_paged_prefill's unit records, of up to `columns` columns (128;
  * 64 where every request has at most 64; 256 for head sizes 80 ... 128), and
- * partials, [slots][num_kv_heads][columns], the rows in fp32.
+ * partials, [slots][num_kv_heads][columns], the rows in fp32.  scale must be
+ * positive.
  */
 int lvamd_paged_prefill_q8(const void* q, int64_t q_token_stride, int64_t q_head_stride,
                            const void* key_pool, const float* key_scales,
@@ -598,7 +599,8 @@ typedef struct lvamd_attention_plan_q8 {
  * append (unless new_key / new_value are NULL), then the decode, merge, prefill
  * and merge launches.  A query attends what the cache holds, its own token's
  * stored K and V included.  With slots NULL the decode launch appends; there
- * must be no prefill units then.  Arguments as lvamd_paged_attention.
+ * must be no prefill units then.  With prefill units scale must be positive.
+ * Arguments as lvamd_paged_attention.
  */
 int lvamd_paged_attention_q8(const lvamd_attention_plan_q8* plan,
                              const void* q, int64_t q_token_stride, int64_t q_head_stride,

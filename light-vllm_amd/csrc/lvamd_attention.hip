@@ -69,6 +69,7 @@ extern "C" int lvamd_paged_attention_q8(const lvamd_attention_plan_q8* plan,
   int status = LVAMD_OK;
   const bool fused = new_key && !plan->slots;
   if (fused && p.num_units > 0) return LVAMD_ERR_INVALID_ARGUMENT;
+  if (p.num_units > 0 && !(scale > 0.f)) return LVAMD_ERR_INVALID_ARGUMENT;  // (before anything is appended)
   if (new_key && !fused) {
     status = lvamd_kv_append_q8(new_key, new_key_token_stride, new_key_head_stride, new_value, new_value_token_stride,
                                 new_value_head_stride, key_pool, key_scales, value_pool, value_scales, plan->slots,

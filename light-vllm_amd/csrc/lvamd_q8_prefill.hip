@@ -573,6 +573,8 @@ extern "C" int lvamd_paged_prefill_q8(const void* q, int64_t q_token_stride, int
   if (num_units < 0 || num_kv_heads <= 0 || group <= 0 || block_size <= 0 || num_partial_slots < 0)
     return LVAMD_ERR_INVALID_ARGUMENT;
   if (num_units == 0) return LVAMD_OK;
+  // (The running maximum is taken of the unscaled scores, masked ones -inf.)
+  if (!(scale > 0.f)) return LVAMD_ERR_INVALID_ARGUMENT;
   if (!q || !key_pool || !key_scales || !value_pool || !value_scales || !out || !tables || !vis || !units)
     return LVAMD_ERR_INVALID_ARGUMENT;
   if (num_partial_slots > 0 && (!part_acc || !part_ml)) return LVAMD_ERR_WORKSPACE;

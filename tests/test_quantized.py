@@ -203,6 +203,19 @@ def test_attention_entry_point_checks() -> None:
     assert call(ctypes.addressof(plan)) == -1
 
 
+def test_prefill_takes_a_positive_scale_only() -> None:
+    # Its running maximum is that of the unscaled scores, its masked ones -inf.
+    lib = native.load()
+    units = native.AttentionPlanQ8(base=native.AttentionPlan(num_units=1, num_kv_heads=4, group=7, head_size=128, block_size=16,
+                                                             dtype=2, prefill_col_tiles=8))
+    empty = (None, 0, 0, None, 0, 0)
+    for scale in (0.0, -0.125, float("nan")):
+        f = ctypes.c_float(scale)
+        assert lib.lvamd_paged_prefill_q8(X, 3584, 128, X, X, X, X, X, 3584, 128, X, X, X, 1, None, None, 0, 4, 7, 128, 128, 16, f,
+                                          2, None) == -1
+        assert lib.lvamd_paged_attention_q8(ctypes.addressof(units), X, 3584, 128, *empty, X, X, X, 3584, 128, f, None) == -1
+
+
 def test_compact_entry_point_checks() -> None:
     lib = native.load()
 
