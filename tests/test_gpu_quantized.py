@@ -178,6 +178,30 @@ def test_token_by_token_append_equals_the_whole_prompt() -> None:
     _same(one, _state(whole))
 
 
+def _bound(rows, scale):
+    """What the cache states of a row's error at its block's scale."""
+    return 2.0**-4 * rows.abs() + 2.0**-9 * scale
+
+
+@pytest.mark.parametrize("dtype", ("bf16", "fp16"))
+def test_growing_scales_stay_within_the_stated_bound(dtype) -> None:
+    # A token at a time, each larger than those before: codes become subnormal.
+    print(f"[gpu] q8 append, growing scales {dtype}", file=sys.stderr, flush=True)
+    t = DTYPES[dtype]
+    gen = torch.Generator(device=DEV).manual_seed(34)
+    cache = _cache(8, 4, 64, 16, 2, t)
+    size = torch.exp2(torch.rand((16, 4, 1), generator=gen, device=DEV).mul(14).sort(dim=0).values)
+    x = ((torch.rand((16, 4, 64), generator=gen, device=DEV) * 2 - 1) * size).to(t)
+    for i in range(16):
+        _write_and_compare(cache, x[i : i + 1], x[i : i + 1].flip(2), torch.tensor([i], device=DEV))
+    layer = cache.layer("layer0")
+    for codes, scales, rows in ((layer.keys, layer.key_scales, x), (layer.values, layer.value_scales, x.flip(2))):
+        scale = scales[0, :, None]
+        err = (codes[0].float() * scale - rows.float()).abs()
+        assert float((err / _bound(rows.float(), scale)).max()) < 1.0
+        assert float((err / _bound(rows.float(), 0 * scale)).nan_to_num().max()) > 1.0  # (the second term counts)
+
+
 def test_write_refusals() -> None:
     cache = _cache(4, 2, 64, 16, 4, torch.bfloat16)
     x = torch.zeros((2, 2, 64), dtype=torch.bfloat16, device=DEV)

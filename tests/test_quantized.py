@@ -48,6 +48,26 @@ def test_token_at_a_time_gives_what_a_whole_prompt_gives() -> None:
     np.testing.assert_array_equal(os_, ws)
 
 
+def test_growing_scales_stay_within_the_stated_bound() -> None:
+    """A row is rounded when it is written (half a step of its value, 2^-4 of it, or
+    half the smallest subnormal code, 2^-10 of the scale then) and again at each
+    growth that makes its code subnormal: 2^-10 of scales that at least double, in
+    all less than 2^-9 of the last one.  One rounding's bound does not hold."""
+    rng = np.random.default_rng(3)
+    worst = one_rounding = 0.0
+    for _ in range(100):
+        sizes = np.exp2(np.sort(rng.uniform(0, 14, 12)))
+        rows = rng.uniform(-1, 1, (12, 1, 64)) * sizes[:, None, None]
+        rows[:, 0, 0] = sizes
+        codes, scales = np.zeros((1, 16, 1, 64)), np.full((1, 1), 2.0**-100)
+        for i in range(12):
+            Q.append(codes, scales, rows[i : i + 1], [i], 1.875 * 2.0**127)
+        err = np.abs(codes[0, :12] * scales[0, 0] - rows)
+        worst = max(worst, float((err / (2.0**-4 * np.abs(rows) + 2.0**-9 * scales[0, 0])).max()))
+        one_rounding = max(one_rounding, float((err / np.maximum(2.0**-4 * np.abs(rows), 2.0**-10 * scales[0, 0])).max()))
+    assert worst < 1.0 < one_rounding
+
+
 @pytest.mark.parametrize("mode", ("chain", "tree"))
 def test_verified_tokens_follow_the_target(mode) -> None:
     # The first emitted token over a grid of uniforms (and, for the chain, every
