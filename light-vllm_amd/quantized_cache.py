@@ -13,8 +13,9 @@ exponent (at least -100) that brings the largest finite magnitude of the rows
 within 448, e4m3's largest.  A block that is written at its offset 0 starts
 anew; later rows can only raise its scale, and then the block's other rows are
 re-scaled, which a power of two makes exact (unless a code becomes subnormal):
-a token at a time gives the codes that a whole prompt gives.  Non-finite values
-are stored as NaN and do not count for the scale.
+a token at a time gives the codes that a whole prompt gives.  Every row written
+since offset 0 counts, a rejected draft's too: ``compact`` keeps the scale.
+Non-finite values are stored as NaN and do not count for the scale.
 """
 
 from __future__ import annotations

@@ -3,8 +3,8 @@
 light-vllm verifies draft trees greedily: a draft is accepted when it is the
 target's most likely token (``GreedyTreeAcceptanceSampler``,
 src/light_vllm/runtime/execution/speculative.py:220-257).  ``verify_drafts``
-verifies them for sampled decoding: the tokens that come out follow the target's
-distribution, whatever was drafted.  It runs in the gfx950 kernels of
+verifies them for sampled decoding: the tokens that come out follow the given
+target probabilities, whatever was drafted.  It runs in the gfx950 kernels of
 ``liblvamd_hip.so`` on the device's probabilities; the random numbers are the
 caller's.
 """

@@ -202,6 +202,39 @@ def test_growing_scales_stay_within_the_stated_bound(dtype) -> None:
         assert float((err / _bound(rows.float(), 0 * scale)).nan_to_num().max()) > 1.0  # (the second term counts)
 
 
+def test_a_rejected_drafts_scale_stays() -> None:
+    """A draft that is far larger than the history of its block raises the block's
+    scale for all its rows, and its rejection does not lower it: the history keeps
+    the stated bound, at that scale.  Other blocks and heads are as they were."""
+    print("[gpu] q8 a rejected draft of 2^14", file=sys.stderr, flush=True)
+    gen = torch.Generator(device=DEV).manual_seed(35)
+    cache = _cache(4, 2, 64, 16, 3, torch.bfloat16)
+    x = torch.randn((26, 2, 64), generator=gen, device=DEV).to(torch.bfloat16)
+    cache.write("layer0", x, x, torch.arange(26, device=DEV))
+    layer = cache.layer("layer0")
+    before = [t.clone() for t in (layer.keys.float(), layer.key_scales)]
+    drafts = torch.randn((3, 2, 64), generator=gen, device=DEV).to(torch.bfloat16)
+    drafts[2, 0, 7] = 2.0**14
+    md = lv.PagedAttentionMetadata(block_tables=((0, 1),), num_computed_tokens=(26,), query_layouts=(lv.QueryLayout((-1, 0, 0)),))
+    q = torch.randn((3, 4, 64), generator=gen, device=DEV).to(torch.bfloat16)
+    want = _state(cache)
+    for codes, scales in want:
+        Q.append(codes, scales, drafts.double().cpu().numpy(), [26, 27, 28], LARGEST[torch.bfloat16])
+    out = lv.HipPagedAttentionBackend().create(cache, md).forward("layer0", q, drafts, drafts, scale=0.125)
+    _same(cache, want)
+    _check(out[:2], *(e[:2] for e in _expected(cache, md, q, want)), torch.bfloat16)
+    assert cache.compact(block_ids=(0, 1), num_computed_tokens=26, num_query_tokens=3, num_reserved_query_tokens=3,
+                         retained_query_indices=(0, 1)) == 0
+    torch.cuda.synchronize()
+    scale = layer.key_scales
+    assert float(scale[1, 0]) == 64.0 and float(scale[1, 1]) == float(before[1][1, 1])
+    assert torch.equal(scale[0], before[1][0]) and torch.equal(layer.keys.float()[0], before[0][0])
+    held = layer.keys[1, :10].float() * scale[1][None, :, None]
+    err = (held - x[16:].float()).abs()
+    assert float((err / _bound(x[16:].float(), scale[1][None, :, None])).max()) < 1.0
+    assert float(err[:, 0].max()) > 0.03125  # the price: steps of 2^-9 x 64 instead of 2^-9 x 2^-6
+
+
 def test_write_refusals() -> None:
     cache = _cache(4, 2, 64, 16, 4, torch.bfloat16)
     x = torch.zeros((2, 2, 64), dtype=torch.bfloat16, device=DEV)
