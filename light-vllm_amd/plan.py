@@ -26,6 +26,7 @@ and goes through a pinned staging buffer that is reused step after step
 
 from __future__ import annotations
 
+import collections
 from dataclasses import dataclass
 
 import numpy as np
@@ -90,6 +91,18 @@ def current_stream(device: torch.device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
 
 
+# (event, buffer) of rings that were dropped while a graph was captured.
+_LEFT: collections.deque = collections.deque()
+
+
+def _free_left() -> None:
+    """Drop what ``_LEFT`` holds, once its copies have finished."""
+
+    while _LEFT and not torch.cuda.is_current_stream_capturing():
+        event, _host = _LEFT.popleft()  # (held until its copy is done)
+        event.synchronize()
+
+
 class Staging:
     """Pinned host buffers for per-step uploads, reused round-robin.
 
@@ -98,6 +111,10 @@ class Staging:
     buffer waits for the previous copy, cuda_staging.py:27-49); with several
     buffers in the ring that wait is normally already over.  On a CPU device
     the arrays are handed over as CPU tensors (the planner's tests).
+
+    Dropping a ring (a backend, or a cache that moved rows) waits for its pending
+    uploads; dropped while a graph is captured, which no host wait may interrupt,
+    it leaves its buffers to the next ring's first use.
     """
 
     DEPTH = 4
@@ -113,12 +130,16 @@ class Staging:
         self._next = 0
         self._slot = -1
 
-    def __del__(self) -> None:
+    def __del__(self, _left=_LEFT) -> None:
         # The copies are the library's: torch's pinned allocator does not know of
         # them and would hand a freed buffer out again while one still reads it.
-        for event in getattr(self, "_events", ()):
-            if event is not None:
-                event.synchronize()
+        pending = [(event, host) for event, host in zip(getattr(self, "_events", ()), getattr(self, "_host", ()))
+                   if event is not None]
+        if pending and torch.cuda.is_current_stream_capturing():
+            _left.extend(pending)
+            return
+        for event, _ in pending:
+            event.synchronize()
 
     def take(self, n: int = 0) -> np.ndarray:
         """The next buffer of the ring, whole (at least ``n`` int32 entries),
@@ -142,6 +163,7 @@ class Staging:
 
         if not self._gpu:
             return np.zeros(max(n, self.MIN_ENTRIES), dtype=np.int32)
+        _free_left()
         slot = self._slot
         old = self._host[slot]
         size = max(n, self.MIN_ENTRIES, 2 * old.numel() if old is not None else 0)

@@ -55,3 +55,28 @@ def test_a_dropped_staging_ring_has_finished_its_copies() -> None:
     del ring, buf
     assert event.query()  # waited for
     assert bool((dev == 7).all())
+
+
+def test_a_ring_dropped_in_a_capture_leaves_it_whole() -> None:
+    print("[gpu] a staging ring dropped while a graph is captured", file=sys.stderr, flush=True)
+    from light_vllm_amd import plan
+
+    ring = Staging(DEV)
+    buf = ring.buffer(1024)
+    buf[:] = 7
+    dev = ring.upload(buf).float()
+    del buf
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        twice = dev * 2
+        del ring
+        out = twice + 1
+    assert len(plan._LEFT) == 1
+    for i in range(3):
+        dev.fill_(float(i))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert bool((out == 2.0 * i + 1).all())
+    Staging(DEV).buffer(16)  # the next ring's first use frees it
+    assert not plan._LEFT

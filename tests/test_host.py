@@ -1333,3 +1333,30 @@ def test_attend_tensors_passes_the_tensors_and_refuses_what_the_fast_path_cannot
     assert host.attend_tensors(other_device, *pools, 0x4000, q, k, v, 0.5) == not_fast
     with pytest.raises(ValueError):
         host.attend_tensors(shape[:11], *pools, 0x4000, q, k, v, 0.5)
+
+
+@pytest.mark.parametrize("capturing", (False, True))
+def test_a_dropped_staging_ring_waits_but_not_in_a_capture(monkeypatch, capturing) -> None:
+    from light_vllm_amd import plan
+
+    waited = []
+
+    class Event:
+        def synchronize(self):
+            assert not torch.cuda.is_current_stream_capturing()
+            waited.append(self)
+
+    state = {"capturing": capturing}
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: state["capturing"])
+    ring, events = Staging(CPU), [Event(), Event()]
+    ring._events[:2], ring._host[:2] = events, [torch.zeros(4), torch.zeros(4)]
+    kept = ring._host[1].data_ptr()
+    ring.__del__()
+    ring._events = []  # (its own end finds nothing more)
+    assert waited == ([] if capturing else events)
+    assert [h.data_ptr() for _, h in plan._LEFT][1:] == ([kept] if capturing else [])
+    plan._free_left()
+    assert len(plan._LEFT) == (2 if capturing else 0)
+    state["capturing"] = False
+    plan._free_left()
+    assert waited == events and not plan._LEFT
