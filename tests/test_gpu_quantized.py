@@ -476,6 +476,40 @@ def test_long_tree_and_deep_split() -> None:
     _attend_and_check(*_step(7, 1, 128, 16, torch.bfloat16, [9000, 20], [1, 1], seed=10), torch.bfloat16)
 
 
+@pytest.mark.parametrize("seed", range(24))
+def test_random_steps(seed) -> None:
+    """Any mix of decode rows, runs, prompts and trees, over any head layout, block
+    size and shared prefix; and the same bits when it runs again."""
+    rng = np.random.default_rng(1000 + seed)
+    hkv = int(rng.integers(1, 6))
+    group = int(rng.choice([1, 2, 3, 4, 7, 8, 16, 17, 40]))
+    d, bs = 16 * int(rng.integers(2, 17)), int(rng.choice([1, 3, 8, 16, 16, 32, 64, 100, 128]))
+    dtype = (torch.bfloat16, torch.float16)[seed % 2]
+    n = int(rng.integers(1, 9))
+    prefix = int(rng.integers(0, 4)) if rng.random() < 0.3 else 0
+    computed = [prefix * bs + int(np.exp2(rng.uniform(0, 10.5))) - 1 for _ in range(n)]
+    layouts = []
+    for _ in range(n):
+        m = int(np.exp2(rng.uniform(0, 7.5)))
+        kind = rng.random()
+        layouts.append(1 if kind < 0.4 else m if kind < 0.7 else
+                       tuple([-1] + [int(rng.integers(max(-1, i - 9), i)) for i in range(1, m)]))
+    print(f"[gpu] q8 random step {seed}: {hkv * group}/{hkv}x{d} bs {bs} {dtype} prefix {prefix} {computed} "
+          f"{[x if isinstance(x, int) else -len(x) for x in layouts]}", file=sys.stderr, flush=True)
+    cache, md, q, k, v = _step(hkv * group, hkv, d, bs, dtype, computed, layouts, seed=seed, prefix=prefix)
+    layer = cache.layer("layer0")
+    parts = (layer.keys.view(torch.uint8), layer.key_scales, layer.values.view(torch.uint8), layer.value_scales)
+    before = [p.clone() for p in parts]
+    out = _attend_and_check(cache, md, q, k, v, dtype)
+    after = [p.clone() for p in parts]
+    for p, b in zip(parts, before):
+        p.copy_(b)
+    again = lv.HipPagedAttentionBackend().create(cache, md).forward("layer0", q, k, v, scale=1.0 / math.sqrt(d))
+    assert torch.equal(again.view(torch.int16), out.view(torch.int16))
+    for p, b in zip(parts, after):
+        assert torch.equal(p, b)
+
+
 def test_shared_prefix_spans_and_options() -> None:
     print("[gpu] q8 attention shared prefix", file=sys.stderr, flush=True)
     args = _step(12, 2, 128, 16, torch.bfloat16, [256 + 5 * i for i in range(6)], [TREE] * 6, seed=11, prefix=16)
