@@ -129,6 +129,10 @@ def verify_drafts(batch: DraftBatch, target_probs: Tensor, node_uniforms: Tensor
     token is drawn from what is left there: p without the children's tokens, or
     max(p - q, 0); p itself where nothing is left.  A row with no positive
     probability gives token -1.  Sums are in fp64.
+
+    A probability that accepts a draft counts as given, the draw divides by the
+    sum of what is left: where a row does not sum to one (by the rounding of fp16
+    or bf16 rows, say), the tokens' distribution is off by as much.
     """
 
     vocab = target_probs.shape[1] if isinstance(target_probs, Tensor) and target_probs.ndim == 2 else 0
