@@ -194,15 +194,15 @@ __global__ __launch_bounds__(64 * kAppendWaves) void q8_append_kernel(const int6
 
 // ---------------------------------------------------------------------------
 // Compact of accepted rows that the kernel after this one does not take (more
-// pairs, a request of more than 32, tables that share blocks), two launches: the first copies every pair's row
-// (codes and its block's scale, for every layer, K and V) to the workspace,
-// the second writes them.  Pairs come grouped by destination block; one wave
+// pairs, a request of more than 32, tables that share blocks), two launches: the
+// first copies every pair's row (codes and its block's scale, for every layer, K
+// and V) to the workspace, the second writes them.  Pairs come grouped by destination block; one wave
 // per (destination block, layer, K or V, kv head) takes the larger of the
 // block's scale and those its rows come with, re-scales the block's rows if
 // that is above its own, then writes the moved rows at it.  (Every source is
 // read before any block changes: a source's block may be another's
-// destination.)  Latency-bound: 128 requests' rows of 12 layers, 2 kv heads, D =
-// 128 (4.5 MB) take 3.1 + 4.4 us.
+// destination.)  Latency-bound: 145 rows of 128 requests, 12 layers, 2 kv heads,
+// D = 128 (1.8 MB read and written) take 3.1 + 4.4 us.
 // ---------------------------------------------------------------------------
 struct Q8CompactArgs {
   const uint64_t* layer_keys;
@@ -292,7 +292,7 @@ __global__ __launch_bounds__(64 * kAppendWaves) void q8_scatter_kernel(const int
 // 16 per lane and pass) before it writes any.  Lane i has pair i's slots and
 // scales; a segmented scan gives each destination block's new scale.  A chain of
 // three round trips (scales and rows, re-scaled rows, stores): 3.4 us for one
-// request's rows of 12 layers, 4.2 for those of 128, against 7.5 in two launches
+// row of 12 layers, 4.2 for 145 of 128 requests, against 7.5 in two launches
 // behind an upload (a call of 128 requests 28.5 us against 41).
 // ---------------------------------------------------------------------------
 constexpr int kFewPairs = 32;     // of a chunk

@@ -36,8 +36,8 @@
 //     (poison, below; code that no ordinary step enters).
 //
 // HBM-bound in long steps, a chain of dependent round trips in short ones.  28
-// heads over 4, D = 128: 64 sequences of 512-4095 tokens (bf16) 33 us for 159 MB,
-// 4.8 TB/s; 16 of 32767 (fp16) 88 us for 537 MB, 6.1 TB/s.  4 sequences of
+// heads over 4, D = 128: 64 sequences of 512-4095 tokens (bf16) 34 us for 159 MB,
+// 4.7 TB/s; 16 of 32767 (fp16) 86-91 us for 537 MB, 5.9-6.2 TB/s.  4 sequences of
 // 37-511 tokens, 14 heads over 2, D = 64: 8 us with the append.
 
 #include <cmath>
@@ -454,7 +454,9 @@ __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(1, 1))) void
     for (int s = 0; s < SUB; ++s)
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        // The weights are rounded to T for the products with V; the sum that
+        // The weights are rounded to T for the products with V (a matrix
+        // instruction's operands are of one type; bf16 output is off by 1.3 times
+        // its own rounding in all, twice the products would spare 0.3); the sum that
         // divides them counts them as rounded, so a weight's rounding moves the
         // result by its share of v - out, not of v.
         const T pr = from_f32<T>(fast_exp2(st[s][r] + base));

@@ -28,8 +28,8 @@
 // The second launch is one wave per request, without a barrier: it scans the
 // chunks' sums, then the one chunk that holds the draw.
 //
-// One request of 4 drafts, 151,936 tokens, fp32 with q: 4.8 + 4.0 us.  128 trees
-// over 100,003 tokens, bf16: 12.5 + 4.8 us for 26 MB, of which the walk's two
+// One request of 4 drafts, 151,936 tokens, fp32 with q: 4.9 + 4.0 us.  128 trees
+// over 100,003 tokens, bf16: 12.9 + 4.8 us for 26 MB, of which the walk's two
 // rounds of loads take about 4.  One launch of a workgroup per request won 1-2 us
 // below 1000 tokens and lost up to four times at 151,936 (one CU then converts
 // and adds every element).
