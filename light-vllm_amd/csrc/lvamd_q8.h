@@ -136,4 +136,38 @@ __device__ __forceinline__ uint4 q8_without_nan16(uint4 c) {
 // cover all 64 banks evenly.
 constexpr int q8_row_stride(int chunks) { return chunks + (chunks % 4 == 0 ? 2 : 0); }
 
+// ---- host: the types and head sizes that the attention kernels are built for
+inline bool q8_head_size(int d) { return d >= 32 && d <= 256 && d % 16 == 0; }
+
+template <typename T, typename F>
+int q8_with_head_size(int head_size, F& f) {
+  switch (head_size) {
+    case 32: return f.template operator()<T, 32>();
+    case 48: return f.template operator()<T, 48>();
+    case 64: return f.template operator()<T, 64>();
+    case 80: return f.template operator()<T, 80>();
+    case 96: return f.template operator()<T, 96>();
+    case 112: return f.template operator()<T, 112>();
+    case 128: return f.template operator()<T, 128>();
+    case 144: return f.template operator()<T, 144>();
+    case 160: return f.template operator()<T, 160>();
+    case 176: return f.template operator()<T, 176>();
+    case 192: return f.template operator()<T, 192>();
+    case 208: return f.template operator()<T, 208>();
+    case 224: return f.template operator()<T, 224>();
+    case 240: return f.template operator()<T, 240>();
+    case 256: return f.template operator()<T, 256>();
+    default: return LVAMD_ERR_UNSUPPORTED;
+  }
+}
+template <typename F>
+int q8_dispatch(int dtype, int head_size, F f) {
+  if (!q8_head_size(head_size)) return LVAMD_ERR_UNSUPPORTED;
+  switch (dtype) {
+    case LVAMD_BF16: return q8_with_head_size<__bf16>(head_size, f);
+    case LVAMD_F16: return q8_with_head_size<_Float16>(head_size, f);
+    default: return LVAMD_ERR_UNSUPPORTED;
+  }
+}
+
 }  // namespace lvamd

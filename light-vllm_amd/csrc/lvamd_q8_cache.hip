@@ -381,7 +381,6 @@ __global__ __launch_bounds__(64) void q8_compact_few_kernel(const Q8FewArgs<PAIR
   }
 }
 
-static bool q8_head_size(int d) { return d >= 32 && d <= 256 && d % 16 == 0; }
 static bool aligned_to(const void* p, unsigned n) { return ((uintptr_t)p & (n - 1)) == 0; }
 
 }  // namespace lvamd

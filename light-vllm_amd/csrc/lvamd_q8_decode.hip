@@ -540,39 +540,7 @@ __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(1, 1))) void
   }
 }
 
-static bool q8_head_size(int d) { return d >= 32 && d <= 256 && d % 16 == 0; }
 static bool aligned16(const void* p) { return ((uintptr_t)p & 15u) == 0; }
-
-template <typename T, typename F>
-static int q8_with_head_size(int head_size, F& f) {
-  switch (head_size) {
-    case 32: return f.template operator()<T, 32>();
-    case 48: return f.template operator()<T, 48>();
-    case 64: return f.template operator()<T, 64>();
-    case 80: return f.template operator()<T, 80>();
-    case 96: return f.template operator()<T, 96>();
-    case 112: return f.template operator()<T, 112>();
-    case 128: return f.template operator()<T, 128>();
-    case 144: return f.template operator()<T, 144>();
-    case 160: return f.template operator()<T, 160>();
-    case 176: return f.template operator()<T, 176>();
-    case 192: return f.template operator()<T, 192>();
-    case 208: return f.template operator()<T, 208>();
-    case 224: return f.template operator()<T, 224>();
-    case 240: return f.template operator()<T, 240>();
-    case 256: return f.template operator()<T, 256>();
-    default: return LVAMD_ERR_UNSUPPORTED;
-  }
-}
-template <typename F>
-static int q8_dispatch(int dtype, int head_size, F f) {
-  if (!q8_head_size(head_size)) return LVAMD_ERR_UNSUPPORTED;
-  switch (dtype) {
-    case LVAMD_BF16: return q8_with_head_size<__bf16>(head_size, f);
-    case LVAMD_F16: return q8_with_head_size<_Float16>(head_size, f);
-    default: return LVAMD_ERR_UNSUPPORTED;
-  }
-}
 
 }  // namespace lvamd
 

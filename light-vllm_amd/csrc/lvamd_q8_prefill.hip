@@ -489,30 +489,9 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(prefill_
 namespace {
 
 bool prefill_q8_supported(int dtype, int head_size) {
-  return (dtype == LVAMD_BF16 || dtype == LVAMD_F16) && head_size >= 32 && head_size <= 256 && head_size % 16 == 0;
+  return (dtype == LVAMD_BF16 || dtype == LVAMD_F16) && q8_head_size(head_size);
 }
 
-template <typename T, int CT, int W, typename F>
-int with_prefill_head_size(int head_size, F& f) {
-  switch (head_size) {
-    case 32: return f.template operator()<T, 32, CT, W>();
-    case 48: return f.template operator()<T, 48, CT, W>();
-    case 64: return f.template operator()<T, 64, CT, W>();
-    case 80: return f.template operator()<T, 80, CT, W>();
-    case 96: return f.template operator()<T, 96, CT, W>();
-    case 112: return f.template operator()<T, 112, CT, W>();
-    case 128: return f.template operator()<T, 128, CT, W>();
-    case 144: return f.template operator()<T, 144, CT, W>();
-    case 160: return f.template operator()<T, 160, CT, W>();
-    case 176: return f.template operator()<T, 176, CT, W>();
-    case 192: return f.template operator()<T, 192, CT, W>();
-    case 208: return f.template operator()<T, 208, CT, W>();
-    case 224: return f.template operator()<T, 224, CT, W>();
-    case 240: return f.template operator()<T, 240, CT, W>();
-    case 256: return f.template operator()<T, 256, CT, W>();
-    default: return LVAMD_ERR_UNSUPPORTED;
-  }
-}
 // (Units of 256 columns: the head sizes whose two tiles per wave fit the
 // registers, and whose products are long enough to gain by them.)
 template <typename T, typename F>
@@ -531,11 +510,9 @@ int dispatch_prefill(int dtype, int head_size, int columns, F f) {
   const bool bf16 = dtype == LVAMD_BF16;
   switch (columns) {
     case 64:
-      return bf16 ? with_prefill_head_size<__bf16, 1, 4>(head_size, f)
-                  : with_prefill_head_size<_Float16, 1, 4>(head_size, f);
+      return q8_dispatch(dtype, head_size, [&]<typename T, int D>() { return f.template operator()<T, D, 1, 4>(); });
     case 128:
-      return bf16 ? with_prefill_head_size<__bf16, 1, 8>(head_size, f)
-                  : with_prefill_head_size<_Float16, 1, 8>(head_size, f);
+      return q8_dispatch(dtype, head_size, [&]<typename T, int D>() { return f.template operator()<T, D, 1, 8>(); });
     default: return bf16 ? with_wide_head_size<__bf16>(head_size, f) : with_wide_head_size<_Float16>(head_size, f);
   }
 }
