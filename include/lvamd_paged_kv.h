@@ -684,6 +684,76 @@ int lvamd_verify_drafts(const void* target, int64_t target_row_stride, const voi
                         int64_t* out_tokens, void* workspace, int64_t workspace_bytes, lvamd_stream_t stream);
 int64_t lvamd_verify_drafts_workspace_size(int64_t num_requests, int64_t num_drafts, int32_t vocab, int32_t dtype);
 
+/*
+ * Rotary angles: pair i of position p turns by p * turns[i] (fp64, in turns);
+ * cosines and sines, times magnitude, go to rows of repeat * half values of
+ * dtype (repeat 2: every row's values twice, one half after the other).
+ * positions: int32 or int64 (position_bytes 4 or 8).
+ *
+ * Replaces: _rotary_embeddings (src/light_vllm/modeling/models/qwen2.py), whose
+ *   angles are fp32 products.
+ */
+int lvamd_rotary_angles(const void* positions, int32_t position_bytes, int64_t num_tokens, const double* turns,
+                        int32_t half, float magnitude, void* cosines, void* sines, int32_t repeat, int32_t dtype,
+                        lvamd_stream_t stream);
+
+/*
+ * A paged cache of latent vectors (light-vllm has no counterpart).  Per layer
+ * one pool [num_blocks, block_size, latent_size + rope_size], contiguous, of
+ * dtype bf16 or fp16: a token's latent, then its rotated key, both shared by all
+ * heads.  latent_size: 128, 256, 384 or 512; rope_size: 32 or 64.
+ *
+ * Append: entry i writes token sources[i] (NULL: i) to slots[i]; slots outside
+ * [0, num_slots) are not written.  With cosines and sines (fp32,
+ * [tokens][rope_size / 2], rows 16-byte aligned) the keys are turned: pairs (2i,
+ * 2i + 1) if interleaved, else (i, i + rope_size / 2).  query_rope (NULL, or
+ * [tokens][heads][rope_size] with angles): turned too, into rotated (contiguous).
+ */
+int lvamd_latent_append(const void* latent, int64_t latent_token_stride, const void* rope_key,
+                        int64_t rope_key_token_stride, void* pool, int64_t num_slots, const int64_t* slots,
+                        const int64_t* sources, int64_t num_entries, const float* cosines, const float* sines,
+                        int64_t angle_token_stride, int32_t interleaved, const void* query_rope,
+                        int64_t query_token_stride, int64_t query_head_stride, void* rotated, int64_t num_tokens,
+                        int32_t num_heads, int32_t latent_size, int32_t rope_size, int32_t dtype,
+                        lvamd_stream_t stream);
+
+/*
+ * Row src[i] of every layer's pool (rows of row_bytes, a multiple of 16: tokens,
+ * or whole blocks) to row dst[i]; destinations are unique.  With a workspace of
+ * lvamd_latent_move_workspace_size bytes every source is read before any
+ * destination is written; without one (NULL) no source may be a destination.
+ * _few: at most lvamd_latent_move_few_pairs() pairs in HOST memory, no
+ * workspace, sources read first.  pools: device array of pool addresses.
+ */
+int lvamd_latent_move(const uint64_t* pools, int32_t num_layers, int64_t row_bytes, const int64_t* src,
+                      const int64_t* dst, int64_t num_pairs, void* workspace, int64_t workspace_bytes,
+                      lvamd_stream_t stream);
+int lvamd_latent_move_few(const uint64_t* pools, int32_t num_layers, int64_t row_bytes, const int64_t* src,
+                          const int64_t* dst, int64_t num_pairs, lvamd_stream_t stream);
+int64_t lvamd_latent_move_few_pairs(void);
+int64_t lvamd_latent_move_workspace_size(int64_t num_pairs, int32_t num_layers, int64_t row_bytes);
+
+/*
+ * Attention in latent space: query [tokens][heads][latent_size] (multiplied by
+ * the heads' key weights), query_rope [tokens][heads][rope_size] (turned), out
+ * [tokens][heads][latent_size] (to be multiplied by the heads' value weights).
+ * pieces and jobs as lvamd_paged_decode's with one kv head, the workgroup of
+ * 16 * col_tiles columns (1, 2, 4 or 8) in the wave's place; group_first holds
+ * num_groups + 1 entries.  Split segments go through part_acc (fp32
+ * [num_partial_slots][16 * col_tiles][latent_size]) and part_ml and are merged.
+ */
+int lvamd_latent_decode(const void* query, int64_t query_token_stride, int64_t query_head_stride,
+                        const void* query_rope, int64_t rope_token_stride, int64_t rope_head_stride,
+                        const void* pool, void* out, int64_t out_token_stride, int64_t out_head_stride,
+                        const int32_t* pieces, const int32_t* group_first, int32_t num_groups,
+                        const int32_t* jobs, int32_t num_jobs, int32_t merge_columns, const int32_t* tables,
+                        const uint32_t* vis, float* part_acc, float* part_ml, int64_t num_partial_slots,
+                        int32_t num_heads, int32_t latent_size, int32_t rope_size, int32_t col_tiles,
+                        int32_t block_size, float scale, int32_t dtype, lvamd_stream_t stream);
+int lvamd_latent_decode_tile_tokens(void);
+/* Workgroups of lvamd_latent_decode the current GPU holds at once. */
+int lvamd_latent_decode_resident_groups(int32_t dtype, int32_t latent_size, int32_t rope_size, int32_t col_tiles);
+
 #ifdef __cplusplus
 }
 #endif

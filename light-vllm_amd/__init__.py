@@ -45,6 +45,15 @@ from light_vllm_amd.quantized_cache import (  # noqa: E402
     QuantizedPagedLayerCache,
     quantized_kv_cache_bytes_per_block,
 )
+from light_vllm_amd.latent_attention import HipLatentPagedAttention  # noqa: E402
+from light_vllm_amd.latent_cache import (  # noqa: E402
+    LatentKVCacheSpec,
+    LatentLayerSpec,
+    LatentPagedKVCache,
+    LatentPagedLayerCache,
+    latent_kv_cache_bytes_per_block,
+)
+from light_vllm_amd.rotary import RotaryEmbedding, RotaryScaling, rotary_frequencies  # noqa: E402
 from light_vllm_amd.verify import DraftBatch, DraftVerdict, verify_drafts  # noqa: E402
 
 # ``from light_vllm_amd import errors`` registers the submodule under the
@@ -65,11 +74,16 @@ __all__ = [
     "DraftVerdict",
     "ExecutionError",
     "ExecutionNotReadyError",
+    "HipLatentPagedAttention",
     "HipPagedAttention",
     "HipPagedAttentionBackend",
     "HipQuantizedPagedAttention",
     "KVCacheCapacityError",
     "KVCacheError",
+    "LatentKVCacheSpec",
+    "LatentLayerSpec",
+    "LatentPagedKVCache",
+    "LatentPagedLayerCache",
     "ModelKVCacheSpec",
     "PagedAttentionMetadata",
     "PagedKVCache",
@@ -80,15 +94,19 @@ __all__ = [
     "QuantizedPagedKVCache",
     "QuantizedPagedLayerCache",
     "QueryLayout",
+    "RotaryEmbedding",
+    "RotaryScaling",
     "SharedPrefix",
     "append_draft_layout",
     "copy_commands",
     "hip_block_copy",
     "hip_compact",
     "kv_cache_bytes_per_block",
+    "latent_kv_cache_bytes_per_block",
     "linear_query_layout",
     "quantized_kv_cache_bytes_per_block",
     "query_visibility",
+    "rotary_frequencies",
     "semantic_positions",
     "share_prefix",
     "verify_drafts",

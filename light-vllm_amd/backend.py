@@ -34,8 +34,11 @@ from torch import Tensor
 
 from light_vllm_amd import errors, native
 from light_vllm_amd.facts import facts_of
+from light_vllm_amd.latent_attention import HipLatentPagedAttention, LatentStepPlan
+from light_vllm_amd.latent_cache import is_latent
 from light_vllm_amd.metadata import PagedAttentionMetadata
 from light_vllm_amd.paged_cache import current_stream, dtype_code, hip_append_rotary, is_quantized
+from light_vllm_amd.quantized_cache import on_device
 from light_vllm_amd.plan import (
     DECODE_MAX_COLUMNS, DECODE_MERGE_PIECES, DECODE_MIN_UNITS_PER_WAVE, PREFILL_MIN_TILES, UNIT_TOKENS, LayerShapes,
     Staging, StepPlan,
@@ -793,13 +796,36 @@ class HipPagedAttentionBackend:
                 if spec.head_size in SUPPORTED_HEAD_SIZES)
         return found
 
-    def create(self, cache, metadata) -> HipPagedAttention:
+    def _create_latent(self, cache, key, metadata) -> HipLatentPagedAttention:
+        """``create`` over a ``LatentPagedKVCache``."""
+
+        config = cache.config
+        geometry = (config.num_blocks, config.block_size, config.device, config.dtype, HipLatentPagedAttention)
+        last = self._last
+        if last is None or last[1] is not key or last[0] != geometry:
+            staging = self._staging.get(config.device)
+            if staging is None:
+                staging = self._staging[config.device] = Staging(config.device)
+            with on_device(config.device):
+                plan = LatentStepPlan(metadata, block_size=config.block_size, device=config.device,
+                                      num_blocks=config.num_blocks, staging=staging, defer_upload=True)
+                for spec in cache.model_spec.layers:
+                    plan.shape(spec, dtype_code(config.dtype))
+                plan.commit()
+        else:
+            plan = last[2]
+        self._last = (geometry, key, plan, weakref.ref(cache))
+        return HipLatentPagedAttention(self, cache, plan)
+
+    def create(self, cache, metadata) -> "HipPagedAttention | HipLatentPagedAttention":
         # This package's metadata is recognised by its facts object, which the
         # plan holds anyway: the metadata itself (a step's worth of tuples) is
         # not kept alive, so the caller frees it, not the next create().  The
         # same metadata on the same cache object takes the last plan with no
         # rule to re-check (the cache's configuration does not change).
         key = metadata.facts if isinstance(metadata, PagedAttentionMetadata) else metadata
+        if is_latent(cache):
+            return self._create_latent(cache, key, metadata)
         last = self._last
         context = HipQuantizedPagedAttention if is_quantized(cache) else HipPagedAttention
         if last is not None and last[1] is key and last[3]() is cache:

@@ -951,6 +951,9 @@ struct DecodeParams {
   int64_t split_groups = 0;  // resident workgroups of the workgroup-split kernel (0: not built)
   int64_t split_waves = 0;   // its waves per workgroup
   int64_t merge_pieces = 0;  // most pieces of a segment the merge takes well (0: kMergePiecesMax)
+  // A linear request's column group ends at its last query's own token (the
+  // groups of the other kernels' segments all span the whole request).
+  bool trim = false;
 };
 
 // Workgroup split of the decode kernel: workgroups of split_waves waves, one
@@ -995,22 +998,25 @@ constexpr int64_t kSplitBusyGroups = 128;
 void build_decode(const Requests& q, const int32_t* ids, int64_t nflat, const DecodeParams& d, DecodeLists& out) {
   struct Seg {
     int32_t req, group;
-    int64_t start, tiles;
+    int64_t start, tiles, end;  // end: tokens
   };
   std::vector<Seg> segs;
   int64_t total = 0;
   for (int64_t r = 0; r < q.batch; ++r) {
     const int64_t columns = q.q_len(r) * d.group;
     if (d.max_cols > 0 && columns > d.max_cols) continue;
-    const int64_t tiles = (q.computed(r) + q.q_len(r) + d.unit - 1) / d.unit;
     const int64_t ngroups = ((columns + 15) / 16 + d.col_tiles - 1) / d.col_tiles;
+    const bool trim = d.trim && q.row(r)[5] < 0;
     for (int64_t g = 0; g < ngroups; ++g) {
-      segs.push_back({(int32_t)r, (int32_t)g, total, tiles});
+      const int64_t last = trim ? std::min(columns, (g + 1) * 16 * d.col_tiles) - 1 : columns - 1;
+      const int64_t end = q.computed(r) + last / d.group + 1, tiles = (end + d.unit - 1) / d.unit;
+      segs.push_back({(int32_t)r, (int32_t)g, total, tiles, end});
       total += tiles;
     }
   }
   if (total == 0) return;
-  int64_t cap = std::max<int64_t>(1, ((kTableSlice - 2) * d.bs) / d.unit);
+  // (The latent kernel holds no table slice in LDS.)
+  int64_t cap = d.trim ? total : std::max<int64_t>(1, ((kTableSlice - 2) * d.bs) / d.unit);
   if (d.max_units > 0) cap = std::max<int64_t>(1, std::min(cap, d.max_units));
   // Shares of at least min_units tiles, and long enough that no segment is
   // cut into more pieces than the merge takes well (a segment of T tiles over
@@ -1078,7 +1084,7 @@ void build_decode(const Requests& q, const int32_t* ids, int64_t nflat, const De
     o[0] = sg.req;
     o[1] = sg.group;
     o[2] = (int32_t)tok_begin;
-    o[3] = (int32_t)std::min((x.hi - sg.start) * d.unit, q.computed(sg.req) + q.q_len(sg.req));
+    o[3] = (int32_t)std::min((x.hi - sg.start) * d.unit, sg.end);
     o[4] = multi ? out.slots : -1;
     o[5] = m[0];   // table_off
     o[6] = m[2];   // computed
@@ -1616,6 +1622,32 @@ PyObject* decode_work(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     PyErr_SetString(PyExc_ValueError, "decode_work: inconsistent arguments");
     return nullptr;
   }
+  DecodeLists out;
+  build_decode(q, flat.data<int32_t>(), flat.count(), d, out);
+  return decode_result(out);
+}
+
+// latent_work(req_meta i32[B*8], flat i32, heads, col_tiles, resident,
+//             block_size, unit, merge_pieces)
+//   -> as decode_work
+// The pieces of the attention over latent vectors: one kv head whose group is
+// every head, workgroups of 16 * col_tiles columns in the waves' place.
+PyObject* latent_work(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  if (!want_args(nargs, 8, "latent_work")) return nullptr;
+  Buf meta(args[0], false, 4, "req_meta"), flat(args[1], false, 4, "flat");
+  if (!meta.ok() || !flat.ok()) return nullptr;
+  Requests q;
+  if (!requests_of(meta, &q, "latent_work")) return nullptr;
+  DecodeParams d{};
+  int64_t* fields[] = {&d.group, &d.col_tiles, &d.resident, &d.bs, &d.unit, &d.merge_pieces};
+  for (int i = 0; i < 6; ++i)
+    if (!as_i64(args[2 + i], fields[i])) return nullptr;
+  if (d.group <= 0 || d.col_tiles <= 0 || d.resident <= 0 || d.bs <= 0 || d.unit <= 0) {
+    PyErr_SetString(PyExc_ValueError, "latent_work: inconsistent arguments");
+    return nullptr;
+  }
+  d.hkv = d.min_units = 1;
+  d.trim = true;
   DecodeLists out;
   build_decode(q, flat.data<int32_t>(), flat.count(), d, out);
   return decode_result(out);
@@ -2625,6 +2657,7 @@ PyMethodDef kMethods[] = {
     {"metadata", (PyCFunction)(void (*)(void))metadata, METH_FASTCALL, "metadata fields -> rule or (fields, facts)"},
     {"stage", (PyCFunction)(void (*)(void))stage, METH_FASTCALL, "slots and per-request records into buffers"},
     {"decode_work", (PyCFunction)(void (*)(void))decode_work, METH_FASTCALL, "stream-K decode pieces"},
+    {"latent_work", (PyCFunction)(void (*)(void))latent_work, METH_FASTCALL, "stream-K pieces over latent vectors"},
     {"prefill_work", (PyCFunction)(void (*)(void))prefill_work, METH_FASTCALL, "prefill units and merge jobs"},
     {"layer_work", (PyCFunction)(void (*)(void))layer_work, METH_FASTCALL, "one layer shape's choices and lists"},
     {"plan_step", (PyCFunction)(void (*)(void))plan_step, METH_FASTCALL, "a whole step, staged into one buffer"},

@@ -19,7 +19,7 @@ from pathlib import Path
 from light_vllm_amd import errors
 
 LIB_NAME = "liblvamd_hip.so"
-ABI_VERSION = 21
+ABI_VERSION = 22
 PACKAGE_DIR = Path(__file__).resolve().parent
 REPO_ROOT = PACKAGE_DIR.parent
 HEADER = REPO_ROOT / "include" / "lvamd_paged_kv.h"
@@ -143,6 +143,23 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
         [_p, _i64, _p, _i64, _i32, _i32, _p, _p, _p, _p, _i64, _i64, _p, _p, _i32, _p, _p, _i32, _p, _p, _i64, _p],
     ),
     "lvamd_verify_drafts_workspace_size": (_i64, [_i64, _i64, _i32, _i32]),
+    "lvamd_rotary_angles": (ctypes.c_int, [_p, _i32, _i64, _p, _i32, _f32, _p, _p, _i32, _i32, _p]),
+    "lvamd_latent_append": (
+        ctypes.c_int,
+        [_p, _i64, _p, _i64, _p, _i64, _p, _p, _i64, _p, _p, _i64, _i32, _p, _i64, _i64, _p, _i64,
+         _i32, _i32, _i32, _i32, _p],
+    ),
+    "lvamd_latent_move": (ctypes.c_int, [_p, _i32, _i64, _p, _p, _i64, _p, _i64, _p]),
+    "lvamd_latent_move_few": (ctypes.c_int, [_p, _i32, _i64, _p, _p, _i64, _p]),
+    "lvamd_latent_move_few_pairs": (_i64, []),
+    "lvamd_latent_move_workspace_size": (_i64, [_i64, _i32, _i64]),
+    "lvamd_latent_decode": (
+        ctypes.c_int,
+        [_p, _i64, _i64, _p, _i64, _i64, _p, _p, _i64, _i64, _p, _p, _i32, _p, _i32, _i32, _p, _p, _p, _p, _i64,
+         _i32, _i32, _i32, _i32, _i32, _f32, _i32, _p],
+    ),
+    "lvamd_latent_decode_tile_tokens": (ctypes.c_int, []),
+    "lvamd_latent_decode_resident_groups": (ctypes.c_int, [_i32, _i32, _i32, _i32]),
     "lvamd_stage_upload": (ctypes.c_int, [_p, _p, _i64, _p, _p]),
     "lvamd_hbm_read_probe": (ctypes.c_int, [_p, _i64, _p, _i32, _p]),
 }
@@ -358,6 +375,18 @@ def prefill_q8_resident_units(dtype_code: int, head_size: int, columns: int) -> 
 
     found = int(load().lvamd_paged_prefill_q8_resident_units(dtype_code, head_size, columns))
     check(min(found, 0), "lvamd_paged_prefill_q8_resident_units")
+    return found
+
+
+def latent_decode_resident_groups(dtype_code: int, latent_size: int, rope_size: int, col_tiles: int) -> int:
+    """Workgroups of the latent decode kernel of this width the current GPU holds at once."""
+
+    key = (dtype_code, latent_size, rope_size, col_tiles, "latent")
+    found = _RESIDENT.get(key)
+    if found is None:
+        found = int(load().lvamd_latent_decode_resident_groups(dtype_code, latent_size, rope_size, col_tiles))
+        check(min(found, 0), "lvamd_latent_decode_resident_groups")
+        _RESIDENT[key] = found
     return found
 
 

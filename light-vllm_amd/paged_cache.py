@@ -148,6 +148,13 @@ def is_quantized(cache) -> bool:
     return getattr(cache, "quantized", False) is True
 
 
+def _moves_itself(cache) -> bool:
+    """Whether ``cache`` has rows of its own kind, which only its own methods move
+    (8-bit codes with scales; latent vectors)."""
+
+    return is_quantized(cache) or getattr(cache, "latent", False) is True
+
+
 def _require_gpu(cache) -> None:
     if cache.config.device.type != "cuda":
         raise errors.KVCacheError("the HIP paged KV path requires a GPU KV cache")
@@ -156,6 +163,8 @@ def _require_gpu(cache) -> None:
 def _require_rows(cache) -> None:
     if is_quantized(cache):
         raise errors.KVCacheError("an 8-bit KV cache takes tokens by its own write_prepared")
+    if _moves_itself(cache):
+        raise errors.KVCacheError("a latent KV cache takes tokens by its own write_prepared")
 
 
 def hip_append(cache, layer_id: str, key: Tensor, value: Tensor, slots_ptr: int, num_tokens: int) -> None:
@@ -309,7 +318,7 @@ def hip_compact_many(cache, requests) -> tuple[int, ...]:
     _require_gpu(cache)
     if not isinstance(requests, (list, tuple)):
         requests = tuple(requests)
-    if is_quantized(cache):
+    if _moves_itself(cache):
         return cache.compact_many(requests)
     moved, src, dst = _compact_plan(cache.config, requests)
     if src.size:
@@ -412,7 +421,7 @@ def hip_block_copy(cache, src_blocks, dst_blocks) -> None:
     src, dst = _block_copy_pairs(cache, src_blocks, dst_blocks)
     if not src:
         return
-    if is_quantized(cache):
+    if _moves_itself(cache):
         cache.copy_blocks(src, dst)
         return
     pointers = _layer_pointers(cache)
