@@ -754,6 +754,47 @@ int lvamd_latent_decode_tile_tokens(void);
 /* Workgroups of lvamd_latent_decode the current GPU holds at once. */
 int lvamd_latent_decode_resident_groups(int32_t dtype, int32_t latent_size, int32_t rope_size, int32_t col_tiles);
 
+/*
+ * y[t][h] = weights[h] x[t][h] for the tokens rows[0..num_rows) (NULL: tokens 0
+ * .. num_rows): weights [heads][n][k], contiguous, k and n multiples of 64.  key_up^T
+ * takes queries into latent space, value_up results out of it.
+ */
+int lvamd_latent_heads(const void* x, int64_t x_token_stride, int64_t x_head_stride, const void* weights, void* y,
+                       int64_t y_token_stride, int64_t y_head_stride, const int32_t* rows, int64_t num_rows,
+                       int32_t num_heads, int32_t k, int32_t n, int32_t dtype, lvamd_stream_t stream);
+
+/*
+ * Per-head keys and values of cached rows: block record b (int32 [num_blocks][4]:
+ * table offset, first position, the request's positions, 0; an even number of
+ * them) names the positions of workspace rows 64 b .. 64 b + 63; those past the
+ * request's are its last again.  keys [heads][64 num_blocks][nope_size] = key_up
+ * [heads][nope_size][latent_size] times the latents, values likewise, rope_keys
+ * [64 num_blocks][rope_size] the rotated keys.  nope_size, value_size: 64 or 128.
+ * Values beyond fp16's largest are held at it.
+ */
+int lvamd_latent_expand(const void* pool, const int32_t* blocks, int32_t num_blocks, const int32_t* tables,
+                        const void* key_up, const void* value_up, void* keys, void* values, void* rope_keys,
+                        int32_t num_heads, int32_t latent_size, int32_t rope_size, int32_t nope_size,
+                        int32_t value_size, int32_t block_size, int32_t dtype, lvamd_stream_t stream);
+
+/*
+ * Attention of linear requests over lvamd_latent_expand's keys and values.  units
+ * and jobs as lvamd_paged_prefill's with a group of one and units of 128 queries
+ * and 64 keys, the table offset naming the request's first 64 rows of the
+ * workspace (num_keys rows in all); partials are fp32, [num_partial_slots][heads][128]
+ * [value_size], and merged.
+ */
+int lvamd_latent_prefill(const void* query, int64_t query_token_stride, int64_t query_head_stride,
+                         const void* query_rope, int64_t rope_token_stride, int64_t rope_head_stride,
+                         const void* keys, const void* values, const void* rope_keys, int64_t num_keys, void* out,
+                         int64_t out_token_stride, int64_t out_head_stride, const int32_t* units,
+                         int32_t num_units, const int32_t* jobs, int32_t num_jobs, int32_t merge_columns,
+                         float* part_acc, float* part_ml, int64_t num_partial_slots, int32_t num_heads,
+                         int32_t nope_size, int32_t rope_size, int32_t value_size, float scale, int32_t dtype,
+                         lvamd_stream_t stream);
+/* Workgroups of lvamd_latent_prefill the current GPU holds at once. */
+int lvamd_latent_prefill_resident_units(int32_t dtype, int32_t nope_size, int32_t rope_size, int32_t value_size);
+
 #ifdef __cplusplus
 }
 #endif

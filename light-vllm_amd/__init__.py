@@ -45,7 +45,7 @@ from light_vllm_amd.quantized_cache import (  # noqa: E402
     QuantizedPagedLayerCache,
     quantized_kv_cache_bytes_per_block,
 )
-from light_vllm_amd.latent_attention import HipLatentPagedAttention  # noqa: E402
+from light_vllm_amd.latent_attention import HipLatentPagedAttention, LatentWeights  # noqa: E402
 from light_vllm_amd.latent_cache import (  # noqa: E402
     LatentKVCacheSpec,
     LatentLayerSpec,
@@ -84,6 +84,7 @@ __all__ = [
     "LatentLayerSpec",
     "LatentPagedKVCache",
     "LatentPagedLayerCache",
+    "LatentWeights",
     "ModelKVCacheSpec",
     "PagedAttentionMetadata",
     "PagedKVCache",

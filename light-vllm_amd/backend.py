@@ -656,6 +656,7 @@ class HipPagedAttentionBackend:
         self._head_sizes_ok: "weakref.WeakSet[object]" = weakref.WeakSet()
         self._statics: "weakref.WeakKeyDictionary[object, dict]" = weakref.WeakKeyDictionary()
         self._shape_counts: "weakref.WeakKeyDictionary[object, dict]" = weakref.WeakKeyDictionary()
+        self._latent_forms: "weakref.WeakKeyDictionary[object, tuple | None]" = weakref.WeakKeyDictionary()
         # (geometry, metadata key, plan, weak reference to the cache) of the
         # most recent create().
         self._last: tuple[object, object, StepPlan, weakref.ref] | None = None
@@ -796,6 +797,11 @@ class HipPagedAttentionBackend:
                 if spec.head_size in SUPPORTED_HEAD_SIZES)
         return found
 
+    def note_latent_form(self, cache, sizes: tuple[int, int] | None) -> None:
+        """Which form a latent cache's steps take (the weights' sizes, or None)."""
+
+        self._latent_forms[cache] = sizes
+
     def _create_latent(self, cache, key, metadata) -> HipLatentPagedAttention:
         """``create`` over a ``LatentPagedKVCache``."""
 
@@ -809,8 +815,10 @@ class HipPagedAttentionBackend:
             with on_device(config.device):
                 plan = LatentStepPlan(metadata, block_size=config.block_size, device=config.device,
                                       num_blocks=config.num_blocks, staging=staging, defer_upload=True)
+                # (The lists of the form that the cache's steps took last; another is
+                # planned where it first runs.)
                 for spec in cache.model_spec.layers:
-                    plan.shape(spec, dtype_code(config.dtype))
+                    plan.shape(spec, dtype_code(config.dtype), self._latent_forms.get(cache))
                 plan.commit()
         else:
             plan = last[2]

@@ -1,61 +1,89 @@
-"""Attention over a ``LatentPagedKVCache``: the per-step context.
+"""Attention over a ``LatentPagedKVCache``: the heads' weights and the per-step
+context.
 
 Head h's key of a token is ``[key_up[h] c, r]`` and its value ``value_up[h] c``,
-with the token's latent c and rotated key r.  Multiplied out the other way
-round, key_up^T into the query and value_up behind the softmax, every head
-attends the rows of the cache themselves (the absorbed form): a row is read
-once for all heads.
+with the token's latent c and rotated key r.  There are two ways to the same
+result:
+
+* absorbed: key_up^T is multiplied into the query and value_up behind the
+  softmax, and every head attends the rows of the cache themselves: a row is
+  read once for all heads, a (query, key) pair costs 2 L + P products;
+* expanded: the request's keys and values are formed per head first, and a
+  pair costs N + P + V.
+
+Single tokens, short runs and draft trees take the first, long prompt chunks the
+second (``_expanded``).
 """
 
 from __future__ import annotations
 
+import numpy as np
 import torch
 from torch import Tensor
 
 from light_vllm_amd import errors, native
 from light_vllm_amd.latent_cache import LatentLayerSpec, aligned_rows, append_rows, check_rotary, check_rows
 from light_vllm_amd.paged_cache import dtype_code
-from light_vllm_amd.plan import DECODE_MERGE_PIECES, StepPlan, current_stream
+from light_vllm_amd.plan import DECODE_MERGE_PIECES, PREFILL_MIN_TILES, StepPlan, current_stream
 from light_vllm_amd.quantized_cache import on_device
 
-# Column tiles (of 16) per workgroup that the kernel is built for.
+# Column tiles (of 16) per workgroup that the latent-space kernel is built for.
 COL_TILES = (1, 2, 4)
+WEIGHT_SIZES = (64, 128)
+# Queries per unit, keys per tile and rows per expanded block of the chunk kernels.
+UNIT_QUERIES, UNIT_KEYS = 128, 64
+# Most bytes of expanded keys and values at a time: heads go in groups beyond it.
+EXPANDED_BYTES = 1 << 30
+
+
+class LatentWeights:
+    """The heads' weights of one layer, laid out once: ``key_up`` ``[heads,
+    nope_size, latent_size]`` and ``value_up`` ``[heads, value_size, latent_size]``
+    (rows as a linear layer's, per head)."""
+
+    __slots__ = ("key_up", "value_up", "key_down", "heads", "latent_size", "nope_size", "value_size")
+
+    def __init__(self, key_up: Tensor, value_up: Tensor) -> None:
+        for holds, message in (
+            (lambda: key_up.ndim == 3 and value_up.ndim == 3, "latent weights must have three dimensions"),
+            (lambda: key_up.shape[0] == value_up.shape[0] and key_up.shape[2] == value_up.shape[2],
+             "latent weights must agree in heads and latent size"),
+            (lambda: key_up.shape[1] in WEIGHT_SIZES and value_up.shape[1] in WEIGHT_SIZES,
+             f"nope_size and value_size must be one of {WEIGHT_SIZES}"),
+            (lambda: key_up.dtype == value_up.dtype and key_up.dtype in (torch.bfloat16, torch.float16),
+             "latent weights must be bfloat16 or float16, both of one dtype"),
+            (lambda: key_up.device == value_up.device and key_up.device.type == "cuda",
+             "latent weights must be on one GPU (cuda) device"),
+        ):
+            if not holds():
+                raise ValueError(message)
+        # (Copies, so that the rows are 16-byte chunks wherever the weights lay.)
+        self.key_up = key_up.detach().clone(memory_format=torch.contiguous_format)
+        self.value_up = value_up.detach().clone(memory_format=torch.contiguous_format)
+        self.key_down = self.key_up.transpose(1, 2).contiguous()  # into latent space
+        self.heads, self.nope_size, self.latent_size = key_up.shape
+        self.value_size = value_up.shape[1]
+
+
+class _Lists:
+    """int32 arrays of a layer shape's work, in the form ``StepPlan`` uploads:
+    ``ptr[name]`` is an array's device address."""
+
+    def __init__(self, **arrays: np.ndarray) -> None:
+        self._arrays = {name: a for name, a in arrays.items() if a.size}
+        for name in arrays:
+            setattr(self, name, None)
+
+    def parts(self):
+        return list(self._arrays.items())
 
 
 class _Shape:
     """One layer shape's launch facts in a step plan."""
 
-    __slots__ = ("work", "col_tiles", "acc_bytes", "workspace_bytes")
-
-    def __init__(self, work, col_tiles: int, latent_size: int) -> None:
-        self.work, self.col_tiles = work, col_tiles
-        columns = work.num_partial_slots * 16 * col_tiles
-        self.acc_bytes = columns * latent_size * 4
-        self.workspace_bytes = self.acc_bytes + columns * 8
-
-
-class _Work:
-    """Work lists of one layer shape, in the form ``StepPlan`` uploads."""
-
-    __slots__ = ("pieces_host", "first_host", "jobs_host", "pieces_ptr", "first_ptr", "jobs_ptr", "num_groups",
-                 "num_partial_slots", "merge_columns", "num_jobs")
-
-    def __init__(self, found) -> None:
-        pieces, first, jobs, groups, _, slots, columns, _, _ = found
-        self.pieces_host, self.first_host, self.jobs_host = (_i32(x) for x in (pieces, first, jobs))
-        self.pieces_ptr = self.first_ptr = self.jobs_ptr = None
-        self.num_groups, self.num_partial_slots, self.merge_columns = int(groups), int(slots), int(columns)
-        self.num_jobs = self.jobs_host.size // native.MERGE_FIELDS
-
-    def parts(self):
-        found = [("pieces_ptr", self.pieces_host), ("first_ptr", self.first_host), ("jobs_ptr", self.jobs_host)]
-        return [(name, array) for name, array in found if array.size]
-
-
-def _i32(data):
-    import numpy as np
-
-    return np.frombuffer(data, dtype=np.int32)
+    __slots__ = ("lists", "col_tiles", "num_groups", "num_jobs", "merge_columns", "num_slots", "acc_bytes", "latent_bytes",
+                 "num_rows", "row_base", "row_span", "every_row", "num_blocks", "num_units", "num_unit_jobs",
+                 "unit_merge_columns", "num_unit_slots")
 
 
 def choose_col_tiles(q_lens, heads: int) -> int:
@@ -67,22 +95,85 @@ def choose_col_tiles(q_lens, heads: int) -> int:
     return next((t for t in COL_TILES if t >= widest), COL_TILES[-1])
 
 
-class LatentStepPlan(StepPlan):
-    """A step plan with the latent kernels' work lists per (heads, sizes)."""
+def _expanded(facts, spec: LatentLayerSpec, nope: int, value: int) -> np.ndarray:
+    """Which requests take the expanded form: linear ones where its products are
+    fewer (queries count in whole units, and the expansion of every key is part
+    of them)."""
 
-    def shape(self, spec: LatentLayerSpec, code: int) -> _Shape:
-        key = (spec.num_query_heads, spec.latent_size, spec.rope_size, code)
+    n, c = facts.q_lens.astype(np.float64), facts.computed.astype(np.float64)
+    latent, rope = spec.latent_size, spec.rope_size
+    keys = c + n / 2
+    absorbed = n * keys * (2 * latent + rope) + n * latent * (nope + value)
+    expanded = np.maximum(n, UNIT_QUERIES) * keys * (nope + rope + value) + (c + n) * latent * (nope + value)
+    return (facts.vis_off < 0) & (expanded < absorbed)
+
+
+class LatentStepPlan(StepPlan):
+    """A step plan with the latent kernels' work lists per layer shape."""
+
+    def shape(self, spec: LatentLayerSpec, code: int, weights: tuple[int, int] | None) -> _Shape:
+        """``weights``: (nope_size, value_size), or None where queries come
+        absorbed."""
+
+        key = (spec.num_query_heads, spec.latent_size, spec.rope_size, code, weights)
         found = self.launches.get(key)
         if found is None:
-            heads = spec.num_query_heads
-            tiles = choose_col_tiles(self.facts.q_lens, heads)
-            resident = native.latent_decode_resident_groups(code, spec.latent_size, spec.rope_size, tiles)
-            work = _Work(native.host().latent_work(
-                self._req_meta, self.facts.flat, heads, tiles, resident, self.block_size,
-                int(native.load().lvamd_latent_decode_tile_tokens()), DECODE_MERGE_PIECES))
-            self._register(key, work)
-            found = self.launches[key] = _Shape(work, tiles, spec.latent_size)
+            if self._committed and torch.cuda.is_current_stream_capturing():
+                raise errors.ExecutionError("a step of this form must run once before it is captured (its work lists are "
+                                            "uploaded then)")
+            found = self.launches[key] = self._plan_shape(spec, code, weights)
+            self._register(key, found.lists)
         return found
+
+    def _plan_shape(self, spec: LatentLayerSpec, code: int, weights: tuple[int, int] | None) -> _Shape:
+        facts, heads, host = self.facts, spec.num_query_heads, native.host()
+        none = np.zeros(0, np.int32)
+        meta = self._req_meta.reshape(-1, native.REQ_FIELDS)
+        long = np.zeros(self.batch_size, bool) if weights is None else _expanded(facts, spec, *weights)
+        short = ~long
+        x = _Shape()
+        pieces = first = jobs = rows = blocks = units = unit_jobs = none
+        x.num_groups = x.num_jobs = x.num_slots = x.merge_columns = x.num_rows = 0
+        x.row_base, x.row_span, x.every_row, x.col_tiles = 0, 0, True, COL_TILES[0]
+        x.num_blocks = x.num_units = x.num_unit_jobs = x.unit_merge_columns = x.num_unit_slots = 0
+        if short.any():
+            x.col_tiles = choose_col_tiles(facts.q_lens[short], heads)
+            resident = native.latent_decode_resident_groups(code, spec.latent_size, spec.rope_size, x.col_tiles)
+            mine = meta[short].copy()
+            x.row_base = int(mine[0, 4])
+            x.row_span = int(mine[-1, 4] + mine[-1, 3]) - x.row_base
+            found = host.latent_work(mine, facts.flat, heads, x.col_tiles, resident, self.block_size,
+                                     int(native.load().lvamd_latent_decode_tile_tokens()), DECODE_MERGE_PIECES)
+            pieces, first, jobs = (np.frombuffer(a, dtype=np.int32) for a in found[:3])
+            x.num_groups, x.num_slots, x.merge_columns = int(found[3]), int(found[5]), int(found[6])
+            x.num_jobs = jobs.size // native.MERGE_FIELDS
+            x.num_rows = int(facts.q_lens[short].sum())
+            x.every_row = x.num_rows == x.row_span
+            if not x.every_row:
+                rows = np.concatenate([np.arange(s, s + n, dtype=np.int32) for s, n in zip(mine[:, 4], mine[:, 3])]) - x.row_base
+        if long.any():
+            mine = meta[long].copy()
+            total = (mine[:, 2] + mine[:, 3]).astype(np.int64)
+            per = -(-total // UNIT_KEYS)
+            base = np.cumsum(per) - per
+            blocks = np.zeros((int(per.sum() + 1) // 2 * 2, 4), np.int32)
+            blocks[:, 2] = 1  # (a padding block repeats the first table's first row)
+            for b, k, off, t in zip(base, per, mine[:, 0], total):
+                blocks[b:b + k, 0], blocks[b:b + k, 1], blocks[b:b + k, 2] = off, np.arange(k) * UNIT_KEYS, t
+            mine[:, 0], mine[:, 1] = base, per
+            resident = native.latent_prefill_resident_units(code, weights[0], spec.rope_size, weights[1])
+            found = host.prefill_work(mine, np.zeros(blocks.shape[0], np.int32), 1, UNIT_QUERIES, UNIT_KEYS, resident // heads,
+                                      PREFILL_MIN_TILES, 0, UNIT_KEYS, 0, heads, 0, 2)
+            units, unit_jobs = (np.frombuffer(a, dtype=np.int32) for a in found[:2])
+            x.num_blocks, x.num_units = blocks.shape[0], units.size // native.PREFILL_FIELDS
+            x.num_unit_jobs, x.num_unit_slots = unit_jobs.size // native.MERGE_FIELDS, int(found[2])
+            x.unit_merge_columns = int(found[4])
+        columns = x.num_slots * 16 * x.col_tiles
+        x.acc_bytes = columns * spec.latent_size * 4
+        x.latent_bytes = x.acc_bytes + columns * 8
+        x.lists = _Lists(pieces=pieces, first=first, jobs=jobs, rows=rows, blocks=blocks.reshape(-1), units=units,
+                         unit_jobs=unit_jobs)
+        return x
 
 
 class HipLatentPagedAttention:
@@ -106,16 +197,21 @@ class HipLatentPagedAttention:
         return self._plan
 
     def forward(self, layer_id: str, query: Tensor, latent: Tensor, rope_key: Tensor, *, scale: float,
-                rotary: tuple[Tensor, Tensor] | None = None) -> Tensor:
+                rotary: tuple[Tensor, Tensor] | None = None, weights: LatentWeights | None = None) -> Tensor:
         """Append this layer's rows, then attend what the cache holds.
 
-        ``query`` ``[tokens, heads, latent_size + rope_size]``: the heads' queries
-        multiplied by their key weights, then their rotated parts; returns
-        ``[tokens, heads, latent_size]``, to be multiplied by the heads' value
-        weights.  ``latent`` ``[tokens, latent_size]`` and ``rope_key`` ``[tokens,
-        rope_size]`` are the step's rows.  With ``rotary=(cosines, sines)`` (fp32
-        ``[tokens, rope_size / 2]``, ``RotaryEmbedding``) keys and queries come
-        unrotated and the append's launch turns both."""
+        With ``weights``: ``query`` ``[tokens, heads, nope_size + rope_size]``, returns
+        ``[tokens, heads, value_size]``.  Without: ``query`` ``[tokens, heads,
+        latent_size + rope_size]``, the heads' queries multiplied by their key weights
+        already, and what returns, ``[tokens, heads, latent_size]``, has yet to be
+        multiplied by their value weights.  ``latent`` ``[tokens, latent_size]`` and
+        ``rope_key`` ``[tokens, rope_size]`` are the step's rows.  With
+        ``rotary=(cosines, sines)`` (fp32 ``[tokens, rope_size / 2]``,
+        ``RotaryEmbedding``) keys and queries come unrotated and the append's launch
+        turns both.
+
+        With weights, a query's part in latent space and what attention gives there
+        are rounded to the cache's dtype, as are a long chunk's keys and values."""
 
         cache, plan = self._cache, self._plan
         cfg = cache.config
@@ -123,11 +219,16 @@ class HipLatentPagedAttention:
             raise errors.KVCacheError(f"paged attention layer {layer_id!r} ran more than once")
         self._layer_ids.add(layer_id)
         spec = cache.layer_spec(layer_id)
-        heads, size, rope = spec.num_query_heads, spec.latent_size, spec.rope_size
+        heads, rope = spec.num_query_heads, spec.rope_size
+        size = spec.latent_size if weights is None else weights.nope_size
         for holds, message in (
             (lambda: query.ndim == 3, "paged attention query must have three dimensions"),
             (lambda: query.shape[0] == plan.num_query_tokens,
              "paged attention metadata token count does not match query"),
+            (lambda: weights is None or (weights.heads, weights.latent_size) == (heads, spec.latent_size),
+             "latent weights do not match the layer spec"),
+            (lambda: weights is None or (weights.key_up.dtype == cfg.dtype and weights.key_up.device == cfg.device),
+             "latent weights dtype and device must match the KV cache"),
             (lambda: tuple(query.shape[1:]) == (heads, size + rope),
              "paged attention query shape does not match the layer spec"),
             (lambda: latent.ndim == 2 and latent.shape[0] == query.shape[0],
@@ -141,22 +242,86 @@ class HipLatentPagedAttention:
         angles = check_rotary(spec, rotary, latent)
         query = aligned_rows(query)
         query_rope = query[..., size:]
+        sizes = None if weights is None else (weights.nope_size, weights.value_size)
         with on_device(cfg.device):
-            code = dtype_code(cfg.dtype)
-            shape = plan.shape(spec, code)
+            code, stream = dtype_code(cfg.dtype), current_stream(cfg.device)
+            shape = plan.shape(spec, code, sizes)
+            self._backend.note_latent_form(cache, sizes)
             turned = append_rows(cache, spec, latent, rope_key, angles, plan.slots_ptr, None, plan.num_tokens,
                                  None if angles is None else query_rope)
             query_rope = query_rope if turned is None else turned
-            out = torch.empty((query.shape[0], heads, size), dtype=cfg.dtype, device=cfg.device)
-            # (Of the call's own stream or graph: no two share one.)
-            workspace = torch.empty(shape.workspace_bytes, dtype=torch.uint8, device=cfg.device)
-            part_acc = workspace.data_ptr() if shape.workspace_bytes else None
-            work = shape.work
-            native.check(native.load().lvamd_latent_decode(
-                query.data_ptr(), query.stride(0), query.stride(1), query_rope.data_ptr(), query_rope.stride(0),
-                query_rope.stride(1), cache.layer(layer_id).rows.data_ptr(), out.data_ptr(), out.stride(0), out.stride(1),
-                work.pieces_ptr, work.first_ptr, work.num_groups, work.jobs_ptr, work.num_jobs, work.merge_columns,
-                plan.tables_ptr, plan.vis_ptr, part_acc, None if part_acc is None else part_acc + shape.acc_bytes,
-                work.num_partial_slots, heads, size, rope, shape.col_tiles, plan.block_size, float(scale), code,
-                current_stream(cfg.device)), "lvamd_latent_decode")
+            width = spec.latent_size if weights is None else weights.value_size
+            out = torch.empty((query.shape[0], heads, width), dtype=cfg.dtype, device=cfg.device)
+            rows = cache.layer(layer_id).rows
+            if weights is None:
+                self._attend_latent(spec, shape, query, query_rope, rows, out, 0, scale, code, stream)
+            else:
+                if shape.num_rows:
+                    self._attend_short(spec, shape, weights, query, query_rope, rows, out, scale, code, stream)
+                if shape.num_units:
+                    self._attend_long(spec, shape, weights, query, query_rope, rows, out, scale, code, stream)
         return out
+
+    def _attend_latent(self, spec, shape, query, query_rope, rows, out, base: int, scale, code, stream) -> None:
+        """The latent-space kernel and its merge; token t of the step is row t - base
+        of ``query`` and ``out``."""
+
+        plan, lists = self._plan, shape.lists
+        # (Of the call's own stream or graph: no two share one.)
+        workspace = torch.empty(shape.latent_bytes, dtype=torch.uint8, device=rows.device)
+        acc = workspace.data_ptr() if shape.latent_bytes else None
+        es = query.element_size()
+        native.check(native.load().lvamd_latent_decode(
+            query.data_ptr() - base * query.stride(0) * es, query.stride(0), query.stride(1), query_rope.data_ptr(),
+            query_rope.stride(0), query_rope.stride(1), rows.data_ptr(), out.data_ptr() - base * out.stride(0) * es,
+            out.stride(0), out.stride(1), lists.pieces, lists.first, shape.num_groups, lists.jobs, shape.num_jobs,
+            shape.merge_columns, plan.tables_ptr, plan.vis_ptr, acc, None if acc is None else acc + shape.acc_bytes,
+            shape.num_slots, spec.num_query_heads, spec.latent_size, spec.rope_size, shape.col_tiles, plan.block_size,
+            float(scale), code, stream), "lvamd_latent_decode")
+
+    def _attend_short(self, spec, shape, weights, query, query_rope, rows, out, scale, code, stream) -> None:
+        """The absorbed form: into latent space, attention there, and out of it."""
+
+        lib, heads, base = native.load(), spec.num_query_heads, shape.row_base
+        both = torch.empty((2, shape.row_span, heads, spec.latent_size), dtype=query.dtype, device=query.device)
+        absorbed, attended = both.unbind(0)
+        where = None if shape.every_row else shape.lists.rows
+        es = query.element_size()
+        native.check(lib.lvamd_latent_heads(
+            query.data_ptr() + base * query.stride(0) * es, query.stride(0), query.stride(1), weights.key_down.data_ptr(),
+            absorbed.data_ptr(), absorbed.stride(0), absorbed.stride(1), where, shape.num_rows, heads, weights.nope_size,
+            spec.latent_size, code, stream), "lvamd_latent_heads")
+        self._attend_latent(spec, shape, absorbed, query_rope, rows, attended, base, scale, code, stream)
+        native.check(lib.lvamd_latent_heads(
+            attended.data_ptr(), attended.stride(0), attended.stride(1), weights.value_up.data_ptr(),
+            out.data_ptr() + base * out.stride(0) * es, out.stride(0), out.stride(1), where, shape.num_rows, heads,
+            spec.latent_size, weights.value_size, code, stream), "lvamd_latent_heads")
+
+    def _attend_long(self, spec, shape, weights, query, query_rope, rows, out, scale, code, stream) -> None:
+        """The expanded form: per-head keys and values, then attention over them."""
+
+        lib, plan, lists, heads = native.load(), self._plan, shape.lists, spec.num_query_heads
+        keys, es = shape.num_blocks * UNIT_KEYS, query.element_size()
+        nope, value, latent = weights.nope_size, weights.value_size, spec.latent_size
+        per_head = keys * (nope + value) * es
+        groups = min(heads, -(-heads * per_head // EXPANDED_BYTES))
+        group = -(-heads // groups)
+        columns = shape.num_unit_slots * UNIT_QUERIES * group
+        sizes = (keys * nope * es * group, keys * value * es * group, keys * spec.rope_size * es, columns * value * 4,
+                 columns * 8)
+        workspace = torch.empty(sum(sizes), dtype=torch.uint8, device=rows.device)
+        at = [workspace.data_ptr() + sum(sizes[:i]) for i in range(5)]
+        for h in range(0, heads, group):
+            n = min(group, heads - h)
+            native.check(lib.lvamd_latent_expand(
+                rows.data_ptr(), lists.blocks, shape.num_blocks, plan.tables_ptr,
+                weights.key_up.data_ptr() + h * nope * latent * es, weights.value_up.data_ptr() + h * value * latent * es,
+                at[0], at[1], at[2], n, latent, spec.rope_size, nope, value, plan.block_size, code, stream),
+                "lvamd_latent_expand")
+            native.check(lib.lvamd_latent_prefill(
+                query.data_ptr() + h * query.stride(1) * es, query.stride(0), query.stride(1),
+                query_rope.data_ptr() + h * query_rope.stride(1) * es, query_rope.stride(0), query_rope.stride(1),
+                at[0], at[1], at[2], keys, out.data_ptr() + h * out.stride(1) * es, out.stride(0), out.stride(1),
+                lists.units, shape.num_units, lists.unit_jobs, shape.num_unit_jobs, shape.unit_merge_columns,
+                at[3] if columns else None, at[4] if columns else None, shape.num_unit_slots, n, nope, spec.rope_size, value,
+                float(scale), code, stream), "lvamd_latent_prefill")

@@ -160,6 +160,16 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     ),
     "lvamd_latent_decode_tile_tokens": (ctypes.c_int, []),
     "lvamd_latent_decode_resident_groups": (ctypes.c_int, [_i32, _i32, _i32, _i32]),
+    "lvamd_latent_heads": (
+        ctypes.c_int, [_p, _i64, _i64, _p, _p, _i64, _i64, _p, _i64, _i32, _i32, _i32, _i32, _p]),
+    "lvamd_latent_expand": (
+        ctypes.c_int, [_p, _p, _i32, _p, _p, _p, _p, _p, _p, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _p]),
+    "lvamd_latent_prefill": (
+        ctypes.c_int,
+        [_p, _i64, _i64, _p, _i64, _i64, _p, _p, _p, _i64, _p, _i64, _i64, _p, _i32, _p, _i32, _i32, _p, _p, _i64,
+         _i32, _i32, _i32, _i32, _f32, _i32, _p],
+    ),
+    "lvamd_latent_prefill_resident_units": (ctypes.c_int, [_i32, _i32, _i32, _i32]),
     "lvamd_stage_upload": (ctypes.c_int, [_p, _p, _i64, _p, _p]),
     "lvamd_hbm_read_probe": (ctypes.c_int, [_p, _i64, _p, _i32, _p]),
 }
@@ -386,6 +396,18 @@ def latent_decode_resident_groups(dtype_code: int, latent_size: int, rope_size: 
     if found is None:
         found = int(load().lvamd_latent_decode_resident_groups(dtype_code, latent_size, rope_size, col_tiles))
         check(min(found, 0), "lvamd_latent_decode_resident_groups")
+        _RESIDENT[key] = found
+    return found
+
+
+def latent_prefill_resident_units(dtype_code: int, nope_size: int, rope_size: int, value_size: int) -> int:
+    """Workgroups of the latent prefill kernel the current GPU holds at once."""
+
+    key = (dtype_code, nope_size, rope_size, value_size, "latent prefill")
+    found = _RESIDENT.get(key)
+    if found is None:
+        found = int(load().lvamd_latent_prefill_resident_units(dtype_code, nope_size, rope_size, value_size))
+        check(min(found, 0), "lvamd_latent_prefill_resident_units")
         _RESIDENT[key] = found
     return found
 
