@@ -737,16 +737,17 @@ int64_t lvamd_latent_move_workspace_size(int64_t num_pairs, int32_t num_layers, 
  * Attention in latent space: query [tokens][heads][latent_size] (multiplied by
  * the heads' key weights), query_rope [tokens][heads][rope_size] (turned), out
  * [tokens][heads][latent_size] (to be multiplied by the heads' value weights).
- * pieces and jobs as lvamd_paged_decode's with one kv head, the workgroup of
- * 16 * col_tiles columns (1, 2, 4 or 8) in the wave's place; group_first holds
- * num_groups + 1 entries.  Split segments go through part_acc (fp32
+ * jobs as lvamd_paged_decode's with one kv head and 16 * col_tiles columns a slot
+ * (col_tiles: 1, 2, 4 or 8); pieces likewise up to field 10, then the index of the
+ * workgroup's next piece (-1: none) and its first four table entries (-1: not
+ * given); workgroup w of num_groups begins with piece w.  Split segments go through part_acc (fp32
  * [num_partial_slots][16 * col_tiles][latent_size]) and part_ml and are merged.
  */
 int lvamd_latent_decode(const void* query, int64_t query_token_stride, int64_t query_head_stride,
                         const void* query_rope, int64_t rope_token_stride, int64_t rope_head_stride,
                         const void* pool, void* out, int64_t out_token_stride, int64_t out_head_stride,
-                        const int32_t* pieces, const int32_t* group_first, int32_t num_groups,
-                        const int32_t* jobs, int32_t num_jobs, int32_t merge_columns, const int32_t* tables,
+                        const int32_t* pieces, int32_t num_groups, const int32_t* jobs, int32_t num_jobs,
+                        int32_t merge_columns, const int32_t* tables,
                         const uint32_t* vis, float* part_acc, float* part_ml, int64_t num_partial_slots,
                         int32_t num_heads, int32_t latent_size, int32_t rope_size, int32_t col_tiles,
                         int32_t block_size, float scale, int32_t dtype, lvamd_stream_t stream);

@@ -1629,9 +1629,12 @@ PyObject* decode_work(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
 
 // latent_work(req_meta i32[B*8], flat i32, heads, col_tiles, resident,
 //             block_size, unit, merge_pieces)
-//   -> as decode_work
+//   -> (pieces i32 [n, 16], jobs i32 [m, 8], workgroups, partial slots, most
+//       columns of a merge job, pieces of the deepest merge job)
 // The pieces of the attention over latent vectors: one kv head whose group is
-// every head, workgroups of 16 * col_tiles columns in the waves' place.
+// every head, workgroups of 16 * col_tiles columns in the waves' place.  Piece w is
+// workgroup w's first; field 11 is the index of its next (-1: none), fields 12 to
+// 15 its first four table entries (-1 where a tile may span more blocks).
 PyObject* latent_work(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   if (!want_args(nargs, 8, "latent_work")) return nullptr;
   Buf meta(args[0], false, 4, "req_meta"), flat(args[1], false, 4, "flat");
@@ -1649,8 +1652,32 @@ PyObject* latent_work(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   d.hkv = d.min_units = 1;
   d.trim = true;
   DecodeLists out;
-  build_decode(q, flat.data<int32_t>(), flat.count(), d, out);
-  return decode_result(out);
+  const int32_t* ids = flat.data<int32_t>();
+  build_decode(q, ids, flat.count(), d, out);
+  std::vector<int32_t> pieces(out.pieces.size());
+  for (int64_t w = 0, rest = out.waves; w < out.waves; ++w) {
+    const int64_t p0 = out.first[(size_t)w], p1 = out.first[(size_t)w + 1];
+    for (int64_t p = p0, at = w; p < p1; ++p) {
+      int32_t* o = pieces.data() + at * kPieceFields;
+      const int32_t* x = out.pieces.data() + p * kPieceFields;
+      std::memcpy(o, x, 11 * sizeof(int32_t));
+      o[11] = p + 1 < p1 ? (int32_t)rest : -1;
+      const int64_t lb0 = x[2] / d.bs;
+      for (int64_t k = 0; k < 4; ++k) {
+        const int64_t lb = lb0 + k, i = x[5] + lb;
+        o[12 + k] = (x[2] % d.bs + d.unit - 1) / d.bs >= 4 ? -1 : lb * d.bs < x[3] && i < flat.count() ? ids[i] : 0;
+      }
+      if (p + 1 < p1) at = rest++;
+    }
+  }
+  PyObject* a = to_bytearray(pieces);
+  PyObject* b = to_bytearray(out.jobs);
+  PyObject* result = (a && b) ? Py_BuildValue("(OOLiLi)", a, b, (long long)out.waves, out.slots, (long long)out.merge_cols,
+                                              out.depth)
+                              : nullptr;
+  Py_XDECREF(a);
+  Py_XDECREF(b);
+  return result;
 }
 
 // prefill_work(req_meta i32[B*8], flat i32, group, columns, key_tokens,

@@ -9,16 +9,17 @@
 // step's tokens are in the cache already.
 //
 // Mapping onto CDNA4:
-//   * A column is a (query, head) pair of one request; a workgroup of four waves
-//     holds up to 16 NC of them and walks over tiles of 32 rows: stream-K pieces
-//     of (request, column group) segments, split segments merged below.
+//   * A column is a (query, head) pair of one request; a workgroup (four waves, or
+//     eight of 64 columns and more) holds up to 16 NC of them and walks over tiles
+//     of 32 rows: stream-K pieces of (request, column group) segments, split
+//     segments merged below.
 //   * The rows of a tile are loaded once, straight into LDS (global_load_lds, no
 //     registers), while the tile before is computed; they serve as keys (rows
 //     read as they lie) and as values (transpose reads).
 //   * Scores: S^T = K Q^T on MFMA 16x16x32, the 16-row halves of the tile and the
 //     column tiles dealt to the waves, queries in registers.  Products: O^T = V^T
-//     P^T, a quarter of the latent's dimensions per wave for all columns, so an
-//     accumulator takes a quarter of the registers that a whole row would, and
+//     P^T, a share of the latent's dimensions per wave for all columns, so an
+//     accumulator takes a share of the registers that a whole row would, and
 //     each value is read from LDS once.  The probabilities cross over through
 //     LDS (the accumulator layout of S^T is the operand layout of P^T).
 //   * The waves share each column's running maximum, which moves only when some
@@ -41,7 +42,6 @@ namespace {
 
 constexpr float kSlack = 8.0f;  // lazy-rescale threshold, log2 units
 constexpr int KT = 32;          // rows per tile
-constexpr int kWaves = 4;
 
 typedef const __attribute__((address_space(1))) void* lds_gptr;
 typedef __attribute__((address_space(3))) void* lds_lptr;
@@ -63,24 +63,25 @@ struct LatentDecodeArgs {
   float scale_log2;
 };
 
+// A piece's record: pieces[blockIdx.x] is a workgroup's first, next its next (-1:
+// none); blocks are the first four of its table entries (-1: look them up).
 struct LatentPiece {
-  int group, tok_begin, tok_end, slot, table_off, computed, q_len, q_start, vis_off, vis_words;
+  int group, tok_begin, tok_end, slot, table_off, computed, q_len, q_start, vis_off, vis_words, next;
 };
 __device__ __forceinline__ LatentPiece read_latent_piece(const int32_t* __restrict__ pieces, int p) {
   const int32_t* r = pieces + (int64_t)p * LVAMD_PIECE_FIELDS;
-  return {r[1], r[2], r[3], r[4], r[5], r[6], r[7], r[8], r[9], r[10]};
+  return {r[1], r[2], r[3], r[4], r[5], r[6], r[7], r[8], r[9], r[10], r[11]};
 }
 
 __device__ __forceinline__ constexpr int swizzle(int row) {
   return (((row >> 2) & 1) << 1) | ((((row >> 3) ^ (row >> 1)) & 1) << 2);
 }
 
-// Orders LDS accesses around a workgroup barrier (global loads stay in flight).
-__device__ __forceinline__ void lds_barrier() {
-  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
-  __builtin_amdgcn_s_barrier();
-  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
-}
+// Orders LDS accesses around a workgroup barrier.  (A release fence would also
+// wait for the tile loads in flight, which write LDS too.)
+__device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
+constexpr int wait_vm(int n) { return 0x0F70 | (n & 15) | ((n >> 4) << 14); }  // s_waitcnt vmcnt(n)
 
 template <int L, int P, int NC>
 struct LatentShape {
@@ -89,11 +90,11 @@ struct LatentShape {
   static constexpr int GR = (CPR + 7) / 8;            // 128-byte groups
   static constexpr int TILE_BYTES = GR * KT * 128;
   static constexpr int KSTEPS = ROW / 32;             // MFMA steps of a score
-  static constexpr int DT = L / 64;                   // 16-dimension tiles per wave
+  static constexpr int W = NC >= 4 ? 8 : 4;           // waves
+  static constexpr int DT = L / (16 * W);             // 16-dimension tiles per wave
   static constexpr int QKS = NC == 8 ? 2 : 1;         // 16-row halves a wave scores
-  static constexpr int QCT = NC >= 4 ? 2 : 1;         // column tiles a wave scores
-  static constexpr int REGS = DT * NC * 4 + QCT * KSTEPS * 4;  // accumulators and queries
-  static constexpr int WAVES_PER_EU = REGS <= 176 ? 2 : 1;
+  static constexpr int NB = 2;                        // tiles in LDS
+  static constexpr int WAVES_PER_EU = 2;
   static_assert(L % 128 == 0 && P % 32 == 0);
 };
 
@@ -105,11 +106,11 @@ __device__ __forceinline__ bool not_finite(T x) {
 }  // namespace
 
 template <typename T, int L, int P, int NC>
-__global__ __launch_bounds__(64 * kWaves)
+__global__ __launch_bounds__(NC >= 4 ? 512 : 256)
 __attribute__((amdgpu_waves_per_eu(LatentShape<L, P, NC>::WAVES_PER_EU))) void latent_decode_kernel(
-    const int32_t* __restrict__ wave_first, const int32_t* __restrict__ pieces, const LatentDecodeArgs a) {
+    const int32_t* __restrict__ pieces, const LatentDecodeArgs a) {
   using S = LatentShape<L, P, NC>;
-  constexpr int GR = S::GR, KSTEPS = S::KSTEPS, DT = S::DT, QKS = S::QKS, QCT = S::QCT;
+  constexpr int GR = S::GR, KSTEPS = S::KSTEPS, DT = S::DT, QKS = S::QKS, W = S::W;
   constexpr int COLS = 16 * NC;
   using V8 = typename std::conditional<std::is_same<T, __bf16>::value, bf16x8, f16x8>::type;
   // Separate objects: a load into one does not alias a read of another.
@@ -117,54 +118,48 @@ __attribute__((amdgpu_waves_per_eu(LatentShape<L, P, NC>::WAVES_PER_EU))) void l
   __shared__ __attribute__((aligned(1024))) char tile1[S::TILE_BYTES];
   __shared__ __attribute__((aligned(16))) uint2 probs[NC * 64 * 2];  // [column tile][lane][half]
   __shared__ float tile_max[2][COLS], col_max[COLS], col_sum[2][COLS];
-  __shared__ __attribute__((aligned(16))) uint32_t votes[kWaves];
+  __shared__ __attribute__((aligned(16))) uint32_t votes[W];
 
-  const int tid = threadIdx.x & (64 * kWaves - 1);
+  const int tid = threadIdx.x & (64 * W - 1);
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int lane = tid & 63;
-  const int l16 = lane & 15;
-  const int g = lane >> 4;
-  int p = wave_first[blockIdx.x];
-  const int p_end = wave_first[blockIdx.x + 1];
-  if (p >= p_end) return;
 
-  // ---- this wave's scores: rows [16 ks0, 16 (ks0 + QKS)) of a tile, column
-  // tiles ct0 .. ct0 + QCT.
+  // ---- this wave's scores: rows [16 ks0, 16 (ks0 + QKS)) of a tile, column tile ct0.
   const bool scores = NC > 1 || wave < 2;
   const int ks0 = NC == 8 ? 0 : wave & 1;
-  const int ct0 = NC == 1 ? 0 : NC == 8 ? 2 * wave : QCT * (wave >> 1);
+  const int ct0 = NC == 1 ? 0 : NC == 8 ? wave : wave >> 1;
 
-  // ---- tile loads: wave w loads rows 8 w .. 8 w + 7, lane l row 8 w + l / 8
-  // into chunk slot l % 8 of every group.
-  const int lrow = 8 * wave + (lane >> 3);
-  const int lchunk = (lane & 7) ^ swizzle(lrow);
+  // ---- tile loads: wave w loads rows 8 (w % 4) .. + 7 of the groups w / 4, + W / 4,
+  // ..; lane l row l / 8 of them into chunk slot l % 8 of a group.
+  constexpr int GSTEP = W / 4;
+  const int rb = wave & 3;
   struct Row {
     int entry, off;
   };
-  auto lookup = [&](int table_off, int t0, int tok_end) -> Row {
-    const int pos = min(t0 + lrow, tok_end - 1);
+  auto lookup = [&](int ln, int table_off, int t0, int tok_end) -> Row {
+    const int pos = min(t0 + 8 * rb + (ln >> 3), tok_end - 1);
     const int lb = fast_div(pos, a.by_block);
     return {a.tables[table_off + lb], pos - lb * a.block_size};
   };
   gptr<const T> const pool = (gptr<const T>)(a.pool);
-  auto issue = [&](const Row& r, char* dst) {
+  auto issue = [&](int ln, const Row& r, char* dst) {
+    const int lchunk = (ln & 7) ^ swizzle(8 * rb + (ln >> 3));
     gptr<const T> const row = pool + ((int64_t)r.entry * a.block_size + r.off) * S::ROW;
 #pragma unroll
-    for (int i = 0; i < GR; ++i) {
-      int c = 8 * i + lchunk;
-      // (A half-used last group's spare slots take the row's last chunks again.)
-      if (8 * GR > S::CPR && i == GR - 1) c = min(c, S::CPR - 1);
-      __builtin_amdgcn_global_load_lds((lds_gptr)(row + 8 * c), (lds_lptr)(dst + i * KT * 128 + wave * 1024), 16, 0, 0);
+    for (int i = 0; i < (GR + GSTEP - 1) / GSTEP; ++i) {
+      const int gr = (wave >> 2) + i * GSTEP;
+      if (GR % GSTEP != 0 && gr >= GR) break;
+      int c = 8 * gr + lchunk;
+      // (A half-used last group's spare slots take the row's last chunk again.)
+      if (8 * GR > S::CPR && gr == GR - 1) c = min(c, S::CPR - 1);
+      // Non-temporal: a launch reads a row once, or a few column groups do at once.
+      __builtin_amdgcn_global_load_lds((lds_gptr)(row + 8 * c), (lds_lptr)(dst + (gr * KT * 128 + rb * 1024)), 16, 0, 2);
     }
   };
 
   // ---- columns: queries in registers, what each sees of the step's tokens
-  struct Columns {
-    int qi[QCT], head[QCT];
-    bool ok[QCT];
-  };
-  auto columns = [&](const LatentPiece& x, int ct, int& qi, int& head) -> bool {
-    const int col = x.group * COLS + 16 * ct + l16, ncols = x.q_len * a.heads;
+  auto columns = [&](int ln, const LatentPiece& x, int ct, int& qi, int& head) -> bool {
+    const int col = x.group * COLS + 16 * ct + (ln & 15), ncols = x.q_len * a.heads;
     const bool ok = col < ncols;
     const int c = ok ? col : ncols - 1;
     qi = fast_div(c, a.by_heads);
@@ -190,80 +185,91 @@ __attribute__((amdgpu_waves_per_eu(LatentShape<L, P, NC>::WAVES_PER_EU))) void l
     return left >= 32 ? bits : bits & ((1u << left) - 1u);
   };
 
-  LatentPiece cur = read_latent_piece(pieces, p);
-  uint4 qf[QCT][KSTEPS];
-  Columns col;
-  auto load_queries = [&](const LatentPiece& x) {
+  LatentPiece cur = read_latent_piece(pieces, blockIdx.x);
+  uint4 qf[KSTEPS];
+  int qi0 = 0;
+  auto load_queries = [&](int ln, const LatentPiece& x) {
+    const int g = ln >> 4;
+    int head;
+    const bool ok = columns(ln, x, ct0, qi0, head);
+    const T* q = static_cast<const T*>(a.q) + (int64_t)(x.q_start + qi0) * a.q_tok_stride + (int64_t)head * a.q_head_stride + 8 * g;
+    const T* qr = static_cast<const T*>(a.qr) + (int64_t)(x.q_start + qi0) * a.qr_tok_stride +
+                  (int64_t)head * a.qr_head_stride + 8 * g;
 #pragma unroll
-    for (int c = 0; c < QCT; ++c) {
-      col.ok[c] = columns(x, ct0 + c, col.qi[c], col.head[c]);
-      const T* q = static_cast<const T*>(a.q) + (int64_t)(x.q_start + col.qi[c]) * a.q_tok_stride +
-                   (int64_t)col.head[c] * a.q_head_stride;
-      const T* qr = static_cast<const T*>(a.qr) + (int64_t)(x.q_start + col.qi[c]) * a.qr_tok_stride +
-                    (int64_t)col.head[c] * a.qr_head_stride;
-#pragma unroll
-      for (int k = 0; k < KSTEPS; ++k) {
-        const T* from = 32 * k < L ? q + 32 * k + 8 * g : qr + 32 * k - L + 8 * g;
-        qf[c][k] = scores && col.ok[c] ? load16(from) : zero_u4();
-      }
-    }
+    for (int k = 0; k < KSTEPS; ++k) qf[k] = scores && ok ? load16(32 * k < L ? q + 32 * k : qr + 32 * k - L) : zero_u4();
   };
 
-  // The cursor is at the tile whose rows were looked up last, one ahead of the
-  // one in flight.
+  // The load cursor: the tile whose rows are looked up next.
   struct Cursor {
-    int p, table_off, t0, tok_end;
+    int table_off, t0, tok_end, next;  // tok_end 0: no more tiles
   };
   auto advance = [&](Cursor& c) {
     c.t0 += KT;
-    if (c.t0 >= c.tok_end && ++c.p < p_end) {
-      const int32_t* r = pieces + (int64_t)c.p * LVAMD_PIECE_FIELDS;
+    if (c.t0 >= c.tok_end) {
+      if (c.next < 0) {
+        c.tok_end = 0;
+        return;
+      }
+      const int32_t* r = pieces + (int64_t)c.next * LVAMD_PIECE_FIELDS;
       c.t0 = r[2];
       c.tok_end = r[3];
       c.table_off = r[5];
+      c.next = r[11];
     }
   };
-  Cursor at = {p, cur.table_off, cur.tok_begin, cur.tok_end};
-  Row row = lookup(at.table_off, at.t0, at.tok_end);
-  issue(row, tile0);
+  Cursor at = {cur.table_off, cur.tok_begin, cur.tok_end, cur.next};
+  Row row;
+  {
+    // The first tile's rows lie in the record's blocks.
+    const int32_t* r = pieces + (int64_t)blockIdx.x * LVAMD_PIECE_FIELDS;
+    const int b0 = r[12], b1 = r[13], b2 = r[14], b3 = r[15];
+    if (b0 >= 0) {
+      const int pos = min(at.t0 + 8 * rb + (lane >> 3), at.tok_end - 1);
+      const int lb = fast_div(pos, a.by_block), k = lb - fast_div(at.t0, a.by_block);
+      row = {k == 0 ? b0 : k == 1 ? b1 : k == 2 ? b2 : b3, pos - lb * a.block_size};
+    } else {
+      row = lookup(lane, at.table_off, at.t0, at.tok_end);
+    }
+  }
+  issue(lane, row, tile0);
+  load_queries(lane, cur);
   advance(at);
-  if (at.p < p_end) row = lookup(at.table_off, at.t0, at.tok_end);
+  if (at.tok_end > 0) row = lookup(lane, at.table_off, at.t0, at.tok_end);
 
-  float m_run[QCT], l_run[QCT];
+  float m_run, l_run;
   f32x4 acc[NC][DT];
   int t0 = cur.tok_begin;
   bool fresh = true;  // the tile is its piece's first
 
-  // LDS offsets of this lane: key reads (row l16 + 16 ks, chunk 4 k + g) and
-  // transpose reads (row 4 g + l16 / 4, +16; 8 bytes of dimensions 16 n + 4 q4).
-  const int kbase = l16 * 128;
-  const int kslot[2] = {16 * (g ^ swizzle(l16)), 16 * ((4 + g) ^ swizzle(l16))};
-  const int vrow = 4 * g + (l16 >> 2);
-  const int q4 = l16 & 3;
-  auto vaddr = [&](const char* tile, int n) -> const char* {
-    const int c = 2 * (wave * DT + n) + (q4 >> 1);
-    return tile + (c >> 3) * (KT * 128) + vrow * 128 + 16 * ((c & 7) ^ swizzle(vrow)) + 8 * (q4 & 1);
-  };
-
   // One tile from `here` while the next lands in `there`; false: it was the last.
   auto step = [&](const char* here, char* there) __attribute__((always_inline)) -> bool {
-    __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): this wave's part of the tile
-    lds_barrier();                       // everyone's, and the last tile's reads are done
-    const bool has_next = at.p < p_end;
-    const bool ends = at.p != p;  // the tile is its piece's last
-    const int nt0 = at.t0, np = at.p;
-    if (has_next) {
-      issue(row, there);
+    // (Everything that depends on the lane is formed anew in each step, a few
+    // instructions: kept from step to step it would not fit the registers of the
+    // wide instances.)
+    int ln = lane;
+    asm volatile("" : "+v"(ln));
+    const int l16 = ln & 15, g = ln >> 4;
+    // LDS offsets: key reads (row l16 + 16 ks, chunk 4 k + g) and transpose reads (row
+    // 4 g + l16 / 4, +16; 8 bytes of dimensions 16 n + 4 q4).  (Each read is one
+    // offset from its tile: the compiler tells a read of one tile from a load into
+    // the other only where few steps of arithmetic lie between the array and the
+    // access; otherwise it waits for the load before every read.)
+    const int kbase = (16 * ks0 + l16) * 128 + 16 * (g ^ swizzle(l16));  // (^ 64: chunk 4 + g)
+    const int vrow = 4 * g + (l16 >> 2), q4 = l16 & 3;
+    auto vaddr = [&](int n) -> int {
+      const int c = 2 * (wave * DT + n) + (q4 >> 1);
+      return (c >> 3) * (KT * 128) + vrow * 128 + 16 * ((c & 7) ^ swizzle(vrow)) + 8 * (q4 & 1);
+    };
+    __builtin_amdgcn_s_waitcnt(wait_vm(0));  // this wave's part of the tile
+    lds_barrier();                           // everyone's, and the last tile's reads are done
+    if (at.tok_end > 0) {
+      issue(ln, row, there);
       advance(at);
-      if (at.p < p_end) row = lookup(at.table_off, at.t0, at.tok_end);
+      if (at.tok_end > 0) row = lookup(ln, at.table_off, at.t0, at.tok_end);
     }
     if (fresh) {
-      load_queries(cur);
-#pragma unroll
-      for (int c = 0; c < QCT; ++c) {
-        m_run[c] = -INFINITY;
-        l_run[c] = 0.f;
-      }
+      m_run = -INFINITY;
+      l_run = 0.f;
 #pragma unroll
       for (int c = 0; c < NC; ++c)
 #pragma unroll
@@ -274,89 +280,89 @@ __attribute__((amdgpu_waves_per_eu(LatentShape<L, P, NC>::WAVES_PER_EU))) void l
     const bool masked = t0 + KT > min(cur.computed, cur.tok_end);
 
     // ---- scores
-    f32x4 st[QCT][QKS];
+    f32x4 st[QKS];
     bool vote = false, odd = false;
     if (scores) {
-      // LDS reads run LEAD ahead of the matrix instructions (held there by
-      // scheduling barriers: left alone the scheduler hoists them all and the
-      // wide instances spill).
-      constexpr int TOT = QKS * KSTEPS, LEAD = 4;
+      // LDS reads run LEAD ahead of the matrix instructions; two sums per score, so
+      // that an instruction does not wait for the one before it.
+      constexpr int TOT = QKS * KSTEPS, LEAD = NC == 8 ? 3 : 4, CH = QKS == 1 ? 2 : 1;
       auto rd = [&](int i) -> uint4 {
-        const int s = i / KSTEPS, k = i % KSTEPS;
-        return *reinterpret_cast<const uint4*>(here + (k >> 1) * (KT * 128) + (ks0 + s) * 16 * 128 + kbase + kslot[k & 1]);
+        return *reinterpret_cast<const uint4*>(here + (((i / QKS) >> 1) * (KT * 128) + (i % QKS) * 16 * 128 + (kbase ^ ((i / QKS) & 1 ? 64 : 0))));
       };
       uint4 key[LEAD];
 #pragma unroll
       for (int i = 0; i < LEAD; ++i) key[i] = rd(i);
-      const f32x4 z = {0.f, 0.f, 0.f, 0.f};
+      f32x4 sum[2];
 #pragma unroll
       for (int i = 0; i < TOT; ++i) {
-        const int s = i / KSTEPS, k = i % KSTEPS;
-#pragma unroll
-        for (int c = 0; c < QCT; ++c) st[c][s] = Mma<T>::qk(key[i % LEAD], qf[c][k], k == 0 ? z : st[c][s]);
+        const int k = i / QKS, to = QKS == 2 ? i % 2 : k % 2;
+        sum[to] = Mma<T>::qk(key[i % LEAD], qf[k], i < 2 ? f32x4{0.f, 0.f, 0.f, 0.f} : sum[to]);
         if (i + LEAD < TOT) key[i % LEAD] = rd(i + LEAD);
-        if constexpr (QCT == 2) __builtin_amdgcn_sched_barrier(0);
+        if constexpr (NC == 8) __builtin_amdgcn_sched_barrier(0);  // (hoisted reads would spill)
+      }
+      if constexpr (CH == 2) {
+        st[0] = sum[0] + sum[1];
+      } else {
+        st[0] = sum[0];
+        st[QKS - 1] = sum[1];
       }
       if (masked) {
         // A row that some column does not see may hold what is not finite (a
         // sibling's draft): zero probabilities do not hide it.  Every score of
         // such a row is not finite either.
-#pragma unroll
-        for (int c = 0; c < QCT; ++c) {
-          const uint32_t bits = window(cur, col.qi[c], t0) >> (16 * ks0 + 4 * g);
-#pragma unroll
-          for (int s = 0; s < QKS; ++s)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-              odd |= !(__builtin_fabsf(st[c][s][r]) < INFINITY);
-              st[c][s][r] = (bits >> (16 * s + r)) & 1u ? st[c][s][r] * a.scale_log2 : -INFINITY;
-            }
-        }
-      } else {
-#pragma unroll
-        for (int c = 0; c < QCT; ++c)
-#pragma unroll
-          for (int s = 0; s < QKS; ++s) st[c][s] *= a.scale_log2;
-      }
-#pragma unroll
-      for (int c = 0; c < QCT; ++c) {
-        float mt = -INFINITY;
+        const uint32_t bits = window(cur, qi0, t0) >> (16 * ks0 + 4 * g);
 #pragma unroll
         for (int s = 0; s < QKS; ++s)
 #pragma unroll
-          for (int r = 0; r < 4; ++r) mt = fmaxf(mt, st[c][s][r]);
-        mt = row_max4(mt);
-        vote |= mt > m_run[c] + kSlack;
-        if (g == 0) tile_max[ks0][16 * (ct0 + c) + l16] = mt;
-      }
-    }
-    auto weigh = [&]() {
-#pragma unroll
-      for (int c = 0; c < QCT; ++c) {
-        const float base = m_run[c] == -INFINITY ? 0.f : -m_run[c];
-#pragma unroll
-        for (int s = 0; s < QKS; ++s) {
-          // The weights are rounded to T for the products (a matrix
-          // instruction's operands are of one type); the sum that divides them
-          // counts them as rounded.
-          T w[4];
-#pragma unroll
           for (int r = 0; r < 4; ++r) {
-            w[r] = from_f32<T>(fast_exp2(st[c][s][r] + base));
-            l_run[c] += to_f32(w[r]);
+            odd |= !(__builtin_fabsf(st[s][r]) < INFINITY);
+            st[s][r] = (bits >> (16 * s + r)) & 1u ? st[s][r] * a.scale_log2 : -INFINITY;
           }
-          uint2 both;
-          __builtin_memcpy(&both, w, 8);
-          probs[((ct0 + c) * 64 + lane) * 2 + ks0 + s] = both;
+        // (Loads of rare branches are waited for in them: where the compiler has to
+        // assume them pending, it would wait for the tile in flight.)
+        __builtin_amdgcn_s_waitcnt(wait_vm(0));
+      } else {
+#pragma unroll
+        for (int s = 0; s < QKS; ++s) st[s] *= a.scale_log2;
+      }
+      float mt = -INFINITY;
+#pragma unroll
+      for (int s = 0; s < QKS; ++s)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) mt = fmaxf(mt, st[s][r]);
+      mt = row_max4(mt);
+      vote = mt > m_run + kSlack;
+      if (g == 0) tile_max[ks0][16 * ct0 + l16] = mt;
+    }
+    // The weights are rounded to T for the products (a matrix instruction's
+    // operands are of one type); the sum that divides them counts them as rounded.
+    auto weigh = [&]() {
+      const float base = m_run == -INFINITY ? 0.f : -m_run;
+#pragma unroll
+      for (int s = 0; s < QKS; ++s) {
+        T w[4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          w[r] = from_f32<T>(fast_exp2(st[s][r] + base));
+          l_run += to_f32(w[r]);
         }
+        uint2 both;
+        __builtin_memcpy(&both, w, 8);
+        probs[(ct0 * 64 + ln) * 2 + ks0 + s] = both;
       }
     };
     const bool any_vote = __any(vote), any_odd = __any(odd);
+    const float l_before = l_run;
     if (scores && !any_vote) weigh();
-    if (lane == 0) votes[wave] = (any_vote ? 1u : 0u) | (any_odd ? 2u : 0u);
+    if (ln == 0) votes[wave] = (any_vote ? 1u : 0u) | (any_odd ? 2u : 0u);
     lds_barrier();
-    const uint4 vw = *reinterpret_cast<const uint4*>(votes);
-    const uint32_t said = __builtin_amdgcn_readfirstlane(vw.x | vw.y | vw.z | vw.w);
+    uint32_t said = 0;
+#pragma unroll
+    for (int w = 0; w < W; w += 4) {
+      const uint4 v = *reinterpret_cast<const uint4*>(votes + w);
+      said |= v.x | v.y | v.z | v.w;
+    }
+    said = __builtin_amdgcn_readfirstlane(said);
     if (said & 1u) {
       // Some column's maximum moves: all waves move every column to its own.
       auto moved = [&](int c, float& before) -> float {
@@ -373,69 +379,76 @@ __attribute__((amdgpu_waves_per_eu(LatentShape<L, P, NC>::WAVES_PER_EU))) void l
         for (int n = 0; n < DT; ++n) acc[c][n] *= alpha;
       }
       if (scores) {
-        // (Weights that were formed with the old maximum are taken back.)
-        if (!any_vote) {
-#pragma unroll
-          for (int c = 0; c < QCT; ++c)
-#pragma unroll
-            for (int s = 0; s < QKS; ++s) {
-              const uint2 both = probs[((ct0 + c) * 64 + lane) * 2 + ks0 + s];
-              T w[4];
-              __builtin_memcpy(w, &both, 8);
-#pragma unroll
-              for (int r = 0; r < 4; ++r) l_run[c] -= to_f32(w[r]);
-            }
-        }
-#pragma unroll
-        for (int c = 0; c < QCT; ++c) {
-          float before;
-          const float after = moved(ct0 + c, before);
-          l_run[c] *= ratio(before, after);
-          m_run[c] = after;
-        }
+        // (Weights that were formed with the old maximum count anew.)
+        float before;
+        const float after = moved(ct0, before);
+        l_run = l_before * ratio(before, after);
+        m_run = after;
         weigh();
       }
       lds_barrier();
-      if (scores && g == 0 && ks0 == 0) {
-#pragma unroll
-        for (int c = 0; c < QCT; ++c) col_max[16 * (ct0 + c) + l16] = m_run[c];
-      }
+      if (scores && g == 0 && ks0 == 0) col_max[16 * ct0 + l16] = m_run;
     }
     const bool poisoned = (said & 2u) != 0;
     if (poisoned) {
       // The step's rows without their values that are not finite (and none of
       // the repeated rows past the piece's end).
-      const int pos = t0 + lrow;
-      if (pos >= cur.computed) {
+      const int lrow = 8 * rb + (ln >> 3);
+      if (t0 + lrow >= cur.computed && wave < 4) {
 #pragma unroll 1
         for (int c = 0; c < L / 8; ++c) {
-          if ((c & 7) != lchunk) continue;
-          T* at8 = reinterpret_cast<T*>(const_cast<char*>(here) + (c >> 3) * (KT * 128) + wave * 1024 + lane * 16);
+          if ((c & 7) != ((ln & 7) ^ swizzle(lrow))) continue;
+          uint4* const at8 = reinterpret_cast<uint4*>(const_cast<char*>(here) + ((c >> 3) * (KT * 128) + rb * 1024 + ln * 16));
+          T v[8];
+          const uint4 had = *at8;
+          __builtin_memcpy(v, &had, 16);
 #pragma unroll
           for (int e = 0; e < 8; ++e)
-            if (not_finite(at8[e])) at8[e] = from_f32<T>(0.f);
+            if (not_finite(v[e])) v[e] = from_f32<T>(0.f);
+          uint4 has;
+          __builtin_memcpy(&has, v, 16);
+          *at8 = has;
         }
       }
       lds_barrier();
     }
 
-    // ---- O^T += V^T P^T
-    V8 pb[NC];
-#pragma unroll
-    for (int c = 0; c < NC; ++c) pb[c] = bitcast<V8>(*reinterpret_cast<const uint4*>(probs + (c * 64 + lane) * 2));
-#pragma unroll
-    for (int n = 0; n < DT; ++n) {
-      const char* at8 = vaddr(here, n);
-      const s16x4 v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_t*)(at8));
-      const s16x4 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_t*)(at8 + 16 * 128));
-      const s16x4 both[2] = {v0, v1};
-#pragma unroll
-      for (int c = 0; c < NC; ++c) {
+    // ---- O^T += V^T P^T.  The fewer of the two operands' registers are held (all
+    // of a wave's values, or all columns' weights), the other is read LEAD ahead.
+    {
+      auto rdv = [&](int n) -> V8 {
+        const int at8 = vaddr(n);
+        const s16x4 v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_t*)(here + at8));
+        const s16x4 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_t*)(here + (at8 + 16 * 128)));
+        const s16x4 both[2] = {v0, v1};
+        return bitcast<V8>(both);
+      };
+      auto rdp = [&](int c) -> V8 { return bitcast<V8>(*reinterpret_cast<const uint4*>(probs + (c * 64 + ln) * 2)); };
+      auto mm = [&](V8 v, V8 w, f32x4 x) -> f32x4 {
         if constexpr (std::is_same<T, __bf16>::value) {
-          acc[c][n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(bitcast<V8>(both), pb[c], acc[c][n], 0, 0, 0);
+          return __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, w, x, 0, 0, 0);
         } else {
-          acc[c][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(bitcast<V8>(both), pb[c], acc[c][n], 0, 0, 0);
+          return __builtin_amdgcn_mfma_f32_16x16x32_f16(v, w, x, 0, 0, 0);
         }
+      };
+      constexpr bool HOLD_V = NC > DT;
+      constexpr int HELD = HOLD_V ? DT : NC, TOT = HOLD_V ? NC : DT, LEAD = TOT < 2 ? TOT : 2;
+      V8 held[HELD], ahead[LEAD];
+#pragma unroll
+      for (int i = 0; i < HELD; ++i) held[i] = HOLD_V ? rdv(i) : rdp(i);
+#pragma unroll
+      for (int i = 0; i < LEAD; ++i) ahead[i] = HOLD_V ? rdp(i) : rdv(i);
+      if constexpr (NC == 8) __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int i = 0; i < TOT; ++i) {
+        const V8 x = ahead[i % LEAD];
+        if (i + LEAD < TOT) ahead[i % LEAD] = HOLD_V ? rdp(i + LEAD) : rdv(i + LEAD);
+#pragma unroll
+        for (int k = 0; k < HELD; ++k) {
+          f32x4& to = acc[HOLD_V ? i : k][HOLD_V ? k : i];
+          to = HOLD_V ? mm(held[k], x, to) : mm(x, held[k], to);
+        }
+        if constexpr (NC == 8) __builtin_amdgcn_sched_barrier(0);
       }
     }
     if (poisoned) {
@@ -447,63 +460,65 @@ __attribute__((amdgpu_waves_per_eu(LatentShape<L, P, NC>::WAVES_PER_EU))) void l
         const int lb = fast_div(pos, a.by_block);
         gptr<const T> const v =
             pool + ((int64_t)a.tables[cur.table_off + lb] * a.block_size + (pos - lb * a.block_size)) * S::ROW;
-        f32x4 zero_or_nan[DT];
-#pragma unroll
-        for (int n = 0; n < DT; ++n)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) zero_or_nan[n][r] = to_f32((T)v[16 * (wave * DT + n) + 4 * g + r]) * 0.f;
+        uint32_t sees = 0;  // bit c: this lane's column of tile c
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
           int qi, head;
-          columns(cur, c, qi, head);
-          const bool sees = (window(cur, qi, t0) >> (pos - t0)) & 1u;
+          columns(ln, cur, c, qi, head);
+          sees |= ((window(cur, qi, t0) >> (pos - t0)) & 1u) << c;
+        }
 #pragma unroll
-          for (int n = 0; n < DT; ++n)
+        for (int n = 0; n < DT; ++n) {
+          f32x4 zero_or_nan;
 #pragma unroll
-            for (int r = 0; r < 4; ++r) acc[c][n][r] += sees ? zero_or_nan[n][r] : 0.f;
+          for (int r = 0; r < 4; ++r) zero_or_nan[r] = to_f32((T)v[16 * (wave * DT + n) + 4 * g + r]) * 0.f;
+#pragma unroll
+          for (int c = 0; c < NC; ++c)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) acc[c][n][r] += (sees >> c) & 1u ? zero_or_nan[r] : 0.f;
         }
       }
+      __builtin_amdgcn_s_waitcnt(wait_vm(0));
     }
 
+    t0 += KT;
+    if (t0 < cur.tok_end) return true;
     // ---- a finished piece: its output rows, or its partials
-    if (ends) {
-      if (scores) {
-#pragma unroll
-        for (int c = 0; c < QCT; ++c) {
-          const float l = row_sum4(l_run[c]);
-          if (g == 0) col_sum[ks0][16 * (ct0 + c) + l16] = l;
-        }
-      }
-      lds_barrier();
-#pragma unroll
-      for (int c = 0; c < NC; ++c) {
-        const int i = 16 * c + l16;
-        const float l_tot = QKS == 2 ? col_sum[0][i] : col_sum[0][i] + col_sum[1][i];
-        const float inv = l_tot > 0.f ? 1.f / l_tot : l_tot == l_tot ? 0.f : l_tot;
-        int qi, head;
-        if (!columns(cur, c, qi, head)) continue;
-        if (cur.slot < 0) {
-          T* to = static_cast<T*>(a.out) + (int64_t)(cur.q_start + qi) * a.out_tok_stride + (int64_t)head * a.out_head_stride;
-#pragma unroll
-          for (int n = 0; n < DT; ++n) store_partial4<false, T>(to + 16 * (wave * DT + n) + 4 * g, acc[c][n], inv);
-        } else {
-          const int64_t cs = (int64_t)cur.slot * COLS + i;
-          float* to = a.part_acc + cs * L;
-#pragma unroll
-          for (int n = 0; n < DT; ++n) store_partial4<false, float>(to + 16 * (wave * DT + n) + 4 * g, acc[c][n], inv);
-          // (A NaN sum keeps a finite maximum: the merge passes over a partial
-          // whose maximum is -inf.)
-          const float m = col_max[i];
-          if (wave == 0 && g == 0)
-            *reinterpret_cast<float2*>(a.part_ml + cs * 2) = make_float2(l_tot == l_tot || m != -INFINITY ? m : 0.f, l_tot);
-        }
-      }
-      if (!has_next) return false;
-      p = np;
-      cur = read_latent_piece(pieces, p);
-      fresh = true;
+    if (scores) {
+      const float l = row_sum4(l_run);
+      if (g == 0) col_sum[ks0][16 * ct0 + l16] = l;
     }
-    t0 = nt0;
+    lds_barrier();
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+      const int i = 16 * c + l16;
+      const float l_tot = QKS == 2 ? col_sum[0][i] : col_sum[0][i] + col_sum[1][i];
+      const float inv = l_tot > 0.f ? 1.f / l_tot : l_tot == l_tot ? 0.f : l_tot;
+      int qi, head;
+      if (!columns(ln, cur, c, qi, head)) continue;
+      if (cur.slot < 0) {
+        T* to = static_cast<T*>(a.out) + (int64_t)(cur.q_start + qi) * a.out_tok_stride + (int64_t)head * a.out_head_stride;
+#pragma unroll
+        for (int n = 0; n < DT; ++n) store_partial4<false, T>(to + 16 * (wave * DT + n) + 4 * g, acc[c][n], inv);
+      } else {
+        const int64_t cs = (int64_t)cur.slot * COLS + i;
+        float* to = a.part_acc + cs * L;
+#pragma unroll
+        for (int n = 0; n < DT; ++n) store_partial4<false, float>(to + 16 * (wave * DT + n) + 4 * g, acc[c][n], inv);
+        // (A NaN sum keeps a finite maximum: the merge passes over a partial
+        // whose maximum is -inf.)
+        const float m = col_max[i];
+        if (wave == 0 && g == 0)
+          *reinterpret_cast<float2*>(a.part_ml + cs * 2) = make_float2(l_tot == l_tot || m != -INFINITY ? m : 0.f, l_tot);
+      }
+    }
+    if (cur.next < 0) return false;
+    // (The next piece's queries arrive with its first tile: the wait at the top
+    // of a step is for both.)
+    cur = read_latent_piece(pieces, cur.next);
+    load_queries(ln, cur);
+    t0 = cur.tok_begin;
+    fresh = true;
     return true;
   };
   while (step(tile0, tile1) && step(tile1, tile0)) {
@@ -526,6 +541,7 @@ __global__ __launch_bounds__(L / 4) void latent_merge_kernel(const int32_t* __re
   const float* ml = a.part_ml + ((int64_t)slot0 * cols + i) * 2;
   const int64_t ml_step = 2 * cols;
   float m = -INFINITY;
+#pragma unroll 8
   for (int k = 0; k < np; ++k) m = fmaxf(m, ml[k * ml_step]);
   const float* from = a.part_acc + ((int64_t)slot0 * cols + i) * L + 4 * threadIdx.x;
   f32x4 sum = {0.f, 0.f, 0.f, 0.f};
@@ -550,6 +566,7 @@ static const void* latent_decode_fn(int col_tiles) {
     case 1: return (const void*)&latent_decode_kernel<T, L, P, 1>;
     case 2: return (const void*)&latent_decode_kernel<T, L, P, 2>;
     case 4: return (const void*)&latent_decode_kernel<T, L, P, 4>;
+    case 8: return (const void*)&latent_decode_kernel<T, L, P, 8>;
     default: return nullptr;
   }
 }
@@ -567,7 +584,7 @@ extern "C" int lvamd_latent_decode_resident_groups(int32_t dtype, int32_t latent
     if (!fn) return LVAMD_ERR_UNSUPPORTED;
     if (hipGetDevice(&device) != hipSuccess) return LVAMD_ERR_LAUNCH;
     if (hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, device) != hipSuccess) return LVAMD_ERR_LAUNCH;
-    if (hipOccupancyMaxActiveBlocksPerMultiprocessor(&per_cu, fn, 64 * kWaves, 0) != hipSuccess) return LVAMD_ERR_LAUNCH;
+    if (hipOccupancyMaxActiveBlocksPerMultiprocessor(&per_cu, fn, col_tiles >= 4 ? 512 : 256, 0) != hipSuccess) return LVAMD_ERR_LAUNCH;
     return per_cu * cus;
   });
 }
@@ -575,7 +592,7 @@ extern "C" int lvamd_latent_decode_resident_groups(int32_t dtype, int32_t latent
 extern "C" int lvamd_latent_decode(const void* query, int64_t query_token_stride, int64_t query_head_stride,
                                    const void* query_rope, int64_t rope_token_stride, int64_t rope_head_stride,
                                    const void* pool, void* out, int64_t out_token_stride, int64_t out_head_stride,
-                                   const int32_t* pieces, const int32_t* group_first, int32_t num_groups,
+                                   const int32_t* pieces, int32_t num_groups,
                                    const int32_t* jobs, int32_t num_jobs, int32_t merge_columns, const int32_t* tables,
                                    const uint32_t* vis, float* part_acc, float* part_ml, int64_t num_partial_slots,
                                    int32_t num_heads, int32_t latent_size, int32_t rope_size, int32_t col_tiles,
@@ -585,7 +602,7 @@ extern "C" int lvamd_latent_decode(const void* query, int64_t query_token_stride
       merge_columns > 65535)
     return LVAMD_ERR_INVALID_ARGUMENT;
   if (num_groups == 0) return LVAMD_OK;
-  if (!query || !query_rope || !pool || !out || !pieces || !group_first || !tables || !vis || (num_jobs > 0 && !jobs))
+  if (!query || !query_rope || !pool || !out || !pieces || !tables || !vis || (num_jobs > 0 && !jobs))
     return LVAMD_ERR_INVALID_ARGUMENT;
   if (num_partial_slots > 0 && (!part_acc || !part_ml)) return LVAMD_ERR_WORKSPACE;
   if (!rows16(query, {query_token_stride, query_head_stride}) || !rows16(query_rope, {rope_token_stride, rope_head_stride}) ||
@@ -611,11 +628,15 @@ extern "C" int lvamd_latent_decode(const void* query, int64_t query_token_stride
   a.scale_log2 = scale * 1.4426950408889634f;
   hipStream_t s = static_cast<hipStream_t>(stream);
   return latent_dispatch(dtype, latent_size, rope_size, [&]<typename T, int L, int P>() -> int {
-    const dim3 grid((unsigned)num_groups), block(64 * kWaves);
+    auto launch = [&]<int NC>() {
+      hipLaunchKernelGGL((latent_decode_kernel<T, L, P, NC>), dim3((unsigned)num_groups), dim3(64 * LatentShape<L, P, NC>::W),
+                         0, s, pieces, a);
+    };
     switch (col_tiles) {
-      case 1: hipLaunchKernelGGL((latent_decode_kernel<T, L, P, 1>), grid, block, 0, s, group_first, pieces, a); break;
-      case 2: hipLaunchKernelGGL((latent_decode_kernel<T, L, P, 2>), grid, block, 0, s, group_first, pieces, a); break;
-      case 4: hipLaunchKernelGGL((latent_decode_kernel<T, L, P, 4>), grid, block, 0, s, group_first, pieces, a); break;
+      case 1: launch.template operator()<1>(); break;
+      case 2: launch.template operator()<2>(); break;
+      case 4: launch.template operator()<4>(); break;
+      case 8: launch.template operator()<8>(); break;
       default: return LVAMD_ERR_UNSUPPORTED;
     }
     if (const int status = launch_status(); status != LVAMD_OK) return status;

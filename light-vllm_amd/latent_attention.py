@@ -28,7 +28,7 @@ from light_vllm_amd.plan import DECODE_MERGE_PIECES, PREFILL_MIN_TILES, StepPlan
 from light_vllm_amd.quantized_cache import on_device
 
 # Column tiles (of 16) per workgroup that the latent-space kernel is built for.
-COL_TILES = (1, 2, 4)
+COL_TILES = (1, 2, 4, 8)
 WEIGHT_SIZES = (64, 128)
 # Queries per unit, keys per tile and rows per expanded block of the chunk kernels.
 UNIT_QUERIES, UNIT_KEYS = 128, 64
@@ -132,7 +132,7 @@ class LatentStepPlan(StepPlan):
         long = np.zeros(self.batch_size, bool) if weights is None else _expanded(facts, spec, *weights)
         short = ~long
         x = _Shape()
-        pieces = first = jobs = rows = blocks = units = unit_jobs = none
+        pieces = jobs = rows = blocks = units = unit_jobs = none
         x.num_groups = x.num_jobs = x.num_slots = x.merge_columns = x.num_rows = 0
         x.row_base, x.row_span, x.every_row, x.col_tiles = 0, 0, True, COL_TILES[0]
         x.num_blocks = x.num_units = x.num_unit_jobs = x.unit_merge_columns = x.num_unit_slots = 0
@@ -144,8 +144,8 @@ class LatentStepPlan(StepPlan):
             x.row_span = int(mine[-1, 4] + mine[-1, 3]) - x.row_base
             found = host.latent_work(mine, facts.flat, heads, x.col_tiles, resident, self.block_size,
                                      int(native.load().lvamd_latent_decode_tile_tokens()), DECODE_MERGE_PIECES)
-            pieces, first, jobs = (np.frombuffer(a, dtype=np.int32) for a in found[:3])
-            x.num_groups, x.num_slots, x.merge_columns = int(found[3]), int(found[5]), int(found[6])
+            pieces, jobs = (np.frombuffer(a, dtype=np.int32) for a in found[:2])
+            x.num_groups, x.num_slots, x.merge_columns = (int(v) for v in found[2:5])
             x.num_jobs = jobs.size // native.MERGE_FIELDS
             x.num_rows = int(facts.q_lens[short].sum())
             x.every_row = x.num_rows == x.row_span
@@ -171,7 +171,7 @@ class LatentStepPlan(StepPlan):
         columns = x.num_slots * 16 * x.col_tiles
         x.acc_bytes = columns * spec.latent_size * 4
         x.latent_bytes = x.acc_bytes + columns * 8
-        x.lists = _Lists(pieces=pieces, first=first, jobs=jobs, rows=rows, blocks=blocks.reshape(-1), units=units,
+        x.lists = _Lists(pieces=pieces, jobs=jobs, rows=rows, blocks=blocks.reshape(-1), units=units,
                          unit_jobs=unit_jobs)
         return x
 
@@ -274,7 +274,7 @@ class HipLatentPagedAttention:
         native.check(native.load().lvamd_latent_decode(
             query.data_ptr() - base * query.stride(0) * es, query.stride(0), query.stride(1), query_rope.data_ptr(),
             query_rope.stride(0), query_rope.stride(1), rows.data_ptr(), out.data_ptr() - base * out.stride(0) * es,
-            out.stride(0), out.stride(1), lists.pieces, lists.first, shape.num_groups, lists.jobs, shape.num_jobs,
+            out.stride(0), out.stride(1), lists.pieces, shape.num_groups, lists.jobs, shape.num_jobs,
             shape.merge_columns, plan.tables_ptr, plan.vis_ptr, acc, None if acc is None else acc + shape.acc_bytes,
             shape.num_slots, spec.num_query_heads, spec.latent_size, spec.rope_size, shape.col_tiles, plan.block_size,
             float(scale), code, stream), "lvamd_latent_decode")

@@ -78,7 +78,7 @@ def test_the_library_refuses_bad_arguments() -> None:
     assert lib.lvamd_latent_move(p, 2, 1152, p, p, 3, p, 3 * 2 * 1152 - 1, None) == -3
     assert lib.lvamd_latent_move(p, 2, 1152, p, None, 3, None, 0, None) == -1
     decode = lambda **k: lib.lvamd_latent_decode(*{**dict(  # noqa: E731
-        q=p, qt=8, qh=8, qr=p, rt=8, rh=8, pool=p, out=p, ot=8, oh=8, pieces=p, first=p, groups=1, jobs=None, njobs=0,
+        q=p, qt=8, qh=8, qr=p, rt=8, rh=8, pool=p, out=p, ot=8, oh=8, pieces=p, groups=1, jobs=None, njobs=0,
         cols=1, tables=p, vis=p, acc=None, ml=None, slots=0, heads=1, size=512, rope=64, tiles=1, block=16, scale=1.0,
         dtype=native.DTYPE_F16, stream=None), **k}.values())
     for bad, status in ((dict(size=576), -2), (dict(dtype=native.DTYPE_F32), -2), (dict(tiles=3), -2), (dict(groups=-1), -1),
@@ -144,7 +144,7 @@ def test_rotary_needs_a_gpu() -> None:
 def test_pieces_cover_every_column_group_once(seed) -> None:
     rng = np.random.default_rng(seed)
     bs, heads = int(rng.choice((1, 12, 16, 64))), int(rng.choice((1, 5, 16, 128)))
-    tiles, resident = int(rng.choice((1, 2, 4))), int(rng.choice((3, 64, 512)))
+    tiles, resident = int(rng.choice((1, 2, 4, 8))), int(rng.choice((3, 64, 512)))
     computed, layouts = [], []
     for _ in range(int(rng.integers(1, 9))):
         n = int(rng.choice((1, 1, 2, 9, 33, 70)))
@@ -158,14 +158,24 @@ def test_pieces_cover_every_column_group_once(seed) -> None:
                                    query_layouts=tuple(lv.QueryLayout(p) for p in layouts))
     plan = StepPlan(md, block_size=bs, device=CPU, num_blocks=sum(need))
     found = native.host().latent_work(plan._req_meta, plan.facts.flat, heads, tiles, resident, bs, 32, 256)
-    pieces, first, jobs, groups, _, slots, most, _, depth = found
+    pieces, jobs, groups, slots, most, depth = found
     pieces = np.frombuffer(pieces, np.int32).reshape(-1, native.PIECE_FIELDS)
-    first = np.frombuffer(first, np.int32)
     jobs = np.frombuffer(jobs, np.int32).reshape(-1, native.MERGE_FIELDS)
     assert groups <= resident or groups * 32 * 256 >= sum(c + len(p) for c, p in zip(computed, layouts))
-    assert len(first) == groups + 1 and first[0] == 0 and first[-1] == len(pieces) and np.all(np.diff(first) > 0)
+    order = []  # as the workgroups walk them
+    for w in range(groups):
+        while w >= 0:
+            order.append(w)
+            w = int(pieces[w][11])
+    assert sorted(order) == list(range(len(pieces)))
     by_segment: dict = {}
-    for x in pieces:
+    for x in pieces[order]:
+        off, lb = sum(need[:x[0]]), x[2] // bs
+        if (x[2] % bs + 31) // bs >= 4:
+            assert (x[12:] == -1).all()
+        else:
+            table = tables[x[0]][lb:-(-int(x[3]) // bs)][:4]
+            assert tuple(x[12:12 + len(table)]) == table
         by_segment.setdefault((int(x[0]), int(x[1])), []).append(x)
         off = sum(need[:x[0]])
         assert x[5] == off and x[6] == computed[x[0]] and x[7] == len(layouts[x[0]])
