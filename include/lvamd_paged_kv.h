@@ -735,8 +735,11 @@ int64_t lvamd_latent_move_workspace_size(int64_t num_pairs, int32_t num_layers, 
 
 /*
  * Attention in latent space: query [tokens][heads][latent_size] (multiplied by
- * the heads' key weights), query_rope [tokens][heads][rope_size] (turned), out
+ * the heads' key weights), query_rope [tokens][heads][rope_size], out
  * [tokens][heads][latent_size] (to be multiplied by the heads' value weights).
+ * With latent and rope_key (else NULL: the pool holds them; NULL with col_tiles 8)
+ * the launch appends the step's rows; with cosines and sines (as lvamd_latent_append's) it turns
+ * query_rope and those keys first.
  * jobs as lvamd_paged_decode's with one kv head and 16 * col_tiles columns a slot
  * (col_tiles: 1, 2, 4 or 8); pieces likewise up to field 10, then the index of the
  * workgroup's next piece (-1: none) and its first four table entries (-1: not
@@ -745,8 +748,10 @@ int64_t lvamd_latent_move_workspace_size(int64_t num_pairs, int32_t num_layers, 
  */
 int lvamd_latent_decode(const void* query, int64_t query_token_stride, int64_t query_head_stride,
                         const void* query_rope, int64_t rope_token_stride, int64_t rope_head_stride,
-                        const void* pool, void* out, int64_t out_token_stride, int64_t out_head_stride,
-                        const int32_t* pieces, int32_t num_groups, const int32_t* jobs, int32_t num_jobs,
+                        const void* latent, int64_t latent_token_stride, const void* rope_key,
+                        int64_t rope_key_token_stride, const float* cosines, const float* sines,
+                        int64_t angle_token_stride, int32_t interleaved, void* pool, void* out,
+                        int64_t out_token_stride, int64_t out_head_stride, const int32_t* pieces, int32_t num_groups, const int32_t* jobs, int32_t num_jobs,
                         int32_t merge_columns, const int32_t* tables,
                         const uint32_t* vis, float* part_acc, float* part_ml, int64_t num_partial_slots,
                         int32_t num_heads, int32_t latent_size, int32_t rope_size, int32_t col_tiles,

@@ -43,6 +43,49 @@ int latent_dispatch(int dtype, int latent, int rope, F f) {
   }
 }
 
+// A pair turned by an angle of cosine c and sine s.  (Written as these products,
+// so that every kernel rounds alike.)
+__device__ __forceinline__ void turn_pair(float x, float y, float c, float s, float& a, float& b) {
+  a = __builtin_fmaf(x, c, -(y * s));
+  b = __builtin_fmaf(y, c, x * s);
+}
+// Eight values, four pairs (2i, 2i + 1); c and s are four floats each, 16-byte aligned.
+template <typename T>
+__device__ __forceinline__ uint4 turn_chunk(uint4 x, const float* c, const float* s) {
+  const f32x4 cv = *reinterpret_cast<const f32x4*>(c), sv = *reinterpret_cast<const f32x4*>(s);
+  T e[8];
+  __builtin_memcpy(e, &x, 16);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    float a, b;
+    turn_pair(to_f32(e[2 * i]), to_f32(e[2 * i + 1]), cv[i], sv[i], a, b);
+    e[2 * i] = from_f32<T>(a);
+    e[2 * i + 1] = from_f32<T>(b);
+  }
+  __builtin_memcpy(&x, e, 16);
+  return x;
+}
+// Sixteen values, eight pairs (lo i, hi i).
+template <typename T>
+__device__ __forceinline__ void turn_chunks(uint4& lo, uint4& hi, const float* c, const float* s) {
+  T x[8], y[8];
+  __builtin_memcpy(x, &lo, 16);
+  __builtin_memcpy(y, &hi, 16);
+#pragma unroll
+  for (int i = 0; i < 8; i += 4) {
+    const f32x4 cv = *reinterpret_cast<const f32x4*>(c + i), sv = *reinterpret_cast<const f32x4*>(s + i);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      float a, b;
+      turn_pair(to_f32(x[i + k]), to_f32(y[i + k]), cv[k], sv[k], a, b);
+      x[i + k] = from_f32<T>(a);
+      y[i + k] = from_f32<T>(b);
+    }
+  }
+  __builtin_memcpy(&lo, x, 16);
+  __builtin_memcpy(&hi, y, 16);
+}
+
 // Whether rows at p, of these element strides, are made of whole 16-byte chunks.
 inline bool rows16(const void* p, std::initializer_list<int64_t> strides) {
   if (((uintptr_t)p & 15u) != 0) return false;

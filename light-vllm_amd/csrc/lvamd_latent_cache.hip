@@ -86,36 +86,13 @@ template <typename T, Layout K>
 __device__ __forceinline__ void turn(const T* src, T* dst, int w, int pairs, const float* cs, const float* sn) {
   if constexpr (K == Layout::kNone) {
     store16((gptr<T>)(dst + 8 * w), load16(src + 8 * w));
+  } else if constexpr (K == Layout::kInterleaved) {
+    store16((gptr<T>)(dst + 8 * w), turn_chunk<T>(load16(src + 8 * w), cs + 4 * w, sn + 4 * w));
   } else {
-    // Pairs (x, y): four of one chunk, or eight of two chunks half a vector apart.
-    constexpr int N = K == Layout::kHalf ? 8 : 4;
-    T in[2 * N], out[2 * N];
-    float c[N], s[N];
-    const uint4 lo = load16(src + 8 * w);
-    __builtin_memcpy(in, &lo, 16);
-    if constexpr (K == Layout::kHalf) {
-      const uint4 hi = load16(src + 8 * w + pairs);
-      __builtin_memcpy(in + 8, &hi, 16);
-    }
-#pragma unroll
-    for (int i = 0; i < N; i += 4) {
-      __builtin_memcpy(c + i, cs + N * w + i, 16);
-      __builtin_memcpy(s + i, sn + N * w + i, 16);
-    }
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int a = K == Layout::kHalf ? i : 2 * i, b = K == Layout::kHalf ? i + 8 : 2 * i + 1;
-      const float x = to_f32(in[a]), y = to_f32(in[b]);
-      out[a] = from_f32<T>(x * c[i] - y * s[i]);
-      out[b] = from_f32<T>(y * c[i] + x * s[i]);
-    }
-    uint4 r;
-    __builtin_memcpy(&r, out, 16);
-    store16((gptr<T>)(dst + 8 * w), r);
-    if constexpr (K == Layout::kHalf) {
-      __builtin_memcpy(&r, out + 8, 16);
-      store16((gptr<T>)(dst + 8 * w + pairs), r);
-    }
+    uint4 lo = load16(src + 8 * w), hi = load16(src + 8 * w + pairs);
+    turn_chunks<T>(lo, hi, cs + 8 * w, sn + 8 * w);
+    store16((gptr<T>)(dst + 8 * w), lo);
+    store16((gptr<T>)(dst + 8 * w + pairs), hi);
   }
 }
 

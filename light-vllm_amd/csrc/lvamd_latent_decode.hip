@@ -6,7 +6,7 @@
 //
 // Query j of a request with c computed tokens sees logical positions [0, c) and
 // {c + i : i <= j} (linear) or {c + i : i an ancestor of j, or j} (tree).  The
-// step's tokens are in the cache already.
+// step's tokens are in the cache already, or the launch appends them.
 //
 // Mapping onto CDNA4:
 //   * A column is a (query, head) pair of one request; a workgroup (four waves, or
@@ -24,6 +24,9 @@
 //     LDS (the accumulator layout of S^T is the operand layout of P^T).
 //   * The waves share each column's running maximum, which moves only when some
 //     score passes it by 2^8 (lazy rescaling): a vote per tile in LDS.
+//   * Append: a tile's rows of this step are loaded from the step's tensors, and
+//     one column group writes them to the pool; keys and queries are turned on the
+//     way.  It saves the append's launch (4-6 us with its gap).
 //   * A tile has two barriers: its rows are there, its probabilities are there.
 //
 // LDS tile layout: groups of 64 columns (128 bytes of every row), group-major;
@@ -51,14 +54,21 @@ struct LatentDecodeArgs {
   int64_t q_tok_stride, q_head_stride;
   const void* qr;  // [tokens][heads][P], the rotated part
   int64_t qr_tok_stride, qr_head_stride;
-  const void* pool;  // [slots][L + P]
-  void* out;         // [tokens][heads][L]
+  void* pool;  // [slots][L + P]
+  // The step's rows, where this launch appends them, or null: the pool has them.
+  const void* latent_new;
+  const void* rope_new;
+  int64_t latent_stride, rope_stride;
+  const float* cosines;  // [tokens][P / 2], or null: queries and keys are turned already
+  const float* sines;
+  int64_t angle_stride;
+  void* out;  // [tokens][heads][L]
   int64_t out_tok_stride, out_head_stride;
   const int32_t* __restrict__ tables;
   const uint32_t* __restrict__ vis;
   float* part_acc;  // [slots][16 NC][L] fp32, rows normalised
   float* part_ml;   // [slots][16 NC][2]: (max, sum)
-  int32_t heads, block_size;
+  int32_t heads, block_size, interleaved;
   FastDiv by_block, by_heads;
   float scale_log2;
 };
@@ -95,6 +105,7 @@ struct LatentShape {
   static constexpr int QKS = NC == 8 ? 2 : 1;         // 16-row halves a wave scores
   static constexpr int NB = 2;                        // tiles in LDS
   static constexpr int WAVES_PER_EU = 2;
+  static constexpr bool APPEND = NC < 8;              // (128 columns: no registers left for it)
   static_assert(L % 128 == 0 && P % 32 == 0);
 };
 
@@ -112,6 +123,7 @@ __attribute__((amdgpu_waves_per_eu(LatentShape<L, P, NC>::WAVES_PER_EU))) void l
   using S = LatentShape<L, P, NC>;
   constexpr int GR = S::GR, KSTEPS = S::KSTEPS, DT = S::DT, QKS = S::QKS, W = S::W;
   constexpr int COLS = 16 * NC;
+  constexpr bool APPEND = S::APPEND;
   using V8 = typename std::conditional<std::is_same<T, __bf16>::value, bf16x8, f16x8>::type;
   // Separate objects: a load into one does not alias a read of another.
   __shared__ __attribute__((aligned(1024))) char tile0[S::TILE_BYTES];
@@ -126,25 +138,36 @@ __attribute__((amdgpu_waves_per_eu(LatentShape<L, P, NC>::WAVES_PER_EU))) void l
 
   // ---- this wave's scores: rows [16 ks0, 16 (ks0 + QKS)) of a tile, column tile ct0.
   const bool scores = NC > 1 || wave < 2;
-  const int ks0 = NC == 8 ? 0 : wave & 1;
-  const int ct0 = NC == 1 ? 0 : NC == 8 ? wave : wave >> 1;
+  const int ks0 = QKS == 2 ? 0 : wave & 1;
+  const int ct0 = NC == 1 ? 0 : QKS == 2 ? wave : wave >> 1;
 
   // ---- tile loads: wave w loads rows 8 (w % 4) .. + 7 of the groups w / 4, + W / 4,
   // ..; lane l row l / 8 of them into chunk slot l % 8 of a group.
   constexpr int GSTEP = W / 4;
   const int rb = wave & 3;
+  // The load cursor: the tile whose rows are looked up next.  first_new: the
+  // position from which rows are the step's own, read from its tensors.
+  struct Cursor {
+    int table_off, t0, tok_end, next;  // tok_end 0: no more tiles
+    int first_new, q_start;
+  };
   struct Row {
-    int entry, off;
+    int entry, off, tok;  // tok: of the step, or -1
   };
-  auto lookup = [&](int ln, int table_off, int t0, int tok_end) -> Row {
-    const int pos = min(t0 + 8 * rb + (ln >> 3), tok_end - 1);
+  auto first_new = [&](int computed) { return APPEND && a.latent_new ? computed : 0x7fffffff; };
+  auto lookup = [&](int ln, const Cursor& c) -> Row {
+    const int pos = min(c.t0 + 8 * rb + (ln >> 3), c.tok_end - 1);
     const int lb = fast_div(pos, a.by_block);
-    return {a.tables[table_off + lb], pos - lb * a.block_size};
+    return {a.tables[c.table_off + lb], pos - lb * a.block_size, pos >= c.first_new ? c.q_start + pos - c.first_new : -1};
   };
-  gptr<const T> const pool = (gptr<const T>)(a.pool);
+  gptr<T> const pool = (gptr<T>)(a.pool);
   auto issue = [&](int ln, const Row& r, char* dst) {
     const int lchunk = (ln & 7) ^ swizzle(8 * rb + (ln >> 3));
-    gptr<const T> const row = pool + ((int64_t)r.entry * a.block_size + r.off) * S::ROW;
+    gptr<const T> row = pool + ((int64_t)r.entry * a.block_size + r.off) * S::ROW, key = row;
+    if (APPEND && __any(r.tok >= 0)) {
+      row = r.tok >= 0 ? (gptr<const T>)(a.latent_new) + r.tok * a.latent_stride : row;
+      key = r.tok >= 0 ? (gptr<const T>)(a.rope_new) + r.tok * a.rope_stride - L : key;
+    }
 #pragma unroll
     for (int i = 0; i < (GR + GSTEP - 1) / GSTEP; ++i) {
       const int gr = (wave >> 2) + i * GSTEP;
@@ -153,7 +176,8 @@ __attribute__((amdgpu_waves_per_eu(LatentShape<L, P, NC>::WAVES_PER_EU))) void l
       // (A half-used last group's spare slots take the row's last chunk again.)
       if (8 * GR > S::CPR && gr == GR - 1) c = min(c, S::CPR - 1);
       // Non-temporal: a launch reads a row once, or a few column groups do at once.
-      __builtin_amdgcn_global_load_lds((lds_gptr)(row + 8 * c), (lds_lptr)(dst + (gr * KT * 128 + rb * 1024)), 16, 0, 2);
+      __builtin_amdgcn_global_load_lds((lds_gptr)((gr < L / 64 ? row : key) + 8 * c),
+                                       (lds_lptr)(dst + (gr * KT * 128 + rb * 1024)), 16, 0, 2);
     }
   };
 
@@ -195,14 +219,29 @@ __attribute__((amdgpu_waves_per_eu(LatentShape<L, P, NC>::WAVES_PER_EU))) void l
     const T* q = static_cast<const T*>(a.q) + (int64_t)(x.q_start + qi0) * a.q_tok_stride + (int64_t)head * a.q_head_stride + 8 * g;
     const T* qr = static_cast<const T*>(a.qr) + (int64_t)(x.q_start + qi0) * a.qr_tok_stride +
                   (int64_t)head * a.qr_head_stride + 8 * g;
+    const bool mine = scores && ok;
 #pragma unroll
-    for (int k = 0; k < KSTEPS; ++k) qf[k] = scores && ok ? load16(32 * k < L ? q + 32 * k : qr + 32 * k - L) : zero_u4();
+    for (int k = 0; k < KSTEPS; ++k) qf[k] = mine ? load16(32 * k < L ? q + 32 * k : qr + 32 * k - L) : zero_u4();
+    if (APPEND && a.cosines) {
+      // Turned here: chunk (32 k - L) / 8 + g of the rotated part.
+      const float* cs = a.cosines + (int64_t)(x.q_start + qi0) * a.angle_stride;
+      const float* sn = a.sines + (int64_t)(x.q_start + qi0) * a.angle_stride;
+#pragma unroll
+      for (int k = L / 32; k < KSTEPS; ++k) {
+        const int c = (32 * k - L) / 8 + g;
+        if (mine && a.interleaved) qf[k] = turn_chunk<T>(qf[k], cs + 4 * c, sn + 4 * c);
+        if (mine && !a.interleaved) {
+          constexpr int HALF = P / 16;  // chunks of half a vector
+          const int at = 8 * (c & (HALF - 1));
+          uint4 lo = load16(qr - 8 * g + 8 * (c & (HALF - 1))), hi = load16(qr - 8 * g + 8 * (c | HALF));
+          turn_chunks<T>(lo, hi, cs + at, sn + at);
+          const bool low = c < HALF;
+          qf[k] = make_uint4(low ? lo.x : hi.x, low ? lo.y : hi.y, low ? lo.z : hi.z, low ? lo.w : hi.w);
+        }
+      }
+    }
   };
 
-  // The load cursor: the tile whose rows are looked up next.
-  struct Cursor {
-    int table_off, t0, tok_end, next;  // tok_end 0: no more tiles
-  };
   auto advance = [&](Cursor& c) {
     c.t0 += KT;
     if (c.t0 >= c.tok_end) {
@@ -214,10 +253,12 @@ __attribute__((amdgpu_waves_per_eu(LatentShape<L, P, NC>::WAVES_PER_EU))) void l
       c.t0 = r[2];
       c.tok_end = r[3];
       c.table_off = r[5];
+      c.first_new = first_new(r[6]);
+      c.q_start = r[8];
       c.next = r[11];
     }
   };
-  Cursor at = {cur.table_off, cur.tok_begin, cur.tok_end, cur.next};
+  Cursor at = {cur.table_off, cur.tok_begin, cur.tok_end, cur.next, first_new(cur.computed), cur.q_start};
   Row row;
   {
     // The first tile's rows lie in the record's blocks.
@@ -226,15 +267,16 @@ __attribute__((amdgpu_waves_per_eu(LatentShape<L, P, NC>::WAVES_PER_EU))) void l
     if (b0 >= 0) {
       const int pos = min(at.t0 + 8 * rb + (lane >> 3), at.tok_end - 1);
       const int lb = fast_div(pos, a.by_block), k = lb - fast_div(at.t0, a.by_block);
-      row = {k == 0 ? b0 : k == 1 ? b1 : k == 2 ? b2 : b3, pos - lb * a.block_size};
+      row = {k == 0 ? b0 : k == 1 ? b1 : k == 2 ? b2 : b3, pos - lb * a.block_size,
+             pos >= at.first_new ? at.q_start + pos - at.first_new : -1};
     } else {
-      row = lookup(lane, at.table_off, at.t0, at.tok_end);
+      row = lookup(lane, at);
     }
   }
   issue(lane, row, tile0);
   load_queries(lane, cur);
   advance(at);
-  if (at.tok_end > 0) row = lookup(lane, at.table_off, at.t0, at.tok_end);
+  if (at.tok_end > 0) row = lookup(lane, at);
 
   float m_run, l_run;
   f32x4 acc[NC][DT];
@@ -265,7 +307,7 @@ __attribute__((amdgpu_waves_per_eu(LatentShape<L, P, NC>::WAVES_PER_EU))) void l
     if (at.tok_end > 0) {
       issue(ln, row, there);
       advance(at);
-      if (at.tok_end > 0) row = lookup(ln, at.table_off, at.t0, at.tok_end);
+      if (at.tok_end > 0) row = lookup(ln, at);
     }
     if (fresh) {
       m_run = -INFINITY;
@@ -278,6 +320,44 @@ __attribute__((amdgpu_waves_per_eu(LatentShape<L, P, NC>::WAVES_PER_EU))) void l
       fresh = false;
     }
     const bool masked = t0 + KT > min(cur.computed, cur.tok_end);
+    // ---- the step's own rows among the tile's: their keys are turned in LDS; the
+    // group with a token's first column writes its row to the pool (below, behind the
+    // tile's matrix work: the table's entry is on its way meanwhile).
+    int slot = -1;
+    if (APPEND && masked && a.latent_new) {
+      const int pos = t0 + 8 * rb + (ln >> 3), j = pos - cur.computed;
+      const int col = j * a.heads - cur.group * COLS, lb = fast_div(pos, a.by_block);
+      const bool mine = j >= 0 && pos < cur.tok_end && col >= 0 && col < COLS;
+      int entry = 0;
+      if (mine) entry = a.tables[cur.table_off + lb];
+      if (a.cosines) {
+        constexpr int HALF = P / 16;
+        const int per = a.interleaved ? 2 * HALF : HALF;  // chunks, or pairs of them, of a key
+        for (int i = tid; i < KT * per; i += 64 * W) {
+          const int r = i / per, c = i - r * per, pos = t0 + r;
+          if (pos < cur.computed || pos >= cur.tok_end) continue;
+          const int64_t tok = cur.q_start + pos - cur.computed;
+          auto chunk = [&](int ch) -> uint4* {  // of the key
+            const int full = L / 8 + ch;
+            return reinterpret_cast<uint4*>(const_cast<char*>(here) +
+                                            ((full >> 3) * (KT * 128) + r * 128 + 16 * ((full & 7) ^ swizzle(r))));
+          };
+          const float* cs = a.cosines + tok * a.angle_stride;
+          const float* sn = a.sines + tok * a.angle_stride;
+          if (a.interleaved) {
+            *chunk(c) = turn_chunk<T>(*chunk(c), cs + 4 * c, sn + 4 * c);
+          } else {
+            uint4 lo = *chunk(c), hi = *chunk(c + HALF);
+            turn_chunks<T>(lo, hi, cs + 8 * c, sn + 8 * c);
+            *chunk(c) = lo;
+            *chunk(c + HALF) = hi;
+          }
+        }
+        lds_barrier();
+      }
+      if (mine) slot = entry * a.block_size + (pos - lb * a.block_size);
+      __builtin_amdgcn_s_waitcnt(wait_vm(0));
+    }
 
     // ---- scores
     f32x4 st[QKS];
@@ -389,6 +469,18 @@ __attribute__((amdgpu_waves_per_eu(LatentShape<L, P, NC>::WAVES_PER_EU))) void l
       lds_barrier();
       if (scores && g == 0 && ks0 == 0) col_max[16 * ct0 + l16] = m_run;
     }
+    if (APPEND && masked && __any(slot >= 0)) {
+      if (slot >= 0) {
+        const int lchunk = (ln & 7) ^ swizzle(8 * rb + (ln >> 3));
+        gptr<T> const to = pool + (int64_t)slot * S::ROW;
+#pragma unroll
+        for (int i = 0; i < (GR + GSTEP - 1) / GSTEP; ++i) {
+          const int gr = (wave >> 2) + i * GSTEP, c = 8 * gr + lchunk;
+          if (c < S::CPR)
+            store16(to + 8 * c, *reinterpret_cast<const uint4*>(here + (gr * (KT * 128) + rb * 1024 + ln * 16)));
+        }
+      }
+    }
     const bool poisoned = (said & 2u) != 0;
     if (poisoned) {
       // The step's rows without their values that are not finite (and none of
@@ -459,7 +551,8 @@ __attribute__((amdgpu_waves_per_eu(LatentShape<L, P, NC>::WAVES_PER_EU))) void l
       for (int pos = max(t0, cur.computed); pos < min(t0 + KT, cur.tok_end); ++pos) {
         const int lb = fast_div(pos, a.by_block);
         gptr<const T> const v =
-            pool + ((int64_t)a.tables[cur.table_off + lb] * a.block_size + (pos - lb * a.block_size)) * S::ROW;
+            APPEND && a.latent_new ? (gptr<const T>)(a.latent_new) + (int64_t)(cur.q_start + pos - cur.computed) * a.latent_stride
+                         : pool + ((int64_t)a.tables[cur.table_off + lb] * a.block_size + (pos - lb * a.block_size)) * S::ROW;
         uint32_t sees = 0;  // bit c: this lane's column of tile c
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
@@ -591,7 +684,10 @@ extern "C" int lvamd_latent_decode_resident_groups(int32_t dtype, int32_t latent
 
 extern "C" int lvamd_latent_decode(const void* query, int64_t query_token_stride, int64_t query_head_stride,
                                    const void* query_rope, int64_t rope_token_stride, int64_t rope_head_stride,
-                                   const void* pool, void* out, int64_t out_token_stride, int64_t out_head_stride,
+                                   const void* latent, int64_t latent_token_stride, const void* rope_key,
+                                   int64_t rope_key_token_stride, const float* cosines, const float* sines,
+                                   int64_t angle_token_stride, int32_t interleaved, void* pool, void* out,
+                                   int64_t out_token_stride, int64_t out_head_stride,
                                    const int32_t* pieces, int32_t num_groups,
                                    const int32_t* jobs, int32_t num_jobs, int32_t merge_columns, const int32_t* tables,
                                    const uint32_t* vis, float* part_acc, float* part_ml, int64_t num_partial_slots,
@@ -608,7 +704,20 @@ extern "C" int lvamd_latent_decode(const void* query, int64_t query_token_stride
   if (!rows16(query, {query_token_stride, query_head_stride}) || !rows16(query_rope, {rope_token_stride, rope_head_stride}) ||
       !rows16(pool, {}) || ((uintptr_t)out & 7u) || out_token_stride % 4 != 0 || out_head_stride % 4 != 0)
     return LVAMD_ERR_INVALID_ARGUMENT;
+  if (col_tiles > 4 && (latent || cosines)) return LVAMD_ERR_UNSUPPORTED;
+  if ((latent == nullptr) != (rope_key == nullptr) || (cosines == nullptr) != (sines == nullptr) ||
+      (latent && (!rows16(latent, {latent_token_stride}) || !rows16(rope_key, {rope_key_token_stride}))) ||
+      (cosines && (((uintptr_t)cosines & 15u) || ((uintptr_t)sines & 15u) || angle_token_stride % 4 != 0)))
+    return LVAMD_ERR_INVALID_ARGUMENT;
   LatentDecodeArgs a{.by_block = FastDiv(block_size), .by_heads = FastDiv(num_heads)};
+  a.latent_new = latent;
+  a.rope_new = rope_key;
+  a.latent_stride = latent_token_stride;
+  a.rope_stride = rope_key_token_stride;
+  a.cosines = cosines;
+  a.sines = sines;
+  a.angle_stride = angle_token_stride;
+  a.interleaved = interleaved;
   a.q = query;
   a.q_tok_stride = query_token_stride;
   a.q_head_stride = query_head_stride;

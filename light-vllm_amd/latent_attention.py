@@ -29,6 +29,8 @@ from light_vllm_amd.quantized_cache import on_device
 
 # Column tiles (of 16) per workgroup that the latent-space kernel is built for.
 COL_TILES = (1, 2, 4, 8)
+# Widest workgroup whose launch appends the step's rows itself.
+APPEND_TILES = 4
 WEIGHT_SIZES = (64, 128)
 # Queries per unit, keys per tile and rows per expanded block of the chunk kernels.
 UNIT_QUERIES, UNIT_KEYS = 128, 64
@@ -84,6 +86,20 @@ class _Shape:
     __slots__ = ("lists", "col_tiles", "num_groups", "num_jobs", "merge_columns", "num_slots", "acc_bytes", "latent_bytes",
                  "num_rows", "row_base", "row_span", "every_row", "num_blocks", "num_units", "num_unit_jobs",
                  "unit_merge_columns", "num_unit_slots")
+
+
+_NO_STEP = ((), (None, 0, None, 0, None, None, 0, 0))
+
+
+def _step_args(spec: LatentLayerSpec, latent: Tensor, rope_key: Tensor, angles) -> tuple:
+    """lvamd_latent_decode's arguments of the step's rows (behind the tensors that they
+    name): the launch appends them."""
+
+    cosines, sines = angles if angles is not None else (None, None)
+    return (latent, rope_key), (
+        latent.data_ptr(), latent.stride(0), rope_key.data_ptr(), rope_key.stride(0),
+        None if cosines is None else cosines.data_ptr(), None if sines is None else sines.data_ptr(),
+        0 if cosines is None else cosines.stride(0), int(spec.rotary_layout == "interleaved"))
 
 
 def choose_col_tiles(q_lens, heads: int) -> int:
@@ -247,22 +263,26 @@ class HipLatentPagedAttention:
             code, stream = dtype_code(cfg.dtype), current_stream(cfg.device)
             shape = plan.shape(spec, code, sizes)
             self._backend.note_latent_form(cache, sizes)
-            turned = append_rows(cache, spec, latent, rope_key, angles, plan.slots_ptr, None, plan.num_tokens,
-                                 None if angles is None else query_rope)
-            query_rope = query_rope if turned is None else turned
             width = spec.latent_size if weights is None else weights.value_size
             out = torch.empty((query.shape[0], heads, width), dtype=cfg.dtype, device=cfg.device)
             rows = cache.layer(layer_id).rows
-            if weights is None:
-                self._attend_latent(spec, shape, query, query_rope, rows, out, 0, scale, code, stream)
+            if shape.num_units or shape.col_tiles > APPEND_TILES:
+                # (The expansion reads the pool: the whole step is appended first.)
+                turned = append_rows(cache, spec, latent, rope_key, angles, plan.slots_ptr, None, plan.num_tokens,
+                                     None if angles is None else query_rope)
+                query_rope = query_rope if turned is None else turned
+                step = _NO_STEP
             else:
-                if shape.num_rows:
-                    self._attend_short(spec, shape, weights, query, query_rope, rows, out, scale, code, stream)
-                if shape.num_units:
-                    self._attend_long(spec, shape, weights, query, query_rope, rows, out, scale, code, stream)
+                step = _step_args(spec, aligned_rows(latent), aligned_rows(rope_key), angles)
+            if weights is None:
+                self._attend_latent(spec, shape, query, query_rope, step, rows, out, 0, scale, code, stream)
+            elif shape.num_rows:
+                self._attend_short(spec, shape, weights, query, query_rope, step, rows, out, scale, code, stream)
+            if shape.num_units:
+                self._attend_long(spec, shape, weights, query, query_rope, rows, out, scale, code, stream)
         return out
 
-    def _attend_latent(self, spec, shape, query, query_rope, rows, out, base: int, scale, code, stream) -> None:
+    def _attend_latent(self, spec, shape, query, query_rope, step, rows, out, base: int, scale, code, stream) -> None:
         """The latent-space kernel and its merge; token t of the step is row t - base
         of ``query`` and ``out``."""
 
@@ -273,13 +293,13 @@ class HipLatentPagedAttention:
         es = query.element_size()
         native.check(native.load().lvamd_latent_decode(
             query.data_ptr() - base * query.stride(0) * es, query.stride(0), query.stride(1), query_rope.data_ptr(),
-            query_rope.stride(0), query_rope.stride(1), rows.data_ptr(), out.data_ptr() - base * out.stride(0) * es,
-            out.stride(0), out.stride(1), lists.pieces, shape.num_groups, lists.jobs, shape.num_jobs,
-            shape.merge_columns, plan.tables_ptr, plan.vis_ptr, acc, None if acc is None else acc + shape.acc_bytes,
-            shape.num_slots, spec.num_query_heads, spec.latent_size, spec.rope_size, shape.col_tiles, plan.block_size,
-            float(scale), code, stream), "lvamd_latent_decode")
+            query_rope.stride(0), query_rope.stride(1), *step[1], rows.data_ptr(),
+            out.data_ptr() - base * out.stride(0) * es, out.stride(0), out.stride(1), lists.pieces, shape.num_groups,
+            lists.jobs, shape.num_jobs, shape.merge_columns, plan.tables_ptr, plan.vis_ptr, acc,
+            None if acc is None else acc + shape.acc_bytes, shape.num_slots, spec.num_query_heads, spec.latent_size,
+            spec.rope_size, shape.col_tiles, plan.block_size, float(scale), code, stream), "lvamd_latent_decode")
 
-    def _attend_short(self, spec, shape, weights, query, query_rope, rows, out, scale, code, stream) -> None:
+    def _attend_short(self, spec, shape, weights, query, query_rope, step, rows, out, scale, code, stream) -> None:
         """The absorbed form: into latent space, attention there, and out of it."""
 
         lib, heads, base = native.load(), spec.num_query_heads, shape.row_base
@@ -291,7 +311,7 @@ class HipLatentPagedAttention:
             query.data_ptr() + base * query.stride(0) * es, query.stride(0), query.stride(1), weights.key_down.data_ptr(),
             absorbed.data_ptr(), absorbed.stride(0), absorbed.stride(1), where, shape.num_rows, heads, weights.nope_size,
             spec.latent_size, code, stream), "lvamd_latent_heads")
-        self._attend_latent(spec, shape, absorbed, query_rope, rows, attended, base, scale, code, stream)
+        self._attend_latent(spec, shape, absorbed, query_rope, step, rows, attended, base, scale, code, stream)
         native.check(lib.lvamd_latent_heads(
             attended.data_ptr(), attended.stride(0), attended.stride(1), weights.value_up.data_ptr(),
             out.data_ptr() + base * out.stride(0) * es, out.stride(0), out.stride(1), where, shape.num_rows, heads,

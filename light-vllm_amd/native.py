@@ -155,8 +155,8 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "lvamd_latent_move_workspace_size": (_i64, [_i64, _i32, _i64]),
     "lvamd_latent_decode": (
         ctypes.c_int,
-        [_p, _i64, _i64, _p, _i64, _i64, _p, _p, _i64, _i64, _p, _i32, _p, _i32, _i32, _p, _p, _p, _p, _i64,
-         _i32, _i32, _i32, _i32, _i32, _f32, _i32, _p],
+        [_p, _i64, _i64, _p, _i64, _i64, _p, _i64, _p, _i64, _p, _p, _i64, _i32, _p, _p, _i64, _i64, _p, _i32, _p, _i32,
+         _i32, _p, _p, _p, _p, _i64, _i32, _i32, _i32, _i32, _i32, _f32, _i32, _p],
     ),
     "lvamd_latent_decode_tile_tokens": (ctypes.c_int, []),
     "lvamd_latent_decode_resident_groups": (ctypes.c_int, [_i32, _i32, _i32, _i32]),

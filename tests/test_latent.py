@@ -78,13 +78,16 @@ def test_the_library_refuses_bad_arguments() -> None:
     assert lib.lvamd_latent_move(p, 2, 1152, p, p, 3, p, 3 * 2 * 1152 - 1, None) == -3
     assert lib.lvamd_latent_move(p, 2, 1152, p, None, 3, None, 0, None) == -1
     decode = lambda **k: lib.lvamd_latent_decode(*{**dict(  # noqa: E731
-        q=p, qt=8, qh=8, qr=p, rt=8, rh=8, pool=p, out=p, ot=8, oh=8, pieces=p, groups=1, jobs=None, njobs=0,
+        q=p, qt=8, qh=8, qr=p, rt=8, rh=8, lat=None, ls=0, rk=None, rs=0, cos=None, sin=None, angle=0, il=1, pool=p, out=p, ot=8, oh=8, pieces=p, groups=1, jobs=None, njobs=0,
         cols=1, tables=p, vis=p, acc=None, ml=None, slots=0, heads=1, size=512, rope=64, tiles=1, block=16, scale=1.0,
         dtype=native.DTYPE_F16, stream=None), **k}.values())
     for bad, status in ((dict(size=576), -2), (dict(dtype=native.DTYPE_F32), -2), (dict(tiles=3), -2), (dict(groups=-1), -1),
                         (dict(heads=0), -1), (dict(block=0), -1), (dict(q=None), -1), (dict(q=p + 8), -1), (dict(rt=4), -1),
                         (dict(out=p + 4), -1), (dict(ot=2), -1), (dict(pool=None), -1), (dict(pieces=None), -1),
-                        (dict(njobs=1), -1), (dict(slots=1), -3), (dict(vis=None), -1)):
+                        (dict(njobs=1), -1), (dict(slots=1), -3), (dict(vis=None), -1), (dict(lat=p), -1),
+                        (dict(lat=p, ls=4, rk=p), -1), (dict(cos=p), -1), (dict(cos=p, sin=p + 8), -1),
+                        (dict(cos=p, sin=p, angle=2), -1),
+                        (dict(lat=p, ls=8, rk=p, rs=8, tiles=8), -2)):
         assert decode(**bad) == status, bad
     assert decode(groups=0) == 0
 
