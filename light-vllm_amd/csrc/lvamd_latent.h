@@ -51,8 +51,7 @@ __device__ __forceinline__ void turn_pair(float x, float y, float c, float s, fl
 }
 // Eight values, four pairs (2i, 2i + 1); c and s are four floats each, 16-byte aligned.
 template <typename T>
-__device__ __forceinline__ uint4 turn_chunk(uint4 x, const float* c, const float* s) {
-  const f32x4 cv = *reinterpret_cast<const f32x4*>(c), sv = *reinterpret_cast<const f32x4*>(s);
+__device__ __forceinline__ uint4 turn_chunk(uint4 x, f32x4 cv, f32x4 sv) {
   T e[8];
   __builtin_memcpy(e, &x, 16);
 #pragma unroll
@@ -65,25 +64,31 @@ __device__ __forceinline__ uint4 turn_chunk(uint4 x, const float* c, const float
   __builtin_memcpy(&x, e, 16);
   return x;
 }
+template <typename T>
+__device__ __forceinline__ uint4 turn_chunk(uint4 x, const float* c, const float* s) {
+  return turn_chunk<T>(x, *reinterpret_cast<const f32x4*>(c), *reinterpret_cast<const f32x4*>(s));
+}
 // Sixteen values, eight pairs (lo i, hi i).
 template <typename T>
-__device__ __forceinline__ void turn_chunks(uint4& lo, uint4& hi, const float* c, const float* s) {
+__device__ __forceinline__ void turn_chunks(uint4& lo, uint4& hi, const f32x4 (&c)[2], const f32x4 (&s)[2]) {
   T x[8], y[8];
   __builtin_memcpy(x, &lo, 16);
   __builtin_memcpy(y, &hi, 16);
 #pragma unroll
-  for (int i = 0; i < 8; i += 4) {
-    const f32x4 cv = *reinterpret_cast<const f32x4*>(c + i), sv = *reinterpret_cast<const f32x4*>(s + i);
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      float a, b;
-      turn_pair(to_f32(x[i + k]), to_f32(y[i + k]), cv[k], sv[k], a, b);
-      x[i + k] = from_f32<T>(a);
-      y[i + k] = from_f32<T>(b);
-    }
+  for (int i = 0; i < 8; ++i) {
+    float a, b;
+    turn_pair(to_f32(x[i]), to_f32(y[i]), c[i / 4][i % 4], s[i / 4][i % 4], a, b);
+    x[i] = from_f32<T>(a);
+    y[i] = from_f32<T>(b);
   }
   __builtin_memcpy(&lo, x, 16);
   __builtin_memcpy(&hi, y, 16);
+}
+template <typename T>
+__device__ __forceinline__ void turn_chunks(uint4& lo, uint4& hi, const float* c, const float* s) {
+  const f32x4 cv[2] = {reinterpret_cast<const f32x4*>(c)[0], reinterpret_cast<const f32x4*>(c)[1]};
+  const f32x4 sv[2] = {reinterpret_cast<const f32x4*>(s)[0], reinterpret_cast<const f32x4*>(s)[1]};
+  turn_chunks<T>(lo, hi, cv, sv);
 }
 
 // Whether rows at p, of these element strides, are made of whole 16-byte chunks.

@@ -181,6 +181,45 @@ __attribute__((amdgpu_waves_per_eu(LatentShape<L, P, NC>::WAVES_PER_EU))) void l
     }
   };
 
+  // Keys of the step's rows that are still to be turned: a lane's chunk of the key
+  // and its angles (with the half layout also the chunk that holds the pairs' other
+  // values), loaded beside the tile.
+  struct Key {
+    uint4 lo, hi;
+    f32x4 c[2], s[2];
+  };
+  constexpr int HALF = P / 16;  // chunks of half a key
+  constexpr int KEY_GROUP = L / 64;
+  auto key_chunk = [&](int ln) -> int {  // -1: not this lane's
+    const int c = (ln & 7) ^ swizzle(8 * rb + (ln >> 3));
+    return (W == 4 || (wave >> 2) == KEY_GROUP % GSTEP) && c < 2 * HALF ? c : -1;
+  };
+  auto key_place = [&](int ln, char* tile) -> uint4* {
+    return reinterpret_cast<uint4*>(tile + (KEY_GROUP * (KT * 128) + rb * 1024 + ln * 16));
+  };
+  auto load_key = [&](int ln, const Row& r, Key& k) {
+    const int c = key_chunk(ln);
+    if (r.tok < 0 || c < 0) return;
+    gptr<const T> const from = (gptr<const T>)(a.rope_new) + (int64_t)r.tok * a.rope_stride;
+    const float* cs = a.cosines + (int64_t)r.tok * a.angle_stride;
+    const float* sn = a.sines + (int64_t)r.tok * a.angle_stride;
+    // (The same loads for both layouts: interleaved pairs need the first of each two.)
+    const int low = c & (HALF - 1), at = a.interleaved ? 4 * c : 8 * low, more = a.interleaved ? 0 : 4;
+    k.c[0] = *reinterpret_cast<const f32x4*>(cs + at);
+    k.s[0] = *reinterpret_cast<const f32x4*>(sn + at);
+    k.c[1] = *reinterpret_cast<const f32x4*>(cs + at + more);
+    k.s[1] = *reinterpret_cast<const f32x4*>(sn + at + more);
+    k.lo = load16(from + 8 * (a.interleaved ? c : low));
+    k.hi = load16(from + 8 * (a.interleaved ? c : low + HALF));
+  };
+  auto turned = [&](int ln, const Key& k) -> uint4 {
+    if (a.interleaved) return turn_chunk<T>(k.lo, k.c[0], k.s[0]);
+    uint4 lo = k.lo, hi = k.hi;
+    turn_chunks<T>(lo, hi, k.c, k.s);
+    const bool low = key_chunk(ln) < HALF;
+    return make_uint4(low ? lo.x : hi.x, low ? lo.y : hi.y, low ? lo.z : hi.z, low ? lo.w : hi.w);
+  };
+
   // ---- columns: queries in registers, what each sees of the step's tokens
   auto columns = [&](int ln, const LatentPiece& x, int ct, int& qi, int& head) -> bool {
     const int col = x.group * COLS + 16 * ct + (ln & 15), ncols = x.q_len * a.heads;
@@ -231,7 +270,6 @@ __attribute__((amdgpu_waves_per_eu(LatentShape<L, P, NC>::WAVES_PER_EU))) void l
         const int c = (32 * k - L) / 8 + g;
         if (mine && a.interleaved) qf[k] = turn_chunk<T>(qf[k], cs + 4 * c, sn + 4 * c);
         if (mine && !a.interleaved) {
-          constexpr int HALF = P / 16;  // chunks of half a vector
           const int at = 8 * (c & (HALF - 1));
           uint4 lo = load16(qr - 8 * g + 8 * (c & (HALF - 1))), hi = load16(qr - 8 * g + 8 * (c | HALF));
           turn_chunks<T>(lo, hi, cs + at, sn + at);
@@ -273,7 +311,10 @@ __attribute__((amdgpu_waves_per_eu(LatentShape<L, P, NC>::WAVES_PER_EU))) void l
       row = lookup(lane, at);
     }
   }
+  Row held = row;  // of the tile that is computed next, while it holds rows of the step
+  Key held_key;
   issue(lane, row, tile0);
+  if (APPEND && a.cosines) load_key(lane, row, held_key);
   load_queries(lane, cur);
   advance(at);
   if (at.tok_end > 0) row = lookup(lane, at);
@@ -304,11 +345,26 @@ __attribute__((amdgpu_waves_per_eu(LatentShape<L, P, NC>::WAVES_PER_EU))) void l
     };
     __builtin_amdgcn_s_waitcnt(wait_vm(0));  // this wave's part of the tile
     lds_barrier();                           // everyone's, and the last tile's reads are done
+    const bool masked = t0 + KT > min(cur.computed, cur.tok_end);
+    // The step's own rows among the tile's: the turned keys go to LDS, and the group
+    // with a token's first column writes its row to the pool (below, behind the
+    // tile's matrix work).
+    const bool has_new = APPEND && masked && a.latent_new;
+    int slot = -1;
+    if (has_new) {
+      if (a.cosines && held.tok >= 0 && key_chunk(ln) >= 0) *key_place(ln, const_cast<char*>(here)) = turned(ln, held_key);
+      const int pos = t0 + 8 * rb + (ln >> 3);
+      const int col = (pos - cur.computed) * a.heads - cur.group * COLS;
+      if (pos >= cur.computed && pos < cur.tok_end && col >= 0 && col < COLS) slot = held.entry * a.block_size + held.off;
+    }
     if (at.tok_end > 0) {
       issue(ln, row, there);
+      if (APPEND) held = row;
+      if (APPEND && a.cosines) load_key(ln, row, held_key);
       advance(at);
       if (at.tok_end > 0) row = lookup(ln, at);
     }
+    if (has_new && a.cosines) lds_barrier();
     if (fresh) {
       m_run = -INFINITY;
       l_run = 0.f;
@@ -319,46 +375,6 @@ __attribute__((amdgpu_waves_per_eu(LatentShape<L, P, NC>::WAVES_PER_EU))) void l
       if (tid < COLS) col_max[tid] = -INFINITY;
       fresh = false;
     }
-    const bool masked = t0 + KT > min(cur.computed, cur.tok_end);
-    // ---- the step's own rows among the tile's: their keys are turned in LDS; the
-    // group with a token's first column writes its row to the pool (below, behind the
-    // tile's matrix work: the table's entry is on its way meanwhile).
-    int slot = -1;
-    if (APPEND && masked && a.latent_new) {
-      const int pos = t0 + 8 * rb + (ln >> 3), j = pos - cur.computed;
-      const int col = j * a.heads - cur.group * COLS, lb = fast_div(pos, a.by_block);
-      const bool mine = j >= 0 && pos < cur.tok_end && col >= 0 && col < COLS;
-      int entry = 0;
-      if (mine) entry = a.tables[cur.table_off + lb];
-      if (a.cosines) {
-        constexpr int HALF = P / 16;
-        const int per = a.interleaved ? 2 * HALF : HALF;  // chunks, or pairs of them, of a key
-        for (int i = tid; i < KT * per; i += 64 * W) {
-          const int r = i / per, c = i - r * per, pos = t0 + r;
-          if (pos < cur.computed || pos >= cur.tok_end) continue;
-          const int64_t tok = cur.q_start + pos - cur.computed;
-          auto chunk = [&](int ch) -> uint4* {  // of the key
-            const int full = L / 8 + ch;
-            return reinterpret_cast<uint4*>(const_cast<char*>(here) +
-                                            ((full >> 3) * (KT * 128) + r * 128 + 16 * ((full & 7) ^ swizzle(r))));
-          };
-          const float* cs = a.cosines + tok * a.angle_stride;
-          const float* sn = a.sines + tok * a.angle_stride;
-          if (a.interleaved) {
-            *chunk(c) = turn_chunk<T>(*chunk(c), cs + 4 * c, sn + 4 * c);
-          } else {
-            uint4 lo = *chunk(c), hi = *chunk(c + HALF);
-            turn_chunks<T>(lo, hi, cs + 8 * c, sn + 8 * c);
-            *chunk(c) = lo;
-            *chunk(c + HALF) = hi;
-          }
-        }
-        lds_barrier();
-      }
-      if (mine) slot = entry * a.block_size + (pos - lb * a.block_size);
-      __builtin_amdgcn_s_waitcnt(wait_vm(0));
-    }
-
     // ---- scores
     f32x4 st[QKS];
     bool vote = false, odd = false;
