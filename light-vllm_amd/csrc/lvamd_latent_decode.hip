@@ -499,6 +499,7 @@ __attribute__((amdgpu_waves_per_eu(LatentShape<L, P, NC>::WAVES_PER_EU))) void l
     }
     const bool poisoned = (said & 2u) != 0;
     if (poisoned) {
+      lds_barrier();  // (the rows on their way to the pool have been read)
       // The step's rows without their values that are not finite (and none of
       // the repeated rows past the piece's end).
       const int lrow = 8 * rb + (ln >> 3);
