@@ -2677,6 +2677,168 @@ PyObject* verify_tensors(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   return PyLong_FromLong(status);
 }
 
+// ---------------------------------------------------------------------------
+// latent_write, latent_attend and rotary_angles: the common case of the latent
+// cache's write, of a latent context's forward and of a rotary embedding in one
+// call each, as attend_tensors: they read the tensors themselves and launch when
+// every rule of the fast path holds, else return kNotFast.
+// ---------------------------------------------------------------------------
+typedef int (*LatentAppendFn)(const void*, int64_t, const void*, int64_t, void*, int64_t, const int64_t*, const int64_t*,
+                              int64_t, const float*, const float*, int64_t, int32_t, const void*, int64_t, int64_t, void*,
+                              int64_t, int32_t, int32_t, int32_t, int32_t, void*);
+typedef int (*LatentDecodeFn)(const void*, int64_t, int64_t, const void*, int64_t, int64_t, const void*, int64_t, const void*,
+                              int64_t, const float*, const float*, int64_t, int32_t, void*, void*, int64_t, int64_t,
+                              const int32_t*, int32_t, const int32_t*, int32_t, int32_t, const int32_t*, const uint32_t*,
+                              float*, float*, int64_t, int32_t, int32_t, int32_t, int32_t, int32_t, float, int32_t, void*);
+typedef int (*LatentHeadsFn)(const void*, int64_t, int64_t, const void*, void*, int64_t, int64_t, const int32_t*, int64_t,
+                             int32_t, int32_t, int32_t, int32_t, void*);
+typedef int (*RotaryAnglesFn)(const void*, int32_t, int64_t, const double*, int32_t, float, void*, void*, int32_t, int32_t,
+                              void*);
+
+// A tuple (dtype object, float32 object, raw-stream getter, device index, n ints).
+struct TensorFacts {
+  PyObject *dtype, *f32, *getter;
+  long device;
+};
+bool facts_of_tuple(PyObject* b, const char* name, int n, TensorFacts* t, int64_t* ints) {
+  if (!PyTuple_Check(b) || PyTuple_GET_SIZE(b) != 4 + n) {
+    PyErr_Format(PyExc_ValueError, "%s: facts must be a %d-tuple", name, 4 + n);
+    return false;
+  }
+  t->dtype = PyTuple_GET_ITEM(b, 0);
+  t->f32 = PyTuple_GET_ITEM(b, 1);
+  t->getter = PyTuple_GET_ITEM(b, 2);
+  t->device = PyLong_AsLong(PyTuple_GET_ITEM(b, 3));
+  for (int i = 0; i < n; ++i) ints[i] = (int64_t)PyLong_AsLongLong(PyTuple_GET_ITEM(b, 4 + i));
+  if (PyErr_Occurred()) return false;
+  if (ints[0] == 0) {
+    PyErr_Format(PyExc_ValueError, "%s: null function", name);
+    return false;
+  }
+  return true;
+}
+
+// The step's rows and angles (cos may be None): 1, 0 or -1 as tensor_facts.
+struct LatentStep {
+  int64_t lat, lat_s, key, key_s, cos = 0, cos_s = 0, sin = 0, sin_s = 0;
+};
+int latent_step(PyObject* latent, PyObject* key, PyObject* cos, PyObject* sin, const TensorFacts& t, int64_t tokens,
+                int64_t size, int64_t rope, LatentStep* o) {
+  int r = row_facts(latent, t.dtype, t.device, tokens, size, &o->lat, &o->lat_s);
+  if (r == 1) r = row_facts(key, t.dtype, t.device, tokens, rope, &o->key, &o->key_s);
+  if (r == 1 && (((o->lat | o->key) & 15) || ((o->lat_s | o->key_s) & 7))) r = 0;
+  if (r != 1 || cos == Py_None) return unless_no_tensor(r);
+  r = row_facts(cos, t.f32, t.device, tokens, rope / 2, &o->cos, &o->cos_s);
+  if (r == 1) r = row_facts(sin, t.f32, t.device, tokens, rope / 2, &o->sin, &o->sin_s);
+  if (r == 1 && (((o->cos | o->sin) & 15) || (o->cos_s & 3) || o->cos_s != o->sin_s)) r = 0;
+  return unless_no_tensor(r);
+}
+
+// latent_write(facts, latent, rope_key, cosines, sines, slots, sources, entries, tokens)
+// ints: fn, pool, slots of the pool, latent size, rope size, dtype code, interleaved
+PyObject* latent_write(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  if (!want_args(nargs, 9, "latent_write")) return nullptr;
+  TensorFacts t;
+  int64_t f[7], v[4];
+  if (!facts_of_tuple(args[0], "latent_write", 7, &t, f)) return nullptr;
+  for (int i = 0; i < 4; ++i) v[i] = (int64_t)PyLong_AsLongLong(args[5 + i]);
+  if (PyErr_Occurred()) return nullptr;
+  LatentStep o;
+  const int r = latent_step(args[1], args[2], args[3], args[4], t, v[3], f[3], f[4], &o);
+  if (r < 0) return nullptr;
+  if (r == 0) return PyLong_FromLong(kNotFast);
+  const int64_t stream = raw_stream(t.getter, t.device);
+  if (PyErr_Occurred()) return nullptr;
+  const LatentAppendFn fn = reinterpret_cast<LatentAppendFn>((intptr_t)f[0]);
+  return PyLong_FromLong(fn(as_ptr(o.lat), o.lat_s, as_ptr(o.key), o.key_s, as_ptr(f[1]), f[2],
+                            (const int64_t*)as_ptr(v[0]), (const int64_t*)as_ptr(v[1]), v[2], (const float*)as_ptr(o.cos),
+                            (const float*)as_ptr(o.sin), o.cos_s, (int32_t)f[6], nullptr, 0, 0, nullptr, v[3], 0,
+                            (int32_t)f[3], (int32_t)f[4], (int32_t)f[5], as_ptr(stream)));
+}
+
+// latent_attend(facts, pool, query, latent, rope_key, cosines, sines, scale, out, workspace, weights)
+// ints: decode fn, heads fn, tokens, heads, latent size, rope size, dtype code, interleaved, pieces, groups, jobs,
+//       jobs' count, merge columns, tables, vis, partial slots, column tiles, block size, bytes of the partial rows,
+//       bytes of the partials, rows' list, rows, first token, tokens spanned
+// weights: None, or (key_down, value_up, nope size, value size); the queries in latent space and the attended
+// latents lie in the workspace behind the partials.
+PyObject* latent_attend(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  if (!want_args(nargs, 11, "latent_attend")) return nullptr;
+  TensorFacts t;
+  int64_t f[24], w[4] = {0, 0, 0, 0};
+  if (!facts_of_tuple(args[0], "latent_attend", 24, &t, f)) return nullptr;
+  const int64_t pool = PyLong_AsLongLong(args[1]), out = PyLong_AsLongLong(args[8]), ws = PyLong_AsLongLong(args[9]);
+  const double scale = PyFloat_AsDouble(args[7]);
+  if (PyErr_Occurred()) return nullptr;
+  const bool weighted = args[10] != Py_None;
+  if (weighted) {
+    if (!PyTuple_Check(args[10]) || PyTuple_GET_SIZE(args[10]) != 4) {
+      PyErr_SetString(PyExc_ValueError, "latent_attend: weights must be a 4-tuple");
+      return nullptr;
+    }
+    for (int i = 0; i < 4; ++i) w[i] = (int64_t)PyLong_AsLongLong(PyTuple_GET_ITEM(args[10], i));
+    if (PyErr_Occurred()) return nullptr;
+  }
+  const int64_t tokens = f[2], heads = f[3], latent = f[4], rope = f[5], size = weighted ? w[2] : latent;
+  int64_t q, qs0, qs1;
+  int r = unless_no_tensor(tensor_facts(args[2], t.dtype, t.device, tokens, heads, size + rope, 2, &q, &qs0, &qs1));
+  LatentStep o;
+  if (r == 1) r = latent_step(args[3], args[4], args[5], args[6], t, tokens, latent, rope, &o);
+  if (r < 0) return nullptr;
+  if (r == 0) return PyLong_FromLong(kNotFast);
+  const int64_t stream = raw_stream(t.getter, t.device);
+  if (PyErr_Occurred()) return nullptr;
+  const LatentDecodeFn decode = reinterpret_cast<LatentDecodeFn>((intptr_t)f[0]);
+  const LatentHeadsFn multiply = reinterpret_cast<LatentHeadsFn>((intptr_t)f[1]);
+  const int32_t code = (int32_t)f[6], h = (int32_t)heads;
+  const int32_t* rows = (const int32_t*)as_ptr(f[20]);
+  const int64_t base = f[22], span = f[23], row = heads * latent;  // (elements of two bytes)
+  const int64_t absorbed = ws + f[19], attended = absorbed + 2 * span * row;
+  if (weighted) {
+    const int status = multiply(as_ptr(q + 2 * base * qs0), qs0, qs1, as_ptr(w[0]), as_ptr(absorbed), row, latent, rows, f[21],
+                                h, (int32_t)size, (int32_t)latent, code, as_ptr(stream));
+    if (status != 0) return PyLong_FromLong(status);
+  }
+  const int64_t from = weighted ? absorbed - 2 * base * row : q, to = weighted ? attended - 2 * base * row : out;
+  int status = decode(as_ptr(from), weighted ? row : qs0, weighted ? latent : qs1, as_ptr(q + 2 * size), qs0, qs1,
+                      as_ptr(o.lat), o.lat_s, as_ptr(o.key), o.key_s, (const float*)as_ptr(o.cos),
+                      (const float*)as_ptr(o.sin), o.cos_s, (int32_t)f[7], as_ptr(pool), as_ptr(to), row, latent,
+                      (const int32_t*)as_ptr(f[8]), (int32_t)f[9], (const int32_t*)as_ptr(f[10]), (int32_t)f[11],
+                      (int32_t)f[12], (const int32_t*)as_ptr(f[13]), (const uint32_t*)as_ptr(f[14]),
+                      f[15] ? (float*)as_ptr(ws) : nullptr, f[15] ? (float*)as_ptr(ws + f[18]) : nullptr, f[15], h,
+                      (int32_t)latent, (int32_t)rope, (int32_t)f[16], (int32_t)f[17], (float)scale, code, as_ptr(stream));
+  if (status == 0 && weighted)
+    status = multiply(as_ptr(attended), row, latent, as_ptr(w[1]), as_ptr(out + 2 * base * heads * w[3]), heads * w[3], w[3],
+                      rows, f[21], h, (int32_t)latent, (int32_t)w[3], code, as_ptr(stream));
+  return PyLong_FromLong(status);
+}
+
+// rotary_angles(facts, positions, count, cosines, sines, repeat, dtype code, magnitude)
+// ints: fn, turns, half; the dtype objects are those of 64- and 32-bit positions
+PyObject* rotary_angles(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  if (!want_args(nargs, 8, "rotary_angles")) return nullptr;
+  TensorFacts t;
+  int64_t f[3], v[5];
+  if (!facts_of_tuple(args[0], "rotary_angles", 3, &t, f)) return nullptr;
+  for (int i = 0; i < 5; ++i) v[i] = (int64_t)PyLong_AsLongLong(args[2 + i]);
+  const double magnitude = PyFloat_AsDouble(args[7]);
+  if (PyErr_Occurred()) return nullptr;
+  int64_t at = 0;
+  int bytes = 8;
+  int r = unless_no_tensor(vector_facts(args[1], t.dtype, t.device, v[0], &at));
+  if (r == 0) {
+    bytes = 4;
+    r = unless_no_tensor(vector_facts(args[1], t.f32, t.device, v[0], &at));
+  }
+  if (r < 0) return nullptr;
+  if (r == 0) return PyLong_FromLong(kNotFast);
+  const int64_t stream = raw_stream(t.getter, t.device);
+  if (PyErr_Occurred()) return nullptr;
+  const RotaryAnglesFn fn = reinterpret_cast<RotaryAnglesFn>((intptr_t)f[0]);
+  return PyLong_FromLong(fn(as_ptr(at), bytes, v[0], (const double*)as_ptr(f[1]), (int32_t)f[2], (float)magnitude,
+                            as_ptr(v[1]), as_ptr(v[2]), (int32_t)v[3], (int32_t)v[4], as_ptr(stream)));
+}
+
 PyMethodDef kMethods[] = {
     {"flatten", (PyCFunction)(void (*)(void))flatten, METH_FASTCALL, "int sequences -> (flat, counts int64, status)"},
     {"validate", (PyCFunction)(void (*)(void))validate, METH_FASTCALL, "block-table rules -> (rule, request)"},
@@ -2697,6 +2859,12 @@ PyMethodDef kMethods[] = {
      "forward's fast path with rotary: the rotary append, then lvamd_paged_attention"},
     {"append_tensors", (PyCFunction)(void (*)(void))append_tensors, METH_FASTCALL,
      "the 8-bit cache's write: tensor rules and the lvamd_kv_append_q8 call"},
+    {"latent_write", (PyCFunction)(void (*)(void))latent_write, METH_FASTCALL,
+     "the latent cache's write: tensor rules and the lvamd_latent_append call"},
+    {"latent_attend", (PyCFunction)(void (*)(void))latent_attend, METH_FASTCALL,
+     "a latent forward: tensor rules, lvamd_latent_decode and the products around it"},
+    {"rotary_angles", (PyCFunction)(void (*)(void))rotary_angles, METH_FASTCALL,
+     "a rotary embedding's rules and the lvamd_rotary_angles call"},
     {"block_runs", (PyCFunction)(void (*)(void))block_runs, METH_FASTCALL, "destination-block runs of a compact's pairs"},
     {"compact_chunks", (PyCFunction)(void (*)(void))compact_chunks, METH_FASTCALL, "compact pairs in independent chunks"},
     {"verify_tensors", (PyCFunction)(void (*)(void))verify_tensors, METH_FASTCALL,

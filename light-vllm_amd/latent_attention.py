@@ -25,7 +25,7 @@ from light_vllm_amd import errors, native
 from light_vllm_amd.latent_cache import LatentLayerSpec, aligned_rows, append_rows, check_rotary, check_rows
 from light_vllm_amd.paged_cache import dtype_code
 from light_vllm_amd.plan import DECODE_MERGE_PIECES, PREFILL_MIN_TILES, StepPlan, current_stream
-from light_vllm_amd.quantized_cache import on_device
+from light_vllm_amd.quantized_cache import _NOT_FAST, _raw_stream, on_device
 
 # Column tiles (of 16) per workgroup that the latent-space kernel is built for.
 COL_TILES = (1, 2, 4, 8)
@@ -43,7 +43,8 @@ class LatentWeights:
     nope_size, latent_size]`` and ``value_up`` ``[heads, value_size, latent_size]``
     (rows as a linear layer's, per head)."""
 
-    __slots__ = ("key_up", "value_up", "key_down", "heads", "latent_size", "nope_size", "value_size")
+    __slots__ = ("key_up", "value_up", "key_down", "heads", "latent_size", "nope_size", "value_size", "sizes", "fits",
+                 "addresses")
 
     def __init__(self, key_up: Tensor, value_up: Tensor) -> None:
         for holds, message in (
@@ -65,6 +66,10 @@ class LatentWeights:
         self.key_down = self.key_up.transpose(1, 2).contiguous()  # into latent space
         self.heads, self.nope_size, self.latent_size = key_up.shape
         self.value_size = value_up.shape[1]
+        self.sizes = (self.nope_size, self.value_size)
+        # What a layer compares, and what a launch takes.
+        self.fits = (self.heads, self.latent_size, self.key_up.dtype, self.key_up.device)
+        self.addresses = (self.key_down.data_ptr(), self.value_up.data_ptr(), self.nope_size, self.value_size)
 
 
 class _Lists:
@@ -83,8 +88,8 @@ class _Lists:
 class _Shape:
     """One layer shape's launch facts in a step plan."""
 
-    __slots__ = ("lists", "col_tiles", "num_groups", "num_jobs", "merge_columns", "num_slots", "acc_bytes", "latent_bytes",
-                 "num_rows", "row_base", "row_span", "every_row", "num_blocks", "num_units", "num_unit_jobs",
+    __slots__ = ("facts", "out_shape", "scratch_bytes", "lists", "col_tiles", "num_groups", "num_jobs", "merge_columns",
+                 "num_slots", "acc_bytes", "latent_bytes", "num_rows", "row_base", "row_span", "every_row", "num_blocks", "num_units", "num_unit_jobs",
                  "unit_merge_columns", "num_unit_slots")
 
 
@@ -141,6 +146,21 @@ class LatentStepPlan(StepPlan):
             self._register(key, found.lists)
         return found
 
+    def bind(self, x: _Shape, spec: LatentLayerSpec, config, code: int, weights: tuple[int, int] | None) -> None:
+        """What one native call takes of a step that needs no launch beside the
+        latent-space kernel's (the lists are uploaded by now)."""
+
+        index = config.device.index if config.device.index is not None else torch.cuda.current_device()
+        heads, lists = spec.num_query_heads, x.lists
+        x.facts = (
+            config.dtype, torch.float32, _raw_stream, index, native.entry("lvamd_latent_decode"),
+            native.entry("lvamd_latent_heads"), self.num_tokens, heads, spec.latent_size, spec.rope_size, code,
+            int(spec.rotary_layout == "interleaved"), lists.pieces, x.num_groups, lists.jobs or 0, x.num_jobs,
+            x.merge_columns, self.tables_ptr, self.vis_ptr, x.num_slots, x.col_tiles, self.block_size, x.acc_bytes,
+            x.latent_bytes, lists.rows or 0, x.num_rows, x.row_base, x.row_span)
+        x.scratch_bytes = x.latent_bytes + (0 if weights is None else 4 * x.row_span * heads * spec.latent_size)
+        x.out_shape = (self.num_tokens, heads, spec.latent_size if weights is None else weights[1])
+
     def _plan_shape(self, spec: LatentLayerSpec, code: int, weights: tuple[int, int] | None) -> _Shape:
         facts, heads, host = self.facts, spec.num_query_heads, native.host()
         none = np.zeros(0, np.int32)
@@ -148,6 +168,7 @@ class LatentStepPlan(StepPlan):
         long = np.zeros(self.batch_size, bool) if weights is None else _expanded(facts, spec, *weights)
         short = ~long
         x = _Shape()
+        x.facts = None
         pieces = jobs = rows = blocks = units = unit_jobs = none
         x.num_groups = x.num_jobs = x.num_slots = x.merge_columns = x.num_rows = 0
         x.row_base, x.row_span, x.every_row, x.col_tiles = 0, 0, True, COL_TILES[0]
@@ -203,6 +224,7 @@ class HipLatentPagedAttention:
         self._cache = cache
         self._plan = plan
         self._layer_ids: set[str] = set()
+        self._attend = native.host().latent_attend
 
     @property
     def layer_ids(self) -> frozenset[str]:
@@ -235,6 +257,38 @@ class HipLatentPagedAttention:
             raise errors.KVCacheError(f"paged attention layer {layer_id!r} ran more than once")
         self._layer_ids.add(layer_id)
         spec = cache.layer_spec(layer_id)
+        # The common case in one native call: it reads the tensors itself and
+        # launches when every rule holds; anything else takes the general path, which
+        # raises the first broken rule's message.
+        sizes = None if weights is None else weights.sizes
+        code = dtype_code(cfg.dtype)
+        shape = plan.launches.get((spec.num_query_heads, spec.latent_size, spec.rope_size, code, sizes))
+        if (shape is not None and shape.num_units == 0 and shape.col_tiles <= APPEND_TILES
+                and (weights is None or weights.fits == (spec.num_query_heads, spec.latent_size, cfg.dtype, cfg.device))
+                and (rotary is None or (type(rotary) is tuple and len(rotary) == 2))):
+            facts = shape.facts
+            if facts is None or facts[11] != (spec.rotary_layout == "interleaved"):
+                plan.bind(shape, spec, cfg, code, sizes)
+                facts = shape.facts
+            if torch.cuda.current_device() == facts[3]:
+                out = torch.empty(shape.out_shape, dtype=cfg.dtype, device=cfg.device)
+                # (Of the call's own stream or graph: no two share one.)
+                scratch = torch.empty(shape.scratch_bytes, dtype=torch.uint8, device=cfg.device) if shape.scratch_bytes else None
+                cosines, sines = rotary if rotary is not None else (None, None)
+                status = self._attend(facts, cache.pool_ptr(layer_id), query, latent, rope_key, cosines, sines, scale,
+                                      out.data_ptr(), 0 if scratch is None else scratch.data_ptr(),
+                                      None if weights is None else weights.addresses)
+                if status == 0:
+                    return out
+                if status != _NOT_FAST:
+                    native.check(status, "lvamd_latent_decode")
+        return self._forward_general(spec, query, latent, rope_key, scale, rotary, weights)
+
+    def _forward_general(self, spec, query, latent, rope_key, scale, rotary, weights) -> Tensor:
+        """Every rule, then the launches for any row strides and forms."""
+
+        cache, plan = self._cache, self._plan
+        cfg, layer_id = cache.config, spec.layer_id
         heads, rope = spec.num_query_heads, spec.rope_size
         size = spec.latent_size if weights is None else weights.nope_size
         for holds, message in (

@@ -11,6 +11,7 @@ src/light_vllm/modeling/attention/interfaces.py:9-36).
 
 from __future__ import annotations
 
+import functools
 import weakref
 from dataclasses import dataclass
 
@@ -24,7 +25,7 @@ from light_vllm_amd.paged_cache import (
     PagedKVCacheConfig, PagedKVWriteMapping, _block_copy_pairs, _compact_bytes, _compact_request, dtype_code,
 )
 from light_vllm_amd.plan import Staging, current_stream
-from light_vllm_amd.quantized_cache import on_device
+from light_vllm_amd.quantized_cache import _NOT_FAST, _raw_stream, on_device
 
 LATENT_SIZES = (128, 256, 384, 512)
 ROPE_SIZES = (32, 64)
@@ -94,6 +95,11 @@ class LatentPagedLayerCache:
     rope_keys: Tensor
 
 
+@functools.lru_cache(maxsize=1)
+def _latent_write():
+    return native.host().latent_write
+
+
 class _State:
     """Per-cache launch state: device tables of the layers' pool addresses by row
     size, and a staging ring."""
@@ -132,6 +138,10 @@ class LatentPagedKVCache:
         self._config = config
         self._layer_specs = {layer.layer_id: layer for layer in model_spec.layers}
         self._layers = {layer.layer_id: self._allocate_layer(layer) for layer in model_spec.layers}
+        self._pool_ptrs = {layer_id: layer.rows.data_ptr() for layer_id, layer in self._layers.items()}
+        # What latent_write takes of a layer, made at its first write.
+        self._write_facts: dict[str, tuple] = {}
+        self._slots = config.num_blocks * config.block_size
 
     @property
     def config(self) -> PagedKVCacheConfig:
@@ -152,6 +162,11 @@ class LatentPagedKVCache:
             return self._layers[layer_id]
         except KeyError as exc:
             raise errors.KVCacheError(f"KV cache layer {layer_id!r} was not found") from exc
+
+    def pool_ptr(self, layer_id: str) -> int:
+        """Address of a layer's rows."""
+
+        return self._pool_ptrs[layer_id]
 
     @torch.inference_mode()
     def prepare_write(self, slot_mapping: Tensor, *, validate: bool = True) -> PagedKVWriteMapping:
@@ -182,15 +197,32 @@ class LatentPagedKVCache:
             source_indices=None if every else torch.from_numpy(written).to(device),
         )
 
-    @torch.inference_mode()
     def write_prepared(self, layer_id: str, latent: Tensor, rope_key: Tensor, mapping: PagedKVWriteMapping, *,
                        rotary: tuple[Tensor, Tensor] | None = None) -> None:
         """Write one layer's rows through a prepared mapping: ``latent``
         ``[tokens, latent_size]`` and ``rope_key`` ``[tokens, rope_size]``, turned by
         ``rotary=(cosines, sines)`` (fp32 ``[tokens, rope_size / 2]``) or as it is."""
 
-        spec = self.layer_spec(layer_id)
+        # The common case in one native call: it reads the tensors itself and launches
+        # when every rule holds; anything else takes the rules below.
         cfg = self._config
+        facts = self._write_facts.get(layer_id) or self._bind_write(layer_id)
+        if (type(mapping) is PagedKVWriteMapping and torch.cuda.current_device() == facts[3]
+                and (rotary is None or (type(rotary) is tuple and len(rotary) == 2))):
+            slots, sources = mapping.slots, mapping.source_indices
+            n = slots.numel()
+            if (slots.dtype == torch.long and slots.ndim == 1 and slots.device == cfg.device and slots.is_contiguous()
+                    and (sources is None and n == mapping.num_query_tokens or sources is not None
+                         and sources.dtype == torch.long and sources.device == cfg.device and sources.shape == slots.shape
+                         and sources.is_contiguous())):
+                cosines, sines = rotary if rotary is not None else (None, None)
+                status = _latent_write()(facts, latent, rope_key, cosines, sines, slots.data_ptr(),
+                                         0 if sources is None else sources.data_ptr(), n, mapping.num_query_tokens)
+                if status == 0:
+                    return
+                if status != _NOT_FAST:
+                    native.check(status, "lvamd_latent_append")
+        spec = self.layer_spec(layer_id)
         check_rows(cfg, spec, latent, rope_key)
         slots, sources = mapping.slots, mapping.source_indices
         count = mapping.num_query_tokens if sources is None else sources.numel()
@@ -208,7 +240,15 @@ class LatentPagedKVCache:
         append_rows(self, spec, latent, rope_key, angles, slots.data_ptr(), None if sources is None else sources.data_ptr(),
                     slots.numel())
 
-    @torch.inference_mode()
+    def _bind_write(self, layer_id: str) -> tuple:
+        spec, cfg = self.layer_spec(layer_id), self._config
+        index = cfg.device.index if cfg.device.index is not None else torch.cuda.current_device()
+        found = self._write_facts[layer_id] = (
+            cfg.dtype, torch.float32, _raw_stream, index, native.entry("lvamd_latent_append"),
+            self.layer(layer_id).rows.data_ptr(), self._slots, spec.latent_size, spec.rope_size, dtype_code(cfg.dtype),
+            int(spec.rotary_layout == "interleaved"))
+        return found
+
     def write(self, layer_id: str, latent: Tensor, rope_key: Tensor, slot_mapping: Tensor, *,
               rotary: tuple[Tensor, Tensor] | None = None) -> None:
         """Write the active tokens' rows to their physical slots."""

@@ -432,6 +432,13 @@ def append_q8_entry() -> int:
     return ctypes.cast(load().lvamd_kv_append_q8, ctypes.c_void_p).value
 
 
+@functools.lru_cache(maxsize=None)
+def entry(name: str) -> int:
+    """Address of a library function, for the host module's calls."""
+
+    return ctypes.cast(getattr(load(), name), ctypes.c_void_p).value
+
+
 def verify_entry() -> int:
     """Address of ``lvamd_verify_drafts``, for the host module's ``verify_tensors``."""
 

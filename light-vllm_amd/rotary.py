@@ -19,7 +19,7 @@ from torch import Tensor
 from light_vllm_amd import errors, native
 from light_vllm_amd.paged_cache import dtype_code
 from light_vllm_amd.plan import current_stream
-from light_vllm_amd.quantized_cache import on_device
+from light_vllm_amd.quantized_cache import _NOT_FAST, _raw_stream, on_device
 
 _KINDS = ("linear", "base", "ramp", "smooth")
 
@@ -127,14 +127,30 @@ class RotaryEmbedding:
             self.device = torch.device("cuda", torch.cuda.current_device())
         self._turns = (freq / (2 * math.pi)).to(self.device)
         self._lib = native.load()
+        self._facts = (torch.int64, torch.int32, _raw_stream, self.device.index, native.entry("lvamd_rotary_angles"),
+                       self._turns.data_ptr(), size // 2)
+        self._angles = native.host().rotary_angles
 
     def __call__(self, positions: Tensor, *, full: bool = False, dtype: torch.dtype = torch.float32) -> tuple[Tensor, Tensor]:
+        # The common case in one native call: it reads the positions and launches
+        # when every rule holds; anything else takes the rules below.
+        n, half = positions.shape[0] if isinstance(positions, Tensor) and positions.ndim == 1 else 0, self.size // 2
+        if 0 < n <= (2**31 - 1) // half and torch.cuda.current_device() == self.device.index:
+            code = dtype_code(dtype)
+            both = torch.empty((2, n, self.size if full else half), dtype=dtype, device=self.device)
+            cosines, sines = both.unbind(0)
+            status = self._angles(self._facts, positions, n, cosines.data_ptr(), sines.data_ptr(), 2 if full else 1, code,
+                                  self.magnitude)
+            if status == 0:
+                return cosines, sines
+            if status != _NOT_FAST:
+                native.check(status, "lvamd_rotary_angles")
         if not isinstance(positions, Tensor) or positions.ndim != 1 or positions.dtype not in (torch.int32, torch.int64):
             raise ValueError("rotary positions must be an int32 or int64 vector")
         if positions.device != self.device:
             raise ValueError("rotary positions must be on the embedding's device")
         code = dtype_code(dtype)
-        n, half = positions.shape[0], self.size // 2
+        n = positions.shape[0]
         if n > (2**31 - 1) // half:
             raise ValueError("too many rotary positions for one call")
         positions = positions.contiguous()
