@@ -324,6 +324,19 @@ __attribute__((amdgpu_waves_per_eu(LatentShape<L, P, NC>::WAVES_PER_EU))) void l
   int t0 = cur.tok_begin;
   bool fresh = true;  // the tile is its piece's first
 
+  auto key_base = [&](int ln) -> int {
+    return (16 * ks0 + (ln & 15)) * 128 + 16 * ((ln >> 4) ^ swizzle(ln & 15));  // (^ 64: chunk 4 + g)
+  };
+  auto value_address = [&](int ln, int n) -> int {
+    const int vrow = 4 * (ln >> 4) + ((ln & 15) >> 2), q4 = ln & 3, c = 2 * (wave * DT + n) + (q4 >> 1);
+    return (c >> 3) * (KT * 128) + vrow * 128 + 16 * ((c & 7) ^ swizzle(vrow)) + 8 * (q4 & 1);
+  };
+  constexpr bool EARLY_V = NC < 8;
+  const int kept_kbase = key_base(lane);
+  int kept_vaddr[DT];
+#pragma unroll
+  for (int n = 0; n < DT; ++n) kept_vaddr[n] = value_address(lane, n);
+
   // One tile from `here` while the next lands in `there`; false: it was the last.
   auto step = [&](const char* here, char* there) __attribute__((always_inline)) -> bool {
     // (Everything that depends on the lane is formed anew in each step, a few
@@ -337,12 +350,8 @@ __attribute__((amdgpu_waves_per_eu(LatentShape<L, P, NC>::WAVES_PER_EU))) void l
     // offset from its tile: the compiler tells a read of one tile from a load into
     // the other only where few steps of arithmetic lie between the array and the
     // access; otherwise it waits for the load before every read.)
-    const int kbase = (16 * ks0 + l16) * 128 + 16 * (g ^ swizzle(l16));  // (^ 64: chunk 4 + g)
-    const int vrow = 4 * g + (l16 >> 2), q4 = l16 & 3;
-    auto vaddr = [&](int n) -> int {
-      const int c = 2 * (wave * DT + n) + (q4 >> 1);
-      return (c >> 3) * (KT * 128) + vrow * 128 + 16 * ((c & 7) ^ swizzle(vrow)) + 8 * (q4 & 1);
-    };
+    const int kbase = EARLY_V ? kept_kbase : key_base(ln);
+    auto vaddr = [&](int n) -> int { return EARLY_V ? kept_vaddr[n] : value_address(ln, n); };
     __builtin_amdgcn_s_waitcnt(wait_vm(0));  // this wave's part of the tile
     lds_barrier();                           // everyone's, and the last tile's reads are done
     const bool masked = t0 + KT > min(cur.computed, cur.tok_end);
@@ -376,12 +385,20 @@ __attribute__((amdgpu_waves_per_eu(LatentShape<L, P, NC>::WAVES_PER_EU))) void l
       fresh = false;
     }
     // ---- scores
+    auto rdv = [&](int n) -> V8 {
+      const int at8 = vaddr(n);
+      const s16x4 v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_t*)(here + at8));
+      const s16x4 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_t*)(here + (at8 + 16 * 128)));
+      const s16x4 both[2] = {v0, v1};
+      return bitcast<V8>(both);
+    };
+    V8 vals[EARLY_V ? DT : 1];
     f32x4 st[QKS];
     bool vote = false, odd = false;
     if (scores) {
       // LDS reads run LEAD ahead of the matrix instructions; two sums per score, so
       // that an instruction does not wait for the one before it.
-      constexpr int TOT = QKS * KSTEPS, LEAD = NC == 8 ? 3 : 4, CH = QKS == 1 ? 2 : 1;
+      constexpr int TOT = QKS * KSTEPS, LEAD = NC == 8 ? 3 : 6, CH = QKS == 1 ? 2 : 1;
       auto rd = [&](int i) -> uint4 {
         return *reinterpret_cast<const uint4*>(here + (((i / QKS) >> 1) * (KT * 128) + (i % QKS) * 16 * 128 + (kbase ^ ((i / QKS) & 1 ? 64 : 0))));
       };
@@ -395,6 +412,10 @@ __attribute__((amdgpu_waves_per_eu(LatentShape<L, P, NC>::WAVES_PER_EU))) void l
         sum[to] = Mma<T>::qk(key[i % LEAD], qf[k], i < 2 ? f32x4{0.f, 0.f, 0.f, 0.f} : sum[to]);
         if (i + LEAD < TOT) key[i % LEAD] = rd(i + LEAD);
         if constexpr (NC == 8) __builtin_amdgcn_sched_barrier(0);  // (hoisted reads would spill)
+      }
+      if constexpr (EARLY_V) {
+#pragma unroll
+        for (int n = 0; n < DT; ++n) vals[n] = rdv(n);
       }
       if constexpr (CH == 2) {
         st[0] = sum[0] + sum[1];
@@ -429,6 +450,10 @@ __attribute__((amdgpu_waves_per_eu(LatentShape<L, P, NC>::WAVES_PER_EU))) void l
       mt = row_max4(mt);
       vote = mt > m_run + kSlack;
       if (g == 0) tile_max[ks0][16 * ct0 + l16] = mt;
+    }
+    if (EARLY_V && !scores) {
+#pragma unroll
+      for (int n = 0; n < DT; ++n) vals[EARLY_V ? n : 0] = rdv(n);
     }
     // The weights are rounded to T for the products (a matrix instruction's
     // operands are of one type); the sum that divides them counts them as rounded.
@@ -520,18 +545,15 @@ __attribute__((amdgpu_waves_per_eu(LatentShape<L, P, NC>::WAVES_PER_EU))) void l
         }
       }
       lds_barrier();
+      if constexpr (EARLY_V) {
+#pragma unroll
+        for (int n = 0; n < DT; ++n) vals[n] = rdv(n);
+      }
     }
 
     // ---- O^T += V^T P^T.  The fewer of the two operands' registers are held (all
     // of a wave's values, or all columns' weights), the other is read LEAD ahead.
     {
-      auto rdv = [&](int n) -> V8 {
-        const int at8 = vaddr(n);
-        const s16x4 v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_t*)(here + at8));
-        const s16x4 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_t*)(here + (at8 + 16 * 128)));
-        const s16x4 both[2] = {v0, v1};
-        return bitcast<V8>(both);
-      };
       auto rdp = [&](int c) -> V8 { return bitcast<V8>(*reinterpret_cast<const uint4*>(probs + (c * 64 + ln) * 2)); };
       auto mm = [&](V8 v, V8 w, f32x4 x) -> f32x4 {
         if constexpr (std::is_same<T, __bf16>::value) {
@@ -540,6 +562,15 @@ __attribute__((amdgpu_waves_per_eu(LatentShape<L, P, NC>::WAVES_PER_EU))) void l
           return __builtin_amdgcn_mfma_f32_16x16x32_f16(v, w, x, 0, 0, 0);
         }
       };
+      if constexpr (EARLY_V) {
+        V8 w[NC];
+#pragma unroll
+        for (int c = 0; c < NC; ++c) w[c] = rdp(c);
+#pragma unroll
+        for (int c = 0; c < NC; ++c)
+#pragma unroll
+          for (int n = 0; n < DT; ++n) acc[c][n] = mm(vals[n], w[c], acc[c][n]);
+      } else {
       constexpr bool HOLD_V = NC > DT;
       constexpr int HELD = HOLD_V ? DT : NC, TOT = HOLD_V ? NC : DT, LEAD = TOT < 2 ? TOT : 2;
       V8 held[HELD], ahead[LEAD];
@@ -558,6 +589,7 @@ __attribute__((amdgpu_waves_per_eu(LatentShape<L, P, NC>::WAVES_PER_EU))) void l
           to = HOLD_V ? mm(held[k], x, to) : mm(x, held[k], to);
         }
         if constexpr (NC == 8) __builtin_amdgcn_sched_barrier(0);
+      }
       }
     }
     if (poisoned) {
@@ -636,38 +668,76 @@ __attribute__((amdgpu_waves_per_eu(LatentShape<L, P, NC>::WAVES_PER_EU))) void l
 }
 
 // ---------------------------------------------------------------------------
-// Merge: a workgroup per (job, column), a thread per four dimensions.  With
-// partial i's maximum m_i (log2) and sum l_i, out = sum 2^(m_i - M) l_i o_i /
-// sum 2^(m_i - M) l_i.
+// Merge: a workgroup per (job, column), a thread per four dimensions and other
+// piece; the two shares of the pieces join in LDS, in order.  With partial i's
+// maximum m_i (log2) and sum l_i, out = sum 2^(m_i - M) l_i o_i / sum 2^(m_i - M) l_i,
+// taken in one pass: a share's sums are scaled when its maximum moves.
 // ---------------------------------------------------------------------------
+constexpr int MERGE_SHARES = 2;
 template <typename T, int L>
-__global__ __launch_bounds__(L / 4) void latent_merge_kernel(const int32_t* __restrict__ jobs, const int32_t cols,
-                                                             const LatentDecodeArgs a) {
+__global__ __launch_bounds__(L / 4 * MERGE_SHARES) void latent_merge_kernel(const int32_t* __restrict__ jobs, const int32_t cols,
+                                                                            const LatentDecodeArgs a) {
+  constexpr int LANES = L / 4, S = MERGE_SHARES, AT_ONCE = 4;
+  __shared__ f32x4 sums[S - 1][LANES];
+  __shared__ float maxima[S], totals[S];
   const int32_t* jb = jobs + (int64_t)blockIdx.x * LVAMD_MERGE_FIELDS;
   const int group = jb[1], slot0 = jb[2], np = jb[3], q_start = jb[4], q_len = jb[5];
   const int i = blockIdx.y;
   const int col = group * cols + i;
   if (col >= q_len * a.heads) return;
-  const float* ml = a.part_ml + ((int64_t)slot0 * cols + i) * 2;
-  const int64_t ml_step = 2 * cols;
-  float m = -INFINITY;
-#pragma unroll 8
-  for (int k = 0; k < np; ++k) m = fmaxf(m, ml[k * ml_step]);
-  const float* from = a.part_acc + ((int64_t)slot0 * cols + i) * L + 4 * threadIdx.x;
+  const int at = threadIdx.x % LANES, share = threadIdx.x / LANES;
+  const float2* ml = reinterpret_cast<const float2*>(a.part_ml) + (int64_t)slot0 * cols + i;
+  const float* from = a.part_acc + ((int64_t)slot0 * cols + i) * L + 4 * at;
   f32x4 sum = {0.f, 0.f, 0.f, 0.f};
-  float total = 0.f;
-#pragma unroll 4
-  for (int k = 0; k < np; ++k) {
-    const f32x4 o = *reinterpret_cast<const f32x4*>(from + (int64_t)k * cols * L);
-    const float mk = ml[k * ml_step];
-    const float w = mk == -INFINITY ? 0.f : fast_exp2(mk - m) * ml[k * ml_step + 1];
-    total += w;
-    sum += o * w;
+  float m = -INFINITY, total = 0.f;
+  for (int k0 = share; k0 < np; k0 += S * AT_ONCE) {
+    f32x4 o[AT_ONCE];
+    float2 of[AT_ONCE];
+    float top = m;
+#pragma unroll
+    for (int j = 0; j < AT_ONCE; ++j) {
+      const int k = min(k0 + S * j, np - 1);
+      of[j] = ml[(int64_t)k * cols];
+      o[j] = *reinterpret_cast<const f32x4*>(from + (int64_t)k * cols * L);
+    }
+#pragma unroll
+    for (int j = 0; j < AT_ONCE; ++j)
+      if (k0 + S * j < np) top = fmaxf(top, of[j].x);
+    const float had = m == -INFINITY ? 0.f : fast_exp2(m - top);
+    sum *= had;
+    total *= had;
+    m = top;
+#pragma unroll
+    for (int j = 0; j < AT_ONCE; ++j) {
+      if (k0 + S * j >= np) break;
+      const float w = of[j].x == -INFINITY ? 0.f : fast_exp2(of[j].x - m) * of[j].y;
+      total += w;
+      sum += o[j] * w;
+    }
+  }
+  if (share) sums[share - 1][at] = sum;
+  if (at == 0) {
+    maxima[share] = m;
+    totals[share] = total;
+  }
+  __syncthreads();
+  if (share) return;
+  float top = m;
+#pragma unroll
+  for (int s = 1; s < S; ++s) top = fmaxf(top, maxima[s]);
+  const float had = m == -INFINITY ? 0.f : fast_exp2(m - top);
+  sum *= had;
+  total *= had;
+#pragma unroll
+  for (int s = 1; s < S; ++s) {
+    const float w = maxima[s] == -INFINITY ? 0.f : fast_exp2(maxima[s] - top);
+    total += totals[s] * w;
+    sum += sums[s - 1][at] * w;
   }
   const int qi = fast_div(col, a.by_heads), head = col - qi * a.heads;
   T* to = static_cast<T*>(a.out) + (int64_t)(q_start + qi) * a.out_tok_stride + (int64_t)head * a.out_head_stride;
   const float inv = total > 0.f ? 1.f / total : total == total ? 0.f : total;
-  store_partial4<false, T>(to + 4 * threadIdx.x, sum, inv);
+  store_partial4<false, T>(to + 4 * at, sum, inv);
 }
 
 template <typename T, int L, int P>
@@ -767,7 +837,7 @@ extern "C" int lvamd_latent_decode(const void* query, int64_t query_token_stride
     }
     if (const int status = launch_status(); status != LVAMD_OK) return status;
     if (num_jobs == 0) return LVAMD_OK;
-    hipLaunchKernelGGL((latent_merge_kernel<T, L>), dim3((unsigned)num_jobs, (unsigned)merge_columns), dim3(L / 4), 0, s,
+    hipLaunchKernelGGL((latent_merge_kernel<T, L>), dim3((unsigned)num_jobs, (unsigned)merge_columns), dim3(L / 4 * MERGE_SHARES), 0, s,
                        jobs, 16 * col_tiles, a);
     return launch_status();
   });
