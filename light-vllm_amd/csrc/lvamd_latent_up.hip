@@ -15,10 +15,6 @@ namespace {
 typedef const __attribute__((address_space(1))) void* lds_gptr;
 typedef __attribute__((address_space(3))) void* lds_lptr;
 
-__device__ __forceinline__ constexpr int swizzle(int row) {
-  return (((row >> 2) & 1) << 1) | ((((row >> 3) ^ (row >> 1)) & 1) << 2);
-}
-
 struct HeadsArgs {
   const void* x;
   int64_t x_tok_stride, x_head_stride;
@@ -69,24 +65,40 @@ __global__ __launch_bounds__(256) void latent_heads_kernel(const HeadsArgs a, co
 }
 
 // ---------------------------------------------------------------------------
-// Expand.  A workgroup of four waves: 128 rows of the cache by NW values of one
-// head's keys or values; steps of 64 latent values through LDS (both operands
-// loaded straight into it, double-buffered).
+// Expand.  A workgroup of four waves: 128 rows of the cache by one head's keys and
+// values, steps of 32 latent values through LDS (both operands loaded straight
+// into it), three steps in LDS: two are on their way while one is multiplied.
+// A wave's tile is 64 rows by the head's keys or by its values.
+//
+// LDS layout of a step: rows of 64 bytes, chunk slots permuted by row bits (reads
+// of 16 rows by 4 chunks then cover every bank evenly).  The weights' rows are
+// dealt to the matrix instructions so that a lane's results of two of them lie
+// side by side: 16-byte stores.
 // ---------------------------------------------------------------------------
 namespace {
 
 constexpr int kBlockRows = 64;  // rows per block record
 constexpr int kTileRows = 128;
+constexpr int kStep = 32;
+
+__device__ __forceinline__ constexpr int swz(int row) {
+  return ((row >> 2) & 1) | ((((row >> 2) ^ (row >> 3)) & 1) << 1);
+}
+
+// The same for the weights, read in fours of rows, eight rows apart.
+__device__ __forceinline__ constexpr int swz_weights(int row) { return (row >> 3) & 3; }
 
 struct ExpandArgs {
   const void* pool;          // [slots][row]
   const int32_t* blocks;     // [n][4]: table offset, first position, positions of the request, 0
   const int32_t* tables;
-  const void* w;             // [heads][NW][latent]
-  void* out;                 // [heads][keys][NW]
-  void* rope;                // [keys][rope], or null
+  const void* key_up;        // [heads][NK][latent]
+  const void* value_up;      // [heads][NV][latent]
+  void* key_out;             // [heads][keys][NK]
+  void* value_out;           // [heads][keys][NV]
+  void* rope;                // [keys][rope]
   int64_t keys;              // rows of the workspace, a multiple of 128
-  int32_t heads, tiles, block_size, latent, row;
+  int32_t heads, tiles, block_size, rope_size;
   FastDiv by_block, by_heads;
 };
 
@@ -102,13 +114,16 @@ __device__ __forceinline__ float held(float x) {
 
 }  // namespace
 
-template <typename T, int NW>
+template <typename T, int L, int NK, int NV>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void latent_expand_kernel(const ExpandArgs a) {
-  constexpr int A_BYTES = kTileRows * 128, B_BYTES = NW * 128;
+  const int ROW = L + a.rope_size;
+  constexpr int A_BYTES = kTileRows * 64, B_BYTES = (NK + NV) * 64;
   __shared__ __attribute__((aligned(1024))) char a0[A_BYTES];
   __shared__ __attribute__((aligned(1024))) char a1[A_BYTES];
+  __shared__ __attribute__((aligned(1024))) char a2[A_BYTES];
   __shared__ __attribute__((aligned(1024))) char b0[B_BYTES];
   __shared__ __attribute__((aligned(1024))) char b1[B_BYTES];
+  __shared__ __attribute__((aligned(1024))) char b2[B_BYTES];
   const int tid = threadIdx.x & 255;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
   const int l16 = lane & 15, g = lane >> 4;
@@ -118,31 +133,31 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void l
   const int tg = fast_div(i, a.by_heads);
   const int h = i - tg * a.heads, tile = tg * 8 + xcd;
   if (tile >= a.tiles) return;
-  // Loads: instruction j of a wave fills rows 8 (4 j + wave) .. + 7, lane l row
-  // l / 8 of them, chunk slot l % 8.
-  constexpr int LA = kTileRows / 32, LB = NW / 32;
+  // Loads: instruction j of a wave fills rows 16 (4 j + wave) .. + 15, lane l row
+  // l / 4 of them, chunk slot l % 4.
+  constexpr int LA = kTileRows / 64, LB = (NK + NV) / 64;
   gptr<const T> arow[LA];
   gptr<const T> brow[LB];
 #pragma unroll
   for (int j = 0; j < LA; ++j) {
-    const int r = 8 * (4 * j + wave) + (lane >> 3);
-    const int32_t* b = a.blocks + 4 * (2 * tile + (r >= kBlockRows ? 1 : 0));
+    const int r = 16 * (4 * j + wave) + (lane >> 2);
+    const int32_t* b = a.blocks + 4 * (2 * tile + j);
     const int pos = min(b[1] + (r & (kBlockRows - 1)), b[2] - 1);
     const int lb = fast_div(pos, a.by_block);
     const int64_t slot = (int64_t)a.tables[b[0] + lb] * a.block_size + (pos - lb * a.block_size);
-    arow[j] = (gptr<const T>)(a.pool) + slot * a.row + 8 * ((lane & 7) ^ swizzle(r));
-    if (a.rope && h == 0) {
-      const int chunks = (a.row - a.latent) / 8;
-      if ((lane & 7) < chunks) {
-        gptr<const T> const from = (gptr<const T>)(a.pool) + slot * a.row + a.latent + 8 * (lane & 7);
-        store16((gptr<T>)(a.rope) + ((int64_t)tile * kTileRows + r) * (a.row - a.latent) + 8 * (lane & 7), load16(from));
-      }
+    arow[j] = (gptr<const T>)(a.pool) + slot * ROW + 8 * ((lane & 3) ^ swz(r));
+    if (h == 0) {
+      gptr<const T> const from = (gptr<const T>)(a.pool) + slot * ROW + L;
+      gptr<T> const to = (gptr<T>)(a.rope) + ((int64_t)tile * kTileRows + r) * a.rope_size;
+      for (int c = 8 * (lane & 3); c < a.rope_size; c += 32) store16(to + c, load16(from + c));
     }
   }
 #pragma unroll
   for (int j = 0; j < LB; ++j) {
-    const int r = 8 * (4 * j + wave) + (lane >> 3);
-    brow[j] = (gptr<const T>)(a.w) + ((int64_t)h * NW + r) * a.latent + 8 * ((lane & 7) ^ swizzle(r));
+    const int r = 16 * (4 * j + wave) + (lane >> 2);
+    gptr<const T> const w = 64 * j < NK ? (gptr<const T>)(a.key_up) + ((int64_t)h * NK + r) * L
+                                        : (gptr<const T>)(a.value_up) + ((int64_t)h * NV + r - NK) * L;
+    brow[j] = w + 8 * ((lane & 3) ^ swz_weights(r));
   }
   auto issue = [&](int k, char* ta, char* tb) {
 #pragma unroll
@@ -152,55 +167,71 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void l
     for (int j = 0; j < LB; ++j)
       __builtin_amdgcn_global_load_lds((lds_gptr)(brow[j] + k), (lds_lptr)(tb + (4 * j + wave) * 1024), 16, 0, 0);
   };
-  // Wave tile: 64 rows (wave / 2) by NW / 2 values (wave % 2).
-  constexpr int RT = 4, NT = NW / 32;
-  const int r0 = 64 * (wave >> 1), n0 = NW / 2 * (wave & 1);
-  f32x4 acc[NT][RT];
+  const bool values = wave & 1;
+  const int r0 = 64 * (wave >> 1);
+  // (Its own loop for each width: the barriers are the same.)
+  auto run = [&]<int WIDTH>(int n0, void* out) __attribute__((always_inline)) {
+    constexpr int RT = 4, NT = WIDTH / 16;
+    f32x4 acc[NT][RT];
 #pragma unroll
-  for (int n = 0; n < NT; ++n)
+    for (int n = 0; n < NT; ++n)
 #pragma unroll
-    for (int r = 0; r < RT; ++r) acc[n][r] = f32x4{0.f, 0.f, 0.f, 0.f};
-  auto compute = [&](const char* ta, const char* tb) __attribute__((always_inline)) {
+      for (int r = 0; r < RT; ++r) acc[n][r] = f32x4{0.f, 0.f, 0.f, 0.f};
+    const int x_at = (r0 + l16) * 64 + 16 * (g ^ swz(l16));
+    // (Row 4 i + e of instruction n is value 32 (n / 2) + 8 i + 4 (n % 2) + e.)
+    const int wrow = 8 * (l16 >> 2) + (l16 & 3);
+    const int w_at = (n0 + wrow) * 64 + 16 * (g ^ swz_weights(wrow));
+    auto compute = [&](const char* ta, const char* tb) __attribute__((always_inline)) {
+      uint4 xf[RT], wf[NT];
 #pragma unroll
-    for (int kk = 0; kk < 2; ++kk) {
-      const int slot = 16 * ((4 * kk + g) ^ swizzle(l16));
-      uint4 wf[NT], xf[RT];
+      for (int r = 0; r < RT; ++r) xf[r] = *reinterpret_cast<const uint4*>(ta + (1024 * r + x_at));
 #pragma unroll
-      for (int n = 0; n < NT; ++n) wf[n] = *reinterpret_cast<const uint4*>(tb + (n0 + 16 * n + l16) * 128 + slot);
-#pragma unroll
-      for (int r = 0; r < RT; ++r) xf[r] = *reinterpret_cast<const uint4*>(ta + (r0 + 16 * r + l16) * 128 + slot);
+      for (int n = 0; n < NT; ++n) wf[n] = *reinterpret_cast<const uint4*>(tb + (2048 * (n / 2) + 256 * (n % 2) + w_at));
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int r = 0; r < RT; ++r) acc[n][r] = Mma<T>::qk(wf[n], xf[r], acc[n][r]);
+    };
+    char *const as[3] = {a0, a1, a2}, *const bs[3] = {b0, b1, b2};
+    constexpr int STEPS = L / kStep;
+#pragma unroll
+    for (int i = 0; i < STEPS; ++i) {
+      // The step's loads have landed (the next one's may be on their way), and every
+      // wave has read the step before, whose place the step after the next takes.
+      if (i + 1 < STEPS) {
+        __builtin_amdgcn_s_waitcnt(0x0F70 | (LA + LB));
+      } else {
+        __builtin_amdgcn_s_waitcnt(0x0F70);
+      }
+      asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+      if (i + 2 < STEPS) issue((i + 2) * kStep, as[(i + 2) % 3], bs[(i + 2) % 3]);
+      __builtin_amdgcn_sched_barrier(0);  // (or the loads would be put off to the step's end)
+      compute(as[i % 3], bs[i % 3]);
+    }
+#pragma unroll
+    for (int r = 0; r < RT; ++r) {
+      const int64_t key = (int64_t)tile * kTileRows + r0 + 16 * r + l16;
+      gptr<T> const to = (gptr<T>)(out) + ((int64_t)h * a.keys + key) * WIDTH + 8 * g;
+#pragma unroll
+      for (int n = 0; n < NT; n += 2) {
+        T v[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = from_f32<T>(held<T>(acc[n + e / 4][r][e % 4]));
+        uint4 both;
+        __builtin_memcpy(&both, v, 16);
+        store16(to + 16 * n, both);
+      }
     }
   };
-  auto done = [&]() {
-    __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
-    __builtin_amdgcn_s_barrier();
-  };
+  __builtin_amdgcn_s_waitcnt(0x0F70);  // (the copies of the rotated keys: a step counts its own loads)
   issue(0, a0, b0);
-  done();
-  // (latent is a multiple of 128: an even number of steps.)
-  for (int k = 0; k < a.latent; k += 128) {
-    issue(k + 64, a1, b1);
-    compute(a0, b0);
-    done();
-    if (k + 128 < a.latent) issue(k + 128, a0, b0);
-    compute(a1, b1);
-    done();
-  }
-#pragma unroll
-  for (int r = 0; r < RT; ++r) {
-    const int64_t key = (int64_t)tile * kTileRows + r0 + 16 * r + l16;
-    T* const to = static_cast<T*>(a.out) + ((int64_t)h * a.keys + key) * NW + n0 + 4 * g;
-#pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      f32x4 v = acc[n][r];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) v[e] = held<T>(v[e]);
-      store_partial4<false, T>(to + 16 * n, v, 1.f);
-    }
+  issue(kStep, a1, b1);
+  if constexpr (NK == NV) {
+    run.template operator()<NK>(values ? NK : 0, values ? a.value_out : a.key_out);
+  } else if (values) {
+    run.template operator()<NV>(NK, a.value_out);
+  } else {
+    run.template operator()<NK>(0, a.key_out);
   }
 }
 
@@ -250,30 +281,38 @@ extern "C" int lvamd_latent_expand(const void* pool, const int32_t* blocks, int3
   const int64_t grid = (int64_t)(tiles + 7) / 8 * 8 * num_heads;
   if (grid > 0x7fffffffLL) return LVAMD_ERR_INVALID_ARGUMENT;
   hipStream_t s = static_cast<hipStream_t>(stream);
-  auto launch = [&]<typename T>(const void* w, void* out, void* rope, int width) -> int {
+  auto launch = [&]<typename T, int L>() -> int {
     ExpandArgs a{.by_block = FastDiv(block_size), .by_heads = FastDiv(num_heads)};
     a.pool = pool;
     a.blocks = blocks;
     a.tables = tables;
-    a.w = w;
-    a.out = out;
-    a.rope = rope;
+    a.key_up = key_up;
+    a.value_up = value_up;
+    a.key_out = keys;
+    a.value_out = values;
+    a.rope = rope_keys;
     a.keys = (int64_t)tiles * kTileRows;
     a.heads = num_heads;
     a.tiles = tiles;
     a.block_size = block_size;
-    a.latent = latent_size;
-    a.row = latent_size + rope_size;
-    if (width == 64) {
-      hipLaunchKernelGGL((latent_expand_kernel<T, 64>), dim3((unsigned)grid), dim3(256), 0, s, a);
+    a.rope_size = rope_size;
+    auto with = [&]<int NK, int NV>() {
+      hipLaunchKernelGGL((latent_expand_kernel<T, L, NK, NV>), dim3((unsigned)grid), dim3(256), 0, s, a);
+    };
+    if (nope_size == 64) {
+      value_size == 64 ? with.template operator()<64, 64>() : with.template operator()<64, 128>();
     } else {
-      hipLaunchKernelGGL((latent_expand_kernel<T, 128>), dim3((unsigned)grid), dim3(256), 0, s, a);
+      value_size == 64 ? with.template operator()<128, 64>() : with.template operator()<128, 128>();
     }
     return launch_status();
   };
-  auto both = [&]<typename T>() -> int {
-    const int status = launch.operator()<T>(key_up, keys, rope_keys, nope_size);
-    return status != LVAMD_OK ? status : launch.operator()<T>(value_up, values, nullptr, value_size);
+  auto sized = [&]<typename T>() -> int {
+    switch (latent_size) {
+      case 128: return launch.template operator()<T, 128>();
+      case 256: return launch.template operator()<T, 256>();
+      case 384: return launch.template operator()<T, 384>();
+      default: return launch.template operator()<T, 512>();
+    }
   };
-  return dtype == LVAMD_BF16 ? both.operator()<__bf16>() : both.operator()<_Float16>();
+  return dtype == LVAMD_BF16 ? sized.operator()<__bf16>() : sized.operator()<_Float16>();
 }
