@@ -29,6 +29,8 @@ from light_vllm_amd.quantized_cache import _NOT_FAST, _raw_stream, on_device
 
 # Column tiles (of 16) per workgroup that the latent-space kernel is built for.
 COL_TILES = (1, 2, 4, 8)
+# Rows of a tile, and the tiles per workgroup from which 128 columns pay.
+TILE_ROWS, WIDE_TILES = 32, 32
 # Widest workgroup whose launch appends the step's rows itself.
 APPEND_TILES = 4
 WEIGHT_SIZES = (64, 128)
@@ -107,13 +109,27 @@ def _step_args(spec: LatentLayerSpec, latent: Tensor, rope_key: Tensor, angles) 
         0 if cosines is None else cosines.stride(0), int(spec.rotary_layout == "interleaved"))
 
 
-def choose_col_tiles(q_lens, heads: int) -> int:
+def choose_col_tiles(q_lens, totals, heads: int, resident) -> int:
     """Column tiles per workgroup of a step: those of its widest request, as far
-    as the kernel is built (a wider workgroup reads a row once for more
-    columns)."""
+    as the kernel is built; 128 columns only where 64 would give each of the
+    ``resident(4)`` workgroups at least ``WIDE_TILES`` tiles.
+
+    A wider workgroup reads a row once for more columns; a narrower one holds two
+    to a CU and writes fewer partials, and up to 64 columns the launch appends.
+    Measured (us, 16/32/64/128 columns): 16 heads, 64 requests x 2300 tokens 43 / 43 /
+    55 / 67; 16 x 32767 tokens 114 / 119 / 146 / 178; 128 heads, 32 x 2300 (18 tiles
+    per workgroup) 99 / 68 / 63 / 63, and with the launches 70 against 74 for the last
+    two; 128 heads, 64 x 2300 (36 tiles) 133 / 106 / 88 for the last three, 8 x 32767
+    (64 tiles) 232 / 164 / 146 / 126; 16 heads, 9 queries, 32 x 8000 (96 tiles) 266 /
+    223 / 192 for the last three."""
 
     widest = -(-int(q_lens.max()) * heads // 16)
-    return next((t for t in COL_TILES if t >= widest), COL_TILES[-1])
+    fits = next((t for t in COL_TILES if t >= widest), COL_TILES[-1])
+    if fits > APPEND_TILES:
+        tiles = int((-(-totals // TILE_ROWS) * -(-q_lens * heads // (16 * APPEND_TILES))).sum())
+        if tiles < WIDE_TILES * resident(APPEND_TILES):
+            return APPEND_TILES
+    return fits
 
 
 def _expanded(facts, spec: LatentLayerSpec, nope: int, value: int) -> np.ndarray:
@@ -174,8 +190,11 @@ class LatentStepPlan(StepPlan):
         x.row_base, x.row_span, x.every_row, x.col_tiles = 0, 0, True, COL_TILES[0]
         x.num_blocks = x.num_units = x.num_unit_jobs = x.unit_merge_columns = x.num_unit_slots = 0
         if short.any():
-            x.col_tiles = choose_col_tiles(facts.q_lens[short], heads)
-            resident = native.latent_decode_resident_groups(code, spec.latent_size, spec.rope_size, x.col_tiles)
+            def groups(col_tiles: int) -> int:
+                return native.latent_decode_resident_groups(code, spec.latent_size, spec.rope_size, col_tiles)
+
+            x.col_tiles = choose_col_tiles(facts.q_lens[short], (facts.computed + facts.q_lens)[short], heads, groups)
+            resident = groups(x.col_tiles)
             mine = meta[short].copy()
             x.row_base = int(mine[0, 4])
             x.row_span = int(mine[-1, 4] + mine[-1, 3]) - x.row_base

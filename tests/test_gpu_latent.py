@@ -24,6 +24,7 @@ import pytest
 import torch
 
 import light_vllm_amd as lv
+from light_vllm_amd import latent_attention
 from oracle import latent_oracle as Z
 
 pytestmark = pytest.mark.gpu
@@ -384,17 +385,24 @@ CASES = [  # heads, latent, rope, block, computed, layouts
 ]
 
 
+@pytest.mark.parametrize("wide", (False, True))
 @pytest.mark.parametrize("dtype", ("bf16", "fp16"))
 @pytest.mark.parametrize("heads, latent, rope, bs, computed, layouts", CASES)
-def test_attention(heads, latent, rope, bs, computed, layouts, dtype) -> None:
-    _say(f"latent attention {heads} heads {latent}+{rope} blocks of {bs} {computed} {dtype}")
+def test_attention(heads, latent, rope, bs, computed, layouts, dtype, wide, monkeypatch) -> None:
+    """``wide``: 128 columns to a workgroup wherever a request has more than 64."""
+    if wide:
+        monkeypatch.setattr(latent_attention, "WIDE_TILES", 0)
+    _say(f"latent attention {heads} heads {latent}+{rope} blocks of {bs} {computed} {dtype} {wide}")
     args = _step(heads, latent, rope, bs, DTYPES[dtype], computed, layouts, seed=heads + bs)
     _attend_and_check(*args)
 
 
+@pytest.mark.parametrize("wide", (False, True))
 @pytest.mark.parametrize("layout", ("interleaved", "half"))
 @pytest.mark.parametrize("heads, latent, rope, bs, computed, layouts", CASES[1:4] + CASES[7:9])
-def test_attention_with_rotation(heads, latent, rope, bs, computed, layouts, layout) -> None:
+def test_attention_with_rotation(heads, latent, rope, bs, computed, layouts, layout, wide, monkeypatch) -> None:
+    if wide:
+        monkeypatch.setattr(latent_attention, "WIDE_TILES", 0)
     _say(f"latent attention with rotation {heads} heads {latent}+{rope} {layout}")
     args = _step(heads, latent, rope, bs, torch.bfloat16, computed, layouts, seed=heads + rope, layout=layout)
     gen = torch.Generator(device=DEV).manual_seed(1)
@@ -435,10 +443,13 @@ def test_strided_queries() -> None:
 
 
 @pytest.mark.parametrize("value", (math.nan, math.inf, -math.inf))
+@pytest.mark.parametrize("wide", (False, True))
 @pytest.mark.parametrize("heads, layouts", [(16, [TREE, 6]), (3, [tuple([-1] + [0] * 40), 40])])
-def test_values_that_are_not_finite_stay_where_they_are_seen(heads, layouts, value) -> None:
+def test_values_that_are_not_finite_stay_where_they_are_seen(heads, layouts, value, wide, monkeypatch) -> None:
     """A draft or later token whose row is not finite does not reach the queries
     that do not see it; those that see it follow the formula."""
+    if wide:
+        monkeypatch.setattr(latent_attention, "WIDE_TILES", 0)
     _say(f"latent attention, {value} in a masked row, {heads} heads")
     cache, md, q, latent, rope_key = _step(heads, 256, 64, 16, torch.bfloat16, [20, 33], layouts, seed=6)
     latent, rope_key = latent.clone(), rope_key.clone()

@@ -238,3 +238,19 @@ def test_oracle_rotation_keeps_lengths_and_angles_add() -> None:
         y = Z.rotate(Z.rotate(x, np.cos(a), np.sin(a), interleaved), np.cos(b), np.sin(b), interleaved)
         assert np.allclose(y, Z.rotate(x, np.cos(a + b), np.sin(a + b), interleaved))
         assert np.allclose(np.linalg.norm(y, axis=-1), np.linalg.norm(x, axis=-1))
+
+
+def test_column_tiles_of_a_step() -> None:
+    """The widest request's columns; 128 only where the workgroups of 64 would have
+    many tiles each."""
+    from light_vllm_amd.latent_attention import TILE_ROWS, WIDE_TILES, choose_col_tiles
+
+    def tiles(heads, q, total, resident=256):
+        return choose_col_tiles(np.asarray(q), np.asarray(total), heads, lambda t: resident)
+
+    assert [tiles(h, [1, 1], [9, 9]) for h in (1, 16, 17, 32, 33, 64, 65, 128)] == [1, 1, 2, 2, 4, 4, 4, 4]
+    assert tiles(16, [1, 3], [5000, 7]) == 4
+    enough = TILE_ROWS * WIDE_TILES * 256  # of one request with 65 to 128 columns: two groups of 64
+    assert tiles(128, [1], [enough // 2]) == 8
+    assert tiles(128, [1], [enough // 2 - TILE_ROWS]) == 4
+    assert tiles(16, [9], [enough // 3 + TILE_ROWS]) == 8
