@@ -27,40 +27,52 @@ struct HeadsArgs {
 
 }  // namespace
 
-// A wave: 16 values of n for 16 MT rows.  Weights and rows go from global memory
+// A wave: 16 NT values of n for 16 MT rows.  Weights and rows go from global memory
 // to operands as they lie (each lane 16 bytes of a row): a step's few tokens
-// leave nothing to reuse that the caches do not hold.
-template <typename T, int MT>
-__global__ __launch_bounds__(256) void latent_heads_kernel(const HeadsArgs a, const int32_t blocks_n) {
+// leave nothing to reuse that the caches do not hold.  With two of NT the rows of
+// the weights are dealt so that a lane's results of both lie side by side.
+template <typename T, int MT, int NT>
+__global__ __launch_bounds__(256) void latent_heads_kernel(const HeadsArgs a, const int32_t waves, const FastDiv by_blocks) {
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
   const int l16 = lane & 15, g = lane >> 4;
-  const int h = blockIdx.x / blocks_n;
-  const int n0 = (blockIdx.x - h * blocks_n) * 64 + 16 * wave;
+  const int i = blockIdx.x * 4 + wave;
+  if (i >= waves) return;
+  const int h = fast_div(i, by_blocks);
+  const int n0 = 16 * NT * (i - h * (a.n / (16 * NT)));
   const int m0 = blockIdx.y * 16 * MT;
-  const T* w = static_cast<const T*>(a.w) + ((int64_t)h * a.n + n0 + l16) * a.k + 8 * g;
+  const int wrow = NT == 1 ? l16 : 8 * (l16 >> 2) + (l16 & 3);
+  const T* w = static_cast<const T*>(a.w) + ((int64_t)h * a.n + n0 + wrow) * a.k + 8 * g;
   const T* x[MT];
   int64_t tok[MT];
-  f32x4 acc[MT];
+  f32x4 acc[MT][NT];
 #pragma unroll
   for (int m = 0; m < MT; ++m) {
     const int r = min(m0 + 16 * m + l16, a.num_rows - 1);
     tok[m] = a.rows ? a.rows[r] : r;
     x[m] = static_cast<const T*>(a.x) + tok[m] * a.x_tok_stride + (int64_t)h * a.x_head_stride + 8 * g;
-    acc[m] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int n = 0; n < NT; ++n) acc[m][n] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
   for (int k = 0; k < a.k; k += 64) {
 #pragma unroll
     for (int kk = 0; kk < 64; kk += 32) {
-      const uint4 wf = load16(w + k + kk);
+      uint4 wf[NT];
 #pragma unroll
-      for (int m = 0; m < MT; ++m) acc[m] = Mma<T>::qk(wf, load16(x[m] + k + kk), acc[m]);
+      for (int n = 0; n < NT; ++n) wf[n] = load16(w + (int64_t)4 * n * a.k + k + kk);
+#pragma unroll
+      for (int m = 0; m < MT; ++m) {
+        const uint4 xf = load16(x[m] + k + kk);
+#pragma unroll
+        for (int n = 0; n < NT; ++n) acc[m][n] = Mma<T>::qk(wf[n], xf, acc[m][n]);
+      }
     }
   }
 #pragma unroll
   for (int m = 0; m < MT; ++m) {
     if (m0 + 16 * m + l16 >= a.num_rows) continue;
-    T* y = static_cast<T*>(a.y) + tok[m] * a.y_tok_stride + (int64_t)h * a.y_head_stride + n0 + 4 * g;
-    store_partial4<false, T>(y, acc[m], 1.f);
+    T* y = static_cast<T*>(a.y) + tok[m] * a.y_tok_stride + (int64_t)h * a.y_head_stride + n0 + 4 * NT * g;
+#pragma unroll
+    for (int n = 0; n < NT; ++n) store_partial4<false, T>(y + 4 * n, acc[m][n], 1.f);
   }
 }
 
@@ -250,19 +262,21 @@ extern "C" int lvamd_latent_heads(const void* x, int64_t x_token_stride, int64_t
     return LVAMD_ERR_INVALID_ARGUMENT;
   HeadsArgs a{x, x_token_stride, x_head_stride, weights, y, y_token_stride, y_head_stride, rows, (int32_t)num_rows, k, n};
   hipStream_t s = static_cast<hipStream_t>(stream);
-  const int blocks_n = n / 64;
-  auto launch = [&]<typename T>() -> int {
-    // 64 rows per wave where that leaves the GPU enough workgroups.
-    if (num_rows > 64 && (int64_t)num_heads * blocks_n * ((num_rows + 63) / 64) >= 512) {
-      hipLaunchKernelGGL((latent_heads_kernel<T, 4>), dim3(num_heads * blocks_n, (unsigned)((num_rows + 63) / 64)), dim3(256),
-                         0, s, a, blocks_n);
-    } else {
-      hipLaunchKernelGGL((latent_heads_kernel<T, 1>), dim3(num_heads * blocks_n, (unsigned)((num_rows + 15) / 16)), dim3(256),
-                         0, s, a, blocks_n);
-    }
+  auto launch = [&]<typename T, int MT, int NT>() -> int {
+    const int blocks = n / (16 * NT), waves = num_heads * blocks;
+    hipLaunchKernelGGL((latent_heads_kernel<T, MT, NT>), dim3((unsigned)(waves + 3) / 4, (unsigned)((num_rows + 16 * MT - 1) / (16 * MT))), dim3(256), 0, s, a,
+                       waves, FastDiv(blocks));
     return launch_status();
   };
-  return dtype == LVAMD_BF16 ? launch.operator()<__bf16>() : launch.operator()<_Float16>();
+  // 64 rows by 32 values a wave where enough waves are left (us, 16 x 16 against
+  // 64 x 32): 16 heads, 128 to 512 values, 96 rows 4.9 / 5.4, 192 rows 8.4 / 5.7, 1536
+  // rows 47 / 24; back to 128, 192 rows 9.6 / 13.4, 384 rows 13.3 / 16.7, 768 rows 24.4 /
+  // 19.2; 128 heads, 96 rows 25.7 / 16.0 and 24.0 / 18.0.
+  auto typed = [&]<typename T>() -> int {
+    const bool wide = num_rows > 32 && (int64_t)num_heads * (n / 64) * ((num_rows + 63) / 64) >= 320;
+    return wide ? launch.template operator()<T, 4, 2>() : launch.template operator()<T, 1, 1>();
+  };
+  return dtype == LVAMD_BF16 ? typed.operator()<__bf16>() : typed.operator()<_Float16>();
 }
 
 extern "C" int lvamd_latent_expand(const void* pool, const int32_t* blocks, int32_t num_blocks, const int32_t* tables,

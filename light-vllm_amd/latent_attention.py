@@ -133,16 +133,24 @@ def choose_col_tiles(q_lens, totals, heads: int, resident) -> int:
 
 
 def _expanded(facts, spec: LatentLayerSpec, nope: int, value: int) -> np.ndarray:
-    """Which requests take the expanded form: linear ones where its products are
-    fewer (queries count in whole units, and the expansion of every key is part
-    of them)."""
+    """Which requests take the expanded form: linear ones where its products (with
+    the expansion of every key) are fewer than 1.2 times the absorbed form's, which
+    run at the lower rate.  Fewer than 64 queries cost as much as 64, keys count in
+    tiles.
+
+    Measured (us, absorbed / expanded; one request, 16 heads, 512 + 64, 128 / 128):
+    behind 1024 tokens 35 / 33 for 16 queries, 47 / 35 for 64, 74 / 39 for 256;
+    behind 8192 53 / 78, 78 / 82, 149 / 99; behind 32768 82 / 256, 149 / 262, 372 / 317,
+    with 512 queries 661 / 383; eight requests behind 8192 105 / 559, 250 / 567, 771 /
+    595.  Over 111 steps of 1 to 128 heads the choice is 2 % off the better form's
+    time, at most 1.5 times (8 requests of 32 queries, no history: 36 / 25)."""
 
     n, c = facts.q_lens.astype(np.float64), facts.computed.astype(np.float64)
     latent, rope = spec.latent_size, spec.rope_size
-    keys = c + n / 2
+    keys, held = c + n / 2, -(-(c + n) // TILE_ROWS) * TILE_ROWS
     absorbed = n * keys * (2 * latent + rope) + n * latent * (nope + value)
-    expanded = np.maximum(n, UNIT_QUERIES) * keys * (nope + rope + value) + (c + n) * latent * (nope + value)
-    return (facts.vis_off < 0) & (expanded < absorbed)
+    expanded = np.maximum(n, 64) * keys * (nope + rope + value) + held * latent * (nope + value)
+    return (facts.vis_off < 0) & (expanded < 1.2 * absorbed)
 
 
 class LatentStepPlan(StepPlan):
