@@ -206,6 +206,19 @@ def test_each_form_at_lengths_that_the_rule_gives_the_other(form, monkeypatch) -
     _run(args)
 
 
+@pytest.mark.parametrize("long", (0, 256))
+def test_many_short_requests(long, monkeypatch) -> None:
+    """Rows enough for the wide tiles of the products with the weights, their last
+    tile in part, with a long request's rows between them."""
+    _say(f"latent layer, 151 short requests, a long one of {long}")
+    _force(monkeypatch, lambda n, linear: n >= 200)
+    layouts = [1 + (i % 7 == 0) for i in range(151)]
+    computed = [(i * 5) % 41 for i in range(151)]
+    if long:
+        layouts[60], computed[60] = long, 10
+    _run(_step(128, 128, 32, 64, 64, 16, torch.bfloat16, computed, layouts, seed=12))
+
+
 def test_heads_in_groups(monkeypatch) -> None:
     _say("latent layer, heads in groups")
     _force(monkeypatch, lambda n, linear: n > 0)
