@@ -703,8 +703,8 @@ int lvamd_rotary_angles(const void* positions, int32_t position_bytes, int64_t n
  * dtype bf16 or fp16: a token's latent, then its rotated key, both shared by all
  * heads.  latent_size: 128, 256, 384 or 512; rope_size: 32 or 64.
  *
- * Append: entry i writes token sources[i] (NULL: i) to slots[i]; slots outside
- * [0, num_slots) are not written.  With cosines and sines (fp32,
+ * Append: entry i writes token sources[i] (NULL: i) to slots[i]; tokens outside
+ * [0, num_tokens) and slots outside [0, num_slots) are not written.  With cosines and sines (fp32,
  * [tokens][rope_size / 2], rows 16-byte aligned) the keys are turned: pairs (2i,
  * 2i + 1) if interleaved, else (i, i + rope_size / 2).  query_rope (NULL, or
  * [tokens][heads][rope_size] with angles): turned too, into rotated (contiguous).
@@ -737,22 +737,23 @@ int64_t lvamd_latent_move_workspace_size(int64_t num_pairs, int32_t num_layers, 
  * Attention in latent space: query [tokens][heads][latent_size] (multiplied by
  * the heads' key weights), query_rope [tokens][heads][rope_size], out
  * [tokens][heads][latent_size] (to be multiplied by the heads' value weights).
- * With latent and rope_key (else NULL: the pool holds them; NULL with col_tiles 8)
- * the launch appends the step's rows; with cosines and sines (as lvamd_latent_append's) it turns
- * query_rope and those keys first.
+ * With latent and rope_key (else NULL: the pool holds them; NULL with col_tiles
+ * 8) the launch appends the step's rows; with cosines and sines (as
+ * lvamd_latent_append's) it turns query_rope and those keys first.
  * jobs as lvamd_paged_decode's with one kv head and 16 * col_tiles columns a slot
  * (col_tiles: 1, 2, 4 or 8); pieces likewise up to field 10, then the index of the
  * workgroup's next piece (-1: none) and its first four table entries (-1: not
- * given); workgroup w of num_groups begins with piece w.  Split segments go through part_acc (fp32
- * [num_partial_slots][16 * col_tiles][latent_size]) and part_ml and are merged.
+ * given); workgroup w of num_groups begins with piece w.  Split segments go
+ * through part_acc (fp32 [num_partial_slots][16 * col_tiles][latent_size]) and
+ * part_ml and are merged.
  */
 int lvamd_latent_decode(const void* query, int64_t query_token_stride, int64_t query_head_stride,
                         const void* query_rope, int64_t rope_token_stride, int64_t rope_head_stride,
                         const void* latent, int64_t latent_token_stride, const void* rope_key,
                         int64_t rope_key_token_stride, const float* cosines, const float* sines,
                         int64_t angle_token_stride, int32_t interleaved, void* pool, void* out,
-                        int64_t out_token_stride, int64_t out_head_stride, const int32_t* pieces, int32_t num_groups, const int32_t* jobs, int32_t num_jobs,
-                        int32_t merge_columns, const int32_t* tables,
+                        int64_t out_token_stride, int64_t out_head_stride, const int32_t* pieces, int32_t num_groups,
+                        const int32_t* jobs, int32_t num_jobs, int32_t merge_columns, const int32_t* tables,
                         const uint32_t* vis, float* part_acc, float* part_ml, int64_t num_partial_slots,
                         int32_t num_heads, int32_t latent_size, int32_t rope_size, int32_t col_tiles,
                         int32_t block_size, float scale, int32_t dtype, lvamd_stream_t stream);

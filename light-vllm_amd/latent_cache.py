@@ -207,21 +207,16 @@ class LatentPagedKVCache:
         # when every rule holds; anything else takes the rules below.
         cfg = self._config
         facts = self._write_facts.get(layer_id) or self._bind_write(layer_id)
-        if (type(mapping) is PagedKVWriteMapping and torch.cuda.current_device() == facts[3]
-                and (rotary is None or (type(rotary) is tuple and len(rotary) == 2))):
-            slots, sources = mapping.slots, mapping.source_indices
-            n = slots.numel()
-            if (slots.dtype == torch.long and slots.ndim == 1 and slots.device == cfg.device and slots.is_contiguous()
-                    and (sources is None and n == mapping.num_query_tokens or sources is not None
-                         and sources.dtype == torch.long and sources.device == cfg.device and sources.shape == slots.shape
-                         and sources.is_contiguous())):
-                cosines, sines = rotary if rotary is not None else (None, None)
-                status = _latent_write()(facts, latent, rope_key, cosines, sines, slots.data_ptr(),
-                                         0 if sources is None else sources.data_ptr(), n, mapping.num_query_tokens)
-                if status == 0:
-                    return
-                if status != _NOT_FAST:
-                    native.check(status, "lvamd_latent_append")
+        if (type(mapping) is PagedKVWriteMapping and torch.cuda.current_device() == facts[4]
+                and (rotary is None or (type(rotary) is tuple and len(rotary) == 2 and rotary[0] is not None))):
+            sources, tokens = mapping.source_indices, mapping.num_query_tokens
+            cosines, sines = rotary if rotary is not None else (None, None)
+            status = _latent_write()(facts, latent, rope_key, cosines, sines, mapping.slots, sources,
+                                     tokens if sources is None else sources.numel(), tokens)
+            if status == 0:
+                return
+            if status != _NOT_FAST:
+                native.check(status, "lvamd_latent_append")
         spec = self.layer_spec(layer_id)
         check_rows(cfg, spec, latent, rope_key)
         slots, sources = mapping.slots, mapping.source_indices
@@ -244,7 +239,7 @@ class LatentPagedKVCache:
         spec, cfg = self.layer_spec(layer_id), self._config
         index = cfg.device.index if cfg.device.index is not None else torch.cuda.current_device()
         found = self._write_facts[layer_id] = (
-            cfg.dtype, torch.float32, _raw_stream, index, native.entry("lvamd_latent_append"),
+            torch.long, cfg.dtype, torch.float32, _raw_stream, index, native.entry("lvamd_latent_append"),
             self.layer(layer_id).rows.data_ptr(), self._slots, spec.latent_size, spec.rope_size, dtype_code(cfg.dtype),
             int(spec.rotary_layout == "interleaved"))
         return found

@@ -137,8 +137,9 @@ class RotaryEmbedding:
         n, half = positions.shape[0] if isinstance(positions, Tensor) and positions.ndim == 1 else 0, self.size // 2
         if 0 < n <= (2**31 - 1) // half and torch.cuda.current_device() == self.device.index:
             code = dtype_code(dtype)
-            both = torch.empty((2, n, self.size if full else half), dtype=dtype, device=self.device)
-            cosines, sines = both.unbind(0)
+            width = self.size if full else half
+            cosines = torch.empty_strided((n, width), (width, 1), dtype=dtype, device=self.device)
+            sines = torch.empty_strided((n, width), (width, 1), dtype=dtype, device=self.device)
             status = self._angles(self._facts, positions, n, cosines.data_ptr(), sines.data_ptr(), 2 if full else 1, code,
                                   self.magnitude)
             if status == 0:

@@ -220,7 +220,8 @@ def test_write_refusals() -> None:
                                (x, r[:1], None, "rope_size"), (x[:1], r[:1], None, "one entry per query"),
                                (x.cpu(), r.cpu(), None, "dtype and device"), (x, r, (c,), "a pair"),
                                (x, r, (c, c[:1]), "sines must have shape"), (x, r, (c.half(), c), "cosines must be float32"),
-                               (x, r, (c, c.cpu()), "sines must be float32")):
+                               (x, r, (c, c.cpu()), "sines must be float32"),
+                               (x, r, (None, None), "cosines must have shape"), (x, r, (c, None), "sines must have shape")):
         with pytest.raises(lv.KVCacheError, match=message):
             cache.write_prepared("layer0", a, b, mapping, rotary=rot)
     with pytest.raises(lv.KVCacheError, match="int64 vectors"):
@@ -231,6 +232,20 @@ def test_write_refusals() -> None:
 
     with pytest.raises(lv.KVCacheError, match="its own write_prepared"):
         hip_append(cache, "layer0", x[:, None], x[:, None], 0, 0)
+
+
+def test_append_passes_over_tokens_that_are_not_there() -> None:
+    """Entries of a mapping made by hand whose token or slot is out of range."""
+    _say("latent append, tokens and slots out of range")
+    cache = _cache(4, 128, 32, 16, 4, torch.bfloat16)
+    _flat(cache).fill_(7)
+    x, r = torch.ones((2, 128), dtype=torch.bfloat16, device=DEV), torch.ones((2, 32), dtype=torch.bfloat16, device=DEV)
+    mapping = lv.PagedKVWriteMapping(torch.tensor([3, 5, 9, 64, -1, 11], device=DEV), 2,
+                                     torch.tensor([0, 2, -1, 1, 1, 1], device=DEV))
+    cache.write_prepared("layer0", x, r, mapping)
+    written = torch.zeros(64, dtype=torch.bool, device=DEV)
+    written[[3, 11]] = True
+    assert (_flat(cache)[written] == 1).all() and (_flat(cache)[~written] == 7).all()
 
 
 # ---- compact and block copies --------------------------------------------------------

@@ -314,6 +314,10 @@ def test_refusals() -> None:
     ):
         with pytest.raises(lv.KVCacheError, match=message):
             lv.HipPagedAttentionBackend().create(cache, md).forward("layer0", *args, scale=0.1, weights=weights)
+    for rot, message in (((None, None), "cosines must have shape"), ((rotary[0], None), "sines must have shape")):
+        with pytest.raises(lv.KVCacheError, match=message):
+            lv.HipPagedAttentionBackend().create(cache, md).forward("layer0", q, latent, rope_key, scale=0.1, rotary=rot,
+                                                                    weights=good)
 
 
 def test_graph_replays(monkeypatch) -> None:
