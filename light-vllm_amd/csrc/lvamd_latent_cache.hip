@@ -13,8 +13,8 @@ namespace lvamd {
 // it is off by less than 2^-52 of its turns (2^-35 of a turn at a million
 // turns); the reduced angle r, |r| <= pi / 4, is an fp32 value (off by 2^-25 r)
 // and sine and cosine are its Taylor sums to r^9 and r^10, whose next terms are
-// below 2^-29 and 2^-33.  A thread per pair; 32760 tokens of 64 take as long as 64 of
-// them, the 7.0 us of the host's call and its two allocations.
+// below 2^-29 and 2^-33.  A thread per pair; 32760 tokens of 64 values take 4.6
+// us, 64 of them 2.3; the host's call and its two allocations take 7.0 for either.
 // ---------------------------------------------------------------------------
 struct AnglesArgs {
   const void* positions;
@@ -59,8 +59,8 @@ __global__ __launch_bounds__(256) void rotary_angles_kernel(const AnglesArgs a) 
 // its key; then the same of every query head's rotated part.  The rotation is
 // fp32, rounded once to T.  Entries whose slot or token is out of range are passed
 // over.  A thread per chunk, for reads and writes of whole lines: 8190 tokens of
-// 512 + 64 (18.9 MB in and out) take under 5.4 us, the time of the host's call; a
-// launch of 64 tokens takes 3.4 us on the GPU.
+// 256 + 32 (10.5 MB in and out) take 4.2 us, 64 of 512 + 64 2.5; the host's call takes
+// 5.5 for either.
 // ---------------------------------------------------------------------------
 struct LatentAppendArgs {
   const void* latent;

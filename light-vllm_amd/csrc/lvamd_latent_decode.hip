@@ -26,8 +26,24 @@
 //     score passes it by 2^8 (lazy rescaling): a vote per tile in LDS.
 //   * Append: a tile's rows of this step are loaded from the step's tensors, and
 //     one column group writes them to the pool; keys and queries are turned on the
-//     way.  It saves the append's launch (4-6 us with its gap).
+//     way.  On the GPU it costs what the append's launch takes (48 requests: 30.4
+//     against 26.1 + 3.4 us), on the host it saves that launch (one request: 23
+//     against 30 us a call).
 //   * A tile has two barriers: its rows are there, its probabilities are there.
+//     The values of up to 64 columns are read before the softmax (43 against 45 us
+//     for 64 requests of 32 columns, 232 against 258 for 8 x 32767 x 128 columns).
+//
+// What bounds it.  Up to 32 columns two workgroups of a CU keep a tile of 37 KB
+// each in flight: 64 requests of 512 to 4,095 tokens (16 heads, 512 + 64, bf16, 182
+// MB) 41 us, 4.4 TB/s, of which 6 pass before the first tile and 31 at the full
+// rate; 16 x 32767 tokens (32 heads, fp16, 605 MB) 109 us, 5.5 TB/s.  From 64 columns on the
+// tile's own work: 1.7 us a tile of 64 columns, of which the matrix units are busy
+// 0.45 and LDS 0.6; the rest is vector instructions (two waves a SIMD) and the
+// round trips between the phases.  32 requests of 128 heads (97 MB, 21 GFLOP) 67 us:
+// 7 to the first tile, 18 to 20 tiles, 3 for the partials.  Eight waves rather than
+// four from 64 columns on: 140 against 145 us for 8 x 32767 x 128 heads.  Tile loads
+// are non-temporal: 50 against 55 us for the 64 requests.  Dealing the loads
+// between the score products measured slower (258 against 232 us).
 //
 // LDS tile layout: groups of 64 columns (128 bytes of every row), group-major;
 // one load of a wave fills 1 KB = 8 whole 128-byte lines of one group.  Chunk c
@@ -669,7 +685,9 @@ __attribute__((amdgpu_waves_per_eu(LatentShape<L, P, NC>::WAVES_PER_EU))) void l
 
 // ---------------------------------------------------------------------------
 // Merge: a workgroup per (job, column), a thread per four dimensions and other
-// piece; the two shares of the pieces join in LDS, in order.  With partial i's
+// piece; the two shares of the pieces join in LDS, in order.  (64 requests of 16
+// heads 5.1 us, 6.8 with one share in two passes; 32 of 144 columns 13.1, 16.8 with
+// four shares; bound by the partials, 2 KB a column and piece.)  With partial i's
 // maximum m_i (log2) and sum l_i, out = sum 2^(m_i - M) l_i o_i / sum 2^(m_i - M) l_i,
 // taken in one pass: a share's sums are scaled when its maximum moves.
 // ---------------------------------------------------------------------------

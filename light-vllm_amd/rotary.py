@@ -110,8 +110,8 @@ def rotary_frequencies(size: int, base: float, scaling: RotaryScaling | None = N
 class RotaryEmbedding:
     """Angles of positions for a rotated part of ``size`` values, on the GPU.
 
-    Made once per model; called once per step with the tokens' positions (int32
-    or int64, any shape flattened to ``[tokens]``; on the embedding's device),
+    Made once per model; called once per step with the tokens' positions (an int32
+    or int64 vector on the embedding's device),
     it returns ``(cosines, sines)``: ``[tokens, size / 2]``, one value per pair,
     or with ``full=True`` ``[tokens, size]``, each half the same (what the half
     layout multiplies a whole row with)."""
