@@ -354,3 +354,45 @@ def test_graph_replays(monkeypatch) -> None:
         torch.cuda.synchronize()
         _check(out, *_expected(cache, md, q, rotary, up, 0.07))
         assert torch.equal(run(backend.create(cache, md)), out)
+
+
+def test_rows_past_32_bits_of_the_pool(monkeypatch) -> None:
+    """A pool of 4.6e9 values (9.2 GB): the same step at its last blocks gives what a
+    small pool gives, in both forms, and so do write, compact and block copies."""
+    _say("latent layer, a pool of 9.2 GB")
+    case = (16, 512, 64, 128, 128, 16, torch.bfloat16)
+    computed, layouts = [40, 5, 100], [300, TREE, 1]
+    big_blocks = 500_000
+    large = lv.LatentPagedKVCache(_step(*case, [0], [1], seed=13)[0].model_spec, lv.PagedKVCacheConfig(
+        num_blocks=big_blocks, block_size=16, dtype=torch.bfloat16, device=DEV))
+    rows_large = large.layer("layer0").rows
+    assert rows_large.numel() > 2**32
+    _force(monkeypatch, lambda n, linear: n >= 200)
+    for wide in (False, True):
+        if wide:
+            monkeypatch.setattr(latent_attention, "WIDE_TILES", 0)
+        small, md, q, latent, rope_key, rotary, up = _step(*case, computed, layouts, seed=13)
+        rows_small = small.layer("layer0").rows
+        n = rows_small.shape[0]
+        off = big_blocks - n
+        rows_large[off:] = rows_small
+        rows_large[:n] = 7
+        far = lv.PagedAttentionMetadata(block_tables=tuple(tuple(b + off for b in t) for t in md.block_tables),
+                                        num_computed_tokens=md.num_computed_tokens, query_layouts=md.query_layouts)
+        outs = [lv.HipPagedAttentionBackend().create(cache, m).forward(
+            "layer0", q, latent, rope_key, scale=0.07, rotary=rotary, weights=lv.LatentWeights(*up))
+            for cache, m in ((small, md), (large, far))]
+        assert torch.equal(outs[0], outs[1])
+
+        def same():
+            a, b = rows_small.view(torch.int16), rows_large[off:].view(torch.int16)  # (bits: some are NaN)
+            assert torch.equal(a, b) and bool((rows_large[:n] == 7).all())
+
+        same()
+        slots = torch.tensor([3, 16 * n - 1], device=DEV)
+        for cache, at in ((small, 0), (large, 16 * off)):
+            cache.write("layer0", latent[:2], rope_key[:2], slots + at, rotary=(rotary[0][:2], rotary[1][:2]))
+            cache.copy_blocks([at // 16], [at // 16 + 1])
+            cache.compact(tuple(b + at // 16 for b in md.block_tables[1]), num_computed_tokens=5, num_query_tokens=9,
+                          num_reserved_query_tokens=9, retained_query_indices=(0, 2, 5))
+        same()
