@@ -155,7 +155,22 @@ def _expanded(facts, spec: LatentLayerSpec, nope: int, value: int) -> np.ndarray
 
 
 class LatentStepPlan(StepPlan):
-    """A step plan with the latent kernels' work lists per layer shape."""
+    """A step plan with the latent kernels' work lists per layer shape.
+
+    It may be used on streams that run after the one it was made on, and dropped
+    while their work is pending."""
+
+    def __init__(self, *args, **kwargs) -> None:
+        super().__init__(*args, **kwargs)
+        self._stream = current_stream(self._staging.device)  # the allocator's, for the lists
+
+    def use_on(self, stream: int) -> None:
+        """Before a launch on ``stream``, the current one: the lists are that
+        stream's until then, whoever drops the plan."""
+
+        if stream != self._stream:
+            for blob in (self._blob, *self._late_blobs):
+                blob.record_stream(torch.cuda.current_stream(self._staging.device))
 
     def shape(self, spec: LatentLayerSpec, code: int, weights: tuple[int, int] | None) -> _Shape:
         """``weights``: (nope_size, value_size), or None where queries come
@@ -167,8 +182,18 @@ class LatentStepPlan(StepPlan):
             if self._committed and torch.cuda.is_current_stream_capturing():
                 raise errors.ExecutionError("a step of this form must run once before it is captured (its work lists are "
                                             "uploaded then)")
-            found = self.launches[key] = self._plan_shape(spec, code, weights)
+            found = self._plan_shape(spec, code, weights)
+            late = self._committed
             self._register(key, found.lists)
+            if late:
+                # (The next launch may be on another stream than this one.)
+                device = self._staging.device
+                torch.cuda.current_stream(device).synchronize()
+                made_on = torch.cuda.ExternalStream(self._stream, device=device) if self._stream else (
+                    torch.cuda.default_stream(device))
+                for blob in self._late_blobs:
+                    blob.record_stream(made_on)
+            self.launches[key] = found
         return found
 
     def bind(self, x: _Shape, spec: LatentLayerSpec, config, code: int, weights: tuple[int, int] | None) -> None:
@@ -300,6 +325,7 @@ class HipLatentPagedAttention:
                 plan.bind(shape, spec, cfg, code, sizes)
                 facts = shape.facts
             if torch.cuda.current_device() == facts[3]:
+                plan.use_on(_raw_stream(facts[3]))
                 out = torch.empty_strided(shape.out_shape, shape.out_strides, dtype=cfg.dtype, device=cfg.device)
                 # (Of the call's own stream or graph: no two share one.)
                 scratch = torch.empty_strided((shape.scratch_bytes,), (1,), dtype=torch.uint8,
@@ -346,6 +372,7 @@ class HipLatentPagedAttention:
         with on_device(cfg.device):
             code, stream = dtype_code(cfg.dtype), current_stream(cfg.device)
             shape = plan.shape(spec, code, sizes)
+            plan.use_on(stream)
             self._backend.note_latent_form(cache, sizes)
             width = spec.latent_size if weights is None else weights.value_size
             out = torch.empty((query.shape[0], heads, width), dtype=cfg.dtype, device=cfg.device)

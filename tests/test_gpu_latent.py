@@ -504,6 +504,30 @@ def test_two_layers_share_a_plan_and_layers_run_once() -> None:
         lv.HipPagedAttentionBackend().create(cache, bad)
 
 
+def test_layers_of_both_rotary_layouts_share_a_plan() -> None:
+    """Layers that differ in the layout alone take the same work lists, each its own turn."""
+    _say("latent attention, layers of both layouts")
+    layouts = ("interleaved", "half", "interleaved")
+    one = {kind: _step(16, 256, 64, 16, torch.bfloat16, [33, 7], [1, TREE], seed=9, layout=kind) for kind in layouts}
+    cache, md, q, latent, rope_key = one["half"]
+    spec = lv.LatentKVCacheSpec(tuple(lv.LatentLayerSpec(f"layer{i}", 16, 256, 64, k) for i, k in enumerate(layouts)))
+    many = lv.LatentPagedKVCache(spec, cache.config)
+    for i in range(3):
+        many.layer(f"layer{i}").rows.copy_(cache.layer("layer0").rows)
+    rotary = _angles(q.shape[0], 64, torch.Generator(device=DEV).manual_seed(1))
+    want = {kind: lv.HipPagedAttentionBackend().create(one[kind][0], md).forward(
+        "layer0", q, latent, rope_key, scale=0.1, rotary=rotary) for kind in layouts[:2]}
+    assert not torch.equal(want["half"], want["interleaved"])
+    backend = lv.HipPagedAttentionBackend()
+    for order in ((0, 1, 2), (1, 0, 2)):
+        context = backend.create(many, md)
+        for i in order:
+            out = context.forward(f"layer{i}", q, latent, rope_key, scale=0.1, rotary=rotary)
+            assert torch.equal(out, want[layouts[i]])
+            a, b = (c.layer(name).rows.view(torch.int16) for c, name in ((many, f"layer{i}"), (one[layouts[i]][0], "layer0")))
+            assert torch.equal(a, b)
+
+
 def test_graph_replays_and_streams() -> None:
     """A captured step replays with new inputs, with eager steps of the same
     backend between; two streams run steps of one backend at once."""

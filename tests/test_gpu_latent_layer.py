@@ -396,3 +396,31 @@ def test_rows_past_32_bits_of_the_pool(monkeypatch) -> None:
             cache.compact(tuple(b + at // 16 for b in md.block_tables[1]), num_computed_tokens=5, num_query_tokens=9,
                           num_reserved_query_tokens=9, retained_query_indices=(0, 2, 5))
         same()
+
+
+def test_steps_on_other_streams_than_their_plans() -> None:
+    """A context whose lists lie on another stream may be dropped while its step is
+    pending, and lists that a first forward uploads are there for every stream."""
+    _say("latent layer, contexts used on other streams")
+    args = _step(16, 256, 64, 128, 64, 16, torch.bfloat16, [300, 40], [1, 5], seed=14)
+    cache, md, q, latent, rope_key, rotary, up = args
+    weights = lv.LatentWeights(*up)
+    call = dict(scale=0.07, rotary=rotary, weights=weights)
+    want = lv.HipPagedAttentionBackend().create(cache, md).forward("layer0", q, latent, rope_key, **call)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for fresh in (True, False):
+        backend = lv.HipPagedAttentionBackend()
+        if not fresh:  # (the form is known: its lists are uploaded by create)
+            backend.create(cache, md).forward("layer0", q, latent, rope_key, **call)
+        torch.cuda.synchronize()
+        contexts = [backend.create(cache, md) for _ in streams]
+        torch.cuda.synchronize()
+        outs = []
+        for stream in streams:
+            with torch.cuda.stream(stream):
+                torch.cuda._sleep(2_000_000)
+                outs.append(contexts.pop(0).forward("layer0", q, latent, rope_key, **call))
+        backend._last = None  # (the last plan's keeper)
+        junk = [torch.full((n,), -1, dtype=torch.int32, device=DEV) for n in (64, 256, 512, 1024, 4096, 1 << 16) for _ in range(8)]
+        torch.cuda.synchronize()
+        assert len(junk) and all(torch.equal(o, want) for o in outs)
