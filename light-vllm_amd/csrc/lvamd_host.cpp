@@ -41,6 +41,7 @@
 #include <climits>
 #include <cstdint>
 #include <cstring>
+#include <exception>
 #include <functional>
 #include <limits>
 #include <numeric>
@@ -1651,33 +1652,37 @@ PyObject* latent_work(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   }
   d.hkv = d.min_units = 1;
   d.trim = true;
-  DecodeLists out;
-  const int32_t* ids = flat.data<int32_t>();
-  build_decode(q, ids, flat.count(), d, out);
-  std::vector<int32_t> pieces(out.pieces.size());
-  for (int64_t w = 0, rest = out.waves; w < out.waves; ++w) {
-    const int64_t p0 = out.first[(size_t)w], p1 = out.first[(size_t)w + 1];
-    for (int64_t p = p0, at = w; p < p1; ++p) {
-      int32_t* o = pieces.data() + at * kPieceFields;
-      const int32_t* x = out.pieces.data() + p * kPieceFields;
-      std::memcpy(o, x, 11 * sizeof(int32_t));
-      o[11] = p + 1 < p1 ? (int32_t)rest : -1;
-      const int64_t lb0 = x[2] / d.bs;
-      for (int64_t k = 0; k < 4; ++k) {
-        const int64_t lb = lb0 + k, i = x[5] + lb;
-        o[12 + k] = (x[2] % d.bs + d.unit - 1) / d.bs >= 4 ? -1 : lb * d.bs < x[3] && i < flat.count() ? ids[i] : 0;
+  try {
+    DecodeLists out;
+    const int32_t* ids = flat.data<int32_t>();
+    build_decode(q, ids, flat.count(), d, out);
+    std::vector<int32_t> pieces(out.pieces.size());
+    for (int64_t w = 0, rest = out.waves; w < out.waves; ++w) {
+      const int64_t p0 = out.first[(size_t)w], p1 = out.first[(size_t)w + 1];
+      for (int64_t p = p0, at = w; p < p1; ++p) {
+        int32_t* o = pieces.data() + at * kPieceFields;
+        const int32_t* x = out.pieces.data() + p * kPieceFields;
+        std::memcpy(o, x, 11 * sizeof(int32_t));
+        o[11] = p + 1 < p1 ? (int32_t)rest : -1;
+        const int64_t lb0 = x[2] / d.bs;
+        for (int64_t k = 0; k < 4; ++k) {
+          const int64_t lb = lb0 + k, i = x[5] + lb;
+          o[12 + k] = (x[2] % d.bs + d.unit - 1) / d.bs >= 4 ? -1 : lb * d.bs < x[3] && i < flat.count() ? ids[i] : 0;
+        }
+        if (p + 1 < p1) at = rest++;
       }
-      if (p + 1 < p1) at = rest++;
     }
+    PyObject* a = to_bytearray(pieces);
+    PyObject* b = to_bytearray(out.jobs);
+    PyObject* result = (a && b) ? Py_BuildValue("(OOLiLi)", a, b, (long long)out.waves, out.slots, (long long)out.merge_cols,
+                                                out.depth)
+                                : nullptr;
+    Py_XDECREF(a);
+    Py_XDECREF(b);
+    return result;
+  } catch (const std::exception&) {  // (lists past what memory or a vector holds)
+    return PyErr_NoMemory();
   }
-  PyObject* a = to_bytearray(pieces);
-  PyObject* b = to_bytearray(out.jobs);
-  PyObject* result = (a && b) ? Py_BuildValue("(OOLiLi)", a, b, (long long)out.waves, out.slots, (long long)out.merge_cols,
-                                              out.depth)
-                              : nullptr;
-  Py_XDECREF(a);
-  Py_XDECREF(b);
-  return result;
 }
 
 // prefill_work(req_meta i32[B*8], flat i32, group, columns, key_tokens,
@@ -2735,7 +2740,8 @@ int latent_step(PyObject* latent, PyObject* key, PyObject* cos, PyObject* sin, c
 }
 
 // latent_write(facts, latent, rope_key, cosines, sines, slots, sources, entries, tokens)
-// facts: the dtype object of slots, then a TensorFacts tuple; ints: fn, pool, slots of the pool, latent size, rope size, dtype code, interleaved
+// facts: the dtype object of slots, then a TensorFacts tuple
+// ints: fn, pool, slots of the pool, latent size, rope size, dtype code, interleaved
 PyObject* latent_write(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   if (!want_args(nargs, 9, "latent_write")) return nullptr;
   TensorFacts t;

@@ -416,7 +416,8 @@ __attribute__((amdgpu_waves_per_eu(LatentShape<L, P, NC>::WAVES_PER_EU))) void l
       // that an instruction does not wait for the one before it.
       constexpr int TOT = QKS * KSTEPS, LEAD = NC == 8 ? 3 : 6, CH = QKS == 1 ? 2 : 1;
       auto rd = [&](int i) -> uint4 {
-        return *reinterpret_cast<const uint4*>(here + (((i / QKS) >> 1) * (KT * 128) + (i % QKS) * 16 * 128 + (kbase ^ ((i / QKS) & 1 ? 64 : 0))));
+        const int group = (i / QKS) >> 1, odd_chunks = (i / QKS) & 1;
+        return *reinterpret_cast<const uint4*>(here + (group * (KT * 128) + (i % QKS) * 16 * 128 + (kbase ^ (odd_chunks ? 64 : 0))));
       };
       uint4 key[LEAD];
 #pragma unroll

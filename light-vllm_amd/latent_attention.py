@@ -214,6 +214,8 @@ class LatentStepPlan(StepPlan):
 
     def _plan_shape(self, spec: LatentLayerSpec, code: int, weights: tuple[int, int] | None) -> _Shape:
         facts, heads, host = self.facts, spec.num_query_heads, native.host()
+        if int(facts.q_lens.max()) * heads > 2**31 - 1:
+            raise errors.KVCacheError("a request's queries times its heads must be below 2**31")
         none = np.zeros(0, np.int32)
         meta = self._req_meta.reshape(-1, native.REQ_FIELDS)
         long = np.zeros(self.batch_size, bool) if weights is None else _expanded(facts, spec, *weights)

@@ -528,6 +528,13 @@ def test_layers_of_both_rotary_layouts_share_a_plan() -> None:
             assert torch.equal(a, b)
 
 
+def test_columns_past_32_bits_are_refused() -> None:
+    cache, md, *_ = _step(1, 128, 32, 16, torch.bfloat16, [3], [2], seed=1)
+    wide = lv.LatentPagedKVCache(lv.LatentKVCacheSpec((lv.LatentLayerSpec("layer0", 2**30, 128, 32, "half"),)), cache.config)
+    with pytest.raises(lv.KVCacheError, match="below 2"):
+        lv.HipPagedAttentionBackend().create(wide, md)
+
+
 def test_graph_replays_and_streams() -> None:
     """A captured step replays with new inputs, with eager steps of the same
     backend between; two streams run steps of one backend at once."""
