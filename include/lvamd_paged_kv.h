@@ -757,7 +757,8 @@ int lvamd_latent_decode(const void* query, int64_t query_token_stride, int64_t q
                         const uint32_t* vis, float* part_acc, float* part_ml, int64_t num_partial_slots,
                         int32_t num_heads, int32_t latent_size, int32_t rope_size, int32_t col_tiles,
                         int32_t block_size, float scale, int32_t dtype, lvamd_stream_t stream);
-int lvamd_latent_decode_tile_tokens(void);
+/* Rows per tile (the unit of pieces). */
+int lvamd_latent_decode_tile_tokens(int32_t col_tiles);
 /* Workgroups of lvamd_latent_decode the current GPU holds at once. */
 int lvamd_latent_decode_resident_groups(int32_t dtype, int32_t latent_size, int32_t rope_size, int32_t col_tiles);
 

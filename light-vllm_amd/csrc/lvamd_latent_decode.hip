@@ -11,12 +11,12 @@
 // Mapping onto CDNA4:
 //   * A column is a (query, head) pair of one request; a workgroup (four waves, or
 //     eight of 64 columns and more) holds up to 16 NC of them and walks over tiles
-//     of 32 rows: stream-K pieces of (request, column group) segments, split
+//     of 32 rows (64 with 64 columns): stream-K pieces of (request, column group) segments, split
 //     segments merged below.
 //   * The rows of a tile are loaded once, straight into LDS (global_load_lds, no
 //     registers), while the tile before is computed; they serve as keys (rows
 //     read as they lie) and as values (transpose reads).
-//   * Scores: S^T = K Q^T on MFMA 16x16x32, the 16-row halves of the tile and the
+//   * Scores: S^T = K Q^T on MFMA 16x16x32, the 16-row parts of the tile and the
 //     column tiles dealt to the waves, queries in registers.  Products: O^T = V^T
 //     P^T, a share of the latent's dimensions per wave for all columns, so an
 //     accumulator takes a share of the registers that a whole row would, and
@@ -37,10 +37,10 @@
 // each in flight: 64 requests of 512 to 4,095 tokens (16 heads, 512 + 64, bf16, 182
 // MB) 41 us, 4.4 TB/s, of which 6 pass before the first tile and 31 at the full
 // rate; 16 x 32767 tokens (32 heads, fp16, 605 MB) 109 us, 5.5 TB/s.  From 64 columns on the
-// tile's own work: 1.7 us a tile of 64 columns, of which the matrix units are busy
-// 0.45 and LDS 0.6; the rest is vector instructions (two waves a SIMD) and the
-// round trips between the phases.  32 requests of 128 heads (97 MB, 21 GFLOP) 67 us:
-// 7 to the first tile, 18 to 20 tiles, 3 for the partials.  Eight waves rather than
+// tile's own work: about 2.8 us for 64 rows and 64 columns, of which the matrix units
+// are busy 0.9 and LDS 1.1; the rest is vector instructions (two waves a SIMD) and
+// the round trips between the phases.  32 requests of 128 heads (97 MB, 21 GFLOP)
+// 61 us: 7 to the first tile, 9 to 10 tiles, 3 for the partials.  Eight waves rather than
 // four from 64 columns on: 140 against 145 us for 8 x 32767 x 128 heads.  Tile loads
 // are non-temporal: 50 against 55 us for the 64 requests.  Dealing the loads
 // between the score products measured slower (258 against 232 us).
@@ -60,7 +60,11 @@ namespace lvamd {
 namespace {
 
 constexpr float kSlack = 8.0f;  // lazy-rescale threshold, log2 units
-constexpr int KT = 32;          // rows per tile
+// Rows per tile.  64 columns leave registers and LDS for 64 rows, which halves a
+// row's share of the barriers and round trips (128 against 147 us for 8 x 32767 tokens
+// of 128 heads, 95 against 104 for 64 x 2300); 128 columns do not, and two workgroups
+// of a CU do not fit with fewer.
+constexpr int tile_rows(int col_tiles) { return col_tiles == 4 ? 64 : 32; }
 
 typedef const __attribute__((address_space(1))) void* lds_gptr;
 typedef __attribute__((address_space(3))) void* lds_lptr;
@@ -114,11 +118,12 @@ struct LatentShape {
   static constexpr int ROW = L + P;                   // elements
   static constexpr int CPR = ROW / 8;                 // 16-byte chunks of a row
   static constexpr int GR = (CPR + 7) / 8;            // 128-byte groups
+  static constexpr int KT = tile_rows(NC);
   static constexpr int TILE_BYTES = GR * KT * 128;
   static constexpr int KSTEPS = ROW / 32;             // MFMA steps of a score
   static constexpr int W = NC >= 4 ? 8 : 4;           // waves
   static constexpr int DT = L / (16 * W);             // 16-dimension tiles per wave
-  static constexpr int QKS = NC == 8 ? 2 : 1;         // 16-row halves a wave scores
+  static constexpr int QKS = NC >= 4 ? 2 : 1;         // 16-row parts a wave scores
   static constexpr int NB = 2;                        // tiles in LDS
   static constexpr int WAVES_PER_EU = 2;
   static constexpr bool APPEND = NC < 8;              // (128 columns: no registers left for it)
@@ -137,14 +142,14 @@ __global__ __launch_bounds__(NC >= 4 ? 512 : 256)
 __attribute__((amdgpu_waves_per_eu(LatentShape<L, P, NC>::WAVES_PER_EU))) void latent_decode_kernel(
     const int32_t* __restrict__ pieces, const LatentDecodeArgs a) {
   using S = LatentShape<L, P, NC>;
-  constexpr int GR = S::GR, KSTEPS = S::KSTEPS, DT = S::DT, QKS = S::QKS, W = S::W;
+  constexpr int KT = S::KT, GR = S::GR, KSTEPS = S::KSTEPS, DT = S::DT, QKS = S::QKS, W = S::W;
   constexpr int COLS = 16 * NC;
   constexpr bool APPEND = S::APPEND;
   using V8 = typename std::conditional<std::is_same<T, __bf16>::value, bf16x8, f16x8>::type;
   // Separate objects: a load into one does not alias a read of another.
   __shared__ __attribute__((aligned(1024))) char tile0[S::TILE_BYTES];
   __shared__ __attribute__((aligned(1024))) char tile1[S::TILE_BYTES];
-  __shared__ __attribute__((aligned(16))) uint2 probs[NC * 64 * 2];  // [column tile][lane][half]
+  __shared__ __attribute__((aligned(16))) uint2 probs[KT / 32 * NC * 64 * 2];  // [32 rows][column tile][lane][half]
   __shared__ float tile_max[2][COLS], col_max[COLS], col_sum[2][COLS];
   __shared__ __attribute__((aligned(16))) uint32_t votes[W];
 
@@ -154,13 +159,14 @@ __attribute__((amdgpu_waves_per_eu(LatentShape<L, P, NC>::WAVES_PER_EU))) void l
 
   // ---- this wave's scores: rows [16 ks0, 16 (ks0 + QKS)) of a tile, column tile ct0.
   const bool scores = NC > 1 || wave < 2;
-  const int ks0 = QKS == 2 ? 0 : wave & 1;
-  const int ct0 = NC == 1 ? 0 : QKS == 2 ? wave : wave >> 1;
+  constexpr int HALVES = KT / (16 * QKS);  // waves that share a column tile
+  const int half = HALVES == 1 ? 0 : wave & 1, ks0 = QKS * half;
+  const int ct0 = NC == 1 ? 0 : HALVES == 1 ? wave : wave >> 1;
 
-  // ---- tile loads: wave w loads rows 8 (w % 4) .. + 7 of the groups w / 4, + W / 4,
+  // ---- tile loads: wave w loads rows 8 (w % RB) .. + 7 of the groups w / RB, + W / RB,
   // ..; lane l row l / 8 of them into chunk slot l % 8 of a group.
-  constexpr int GSTEP = W / 4;
-  const int rb = wave & 3;
+  constexpr int RB = KT / 8, GSTEP = W / RB;
+  const int rb = wave % RB;
   // The load cursor: the tile whose rows are looked up next.  first_new: the
   // position from which rows are the step's own, read from its tensors.
   struct Cursor {
@@ -186,7 +192,7 @@ __attribute__((amdgpu_waves_per_eu(LatentShape<L, P, NC>::WAVES_PER_EU))) void l
     }
 #pragma unroll
     for (int i = 0; i < (GR + GSTEP - 1) / GSTEP; ++i) {
-      const int gr = (wave >> 2) + i * GSTEP;
+      const int gr = wave / RB + i * GSTEP;
       if (GR % GSTEP != 0 && gr >= GR) break;
       int c = 8 * gr + lchunk;
       // (A half-used last group's spare slots take the row's last chunk again.)
@@ -208,7 +214,7 @@ __attribute__((amdgpu_waves_per_eu(LatentShape<L, P, NC>::WAVES_PER_EU))) void l
   constexpr int KEY_GROUP = L / 64;
   auto key_chunk = [&](int ln) -> int {  // -1: not this lane's
     const int c = (ln & 7) ^ swizzle(8 * rb + (ln >> 3));
-    return (W == 4 || (wave >> 2) == KEY_GROUP % GSTEP) && c < 2 * HALF ? c : -1;
+    return (GSTEP == 1 || wave / RB == KEY_GROUP % GSTEP) && c < 2 * HALF ? c : -1;
   };
   auto key_place = [&](int ln, char* tile) -> uint4* {
     return reinterpret_cast<uint4*>(tile + (KEY_GROUP * (KT * 128) + rb * 1024 + ln * 16));
@@ -245,7 +251,7 @@ __attribute__((amdgpu_waves_per_eu(LatentShape<L, P, NC>::WAVES_PER_EU))) void l
     head = c - qi * a.heads;
     return ok;
   };
-  // Bit k: whether query qi sees the tile's row k (rows of the step only;
+  // Bit k: whether query qi sees row t0 + k, 32 rows (rows of the step only;
   // earlier ones are seen by all, those past the piece by none).
   auto window = [&](const LatentPiece& x, int qi, int t0) -> uint32_t {
     const int j0 = t0 - x.computed;
@@ -261,7 +267,7 @@ __attribute__((amdgpu_waves_per_eu(LatentShape<L, P, NC>::WAVES_PER_EU))) void l
       bits = __builtin_amdgcn_alignbit(hi, lo, j0 & 31);
     }
     const int left = x.tok_end - t0;
-    return left >= 32 ? bits : bits & ((1u << left) - 1u);
+    return left >= 32 ? bits : left <= 0 ? 0u : bits & ((1u << left) - 1u);
   };
 
   LatentPiece cur = read_latent_piece(pieces, blockIdx.x);
@@ -401,13 +407,14 @@ __attribute__((amdgpu_waves_per_eu(LatentShape<L, P, NC>::WAVES_PER_EU))) void l
       fresh = false;
     }
     // ---- scores
-    auto rdv = [&](int n) -> V8 {
-      const int at8 = vaddr(n);
+    auto rdv = [&](int n, int step = 0) -> V8 {
+      const int at8 = vaddr(n) + step * 32 * 128;
       const s16x4 v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_t*)(here + at8));
       const s16x4 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_t*)(here + (at8 + 16 * 128)));
       const s16x4 both[2] = {v0, v1};
       return bitcast<V8>(both);
     };
+    constexpr int STEPS = KT / 32;
     V8 vals[EARLY_V ? DT : 1];
     f32x4 st[QKS];
     bool vote = false, odd = false;
@@ -444,7 +451,7 @@ __attribute__((amdgpu_waves_per_eu(LatentShape<L, P, NC>::WAVES_PER_EU))) void l
         // A row that some column does not see may hold what is not finite (a
         // sibling's draft): zero probabilities do not hide it.  Every score of
         // such a row is not finite either.
-        const uint32_t bits = window(cur, qi0, t0) >> (16 * ks0 + 4 * g);
+        const uint32_t bits = window(cur, qi0, t0 + 16 * (ks0 & ~1)) >> (16 * (ks0 & 1) + 4 * g);
 #pragma unroll
         for (int s = 0; s < QKS; ++s)
 #pragma unroll
@@ -466,7 +473,7 @@ __attribute__((amdgpu_waves_per_eu(LatentShape<L, P, NC>::WAVES_PER_EU))) void l
         for (int r = 0; r < 4; ++r) mt = fmaxf(mt, st[s][r]);
       mt = row_max4(mt);
       vote = mt > m_run + kSlack;
-      if (g == 0) tile_max[ks0][16 * ct0 + l16] = mt;
+      if (g == 0) tile_max[half][16 * ct0 + l16] = mt;
     }
     if (EARLY_V && !scores) {
 #pragma unroll
@@ -486,7 +493,7 @@ __attribute__((amdgpu_waves_per_eu(LatentShape<L, P, NC>::WAVES_PER_EU))) void l
         }
         uint2 both;
         __builtin_memcpy(&both, w, 8);
-        probs[(ct0 * 64 + ln) * 2 + ks0 + s] = both;
+        probs[(((ks0 + s) / 2 * NC + ct0) * 64 + ln) * 2 + (ks0 + s) % 2] = both;
       }
     };
     const bool any_vote = __any(vote), any_odd = __any(odd);
@@ -506,7 +513,7 @@ __attribute__((amdgpu_waves_per_eu(LatentShape<L, P, NC>::WAVES_PER_EU))) void l
       auto moved = [&](int c, float& before) -> float {
         const int i = 16 * c + l16;
         before = col_max[i];
-        return fmaxf(before, QKS == 2 ? tile_max[0][i] : fmaxf(tile_max[0][i], tile_max[1][i]));
+        return fmaxf(before, HALVES == 1 ? tile_max[0][i] : fmaxf(tile_max[0][i], tile_max[1][i]));
       };
       auto ratio = [](float before, float after) { return after == -INFINITY ? 1.f : fast_exp2(before - after); };
 #pragma unroll
@@ -525,7 +532,7 @@ __attribute__((amdgpu_waves_per_eu(LatentShape<L, P, NC>::WAVES_PER_EU))) void l
         weigh();
       }
       lds_barrier();
-      if (scores && g == 0 && ks0 == 0) col_max[16 * ct0 + l16] = m_run;
+      if (scores && g == 0 && half == 0) col_max[16 * ct0 + l16] = m_run;
     }
     if (APPEND && masked && __any(slot >= 0)) {
       if (slot >= 0) {
@@ -533,7 +540,7 @@ __attribute__((amdgpu_waves_per_eu(LatentShape<L, P, NC>::WAVES_PER_EU))) void l
         gptr<T> const to = pool + (int64_t)slot * S::ROW;
 #pragma unroll
         for (int i = 0; i < (GR + GSTEP - 1) / GSTEP; ++i) {
-          const int gr = (wave >> 2) + i * GSTEP, c = 8 * gr + lchunk;
+          const int gr = wave / RB + i * GSTEP, c = 8 * gr + lchunk;
           if (c < S::CPR)
             store16(to + 8 * c, *reinterpret_cast<const uint4*>(here + (gr * (KT * 128) + rb * 1024 + ln * 16)));
         }
@@ -545,7 +552,7 @@ __attribute__((amdgpu_waves_per_eu(LatentShape<L, P, NC>::WAVES_PER_EU))) void l
       // The step's rows without their values that are not finite (and none of
       // the repeated rows past the piece's end).
       const int lrow = 8 * rb + (ln >> 3);
-      if (t0 + lrow >= cur.computed && wave < 4) {
+      if (t0 + lrow >= cur.computed && wave < RB) {
 #pragma unroll 1
         for (int c = 0; c < L / 8; ++c) {
           if ((c & 7) != ((ln & 7) ^ swizzle(lrow))) continue;
@@ -580,13 +587,24 @@ __attribute__((amdgpu_waves_per_eu(LatentShape<L, P, NC>::WAVES_PER_EU))) void l
         }
       };
       if constexpr (EARLY_V) {
-        V8 w[NC];
 #pragma unroll
-        for (int c = 0; c < NC; ++c) w[c] = rdp(c);
+        for (int step = 0; step < STEPS; ++step) {
+          V8 w[NC], more[DT];
 #pragma unroll
-        for (int c = 0; c < NC; ++c)
+          for (int c = 0; c < NC; ++c) w[c] = rdp(step * NC + c);
+          if (step + 1 < STEPS) {
 #pragma unroll
-          for (int n = 0; n < DT; ++n) acc[c][n] = mm(vals[n], w[c], acc[c][n]);
+            for (int n = 0; n < DT; ++n) more[n] = rdv(n, step + 1);
+          }
+#pragma unroll
+          for (int c = 0; c < NC; ++c)
+#pragma unroll
+            for (int n = 0; n < DT; ++n) acc[c][n] = mm(vals[n], w[c], acc[c][n]);
+          if (step + 1 < STEPS) {
+#pragma unroll
+            for (int n = 0; n < DT; ++n) vals[n] = more[n];
+          }
+        }
       } else {
       constexpr bool HOLD_V = NC > DT;
       constexpr int HELD = HOLD_V ? DT : NC, TOT = HOLD_V ? NC : DT, LEAD = TOT < 2 ? TOT : 2;
@@ -624,7 +642,7 @@ __attribute__((amdgpu_waves_per_eu(LatentShape<L, P, NC>::WAVES_PER_EU))) void l
         for (int c = 0; c < NC; ++c) {
           int qi, head;
           columns(ln, cur, c, qi, head);
-          sees |= ((window(cur, qi, t0) >> (pos - t0)) & 1u) << c;
+          sees |= ((window(cur, qi, t0 + ((pos - t0) & ~31)) >> ((pos - t0) & 31)) & 1u) << c;
         }
 #pragma unroll
         for (int n = 0; n < DT; ++n) {
@@ -645,13 +663,13 @@ __attribute__((amdgpu_waves_per_eu(LatentShape<L, P, NC>::WAVES_PER_EU))) void l
     // ---- a finished piece: its output rows, or its partials
     if (scores) {
       const float l = row_sum4(l_run);
-      if (g == 0) col_sum[ks0][16 * ct0 + l16] = l;
+      if (g == 0) col_sum[half][16 * ct0 + l16] = l;
     }
     lds_barrier();
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
       const int i = 16 * c + l16;
-      const float l_tot = QKS == 2 ? col_sum[0][i] : col_sum[0][i] + col_sum[1][i];
+      const float l_tot = HALVES == 1 ? col_sum[0][i] : col_sum[0][i] + col_sum[1][i];
       const float inv = l_tot > 0.f ? 1.f / l_tot : l_tot == l_tot ? 0.f : l_tot;
       int qi, head;
       if (!columns(ln, cur, c, qi, head)) continue;
@@ -774,7 +792,7 @@ static const void* latent_decode_fn(int col_tiles) {
 
 using namespace lvamd;
 
-extern "C" int lvamd_latent_decode_tile_tokens(void) { return KT; }
+extern "C" int lvamd_latent_decode_tile_tokens(int32_t col_tiles) { return tile_rows(col_tiles); }
 
 extern "C" int lvamd_latent_decode_resident_groups(int32_t dtype, int32_t latent_size, int32_t rope_size, int32_t col_tiles) {
   return latent_dispatch(dtype, latent_size, rope_size, [&]<typename T, int L, int P>() -> int {

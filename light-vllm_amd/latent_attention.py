@@ -29,8 +29,8 @@ from light_vllm_amd.quantized_cache import _NOT_FAST, _raw_stream, on_device
 
 # Column tiles (of 16) per workgroup that the latent-space kernel is built for.
 COL_TILES = (1, 2, 4, 8)
-# Rows of a tile, and the tiles per workgroup from which 128 columns pay.
-TILE_ROWS, WIDE_TILES = 32, 32
+# Rows of a 64-column workgroup's tile, and the tiles from which 128 columns pay.
+TILE_ROWS, WIDE_TILES = 64, 24
 # Widest workgroup whose launch appends the step's rows itself.
 APPEND_TILES = 4
 WEIGHT_SIZES = (64, 128)
@@ -118,11 +118,11 @@ def choose_col_tiles(q_lens, totals, heads: int, resident) -> int:
     A wider workgroup reads a row once for more columns; a narrower one holds two
     to a CU and writes fewer partials, and up to 64 columns the launch appends.
     Measured (us, 16/32/64/128 columns): 16 heads, 64 requests x 2300 tokens 43 / 43 /
-    55 / 67; 16 x 32767 tokens 114 / 119 / 146 / 178; 128 heads, 32 x 2300 (18 tiles
-    per workgroup) 99 / 68 / 63 / 63, and with the launches 70 against 74 for the last
-    two; 128 heads, 64 x 2300 (36 tiles) 133 / 106 / 88 for the last three, 8 x 32767
-    (64 tiles) 232 / 164 / 146 / 126; 16 heads, 9 queries, 32 x 8000 (96 tiles) 266 /
-    223 / 192 for the last three."""
+    49 / 67; 16 x 32767 tokens 114 / 119 / 146 / 178; 128 heads, 32 x 2300 (9 tiles
+    per workgroup) 99 / 68 / 63 / 63, 64 x 2300 (18 tiles) 95 / 88 for the last two,
+    128 x 1000 (16 tiles) 80 / 85, 8 x 32767 (32 tiles) 232 / 164 / 129 / 126; 16 heads, 9
+    queries, 32 x 8000 (48 tiles) 200 / 192 for the last two, each time with 5 to 10
+    more for the launches of 128 columns where the host sets the pace."""
 
     widest = -(-int(q_lens.max()) * heads // 16)
     fits = next((t for t in COL_TILES if t >= widest), COL_TILES[-1])
@@ -137,7 +137,7 @@ def _expanded(facts, spec: LatentLayerSpec, nope: int, value: int) -> np.ndarray
     """Which requests take the expanded form: linear ones where its products (with
     the expansion of every key) are fewer than 1.2 times the absorbed form's, which
     run at the lower rate.  Fewer than 64 queries cost as much as 64, keys count in
-    tiles.
+    32s.
 
     Measured (us, absorbed / expanded; one request, 16 heads, 512 + 64, 128 / 128):
     behind 1024 tokens 35 / 33 for 16 queries, 47 / 35 for 64, 74 / 39 for 256;
@@ -148,7 +148,7 @@ def _expanded(facts, spec: LatentLayerSpec, nope: int, value: int) -> np.ndarray
 
     n, c = facts.q_lens.astype(np.float64), facts.computed.astype(np.float64)
     latent, rope = spec.latent_size, spec.rope_size
-    keys, held = c + n / 2, -(-(c + n) // TILE_ROWS) * TILE_ROWS
+    keys, held = c + n / 2, -(-(c + n) // 32) * 32
     absorbed = n * keys * (2 * latent + rope) + n * latent * (nope + value)
     expanded = np.maximum(n, 64) * keys * (nope + rope + value) + held * latent * (nope + value)
     return (facts.vis_off < 0) & (expanded < 1.2 * absorbed)
@@ -236,7 +236,7 @@ class LatentStepPlan(StepPlan):
             x.row_base = int(mine[0, 4])
             x.row_span = int(mine[-1, 4] + mine[-1, 3]) - x.row_base
             found = host.latent_work(mine, facts.flat, heads, x.col_tiles, resident, self.block_size,
-                                     int(native.load().lvamd_latent_decode_tile_tokens()), DECODE_MERGE_PIECES)
+                                     int(native.load().lvamd_latent_decode_tile_tokens(x.col_tiles)), DECODE_MERGE_PIECES)
             pieces, jobs = (np.frombuffer(a, dtype=np.int32) for a in found[:2])
             x.num_groups, x.num_slots, x.merge_columns = (int(v) for v in found[2:5])
             x.num_jobs = jobs.size // native.MERGE_FIELDS

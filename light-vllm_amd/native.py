@@ -158,7 +158,7 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
         [_p, _i64, _i64, _p, _i64, _i64, _p, _i64, _p, _i64, _p, _p, _i64, _i32, _p, _p, _i64, _i64, _p, _i32, _p, _i32,
          _i32, _p, _p, _p, _p, _i64, _i32, _i32, _i32, _i32, _i32, _f32, _i32, _p],
     ),
-    "lvamd_latent_decode_tile_tokens": (ctypes.c_int, []),
+    "lvamd_latent_decode_tile_tokens": (ctypes.c_int, [_i32]),
     "lvamd_latent_decode_resident_groups": (ctypes.c_int, [_i32, _i32, _i32, _i32]),
     "lvamd_latent_heads": (
         ctypes.c_int, [_p, _i64, _i64, _p, _p, _i64, _i64, _p, _i64, _i32, _i32, _i32, _i32, _p]),
