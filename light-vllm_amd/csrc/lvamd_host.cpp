@@ -1629,15 +1629,17 @@ PyObject* decode_work(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
 }
 
 // latent_work(req_meta i32[B*8], flat i32, heads, col_tiles, resident,
-//             block_size, unit, merge_pieces)
+//             block_size, unit, merge_pieces, xcds)
 //   -> (pieces i32 [n, 16], jobs i32 [m, 8], workgroups, partial slots, most
 //       columns of a merge job, pieces of the deepest merge job)
 // The pieces of the attention over latent vectors: one kv head whose group is
 // every head, workgroups of 16 * col_tiles columns in the waves' place.  Piece w is
 // workgroup w's first; field 11 is the index of its next (-1: none), fields 12 to
-// 15 its first four table entries (-1 where a tile may span more blocks).
+// 15 its first four table entries (-1 where a tile may span more blocks).  Where a
+// request has several column groups, the workgroups of the same tokens run on one
+// of the xcds (workgroup w on w % xcds), at once: its L2 serves all but the first.
 PyObject* latent_work(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
-  if (!want_args(nargs, 8, "latent_work")) return nullptr;
+  if (!want_args(nargs, 9, "latent_work")) return nullptr;
   Buf meta(args[0], false, 4, "req_meta"), flat(args[1], false, 4, "flat");
   if (!meta.ok() || !flat.ok()) return nullptr;
   Requests q;
@@ -1646,7 +1648,9 @@ PyObject* latent_work(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   int64_t* fields[] = {&d.group, &d.col_tiles, &d.resident, &d.bs, &d.unit, &d.merge_pieces};
   for (int i = 0; i < 6; ++i)
     if (!as_i64(args[2 + i], fields[i])) return nullptr;
-  if (d.group <= 0 || d.col_tiles <= 0 || d.resident <= 0 || d.bs <= 0 || d.unit <= 0) {
+  int64_t xcds = 0;
+  if (!as_i64(args[8], &xcds)) return nullptr;
+  if (d.group <= 0 || d.col_tiles <= 0 || d.resident <= 0 || d.bs <= 0 || d.unit <= 0 || xcds <= 0) {
     PyErr_SetString(PyExc_ValueError, "latent_work: inconsistent arguments");
     return nullptr;
   }
@@ -1657,9 +1661,24 @@ PyObject* latent_work(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     const int32_t* ids = flat.data<int32_t>();
     build_decode(q, ids, flat.count(), d, out);
     std::vector<int32_t> pieces(out.pieces.size());
+    // place[w]: the workgroup that takes the planner's w-th share.
+    std::vector<int64_t> place((size_t)out.waves);
+    std::iota(place.begin(), place.end(), 0);
+    bool groups = false;
+    for (int64_t r = 0; r < q.batch; ++r) groups = groups || q.q_len(r) * d.group > 16 * d.col_tiles;
+    if (groups) {
+      std::vector<int64_t> order = place;
+      auto first = [&](int64_t w) { return out.pieces.data() + (int64_t)out.first[(size_t)w] * kPieceFields; };
+      std::stable_sort(order.begin(), order.end(), [&](int64_t x, int64_t y) {
+        const int32_t *a = first(x), *b = first(y);  // (by request, then first token)
+        return a[8] != b[8] ? a[8] < b[8] : a[2] < b[2];
+      });
+      for (int64_t x = 0, i = 0; x < xcds; ++x)
+        for (int64_t w = x; w < out.waves; w += xcds) place[(size_t)order[(size_t)i++]] = w;
+    }
     for (int64_t w = 0, rest = out.waves; w < out.waves; ++w) {
       const int64_t p0 = out.first[(size_t)w], p1 = out.first[(size_t)w + 1];
-      for (int64_t p = p0, at = w; p < p1; ++p) {
+      for (int64_t p = p0, at = place[(size_t)w]; p < p1; ++p) {
         int32_t* o = pieces.data() + at * kPieceFields;
         const int32_t* x = out.pieces.data() + p * kPieceFields;
         std::memcpy(o, x, 11 * sizeof(int32_t));

@@ -40,10 +40,12 @@
 // tile's own work: about 2.8 us for 64 rows and 64 columns, of which the matrix units
 // are busy 0.9 and LDS 1.1; the rest is vector instructions (two waves a SIMD) and
 // the round trips between the phases.  32 requests of 128 heads (97 MB, 21 GFLOP)
-// 61 us: 7 to the first tile, 9 to 10 tiles, 3 for the partials.  Eight waves rather than
-// four from 64 columns on: 140 against 145 us for 8 x 32767 x 128 heads.  Tile loads
-// are non-temporal: 50 against 55 us for the 64 requests.  Dealing the loads
-// between the score products measured slower (258 against 232 us).
+// 54 us: 7 to the first tile, 9 to 10 tiles, 3 for the partials.  The groups of one
+// request over the same tokens run on one XCD, whose L2 serves the second: 63 to 51 us
+// for 32 x 2300 tokens.  Eight waves rather than four from 64 columns on: 140 against
+// 145 us for 8 x 32767 x 128 heads.  Up to 32 columns tile loads are non-temporal: 50
+// against 55 us for the 64 requests.  Dealing the loads between the score products
+// measured slower (258 against 232 us).
 //
 // LDS tile layout: groups of 64 columns (128 bytes of every row), group-major;
 // one load of a wave fills 1 KB = 8 whole 128-byte lines of one group.  Chunk c
@@ -197,9 +199,11 @@ __attribute__((amdgpu_waves_per_eu(LatentShape<L, P, NC>::WAVES_PER_EU))) void l
       int c = 8 * gr + lchunk;
       // (A half-used last group's spare slots take the row's last chunk again.)
       if (8 * GR > S::CPR && gr == GR - 1) c = min(c, S::CPR - 1);
-      // Non-temporal: a launch reads a row once, or a few column groups do at once.
+      // Non-temporal where a row is read once (16 and 32 columns are a whole request);
+    // 64 columns are often one of several groups, which read it from one L2 (51 against
+    // 56 us for 32 x 2300 tokens of 128 heads).  128 measured alike either way.
       __builtin_amdgcn_global_load_lds((lds_gptr)((gr < L / 64 ? row : key) + 8 * c),
-                                       (lds_lptr)(dst + (gr * KT * 128 + rb * 1024)), 16, 0, 2);
+                                       (lds_lptr)(dst + (gr * KT * 128 + rb * 1024)), 16, 0, NC == 4 ? 0 : 2);
     }
   };
 

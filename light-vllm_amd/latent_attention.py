@@ -118,11 +118,11 @@ def choose_col_tiles(q_lens, totals, heads: int, resident) -> int:
     A wider workgroup reads a row once for more columns; a narrower one holds two
     to a CU and writes fewer partials, and up to 64 columns the launch appends.
     Measured (us, 16/32/64/128 columns): 16 heads, 64 requests x 2300 tokens 43 / 43 /
-    49 / 67; 16 x 32767 tokens 114 / 119 / 146 / 178; 128 heads, 32 x 2300 (9 tiles
-    per workgroup) 99 / 68 / 63 / 63, 64 x 2300 (18 tiles) 95 / 88 for the last two,
-    128 x 1000 (16 tiles) 80 / 85, 8 x 32767 (32 tiles) 232 / 164 / 129 / 126; 16 heads, 9
-    queries, 32 x 8000 (48 tiles) 200 / 192 for the last two, each time with 5 to 10
-    more for the launches of 128 columns where the host sets the pace."""
+    49 / 67; 16 x 32767 tokens 114 / 119 / 146 / 178; 64 columns against 128: 128 heads,
+    32 x 2300 (9 tiles per workgroup) 51 / 63, 64 x 2300 (18 tiles) 87 / 88, 256 x 1000 (32
+    tiles) 152 / 113, 8 x 32767 (32 tiles) 128 / 119; 16 heads, 9 queries, 32 x 8000 (48
+    tiles) 195 / 192, and some 5 more for the launches of 128 columns where the host
+    sets the pace."""
 
     widest = -(-int(q_lens.max()) * heads // 16)
     fits = next((t for t in COL_TILES if t >= widest), COL_TILES[-1])
@@ -236,7 +236,8 @@ class LatentStepPlan(StepPlan):
             x.row_base = int(mine[0, 4])
             x.row_span = int(mine[-1, 4] + mine[-1, 3]) - x.row_base
             found = host.latent_work(mine, facts.flat, heads, x.col_tiles, resident, self.block_size,
-                                     int(native.load().lvamd_latent_decode_tile_tokens(x.col_tiles)), DECODE_MERGE_PIECES)
+                                     int(native.load().lvamd_latent_decode_tile_tokens(x.col_tiles)), DECODE_MERGE_PIECES,
+                                     native.xcd_count())
             pieces, jobs = (np.frombuffer(a, dtype=np.int32) for a in found[:2])
             x.num_groups, x.num_slots, x.merge_columns = (int(v) for v in found[2:5])
             x.num_jobs = jobs.size // native.MERGE_FIELDS

@@ -160,7 +160,8 @@ def test_pieces_cover_every_column_group_once(seed) -> None:
     md = lv.PagedAttentionMetadata(block_tables=tables, num_computed_tokens=tuple(computed),
                                    query_layouts=tuple(lv.QueryLayout(p) for p in layouts))
     plan = StepPlan(md, block_size=bs, device=CPU, num_blocks=sum(need))
-    found = native.host().latent_work(plan._req_meta, plan.facts.flat, heads, tiles, resident, bs, 32, 256)
+    xcds = int(rng.choice((1, 4, 8)))
+    found = native.host().latent_work(plan._req_meta, plan.facts.flat, heads, tiles, resident, bs, 32, 256, xcds)
     pieces, jobs, groups, slots, most, depth = found
     pieces = np.frombuffer(pieces, np.int32).reshape(-1, native.PIECE_FIELDS)
     jobs = np.frombuffer(jobs, np.int32).reshape(-1, native.MERGE_FIELDS)
@@ -182,6 +183,8 @@ def test_pieces_cover_every_column_group_once(seed) -> None:
         by_segment.setdefault((int(x[0]), int(x[1])), []).append(x)
         off = sum(need[:x[0]])
         assert x[5] == off and x[6] == computed[x[0]] and x[7] == len(layouts[x[0]])
+    for got in by_segment.values():
+        got.sort(key=lambda x: x[2])  # (the workgroups are dealt to the XCDs)
     want = set()
     for r, (c, p) in enumerate(zip(computed, layouts)):
         columns = len(p) * heads
@@ -206,9 +209,27 @@ def test_pieces_cover_every_column_group_once(seed) -> None:
         assert min(columns, 16 * tiles) <= most
 
 
+def test_column_groups_of_the_same_tokens_share_an_xcd() -> None:
+    """Four column groups per request, four shares each: the workgroups over the same
+    tokens of a request differ by whole rounds of the XCDs."""
+    md = lv.PagedAttentionMetadata(block_tables=tuple(tuple(range(64 * r, 64 * r + 64)) for r in range(16)),
+                                   num_computed_tokens=(1023,) * 16, query_layouts=(lv.linear_query_layout(1),) * 16)
+    plan = StepPlan(md, block_size=16, device=CPU, num_blocks=1024)
+    pieces, _, groups, *_ = native.host().latent_work(plan._req_meta, plan.facts.flat, 64, 1, 256, 16, 32, 256, 8)
+    pieces = np.frombuffer(pieces, np.int32).reshape(-1, native.PIECE_FIELDS)
+    assert groups == 256 == len(pieces)
+    where: dict = {}
+    for w, x in enumerate(pieces):
+        where.setdefault((int(x[0]), int(x[2])), []).append((int(x[1]), w % 8))
+    assert len(where) == 64
+    for found in where.values():
+        assert sorted(g for g, _ in found) == [0, 1, 2, 3] and len({xcd for _, xcd in found}) == 1
+
+
 def test_latent_work_refuses_nonsense() -> None:
     meta, flat = np.zeros(8, np.int32), np.zeros(1, np.int32)
-    for args in ((0, 1, 4, 16, 32, 256), (16, 0, 4, 16, 32, 256), (16, 1, 0, 16, 32, 256), (16, 1, 4, 0, 32, 256)):
+    for args in ((0, 1, 4, 16, 32, 256, 8), (16, 0, 4, 16, 32, 256, 8), (16, 1, 0, 16, 32, 256, 8), (16, 1, 4, 0, 32, 256, 8),
+                 (16, 1, 4, 16, 32, 256, 0)):
         with pytest.raises(ValueError, match="inconsistent"):
             native.host().latent_work(meta, flat, *args)
 
