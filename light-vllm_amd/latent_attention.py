@@ -140,11 +140,11 @@ def _expanded(facts, spec: LatentLayerSpec, nope: int, value: int) -> np.ndarray
     32s.
 
     Measured (us, absorbed / expanded; one request, 16 heads, 512 + 64, 128 / 128):
-    behind 1024 tokens 35 / 33 for 16 queries, 47 / 35 for 64, 74 / 39 for 256;
-    behind 8192 53 / 78, 78 / 82, 149 / 99; behind 32768 82 / 256, 149 / 262, 372 / 317,
-    with 512 queries 661 / 383; eight requests behind 8192 105 / 559, 250 / 567, 771 /
-    595.  Over 111 steps of 1 to 128 heads the choice is 2 % off the better form's
-    time, at most 1.5 times (8 requests of 32 queries, no history: 36 / 25)."""
+    behind 1024 tokens 32 / 32 for 16 queries, 45 / 34 for 64, 65 / 38 for 256;
+    behind 8192 44 / 80, 66 / 87, 150 / 108; behind 32768 60 / 259, 144 / 265, 379 / 319,
+    with 512 queries 688 / 389; eight requests behind 8192 95 / 559, 242 / 565, 716 /
+    601.  Over 111 steps of 16 to 128 heads the choice is 1.5 % off the better form's
+    time, at most 1.4 times (32 queries of 128 heads, no history: 37 / 52)."""
 
     n, c = facts.q_lens.astype(np.float64), facts.computed.astype(np.float64)
     latent, rope = spec.latent_size, spec.rope_size
