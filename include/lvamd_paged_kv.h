@@ -745,7 +745,7 @@ int64_t lvamd_latent_move_workspace_size(int64_t num_pairs, int32_t num_layers, 
  * workgroup's next piece (-1: none) and its first four table entries (-1: not
  * given); workgroup w of num_groups begins with piece w.  Split segments go
  * through part_acc (fp32 [num_partial_slots][16 * col_tiles][latent_size]) and
- * part_ml and are merged.
+ * part_ml and are merged.  A query all of whose scores are -inf gets NaN.
  */
 int lvamd_latent_decode(const void* query, int64_t query_token_stride, int64_t query_head_stride,
                         const void* query_rope, int64_t rope_token_stride, int64_t rope_head_stride,

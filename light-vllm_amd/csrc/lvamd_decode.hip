@@ -989,6 +989,7 @@ struct MergeArgs {
   void* out;
   int64_t out_tok_stride, out_head_stride;
   FastDiv by_group, by_cols;  // / group, / columns per partial slot
+  float of_nothing;  // what a row of weights that sum to zero is multiplied with
 };
 
 constexpr int kMergeRoundTrip = 16;  // partials a wave requests at once
@@ -1127,7 +1128,7 @@ __global__ __launch_bounds__(64 * merge_waves(P)) void paged_merge_kernel(
     }
   }
   if (!act) return;
-  const float inv = lsum > 0.f ? 1.f / lsum : 0.f;
+  const float inv = lsum > 0.f ? 1.f / lsum : a.of_nothing;
   TO* orow = static_cast<TO*>(a.out) + (int64_t)(q_start + qi) * a.out_tok_stride + (int64_t)qhead * a.out_head_stride;
 #pragma unroll
   for (int k = 0; k < EPC; ++k) orow[ch * EPC + k] = from_f32<TO>(o[k] * inv);
@@ -1240,7 +1241,7 @@ static int merge_sharing(int64_t num_jobs, int64_t num_partials, int64_t merge_d
 int launch_merge(const void* part_acc, const float* part_ml, void* out, int64_t out_token_stride,
                  int64_t out_head_stride, const int32_t* jobs, int32_t num_jobs, int64_t num_partials,
                  int64_t merge_depth, int32_t num_kv_heads, int32_t group, int32_t head_size, int32_t col_tiles, int32_t max_columns,
-                 int32_t dtype, hipStream_t s, bool fp32_partials) {
+                 int32_t dtype, hipStream_t s, bool fp32_partials, float of_nothing) {
   if (dtype_size(dtype) == 0 || !head_size_supported(head_size) || col_tiles < 1 || col_tiles > 16)
     return LVAMD_ERR_UNSUPPORTED;
   if (max_columns < 1 || max_columns > 16 * col_tiles) return LVAMD_ERR_INVALID_ARGUMENT;
@@ -1253,6 +1254,7 @@ int launch_merge(const void* part_acc, const float* part_ml, void* out, int64_t 
   a.out = out;
   a.out_tok_stride = out_token_stride;
   a.out_head_stride = out_head_stride;
+  a.of_nothing = of_nothing;
   const int64_t job_heads = (int64_t)num_jobs * num_kv_heads;
   if (fp32_partials && dtype_size(dtype) == 2) {
     return dispatch_decode(dtype, head_size, 1, [&]<typename T, int D, int CTW>() -> int {

@@ -674,7 +674,9 @@ __attribute__((amdgpu_waves_per_eu(LatentShape<L, P, NC>::WAVES_PER_EU))) void l
     for (int c = 0; c < NC; ++c) {
       const int i = 16 * c + l16;
       const float l_tot = HALVES == 1 ? col_sum[0][i] : col_sum[0][i] + col_sum[1][i];
-      const float inv = l_tot > 0.f ? 1.f / l_tot : l_tot == l_tot ? 0.f : l_tot;
+      // (A piece may hold no row that a column sees, and weighs nothing then; a whole
+      // request's softmax without a finite score is NaN.)
+      const float inv = l_tot > 0.f ? 1.f / l_tot : cur.slot < 0 ? NAN : l_tot == l_tot ? 0.f : l_tot;
       int qi, head;
       if (!columns(ln, cur, c, qi, head)) continue;
       if (cur.slot < 0) {
@@ -777,7 +779,7 @@ __global__ __launch_bounds__(L / 4 * MERGE_SHARES) void latent_merge_kernel(cons
   }
   const int qi = fast_div(col, a.by_heads), head = col - qi * a.heads;
   T* to = static_cast<T*>(a.out) + (int64_t)(q_start + qi) * a.out_tok_stride + (int64_t)head * a.out_head_stride;
-  const float inv = total > 0.f ? 1.f / total : total == total ? 0.f : total;
+  const float inv = total > 0.f ? 1.f / total : NAN;  // (no finite score in any piece)
   store_partial4<false, T>(to + 4 * at, sum, inv);
 }
 

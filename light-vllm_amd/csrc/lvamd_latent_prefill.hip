@@ -317,7 +317,9 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void l
   for (int ct = 0; ct < CT; ++ct) {
     if (!ok[ct]) continue;
     const float l_tot = l_run[ct][0];
-    const float inv = l_tot > 0.f ? 1.f / l_tot : l_tot == l_tot ? 0.f : l_tot;
+    // (A unit over a key range may hold no key that a query sees, and weighs nothing
+    // then; a whole softmax without a finite score is NaN.)
+    const float inv = l_tot > 0.f ? 1.f / l_tot : slot < 0 ? NAN : l_tot == l_tot ? 0.f : l_tot;
     if (slot >= 0) {
       const int64_t cs = ((int64_t)slot * a.heads + h) * kUnitColumns + 16 * (CT * wave + ct) + l16;
 #pragma unroll
@@ -411,5 +413,5 @@ extern "C" int lvamd_latent_prefill(const void* query, int64_t query_token_strid
   });
   if (status != LVAMD_OK || num_units == 0 || num_jobs == 0) return status;
   return launch_merge(part_acc, part_ml, out, out_token_stride, out_head_stride, jobs, num_jobs, num_partial_slots, 0,
-                      num_heads, 1, value_size, kUnitColumns / 16, merge_columns, dtype, s, true);
+                      num_heads, 1, value_size, kUnitColumns / 16, merge_columns, dtype, s, true, NAN);
 }
