@@ -778,7 +778,7 @@ int lvamd_latent_heads(const void* x, int64_t x_token_stride, int64_t x_head_str
  * request's are its last again.  keys [heads][64 num_blocks][nope_size] = key_up
  * [heads][nope_size][latent_size] times the latents, values likewise, rope_keys
  * [64 num_blocks][rope_size] the rotated keys.  nope_size, value_size: 64 or 128.
- * Values beyond fp16's largest are held at it.
+ * A row whose key or value of a head is not a number of dtype has a key of NaN there.
  */
 int lvamd_latent_expand(const void* pool, const int32_t* blocks, int32_t num_blocks, const int32_t* tables,
                         const void* key_up, const void* value_up, void* keys, void* values, void* rope_keys,

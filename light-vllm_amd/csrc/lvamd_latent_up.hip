@@ -18,6 +18,7 @@ namespace {
 
 typedef const __attribute__((address_space(1))) void* lds_gptr;
 typedef __attribute__((address_space(3))) void* lds_lptr;
+typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
 
 struct HeadsArgs {
   const void* x;
@@ -122,14 +123,15 @@ struct ExpandArgs {
   FastDiv by_block, by_heads;
 };
 
-// The largest value of T holds what is beyond it (a masked row's infinity would
-// not stay where it is); NaN for sums that are not finite.
+// The larger of each half's magnitude, as bits: what is not a number of T is at
+// least its infinity's.
+__device__ __forceinline__ uint32_t larger_bits(uint32_t most, uint32_t x) {
+  return bitcast<uint32_t>(__builtin_elementwise_max(bitcast<u16x2>(most), bitcast<u16x2>(x & 0x7fff7fffu)));
+}
 template <typename T>
-__device__ __forceinline__ float held(float x) {
-  if constexpr (std::is_same<T, _Float16>::value) {
-    return __builtin_fabsf(x) < INFINITY ? __builtin_amdgcn_fmed3f(x, -65504.f, 65504.f) : __uint_as_float(0x7fc00000u);
-  }
-  return x;
+__device__ __forceinline__ bool all_numbers(uint32_t most) {
+  constexpr uint32_t infinity = std::is_same<T, __bf16>::value ? 0x7f80u : 0x7c00u;
+  return max(most & 0xffffu, most >> 16) < infinity;
 }
 
 }  // namespace
@@ -144,6 +146,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void l
   __shared__ __attribute__((aligned(1024))) char b0[B_BYTES];
   __shared__ __attribute__((aligned(1024))) char b1[B_BYTES];
   __shared__ __attribute__((aligned(1024))) char b2[B_BYTES];
+  __shared__ uint32_t lost[kTileRows];
   const int tid = threadIdx.x & 255;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
   const int l16 = lane & 15, g = lane >> 4;
@@ -189,6 +192,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void l
   };
   const bool values = wave & 1;
   const int r0 = 64 * (wave >> 1);
+  if (tid < kTileRows) lost[tid] = 0;  // (the steps' barriers come before its first use)
   // (Its own loop for each width: the barriers are the same.)
   auto run = [&]<int WIDTH>(int n0, void* out) __attribute__((always_inline)) {
     constexpr int RT = 4, NT = WIDTH / 16;
@@ -228,19 +232,36 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void l
       __builtin_amdgcn_sched_barrier(0);  // (or the loads would be put off to the step's end)
       compute(as[i % 3], bs[i % 3]);
     }
+    auto place = [&](int r) -> gptr<T> {
+      const int64_t key = (int64_t)tile * kTileRows + r0 + 16 * r + l16;
+      return (gptr<T>)(out) + ((int64_t)h * a.keys + key) * WIDTH + 8 * g;
+    };
 #pragma unroll
     for (int r = 0; r < RT; ++r) {
-      const int64_t key = (int64_t)tile * kTileRows + r0 + 16 * r + l16;
-      gptr<T> const to = (gptr<T>)(out) + ((int64_t)h * a.keys + key) * WIDTH + 8 * g;
+      uint32_t most = 0;
 #pragma unroll
       for (int n = 0; n < NT; n += 2) {
         T v[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = from_f32<T>(held<T>(acc[n + e / 4][r][e % 4]));
-        uint4 both;
-        __builtin_memcpy(&both, v, 16);
-        store16(to + 16 * n, both);
+        for (int e = 0; e < 8; ++e) v[e] = from_f32<T>(acc[n + e / 4][r][e % 4]);
+        uint4 x;
+        __builtin_memcpy(&x, v, 16);
+        store16(place(r) + 16 * n, x);
+        most = larger_bits(larger_bits(larger_bits(larger_bits(most, x.x), x.y), x.z), x.w);
       }
+      if (!all_numbers<T>(most)) lost[r0 + 16 * r + l16] = 1;
+    }
+    // A row whose key or value T does not hold gets a key of NaN (by the threads that
+    // wrote it): every score of it shows that it is not finite, so it reaches all queries
+    // that see it and, its values taken out, no others (a zero weight would not hide an
+    // infinite value).
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    if (values) return;
+#pragma unroll 1
+    for (int r = 0; r < RT; ++r) {
+      if (!lost[r0 + 16 * r + l16]) continue;
+#pragma unroll
+      for (int n = 0; n < NT; n += 2) store16(place(r) + 16 * n, make_uint4(~0u, ~0u, ~0u, ~0u));
     }
   };
   __builtin_amdgcn_s_waitcnt(0x0F70);  // (the copies of the rotated keys: a step counts its own loads)

@@ -88,3 +88,55 @@ def test_scores_that_are_all_minus_infinity_with_weights(dtype, expanded, split,
     nan = np.isnan(want).all(axis=2)
     assert sorted(gone) == sorted(map(tuple, np.argwhere(nan).tolist())) and not np.isnan(want[~nan]).any()
     layer._check(out, want, bound, "scores of -inf")
+
+
+# ---- a chunk's keys or values past the type's largest ----------------------------------
+
+@pytest.mark.parametrize("dtype, large", [("fp16", 60000.0), ("bf16", 3e38)])
+@pytest.mark.parametrize("of", ("keys", "values"))
+def test_a_chunks_keys_and_values_past_the_largest(of, dtype, large, monkeypatch) -> None:
+    """A token whose key or value of one head is not representable: the queries that
+    see it get NaN from that head, in every value; other queries and heads do not know
+    of it."""
+    latent_space._say(f"latent layer, {of} past {dtype}'s largest")
+    layer._force(monkeypatch, lambda n, linear: n >= 200)
+    t = DTYPES[dtype]
+    cache, md, q, latent, rope_key, _, up = layer._step(4, 128, 32, 64, 64, 16, t, [20, 3], [300, 2], seed=6)
+    # Head 1's key (value) of token 250 is the sum of magnitudes in one place; elsewhere
+    # and for the other heads the weights are so small that nothing comes near.
+    up = [w * 2.0**-12 for w in up]
+    which = 0 if of == "keys" else 1
+    up[which][1, 3] = torch.sign(up[which][1, 3]) * 0.5
+    latent[250] = large * torch.sign(up[which][1, 3].float()).to(t)
+    largest = torch.finfo(t).max
+    per_head = [np.abs(latent_space._np(latent[250]) @ latent_space._np(w).transpose(0, 2, 1)).max(axis=1) for w in up]
+    assert per_head[which][1] > 2 * largest
+    others = [x for i, p in enumerate(per_head) for h, x in enumerate(p) if (i, h) != (which, 1)]
+    assert max(others) < largest / 2
+    out = lv.HipPagedAttentionBackend().create(cache, md).forward("layer0", q, latent, rope_key, scale=1e-3,
+                                                                  weights=lv.LatentWeights(*up))
+    got = latent_space._np(out)
+    assert np.isnan(got[250:300, 1]).all()
+    clean = [*range(250), 300, 301]
+    assert np.isfinite(got[clean]).all()
+    want, bound = layer._expected(cache, md, q, None, up, 1e-3)
+    assert (np.abs(got - want)[clean] <= bound[clean]).all()
+    if dtype == "fp16":  # (bf16's scores of that token pass fp32's largest for every head)
+        rest = [0, 2, 3]
+        assert (np.abs(got - want)[:, rest] <= bound[:, rest]).all()
+
+
+@pytest.mark.parametrize("dtype", ("bf16", "fp16"))
+@pytest.mark.parametrize("value", (math.nan, math.inf, -math.inf))
+def test_a_chunks_row_that_is_not_finite_reaches_every_query_that_sees_it(value, dtype, monkeypatch) -> None:
+    latent_space._say(f"latent layer, {value} in a row of a chunk, {dtype}")
+    layer._force(monkeypatch, lambda n, linear: n >= 200)
+    cache, md, q, latent, rope_key, _, up = layer._step(4, 256, 64, 128, 128, 16, DTYPES[dtype], [20, 500], [400, 5], seed=5)
+    latent[300, 7] = value
+    out = lv.HipPagedAttentionBackend().create(cache, md).forward("layer0", q, latent, rope_key, scale=0.07,
+                                                                  weights=lv.LatentWeights(*up))
+    got = latent_space._np(out)
+    clean = [*range(300), *range(400, 405)]
+    want, bound = layer._expected(cache, md, q, None, up, 0.07)
+    assert np.isnan(got[300:400]).all() and np.isfinite(got[clean]).all()
+    assert (np.abs(got - want)[clean] <= bound[clean]).all()
