@@ -43,6 +43,14 @@ int latent_dispatch(int dtype, int latent, int rope, F f) {
   }
 }
 
+// Softmax weights are rounded to T as 2^kWeightLift times themselves (their sum counts
+// them so too).  fp16 has a fixed step of 2^-24 below 2^-14: unlifted, a weight less than
+// 2^-25 of the largest would count as nothing, and thousands of such keys with it;
+// lifted that is 2^-32.  The largest weight stays below fp16's largest: 2^7 times the
+// 2^8 by which a running maximum may lag.
+template <typename T>
+inline constexpr float kWeightLift = std::is_same<T, _Float16>::value ? 7.f : 0.f;
+
 // A pair turned by an angle of cosine c and sine s.  (Written as these products,
 // so that every kernel rounds alike.)
 __device__ __forceinline__ void turn_pair(float x, float y, float c, float s, float& a, float& b) {

@@ -486,7 +486,7 @@ __attribute__((amdgpu_waves_per_eu(LatentShape<L, P, NC>::WAVES_PER_EU))) void l
     // The weights are rounded to T for the products (a matrix instruction's
     // operands are of one type); the sum that divides them counts them as rounded.
     auto weigh = [&]() {
-      const float base = m_run == -INFINITY ? 0.f : -m_run;
+      const float base = m_run == -INFINITY ? 0.f : kWeightLift<T> - m_run;
 #pragma unroll
       for (int s = 0; s < QKS; ++s) {
         T w[4];

@@ -237,7 +237,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void l
         for (int n = 0; n < NT; ++n) acc[ct][n] *= alpha;
         m_run[ct] = m_new;
       }
-      const float nbase = (m_run[ct] == -INFINITY) ? 0.f : -m_run[ct];
+      const float nbase = (m_run[ct] == -INFINITY) ? 0.f : kWeightLift<T> - m_run[ct];
 #pragma unroll
       for (int s = 0; s < KS; ++s)
 #pragma unroll

@@ -11,7 +11,7 @@ import torch
 import light_vllm_amd as lv
 import test_gpu_latent as latent_space
 import test_gpu_latent_layer as layer
-from light_vllm_amd import latent_attention
+from light_vllm_amd import latent_attention, native
 
 pytestmark = pytest.mark.gpu
 
@@ -140,3 +140,96 @@ def test_a_chunks_row_that_is_not_finite_reaches_every_query_that_sees_it(value,
     want, bound = layer._expected(cache, md, q, None, up, 0.07)
     assert np.isnan(got[300:400]).all() and np.isfinite(got[clean]).all()
     assert (np.abs(got - want)[clean] <= bound[clean]).all()
+
+
+# ---- fp16 weights far below the largest ------------------------------------------------
+
+def _tail(t, heads, rows, rope, tokens, scale):
+    """Rows whose first score stands 2^26.4 above all others', which together weigh
+    about rows * 2^-26.4: (latents, queries' value at latent 0, what comes out)."""
+    latents = torch.zeros((rows, 128), device=DEV)
+    latents[0, 0] = 40.0
+    latents[1:, 1] = 1.0
+    q0 = torch.tensor(26.4 * math.log(2) / (40.0 * scale)).to(t)
+    w = math.exp(-float(q0) * 40.0 * scale)
+    seen = rows - tokens + np.arange(tokens)  # of the others, by query
+    return latents.to(t), float(q0), seen * w / (1 + seen * w)
+
+
+@pytest.mark.parametrize("weighted", (None, "absorbed", "expanded"))
+def test_many_small_fp16_weights(weighted, monkeypatch) -> None:
+    """Thousands of keys, each weighing less than half of fp16's smallest step beside
+    the largest weight, count.
+
+    The weights are rounded as 2^7 and more times themselves (relative to the largest),
+    so each is off by at most 2^-24 / 2 / 2^7 = 2^-32 or its half step: rows * 2^-32 +
+    u |out|; the result, the attended latent and the value are rounded: 3 u |out|; the
+    score is off by the fp32 sums' 128 * 2^-24 of 26.4 ln 2 (the numbers are chosen so
+    that no product is rounded but the query's, which the formula takes as it is):
+    1.5e-4 |out|."""
+    latent_space._say(f"latent attention, many small fp16 weights, {weighted}")
+    t, rows, tokens, scale = torch.float16, 8192, 200 if weighted == "expanded" else 2, 0.25
+    # One workgroup for a request's whole length: pieces have maxima of their own.
+    monkeypatch.setattr(native, "latent_decode_resident_groups", lambda *a: 1)
+    monkeypatch.setattr(native, "latent_prefill_resident_units", lambda *a: 1)
+    layer._force(monkeypatch, lambda n, linear: (n > 0) & (weighted == "expanded"))
+    latents, q0, want = _tail(t, 2, rows, 32, tokens, scale)
+    spec = lv.LatentKVCacheSpec((lv.LatentLayerSpec("layer0", 2, 128, 32),))
+    cache = lv.LatentPagedKVCache(spec, lv.PagedKVCacheConfig(num_blocks=rows // 16, block_size=16, dtype=t, device=DEV))
+    flat = cache.layer("layer0").rows.view(rows, 160)
+    flat[: rows - tokens, :128] = latents[: rows - tokens]
+    md = lv.PagedAttentionMetadata(block_tables=(tuple(range(rows // 16)),), num_computed_tokens=(rows - tokens,),
+                                   query_layouts=(lv.linear_query_layout(tokens),))
+    size = 128 if weighted is None else 64
+    q = torch.zeros((tokens, 2, size + 32), dtype=t, device=DEV)
+    q[..., 0] = q0
+    weights = None
+    if weighted:
+        key_up, value_up = torch.zeros((2, 2, 64, 128), dtype=t, device=DEV)
+        key_up[:, 0, 0] = 1
+        value_up[:, 1, 1] = 1
+        weights = lv.LatentWeights(key_up, value_up)
+    context = lv.HipPagedAttentionBackend().create(cache, md)
+    out = context.forward("layer0", q, latents[rows - tokens:], torch.zeros((tokens, 32), dtype=t, device=DEV), scale=scale,
+                          weights=weights)
+    assert not any(x.num_jobs or x.num_unit_jobs for x in context.plan.launches.values())
+    got = latent_space._np(out)[..., 1]
+    u = 2.0**-11
+    assert (np.abs(got - want[:, None]) <= (rows * 2.0**-32 + (4 * u + 1.5e-4) * want)[:, None]).all()
+
+
+@pytest.mark.parametrize("weighted", (None, "expanded"))
+@pytest.mark.parametrize("lag", (7.9, 8.1, 40.0))
+def test_fp16_weights_of_a_maximum_that_rises_late(lag, weighted, monkeypatch) -> None:
+    """Scores that stand 2^lag above all earlier ones, below and above the 2^8 by which
+    the running maximum may lag: no weight passes fp16's largest.
+
+    Weights, result, attended latent and value are rounded: 5 u; a score is off by fp32
+    sums of 128 * 2^-24 of lag: 2.2e-4."""
+    latent_space._say(f"latent attention, fp16 weights of a maximum that rises by 2^{lag}, {weighted}")
+    t, rows, tokens, scale = torch.float16, 1024, 200 if weighted else 2, 0.25
+    monkeypatch.setattr(native, "latent_decode_resident_groups", lambda *a: 1)
+    monkeypatch.setattr(native, "latent_prefill_resident_units", lambda *a: 1)
+    layer._force(monkeypatch, lambda n, linear: n > 0)
+    first = 512
+    latents = torch.zeros((rows, 128), device=DEV)
+    latents[first:, 0], latents[:first, 1], latents[first:, 2] = 40.0, 1.0, 1.0
+    latents = latents.to(t)
+    q0 = torch.tensor(lag * math.log(2) / (40.0 * scale)).to(t)
+    spec = lv.LatentKVCacheSpec((lv.LatentLayerSpec("layer0", 2, 128, 32),))
+    cache = lv.LatentPagedKVCache(spec, lv.PagedKVCacheConfig(num_blocks=rows // 16, block_size=16, dtype=t, device=DEV))
+    cache.layer("layer0").rows.view(rows, 160)[: rows - tokens, :128] = latents[: rows - tokens]
+    md = lv.PagedAttentionMetadata(block_tables=(tuple(range(rows // 16)),), num_computed_tokens=(rows - tokens,),
+                                   query_layouts=(lv.linear_query_layout(tokens),))
+    q = torch.zeros((tokens, 2, (64 if weighted else 128) + 32), dtype=t, device=DEV)
+    q[..., 0] = q0
+    key_up, value_up = torch.zeros((2, 2, 64, 128), dtype=t, device=DEV)
+    key_up[:, 0, 0] = value_up[:, 1, 1] = value_up[:, 2, 2] = 1
+    out = lv.HipPagedAttentionBackend().create(cache, md).forward(
+        "layer0", q, latents[rows - tokens:], torch.zeros((tokens, 32), dtype=t, device=DEV), scale=scale,
+        weights=lv.LatentWeights(key_up, value_up) if weighted else None)
+    got, n = latent_space._np(out), rows - tokens + 1 + np.arange(tokens) - first
+    w = math.exp(float(q0) * 40.0 * scale)
+    for place, want in ((1, first / (first + n * w)), (2, n * w / (first + n * w))):
+        off = np.abs(got[..., place] - want[:, None])
+        assert (off <= ((5 * 2.0**-11 + 2.2e-4) * want + 2.0**-25)[:, None]).all()
