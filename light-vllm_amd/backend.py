@@ -656,10 +656,12 @@ class HipPagedAttentionBackend:
         self._head_sizes_ok: "weakref.WeakSet[object]" = weakref.WeakSet()
         self._statics: "weakref.WeakKeyDictionary[object, dict]" = weakref.WeakKeyDictionary()
         self._shape_counts: "weakref.WeakKeyDictionary[object, dict]" = weakref.WeakKeyDictionary()
-        self._latent_forms: "weakref.WeakKeyDictionary[object, tuple | None]" = weakref.WeakKeyDictionary()
+        # The forms that a latent cache's steps have taken: (heads, latent_size,
+        # rope_size, dtype code, the weights' sizes or None) -> a layer's spec.
+        self._latent_forms: "weakref.WeakKeyDictionary[object, dict]" = weakref.WeakKeyDictionary()
         # (geometry, metadata key, plan, weak reference to the cache) of the
-        # most recent create().
-        self._last: tuple[object, object, StepPlan, weakref.ref] | None = None
+        # most recent create(), and a latent cache's forms.
+        self._last: tuple | None = None
         # What every context's fast forward calls, looked up once.
         self._lib = native.load()
         self._attend_tensors = native.host().attend_tensors
@@ -797,33 +799,36 @@ class HipPagedAttentionBackend:
                 if spec.head_size in SUPPORTED_HEAD_SIZES)
         return found
 
-    def note_latent_form(self, cache, sizes: tuple[int, int] | None) -> None:
-        """Which form a latent cache's steps take (the weights' sizes, or None)."""
-
-        self._latent_forms[cache] = sizes
-
     def _create_latent(self, cache, key, metadata) -> HipLatentPagedAttention:
         """``create`` over a ``LatentPagedKVCache``."""
 
-        config = cache.config
-        geometry = (config.num_blocks, config.block_size, config.device, config.dtype, HipLatentPagedAttention)
-        last = self._last
-        if last is None or last[1] is not key or last[0] != geometry:
+        config, last = cache.config, self._last
+        if last is not None and last[1] is key and last[3]() is cache:
+            geometry, _, plan, _, forms = last
+        else:
+            geometry = (config.num_blocks, config.block_size, config.device, config.dtype, HipLatentPagedAttention)
+            plan = last[2] if last is not None and last[1] is key and last[0] == geometry else None
+            forms = self._latent_forms.get(cache)
+            if forms is None:
+                forms = self._latent_forms[cache] = {}
+        if plan is not None and not forms.keys() <= plan.launches.keys() and not torch.cuda.is_current_stream_capturing():
+            plan = None  # (made for another cache's layers)
+        if plan is None:
             staging = self._staging.get(config.device)
             if staging is None:
                 staging = self._staging[config.device] = Staging(config.device)
             with on_device(config.device):
                 plan = LatentStepPlan(metadata, block_size=config.block_size, device=config.device,
                                       num_blocks=config.num_blocks, staging=staging, defer_upload=True)
-                # (The lists of the form that the cache's steps took last; another is
+                # (The lists of every form that the cache's steps have taken; another is
                 # planned where it first runs.)
-                for spec in cache.model_spec.layers:
-                    plan.shape(spec, dtype_code(config.dtype), self._latent_forms.get(cache))
+                code = dtype_code(config.dtype)
+                for spec, sizes in [(spec, form[4]) for form, spec in forms.items()] or [
+                        (spec, None) for spec in cache.model_spec.layers]:
+                    plan.shape(spec, code, sizes)
                 plan.commit()
-        else:
-            plan = last[2]
-        self._last = (geometry, key, plan, weakref.ref(cache))
-        return HipLatentPagedAttention(self, cache, plan)
+        self._last = (geometry, key, plan, weakref.ref(cache), forms)
+        return HipLatentPagedAttention(cache, plan, forms)
 
     def create(self, cache, metadata) -> "HipPagedAttention | HipLatentPagedAttention":
         # This package's metadata is recognised by its facts object, which the

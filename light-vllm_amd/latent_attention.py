@@ -276,11 +276,13 @@ class HipLatentPagedAttention:
     # forward takes rotary=(cosines, sines): the append turns keys and queries.
     supports_rotary = True
 
-    def __init__(self, backend, cache, plan: LatentStepPlan) -> None:
-        self._backend = backend
+    def __init__(self, cache, plan: LatentStepPlan, forms: dict) -> None:
+        """``forms``: of the backend, what the cache's steps have taken."""
+
         self._cache = cache
         self._plan = plan
         self._layer_ids: set[str] = set()
+        self._forms = forms
         self._attend = native.host().latent_attend
 
     @property
@@ -319,7 +321,8 @@ class HipLatentPagedAttention:
         # raises the first broken rule's message.
         sizes = None if weights is None else weights.sizes
         code = dtype_code(cfg.dtype)
-        shape = plan.launches.get((spec.num_query_heads, spec.latent_size, spec.rope_size, code, sizes))
+        form = (spec.num_query_heads, spec.latent_size, spec.rope_size, code, sizes)
+        shape = plan.launches.get(form)
         if (shape is not None and shape.num_units == 0 and shape.col_tiles <= APPEND_TILES
                 and (weights is None or weights.fits == (spec.num_query_heads, spec.latent_size, cfg.dtype, cfg.device))
                 and (rotary is None or (type(rotary) is tuple and len(rotary) == 2 and rotary[0] is not None))):
@@ -338,6 +341,8 @@ class HipLatentPagedAttention:
                                       out.data_ptr(), 0 if scratch is None else scratch.data_ptr(),
                                       None if weights is None else weights.addresses)
                 if status == 0:
+                    if form not in self._forms:
+                        self._forms[form] = spec
                     return out
                 if status != _NOT_FAST:
                     native.check(status, "lvamd_latent_decode")
@@ -376,7 +381,7 @@ class HipLatentPagedAttention:
             code, stream = dtype_code(cfg.dtype), current_stream(cfg.device)
             shape = plan.shape(spec, code, sizes)
             plan.use_on(stream)
-            self._backend.note_latent_form(cache, sizes)
+            self._forms[(heads, spec.latent_size, rope, code, sizes)] = spec
             width = spec.latent_size if weights is None else weights.value_size
             out = torch.empty((query.shape[0], heads, width), dtype=cfg.dtype, device=cfg.device)
             rows = cache.layer(layer_id).rows
