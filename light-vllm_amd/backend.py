@@ -827,6 +827,8 @@ class HipPagedAttentionBackend:
                         (spec, None) for spec in cache.model_spec.layers]:
                     plan.shape(spec, code, sizes)
                 plan.commit()
+        else:
+            plan.reuse()
         self._last = (geometry, key, plan, weakref.ref(cache), forms)
         return HipLatentPagedAttention(cache, plan, forms)
 

@@ -157,12 +157,29 @@ def _expanded(facts, spec: LatentLayerSpec, nope: int, value: int) -> np.ndarray
 class LatentStepPlan(StepPlan):
     """A step plan with the latent kernels' work lists per layer shape.
 
-    It may be used on streams that run after the one it was made on, and dropped
-    while their work is pending."""
+    It may be used on streams that run after the one it was made on (``reuse`` sees to
+    that where a later step takes it), and dropped while their work is pending."""
 
     def __init__(self, *args, **kwargs) -> None:
         super().__init__(*args, **kwargs)
         self._stream = current_stream(self._staging.device)  # the allocator's, for the lists
+        self._behind = {self._stream}  # streams that run after the lists' upload
+        index = self._staging.device.index
+        self._index = torch.cuda.current_device() if index is None else index
+
+    def _made_on(self):
+        device = self._staging.device
+        return torch.cuda.ExternalStream(self._stream, device=device) if self._stream else torch.cuda.default_stream(device)
+
+    def reuse(self) -> None:
+        """Before another context of this plan: the current stream waits for the upload
+        if that is another's.  (A stream that is captured can wait for nothing outside
+        its graph: the capture began after the upload.)"""
+
+        stream = _raw_stream(self._index)
+        if stream not in self._behind and not torch.cuda.is_current_stream_capturing():
+            torch.cuda.current_stream(self._staging.device).wait_stream(self._made_on())
+            self._behind.add(stream)
 
     def use_on(self, stream: int) -> None:
         """Before a launch on ``stream``, the current one: the lists are that
@@ -187,12 +204,9 @@ class LatentStepPlan(StepPlan):
             self._register(key, found.lists)
             if late:
                 # (The next launch may be on another stream than this one.)
-                device = self._staging.device
-                torch.cuda.current_stream(device).synchronize()
-                made_on = torch.cuda.ExternalStream(self._stream, device=device) if self._stream else (
-                    torch.cuda.default_stream(device))
+                torch.cuda.current_stream(self._staging.device).synchronize()
                 for blob in self._late_blobs:
-                    blob.record_stream(made_on)
+                    blob.record_stream(self._made_on())
             self.launches[key] = found
         return found
 

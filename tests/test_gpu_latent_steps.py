@@ -98,3 +98,26 @@ def test_a_plan_of_another_caches_layers_is_not_taken() -> None:
     again = run(backend.create(cache, md))
     torch.cuda.synchronize()
     assert torch.equal(out, want_other) and all(torch.equal(a, b) for a, b in zip(again, want))
+
+
+@pytest.mark.parametrize("known", (False, True))
+def test_a_plan_whose_upload_is_pending_on_another_stream(known) -> None:
+    """Two streams create contexts for the same metadata: the second waits for the lists
+    that the first uploads."""
+    latent_space._say(f"latent layers, lists pending on another stream, form known: {known}")
+    cache, metadata, run = _two_forms("none")
+    want = run(lv.HipPagedAttentionBackend().create(cache, metadata()))
+    backend, md = lv.HipPagedAttentionBackend(), metadata()
+    if known:
+        run(backend.create(cache, metadata()))
+    first, second = torch.cuda.Stream(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(first):
+        torch.cuda._sleep(50_000_000)
+        kept = backend.create(cache, md)
+    with torch.cuda.stream(second):
+        context = backend.create(cache, md)
+        got = run(context)
+    assert context.plan is kept.plan
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
