@@ -734,9 +734,10 @@ int64_t lvamd_latent_move_few_pairs(void);
 int64_t lvamd_latent_move_workspace_size(int64_t num_pairs, int32_t num_layers, int64_t row_bytes);
 
 /*
- * Attention in latent space: query [tokens][heads][latent_size] (multiplied by
+ * Attention in latent space: query [rows][heads][latent_size] (multiplied by
  * the heads' key weights), query_rope [tokens][heads][rope_size], out
- * [tokens][heads][latent_size] (to be multiplied by the heads' value weights).
+ * [rows][heads][latent_size] (to be multiplied by the heads' value weights); field 0
+ * of pieces and jobs is the request's first row of query and out.
  * With latent and rope_key (else NULL: the pool holds them; NULL with col_tiles
  * 8) the launch appends the step's rows; with cosines and sines (as
  * lvamd_latent_append's) it turns query_rope and those keys first.
@@ -763,13 +764,13 @@ int lvamd_latent_decode_tile_tokens(int32_t col_tiles);
 int lvamd_latent_decode_resident_groups(int32_t dtype, int32_t latent_size, int32_t rope_size, int32_t col_tiles);
 
 /*
- * y[t][h] = weights[h] x[t][h] for the tokens rows[0..num_rows) (NULL: tokens 0
- * .. num_rows): weights [heads][n][k], contiguous, k and n multiples of 64.  key_up^T
+ * y[y_rows[i]][h] = weights[h] x[x_rows[i]][h] for i in [0, num_rows) (NULL: row i):
+ * weights [heads][n][k], contiguous, k and n multiples of 64.  key_up^T
  * takes queries into latent space, value_up results out of it.
  */
 int lvamd_latent_heads(const void* x, int64_t x_token_stride, int64_t x_head_stride, const void* weights, void* y,
-                       int64_t y_token_stride, int64_t y_head_stride, const int32_t* rows, int64_t num_rows,
-                       int32_t num_heads, int32_t k, int32_t n, int32_t dtype, lvamd_stream_t stream);
+                       int64_t y_token_stride, int64_t y_head_stride, const int32_t* x_rows, const int32_t* y_rows,
+                       int64_t num_rows, int32_t num_heads, int32_t k, int32_t n, int32_t dtype, lvamd_stream_t stream);
 
 /*
  * Per-head keys and values of cached rows: block record b (int32 [num_blocks][4]:

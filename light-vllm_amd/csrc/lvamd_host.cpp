@@ -1632,7 +1632,8 @@ PyObject* decode_work(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
 //             block_size, unit, merge_pieces, xcds)
 //   -> (pieces i32 [n, 16], jobs i32 [m, 8], workgroups, partial slots, most
 //       columns of a merge job, pieces of the deepest merge job)
-// The pieces of the attention over latent vectors: one kv head whose group is
+// The pieces of the attention over latent vectors (field 0 of pieces and jobs is the
+// request's index, which the caller replaces by its first row): one kv head whose group is
 // every head, workgroups of 16 * col_tiles columns in the waves' place.  Piece w is
 // workgroup w's first; field 11 is the index of its next (-1: none), fields 12 to
 // 15 its first four table entries (-1 where a tile may span more blocks).  Where a
@@ -2714,8 +2715,8 @@ typedef int (*LatentDecodeFn)(const void*, int64_t, int64_t, const void*, int64_
                               int64_t, const float*, const float*, int64_t, int32_t, void*, void*, int64_t, int64_t,
                               const int32_t*, int32_t, const int32_t*, int32_t, int32_t, const int32_t*, const uint32_t*,
                               float*, float*, int64_t, int32_t, int32_t, int32_t, int32_t, int32_t, float, int32_t, void*);
-typedef int (*LatentHeadsFn)(const void*, int64_t, int64_t, const void*, void*, int64_t, int64_t, const int32_t*, int64_t,
-                             int32_t, int32_t, int32_t, int32_t, void*);
+typedef int (*LatentHeadsFn)(const void*, int64_t, int64_t, const void*, void*, int64_t, int64_t, const int32_t*,
+                             const int32_t*, int64_t, int32_t, int32_t, int32_t, int32_t, void*);
 typedef int (*RotaryAnglesFn)(const void*, int32_t, int64_t, const double*, int32_t, float, void*, void*, int32_t, int32_t,
                               void*);
 
@@ -2787,14 +2788,14 @@ PyObject* latent_write(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
 // latent_attend(facts, pool, query, latent, rope_key, cosines, sines, scale, out, workspace, weights)
 // ints: decode fn, heads fn, tokens, heads, latent size, rope size, dtype code, interleaved, pieces, groups, jobs,
 //       jobs' count, merge columns, tables, vis, partial slots, column tiles, block size, bytes of the partial rows,
-//       bytes of the partials, rows' list, rows, first token, tokens spanned
+//       bytes of the partials, the rows' tokens (0: consecutive ones), rows, first token
 // weights: None, or (key_down, value_up, nope size, value size); the queries in latent space and the attended
 // latents lie in the workspace behind the partials.
 PyObject* latent_attend(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   if (!want_args(nargs, 11, "latent_attend")) return nullptr;
   TensorFacts t;
-  int64_t f[24], w[4] = {0, 0, 0, 0};
-  if (!facts_of_tuple(args[0], "latent_attend", 24, &t, f)) return nullptr;
+  int64_t f[23], w[4] = {0, 0, 0, 0};
+  if (!facts_of_tuple(args[0], "latent_attend", 23, &t, f)) return nullptr;
   const int64_t pool = PyLong_AsLongLong(args[1]), out = PyLong_AsLongLong(args[8]), ws = PyLong_AsLongLong(args[9]);
   const double scale = PyFloat_AsDouble(args[7]);
   if (PyErr_Occurred()) return nullptr;
@@ -2820,14 +2821,14 @@ PyObject* latent_attend(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   const LatentHeadsFn multiply = reinterpret_cast<LatentHeadsFn>((intptr_t)f[1]);
   const int32_t code = (int32_t)f[6], h = (int32_t)heads;
   const int32_t* rows = (const int32_t*)as_ptr(f[20]);
-  const int64_t base = f[22], span = f[23], row = heads * latent;  // (elements of two bytes)
-  const int64_t absorbed = ws + f[19], attended = absorbed + 2 * span * row;
+  const int64_t base = rows ? 0 : f[22], row = heads * latent;  // (elements of two bytes)
+  const int64_t absorbed = ws + f[19], attended = absorbed + 2 * f[21] * row;
   if (weighted) {
-    const int status = multiply(as_ptr(q + 2 * base * qs0), qs0, qs1, as_ptr(w[0]), as_ptr(absorbed), row, latent, rows, f[21],
-                                h, (int32_t)size, (int32_t)latent, code, as_ptr(stream));
+    const int status = multiply(as_ptr(q + 2 * base * qs0), qs0, qs1, as_ptr(w[0]), as_ptr(absorbed), row, latent, rows,
+                                nullptr, f[21], h, (int32_t)size, (int32_t)latent, code, as_ptr(stream));
     if (status != 0) return PyLong_FromLong(status);
   }
-  const int64_t from = weighted ? absorbed - 2 * base * row : q, to = weighted ? attended - 2 * base * row : out;
+  const int64_t from = weighted ? absorbed : q, to = weighted ? attended : out;
   int status = decode(as_ptr(from), weighted ? row : qs0, weighted ? latent : qs1, as_ptr(q + 2 * size), qs0, qs1,
                       as_ptr(o.lat), o.lat_s, as_ptr(o.key), o.key_s, (const float*)as_ptr(o.cos),
                       (const float*)as_ptr(o.sin), o.cos_s, (int32_t)f[7], as_ptr(pool), as_ptr(to), row, latent,
@@ -2837,7 +2838,7 @@ PyObject* latent_attend(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
                       (int32_t)latent, (int32_t)rope, (int32_t)f[16], (int32_t)f[17], (float)scale, code, as_ptr(stream));
   if (status == 0 && weighted)
     status = multiply(as_ptr(attended), row, latent, as_ptr(w[1]), as_ptr(out + 2 * base * heads * w[3]), heads * w[3], w[3],
-                      rows, f[21], h, (int32_t)latent, (int32_t)w[3], code, as_ptr(stream));
+                      nullptr, rows, f[21], h, (int32_t)latent, (int32_t)w[3], code, as_ptr(stream));
   return PyLong_FromLong(status);
 }
 

@@ -72,7 +72,7 @@ typedef const __attribute__((address_space(1))) void* lds_gptr;
 typedef __attribute__((address_space(3))) void* lds_lptr;
 
 struct LatentDecodeArgs {
-  const void* q;  // [tokens][heads][L], the latent part
+  const void* q;  // [rows][heads][L], the latent part; a piece names its request's first row
   int64_t q_tok_stride, q_head_stride;
   const void* qr;  // [tokens][heads][P], the rotated part
   int64_t qr_tok_stride, qr_head_stride;
@@ -84,7 +84,7 @@ struct LatentDecodeArgs {
   const float* cosines;  // [tokens][P / 2], or null: queries and keys are turned already
   const float* sines;
   int64_t angle_stride;
-  void* out;  // [tokens][heads][L]
+  void* out;  // [rows][heads][L]
   int64_t out_tok_stride, out_head_stride;
   const int32_t* __restrict__ tables;
   const uint32_t* __restrict__ vis;
@@ -98,11 +98,11 @@ struct LatentDecodeArgs {
 // A piece's record: pieces[blockIdx.x] is a workgroup's first, next its next (-1:
 // none); blocks are the first four of its table entries (-1: look them up).
 struct LatentPiece {
-  int group, tok_begin, tok_end, slot, table_off, computed, q_len, q_start, vis_off, vis_words, next;
+  int row, group, tok_begin, tok_end, slot, table_off, computed, q_len, q_start, vis_off, vis_words, next;
 };
 __device__ __forceinline__ LatentPiece read_latent_piece(const int32_t* __restrict__ pieces, int p) {
   const int32_t* r = pieces + (int64_t)p * LVAMD_PIECE_FIELDS;
-  return {r[1], r[2], r[3], r[4], r[5], r[6], r[7], r[8], r[9], r[10], r[11]};
+  return {r[0], r[1], r[2], r[3], r[4], r[5], r[6], r[7], r[8], r[9], r[10], r[11]};
 }
 
 __device__ __forceinline__ constexpr int swizzle(int row) {
@@ -281,7 +281,7 @@ __attribute__((amdgpu_waves_per_eu(LatentShape<L, P, NC>::WAVES_PER_EU))) void l
     const int g = ln >> 4;
     int head;
     const bool ok = columns(ln, x, ct0, qi0, head);
-    const T* q = static_cast<const T*>(a.q) + (int64_t)(x.q_start + qi0) * a.q_tok_stride + (int64_t)head * a.q_head_stride + 8 * g;
+    const T* q = static_cast<const T*>(a.q) + (int64_t)(x.row + qi0) * a.q_tok_stride + (int64_t)head * a.q_head_stride + 8 * g;
     const T* qr = static_cast<const T*>(a.qr) + (int64_t)(x.q_start + qi0) * a.qr_tok_stride +
                   (int64_t)head * a.qr_head_stride + 8 * g;
     const bool mine = scores && ok;
@@ -680,7 +680,7 @@ __attribute__((amdgpu_waves_per_eu(LatentShape<L, P, NC>::WAVES_PER_EU))) void l
       int qi, head;
       if (!columns(ln, cur, c, qi, head)) continue;
       if (cur.slot < 0) {
-        T* to = static_cast<T*>(a.out) + (int64_t)(cur.q_start + qi) * a.out_tok_stride + (int64_t)head * a.out_head_stride;
+        T* to = static_cast<T*>(a.out) + (int64_t)(cur.row + qi) * a.out_tok_stride + (int64_t)head * a.out_head_stride;
 #pragma unroll
         for (int n = 0; n < DT; ++n) store_partial4<false, T>(to + 16 * (wave * DT + n) + 4 * g, acc[c][n], inv);
       } else {
@@ -724,7 +724,7 @@ __global__ __launch_bounds__(L / 4 * MERGE_SHARES) void latent_merge_kernel(cons
   __shared__ f32x4 sums[S - 1][LANES];
   __shared__ float maxima[S], totals[S];
   const int32_t* jb = jobs + (int64_t)blockIdx.x * LVAMD_MERGE_FIELDS;
-  const int group = jb[1], slot0 = jb[2], np = jb[3], q_start = jb[4], q_len = jb[5];
+  const int row = jb[0], group = jb[1], slot0 = jb[2], np = jb[3], q_len = jb[5];
   const int i = blockIdx.y;
   const int col = group * cols + i;
   if (col >= q_len * a.heads) return;
@@ -778,7 +778,7 @@ __global__ __launch_bounds__(L / 4 * MERGE_SHARES) void latent_merge_kernel(cons
     sum += sums[s - 1][at] * w;
   }
   const int qi = fast_div(col, a.by_heads), head = col - qi * a.heads;
-  T* to = static_cast<T*>(a.out) + (int64_t)(q_start + qi) * a.out_tok_stride + (int64_t)head * a.out_head_stride;
+  T* to = static_cast<T*>(a.out) + (int64_t)(row + qi) * a.out_tok_stride + (int64_t)head * a.out_head_stride;
   const float inv = total > 0.f ? 1.f / total : NAN;  // (no finite score in any piece)
   store_partial4<false, T>(to + 4 * at, sum, inv);
 }

@@ -26,7 +26,7 @@ struct HeadsArgs {
   const void* w;  // [heads][n][k]
   void* y;
   int64_t y_tok_stride, y_head_stride;
-  const int32_t* rows;  // token of row i, or null: token i
+  const int32_t *x_rows, *y_rows;  // where row i lies in x and y, or null: i
   int32_t num_rows, k, n;
 };
 
@@ -48,13 +48,14 @@ __global__ __launch_bounds__(256) void latent_heads_kernel(const HeadsArgs a, co
   const int wrow = NT == 1 ? l16 : 8 * (l16 >> 2) + (l16 & 3);
   const T* w = static_cast<const T*>(a.w) + ((int64_t)h * a.n + n0 + wrow) * a.k + 8 * g;
   const T* x[MT];
-  int64_t tok[MT];
+  int to[MT];
   f32x4 acc[MT][NT];
 #pragma unroll
   for (int m = 0; m < MT; ++m) {
     const int r = min(m0 + 16 * m + l16, a.num_rows - 1);
-    tok[m] = a.rows ? a.rows[r] : r;
-    x[m] = static_cast<const T*>(a.x) + tok[m] * a.x_tok_stride + (int64_t)h * a.x_head_stride + 8 * g;
+    to[m] = a.y_rows ? a.y_rows[r] : r;
+    const int64_t at = a.x_rows ? a.x_rows[r] : r;
+    x[m] = static_cast<const T*>(a.x) + at * a.x_tok_stride + (int64_t)h * a.x_head_stride + 8 * g;
 #pragma unroll
     for (int n = 0; n < NT; ++n) acc[m][n] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
@@ -75,7 +76,7 @@ __global__ __launch_bounds__(256) void latent_heads_kernel(const HeadsArgs a, co
 #pragma unroll
   for (int m = 0; m < MT; ++m) {
     if (m0 + 16 * m + l16 >= a.num_rows) continue;
-    T* y = static_cast<T*>(a.y) + tok[m] * a.y_tok_stride + (int64_t)h * a.y_head_stride + n0 + 4 * NT * g;
+    T* y = static_cast<T*>(a.y) + to[m] * a.y_tok_stride + (int64_t)h * a.y_head_stride + n0 + 4 * NT * g;
 #pragma unroll
     for (int n = 0; n < NT; ++n) store_partial4<false, T>(y + 4 * n, acc[m][n], 1.f);
   }
@@ -281,15 +282,16 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void l
 using namespace lvamd;
 
 extern "C" int lvamd_latent_heads(const void* x, int64_t x_token_stride, int64_t x_head_stride, const void* weights, void* y,
-                                  int64_t y_token_stride, int64_t y_head_stride, const int32_t* rows, int64_t num_rows,
-                                  int32_t num_heads, int32_t k, int32_t n, int32_t dtype, lvamd_stream_t stream) {
+                                  int64_t y_token_stride, int64_t y_head_stride, const int32_t* x_rows, const int32_t* y_rows,
+                                  int64_t num_rows, int32_t num_heads, int32_t k, int32_t n, int32_t dtype, lvamd_stream_t stream) {
   if (!latent_dtype(dtype) || k <= 0 || k % 64 != 0 || n <= 0 || n % 64 != 0) return LVAMD_ERR_UNSUPPORTED;
   if (num_rows < 0 || num_rows > 65535 * 16LL || num_heads <= 0) return LVAMD_ERR_INVALID_ARGUMENT;
   if (num_rows == 0) return LVAMD_OK;
   if (!x || !weights || !y || !rows16(x, {x_token_stride, x_head_stride}) || !rows16(weights, {}) || ((uintptr_t)y & 7u) ||
       y_token_stride % 4 != 0 || y_head_stride % 4 != 0)
     return LVAMD_ERR_INVALID_ARGUMENT;
-  HeadsArgs a{x, x_token_stride, x_head_stride, weights, y, y_token_stride, y_head_stride, rows, (int32_t)num_rows, k, n};
+  HeadsArgs a{x, x_token_stride, x_head_stride, weights, y, y_token_stride, y_head_stride, x_rows, y_rows,
+              (int32_t)num_rows, k, n};
   hipStream_t s = static_cast<hipStream_t>(stream);
   auto launch = [&]<typename T, int MT, int NT>() -> int {
     const int blocks = n / (16 * NT), waves = num_heads * blocks;

@@ -91,9 +91,8 @@ class _Shape:
     """One layer shape's launch facts in a step plan."""
 
     __slots__ = ("facts", "out_shape", "out_strides", "scratch_bytes", "lists", "col_tiles", "num_groups", "num_jobs",
-                 "merge_columns", "num_slots", "acc_bytes", "latent_bytes", "num_rows", "row_base", "row_span", "every_row",
-                 "num_blocks", "num_units", "num_unit_jobs",
-                 "unit_merge_columns", "num_unit_slots")
+                 "merge_columns", "num_slots", "acc_bytes", "latent_bytes", "num_rows", "row_base", "num_blocks",
+                 "num_units", "num_unit_jobs", "unit_merge_columns", "num_unit_slots")
 
 
 _NO_STEP = ((), (None, 0, None, 0, None, None, 0, 0))
@@ -221,8 +220,8 @@ class LatentStepPlan(StepPlan):
             native.entry("lvamd_latent_heads"), self.num_tokens, heads, spec.latent_size, spec.rope_size, code,
             int(spec.rotary_layout == "interleaved"), lists.pieces, x.num_groups, lists.jobs or 0, x.num_jobs,
             x.merge_columns, self.tables_ptr, self.vis_ptr, x.num_slots, x.col_tiles, self.block_size, x.acc_bytes,
-            x.latent_bytes, lists.rows or 0, x.num_rows, x.row_base, x.row_span)
-        x.scratch_bytes = x.latent_bytes + (0 if weights is None else 4 * x.row_span * heads * spec.latent_size)
+            x.latent_bytes, lists.rows or 0, x.num_rows, x.row_base)
+        x.scratch_bytes = x.latent_bytes + (0 if weights is None else 4 * x.num_rows * heads * spec.latent_size)
         width = spec.latent_size if weights is None else weights[1]
         x.out_shape, x.out_strides = (self.num_tokens, heads, width), (heads * width, width, 1)
 
@@ -238,7 +237,7 @@ class LatentStepPlan(StepPlan):
         x.facts = None
         pieces = jobs = rows = blocks = units = unit_jobs = none
         x.num_groups = x.num_jobs = x.num_slots = x.merge_columns = x.num_rows = 0
-        x.row_base, x.row_span, x.every_row, x.col_tiles = 0, 0, True, COL_TILES[0]
+        x.row_base, x.col_tiles = 0, COL_TILES[0]
         x.num_blocks = x.num_units = x.num_unit_jobs = x.unit_merge_columns = x.num_unit_slots = 0
         if short.any():
             def groups(col_tiles: int) -> int:
@@ -247,18 +246,22 @@ class LatentStepPlan(StepPlan):
             x.col_tiles = choose_col_tiles(facts.q_lens[short], (facts.computed + facts.q_lens)[short], heads, groups)
             resident = groups(x.col_tiles)
             mine = meta[short].copy()
-            x.row_base = int(mine[0, 4])
-            x.row_span = int(mine[-1, 4] + mine[-1, 3]) - x.row_base
             found = host.latent_work(mine, facts.flat, heads, x.col_tiles, resident, self.block_size,
                                      int(native.load().lvamd_latent_decode_tile_tokens(x.col_tiles)), DECODE_MERGE_PIECES,
                                      native.xcd_count())
             pieces, jobs = (np.frombuffer(a, dtype=np.int32) for a in found[:2])
             x.num_groups, x.num_slots, x.merge_columns = (int(v) for v in found[2:5])
             x.num_jobs = jobs.size // native.MERGE_FIELDS
-            x.num_rows = int(facts.q_lens[short].sum())
-            x.every_row = x.num_rows == x.row_span
-            if not x.every_row:
-                rows = np.concatenate([np.arange(s, s + n, dtype=np.int32) for s, n in zip(mine[:, 4], mine[:, 3])]) - x.row_base
+            # Rows in latent space: the short requests' one after the other (without weights
+            # the step's own).
+            ends = np.cumsum(mine[:, 3], dtype=np.int32)
+            first = mine[:, 4] if weights is None else ends - mine[:, 3]
+            for records, fields in ((pieces, native.PIECE_FIELDS), (jobs, native.MERGE_FIELDS)):
+                request = records.reshape(-1, fields)[:, 0]
+                request[:] = first[request]
+            x.num_rows, x.row_base = int(ends[-1]), int(mine[0, 4])
+            if x.num_rows != int(mine[-1, 4] + mine[-1, 3]) - x.row_base:
+                rows = np.concatenate([np.arange(s, s + n, dtype=np.int32) for s, n in zip(mine[:, 4], mine[:, 3])])
         if long.any():
             mine = meta[long].copy()
             total = (mine[:, 2] + mine[:, 3]).astype(np.int64)
@@ -408,26 +411,24 @@ class HipLatentPagedAttention:
             else:
                 step = _step_args(spec, aligned_rows(latent), aligned_rows(rope_key), angles)
             if weights is None:
-                self._attend_latent(spec, shape, query, query_rope, step, rows, out, 0, scale, code, stream)
+                self._attend_latent(spec, shape, query, query_rope, step, rows, out, scale, code, stream)
             elif shape.num_rows:
                 self._attend_short(spec, shape, weights, query, query_rope, step, rows, out, scale, code, stream)
             if shape.num_units:
                 self._attend_long(spec, shape, weights, query, query_rope, rows, out, scale, code, stream)
         return out
 
-    def _attend_latent(self, spec, shape, query, query_rope, step, rows, out, base: int, scale, code, stream) -> None:
-        """The latent-space kernel and its merge; token t of the step is row t - base
-        of ``query`` and ``out``."""
+    def _attend_latent(self, spec, shape, query, query_rope, step, rows, out, scale, code, stream) -> None:
+        """The latent-space kernel and its merge."""
 
         plan, lists = self._plan, shape.lists
         # (Of the call's own stream or graph: no two share one.)
         workspace = torch.empty(shape.latent_bytes, dtype=torch.uint8, device=rows.device)
         acc = workspace.data_ptr() if shape.latent_bytes else None
-        es = query.element_size()
         native.check(native.load().lvamd_latent_decode(
-            query.data_ptr() - base * query.stride(0) * es, query.stride(0), query.stride(1), query_rope.data_ptr(),
+            query.data_ptr(), query.stride(0), query.stride(1), query_rope.data_ptr(),
             query_rope.stride(0), query_rope.stride(1), *step[1], rows.data_ptr(),
-            out.data_ptr() - base * out.stride(0) * es, out.stride(0), out.stride(1), lists.pieces, shape.num_groups,
+            out.data_ptr(), out.stride(0), out.stride(1), lists.pieces, shape.num_groups,
             lists.jobs, shape.num_jobs, shape.merge_columns, plan.tables_ptr, plan.vis_ptr, acc,
             None if acc is None else acc + shape.acc_bytes, shape.num_slots, spec.num_query_heads, spec.latent_size,
             spec.rope_size, shape.col_tiles, plan.block_size, float(scale), code, stream), "lvamd_latent_decode")
@@ -435,19 +436,19 @@ class HipLatentPagedAttention:
     def _attend_short(self, spec, shape, weights, query, query_rope, step, rows, out, scale, code, stream) -> None:
         """The absorbed form: into latent space, attention there, and out of it."""
 
-        lib, heads, base = native.load(), spec.num_query_heads, shape.row_base
-        both = torch.empty((2, shape.row_span, heads, spec.latent_size), dtype=query.dtype, device=query.device)
+        lib, heads, where = native.load(), spec.num_query_heads, shape.lists.rows
+        base = shape.row_base if where is None else 0
+        both = torch.empty((2, shape.num_rows, heads, spec.latent_size), dtype=query.dtype, device=query.device)
         absorbed, attended = both.unbind(0)
-        where = None if shape.every_row else shape.lists.rows
         es = query.element_size()
         native.check(lib.lvamd_latent_heads(
             query.data_ptr() + base * query.stride(0) * es, query.stride(0), query.stride(1), weights.key_down.data_ptr(),
-            absorbed.data_ptr(), absorbed.stride(0), absorbed.stride(1), where, shape.num_rows, heads, weights.nope_size,
+            absorbed.data_ptr(), absorbed.stride(0), absorbed.stride(1), where, None, shape.num_rows, heads, weights.nope_size,
             spec.latent_size, code, stream), "lvamd_latent_heads")
-        self._attend_latent(spec, shape, absorbed, query_rope, step, rows, attended, base, scale, code, stream)
+        self._attend_latent(spec, shape, absorbed, query_rope, step, rows, attended, scale, code, stream)
         native.check(lib.lvamd_latent_heads(
             attended.data_ptr(), attended.stride(0), attended.stride(1), weights.value_up.data_ptr(),
-            out.data_ptr() + base * out.stride(0) * es, out.stride(0), out.stride(1), where, shape.num_rows, heads,
+            out.data_ptr() + base * out.stride(0) * es, out.stride(0), out.stride(1), None, where, shape.num_rows, heads,
             spec.latent_size, weights.value_size, code, stream), "lvamd_latent_heads")
 
     def _attend_long(self, spec, shape, weights, query, query_rope, rows, out, scale, code, stream) -> None:

@@ -19,7 +19,7 @@ from pathlib import Path
 from light_vllm_amd import errors
 
 LIB_NAME = "liblvamd_hip.so"
-ABI_VERSION = 22
+ABI_VERSION = 23
 PACKAGE_DIR = Path(__file__).resolve().parent
 REPO_ROOT = PACKAGE_DIR.parent
 HEADER = REPO_ROOT / "include" / "lvamd_paged_kv.h"
@@ -161,7 +161,7 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "lvamd_latent_decode_tile_tokens": (ctypes.c_int, [_i32]),
     "lvamd_latent_decode_resident_groups": (ctypes.c_int, [_i32, _i32, _i32, _i32]),
     "lvamd_latent_heads": (
-        ctypes.c_int, [_p, _i64, _i64, _p, _p, _i64, _i64, _p, _i64, _i32, _i32, _i32, _i32, _p]),
+        ctypes.c_int, [_p, _i64, _i64, _p, _p, _i64, _i64, _p, _p, _i64, _i32, _i32, _i32, _i32, _p]),
     "lvamd_latent_expand": (
         ctypes.c_int, [_p, _p, _i32, _p, _p, _p, _p, _p, _p, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _p]),
     "lvamd_latent_prefill": (

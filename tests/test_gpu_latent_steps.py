@@ -1,4 +1,5 @@
-"""GPU: steps over the latent cache whose layers take several forms."""
+"""GPU: steps over the latent cache whose layers take several forms, and what a step
+allocates."""
 
 from __future__ import annotations
 
@@ -121,3 +122,37 @@ def test_a_plan_whose_upload_is_pending_on_another_stream(known) -> None:
     assert context.plan is kept.plan
     torch.cuda.synchronize()
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_short_requests_around_a_long_one_take_memory_for_themselves(monkeypatch) -> None:
+    """Two decoding requests of 128 heads with a chunk of 8192 tokens between them: no
+    scratch for the chunk's rows in latent space (2.1 GB)."""
+    latent_space._say("latent layer, memory of short requests around a chunk")
+    layer._force(monkeypatch, lambda n, linear: n >= 200)
+    heads, chunk = 128, 8192
+    cache, md, q, latent, rope_key, _, up = layer._step(heads, 512, 64, 128, 128, 16, torch.bfloat16, [40, 0, 90], [1, chunk, 2],
+                                                        seed=3)
+    weights, backend = lv.LatentWeights(*up), lv.HipPagedAttentionBackend()
+    run = lambda: backend.create(cache, md).forward("layer0", q, latent, rope_key, scale=0.07, weights=weights)  # noqa: E731
+    want = run()
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    got = run()
+    torch.cuda.synchronize()
+    took = torch.cuda.max_memory_allocated() - before
+    result, expanded = q.shape[0] * heads * 128 * 2, chunk * heads * (128 + 128) * 2 + chunk * 64 * 2
+    assert took < result + expanded + (64 << 20)  # (and the splits' partials, the short requests' own)
+    assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("expanded", (False, True))
+def test_short_requests_anywhere_in_the_step(expanded, monkeypatch) -> None:
+    """Short requests first, last, on both sides of long ones and alone: rows in latent
+    space are theirs alone, tokens the step's."""
+    latent_space._say(f"latent layer, places of short requests, expanded={expanded}")
+    layer._force(monkeypatch, lambda n, linear: (n >= 70) & linear & expanded)
+    for layouts in ([1, 80], [80, 1], [1, 80, TREE], [80, 3, 90], [2, 80, 1, 90, 1], [80, 1, TREE, 3, 70]):
+        computed = [(37 * i) % 130 for i in range(len(layouts))]
+        for rotary in (False, True):
+            layer._run(layer._step(5, 256, 64, 64, 128, 16, torch.bfloat16, computed, layouts, seed=len(layouts)), rotary=rotary)
