@@ -1,5 +1,5 @@
-"""Steps of a layer over the latent cache with its heads' weights, their result in
-fp64, and how far a kernel's result may be from it.
+"""Steps of a layer over the latent cache, with its heads' weights or (``nope`` None)
+in latent space, their result in fp64, and how far a kernel's result may be from it.
 
 The bound is on the norm of a (token, head)'s error.  What the kernels round on the way
 (u = eps / 2 of the step's type): turned queries, softmax weights (the sum that divides
@@ -65,9 +65,11 @@ def make(case, dtype, seed: int, layout: str = "interleaved") -> dict:
         at = torch.arange(c)
         rows[torch.tensor(table)[at // bs] * bs + at % bs] = torch.randn((c, latent + rope), generator=gen).to(dtype)
     t = sum(map(len, layouts))
-    query = (1.5 * torch.randn((t, heads, nope + rope), generator=gen)).to(dtype)
+    size = latent if nope is None else nope
+    query = (1.5 * torch.randn((t, heads, size + rope), generator=gen)).to(dtype)
     both = torch.randn((t, latent + rope), generator=gen).to(dtype)
-    up = [(torch.randn((heads, n, latent), generator=gen) * latent**-0.5).to(dtype) for n in (nope, value)]
+    up = None if nope is None else [(torch.randn((heads, n, latent), generator=gen) * latent**-0.5).to(dtype)
+                                    for n in (nope, value)]
     angle = 100000.0 * torch.rand((t, rope // 2), generator=gen, dtype=torch.float64)
     md = lv.PagedAttentionMetadata(block_tables=tuple(tables), num_computed_tokens=tuple(computed),
                                    query_layouts=tuple(lv.QueryLayout(p) for p in layouts))
@@ -104,7 +106,7 @@ def attend(step: dict, rows: torch.Tensor, expanded, *, scale: float, rotary: bo
         q[..., -rope:] = Z.rotate(q[..., -rope:], *(a.double().numpy() for a in step["rotary"]),
                                   layer.rotary_layout == "interleaved")
     q = torch.from_numpy(q).to(device)
-    key_up, value_up = (w.to(device).double() for w in step["up"])
+    up = None if step["up"] is None else [w.to(device).double() for w in step["up"]]
     heads = range(q.shape[1]) if heads is None else heads
 
     def rounded(x):
@@ -123,16 +125,25 @@ def attend(step: dict, rows: torch.Tensor, expanded, *, scale: float, rotary: bo
             h = (h + shift) % q.shape[1]
             qn, qr = q[t0:t0 + n, h, :-rope], q[t0:t0 + n, h, -rope:]
             s = (rounded(qr) if rotary else qr) @ r_.T
-            v = c_ @ value_up[h].T
-            if expanded[r]:
-                s = s + qn @ rounded(c_ @ key_up[h].T).T
+            if up is None:
+                s = s + qn @ c_.T
+            elif expanded[r]:
+                s = s + qn @ rounded(c_ @ up[0][h].T).T
             else:
-                s = s + rounded(qn @ key_up[h]) @ c_.T
+                s = s + rounded(qn @ up[0][h]) @ c_.T
             s = (s * scale).masked_fill(~mask, -torch.inf)
-            w = torch.exp(s - s.amax(dim=1, keepdim=True))
-            w = rounded(w)
+            w = rounded(torch.exp(s - s.amax(dim=1, keepdim=True)))
             w = w / w.sum(dim=1, keepdim=True)
-            out.append(rounded(w @ rounded(v) if expanded[r] else rounded(w @ c_) @ value_up[h].T))
+            if up is None:
+                v = c_
+                o = w @ v
+            elif expanded[r]:
+                v = c_ @ up[1][h].T
+                o = w @ rounded(v)
+            else:
+                v = c_ @ up[1][h].T
+                o = rounded(w @ c_) @ up[1][h].T
+            out.append(rounded(o))
             size.append(w @ v.abs())
         outs.append(torch.stack(out, dim=1))
         sizes.append(torch.stack(size, dim=1))
@@ -152,4 +163,4 @@ def bound(step: dict, rows: torch.Tensor, expanded, want, size, **kw):
 
 
 def scale_of(case) -> float:
-    return (case[3] + case[2]) ** -0.5
+    return ((case[3] or 128) + case[2]) ** -0.5

@@ -1,6 +1,7 @@
-"""GPU: layers over the latent cache with their heads' weights, both forms, held to
-the bound of ``latent_cases`` (the norm of each token's and head's error; that mistakes
-pass it is tested on the CPU), and the rows that the step left in the pool."""
+"""GPU: steps over the latent cache, with their heads' weights in both forms and in
+latent space, held to the bound of ``latent_cases`` (the norm of each token's and head's
+error; that mistakes pass it is tested on the CPU), and the rows that the step left in
+the pool."""
 
 from __future__ import annotations
 
@@ -57,21 +58,23 @@ def _check_pool(step, pool, rotary) -> None:
 
 
 def _run(case, expanded, monkeypatch, *, dtype="bf16", seed=3, layout="interleaved", rotary=True, scale=None, heads=None):
-    """``expanded(queries, linear)``: which requests take that form."""
+    """``expanded(queries, linear)``: which requests take that form (None: by the rule)."""
 
     step = L.make(case, L.DTYPES[dtype], seed, layout)
-    monkeypatch.setattr(latent_attention, "_expanded", lambda facts, *a: expanded(facts.q_lens, facts.vis_off < 0))
+    if expanded is not None:
+        monkeypatch.setattr(latent_attention, "_expanded", lambda facts, *a: expanded(facts.q_lens, facts.vis_off < 0))
     scale = L.scale_of(case) if scale is None else scale
     print(f"[gpu] latent norms {case} {dtype} {layout} rotary={rotary} scale={scale:.3f}", file=sys.stderr, flush=True)
-    cache, md = _cache(step), step["metadata"]
+    cache, md, up = _cache(step), step["metadata"], step["up"]
     context = lv.HipPagedAttentionBackend().create(cache, md)
     out = context.forward("layer0", step["query"].to(DEV), step["latent"].to(DEV), step["rope_key"].to(DEV), scale=scale,
                           rotary=tuple(a.to(DEV) for a in step["rotary"]) if rotary else None,
-                          weights=lv.LatentWeights(*(w.to(DEV) for w in step["up"])))
+                          weights=None if up is None else lv.LatentWeights(*(w.to(DEV) for w in up)))
     torch.cuda.synchronize()
     pool = cache.layer("layer0").rows.view(len(step["rows"]), -1)
     _check_pool(step, pool.cpu(), rotary)
-    forms = [bool(x) for x in expanded(md.facts.q_lens, md.facts.vis_off < 0)]
+    forms = [False] * len(md.query_layouts) if up is None else [bool(x) for x in latent_attention._expanded(
+        md.facts, step["spec"].layers[0], case[3], case[4])]
     kw = dict(scale=scale, rotary=rotary, heads=heads)
     want, size = L.attend(step, pool, forms, **kw)
     assert want.isfinite().all()
@@ -138,3 +141,37 @@ def test_heads_in_groups(monkeypatch) -> None:
 @pytest.mark.parametrize("scale", (1.0, -0.5, 0.0))
 def test_scales(scale, dtype, monkeypatch) -> None:
     _run((4, 128, 32, 64, 64, 16, [200, 30], [300, 2]), lambda n, linear: n >= 200, monkeypatch, dtype=dtype, scale=scale)
+
+
+def _random_case(rng):
+    heads = int(rng.choice((1, 3, 5, 8, 16, 16, 20, 40, 64, 128)))
+    latent, rope = int(rng.choice((512, 512, 384, 256, 128))), int(rng.choice((64, 32)))
+    nope, value = (None, None) if rng.random() < 0.4 else (int(rng.choice((64, 128))), int(rng.choice((64, 128))))
+    computed, layouts = [], []
+    for _ in range(int(rng.integers(1, 9))):
+        kind = rng.random()
+        if kind < 0.5:
+            n = int(rng.choice((1, 1, 1, 2, 5)))
+            parents, far = n, 3000
+        elif kind < 0.75:
+            n = int(rng.integers(2, 40))
+            parents, far = tuple([-1] + [int(rng.integers(max(0, i - 6), i)) for i in range(1, n)]), 1500
+        else:
+            parents, far = int(rng.integers(6, 420)), 900
+        layouts.append(parents)
+        computed.append(int(rng.choice((0, int(rng.integers(0, 70)), int(rng.integers(0, far))))))
+    return heads, latent, rope, nope, value, int(rng.choice((16, 16, 1, 12, 32, 64))), computed, layouts
+
+
+@pytest.mark.parametrize("seed", range(40))
+def test_random_steps(seed, monkeypatch) -> None:
+    """Any forms, widths, lengths, trees and blocks together, twice: the same bits."""
+    rng = np.random.default_rng(seed)
+    case = _random_case(rng)
+    if seed % 3 == 0:
+        monkeypatch.setattr(latent_attention, "WIDE_TILES", 0)
+    kw = dict(dtype=str(rng.choice(("bf16", "fp16"))), layout=str(rng.choice(("interleaved", "half"))), seed=seed,
+              rotary=bool(rng.random() < 0.7), heads=sorted({0, case[0] // 2, case[0] - 1}))
+    _, first = _run(case, None, monkeypatch, **kw)
+    _, again = _run(case, None, monkeypatch, **kw)
+    assert torch.equal(first, again)

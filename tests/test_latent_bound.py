@@ -1,4 +1,4 @@
-"""The bound that tests of latent layers hold kernels to (``latent_cases``), on the CPU:
+"""The bound that tests of latent steps hold kernels to (``latent_cases``), on the CPU:
 results with a mistake in them pass it by far."""
 
 from __future__ import annotations
@@ -8,7 +8,9 @@ import torch
 
 import latent_cases as L
 
-CASES = [(c, False) for c in L.SHORT] + [(c, True) for c in L.LONG] + [(L.EVERY_LENGTH, True), (L.EVERY_LENGTH, False)]
+LATENT_SPACE = (16, 512, 64, None, None, 16, [0, 431, 700], [1, L.TREE, 40])
+CASES = [(c, False) for c in L.SHORT] + [(c, True) for c in L.LONG] + [
+    (L.EVERY_LENGTH, True), (L.EVERY_LENGTH, False), (LATENT_SPACE, False)]
 
 
 def _heads(case):
