@@ -814,6 +814,9 @@ class HipPagedAttentionBackend:
         if plan is not None and not forms.keys() <= plan.launches.keys() and not torch.cuda.is_current_stream_capturing():
             plan = None  # (made for another cache's layers)
         if plan is None:
+            # (A replay would copy the lists from a staging buffer that later steps reuse.)
+            if torch.cuda.is_current_stream_capturing():
+                raise errors.ExecutionError("the context of a captured step must be created before the capture")
             staging = self._staging.get(config.device)
             if staging is None:
                 staging = self._staging[config.device] = Staging(config.device)

@@ -304,6 +304,9 @@ class LatentPagedKVCache:
                     native.check(lib.lvamd_latent_move_few(table.data_ptr(), layers, row_bytes * rows, src.ctypes.data,
                                                            dst.ctypes.data, n, stream), "lvamd_latent_move_few")
                 return
+            # (A replay would copy the places from a staging buffer that later calls reuse.)
+            if torch.cuda.is_current_stream_capturing():
+                raise errors.ExecutionError(f"a graph captures at most {state.few} moved tokens or copied blocks a call")
             blob, (at_src, at_dst) = state.staging.stage([src.view(np.int32), dst.view(np.int32)])
             at = blob.data_ptr()
             for row_bytes, layers, table in state.groups:

@@ -156,3 +156,45 @@ def test_short_requests_anywhere_in_the_step(expanded, monkeypatch) -> None:
         computed = [(37 * i) % 130 for i in range(len(layouts))]
         for rotary in (False, True):
             layer._run(layer._step(5, 256, 64, 64, 128, 16, torch.bfloat16, computed, layouts, seed=len(layouts)), rotary=rotary)
+
+
+def test_uploads_are_not_captured() -> None:
+    """What a replay would read from a reused staging buffer is refused: a context that
+    is created inside a capture, moves of more tokens or blocks than a launch's arguments
+    hold.  Fewer are captured and replay."""
+    latent_space._say("latent steps, uploads in a capture")
+    cache, metadata, run = _two_forms("none")
+    backend = lv.HipPagedAttentionBackend()
+    want = run(backend.create(cache, metadata()))
+    wide = lv.LatentPagedKVCache(cache.model_spec, lv.PagedKVCacheConfig(num_blocks=80, block_size=16, dtype=torch.bfloat16,
+                                                                         device=DEV))
+    wide.copy_blocks([0], [1])  # (its table of layers is made at the first move)
+    few = 32
+    kept = tuple(range(2, 2 + few + 1))
+    request = dict(block_ids=(0, 1, 2, 3), num_computed_tokens=10, num_query_tokens=40, num_reserved_query_tokens=40)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        with pytest.raises(lv.ExecutionError, match="before the capture"):
+            backend.create(cache, metadata())
+        with pytest.raises(lv.ExecutionError, match="at most 32"):
+            wide.copy_blocks(list(range(few + 1)), list(range(40, 40 + few + 1)))
+        with pytest.raises(lv.ExecutionError, match="at most 32"):
+            wide.compact(**request, retained_query_indices=kept)
+        wide.copy_blocks(list(range(few)), list(range(40, 40 + few)))
+        assert wide.compact(**request, retained_query_indices=kept[:few]) == few
+    gen = torch.Generator(device=DEV).manual_seed(6)
+    for _ in range(3):
+        expect = {}
+        for name in ("layer0", "layer1"):
+            rows = wide.layer(name).rows
+            rows.normal_(generator=gen)
+            expect[name] = rows.clone()
+            expect[name][40:40 + few] = rows[:few]
+            flat = expect[name].view(-1, rows.shape[-1])
+            flat[10:10 + few] = flat[12:12 + few].clone()
+        graph.replay()
+        got = run(backend.create(cache, metadata()))
+        torch.cuda.synchronize()
+        assert all(torch.equal(wide.layer(name).rows, x) for name, x in expect.items())
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
