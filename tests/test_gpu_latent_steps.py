@@ -198,3 +198,26 @@ def test_uploads_are_not_captured() -> None:
         torch.cuda.synchronize()
         assert all(torch.equal(wide.layer(name).rows, x) for name, x in expect.items())
         assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_the_framework_s_functions_move_latent_rows() -> None:
+    """``hip_compact`` and ``hip_compact_many`` do what the cache's own methods do."""
+    latent_space._say("latent compact through the functions")
+    gen = torch.Generator(device=DEV).manual_seed(5)
+    spec = lv.LatentKVCacheSpec((lv.LatentLayerSpec("a", 4, 256, 64), lv.LatentLayerSpec("b", 4, 128, 32)))
+    caches = [lv.LatentPagedKVCache(spec, lv.PagedKVCacheConfig(num_blocks=12, block_size=8, dtype=torch.bfloat16, device=DEV))
+              for _ in range(3)]
+    for name in ("a", "b"):
+        rows = caches[0].layer(name).rows
+        rows.normal_(generator=gen)
+        for cache in caches[1:]:
+            cache.layer(name).rows.copy_(rows)
+    requests = [dict(block_ids=(5, 2, 9), num_computed_tokens=11, num_query_tokens=9, num_reserved_query_tokens=9,
+                     retained_query_indices=(0, 3, 4, 8)),
+                dict(block_ids=(1, 7), num_computed_tokens=3, num_query_tokens=7, num_reserved_query_tokens=7,
+                     retained_query_indices=(6, 1))]
+    want = tuple(caches[0].compact(**r) for r in requests)
+    assert lv.paged_cache.hip_compact_many(caches[1], requests) == want == (3, 1)
+    assert tuple(lv.hip_compact(caches[2], **r) for r in requests) == want
+    for cache in caches[1:]:
+        assert all(torch.equal(cache.layer(name).rows, caches[0].layer(name).rows) for name in ("a", "b"))
