@@ -10,8 +10,8 @@ namespace lvamd {
 // ---------------------------------------------------------------------------
 // Angles.  Pair i of a position p turns by p * f_i; the host gives f_i in turns
 // (fp64).  p * f_i is formed and reduced to an eighth of a turn in fp64, where
-// it is off by less than 2^-52 of its turns (2^-35 of a turn at a million
-// turns); the reduced angle r, |r| <= pi / 4, is an fp32 value (off by 2^-25 r)
+// it is off by less than 2^-51 of its turns, the frequency's own roundings included
+// (2^-31 of a turn at a million turns); the reduced angle r, |r| <= pi / 4, is an fp32 value (off by 2^-25 r)
 // and sine and cosine are its Taylor sums to r^9 and r^10, whose next terms are
 // below 2^-29 and 2^-33.  A thread per pair; 32760 tokens of 64 values take 4.6
 // us, 64 of them 2.3; the host's call and its two allocations take 7.0 for either.

@@ -11,8 +11,8 @@
 // Mapping onto CDNA4:
 //   * A column is a (query, head) pair of one request; a workgroup (four waves, or
 //     eight of 64 columns and more) holds up to 16 NC of them and walks over tiles
-//     of 32 rows (64 with 64 columns): stream-K pieces of (request, column group) segments, split
-//     segments merged below.
+//     of 32 rows (64 with 64 columns): stream-K pieces of (request, column group)
+//     segments, split segments merged below.
 //   * The rows of a tile are loaded once, straight into LDS (global_load_lds, no
 //     registers), while the tile before is computed; they serve as keys (rows
 //     read as they lie) and as values (transpose reads).
@@ -24,6 +24,10 @@
 //     LDS (the accumulator layout of S^T is the operand layout of P^T).
 //   * The waves share each column's running maximum, which moves only when some
 //     score passes it by 2^8 (lazy rescaling): a vote per tile in LDS.
+//   * A row that some column does not see may hold anything: its scores, which are not
+//     finite then, raise a flag beside the vote.  Scores and weights stay; the tile's
+//     values that are not finite become zeros in LDS, and each column that sees such a
+//     row adds the row's values times zero.
 //   * Append: a tile's rows of this step are loaded from the step's tensors, and
 //     one column group writes them to the pool; keys and queries are turned on the
 //     way.  On the GPU it costs what the append's launch takes (48 requests: 30.4
@@ -35,14 +39,15 @@
 //
 // What bounds it.  Up to 32 columns two workgroups of a CU keep a tile of 37 KB
 // each in flight: 64 requests of 512 to 4,095 tokens (16 heads, 512 + 64, bf16, 182
-// MB) 41 us, 4.4 TB/s, of which 6 pass before the first tile and 31 at the full
-// rate; 16 x 32767 tokens (32 heads, fp16, 605 MB) 109 us, 5.5 TB/s.  From 64 columns on the
-// tile's own work: about 2.8 us for 64 rows and 64 columns, of which the matrix units
-// are busy 0.9 and LDS 1.1; the rest is vector instructions (two waves a SIMD) and
-// the round trips between the phases.  32 requests of 128 heads (97 MB, 21 GFLOP)
-// 54 us: 7 to the first tile, 9 to 10 tiles, 3 for the partials.  The groups of one
-// request over the same tokens run on one XCD, whose L2 serves the second: 63 to 51 us
-// for 32 x 2300 tokens.  Eight waves rather than four from 64 columns on: 140 against
+// MB) 41 to 43 us, 4.4 TB/s, of which 6 pass before the first tile and 31 at the full
+// rate; 16 x 32767 tokens (32 heads, fp16, 605 MB) 109 us, 5.5 TB/s.  From 64 columns on
+// the tile's own work: about 2.8 us for 64 rows and 64 columns, of which the matrix units
+// are busy 0.9 and LDS 1.1; the rest is vector instructions (two waves a SIMD, one
+// workgroup a CU) and the round trips between the phases.  32 requests of 128 heads (97
+// MB, 21 GFLOP) 54 us: 7 to the first tile, 9 to 10 tiles, 3 for the partials; over the
+// launch the matrix units are busy 16 %, LDS 14 %, waves wait 43 %.  The groups of one
+// request over the same tokens run on one XCD, whose L2 serves a part of the second's (159
+// of 209 MB come from memory): 63 to 51 us for 32 x 2300 tokens.  Eight waves rather than four from 64 columns on: 140 against
 // 145 us for 8 x 32767 x 128 heads.  Up to 32 columns tile loads are non-temporal: 50
 // against 55 us for the 64 requests.  Dealing the loads between the score products
 // measured slower (258 against 232 us).
@@ -200,8 +205,8 @@ __attribute__((amdgpu_waves_per_eu(LatentShape<L, P, NC>::WAVES_PER_EU))) void l
       // (A half-used last group's spare slots take the row's last chunk again.)
       if (8 * GR > S::CPR && gr == GR - 1) c = min(c, S::CPR - 1);
       // Non-temporal where a row is read once (16 and 32 columns are a whole request);
-    // 64 columns are often one of several groups, which read it from one L2 (51 against
-    // 56 us for 32 x 2300 tokens of 128 heads).  128 measured alike either way.
+      // 64 columns are often one of several groups, which share an L2 (51 against 56 us
+      // for 32 x 2300 tokens of 128 heads).  128 measured alike either way.
       __builtin_amdgcn_global_load_lds((lds_gptr)((gr < L / 64 ? row : key) + 8 * c),
                                        (lds_lptr)(dst + (gr * KT * 128 + rb * 1024)), 16, 0, NC == 4 ? 0 : 2);
     }
@@ -453,8 +458,8 @@ __attribute__((amdgpu_waves_per_eu(LatentShape<L, P, NC>::WAVES_PER_EU))) void l
       }
       if (masked) {
         // A row that some column does not see may hold what is not finite (a
-        // sibling's draft): zero probabilities do not hide it.  Every score of
-        // such a row is not finite either.
+        // sibling's draft): zero weights do not hide it.  Every score of such a row is not
+        // finite either (the row is the key too).
         const uint32_t bits = window(cur, qi0, t0 + 16 * (ks0 & ~1)) >> (16 * (ks0 & 1) + 4 * g);
 #pragma unroll
         for (int s = 0; s < QKS; ++s)
@@ -610,25 +615,25 @@ __attribute__((amdgpu_waves_per_eu(LatentShape<L, P, NC>::WAVES_PER_EU))) void l
           }
         }
       } else {
-      constexpr bool HOLD_V = NC > DT;
-      constexpr int HELD = HOLD_V ? DT : NC, TOT = HOLD_V ? NC : DT, LEAD = TOT < 2 ? TOT : 2;
-      V8 held[HELD], ahead[LEAD];
+        constexpr bool HOLD_V = NC > DT;
+        constexpr int HELD = HOLD_V ? DT : NC, TOT = HOLD_V ? NC : DT, LEAD = TOT < 2 ? TOT : 2;
+        V8 held[HELD], ahead[LEAD];
 #pragma unroll
-      for (int i = 0; i < HELD; ++i) held[i] = HOLD_V ? rdv(i) : rdp(i);
+        for (int i = 0; i < HELD; ++i) held[i] = HOLD_V ? rdv(i) : rdp(i);
 #pragma unroll
-      for (int i = 0; i < LEAD; ++i) ahead[i] = HOLD_V ? rdp(i) : rdv(i);
-      if constexpr (NC == 8) __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-      for (int i = 0; i < TOT; ++i) {
-        const V8 x = ahead[i % LEAD];
-        if (i + LEAD < TOT) ahead[i % LEAD] = HOLD_V ? rdp(i + LEAD) : rdv(i + LEAD);
-#pragma unroll
-        for (int k = 0; k < HELD; ++k) {
-          f32x4& to = acc[HOLD_V ? i : k][HOLD_V ? k : i];
-          to = HOLD_V ? mm(held[k], x, to) : mm(x, held[k], to);
-        }
+        for (int i = 0; i < LEAD; ++i) ahead[i] = HOLD_V ? rdp(i) : rdv(i);
         if constexpr (NC == 8) __builtin_amdgcn_sched_barrier(0);
-      }
+#pragma unroll
+        for (int i = 0; i < TOT; ++i) {
+          const V8 x = ahead[i % LEAD];
+          if (i + LEAD < TOT) ahead[i % LEAD] = HOLD_V ? rdp(i + LEAD) : rdv(i + LEAD);
+#pragma unroll
+          for (int k = 0; k < HELD; ++k) {
+            f32x4& to = acc[HOLD_V ? i : k][HOLD_V ? k : i];
+            to = HOLD_V ? mm(held[k], x, to) : mm(x, held[k], to);
+          }
+          if constexpr (NC == 8) __builtin_amdgcn_sched_barrier(0);
+        }
       }
     }
     if (poisoned) {

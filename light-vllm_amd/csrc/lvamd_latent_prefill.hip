@@ -14,11 +14,15 @@
 //     barrier per tile;
 //   * S^T = K Q^T and O^T = V^T P^T on MFMA 16x16x32, the online softmax in the
 //     log2 domain with lazy rescaling, the sums on the matrix cores;
+//   * a later token's row may hold what is not finite: where a score of a tile is not
+//     finite, the tile's values that are not become zeros on their way to the products.
+//     Queries that see such a row get NaN through its score: lvamd_latent_expand makes a
+//     key NaN wherever its value is not finite;
 //   * units over a key range write fp32 partials, merged by
 //     lvamd_paged_attention_merge_q8's kernel.
 //
 // 2,048 queries behind 14,336 tokens, 16 heads, 128 + 64 and 128 (322 GFLOP): 370 to
-// 390 us, 0.83 to 0.87 PFLOP/s, as far as the 16-bit prefill kernel: softmax and LDS
+// 400 us, 0.80 to 0.87 PFLOP/s, as far as the 16-bit prefill kernel: softmax and LDS
 // reads share the issue with the matrix units.
 
 #include <cmath>

@@ -114,8 +114,8 @@ def choose_col_tiles(q_lens, totals, heads: int, resident) -> int:
     as the kernel is built; 128 columns only where 64 would give each of the
     ``resident(4)`` workgroups at least ``WIDE_TILES`` tiles.
 
-    A wider workgroup reads a row once for more columns; a narrower one holds two
-    to a CU and writes fewer partials, and up to 64 columns the launch appends.
+    A wider workgroup reads a row once for more columns; a narrower one writes fewer
+    partials, up to 64 columns the launch appends, and of up to 32 columns two fit a CU.
     Measured (us, 16/32/64/128 columns): 16 heads, 64 requests x 2300 tokens 43 / 43 /
     49 / 67; 16 x 32767 tokens 114 / 119 / 146 / 178; 64 columns against 128: 128 heads,
     32 x 2300 (9 tiles per workgroup) 51 / 63, 64 x 2300 (18 tiles) 87 / 88, 256 x 1000 (32
